@@ -15,9 +15,11 @@ from . import build as _build
 OK = 0
 ERR_BAD_ARG, ERR_NULL, ERR_UNSUPPORTED, ERR_CUDA, ERR_SCRATCH = -1, -2, -3, -4, -5
 ALGO_AUTO, ALGO_GENERIC, ALGO_ROWS, ALGO_TENSOR = 0, 1, 2, 3
+TYPE_F32, TYPE_BF16 = 0, 1
+WEIGHTS_VE, WEIGHTS_EV = 0, 1
 TENSOR_DEFAULT, TENSOR_SPLIT_TF32, TENSOR_TILED, TENSOR_WHOLE_HEAD = 0, 1, 5, 6
 
-_vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
+_vp, _i, _sz, _f, _ull = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_ulonglong
 
 # name -> (restype, argtypes); one entry per declaration in include/hipgpt_attn.h
 SIGNATURES = {
@@ -48,6 +50,11 @@ SIGNATURES = {
     "hipgpt_add_inplace": (_i, [_vp, _vp, C.c_longlong, _vp]),
     "hipgpt_relu": (_i, [_vp, C.c_longlong, _vp]),
     "hipgpt_embedding_lookup": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "hipgpt_embedding_scaled": (_i, [_vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _vp]),
+    "hipgpt_embedding_backward": (_i, [_vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "hipgpt_dropout_counter": (_i, [_vp, _vp, _vp, _f, _ull, _ull, _vp, C.c_longlong, _i, _vp]),
+    "hipgpt_linear_cross_entropy": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "hipgpt_linear_cross_entropy_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "hipgpt_mha_decode_scratch_bytes": (_sz, [_i, _i, _i, _i]),
     "hipgpt_mha_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _vp]),
     "hipgpt_mha_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),

@@ -171,6 +171,10 @@ int launch_matmul_tc_prepared(const float *A, const PackedB *b, const float *bia
 void matmul_tc_release(PackedB *p);
 int gemm_tc_status_fetch(int *status);
 void gemm_tc_release_scratch();
+// the ends of a training step (embedding.cu, linear_loss.cu)
+void embedding_release_scratch();
+void loss_release_scratch();
+int loss_status_fetch(int *status);
 int launch_mha_generic(const float *q, const float *k, const float *v, float *out, float *probs,
                        int B, int S, int E, int H, int causal, cudaStream_t st);
 int launch_sdp(const float *Q, const float *K, float *scores, int B, int S, int D, cudaStream_t st);

@@ -159,13 +159,14 @@ static int fetch_status_words(int *status)
     if (rc == HIPGPT_OK) rc = bf16_status_fetch(&b);
     if (rc == HIPGPT_OK) rc = tc16_status_fetch(&d);
     if (rc == HIPGPT_OK) rc = head_status_fetch(&h);
-    int pr = 0, gm = 0, bw = 0;
+    int pr = 0, gm = 0, bw = 0, ls = 0;
     if (rc == HIPGPT_OK) rc = probe_status_fetch(&pr);
     if (rc == HIPGPT_OK) rc = mha_backward_tc_status_fetch(&bw);
     if (rc == HIPGPT_OK && !bw) rc = mha_backward_head_status_fetch(&bw);
     if (rc == HIPGPT_OK) rc = gemm_tc_status_fetch(&gm);
+    if (rc == HIPGPT_OK) rc = loss_status_fetch(&ls);
     if (rc != HIPGPT_OK) return rc;
-    *status = a ? a : (b ? 100 + b : (d ? 300 + d : (h ? 400 + h : (gm ? 500 + gm : (bw ? 600 + bw : (pr ? 900 + pr : 0))))));
+    *status = a ? a : (b ? 100 + b : (d ? 300 + d : (h ? 400 + h : (gm ? 500 + gm : (bw ? 600 + bw : (ls ? 700 + ls : (pr ? 900 + pr : 0)))))));
     return HIPGPT_OK;
 }
 
@@ -328,6 +329,8 @@ void hipgpt_release_workspace(void)
     tc16_release_scratch();
     gemm_tc_release_scratch();
     mha_backward_tc_release();
+    embedding_release_scratch();
+    loss_release_scratch();
     g_bwd_rows_ws.release();
     std::lock_guard<std::mutex> lock(g_ws.mu);
     if (g_ws.dev) cudaFree(g_ws.dev);
@@ -454,7 +457,7 @@ int hipgpt_shard_range(int B, int world, int rank, int *b_begin, int *b_end)
 int hipgpt_debug_expire_wait(int code, int block)
 {
     const int family = code / 100 * 100, site = code % 100;
-    if ((family != 500 && family != 600) || site == 0 || block < 0 || block >= 1 << 22) return fail(HIPGPT_ERR_BAD_ARG, "no wait has code %d, or block %d", code, block);
+    if ((family != 500 && family != 600 && family != 700) || site == 0 || block < 0 || block >= 1 << 22) return fail(HIPGPT_ERR_BAD_ARG, "no wait has code %d, or block %d", code, block);
     g_expire_family = family;
     g_expire = block << 8 | site;
     return HIPGPT_OK;

@@ -50,16 +50,6 @@ constexpr size_t kGemmSmem = (size_t)kStages * (kAStage + kBStage) + 1024;
 
 __device__ int g_gemm_status = 0;
 
-__device__ __forceinline__ float pow2_scale(float amax)
-{
-    // the power of two that brings `amax` into [2^14, 2^15); 1 for zero, infinite or NaN input
-    if (!(amax > 0.0f && amax <= 3.0e38f)) return 1.0f;
-    const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
-    int sh = 14 - e;
-    sh = sh > 126 ? 126 : (sh < -126 ? -126 : sh);
-    return __uint_as_float((uint32_t)(127 + sh) << 23);
-}
-__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7F000000u - __float_as_uint(p)); }
 
 // largest |x| of n floats -> *out (zeroed before the launch; non-negative floats order like their bit patterns)
 __global__ void __launch_bounds__(256) gemm_amax_kernel(const float *__restrict__ x, size_t n, float *out)

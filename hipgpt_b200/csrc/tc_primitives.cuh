@@ -360,6 +360,17 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
+__device__ __forceinline__ float pow2_scale(float amax)
+{
+    // the power of two that brings `amax` into [2^14, 2^15); 1 for zero, infinite or NaN input
+    if (!(amax > 0.0f && amax <= 3.0e38f)) return 1.0f;
+    const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
+    int sh = 14 - e;
+    sh = sh > 126 ? 126 : (sh < -126 ? -126 : sh);
+    return __uint_as_float((uint32_t)(127 + sh) << 23);
+}
+__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7F000000u - __float_as_uint(p)); }
+
 // byte offset of 16-byte chunk c of row r in a tile of 128-byte rows, SWIZZLE_128B
 __device__ __forceinline__ int sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 

@@ -227,6 +227,47 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
                             int B, int S, int V, int E, void *stream);
 
 /*
+ * The two ends of a training step, in fp32 or with 16-bit storage (`type`; sums and softmax in fp32 either way, each result rounded once).
+ * Buffers of the library (per device and stream, at most eight; hipgpt_release_workspace() frees them; a captured call gets buffers of
+ * its graph) hold what a call keeps between its kernels.  Nothing depends on the order in which blocks run: results are the same bits run
+ * to run.
+ *   hipgpt_embedding_scaled    out[t] = scale tok[id_t] + pos[t mod S], zeros for an id outside [0, V); tok [V][E], pos [S][E] or NULL,
+ *                              out [B*S][E], all of `type`.  (hipgpt_embedding_lookup with a scale, without positions, in either type.)
+ *   hipgpt_embedding_backward  grad_tok[v] = scale * sum of grad_out[t] over the tokens with id v, grad_pos[s] = sum of grad_out over the
+ *                              tokens at position s whose id is inside [0, V); either may be NULL.  Rows of tok that no token has get
+ *                              zeros.  accumulate != 0: added to what the tables hold (and those rows are left as they are).  `type`: of
+ *                              grad_out; `grad_type`: of the tables (fp32 tables also for bf16 gradients; not the other way round).  Replaces
+ *                              embedding_backward_kernel (src/hip_kernels.cpp:1064-1088).
+ *   hipgpt_dropout_counter     out = [residual +] (kept ? in / (1 - p) : 0), where 16 bits of Philox4x32-10 decide for each element: counter
+ *                              (offset + *d_counter) + i / 8, key `seed`, kept if bits >= floor(65536 p + 1/2); 1 - p is that of the
+ *                              16 bits.  The mask is not stored: the backward pass is the same call on the gradient.  d_residual may be NULL, d_out
+ *                              may be d_in or d_residual; a call uses ceil(n / 8) counters.  d_counter: a 64-bit device word added to `offset`
+ *                              (a captured call draws a new mask at each replay if the word has moved on), or NULL.  0 <= p < 1.
+ *   hipgpt_linear_cross_entropy           z = x W^T, lse[n] = log sum_v exp z[n][v], loss[n] = lse[n] - z[n][target_n], without storing z.  x
+ *                              [N][E]; weights [V][E] (HIPGPT_WEIGHTS_VE: a token embedding used twice) or [E][V] (HIPGPT_WEIGHTS_EV: the
+ *                              reference's output projection, src/gpt_model.cpp).  A row whose target is outside [0, V) takes no
+ *                              part: loss = lse = 0, whatever it holds.  Replaces launch_matmul + softmax_loss_kernel (src/hip_kernels.cpp:606-657).
+ *   hipgpt_linear_cross_entropy_backward  gradients of x and the weights from grad_loss[N] (each row's; read only where the target is inside) and the
+ *                              forward's lse; either may be NULL; accumulate_w != 0: added to what grad_w holds.  grad_x of a row that takes no part
+ *                              is zero.
+ *                              Products run on the tensor pipe with fp32 accumulation.  fp32: from two fp16 pieces of each operand under one
+ *                              power of two per matrix (2^-22 of a value down to 2^-17 of the matrix's largest, 2^-40 of that one below).
+ *                              bf16: the gradient of the logits is rounded to bf16 before the second product.
+ */
+#define HIPGPT_TYPE_F32   0
+#define HIPGPT_TYPE_BF16  1
+#define HIPGPT_WEIGHTS_VE 0
+#define HIPGPT_WEIGHTS_EV 1
+HIPGPT_API int hipgpt_embedding_scaled(const int *d_ids, const void *d_tok, const void *d_pos, void *d_out, float scale, int B, int S, int V, int E, int type, void *stream);
+HIPGPT_API int hipgpt_embedding_backward(const void *d_grad_out, const int *d_ids, void *d_grad_tok, void *d_grad_pos, float scale, int accumulate,
+                              int B, int S, int V, int E, int type, int grad_type, void *stream);
+HIPGPT_API int hipgpt_dropout_counter(const void *d_in, const void *d_residual, void *d_out, float p, unsigned long long seed, unsigned long long offset,
+                           const unsigned long long *d_counter, long long n, int type, void *stream);
+HIPGPT_API int hipgpt_linear_cross_entropy(const void *d_x, const void *d_w, const int *d_targets, float *d_loss, float *d_lse, int N, int E, int V, int layout, int type, void *stream);
+HIPGPT_API int hipgpt_linear_cross_entropy_backward(const void *d_x, const void *d_w, const int *d_targets, const float *d_lse, const float *d_grad_loss, void *d_grad_x, void *d_grad_w,
+                                         int accumulate_w, int N, int E, int V, int layout, int type, void *stream);
+
+/*
  * Single-query-row attention over a key/value cache, split over the context (extension; the
  * reference's generation loop, src/gpt_model.cpp:261-280, re-runs the whole window instead).
  *   d_q, d_out       [B][E]          the new token's query / the attention output
@@ -377,7 +418,7 @@ HIPGPT_API int hipgpt_probe_fma(float *d_sink, int blocks, int iters, double *fl
  * waits on hardware barriers are bounded; a block whose wait runs out stores nothing and records
  * which wait it was: 1..8 for the split-TF32 kernel, 100 + site for the bf16 kernel, 300 + site
  * for the tiled fp32 kernel, 400 + site for the whole-head kernel, 500 + site for the tensor-core projections,
- * 600 + site for the attention backward, 900 + site for the test hook
+ * 600 + site for the attention backward, 700 + site for the loss, 900 + site for the test hook
  * hipgpt_debug_wait_expiry.  This call waits for the whole
  * device (cudaDeviceSynchronize), stores the status word in *status and clears it.  0 means every
  * launch since the last call completed normally.  Callers of the device-pointer entry points
@@ -407,7 +448,7 @@ HIPGPT_API int hipgpt_set_full_range(int on);
  *       arrives, with a limit of `limit_cycles` SM cycles (at most 2^24, a few milliseconds).  Afterwards
  *       hipgpt_kernel_status() reports 907 and d_canary[0..n) is untouched.
  *   hipgpt_debug_expire_wait  in the calling thread's next call of a tensor-core projection (code 501 ... 504) or of a tensor-core
- *       backward (601 ... 627) the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
+ *       backward (601 ... 627) or loss, forward or backward (701 ... 704), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
  *       each of the call's launches that has it, if it has to wait at all.
  *   hipgpt_gpt_debug_stall_barrier  makes the NEXT hipgpt_gpt_generate call give up: in the persistent mode it starts with a
  *       grid-barrier counter that cannot complete, and every block gives up at its first barrier; by clusters the first block's
