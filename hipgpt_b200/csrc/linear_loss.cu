@@ -5,12 +5,17 @@
 //   z[n][v] = x[n] . w[v]        lse[n] = log sum_v exp z[n][v]        loss[n] = lse[n] - z[n][t_n]
 //   dz[n][v] = g_n (exp(z[n][v] - lse[n]) - [v = t_n])        dx = dz W        dW = dz^T x
 //
-// Three forms of one product kernel (loss_gemm_kernel), which differ in what they do with an accumulator tile:
-//   kLse   (forward)   a row's maximum and sum of exponentials over 128 columns, kept for loss_join_kernel; the target's logit
-//   kDz    (backward)  forms the logits of a piece of the vocabulary again and stores their gradient as 16-bit numbers: the piece's
-//                      gradient stays within L2 (kPieceBytes) until the next form has read it twice
-//   kOut   (backward)  dx (summed over the pieces in fp32) and the piece's rows of dW, in one launch
+// Two forms of one product kernel (loss_gemm_kernel), which differ in what they do with an accumulator tile:
+//   kForward    a row's maximum and sum of exponentials over 256 columns, kept for loss_join_kernel; the target's logit
+//   kBackward   the vocabulary in pieces.  Of one piece the logits are formed again and their gradient stored as 16-bit numbers (kDz); the
+//               same launch forms, from the gradient of the piece before, that piece's share of dx (kDx, summed over the pieces in fp32) and its rows of
+//               dW (kDw).  Two pieces' gradients exist at a time and stay within L2 (kPieceBytes each).
 // The backward pass costs 6 N E V operations instead of 4, and no [N][V] array exists in either.
+//
+// The two large sums of a launch have few tiles and long reductions (default model, a piece of 1024 columns: 32 tiles of 16 stages and 4 of 128), so the tiles that
+// do not come out even are not dealt out whole: their stages in a row are cut into a length for each pair of blocks (cut_tiles).  A tile that falls to several pairs
+// is left by each as a sum in fp32; the one that comes last adds them up, in the order of their stages.  Nothing waits for another pair, and the order of a sum depends on the
+// sizes alone.
 //
 // Rows whose target lies outside the vocabulary are left out at the start: loss_pack_x_kernel moves the others together, so they cost
 // nothing and what they hold (NaN from padding) meets no product.
@@ -28,60 +33,66 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hipgpt {
 namespace {
 
 constexpr int kHalfM = 128, kTileM = 2 * kHalfM, kTileN = 256, kDeep = 64;
 constexpr int kOperand = kHalfM * kDeep * 2;            // bytes of one block's share of an operand of a stage: 128 rows or columns
-constexpr int kEpiWarps = 8, kThreads = 32 * (kEpiWarps + 2);
+constexpr int kEpiWarps = 16, kThreads = 32 * (kEpiWarps + 2);      // four warps share a row's columns
+constexpr int kWarpChunks = kTileN / 4 / 32;              // 32-column chunks of a warp
 constexpr int kTmemColumns = 512;
 constexpr int kPromote = 2;
-constexpr size_t kPieceBytes = 64u << 20;
+constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
+// What a tile of kDz costs a pair beside its stages, in half stages
+template <int NP> constexpr int kDzExtra = 4;
 template <int NP> constexpr int kRing = NP == 1 ? 6 : 3;
-constexpr size_t kGemmSmem = 6 * 2 * kOperand + 1024;
-
-enum Form { kLse, kDz, kOut };
+constexpr int kRingBytes = 6 * 2 * kOperand;
+enum Form { kForward, kBackward };
+constexpr size_t kGemmSmem = kRingBytes + 1024;
+enum Kind { kDx, kDw, kDz };                            // problems of kBackward; kForward's one problem lies at kDz's place
 
 __device__ int g_loss_status = 0;
 
 // Sizes of one product D = A B (A: M x K, B: K x N), its place in the operands and what becomes of the result.
 struct Problem {
-    int m_tiles, n_tiles, stages;            // of 256, 256 and 64
+    int m_tiles, n_tiles, stages;            // of 256, 256 and 64; n_tiles 0: not asked for
+    int narrow;                              // the last of the n_tiles has at most 128 columns
+    int n_fast;                              // tiles in a row: n runs fastest, or m
     int a_across, b_across;                  // operand contiguous across the reduction (along M or N) instead of along it
-    int a_k0, a_m0, b_k0, b_n0;              // where the product begins in the operands
+    int b_k0, b_n0;                          // where the product begins in B
     int m_by_count, k_by_count;              // M, or K, is the number of rows that take part
-    // kOut
-    void *out;                               // element (row, column) at row * ld + column
+    // kDx, kDw: element (row, column) of the result at row * ld + column
+    void *out;
     long long ld;
     int rows, cols;
-    int by_map;                              // row i of the product is row row_map[i] of the output
-    int accumulate, first, last;             // pieces of the sum over the vocabulary: `sum` (fp32) holds what the earlier ones gave
-    float *sum;
-    int scale_of;                            // kOut: 0 of x's gradient, 1 of W's
+    int accumulate;
 };
 
 struct LossArgs {
-    CUtensorMap a[2], b[2];
-    Problem p[2];
-    int problems;
+    CUtensorMap a[3], b[3];
+    Problem p[3];
     const int *count;                        // rows that take part
     const int *row_map, *targets;            // of the rows that take part
     const float *lse, *g;
-    const unsigned *amax;                    // fp32: bits of the largest |x|, |w|, |g|
-    float2 *part;                            // kLse: [half tile of the vocabulary][row] maximum and sum
+    const float *amax;                       // fp32: the largest |x|, |w|, |g|
+    float2 *part;                            // kForward: [tile of the vocabulary][row] maximum and sum
     float *z_target;
-    uint16_t *dz;                            // kDz: [piece of the operand][rows][ld]
+    float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
+    int *arrived;                            // [tile][block of the pair][warp]: pairs that have left their share of a tile
+    uint16_t *dz;                            // kDz: [plane][rows][ld]
     size_t dz_ld, dz_plane;
+    int first, last;                         // the launch's share of dx is that of the first, the last piece
     size_t rows_alloc;
-    int v0, V;                               // kLse, kDz: first column of the call, and of all
+    int v0, V;                               // first column of the piece whose logits are formed, and of all
     int expire;
 };
 
 // fp32 operands: x = (hi + lo) / scale.  The gradient of the logits is |dz| <= 2 |g|: 2^14 / (power of two above the largest |g|) leaves room
-__device__ __forceinline__ float operand_scale(const unsigned *amax, int which) { return pow2_scale(__uint_as_float(amax[which])); }
-__device__ __forceinline__ float grad_scale(const unsigned *amax) { return operand_scale(amax, 2) * 0.5f; }
+__device__ __forceinline__ float operand_scale(const float *amax, int which) { return pow2_scale(amax[which]); }
+__device__ __forceinline__ float grad_scale(const float *amax) { return operand_scale(amax, 2) * 0.5f; }
 
 __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 {
@@ -91,55 +102,91 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 
 // ---- rows that take part, moved together ------------------------------------------------------------------------------
 
+constexpr int kAmaxBlocks = 296;
+
+// partial[which][block] = largest finite |value| that the block has seen: x (rows that take part), w, g
 __global__ void __launch_bounds__(256)
-loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, unsigned *amax)
+loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial)
 {
     dependency_wait();
     dependents_may_start();
-    const int which = blockIdx.y;
+    __shared__ float warp_max[8];
+    const int which = blockIdx.y, lane = threadIdx.x & 31;
     float m = 0.0f;
     auto take = [&](float v) { v = fabsf(v); m = v <= 3.0e38f ? fmaxf(m, v) : m; };      // (not of infinities and NaN: they stay what they are)
+    auto take4 = [&](const float4 &v) { take(v.x); take(v.y); take(v.z); take(v.w); };
     const long long step = (long long)gridDim.x * 256, at = (long long)blockIdx.x * 256 + threadIdx.x;
     if (which == 1) {
-        const long long total = (long long)V * E;
-        if ((reinterpret_cast<uintptr_t>(w) & 15) == 0) {
-            for (long long i = at; i < total / 4; i += step) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(w) + i);
-                take(v.x); take(v.y); take(v.z); take(v.w);
-            }
-            for (long long i = total / 4 * 4 + at; i < total; i += step) take(w[i]);
-        } else {
-            for (long long i = at; i < total; i += step) take(w[i]);
+        const long long total = (long long)V * E, words = (reinterpret_cast<uintptr_t>(w) & 15) == 0 ? total / 4 : 0;
+        const float4 *w4 = reinterpret_cast<const float4 *>(w);
+        long long i = at;
+        for (; i + 3 * step < words; i += 4 * step) {
+            const float4 a = __ldg(w4 + i), b = __ldg(w4 + i + step), c = __ldg(w4 + i + 2 * step), d = __ldg(w4 + i + 3 * step);
+            take4(a); take4(b); take4(c); take4(d);
+        }
+        for (; i < words; i += step) take4(__ldg(w4 + i));
+        for (i = words * 4 + at; i < total; i += step) take(__ldg(w + i));
+    } else if (which == 2) {
+        for (long long n = at; n < N; n += step) {
+            const int t = __ldg(targets + n);
+            if (t >= 0 && t < V) take(__ldg(g + n));
         }
     } else {
-        const int lane = threadIdx.x & 31;
+        const bool vec = E % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
         for (long long n = at >> 5; n < N; n += step >> 5) {
-            const int t = targets[n];
+            const int t = __ldg(targets + n);
             if (t < 0 || t >= V) continue;
-            if (which == 2) {
-                if (lane == 0) take(g[n]);
+            const float *row = x + (size_t)n * E;
+            if (vec) {
+#pragma unroll 4
+                for (int e = lane * 4; e < E; e += 128) take4(__ldg(reinterpret_cast<const float4 *>(row + e)));
             } else {
-                for (int e = lane; e < E; e += 32) take(x[(size_t)n * E + e]);
+#pragma unroll 4
+                for (int e = lane; e < E; e += 32) take(__ldg(row + e));
             }
         }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0 && m > 0.0f) atomicMax(&amax[which], __float_as_uint(m));
+    if (lane == 0) warp_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, warp_max[i]);
+        partial[which * kAmaxBlocks + blockIdx.x] = m;
+    }
 }
 
-// One row of `cols` values -> a row of `ld` 16-bit ones (zeros behind the last) in each plane, by one warp
+// The largest of a block's `count` values; every thread of 256 gets it
+__device__ __forceinline__ float block_max(const float *v, int count, float (&sh)[8])
+{
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < count; i += 256) m = fmaxf(m, v[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, sh[i]);
+    return m;
+}
+
+// `cols` values of a row from `begin` on -> 16-bit ones in each plane, zeros from `cols` to `ld`; by one warp
 template <typename T>
-__device__ __forceinline__ void pack_row(const T *src, uint16_t *dst, size_t plane, int cols, int ld, float scale, int lane, bool vec)
+__device__ __forceinline__ void pack_row(const T *src, uint16_t *dst, size_t plane, int begin, int end, int cols, float scale, int lane, bool vec)
 {
     if constexpr (sizeof(T) == 2) {
         if (vec) {
-            for (int c = lane * 8; c < ld; c += 256) *reinterpret_cast<uint4 *>(dst + c) = *reinterpret_cast<const uint4 *>(src + c);
+#pragma unroll 4
+            for (int c = begin + lane * 8; c < end; c += 256) *reinterpret_cast<uint4 *>(dst + c) = __ldg(reinterpret_cast<const uint4 *>(src + c));
         } else {
-            for (int c = lane; c < ld; c += 32) dst[c] = c < cols ? reinterpret_cast<const uint16_t *>(src)[c] : (uint16_t)0;
+#pragma unroll 4
+            for (int c = begin + lane; c < end; c += 32) dst[c] = c < cols ? reinterpret_cast<const uint16_t *>(src)[c] : (uint16_t)0;
         }
     } else {
-        for (int c = lane * 4; c < ld; c += 128) {
+#pragma unroll 4
+        for (int c = begin + lane * 4; c < end; c += 128) {
             float v[4];
             if (vec) {
                 load_values<float, 4>(src + c, v);
@@ -156,30 +203,59 @@ __device__ __forceinline__ void pack_row(const T *src, uint16_t *dst, size_t pla
     }
 }
 
-struct PackX {
+struct Pack {
+    const float *partial;                    // fp32: loss_amax_kernel's
+    int amax_blocks;
+    float *amax;
+    // the rows of x
     const int *targets;
     const float *lse, *g;                    // backward
-    int N, E, V, ld, per_block;
+    int N, E, V, ld, per_block, x_blocks, x_vec;
     uint16_t *xp;
     size_t plane;
     int *count, *row_map, *c_targets;
     float *c_lse, *c_g;
-    const unsigned *amax;
     float *zero_loss, *zero_lse;             // forward: what rows that take no part get
     uint8_t *zero_grad;                      // backward: their rows of the gradient
+    int *zero_ints;
+    int zeros;
+    // the weights, in pieces of kPackCols columns of a row
+    uint16_t *wp;
+    size_t w_plane;
+    int w_rows, w_cols, w_ld, w_col_pieces, w_vec;
 };
+constexpr int kPackCols = 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-loss_pack_x_kernel(const T *__restrict__ x, PackX p, int vec)
+loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
 {
     dependency_wait();
     dependents_may_start();
     __shared__ int warp_sum[8];
+    __shared__ float warp_max[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if ((int)blockIdx.x >= p.x_blocks) {     // eight pieces of rows of the weights a block
+        const float scale = sizeof(T) == 4 ? pow2_scale(block_max(p.partial + kAmaxBlocks, p.amax_blocks, warp_max)) : 1.0f;
+        const long long job = (long long)(blockIdx.x - p.x_blocks) * 8 + warp;
+        const int r = (int)(job / p.w_col_pieces), c = (int)(job % p.w_col_pieces) * kPackCols;
+        if (r < p.w_rows) pack_row<T>(w + (size_t)r * p.w_cols, p.wp + (size_t)r * p.w_ld, p.w_plane, c, min(p.w_ld, c + kPackCols), p.w_cols, scale, lane, p.w_vec != 0);
+        return;
+    }
+    float scale = 1.0f, gscale = 1.0f;
+    if constexpr (sizeof(T) == 4) {
+        float most[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) most[i] = i < 2 || p.g ? block_max(p.partial + i * kAmaxBlocks, p.amax_blocks, warp_max) : 0.0f;
+        if (blockIdx.x == 0 && tid < 3) p.amax[tid] = most[tid];
+        scale = pow2_scale(most[0]);
+        gscale = grad_scale(most);
+    }
+    for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
     const int from = blockIdx.x * p.per_block, to = min(p.N, from + p.per_block);
     auto inside = [&](int t) { return t >= 0 && t < p.V; };
     int before = 0;
+#pragma unroll 8
     for (int i = tid; i < from; i += 256) before += inside(__ldg(p.targets + i));
 #pragma unroll
     for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
@@ -187,8 +263,7 @@ loss_pack_x_kernel(const T *__restrict__ x, PackX p, int vec)
     __syncthreads();
     int base = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) base += warp_sum[w];
-    const float scale = sizeof(T) == 4 ? operand_scale(p.amax, 0) : 1.0f, gscale = sizeof(T) == 4 && p.g ? grad_scale(p.amax) : 1.0f;
+    for (int w8 = 0; w8 < 8; ++w8) base += warp_sum[w8];
     for (int r0 = from; r0 < to; r0 += 32) {
         const int t = r0 + lane < to ? __ldg(p.targets + r0 + lane) : -1;
         const unsigned mask = __ballot_sync(0xffffffffu, inside(t));
@@ -201,7 +276,7 @@ loss_pack_x_kernel(const T *__restrict__ x, PackX p, int vec)
                     p.c_targets[i] = t;
                     if (p.g) { p.c_g[i] = p.g[n] * gscale; p.c_lse[i] = p.lse[n]; }
                 }
-                pack_row<T>(x + (size_t)n * p.E, p.xp + (size_t)i * p.ld, p.plane, p.E, p.ld, scale, lane, vec != 0);
+                pack_row<T>(x + (size_t)n * p.E, p.xp + (size_t)i * p.ld, p.plane, 0, p.ld, p.E, scale, lane, p.x_vec != 0);
             } else {
                 if (p.zero_loss && lane == 0) p.zero_loss[n] = p.zero_lse[n] = 0.0f;
                 if (p.zero_grad) {
@@ -212,25 +287,13 @@ loss_pack_x_kernel(const T *__restrict__ x, PackX p, int vec)
         }
         base += __popc(mask);
     }
-    if (to == p.N && from < p.N) {           // the last block that has rows: their number, and zeros up to a whole stage of the products that sum over them
+    if (to == p.N && from < p.N) {           // the last block that has rows: their number, and zeros up to a whole stage (one at least) of the products that sum over them
         if (tid == 0) *p.count = base;
-        const int end = (base + kDeep - 1) / kDeep * kDeep;
+        const int end = max(kDeep, (base + kDeep - 1) / kDeep * kDeep);
         for (int i = base + warp; i < end; i += 8)
             for (int c = lane * 4; c < p.ld; c += 128)
                 for (int pl = 0; pl < (sizeof(T) == 4 ? 2 : 1); ++pl) *reinterpret_cast<uint2 *>(p.xp + pl * p.plane + (size_t)i * p.ld + c) = make_uint2(0u, 0u);
     }
-}
-
-// W [rows][cols] -> 16-bit rows of ld
-template <typename T>
-__global__ void __launch_bounds__(256)
-loss_pack_w_kernel(const T *__restrict__ w, uint16_t *wp, size_t plane, int rows, int cols, int ld, const unsigned *amax, int vec)
-{
-    dependency_wait();
-    dependents_may_start();
-    const float scale = sizeof(T) == 4 ? operand_scale(amax, 1) : 1.0f;
-    for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8)
-        pack_row<T>(w + (size_t)r * cols, wp + (size_t)r * ld, plane, cols, ld, scale, threadIdx.x & 31, vec != 0);
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------------
@@ -287,7 +350,130 @@ __device__ __forceinline__ void put_columns(T *dst, const float (&v)[32], int co
     }
 }
 
-// T: the storage type of kOut's results; NP: planes of an operand (1: bf16, 2: fp16 hi and lo).  site codes in the status word: 1 stage landed, 2 stage free,
+// How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
+// side by side read the same stages of it), as many whole rounds as leave every pair something over are dealt out tile by tile; the stages of the rest are cut into a length for
+// each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in half stages: a narrow tile's stages count half.
+constexpr int kMostPairs = 128;
+struct Cut {
+    long long total[2], all;                 // of kDx, of both
+    int m_tiles[2], n_tiles[2], stages[2], tiles[2], narrow[2], n_fast[2];
+    int dealt;                               // tiles that are dealt out whole
+    long long begin[kMostPairs + 1];         // each pair's length of the rest
+    long long scan[4];
+    int fits;
+};
+struct Place { int tile, k; };               // tile: kDx's, then kDw's
+
+// Tile u of problem i: its row and column of tiles, and what a stage of it counts
+struct TileOf { int m, n, unit; };
+__device__ __forceinline__ TileOf tile_of(const Cut &c, int i, int u)
+{
+    const int nt = c.n_tiles[i], mt = c.m_tiles[i];
+    const int m = c.n_fast[i] ? u / nt : u % mt, n = c.n_fast[i] ? u % nt : u / mt;
+    return {m, n, c.narrow[i] && n == nt - 1 ? 1 : 2};
+}
+// Half stages before tile t
+__device__ __forceinline__ long long place_before(const Cut &c, int t)
+{
+    const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
+    if (u >= c.tiles[i]) return c.all;
+    const TileOf x = tile_of(c, i, u);
+    const long long stages = c.stages[i];
+    const long long here = c.n_fast[i] ? stages * ((long long)x.m * (2 * c.n_tiles[i] - c.narrow[i]) + 2 * x.n) : stages * (2LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
+    return (i ? c.total[0] : 0) + here;
+}
+__device__ __forceinline__ Place place_of(const Cut &c, long long at)
+{
+    if (at >= c.all) return {c.tiles[0] + c.tiles[1], 0};
+    const int i = at >= c.total[0];
+    if (i) at -= c.total[0];
+    const long long stages = c.stages[i];
+    int u, unit;
+    if (c.n_fast[i]) {
+        const long long row = stages * (2 * c.n_tiles[i] - c.narrow[i]);
+        const long long m = at / row;
+        at -= m * row;
+        const int n = (int)min(at / (2 * stages), (long long)c.n_tiles[i] - 1);
+        at -= n * 2 * stages;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 1 : 2;
+        u = (int)m * c.n_tiles[i] + n;
+    } else {
+        const long long column = 2 * stages * c.m_tiles[i];
+        const int n = (int)min(at / column, (long long)c.n_tiles[i] - 1);
+        at -= n * column;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 1 : 2;
+        const int m = (int)(at / (unit * stages));
+        at -= m * unit * stages;
+        u = n * c.m_tiles[i] + m;
+    }
+    return {(i ? c.tiles[0] : 0) + u, (int)(at / unit)};
+}
+__device__ __forceinline__ bool before(const Place &a, const Place &b) { return a.tile < b.tile || (a.tile == b.tile && a.k < b.k); }
+
+// By the first kMostPairs threads of a block (four warps): the pairs' lengths.  Tiles of kDz are dealt out one by one from pair 0 on and cost dz_cost each.
+__device__ __forceinline__ void cut_tiles(Cut &c, int pairs, int dz_tiles, int dz_cost)
+{
+    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, tiles = c.tiles[0] + c.tiles[1];
+    const long long both = c.all + (long long)dz_cost * dz_tiles;
+    for (int rounds = tiles / pairs;; --rounds) {
+        const int dealt = max(0, rounds) * pairs;
+        long long load = 0, rest = c.all - place_before(c, dealt);
+        if (q < pairs) {
+            for (int t = q; t < dealt; t += pairs) {
+                const int i = t >= c.tiles[0];
+                load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * c.stages[i];
+            }
+            load += (long long)dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
+        }
+        long long incl = load;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) c.scan[warp] = incl;
+        if (q == 0) c.fits = 1;
+        asm volatile("bar.sync 15, 128;" ::: "memory");
+        for (int w = 0; w < warp; ++w) incl += c.scan[w];
+        // what is left for the pairs before this one when each has an equal part of everything; a length of at least four stages each
+        const long long begin = both * q / pairs - (incl - load);
+        const long long mine = both * (q + 1) / pairs - incl - begin;
+        if (q < pairs && mine < 8 && (rest > 0 || dealt > 0)) c.fits = 0;
+        asm volatile("bar.sync 15, 128;" ::: "memory");
+        const bool fits = c.fits != 0;
+        if (!fits && rounds > 0) continue;
+        if (q == 0) c.dealt = dealt;
+        if (q <= pairs) {
+            if (fits) {
+                c.begin[q] = (c.all - rest) + (q < pairs ? begin : rest);
+            } else {                         // too little for equal parts beside kDz's tiles: equal lengths of eight stages or more, for as many pairs as that gives
+                const int active = (int)max(1LL, min((long long)pairs, c.all / 16));
+                c.begin[q] = q >= active ? c.all : c.all * q / active;
+            }
+        }
+        return;
+    }
+}
+
+// What a pair does, one after the other: its tiles of kDx and kDw, its length of the rest of them, its tiles of kDz
+struct Work {
+    int kind, m, n, k0, k1, stages, tile;    // tile: of kDx and kDw, as in Place
+    bool narrow;
+};
+struct Walk {
+    int dealt;
+    Place at, end;
+    int dz, dz_tiles, dz_m_tiles;
+};
+
+// Two parts of a row: (maximum, sum of exponentials relative to it)
+__device__ __forceinline__ float2 join_parts(float2 a, float2 b)
+{
+    const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, a.y * ex2_approx((a.x - ref) * kLog2e) + b.y * ex2_approx((b.x - ref) * kLog2e));
+}
+
+// T: the storage type; operands have one plane (bf16) or two (fp32 as fp16 hi and lo).  site codes in the status word: 1 stage landed, 2 stage free,
 // 3 accumulator complete, 4 accumulator drained
 template <Form FORM, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -300,6 +486,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     __shared__ uint64_t full[RING], empty[RING], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
+    __shared__ float2 part_s[FORM == kForward ? 2 : 1][4][kHalfM];
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     int rank;
@@ -330,85 +517,130 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         if (!gone && !done) seen = loss_wait_slow(bar, parity, site, &abort_flag, peer_flag, args.expire);
     };
 
-    // the tiles of a call: those of the first problem, then those of the second; m runs fastest, so pairs that run side by side share B's columns
-    const int count = *args.count;
-    struct Tile { int which, m, n, stages; };
-    const int pairs = (int)gridDim.x / 2, first_tile = (int)blockIdx.x / 2;
-    int m_tiles[2] = {0, 0}, tiles[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (i < args.problems) {
-            m_tiles[i] = args.p[i].m_by_count ? (count + kTileM - 1) / kTileM : args.p[i].m_tiles;
-            tiles[i] = m_tiles[i] * args.p[i].n_tiles;
+    // No row may take part: one tile of rows of zeros, and one stage, are then worked on (so gradients of zero are written)
+    const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
+    const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
+    __shared__ Cut cut;
+    __shared__ Walk first;
+    if (threadIdx.x == 0) {
+        first = {0, {0, 0}, {0, 0}, pair, 0, count_tiles};
+        if (args.p[kDz].n_tiles) first.dz_tiles = count_tiles * args.p[kDz].n_tiles;
+        cut = {};
+        if constexpr (FORM == kBackward) {
+            for (int i = 0; i < 2; ++i) {
+                const Problem &p = args.p[i];
+                cut.m_tiles[i] = p.m_by_count ? count_tiles : p.m_tiles;
+                cut.n_tiles[i] = p.n_tiles;
+                cut.stages[i] = p.k_by_count ? count_stages : p.stages;
+                cut.tiles[i] = cut.m_tiles[i] * p.n_tiles;
+                cut.narrow[i] = p.narrow;
+                cut.n_fast[i] = p.n_fast;
+                cut.total[i] = (long long)cut.m_tiles[i] * cut.stages[i] * max(0, 2 * p.n_tiles - p.narrow);
+            }
+            cut.all = cut.total[0] + cut.total[1];
         }
-    const int all_tiles = tiles[0] + tiles[1];
-    auto tile_of = [&](int t) {
-        const int which = t >= tiles[0], u = which ? t - tiles[0] : t, mt = which ? m_tiles[1] : m_tiles[0];
-        const Problem &p = args.p[which];
-        return Tile{which, u % mt, u / mt, p.k_by_count ? (count + kDeep - 1) / kDeep : p.stages};
+    }
+    __syncthreads();
+    if constexpr (FORM == kBackward) {
+        if (cut.all) {
+            if (threadIdx.x < kMostPairs) cut_tiles(cut, pairs, first.dz_tiles, 2 * args.p[kDz].stages + kDzExtra<NP>);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                first.dealt = pair < cut.dealt ? pair : cut.dealt;
+                first.at = place_of(cut, cut.begin[pair]);
+                first.end = place_of(cut, cut.begin[pair + 1]);
+            }
+            __syncthreads();
+        }
+    }
+    auto next = [&](Walk &w, Work &x) {
+        if constexpr (FORM == kBackward) {
+            const bool deal = w.dealt < cut.dealt;
+            if (deal || before(w.at, w.end)) {
+                const int t = deal ? w.dealt : w.at.tile, i = t >= cut.tiles[0];
+                const TileOf place = tile_of(cut, i, t - (i ? cut.tiles[0] : 0));
+                x = {i, place.m, place.n, deal ? 0 : w.at.k, deal || t != w.end.tile ? cut.stages[i] : w.end.k, cut.stages[i], t, place.unit == 1};
+                if (deal) w.dealt += pairs; else w.at = {t + 1, 0};
+                return true;
+            }
+        }
+        if (w.dz >= w.dz_tiles) return false;
+        const int stages = args.p[kDz].stages;
+        x = {kDz, w.dz % w.dz_m_tiles, w.dz / w.dz_m_tiles, 0, stages, stages, 0, false};      // m runs fastest, so pairs that run side by side share B's columns
+        w.dz += pairs;
+        return true;
+    };
+    // f(kind) with the kind as a constant: what is read of the problem then lies at a fixed place among the kernel's arguments.  (With the place in a variable a stage took
+    // 950 cycles instead of 740 for the logits, 800 instead of 620 for the sums: copies and products were issued late.)
+    auto by_kind = [](int kind, auto f) {
+        if (FORM == kForward || kind == kDz) f(std::integral_constant<int, kDz>());
+        else if (kind == kDx) f(std::integral_constant<int, kDx>());
+        else f(std::integral_constant<int, kDw>());
     };
 
+    Work x;
+    Walk walk = first;
     if (warp == kEpiWarps) {
         // ---- producer: this block's halves of both operands ----
-        uint32_t full_of_first[RING];
-#pragma unroll
-        for (int s = 0; s < RING; ++s) full_of_first[s] = peer_addr(smem_u32(&full[s]), 0);
+        const uint32_t full_of_first = peer_addr(smem_u32(&full[0]), 0);
         int s = 0, round = 0;
-        for (int t = first_tile; t < all_tiles; t += pairs) {
-            const Tile w = tile_of(t);
-            const Problem &p = args.p[w.which];
-            const CUtensorMap *ma = &args.a[w.which], *mb = &args.b[w.which];
-            const int m0 = p.a_m0 + w.m * kTileM + rank * kHalfM, n0 = p.b_n0 + w.n * kTileN + rank * kHalfM;
-            for (int k = 0; k < w.stages; ++k) {
-                if (round) wait(&empty[s], (uint32_t)((round - 1) & 1), 2);
-                if (lane == 0 && seen) {
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE);
-                    uint32_t bar = full_of_first[0];
+        while (next(walk, x)) {
+            by_kind(x.kind, [&](auto kind) {
+                constexpr int KIND = decltype(kind)::value;
+                const Problem &p = args.p[KIND];
+                const CUtensorMap *ma = &args.a[KIND], *mb = &args.b[KIND];
+                const int m0 = x.m * kTileM + rank * kHalfM, n0 = p.b_n0 + x.n * kTileN + rank * (x.narrow ? kHalfM / 2 : kHalfM);
+                const int end = KIND == kDz ? p.stages : x.k1;
+                for (int k = KIND == kDz ? 0 : x.k0; k < end; ++k) {
+                    if (round) wait(&empty[s], (uint32_t)((round - 1) & 1), 2);
+                    if (elect_one() && seen) {
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE);
+                        const uint32_t bar = full_of_first + (uint32_t)(s * sizeof(uint64_t));
+                        uint8_t *at = ring + s * STAGE;
 #pragma unroll
-                    for (int i = 1; i < RING; ++i) bar = i == s ? full_of_first[i] : bar;
-                    uint8_t *at = ring + s * STAGE;
-#pragma unroll
-                    for (int pl = 0; pl < NP; ++pl) {
-                        uint8_t *a = at + pl * kOperand, *b = at + (NP + pl) * kOperand;
-                        const int ka = p.a_k0 + k * kDeep, kb = p.b_k0 + k * kDeep;
-                        if (p.a_across) {
-                            tma_load_pair(a, ma, m0, ka, pl, bar);
-                            tma_load_pair(a + kOperand / 2, ma, m0 + 64, ka, pl, bar);
-                        } else {
-                            tma_load_pair(a, ma, ka, m0, pl, bar);
-                        }
-                        if (p.b_across) {
-                            tma_load_pair(b, mb, n0, kb, pl, bar);
-                            tma_load_pair(b + kOperand / 2, mb, n0 + 64, kb, pl, bar);
-                        } else {
-                            tma_load_pair(b, mb, kb, n0, pl, bar);
+                        for (int pl = 0; pl < NP; ++pl) {
+                            uint8_t *a = at + pl * kOperand, *b = at + (NP + pl) * kOperand;
+                            const int ka = k * kDeep, kb = p.b_k0 + k * kDeep;
+                            if (p.a_across) {
+                                tma_load_pair(a, ma, m0, ka, pl, bar);
+                                tma_load_pair(a + kOperand / 2, ma, m0 + 64, ka, pl, bar);
+                            } else {
+                                tma_load_pair(a, ma, ka, m0, pl, bar);
+                            }
+                            if (p.b_across) {
+                                tma_load_pair(b, mb, n0, kb, pl, bar);
+                                tma_load_pair(b + kOperand / 2, mb, n0 + 64, kb, pl, bar);
+                            } else {
+                                tma_load_pair(b, mb, kb, n0, pl, bar);
+                            }
                         }
                     }
+                    __syncwarp();
+                    if (++s == RING) { s = 0; ++round; }
                 }
-                __syncwarp();
-                if (++s == RING) { s = 0; ++round; }
-            }
+            });
         }
         if (abort_flag) linger();
     } else if (warp == kEpiWarps + 1) {
         // ---- products, issued by the pair's first block for both ----
         if (rank == 0) {
             int s = 0, round = 0, unit = 0;
-            for (int t = first_tile; t < all_tiles; t += pairs) {
-                const Tile w = tile_of(t);
-                const Problem &p = args.p[w.which];
+            while (next(walk, x)) {
+                by_kind(x.kind, [&](auto kind) {
+                constexpr int KIND = decltype(kind)::value;
+                const Problem &p = args.p[KIND];
                 // operand along the reduction: rows of 128 bytes in groups of 8 (1024 bytes), 16 deep = 32 bytes; across it: blocks of 64 x 64 deep (8192 bytes),
                 // 8 deep = 1024 bytes.  Swizzled by 128 bytes either way.
-                const uint32_t idesc = (1u << 4) | (NP == 1 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)p.a_across << 15) | ((uint32_t)p.b_across << 16) | ((uint32_t)(kTileN >> 3) << 17) |
-                                       ((uint32_t)(kTileM >> 4) << 24);
+                const uint32_t idesc = (1u << 4) | (NP == 1 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)p.a_across << 15) | ((uint32_t)p.b_across << 16) |
+                                       ((uint32_t)((x.narrow ? kTileN / 2 : kTileN) >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
                 const uint32_t a_lbo = p.a_across ? kOperand / 2 : 16, b_lbo = p.b_across ? kOperand / 2 : 16;
                 const uint64_t a_step = p.a_across ? 128 : 2, b_step = p.b_across ? 128 : 2;
-                const int unit_stages = NP == 1 ? w.stages : kPromote;
-                for (int k0 = 0; k0 < w.stages; k0 += unit_stages, ++unit) {
+                const int begin = KIND == kDz ? 0 : x.k0, end = KIND == kDz ? p.stages : x.k1, unit_stages = NP == 1 ? end - begin : kPromote;
+                for (int k0 = begin; k0 < end; k0 += unit_stages, ++unit) {
                     const uint32_t acc = tmem + (uint32_t)((unit & 1) * kTileN);
                     if (unit >= 2) wait(&acc_empty[unit & 1], (uint32_t)((unit / 2 - 1) & 1), 4);
                     tc_fence_after();
-                    const int k1 = min(w.stages, k0 + unit_stages);
+                    const int k1 = min(end, k0 + unit_stages);
                     for (int k = k0; k < k1; ++k) {
                         wait(&full[s], (uint32_t)(round & 1), 1);
                         tc_fence_after();
@@ -430,154 +662,204 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     }
                     if (elect_one()) commit_pair(&acc_full[unit & 1]);
                 }
+                });
             }
             __syncwarp();
             if (abort_flag) linger();
         }
     } else {
-        // ---- what becomes of an accumulator: thread = row = TMEM lane; two warps share a row's columns ----
-        const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+        // ---- what becomes of an accumulator: thread = row = TMEM lane; four warps share a row's columns ----
+        const int quarter = warp & 3, fourth = warp >> 2, row_in_tile = rank * kHalfM + quarter * 32 + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t drained[2] = {peer_addr(smem_u32(&acc_empty[0]), 0), peer_addr(smem_u32(&acc_empty[1]), 0)};
         const float x_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 0)) : 1.0f, w_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 1)) : 1.0f;
         const float z_scale = x_inv * w_inv;
-        int unit = 0;
-        for (int t = first_tile; t < all_tiles; t += pairs) {
-            const Tile w = tile_of(t);
-            const Problem &p = args.p[w.which];
-            const int row = w.m * kTileM + rank * kHalfM + quarter * 32 + lane;
-            const int col0 = w.n * kTileN + half * 128;
+        int unit = 0, part_at = 0;
+        while (next(walk, x)) {
+            const Problem &p = args.p[x.kind];
+            const int row = x.m * kTileM + row_in_tile;
+            const int chunks = x.narrow ? kWarpChunks / 2 : kWarpChunks, mine0 = fourth * 32 * chunks, col0 = x.n * kTileN + mine0;      // its 32-column chunks
             auto release = [&](int buf) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(buf ? drained[1] : drained[0]) : "memory");
             };
+            const bool whole = x.kind == kDz || (x.k0 == 0 && x.k1 == x.stages);
 
             // per row
             const bool here = row < count;
             int target = -1;
-            float lse = 0.0f, g = 0.0f;
-            if constexpr (FORM != kOut) {
-                if (here) target = __ldg(args.targets + row) - args.v0;
-                if constexpr (FORM == kDz) if (here) { lse = __ldg(args.lse + row); g = __ldg(args.g + row); }
-            }
-            float run_max = -INFINITY, run_sum = 0.0f;
+            float lse = 0.0f, g = 0.0f, out_scale = 1.0f, run_max = -INFINITY, run_sum = 0.0f;
             size_t out_row = 0;
-            float out_scale = 1.0f;
             bool out_here = false, out_vec = false;
-            if constexpr (FORM == kOut) {
+            if (FORM == kForward || x.kind == kDz) {
+                if (here) target = __ldg(args.targets + row) - args.v0;
+                if constexpr (FORM == kBackward) if (here) { lse = __ldg(args.lse + row); g = __ldg(args.g + row); }
+            } else {
                 out_here = row < (p.m_by_count ? count : p.rows);
-                if (out_here) out_row = (size_t)(p.by_map ? __ldg(args.row_map + row) : row) * p.ld;
-                if constexpr (NP == 2) out_scale = pow2_inverse(grad_scale(args.amax)) * (p.scale_of ? x_inv : w_inv);
+                if (out_here) out_row = (size_t)(x.kind == kDx ? __ldg(args.row_map + row) : row) * p.ld;
+                if constexpr (NP == 2) out_scale = pow2_inverse(grad_scale(args.amax)) * (x.kind == kDx ? w_inv : x_inv);
                 out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
             }
+            const int left_all = (FORM == kForward || x.kind == kDz ? args.V - args.v0 : p.cols) - col0;           // columns from col0 on
 
-            // 32 columns from col0 + 32 c on
-            auto columns = [&](int c, float (&v)[32]) {
-                const int col = col0 + 32 * c;
-                if constexpr (FORM == kLse) {
-                    const int left = args.V - args.v0 - col;
-                    if (left <= 0) return;
-                    if (left < 32) {
+            // where 32 columns of this thread's row begin in a tile of `shares` or `sum`
+            auto tile_at = [&](int tile, int c) { return ((size_t)tile * (kTileN / 4) + (size_t)((mine0 + 32 * c) / 4)) * kTileM + row_in_tile; };
+
+            // kForward: 32 columns from col0 + 32 c on
+            auto log_sum = [&](int c, float (&v)[32]) {
+                const int col = col0 + 32 * c, left = left_all - 32 * c;
+                if (left <= 0) return;
+                if (left < 32) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) if (j >= left) v[j] = -INFINITY;
-                    }
-                    if (target >= col && target < col + 32 && !abort_flag) {
+                    for (int j = 0; j < 32; ++j) if (j >= left) v[j] = -INFINITY;
+                }
+                if (target >= col && target < col + 32 && !abort_flag) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) if (target - col == j) args.z_target[row] = v[j] * z_scale;
-                    }
-                    float m = run_max;
+                    for (int j = 0; j < 32; ++j) if (target - col == j) args.z_target[row] = v[j] * z_scale;
+                }
+                float m = run_max;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) m = max3(m, v[j] * z_scale, v[j + 1] * z_scale);
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    float s0 = run_sum * ex2_approx((run_max - ref) * kLog2e), s1 = 0.0f;
+                for (int j = 0; j < 32; j += 2) m = max3(m, v[j] * z_scale, v[j + 1] * z_scale);
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float s0 = run_sum * ex2_approx((run_max - ref) * kLog2e), s1 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 d = fmul2(ffma2(make_float2(v[j], v[j + 1]), make_float2(z_scale, z_scale), make_float2(-ref, -ref)), make_float2(kLog2e, kLog2e));
-                        s0 += ex2_approx(d.x);
-                        s1 += ex2_approx(d.y);
-                    }
-                    run_max = m;
-                    run_sum = s0 + s1;
-                } else if constexpr (FORM == kDz) {
-                    const int left = args.V - args.v0 - col;
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 d = fmul2(ffma2(make_float2(v[j], v[j + 1]), make_float2(z_scale, z_scale), make_float2(-ref, -ref)), make_float2(kLog2e, kLog2e));
+                    s0 += ex2_approx(d.x);
+                    s1 += ex2_approx(d.y);
+                }
+                run_max = m;
+                run_sum = s0 + s1;
+            };
+            // kDz: 32 columns of a plane, whole sectors of the thread's row
+            auto put_dz = [&](int c, int plane, const uint32_t (&o)[16]) {
+                if (abort_flag) return;
+                float *dst = reinterpret_cast<float *>(args.dz + plane * args.dz_plane + (size_t)row * args.dz_ld + col0 + 32 * c);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 d = fmul2(ffma2(make_float2(v[j], v[j + 1]), make_float2(z_scale, z_scale), make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
-                        v[j] = ex2_approx(d.x);
-                        v[j + 1] = ex2_approx(d.y);
-                    }
-                    if (target >= col && target < col + 32) {
+                for (int j = 0; j < 16; j += 8)
+                    store_sector(dst + j, __uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]), __uint_as_float(o[j + 4]), __uint_as_float(o[j + 5]),
+                                 __uint_as_float(o[j + 6]), __uint_as_float(o[j + 7]));
+            };
+            auto logit_gradient = [&](int c, float (&v)[32]) {
+                const int col = col0 + 32 * c, left = here ? left_all - 32 * c : 0;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = target - col == j ? v[j] - 1.0f : v[j];
-                    }
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 d = fmul2(ffma2(make_float2(v[j], v[j + 1]), make_float2(z_scale, z_scale), make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
+                    v[j] = ex2_approx(d.x);
+                    v[j + 1] = ex2_approx(d.y);
+                }
+                if (target >= col && target < col + 32) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = here && j < left ? v[j] * g : 0.0f;
-                    if (abort_flag) return;
-                    float *dst = reinterpret_cast<float *>(args.dz + (size_t)row * args.dz_ld + col);
-                    float o[16];
-                    if constexpr (NP == 1) {
+                    for (int j = 0; j < 32; ++j) v[j] -= target - col == j ? 1.0f : 0.0f;
+                }
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(pack_bf16(v[2 * j], v[2 * j + 1]));
-                    } else {
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 d = fmul2(make_float2(v[j], v[j + 1]), make_float2(g, g));
+                    v[j] = d.x;
+                    v[j + 1] = d.y;
+                }
+                if (left < 32) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : 0.0f;
+                }
+                uint32_t o[16];
+                if constexpr (NP == 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                    put_dz(c, 0, o);
+                } else {
+#pragma unroll
+                    for (int plane = 0; plane < 2; ++plane) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                            o[j] = __uint_as_float(*reinterpret_cast<const uint32_t *>(&h));
+                            o[j] = *reinterpret_cast<const uint32_t *>(&h);
                             v[2 * j] -= __low2float(h);
                             v[2 * j + 1] -= __high2float(h);
                         }
+                        put_dz(c, plane, o);
                     }
-                    store_sector(dst, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]);
-                    store_sector(dst + 8, o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]);
-                    if constexpr (NP == 2) {
-                        dst += args.dz_plane / 2;
+                }
+            };
+            // kDx, kDw: 32 columns of a tile that is complete
+            auto finish = [&](int c, float (&v)[32]) {
+                const int left = left_all - 32 * c;
+                if (left <= 0 || abort_flag) return;
+                if (x.kind == kDx && !args.last) {
+                    float4 *sum = args.sum + tile_at(x.tile, c);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                            o[j] = __uint_as_float(*reinterpret_cast<const uint32_t *>(&h));
-                        }
-                        store_sector(dst, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]);
-                        store_sector(dst + 8, o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]);
-                    }
-                } else {
-                    const int left = p.cols - col;
-                    if (!out_here || left <= 0 || abort_flag) return;
-                    if (p.sum && !(p.first && p.last)) {
-                        float *sum = p.sum + (size_t)row * p.cols + col;
-                        const bool vec = p.cols % 4 == 0;
-                        if (!p.first) {              // (past L1: another SM may have written it, in the launch before)
+                    for (int j = 0; j < 8; ++j) __stcg(sum + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    return;
+                }
+                if (!out_here) return;
+                if constexpr (NP == 2) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) if (j < left) v[j] += __ldcg(sum + j);
-                        }
-                        if (!p.last) {
-                            put_columns<float>(sum, v, left, false, vec);
-                            return;
-                        }
-                    }
-                    if constexpr (NP == 2) {
+                    for (int j = 0; j < 32; ++j) v[j] *= out_scale;
+                }
+                put_columns<T>(static_cast<T *>(p.out) + out_row + col0 + 32 * c, v, left, p.accumulate != 0, out_vec);
+            };
+            // ... and of one that is not: into this pair's share
+            auto leave = [&](int c, const float (&v)[32]) {
+                float4 *share = args.shares + tile_at(2 * pair + (x.k0 == 0), c);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= out_scale;
+                for (int j = 0; j < 8; ++j) __stcg(share + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+            };
+
+            // A tile that falls to several pairs (they follow one another, each with a part of its stages): the first of them is usually the last to come to it,
+            // finds the others' shares there and adds them to what it has in hand.  Whichever comes last adds them in the same order.
+            int p0 = pair, p1 = pair, sources = 0;
+            bool complete = whole;
+            int *arrived = nullptr;
+            if (FORM == kBackward && x.kind != kDz) {
+                if (!whole) {
+                    const Place tile_begin = {x.tile, 0}, tile_end = {x.tile, x.stages};
+                    while (p0 > 0 && before(tile_begin, place_of(cut, cut.begin[p0]))) --p0;
+                    while (before(place_of(cut, cut.begin[p1 + 1]), tile_end)) ++p1;
+                    arrived = args.arrived + ((size_t)x.tile * 2 + rank) * kEpiWarps + warp;
+                    if (pair == p0) {
+                        int there = 0;
+                        if (lane == 0) there = *reinterpret_cast<volatile int *>(arrived);
+                        there = __shfl_sync(0xffffffffu, there, 0);
+                        __threadfence();
+                        complete = there == p1 - p0;
+                        if (complete && lane == 0) *arrived = 0;         // for the next launch
                     }
-                    put_columns<T>(static_cast<T *>(p.out) + out_row + col, v, left, p.accumulate != 0, out_vec);
+                }
+                sources = (p1 - p0) + (x.kind == kDx && !args.first);
+            }
+            // source i of what is added to this pair's own part: the pairs behind the first, then dx so far
+            auto source = [&](int i, int c) { return i < p1 - p0 ? args.shares + tile_at(2 * (p0 + 1 + i), c) : args.sum + tile_at(x.tile, c); };
+
+            auto add_sources = [&](int c, float (&v)[32]) {
+#pragma unroll 1
+                for (int i = 0; i < sources; ++i) {
+                    const float4 *from = source(i, c);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 o = __ldcg(from + j * kTileM);
+                        v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
+                    }
                 }
             };
 
+            // Everything leaves TMEM before anything is stored: the arrival that gives an accumulator back would wait for stores before it.
+            float acc[kWarpChunks][32];
             if constexpr (NP == 2) {
-                float acc[4][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < kWarpChunks; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
-                for (int k0 = 0; k0 < w.stages; k0 += kPromote, ++unit) {
+                for (int k0 = x.k0; k0 < x.k1; k0 += kPromote, ++unit) {
                     wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
                     tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < kWarpChunks; ++c) {
+                        if (c >= chunks) continue;
 #pragma unroll
                         for (int h = 0; h < 32; h += 16) {
                             float v[16];
-                            tmem_ld16(lane_base + (uint32_t)((unit & 1) * kTileN + 32 * c + h), v);
+                            tmem_ld16(lane_base + (uint32_t)((unit & 1) * kTileN + mine0 + 32 * c + h), v);
                             tmem_wait_ld();
 #pragma unroll
                             for (int j = 0; j < 16; ++j) acc[c][h + j] += v[j];
@@ -585,30 +867,66 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     }
                     release(unit & 1);
                 }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) columns(c, acc[c]);
             } else {
-                if (w.stages) {
-                    wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
-                    tc_fence_after();
-                }
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    if (w.stages) {
-                        tmem_ld32(lane_base + (uint32_t)((unit & 1) * kTileN + 32 * c), v);
-                        tmem_wait_ld();
-                        if (c == 3) release(unit & 1);
-                    } else {
+                wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
+                tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                    }
-                    columns(c, v);
-                }
-                if (w.stages) ++unit;
+                for (int c = 0; c < kWarpChunks; ++c)        // (of a narrow tile the last one is not looked at)
+                    tmem_ld32(lane_base + (uint32_t)((unit & 1) * kTileN + (mine0 + 32 * c) % kTileN), acc[c]);
+                tmem_wait_ld();
+                release(unit & 1);
+                ++unit;
             }
-            if constexpr (FORM == kLse)
-                if (here && !abort_flag) args.part[(size_t)(2 * w.n + half) * args.rows_alloc + row] = make_float2(run_max, run_sum);
+#pragma unroll
+            for (int c = 0; c < kWarpChunks; ++c) {
+                if constexpr (FORM == kForward) {
+                    log_sum(c, acc[c]);
+                } else if (x.kind == kDz) {
+                    logit_gradient(c, acc[c]);
+                } else if (c < chunks) {
+                    if (complete) {
+                        add_sources(c, acc[c]);
+                        finish(c, acc[c]);
+                    } else {
+                        leave(c, acc[c]);
+                    }
+                }
+            }
+            if constexpr (FORM == kForward) {
+                // the four warps that share these rows meet; one joins what they have (two buffers: a warp is at most a tile ahead)
+                float2 (&mine)[4][kHalfM] = part_s[part_at];
+                part_at ^= 1;
+                mine[fourth][quarter * 32 + lane] = make_float2(run_max, run_sum);
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+                if (fourth == 0 && here && !abort_flag) {
+                    float2 all = mine[0][quarter * 32 + lane];
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) all = join_parts(all, mine[i][quarter * 32 + lane]);
+                    args.part[(size_t)x.n * args.rows_alloc + row] = all;
+                }
+            } else if (!complete) {
+                __threadfence();
+                __syncwarp();
+                int seen_before = 0;
+                if (lane == 0 && !abort_flag) seen_before = atomicAdd(arrived, 1);
+                seen_before = __shfl_sync(0xffffffffu, seen_before, 0);
+                __threadfence();
+                if (seen_before == p1 - p0) {        // the last of them: all shares are there
+                    if (lane == 0) *arrived = 0;
+#pragma unroll 1
+                    for (int c = 0; c < chunks; ++c) {
+                        float v[32];
+                        const float4 *own = args.shares + tile_at(2 * p0 + 1, c);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 o = __ldcg(own + j * kTileM);
+                            v[4 * j] = o.x; v[4 * j + 1] = o.y; v[4 * j + 2] = o.z; v[4 * j + 3] = o.w;
+                        }
+                        add_sources(c, v);
+                        finish(c, v);
+                    }
+                }
+            }
         }
     }
     __syncwarp();
@@ -629,24 +947,17 @@ loss_join_kernel(const float2 *__restrict__ part, int parts, size_t rows_alloc, 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *count;
     for (int r0 = blockIdx.x * 32; r0 < n; r0 += gridDim.x * 32) {
         const int row = r0 + lane;
-        float m = -INFINITY, s = 0.0f;
-        auto join = [&](float2 x) {
-            const float mn = fmaxf(m, x.x), ref = mn == -INFINITY ? 0.0f : mn;
-            s = s * ex2_approx((m - ref) * kLog2e) + x.y * ex2_approx((x.x - ref) * kLog2e);
-            m = mn;
-        };
+        float2 all = make_float2(-INFINITY, 0.0f);
         if (row < n) {
 #pragma unroll 8
-            for (int i = warp; i < parts; i += 8) join(__ldg(part + (size_t)i * rows_alloc + row));
+            for (int i = warp; i < parts; i += 8) all = join_parts(all, __ldg(part + (size_t)i * rows_alloc + row));
         }
-        sh[warp][lane] = make_float2(m, s);
+        sh[warp][lane] = all;
         __syncthreads();
         if (warp == 0 && row < n) {
-            m = -INFINITY;
-            s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) join(sh[w][lane]);
-            const float l = m + logf(s);
+            for (int w = 1; w < 8; ++w) all = join_parts(all, sh[w][lane]);
+            const float l = all.x + logf(all.y);
             const int at = row_map[row];
             lse[at] = l;
             loss[at] = l - z_target[row];
@@ -676,17 +987,22 @@ int operand_map(CUtensorMap *m, const void *base, bool half, long long inner, lo
     return HIPGPT_OK;
 }
 
+// The grid of a call: a pair of blocks for each two SMs, or for each tile where there are fewer
+int loss_pairs(int dev, long long most, int *pairs)
+{
+    int sms = 0;
+    const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_gemm_kernel: %s", cudaGetErrorString(e));
+    *pairs = (int)std::max<long long>(1, std::min<long long>(most, std::min(sms / 2, kMostPairs - 1)));
+    return HIPGPT_OK;
+}
+
 template <Form FORM, typename T>
-int launch_loss_gemm(LossArgs &a, long long most_tiles, int dev, cudaStream_t st)
+int launch_loss_gemm(LossArgs &a, int pairs, int dev, cudaStream_t st)
 {
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = once_per_device(done, dev, [] { return cudaFuncSetAttribute(loss_gemm_kernel<FORM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmSmem); });
-    int sms = 0;
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_gemm_kernel: %s", cudaGetErrorString(e));
-    if (most_tiles > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "%lld tiles are beyond one call", most_tiles);
-    const long long pairs = std::min<long long>(most_tiles, sms / 2);
-    e = launch_overlapped_clusters(loss_gemm_kernel<FORM, T>, 2, dim3((unsigned)(2 * pairs)), dim3(kThreads), kGemmSmem, st, a);
+    if (e == cudaSuccess) e = launch_overlapped_clusters(loss_gemm_kernel<FORM, T>, 2, dim3((unsigned)(2 * pairs)), dim3(kThreads), kGemmSmem, st, a);
     return e == cudaSuccess ? check_launch("loss_gemm_kernel") : fail(HIPGPT_ERR_CUDA, "loss_gemm_kernel: %s", cudaGetErrorString(e));
 }
 
@@ -722,7 +1038,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
     p.w_at = take(p.pack_w ? NP * p.w_plane * 2 : 0);
     p.ints_at = take((1 + 2 * (size_t)p.rows_alloc) * sizeof(int));
     p.floats_at = take(2 * (size_t)p.rows_alloc * sizeof(float));
-    p.amax_at = take(16);
+    p.amax_at = take((3 + 3 * kAmaxBlocks) * sizeof(float));
     p.end = at;
     return HIPGPT_OK;
 }
@@ -730,45 +1046,48 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
 // Fills what the plan has in the workspace, and of `a` what every form reads
 template <typename T>
 int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, const int *targets, const float *lse, const float *g, float *zero_loss, float *zero_lse, void *zero_grad,
-              cudaStream_t st, const void **w_base)
+              int *zero_ints, int zeros, cudaStream_t st, const void **w_base)
 {
-    unsigned *amax = reinterpret_cast<unsigned *>(ws + p.amax_at);
     int *ints = reinterpret_cast<int *>(ws + p.ints_at);
-    float *floats = reinterpret_cast<float *>(ws + p.floats_at);
+    float *floats = reinterpret_cast<float *>(ws + p.floats_at), *amax = reinterpret_cast<float *>(ws + p.amax_at);
+    Pack k = {};
     cudaError_t e;
     if constexpr (sizeof(T) == 4) {
-        e = cudaMemsetAsync(amax, 0, 16, st);
-        if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
-        const long long blocks = std::min<long long>(592, std::max<long long>(((long long)p.V * p.E + 4095) / 4096, ((long long)p.N + 7) / 8));
-        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)blocks, g ? 3 : 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, amax);
+        k.amax_blocks = (int)std::min<long long>(kAmaxBlocks, std::max<long long>(((long long)p.V * p.E + 4095) / 4096, ((long long)p.N + 7) / 8));
+        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, g ? 3 : 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, amax + 3);
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_amax_kernel: %s", cudaGetErrorString(e));
     }
+    k.partial = amax + 3;
+    k.amax = amax;
+    k.targets = targets; k.lse = lse; k.g = g;
+    k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
+    k.per_block = (int)(p.N <= 16384 ? 8 : round_up((p.N + 2047) / 2048, 8));      // (a block counts the targets before its rows)
+    k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
+    k.x_vec = p.E % kPer16<T> == 0 && p.E == p.x_ld && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
+    k.plane = p.x_plane;
+    k.count = ints; k.row_map = ints + 1; k.c_targets = ints + 1 + p.rows_alloc;
+    k.c_lse = floats; k.c_g = floats + p.rows_alloc;
+    k.zero_loss = zero_loss; k.zero_lse = zero_lse; k.zero_grad = static_cast<uint8_t *>(zero_grad);
+    k.zero_ints = zero_ints; k.zeros = zeros;
+    long long w_blocks = 0;
     if (p.pack_w) {
-        const bool vec = p.w_cols % kPer16<T> == 0 && p.w_cols == p.w_ld && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
-        const long long blocks = std::min<long long>((p.w_rows + 7) / 8, 148 * 16);
-        e = launch_overlapped(loss_pack_w_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, w, reinterpret_cast<uint16_t *>(ws + p.w_at), p.w_plane, (int)p.w_rows, (int)p.w_cols, (int)p.w_ld,
-                              (const unsigned *)amax, (int)vec);
-        if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_w_kernel: %s", cudaGetErrorString(e));
+        k.wp = reinterpret_cast<uint16_t *>(ws + p.w_at);
+        k.w_plane = p.w_plane;
+        k.w_rows = (int)p.w_rows; k.w_cols = (int)p.w_cols; k.w_ld = (int)p.w_ld;
+        k.w_col_pieces = (int)((p.w_ld + kPackCols - 1) / kPackCols);
+        k.w_vec = p.w_cols % kPer16<T> == 0 && p.w_cols == p.w_ld && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+        w_blocks = (p.w_rows * k.w_col_pieces + 7) / 8;
     }
     *w_base = p.pack_w ? static_cast<const void *>(ws + p.w_at) : w;
-    PackX px = {};
-    px.targets = targets; px.lse = lse; px.g = g;
-    px.N = p.N; px.E = p.E; px.V = p.V; px.ld = (int)p.x_ld;
-    px.per_block = (int)std::max<long long>(32, round_up((p.N + 295) / 296, 32));
-    px.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
-    px.plane = p.x_plane;
-    px.count = ints; px.row_map = ints + 1; px.c_targets = ints + 1 + p.rows_alloc;
-    px.c_lse = floats; px.c_g = floats + p.rows_alloc;
-    px.amax = amax;
-    px.zero_loss = zero_loss; px.zero_lse = zero_lse; px.zero_grad = static_cast<uint8_t *>(zero_grad);
-    const bool xvec = p.E % kPer16<T> == 0 && p.E == p.x_ld && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    e = launch_overlapped(loss_pack_x_kernel<T>, dim3((unsigned)((p.N + px.per_block - 1) / px.per_block)), dim3(256), 0, st, x, px, (int)xvec);
-    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_x_kernel: %s", cudaGetErrorString(e));
-    a.count = px.count; a.row_map = px.row_map; a.targets = px.c_targets;
-    a.lse = px.c_lse; a.g = px.c_g; a.amax = amax;
+    if (k.x_blocks + w_blocks > 2147483647LL) return fail(HIPGPT_ERR_UNSUPPORTED, "weights of %lld rows of %lld values are beyond one call", p.w_rows, p.w_cols);
+    e = launch_overlapped(loss_pack_kernel<T>, dim3((unsigned)(k.x_blocks + w_blocks)), dim3(256), 0, st, x, w, k);
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
+    a.count = k.count; a.row_map = k.row_map; a.targets = k.c_targets;
+    a.lse = k.c_lse; a.g = k.c_g; a.amax = amax;
     a.rows_alloc = (size_t)p.rows_alloc;
     a.V = p.V;
-    return HIPGPT_OK;
+    return check_launch("loss_pack_kernel");
 }
 
 // Maps of the operands of one problem: `across`: contiguous across the reduction, boxes of 64 x 64; along it: boxes of 64 x 128 rows
@@ -790,30 +1109,33 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     Plan p;
     int rc = plan_call<T>(p, w, N, E, V, layout);
     if (rc != HIPGPT_OK) return rc;
-    const int n_tiles = (int)((V + kTileN - 1) / kTileN), parts = (int)((V + 127) / 128);
-    const size_t part_at = p.end, zt_at = part_at + padded((size_t)2 * n_tiles * p.rows_alloc * sizeof(float2));
+    const int n_tiles = (int)((V + kTileN - 1) / kTileN), m_tiles = (int)(p.rows_alloc / kTileM);
+    if ((long long)m_tiles * n_tiles > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d V=%d is beyond one call", N, V);
+    const size_t part_at = p.end, zt_at = part_at + padded((size_t)n_tiles * p.rows_alloc * sizeof(float2));
     StreamWorkspace::Lease lease;
     rc = g_loss_ws.enter(st, zt_at + padded((size_t)p.rows_alloc * sizeof(float)), &lease);
     if (rc != HIPGPT_OK) return rc;
     uint8_t *ws = lease.get();
     LossArgs a = {};
     const void *wb = nullptr;
-    rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, st, &wb);
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
-    if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[0], p, ws, false);
-    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[0], p, wb, ev);
+    int pairs = 1;
+    rc = loss_pairs(p.dev, (long long)m_tiles * n_tiles, &pairs);
+    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, st, &wb);
+    if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, false);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb, ev);
     if (rc != HIPGPT_OK) return rc;
-    a.problems = 1;
-    a.p[0].n_tiles = n_tiles;
-    a.p[0].stages = (E + kDeep - 1) / kDeep;
-    a.p[0].b_across = ev;
-    a.p[0].m_by_count = 1;
+    Problem &q = a.p[kDz];
+    q.n_tiles = n_tiles;
+    q.stages = (E + kDeep - 1) / kDeep;
+    q.b_across = ev;
+    q.m_by_count = 1;
     a.part = reinterpret_cast<float2 *>(ws + part_at);
     a.z_target = reinterpret_cast<float *>(ws + zt_at);
     a.expire = take_expiry(700);
-    rc = launch_loss_gemm<kLse, T>(a, (p.rows_alloc / kTileM) * n_tiles, p.dev, st);
+    rc = launch_loss_gemm<kForward, T>(a, pairs, p.dev, st);
     if (rc != HIPGPT_OK) return rc;
-    const cudaError_t e = launch_overlapped(loss_join_kernel, dim3((unsigned)std::min<long long>((N + 31) / 32, 148 * 8)), dim3(256), 0, st, (const float2 *)a.part, parts, a.rows_alloc,
+    const cudaError_t e = launch_overlapped(loss_join_kernel, dim3((unsigned)std::min<long long>((N + 31) / 32, 148 * 8)), dim3(256), 0, st, (const float2 *)a.part, n_tiles, a.rows_alloc,
                                             (const float *)a.z_target, a.row_map, a.count, loss, lse);
     return e == cudaSuccess ? check_launch("loss_join_kernel") : fail(HIPGPT_ERR_CUDA, "loss_join_kernel: %s", cudaGetErrorString(e));
 }
@@ -829,90 +1151,87 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     if (rc != HIPGPT_OK) return rc;
     // pieces of the vocabulary of like size
     const long long most = std::max<long long>(1024, (long long)(kPieceBytes / ((size_t)p.rows_alloc * 2 * NP)) / kTileN * kTileN);
-    const int pieces = (int)((V + most - 1) / most);
-    const long long width = round_up((V + pieces - 1) / pieces, kTileN);
-    const size_t dz_plane = (size_t)p.rows_alloc * width;
-    const size_t dz_at = p.end, sum_at = dz_at + padded(NP * dz_plane * 2);
-    const bool sums = grad_x && pieces > 1;
+    const long long width = round_up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), kTileN);
+    const int pieces = (int)((V + width - 1) / width);
+    const bool ev = layout == HIPGPT_WEIGHTS_EV;
+    const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM), piece_tiles = (int)(width / kTileN);
+    const bool e_narrow = (E - 1) % kTileN < kTileN / 2;
+    const long long dx_tiles = grad_x ? (long long)m_tiles * e_tiles : 0, dw_tiles = grad_w ? (long long)piece_tiles * e_tiles : 0;
+    if (dx_tiles + dw_tiles > 1 << 26 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
+    int pairs = 1;
+    rc = loss_pairs(p.dev, 1 << 30, &pairs);
+    if (rc != HIPGPT_OK) return rc;
+
+    const size_t tile_bytes = (size_t)kTileM * kTileN * sizeof(float), dz_plane = (size_t)p.rows_alloc * width, dz_bytes = padded(NP * dz_plane * 2);
+    const size_t dz_at = p.end, shares_at = dz_at + (pieces > 1 ? 2 : 1) * dz_bytes, sum_at = shares_at + 2 * pairs * tile_bytes, arrived_at = sum_at + (pieces > 1 ? dx_tiles * tile_bytes : 0);
+    const int arrived = (int)(dx_tiles + dw_tiles) * 2 * kEpiWarps;
     StreamWorkspace::Lease lease;
-    rc = g_loss_ws.enter(st, sum_at + (sums ? padded((size_t)p.rows_alloc * E * sizeof(float)) : 0), &lease);
+    rc = g_loss_ws.enter(st, arrived_at + padded((size_t)arrived * sizeof(int)), &lease);
     if (rc != HIPGPT_OK) return rc;
     uint8_t *ws = lease.get();
     LossArgs a = {};
     const void *wb = nullptr;
-    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, st, &wb);
+    a.arrived = reinterpret_cast<int *>(ws + arrived_at);
+    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, st, &wb);
     if (rc != HIPGPT_OK) return rc;
-    const bool ev = layout == HIPGPT_WEIGHTS_EV;
-    const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM);
-    const int expire = take_expiry(700);
-    a.dz = reinterpret_cast<uint16_t *>(ws + dz_at);
+    a.shares = reinterpret_cast<float4 *>(ws + shares_at);
+    a.sum = reinterpret_cast<float4 *>(ws + sum_at);
+    a.expire = take_expiry(700);
     a.dz_ld = (size_t)width;
     a.dz_plane = dz_plane;
-    LossArgs o = a;
-    rc = x_map<T>(&a.a[0], p, ws, false);
-    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[0], p, wb, ev);
-    a.problems = 1;
-    a.p[0].stages = (E + kDeep - 1) / kDeep;
-    a.p[0].b_across = ev;
-    a.p[0].m_by_count = 1;
-    a.expire = o.expire = expire;
-    // dx[n][e] = sum_v dz[n][v] w[v][e]; dW[v][e] = sum_n dz[n][v] x[n][e], or dW[e][v]
-    auto dz_map = [&](CUtensorMap *m, bool across) { return operand_map(m, a.dz, NP == 2, width, p.rows_alloc, width, dz_plane, NP, across ? kDeep : kHalfM); };
-    const int ix = 0, iw = grad_x ? 1 : 0;
-    o.problems = (grad_x ? 1 : 0) + (grad_w ? 1 : 0);
-    if (grad_x) {
-        if (rc == HIPGPT_OK) rc = dz_map(&o.a[ix], false);
-        if (rc == HIPGPT_OK) rc = w_map<T>(&o.b[ix], p, wb, !ev);
-        Problem &q = o.p[ix];
-        q.n_tiles = e_tiles;
-        q.b_across = !ev;
-        q.m_by_count = 1;
-        q.out = grad_x;
-        q.ld = q.cols = E;
-        q.by_map = 1;
-        q.sum = sums ? reinterpret_cast<float *>(ws + sum_at) : nullptr;
-        q.scale_of = 0;
-    }
-    if (grad_w) {
-        Problem &q = o.p[iw];
-        if (rc == HIPGPT_OK) rc = ev ? x_map<T>(&o.a[iw], p, ws, true) : dz_map(&o.a[iw], true);
-        if (rc == HIPGPT_OK) rc = ev ? dz_map(&o.b[iw], true) : x_map<T>(&o.b[iw], p, ws, true);
-        q.a_across = q.b_across = 1;
-        q.k_by_count = 1;
-        q.accumulate = accumulate_w;
-        q.first = q.last = 1;
-        q.scale_of = 1;
-        q.ld = ev ? V : E;
-    }
+    // z[n][v]; dx[n][e] = sum_v dz[n][v] w[v][e]; dW[v][e] = sum_n dz[n][v] x[n][e], or dW[e][v]
+    auto dz_map = [&](CUtensorMap *m, int piece, int box) {
+        return operand_map(m, ws + dz_at + (piece & 1) * dz_bytes, NP == 2, width, p.rows_alloc, width, dz_plane, NP, box);
+    };
+    rc = x_map<T>(&a.a[kDz], p, ws, false);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb, ev);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDx], p, wb, !ev);
+    if (rc == HIPGPT_OK) rc = x_map<T>(ev ? &a.a[kDw] : &a.b[kDw], p, ws, true);
     if (rc != HIPGPT_OK) return rc;
-    for (int i = 0; i < pieces; ++i) {
+    a.p[kDz].stages = (E + kDeep - 1) / kDeep;
+    a.p[kDz].b_across = ev;
+    a.p[kDz].m_by_count = 1;
+    a.p[kDx].narrow = e_narrow;
+    a.p[kDx].n_fast = 1;                             // (the tiles of E next to one another, in both)
+    a.p[kDw].n_fast = !ev;
+    a.p[kDx].b_across = !ev;
+    a.p[kDx].m_by_count = 1;
+    a.p[kDx].out = grad_x;
+    a.p[kDx].ld = a.p[kDx].cols = E;
+    a.p[kDw].a_across = a.p[kDw].b_across = 1;
+    a.p[kDw].k_by_count = 1;
+    a.p[kDw].accumulate = accumulate_w;
+    a.p[kDw].ld = ev ? V : E;
+    for (int i = 0; i <= pieces; ++i) {              // the logits' gradient of piece i, the products with that of piece i - 1
+        Problem &z = a.p[kDz], &dx = a.p[kDx], &dw = a.p[kDw];
         const long long v0 = i * width, here = std::min<long long>(width, V - v0);
-        if (here <= 0) break;
-        const int v_tiles = (int)((here + kTileN - 1) / kTileN);
-        a.v0 = (int)v0;
-        a.p[0].n_tiles = v_tiles;
-        a.p[0].b_n0 = (int)v0;
-        rc = launch_loss_gemm<kDz, T>(a, (long long)m_tiles * v_tiles, p.dev, st);
-        if (rc != HIPGPT_OK) return rc;
-        long long tiles = 0;
-        if (grad_x) {
-            Problem &q = o.p[ix];
-            q.stages = (int)((here + kDeep - 1) / kDeep);
-            q.b_k0 = (int)v0;
-            q.first = i == 0;
-            q.last = v0 + width >= V;
-            tiles += (long long)m_tiles * e_tiles;
+        z.n_tiles = i < pieces ? (int)((here + kTileN - 1) / kTileN) : 0;
+        if (z.n_tiles) {
+            a.v0 = z.b_n0 = (int)v0;
+            a.dz = reinterpret_cast<uint16_t *>(ws + dz_at + (i & 1) * dz_bytes);
         }
-        if (grad_w) {
-            Problem &q = o.p[iw];
-            q.m_tiles = ev ? e_tiles : v_tiles;
-            q.n_tiles = ev ? v_tiles : e_tiles;
-            q.rows = ev ? E : (int)here;
-            q.cols = ev ? (int)here : E;
-            q.out = static_cast<T *>(grad_w) + (ev ? v0 : v0 * E);
-            tiles += (long long)q.m_tiles * q.n_tiles;
+        if (i > 0) {
+            const long long o0 = v0 - width, old = std::min<long long>(width, V - o0);
+            const int v_tiles = (int)((old + kTileN - 1) / kTileN);
+            a.first = i == 1;
+            a.last = i == pieces;
+            if (grad_x) {
+                dx.n_tiles = e_tiles;
+                dx.stages = (int)((old + kDeep - 1) / kDeep);
+                dx.b_k0 = (int)o0;
+                if (rc == HIPGPT_OK) rc = dz_map(&a.a[kDx], i - 1, kHalfM);
+            }
+            if (grad_w) {
+                dw.m_tiles = ev ? e_tiles : v_tiles;
+                dw.n_tiles = ev ? v_tiles : e_tiles;
+                dw.narrow = ev ? (old - 1) % kTileN < kTileN / 2 : e_narrow;
+                dw.rows = ev ? E : (int)old;
+                dw.cols = ev ? (int)old : E;
+                dw.out = static_cast<T *>(grad_w) + (ev ? o0 : o0 * E);
+                if (rc == HIPGPT_OK) rc = dz_map(ev ? &a.b[kDw] : &a.a[kDw], i - 1, kDeep);
+            }
         }
-        rc = launch_loss_gemm<kOut, T>(o, tiles, p.dev, st);
+        if (rc == HIPGPT_OK) rc = launch_loss_gemm<kBackward, T>(a, pairs, p.dev, st);
         if (rc != HIPGPT_OK) return rc;
     }
     return HIPGPT_OK;
