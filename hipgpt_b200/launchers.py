@@ -32,6 +32,29 @@ def _ptr_bf16(t):
     return t.data_ptr()
 
 
+_TYPES = {torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16}
+
+
+def _storage(t):
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"expected float32 or bfloat16, not {t.dtype}") from None
+
+
+def _ptr_of(name, t, dtype, count):
+    """The address of a tensor of at least `count` values on the current device, None for None."""
+    if t is None:
+        return None
+    if not (t.is_cuda and t.is_contiguous() and t.dtype == dtype):
+        raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
+    if t.numel() < count:
+        raise ValueError(f"{name} holds {t.numel()} values, {count} are needed")
+    return t.data_ptr()
+
+
 # the current stream's handle without the Stream object around it (3.2 us of host time per call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = torch.cuda.current_device
@@ -77,6 +100,40 @@ class _ThroughCtypes:
         if nbytes is None:
             nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
         return _capi.lib().hipgpt_mha_decode(*p, nbytes, _int(B), _int(H), _int(D), _int(ctx), _int(cap), _stream())
+
+
+    # training.py's
+    @staticmethod
+    def embedding_scaled(ids, tok, pos, out, scale, B, S, V, E):
+        n, dt = B * S, out.dtype
+        return _capi.lib().hipgpt_embedding_scaled(_ptr_of("ids", ids, torch.int32, n), _ptr_of("tok", tok, dt, V * E), _ptr_of("pos", pos, dt, S * E), _ptr_of("out", out, dt, n * E),
+                                                   scale, B, S, V, E, _storage(out), _stream())
+
+    @staticmethod
+    def embedding_backward(grad_out, ids, grad_tok, grad_pos, scale, accumulate, B, S, V, E):
+        n, table = B * S, grad_tok if grad_tok is not None else grad_pos
+        gt = table.dtype
+        return _capi.lib().hipgpt_embedding_backward(_ptr_of("grad_out", grad_out, grad_out.dtype, n * E), _ptr_of("ids", ids, torch.int32, n), _ptr_of("grad_tok", grad_tok, gt, V * E),
+                                                     _ptr_of("grad_pos", grad_pos, gt, S * E), scale, accumulate, B, S, V, E, _storage(grad_out), _storage(table), _stream())
+
+    @staticmethod
+    def dropout_counter(x, residual, out, counter, p, seed, offset):
+        n, dt, most = out.numel(), out.dtype, (1 << 64) - 1
+        return _capi.lib().hipgpt_dropout_counter(_ptr_of("x", x, dt, n), _ptr_of("residual", residual, dt, n), _ptr_of("out", out, dt, n), p, seed & most, offset & most,
+                                                  _ptr_of("counter", counter, torch.int64, 1), n, _storage(out), _stream())
+
+    @staticmethod
+    def linear_cross_entropy(x, w, targets, loss, lse, N, E, V, layout):
+        dt, f = x.dtype, _FLOAT32
+        return _capi.lib().hipgpt_linear_cross_entropy(_ptr_of("x", x, dt, N * E), _ptr_of("w", w, dt, V * E), _ptr_of("targets", targets, torch.int32, N), _ptr_of("loss", loss, f, N),
+                                                       _ptr_of("lse", lse, f, N), N, E, V, layout, _storage(x), _stream())
+
+    @staticmethod
+    def linear_cross_entropy_backward(x, w, targets, lse, grad_loss, grad_x, grad_w, accumulate, N, E, V, layout):
+        dt, f = x.dtype, _FLOAT32
+        return _capi.lib().hipgpt_linear_cross_entropy_backward(
+            _ptr_of("x", x, dt, N * E), _ptr_of("w", w, dt, V * E), _ptr_of("targets", targets, torch.int32, N), _ptr_of("lse", lse, f, N), _ptr_of("grad_loss", grad_loss, f, N),
+            _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E), accumulate, N, E, V, layout, _storage(x), _stream())
 
 
 class _AtFirstCall:
