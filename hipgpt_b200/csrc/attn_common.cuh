@@ -173,6 +173,7 @@ int gemm_tc_status_fetch(int *status);
 void gemm_tc_release_scratch();
 // the ends of a training step (embedding.cu, linear_loss.cu)
 void embedding_release_scratch();
+int embedding_status_fetch(int *status);
 void loss_release_scratch();
 int loss_status_fetch(int *status);
 int launch_mha_generic(const float *q, const float *k, const float *v, float *out, float *probs,

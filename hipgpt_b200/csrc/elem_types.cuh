@@ -44,6 +44,11 @@ __device__ __forceinline__ void load_values(const T *p, float (&v)[W])
     } else if constexpr (W * sizeof(T) == 16) {
         const uint4 u = *reinterpret_cast<const uint4 *>(p);
         unpack(u, v, T());
+    } else if constexpr (W * sizeof(T) == 8) {
+        static_assert(sizeof(T) == 2, "four of bf16");
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xFFFF0000u);
+        v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xFFFF0000u);
     } else {
         static_assert(W * sizeof(T) == 32 && sizeof(T) == 4, "whole 16-byte words");
         const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
@@ -57,6 +62,8 @@ __device__ __forceinline__ void store_values(T *p, const float (&v)[W])
 {
     if constexpr (W == 1) {
         *p = from_float<T>(v[0]);
+    } else if constexpr (sizeof(T) == 2 && W == 4) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     } else if constexpr (sizeof(T) == 2) {
         static_assert(W == 8, "16 bytes of bf16");
         *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));

@@ -8,16 +8,20 @@
 // Both are bound by HBM: rows read once, rows written once.
 //
 // The gradient sums every row of the table in a fixed order, without atomics on values: the tokens are sorted by id first.
-//   sort_ids_kernel   one cluster of sixteen blocks sorts (id, t) by id, stable (so equal ids keep ascending t): two passes of
+//   sort_ids_kernel   one cluster of up to sixteen blocks sorts (id, t) by id, stable (so equal ids keep ascending t): two passes of
 //                     counting sort for vocabularies up to 2^20, three beyond; then writes where the entries of each row begin.
 //                     Within a pass a block counts its part's digits, the cluster's counts become offsets through
-//                     distributed shared memory, and every warp ranks 32 keys at a time among themselves (match).
-//   embed_sum_kernel  a group of up to 32 lanes takes 16 bytes a lane of one row of the table: adds its entries and stores the row, zeros
-//                     where there are none.  Words are not spread evenly (one id may take a tenth of the tokens, padding half of them), so a
-//                     row of more than C entries is summed in pieces of C by many groups; the group that finishes a row's last piece
-//                     adds the pieces, in ascending order whichever group it is.  The positions' table is summed in the same way over the batch.
+//                     distributed shared memory, and every warp ranks 32 keys at a time among themselves by votes.
+//   zero_rows_kernel  stores zeros in the rows without entries; embed_sum_kernel runs beside it.
+//   embed_sum_kernel  a group of threads fetches the rows of a piece of the sorted entries into shared memory, adds them up in order and stores each row of the table that
+//                     begins and ends in the piece.  Words are not spread evenly (one id may take a tenth of the tokens, padding half of them): pieces are
+//                     equal, not rows.  Of a row that falls to several pieces each leaves a sum in fp32, and the group that comes last adds them in
+//                     ascending order, whichever group it is.  The positions' table is summed
+//                     in the same way over the batch.
 #include "elem_types.cuh"
 #include "stream_workspace.hpp"
+
+#include <algorithm>
 
 namespace hipgpt {
 namespace {
@@ -67,8 +71,8 @@ int launch_embedding_scaled(const int *ids, const void *tok, const void *pos, vo
 
 // ---- the tokens in the order of their ids -----------------------------------------------------------------------------
 
-constexpr int kSortBlocks = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kKeysPerLane = 4, kWarpKeys = 32 * kKeysPerLane, kTileKeys = kSortWarps * kWarpKeys;
+constexpr int kMostSortBlocks = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kKeysPerLane = 4, kTileKeys = kSortThreads * kKeysPerLane;
 constexpr int kMostBits = 10, kMostBins = 1 << kMostBits;
 
 struct SortShared {
@@ -88,7 +92,7 @@ __device__ __forceinline__ int read_peer_int(const int *p, int rank)
 // ids [n] -> (id, t) sorted in `sorted` (ids outside [0, V) as V, last), row_start[v] = first entry of row v (v <= V; row_start[V] = entries inside), and
 // counters[0 .. ncounters) = 0.  `other`: a second buffer of n entries.  npass passes of `bits` bits; the last one ends in `sorted`.
 __global__ void __launch_bounds__(kSortThreads)
-sort_ids_kernel(const int *__restrict__ ids, int n, int V, int bits, int npass, int2 *sorted, int2 *other, int *row_start, int *counters, int ncounters)
+sort_ids_kernel(const int *__restrict__ ids, int n, int V, int blocks, int bits, int npass, int2 *sorted, int2 *other, int *row_start, int *counters, int ncounters)
 {
     extern __shared__ __align__(16) uint8_t sort_smem[];
     SortShared &s = *reinterpret_cast<SortShared *>(sort_smem);
@@ -96,27 +100,84 @@ sort_ids_kernel(const int *__restrict__ ids, int n, int V, int bits, int npass, 
     const int bins = 1 << bits;
     dependency_wait();
     dependents_may_start();
-    for (int i = rank * kSortThreads + tid; i < ncounters; i += kSortBlocks * kSortThreads) counters[i] = 0;
-    const int per = ((n + kSortBlocks - 1) / kSortBlocks + 31) / 32 * 32;
+    for (int i = rank * kSortThreads + tid; i < ncounters; i += blocks * kSortThreads) counters[i] = 0;
+    const int per = ((n + blocks - 1) / blocks + 31) / 32 * 32;
     const int from = min((long long)rank * per, (long long)n), to = min((long long)from + per, (long long)n);
+    // Where a block's part is one tile (up to 65536 tokens) the entries stay in registers between counting and placing, and the warps' counts are the block's
+    const bool single = per <= kTileKeys;
+    const int lane_keys = single ? (per + kSortThreads - 1) / kSortThreads : kKeysPerLane, warp_keys = 32 * lane_keys, warps = single ? (per + warp_keys - 1) / warp_keys : kSortWarps;
     const int2 *src = nullptr;
+    int2 e[kKeysPerLane];
+    int place[kKeysPerLane];
     for (int pass = 0; pass < npass; ++pass) {
         const int shift = pass * bits;
         int2 *dst = (npass - pass) & 1 ? sorted : other;
-        for (int d = tid; d < bins; d += kSortThreads) s.hist[d] = 0;
-        __syncthreads();
         auto entry = [&](int i) {
             if (pass) return __ldcg(src + i);
             const int id = ids[i];
             return make_int2(id >= 0 && id < V ? id : V, i);
         };
-        for (int i = from + tid; i < to; i += kSortThreads) atomicAdd(&s.hist[entry(i).x >> shift & (bins - 1)], 1);
+        // the entries of a tile, and each one's place among those of its digit in its warp; the warps' counts
+        auto rank_tile = [&](int t0) {
+            const int used = bins / 2;                // (two counts a word)
+#pragma unroll
+            for (int k = 0; k < kKeysPerLane; ++k) {
+                const int i = t0 + warp * warp_keys + k * 32 + lane;
+                e[k] = k < lane_keys && i < to ? entry(i) : make_int2(-1, 0);
+            }
+            if (warp < warps) {
+                uint32_t *mine = reinterpret_cast<uint32_t *>(s.warp_count[warp]);
+                for (int d = lane; d < used; d += 32) mine[d] = 0;
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < kKeysPerLane; ++k) {
+                    if (k >= lane_keys) break;
+                    const int d = e[k].x < 0 ? -1 : e[k].x >> shift & (bins - 1);
+                    // the lanes with the same digit, bit by bit (a match of the whole digits takes several times as long: it goes by the different ones)
+                    unsigned same = __ballot_sync(0xffffffffu, d >= 0);
+                    for (int b = 0; b < bits; ++b) {
+                        const unsigned with = __ballot_sync(0xffffffffu, d >> b & 1);
+                        same &= d >> b & 1 ? with : ~with;
+                    }
+                    const int before_me = __popc(same & ((1u << lane) - 1));
+                    const int seen = d >= 0 ? s.warp_count[warp][d] : 0;
+                    __syncwarp();
+                    place[k] = seen + before_me;
+                    if (d >= 0 && before_me == 0) s.warp_count[warp][d] = (unsigned short)(seen + __popc(same));
+                    __syncwarp();
+                }
+            }
+            __syncthreads();
+        };
+        // counts of the warps -> offsets among them; the sum
+        auto over_warps = [&] {
+            int all = 0;
+            if (tid < bins) {
+#pragma unroll 8
+                for (int w = 0; w < warps; ++w) {
+                    const int c = s.warp_count[w][tid];
+                    s.warp_count[w][tid] = (unsigned short)all;
+                    all += c;
+                }
+            }
+            return all;
+        };
+        if (single) {
+            rank_tile(from);
+            const int all = over_warps();
+            if (tid < bins) s.hist[tid] = all;
+        } else {
+            for (int d = tid; d < bins; d += kSortThreads) s.hist[d] = 0;
+            __syncthreads();
+            for (int i = from + tid; i < to; i += kSortThreads) atomicAdd(&s.hist[entry(i).x >> shift & (bins - 1)], 1);
+        }
         cluster_sync();
         // digit d = tid: keys of smaller digits anywhere, and of this digit in the blocks before
         int total = 0, before = 0;
         if (tid < bins)
 #pragma unroll
-            for (int r = 0; r < kSortBlocks; ++r) {
+            for (int r = 0; r < kMostSortBlocks; ++r) {
+                if (r >= blocks) break;
                 const int h = read_peer_int(&s.hist[tid], r);
                 total += h;
                 before += r < rank ? h : 0;
@@ -130,60 +191,39 @@ sort_ids_kernel(const int *__restrict__ ids, int n, int V, int bits, int npass, 
         if (lane == 31) s.warp_sum[warp] = incl;
         __syncthreads();
         int prev = 0;
-        for (int w = 0; w < warp; ++w) prev += s.warp_sum[w];
+        for (int w = 0; w < warp && w < bins / 32; ++w) prev += s.warp_sum[w];
         if (tid < bins) s.base[tid] = prev + incl - total + before;
+        __syncthreads();
         for (int t0 = from; t0 < to; t0 += kTileKeys) {
-            __syncthreads();
-            for (int i = tid; i < kSortWarps * bins; i += kSortThreads) s.warp_count[i >> bits][i & (bins - 1)] = 0;
-            __syncthreads();
-            int2 e[kKeysPerLane];
-            int place[kKeysPerLane];
-#pragma unroll
-            for (int k = 0; k < kKeysPerLane; ++k) {
-                const int i = t0 + warp * kWarpKeys + k * 32 + lane;
-                e[k] = i < to ? entry(i) : make_int2(-1, 0);
-            }
-#pragma unroll
-            for (int k = 0; k < kKeysPerLane; ++k) {
-                const int d = e[k].x < 0 ? -1 : e[k].x >> shift & (bins - 1);
-                const unsigned same = __match_any_sync(0xffffffffu, d);
-                const int mine = __popc(same & ((1u << lane) - 1));
-                const int seen = d >= 0 ? s.warp_count[warp][d] : 0;
-                __syncwarp();
-                place[k] = seen + mine;
-                if (d >= 0 && mine == 0) s.warp_count[warp][d] = (unsigned short)(seen + __popc(same));
-                __syncwarp();
-            }
-            __syncthreads();
-            // counts of the warps -> offsets among them; the next tile begins behind this one
             int all = 0;
-            if (tid < bins) {
-                for (int w = 0; w < kSortWarps; ++w) {
-                    const int c = s.warp_count[w][tid];
-                    s.warp_count[w][tid] = (unsigned short)all;
-                    all += c;
-                }
+            if (!single) {
+                rank_tile(t0);
+                all = over_warps();
+                __syncthreads();
             }
-            __syncthreads();
 #pragma unroll
             for (int k = 0; k < kKeysPerLane; ++k)
                 if (e[k].x >= 0) {
                     const int d = e[k].x >> shift & (bins - 1);
                     __stcg(dst + s.base[d] + s.warp_count[warp][d] + place[k], e[k]);
                 }
-            __syncthreads();
-            if (tid < bins) s.base[tid] += all;
+            if (!single) {
+                __syncthreads();
+                if (tid < bins) s.base[tid] += all;
+                __syncthreads();
+            }
         }
-        __threadfence();
         cluster_sync();                      // the pass's entries are all there, and nobody reads this block's counts any more
         src = dst;
     }
-    // rows between one entry's id and the next begin at the next; each warp fills the gaps of 32 entries together
+    // rows between one entry's id and the next begin at the next; a warp fills long gaps together
     for (int i0 = from + warp * 32; i0 < to; i0 += kSortThreads) {
         const int i = i0 + lane;
         const int key = i < n ? __ldcg(&src[i].x) : V, prev = i == 0 ? -1 : i <= n ? __ldcg(&src[i - 1].x) : V;
         const bool live = i < to;
-        unsigned gaps = __ballot_sync(0xffffffffu, live && key > prev);
+        if (live && key - prev <= 8)          // short gaps by the lane itself
+            for (int v = prev + 1; v <= key; ++v) row_start[v] = i;
+        unsigned gaps = __ballot_sync(0xffffffffu, live && key - prev > 8);
         while (gaps) {
             const int l = __ffs(gaps) - 1;
             gaps &= gaps - 1;
@@ -199,182 +239,248 @@ sort_ids_kernel(const int *__restrict__ ids, int n, int V, int bits, int npass, 
 
 // ---- sums of rows -----------------------------------------------------------------------------------------------------
 
-// Where the work of embed_sum_kernel lies.  Tasks of one group (2^lanes_log lanes, W values each: `slices` of them cover a row) in this order: pieces of
-// long rows, pieces of the batch of the positions' rows, rows.
-struct SumPlan {
-    int n, V, E, B, S;
-    int slices, lanes_log;
-    int piece, pieces;                        // entries of a piece of a long row; pieces of all entries
-    int pos_piece, pos_pieces;                // batches of a piece of a position's row, and how many; 0: no positions' table
-    long long pos_first, row_first, tasks;
-};
-
-template <typename G, int W>
-__device__ __forceinline__ void put_row(G *p, float (&v)[W], float scale, bool accumulate)
+// Rows of the table without entries.  Every block is resident at once, and lets embed_sum_kernel in, which stores the other rows.
+template <typename G>
+__global__ void __launch_bounds__(256)
+zero_rows_kernel(const int *__restrict__ row_start, G *grad_tok, int V, int E, int vec)
 {
+    constexpr int W = 16 / sizeof(G);
+    dependency_wait();
+    dependents_may_start();
+    const int lane = threadIdx.x & 31;
+    for (long long v0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8; v0 < V; v0 += gridDim.x * 64LL) {         // eight rows a warp at a time
+        const int start = __ldg(row_start + min((long long)V, v0 + min(lane, 8)));
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = __fmul_rn(v[j], scale);
-    if (accumulate) {
-        float old[W];
-        load_values<G, W>(p, old);
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = __fadd_rn(old[j], v[j]);
+        for (int i = 0; i < 8; ++i) {
+            if (__shfl_sync(0xffffffffu, start, i) != __shfl_sync(0xffffffffu, start, i + 1) || v0 + i >= V) continue;
+            G *row = grad_tok + (size_t)(v0 + i) * E;
+            if (vec) {
+                for (int e = lane * W; e < E; e += 32 * W) *reinterpret_cast<uint4 *>(row + e) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                for (int e = lane; e < E; e += 32) row[e] = from_float<G>(0.0f);
+            }
+        }
     }
-    store_values<G, W>(p, v);
 }
 
-// The lanes of a group that has stored its piece's sum: whether it is the last of `pieces` to do so (the others' sums are then visible)
-__device__ __forceinline__ bool last_piece(int *counter, int pieces, unsigned mask, int leader)
+// A block has kSumThreads threads, each 16 bytes of a row of gradients; they form groups of 2^row_log threads that cover a slice of a row (at most kSliceBytes).  A
+// group's task: a piece of the sorted entries, or of the batch at one position.  The rows of kRound entries at a time come into shared memory by
+// one bulk copy each, so that a group has all of them on their way at once without a register.
+constexpr int kSumThreads = 128, kSliceBytes = 16 * kSumThreads, kRound = 16, kSuper = 32;
+constexpr size_t kSumRows = (size_t)kSumThreads * 16 * kRound;          // bytes of a round's rows; behind them the entries
+
+__device__ int g_embed_status = 0;            // 1: a round's copies did not come
+
+struct SumPlan {
+    int n, V, E, B, S;
+    int slice, slices, row_log;               // columns of a slice, slices of a row, threads of a group
+    int units;                                // groups of at most a warp that cover a row
+    int piece, pieces;                        // entries of a piece, and how many
+    int pos_piece, pos_pieces;                // batches of a piece of a position's row, and how many; 0: no positions' table
+    long long pos_first, tasks;
+    int part_row;                             // values of a row of partial sums
+    int bulk, vec_out;                        // rows of gradients that a bulk copy can fetch; rows of the tables that take 16 bytes at a time
+};
+
+// Sums of rows that fall to several pieces are joined twice: those of up to kSuper pieces that follow one another, then what these give.  Places:
+// [2 piece + whether the row begins in it][part_row], and the same for each kSuper pieces
+struct Parts {
+    float *piece, *super;
+    int *piece_arrived, *super_arrived;
+};
+
+// Whether this group (a warp or a part of one) is the last of `count` that came here with what it stored; the others' sums are then visible
+__device__ __forceinline__ bool last_of(int *arrived, int count, unsigned mask, int leader)
 {
     __threadfence();
     __syncwarp(mask);
     int seen = 0;
-    if ((int)(threadIdx.x & 31) == leader) seen = atomicAdd(counter, 1);
+    if ((int)(threadIdx.x & 31) == leader) seen = atomicAdd(arrived, 1);
     seen = __shfl_sync(mask, seen, leader);
     __threadfence();
-    return seen == pieces - 1;
+    return seen == count - 1;
 }
 
-template <int W>
-__device__ __forceinline__ void add(float (&a)[W], const float (&b)[W])
+template <typename G, int W>
+__device__ __forceinline__ void put_row(G *p, const float (&sum)[W], float scale, bool accumulate, int left, bool vec)
 {
+    if (vec && left >= W) {
+        float v[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) a[j] = __fadd_rn(a[j], b[j]);
+        for (int j = 0; j < W; ++j) v[j] = __fmul_rn(sum[j], scale);
+        if (accumulate) {
+            float old[W];
+            load_values<G, W>(p, old);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] = __fadd_rn(old[j], v[j]);
+        }
+        store_values<G, W>(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (j < left) {
+                const float v = __fmul_rn(sum[j], scale);
+                p[j] = from_float<G>(accumulate ? __fadd_rn(to_float(p[j]), v) : v);
+            }
+    }
 }
 
-template <typename T, typename G, int W>
-__global__ void __launch_bounds__(256)
-embed_sum_kernel(const T *__restrict__ g, const int *__restrict__ ids, const int2 *__restrict__ sorted, const int *__restrict__ row_start, float *part, float *pos_part, int *counters,
-                 G *grad_tok, G *grad_pos, float scale, int accumulate, SumPlan p)
+template <typename T, typename G>
+__global__ void __launch_bounds__(kSumThreads)
+embed_sum_kernel(const T *__restrict__ g, const int *__restrict__ ids, const int2 *__restrict__ sorted, const int *__restrict__ row_start, Parts tok_parts, Parts pos_parts,
+                 G *grad_tok, G *grad_pos, float scale, int accumulate, int early, SumPlan p)
 {
-    dependency_wait();
+    constexpr int W = kPer16<T>;
+    extern __shared__ __align__(128) uint8_t rows_s[];       // [group][entry of the round][16 bytes a thread]
+    __shared__ uint64_t landed;
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) mbar_init(&landed, kSumThreads);
+    __syncthreads();
+    if (!early) dependency_wait();           // (early: zero_rows_kernel has let this one in, having waited for the sort; it is waited for at the end)
     dependents_may_start();
-    const int lanes = 1 << p.lanes_log, lane = threadIdx.x & 31, sub = lane & (lanes - 1), leader = lane - sub;
-    const unsigned mask = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1) << leader;
-    const long long task = ((long long)blockIdx.x * 256 + threadIdx.x) >> p.lanes_log;
-    if (task >= p.tasks) return;
-    constexpr int kAhead = W == 1 ? 8 : 4;
+    int2 (*entry_s)[kRound] = reinterpret_cast<int2 (*)[kRound]>(rows_s + kSumRows);         // [group][entry of the round]: row of the table, token (-1: not to be added)
+    const int size = 1 << p.row_log, groups = kSumThreads >> p.row_log, group = tid >> p.row_log, sub = tid & (size - 1);
+    const long long task = (long long)blockIdx.x * groups + group;
+    const bool live = task < p.tasks, pos = task >= p.pos_first;
+    const long long r = pos ? task - p.pos_first : task;
+    const int sl = (int)(r % p.slices), at = sl * p.slice, cols = min(p.slice, p.E - at), e = at + sub * W, left = at + cols - e;      // this thread's columns: e ... e + min(W, left)
+    const int s = (int)(r / p.slices % max(1, p.S)), c = (int)(pos ? r / p.slices / p.S : r / p.slices);
+    const int i0 = c * (pos ? p.pos_piece : p.piece), i1 = !live ? i0 : min(pos ? p.B : p.n, i0 + (pos ? p.pos_piece : p.piece));
+    const int longest = max(p.pos_pieces ? p.pos_piece : 0, p.piece);
+    // groups of at most a warp count for themselves
+    const unsigned mask = size >= 32 ? 0xffffffffu : ((1u << size) - 1) << (lane & ~(size - 1));
+    const int leader = size >= 32 ? 0 : lane & ~(size - 1), unit = sl * max(1, size / 32) + sub / 32;
+
+    const int key_before = !live || pos || i0 == 0 ? -1 : __ldg(&sorted[i0 - 1].x), key_behind = !live || pos || i1 == p.n ? -1 : __ldg(&sorted[i1].x);
+
     float acc[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-    // rows a .. b of the sorted entries, in order
-    auto sum_entries = [&](int a, int b, int e) {
-        int i = a;
-        for (; i + kAhead <= b; i += kAhead) {
-            float x[kAhead][W];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) load_values<T, W>(g + (size_t)__ldg(&sorted[i + k].y) * p.E + e, x[k]);
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) add(acc, x[k]);
-        }
-        for (; i < b; ++i) {
-            float x[W];
-            load_values<T, W>(g + (size_t)__ldg(&sorted[i].y) * p.E + e, x);
-            add(acc, x);
-        }
-    };
-    auto sum_parts = [&](const float *first, size_t stride, int count) {
+    auto clear = [&] {
 #pragma unroll
         for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-        int i = 0;
-        for (; i + 8 <= count; i += 8) {
-            float x[8][W];
+    };
+    // (rows of sums are padded: whole 16-byte words, whatever E)
+    auto store = [&](float *row) {
+        if (left <= 0) return;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+        for (int j = 0; j < W; j += 4) __stcg(reinterpret_cast<float4 *>(row + e + j), make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]));
+    };
+    // acc = rows first, first + stride, ... of sums
+    auto add_sums = [&](const float *first, size_t stride, int count) {
+        clear();
+        if (left <= 0) return;
+#pragma unroll (W == 4 ? 8 : 4)
+        for (int i = 0; i < count; ++i)
 #pragma unroll
-                for (int j = 0; j < W; ++j) x[k][j] = __ldcg(first + (i + k) * stride + j);
+            for (int j = 0; j < W; j += 4) {
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(first + i * stride + e + j));
+                acc[j] = __fadd_rn(acc[j], x.x);
+                acc[j + 1] = __fadd_rn(acc[j + 1], x.y);
+                acc[j + 2] = __fadd_rn(acc[j + 2], x.z);
+                acc[j + 3] = __fadd_rn(acc[j + 3], x.w);
+            }
+    };
+    // the sums of pieces `from` ... `to` of places that follow one another; the row begins in piece `begins` (or before)
+    auto join = [&](const float *places, size_t stride, int from, int to, int begins) {
+        if (from != begins) { add_sums(places + (size_t)(2 * from) * stride, 2 * stride, to - from + 1); return; }
+        add_sums(places + (size_t)(2 * from + 1) * stride, 0, 1);
+        float head[W];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) add(acc, x[k]);
-        }
-        for (; i < count; ++i) {
-            float x[W];
+        for (int j = 0; j < W; ++j) head[j] = acc[j];
+        add_sums(places + (size_t)(2 * (from + 1)) * stride, 2 * stride, to - from);
 #pragma unroll
-            for (int j = 0; j < W; ++j) x[j] = __ldcg(first + i * stride + j);
-            add(acc, x);
+        for (int j = 0; j < W; ++j) acc[j] = __fadd_rn(head[j], acc[j]);
+    };
+    // acc is the sum of what piece c has of a row that lies in pieces `first` ... `last`: true where this group then has the whole row's in acc.  stride: of the parts' rows
+    auto complete = [&](const Parts &parts, size_t stride, int first, int last) {
+        if (first == last) return true;
+        store(parts.piece + (size_t)(2 * c + (c == first)) * stride);
+        const int super = c / kSuper, from = max(first, super * kSuper), to = min(last, super * kSuper + kSuper - 1);
+        if (!last_of(parts.piece_arrived + (size_t)(2 * from + (from == first)) * p.units + unit, to - from + 1, mask, leader)) return false;
+        join(parts.piece, stride, from, to, first);
+        const int super0 = first / kSuper, super1 = last / kSuper;
+        if (super0 == super1) return true;
+        store(parts.super + (size_t)(2 * super + (super == super0)) * stride);
+        if (!last_of(parts.super_arrived + (size_t)(2 * super0 + 1) * p.units + unit, super1 - super0 + 1, mask, leader)) return false;
+        join(parts.super, stride, super0, super1, super0);
+        return true;
+    };
+    auto flush = [&](int v) {
+        if (pos) {
+            // places of a position's pieces: [place][S][row]
+            Parts q = pos_parts;
+            q.piece += (size_t)s * p.part_row;
+            q.super += (size_t)s * p.part_row;
+            q.piece_arrived += (size_t)s * 2 * p.pos_pieces * p.units;
+            q.super_arrived += (size_t)s * 2 * ((p.pos_pieces + kSuper - 1) / kSuper) * p.units;
+            if (complete(q, (size_t)p.S * p.part_row, 0, p.pos_pieces - 1)) put_row<G, W>(grad_pos + (size_t)s * p.E + e, acc, 1.0f, accumulate != 0, left, p.vec_out != 0);
+        } else {
+            int first = c, last = c;
+            if (v == key_before || v == key_behind) {        // it falls to several pieces
+                first = __ldg(row_start + v) / p.piece;
+                last = (__ldg(row_start + v + 1) - 1) / p.piece;
+            }
+            if (complete(tok_parts, p.part_row, first, last)) put_row<G, W>(grad_tok + (size_t)v * p.E + e, acc, scale, accumulate != 0, left, p.vec_out != 0);
         }
     };
-    if (task >= p.row_first) {
-        const long long r = task - p.row_first;
-        const int v = (int)(r / p.slices), e = ((int)(r % p.slices) * lanes + sub) * W;
-        if (e >= p.E) return;
-        const int a = __ldg(row_start + v), b = __ldg(row_start + v + 1);
-        if (b - a > p.piece || (accumulate && a == b)) return;      // summed in pieces; nothing to add
-        sum_entries(a, b, e);
-        put_row<G, W>(grad_tok + (size_t)v * p.E + e, acc, scale, accumulate != 0);
-        return;
-    }
-    if (task < p.pos_first) {
-        // a piece of the sorted entries: at most one long row ends or passes in it, and at most one begins
-        const int c = (int)(task / p.slices), sl = (int)(task % p.slices), e0 = (sl * lanes + sub) * W, e = e0 < p.E ? e0 : 0;      // (a lane past the row sums its first values for nothing: its group meets in the counting)
-        const int c0 = c * p.piece, c1 = min(p.n, c0 + p.piece);
-        int i = c0;
-        while (i < c1) {
-            const int v = __ldg(&sorted[i].x);
-            if (v >= p.V) return;
-            const int a = __ldg(row_start + v), b = __ldg(row_start + v + 1);
-            if (b - a > p.piece) {
-                const int first = a / p.piece, count = (b - 1) / p.piece - first + 1;
-#pragma unroll
-                for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-                sum_entries(max(a, c0), min(b, c1), e);
-                // a piece's sum of the row that was there before it, and of the one that begins in it
-                if (e0 < p.E)
-#pragma unroll
-                    for (int j = 0; j < W; ++j) __stcg(part + (size_t)(2 * c + (c == first)) * p.E + e + j, acc[j]);
-                if (last_piece(counters + first * p.slices + sl, count, mask, leader) && e0 < p.E) {
-                    sum_parts(part + (size_t)(2 * first + 1) * p.E + e, 0, 1);
-                    float head[W];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) head[j] = acc[j];
-                    sum_parts(part + (size_t)(2 * (first + 1)) * p.E + e, 2 * (size_t)p.E, count - 1);
-                    add(head, acc);
-                    put_row<G, W>(grad_tok + (size_t)v * p.E + e, head, scale, accumulate != 0);
-                }
+
+    clear();
+    int v = -1;                              // the row that acc belongs to
+    bool gone = false;                       // a round's copies have not come in time: nothing more is added or stored
+    for (int round = 0; round * kRound < longest; ++round) {
+        const int j0 = i0 + round * kRound, here = max(0, min(kRound, i1 - j0));
+        if (round) __syncthreads();          // the round before has been read
+        // the entries, and their rows on their way
+        uint32_t bytes = 0;
+        for (int k = sub; k < here; k += size) {
+            int2 en;
+            if (pos) {
+                const int t = (j0 + k) * p.S + s, id = __ldg(ids + t);
+                en = make_int2(s, id >= 0 && id < p.V ? t : -1);
+            } else {
+                en = __ldg(sorted + j0 + k);
+                if (en.x >= p.V) en.y = -1;
             }
-            i = b;
+            entry_s[group][k] = en;
+            if (p.bulk && !gone && en.y >= 0) bytes += (uint32_t)(cols * sizeof(T));
         }
-        return;
-    }
-    {
-        const long long r = task - p.pos_first;
-        const int sl = (int)(r % p.slices), e0 = (sl * lanes + sub) * W, e = e0 < p.E ? e0 : 0;
-        const int s = (int)(r / p.slices % p.S), c = (int)(r / p.slices / p.S);
-        const int b0 = c * p.pos_piece, b1 = min(p.B, b0 + p.pos_piece);
-        int b = b0;
-        for (; b + kAhead <= b1; b += kAhead) {
-            float x[kAhead][W];
-            bool ok[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const size_t t = (size_t)(b + k) * p.S + s;
-                const int id = __ldg(ids + t);
-                ok[k] = id >= 0 && id < p.V;
-                load_values<T, W>(g + t * p.E + e, x[k]);
+        if (p.bulk && !gone) {
+            mbar_arrive_expect_tx(&landed, bytes);
+            for (int k = sub; k < here; k += size) {
+                const int t = entry_s[group][k].y;
+                if (t >= 0) bulk_load(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16, g + (size_t)t * p.E + at, (uint32_t)(cols * sizeof(T)), &landed);
             }
+            __syncthreads();                 // the entries
+            if (!mbar_wait(&landed, (uint32_t)(round & 1))) {
+                gone = true;
+                atomicCAS(&g_embed_status, 0, 1);
+                linger();
+            }
+        } else {
+            __syncthreads();
+            for (int k = 0; k < here; ++k) {
+                const int t = entry_s[group][k].y;
+                T *to = reinterpret_cast<T *>(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16) + sub * W;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) if (ok[k]) add(acc, x[k]);
+                for (int j = 0; j < W; ++j) if (t >= 0 && j < left) to[j] = g[(size_t)t * p.E + e + j];
+            }
         }
-        for (; b < b1; ++b) {
-            const size_t t = (size_t)b * p.S + s;
-            const int id = __ldg(ids + t);
+        for (int k = 0; k < here && !gone; ++k) {
+            const int2 en = entry_s[group][k];
+            if (en.y < 0 && !pos) continue;
+            if (en.x != v) {
+                if (v >= 0) flush(v);
+                v = en.x;
+                clear();
+            }
+            if (en.y < 0) continue;
             float x[W];
-            load_values<T, W>(g + t * p.E + e, x);
-            if (id >= 0 && id < p.V) add(acc, x);
-        }
-        G *dst = grad_pos + (size_t)s * p.E + e;
-        if (p.pos_pieces == 1) {
-            if (e0 < p.E) put_row<G, W>(dst, acc, 1.0f, accumulate != 0);
-            return;
-        }
-        const size_t row = (size_t)s * p.E + e, stride = (size_t)p.S * p.E;
-        if (e0 < p.E)
+            load_values<T, W>(reinterpret_cast<const T *>(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16) + sub * W, x);
 #pragma unroll
-            for (int j = 0; j < W; ++j) __stcg(pos_part + c * stride + row + j, acc[j]);
-        if (last_piece(counters + p.pieces * p.slices + s * p.slices + sl, p.pos_pieces, mask, leader) && e0 < p.E) {
-            sum_parts(pos_part + row, stride, p.pos_pieces);
-            put_row<G, W>(dst, acc, 1.0f, accumulate != 0);
+            for (int j = 0; j < W; ++j) acc[j] = __fadd_rn(acc[j], x[j]);
         }
     }
+    if (v >= 0 && !gone) flush(v);
+    if (early) dependency_wait();
 }
 
 StreamWorkspace g_embed_ws;
@@ -386,26 +492,31 @@ template <typename T, typename G>
 int launch_embedding_backward(const void *grad_out, const int *ids, void *grad_tok, void *grad_pos, float scale, int accumulate, int B, int S, int V, int E, cudaStream_t st)
 {
     const int n = B * S;
-    // what a piece holds: long enough that few rows come in pieces, short enough that the last of a row's pieces is no long sum over the others
     SumPlan p = {};
     p.n = n; p.V = V; p.E = E; p.B = B; p.S = S;
-    const bool vec = E % kPer16<T> == 0 && all_aligned16({grad_out, grad_tok, grad_pos});
-    const int W = vec ? kPer16<T> : 1, words = ceil_div(E, W);
-    while ((1 << p.lanes_log) < words && p.lanes_log < 5) ++p.lanes_log;
-    p.slices = ceil_div(words, 1 << p.lanes_log);
-    p.piece = n > 65536 ? (n / 1024 + 31) / 32 * 32 : 64;
+    p.slice = std::min(E, kSliceBytes / (int)sizeof(T));
+    p.slices = ceil_div(E, p.slice);
+    while ((1 << p.row_log) * kPer16<T> < p.slice) ++p.row_log;
+    p.units = p.slices * std::max(1, (1 << p.row_log) / 32);
+    // a piece: one round of copies, or as many as leave 2048 pieces (so that joining twice is enough)
+    p.piece = kRound * std::max(1, ceil_div(n, 2048 * kRound));
     p.pieces = ceil_div(n, p.piece);
-    p.pos_piece = B > 4096 ? B / 64 : 64;
+    p.pos_piece = kRound * std::max(1, ceil_div(B, 2048 * kRound));
     p.pos_pieces = grad_pos ? ceil_div(B, p.pos_piece) : 0;
     p.pos_first = grad_tok ? (long long)p.pieces * p.slices : 0;
-    p.row_first = p.pos_first + (long long)p.pos_pieces * S * p.slices;
-    p.tasks = p.row_first + (grad_tok ? (long long)V * p.slices : 0);
-    const long long blocks = ((p.tasks << p.lanes_log) + 255) / 256;
-    const long long ncounters = (long long)p.pieces * p.slices + (p.pos_pieces > 1 ? (long long)S * p.slices : 0);
+    p.tasks = p.pos_first + (long long)p.pos_pieces * S * p.slices;
+    p.bulk = E * sizeof(T) % 16 == 0 && all_aligned16({grad_out});
+    p.vec_out = E % kPer16<T> == 0 && all_aligned16({grad_tok, grad_pos});
+    const int groups = kSumThreads >> p.row_log;
+    const long long blocks = (p.tasks + groups - 1) / groups;
+    p.part_row = (E + 7) / 8 * 8;
+    const int supers = ceil_div(p.pieces, kSuper), pos_supers = ceil_div(p.pos_pieces, kSuper);
+    const bool pos_parts = p.pos_pieces > 1;
+    const long long ncounters = 2LL * p.units * (p.pieces + supers + (pos_parts ? (long long)S * (p.pos_pieces + pos_supers) : 0));
     if (blocks > 2147483647LL || ncounters > 2147483647LL) return fail(HIPGPT_ERR_UNSUPPORTED, "a table of %d rows of %d values is beyond one call", V, E);
 
     const size_t entry_bytes = padded((size_t)n * sizeof(int2)), start_bytes = padded(((size_t)V + 1) * sizeof(int)), counter_bytes = padded((size_t)ncounters * sizeof(int));
-    const size_t part_bytes = padded((size_t)2 * p.pieces * E * sizeof(float)), pos_bytes = p.pos_pieces > 1 ? padded((size_t)p.pos_pieces * S * E * sizeof(float)) : 0;
+    const size_t row = (size_t)p.part_row * sizeof(float), part_bytes = padded(2 * (p.pieces + supers) * row), pos_bytes = pos_parts ? padded(2 * (p.pos_pieces + pos_supers) * S * row) : 0;
     StreamWorkspace::Lease ws;
     int rc = g_embed_ws.enter(st, 2 * entry_bytes + start_bytes + counter_bytes + part_bytes + pos_bytes, &ws);
     if (rc != HIPGPT_OK) return rc;
@@ -413,7 +524,15 @@ int launch_embedding_backward(const void *grad_out, const int *ids, void *grad_t
     auto take = [&](size_t bytes) { uint8_t *r = at; at += bytes; return r; };
     int2 *sorted = reinterpret_cast<int2 *>(take(entry_bytes)), *other = reinterpret_cast<int2 *>(take(entry_bytes));
     int *row_start = reinterpret_cast<int *>(take(start_bytes)), *counters = reinterpret_cast<int *>(take(counter_bytes));
-    float *part = reinterpret_cast<float *>(take(part_bytes)), *pos_part = reinterpret_cast<float *>(take(pos_bytes));
+    Parts tok, pos;
+    tok.piece = reinterpret_cast<float *>(take(part_bytes));
+    tok.super = tok.piece + (size_t)2 * p.pieces * p.part_row;
+    tok.piece_arrived = counters;
+    tok.super_arrived = counters + (size_t)2 * p.pieces * p.units;
+    pos.piece = reinterpret_cast<float *>(take(pos_bytes));
+    pos.super = pos.piece + (size_t)2 * p.pos_pieces * S * p.part_row;
+    pos.piece_arrived = tok.super_arrived + (size_t)2 * supers * p.units;
+    pos.super_arrived = pos.piece_arrived + (size_t)2 * p.pos_pieces * S * p.units;
 
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -428,14 +547,24 @@ int launch_embedding_backward(const void *grad_out, const int *ids, void *grad_t
     const int npass = ceil_div(key_bits, kMostBits), bits = ceil_div(key_bits, npass);
     if (!grad_tok) {                                                       // no order is asked for; nothing of the long rows runs
         if (e == cudaSuccess) e = cudaMemsetAsync(counters, 0, (size_t)ncounters * sizeof(int), st);
-    } else if (e == cudaSuccess) e = launch_overlapped_clusters(sort_ids_kernel, kSortBlocks, dim3(kSortBlocks), dim3(kSortThreads), sizeof(SortShared), st, ids, n, V, bits, npass, sorted, other, row_start,
-                                                         counters, (int)ncounters);
+    } else if (e == cudaSuccess) {
+        const int sort_blocks = n <= 1024 ? 1 : kMostSortBlocks;           // a cluster meets twice a pass, half a microsecond each: not for as few as one round of one block's threads
+        e = launch_overlapped_clusters(sort_ids_kernel, sort_blocks, dim3((unsigned)sort_blocks), dim3(kSortThreads), sizeof(SortShared), st, ids, n, V, sort_blocks, bits, npass, sorted, other,
+                                       row_start, counters, (int)ncounters);
+    }
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "sort_ids_kernel: %s", cudaGetErrorString(e));
     rc = check_launch("sort_ids_kernel");
     if (rc != HIPGPT_OK) return rc;
-    const auto kern = vec ? embed_sum_kernel<T, G, kPer16<T>> : embed_sum_kernel<T, G, 1>;
-    e = launch_overlapped(kern, dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const T *>(grad_out), ids, (const int2 *)sorted, (const int *)row_start, part, pos_part, counters,
-                          static_cast<G *>(grad_tok), static_cast<G *>(grad_pos), scale, accumulate, p);
+    const bool zeros = grad_tok && !accumulate && V > 0;
+    if (zeros) {
+        const int vec = (size_t)E * sizeof(G) % 16 == 0 && all_aligned16({grad_tok});
+        e = launch_overlapped(zero_rows_kernel<G>, dim3((unsigned)std::min(ceil_div(V, 64), 148 * 4)), dim3(256), 0, st, (const int *)row_start, static_cast<G *>(grad_tok), V, E, vec);
+        if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "zero_rows_kernel: %s", cudaGetErrorString(e));
+    }
+    static std::atomic<unsigned long long> sum_done{0};
+    e = once_per_device(sum_done, dev, [] { return cudaFuncSetAttribute(embed_sum_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSumRows + kSumThreads * kRound * sizeof(int2))); });
+    if (e == cudaSuccess) e = launch_overlapped(embed_sum_kernel<T, G>, dim3((unsigned)blocks), dim3(kSumThreads), kSumRows + groups * kRound * sizeof(int2), st, static_cast<const T *>(grad_out), ids, (const int2 *)sorted,
+                                                (const int *)row_start, tok, pos, static_cast<G *>(grad_tok), static_cast<G *>(grad_pos), scale, accumulate, (int)zeros, p);
     return e == cudaSuccess ? check_launch("embed_sum_kernel") : fail(HIPGPT_ERR_CUDA, "embed_sum_kernel: %s", cudaGetErrorString(e));
 }
 
@@ -450,6 +579,16 @@ int check_embedding_sizes(int B, int S, int V, int E, int type)
 }  // namespace
 
 void embedding_release_scratch() { g_embed_ws.release(); }
+
+int embedding_status_fetch(int *status)
+{
+    int v = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_embed_status, sizeof(v));
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
+    if (v) { const int zero = 0; cudaMemcpyToSymbol(g_embed_status, &zero, sizeof(zero)); }
+    *status = v;
+    return HIPGPT_OK;
+}
 
 }  // namespace hipgpt
 

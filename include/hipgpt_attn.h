@@ -418,7 +418,7 @@ HIPGPT_API int hipgpt_probe_fma(float *d_sink, int blocks, int iters, double *fl
  * waits on hardware barriers are bounded; a block whose wait runs out stores nothing and records
  * which wait it was: 1..8 for the split-TF32 kernel, 100 + site for the bf16 kernel, 300 + site
  * for the tiled fp32 kernel, 400 + site for the whole-head kernel, 500 + site for the tensor-core projections,
- * 600 + site for the attention backward, 700 + site for the loss, 900 + site for the test hook
+ * 600 + site for the attention backward, 700 + site for the loss, 801 for the embedding's gradient, 900 + site for the test hook
  * hipgpt_debug_wait_expiry.  This call waits for the whole
  * device (cudaDeviceSynchronize), stores the status word in *status and clears it.  0 means every
  * launch since the last call completed normally.  Callers of the device-pointer entry points
