@@ -43,7 +43,7 @@ constexpr int kOperand = kHalfM * kDeep * 2;            // bytes of one block's 
 constexpr int kEpiWarps = 16, kThreads = 32 * (kEpiWarps + 2);      // four warps share a row's columns
 constexpr int kWarpChunks = kTileN / 4 / 32;              // 32-column chunks of a warp
 constexpr int kTmemColumns = 512;
-constexpr int kPromote = 2;
+constexpr int kPromote = 4;
 constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
 // What a tile of kDz costs a pair beside its stages, in half stages
@@ -51,7 +51,8 @@ template <int NP> constexpr int kDzExtra = 4;
 template <int NP> constexpr int kRing = NP == 1 ? 6 : 3;
 constexpr int kRingBytes = 6 * 2 * kOperand;
 enum Form { kForward, kBackward };
-constexpr size_t kGemmSmem = kRingBytes + 1024;
+constexpr int kOutBytes = 32 * 64;                      // a warp's 32 rows of 64 bytes on their way out
+template <Form FORM> constexpr size_t kGemmSmem = kRingBytes + (FORM == kBackward ? kEpiWarps * kOutBytes : 0) + 1024;
 enum Kind { kDx, kDw, kDz };                            // problems of kBackward; kForward's one problem lies at kDz's place
 
 __device__ int g_loss_status = 0;
@@ -72,7 +73,7 @@ struct Problem {
 };
 
 struct LossArgs {
-    CUtensorMap a[3], b[3];
+    CUtensorMap a[3], b[3], dz_out;
     Problem p[3];
     const int *count;                        // rows that take part
     const int *row_map, *targets;            // of the rows that take part
@@ -82,8 +83,6 @@ struct LossArgs {
     float *z_target;
     float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
     int *arrived;                            // [tile][block of the pair][warp]: pairs that have left their share of a tile
-    uint16_t *dz;                            // kDz: [plane][rows][ld]
-    size_t dz_ld, dz_plane;
     int first, last;                         // the launch's share of dx is that of the first, the last piece
     size_t rows_alloc;
     int v0, V;                               // first column of the piece whose logits are formed, and of all
@@ -172,17 +171,18 @@ __device__ __forceinline__ float block_max(const float *v, int count, float (&sh
     return m;
 }
 
-// `cols` values of a row from `begin` on -> 16-bit ones in each plane, zeros from `cols` to `ld`; by one warp
+// The values of a row of `cols` from `begin` to `end` -> 16-bit ones in each plane, by one warp.  (What lies between `cols` and the next row is never read.)
 template <typename T>
 __device__ __forceinline__ void pack_row(const T *src, uint16_t *dst, size_t plane, int begin, int end, int cols, float scale, int lane, bool vec)
 {
+    end = min(end, cols);
     if constexpr (sizeof(T) == 2) {
         if (vec) {
 #pragma unroll 4
             for (int c = begin + lane * 8; c < end; c += 256) *reinterpret_cast<uint4 *>(dst + c) = __ldg(reinterpret_cast<const uint4 *>(src + c));
         } else {
 #pragma unroll 4
-            for (int c = begin + lane; c < end; c += 32) dst[c] = c < cols ? reinterpret_cast<const uint16_t *>(src)[c] : (uint16_t)0;
+            for (int c = begin + lane; c < end; c += 32) dst[c] = reinterpret_cast<const uint16_t *>(src)[c];
         }
     } else {
 #pragma unroll 4
@@ -674,6 +674,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         const uint32_t drained[2] = {peer_addr(smem_u32(&acc_empty[0]), 0), peer_addr(smem_u32(&acc_empty[1]), 0)};
         const float x_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 0)) : 1.0f, w_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 1)) : 1.0f;
         const float z_scale = x_inv * w_inv;
+        uint8_t *out_s = ring + kRingBytes + warp * kOutBytes;           // (kBackward)
         int unit = 0, part_at = 0;
         while (next(walk, x)) {
             const Problem &p = args.p[x.kind];
@@ -732,14 +733,24 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 run_max = m;
                 run_sum = s0 + s1;
             };
-            // kDz: 32 columns of a plane, whole sectors of the thread's row
-            auto put_dz = [&](int c, int plane, const uint32_t (&o)[16]) {
-                if (abort_flag) return;
-                float *dst = reinterpret_cast<float *>(args.dz + plane * args.dz_plane + (size_t)row * args.dz_ld + col0 + 32 * c);
+            // A thread's 64 bytes of its row into the warp's place in shared memory, swizzled so that a store instruction meets every bank once
+            auto stage_at = [&](int r, int j) { return reinterpret_cast<uint4 *>(out_s + r * 64 + ((j ^ (r >> 1 & 3)) << 4)); };
+            auto stage = [&](const uint32_t (&o)[16]) {
 #pragma unroll
-                for (int j = 0; j < 16; j += 8)
-                    store_sector(dst + j, __uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]), __uint_as_float(o[j + 4]), __uint_as_float(o[j + 5]),
-                                 __uint_as_float(o[j + 6]), __uint_as_float(o[j + 7]));
+                for (int j = 0; j < 4; ++j) *stage_at(lane, j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            };
+            // kDz: 32 columns of a plane by a bulk copy out of there
+            auto put_dz = [&](int c, int plane, const uint32_t (&o)[16]) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // what lay there is out
+                __syncwarp();
+                stage(o);
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0 && !abort_flag) {
+                    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                 ::"l"(reinterpret_cast<uint64_t>(&args.dz_out)), "r"(col0 + 32 * c), "r"(x.m * kTileM + rank * kHalfM + quarter * 32), "r"(plane), "r"(smem_u32(out_s)) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             };
             auto logit_gradient = [&](int c, float (&v)[32]) {
                 const int col = col0 + 32 * c, left = here ? left_all - 32 * c : 0;
@@ -785,19 +796,44 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             // kDx, kDw: 32 columns of a tile that is complete
             auto finish = [&](int c, float (&v)[32]) {
                 const int left = left_all - 32 * c;
-                if (left <= 0 || abort_flag) return;
+                if (left <= 0 || __any_sync(0xffffffffu, abort_flag)) return;
                 if (x.kind == kDx && !args.last) {
                     float4 *sum = args.sum + tile_at(x.tile, c);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) __stcg(sum + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
                     return;
                 }
-                if (!out_here) return;
                 if constexpr (NP == 2) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= out_scale;
                 }
-                put_columns<T>(static_cast<T *>(p.out) + out_row + col0 + 32 * c, v, left, p.accumulate != 0, out_vec);
+                const unsigned rows_here = __ballot_sync(0xffffffffu, out_here);
+                if (p.accumulate || !out_vec || left < 32) {
+                    if (out_here) put_columns<T>(static_cast<T *>(p.out) + out_row + col0 + 32 * c, v, left, p.accumulate != 0, out_vec);
+                    return;
+                }
+                // 64 bytes of each row at a time, four lanes a row: whole sectors, where a thread's own row by itself would be stored 16 bytes here and 16 there
+                constexpr int kPer64 = 64 / (int)sizeof(T);
+#pragma unroll
+                for (int h = 0; h < 32; h += kPer64) {
+                    uint32_t o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if constexpr (NP == 1) o[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                        else o[j] = __float_as_uint(v[h + j]);
+                    }
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+                    stage(o);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * i + (lane >> 2);
+                        const size_t at = __shfl_sync(0xffffffffu, out_row, r);
+                        const uint4 u = *stage_at(r, lane & 3);
+                        if (rows_here >> r & 1) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at + col0 + 32 * c + h + (lane & 3) * kPer16<T>) = u;
+                    }
+                }
             };
             // ... and of one that is not: into this pair's share
             auto leave = [&](int c, const float (&v)[32]) {
@@ -928,6 +964,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 }
             }
         }
+        if (FORM == kBackward && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     tc_fence_before();
@@ -973,16 +1010,16 @@ StreamWorkspace g_loss_ws;
 size_t padded(size_t bytes) { return (bytes + 1023) & ~(size_t)1023; }
 long long round_up(long long a, long long b) { return (a + b - 1) / b * b; }
 
-// {inner, outer, plane} of 16-bit values; box: 64 inner values (128 bytes, swizzled) of `box_outer` outer ones
-int operand_map(CUtensorMap *m, const void *base, bool half, long long inner, long long outer, long long ld, size_t plane, int planes, int box_outer)
+// {inner, outer, plane} of 16-bit values; box: 64 inner values (128 bytes; 32: 64 bytes) of `box_outer` outer ones, swizzled by its width
+int operand_map(CUtensorMap *m, const void *base, bool half, long long inner, long long outer, long long ld, size_t plane, int planes, int box_outer, int box_inner = 64)
 {
     EncodeTiledFn enc = tma_encode_fn();
     if (!enc) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)planes};
     const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1}, estr[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, estr[3] = {1, 1, 1};
     const CUresult r = enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
     return HIPGPT_OK;
 }
@@ -1001,8 +1038,8 @@ template <Form FORM, typename T>
 int launch_loss_gemm(LossArgs &a, int pairs, int dev, cudaStream_t st)
 {
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = once_per_device(done, dev, [] { return cudaFuncSetAttribute(loss_gemm_kernel<FORM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmSmem); });
-    if (e == cudaSuccess) e = launch_overlapped_clusters(loss_gemm_kernel<FORM, T>, 2, dim3((unsigned)(2 * pairs)), dim3(kThreads), kGemmSmem, st, a);
+    cudaError_t e = once_per_device(done, dev, [] { return cudaFuncSetAttribute(loss_gemm_kernel<FORM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmSmem<FORM>); });
+    if (e == cudaSuccess) e = launch_overlapped_clusters(loss_gemm_kernel<FORM, T>, 2, dim3((unsigned)(2 * pairs)), dim3(kThreads), kGemmSmem<FORM>, st, a);
     return e == cudaSuccess ? check_launch("loss_gemm_kernel") : fail(HIPGPT_ERR_CUDA, "loss_gemm_kernel: %s", cudaGetErrorString(e));
 }
 
@@ -1017,19 +1054,20 @@ struct Plan {
 };
 
 template <typename T>
-int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
+int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth)
 {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     p.N = N; p.E = E; p.V = V; p.layout = layout;
     const cudaError_t e = cudaGetDevice(&p.dev);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
-    p.x_ld = round_up(E, 8);
+    p.x_ld = round_up(E, 64);                        // (whole lines)
     p.rows_alloc = round_up(N, kTileM);
     p.w_rows = layout == HIPGPT_WEIGHTS_VE ? V : E;
     p.w_cols = layout == HIPGPT_WEIGHTS_VE ? E : V;
-    // 16-bit weights are read where they lie if TMA can (rows of whole 16-byte words); others are copied once per call
-    p.pack_w = NP == 2 || p.w_cols % 8 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0;
-    p.w_ld = round_up(p.w_cols, 8);
+    // 16-bit weights are read where they lie if TMA can (rows of whole 16-byte words); others are copied once per call, and so are those whose rows do not
+    // begin on lines where there are `worth` rows of x or more: the products then read two lines for each
+    p.pack_w = NP == 2 || p.w_cols % 8 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0 || (p.w_cols % 64 != 0 && N >= worth);
+    p.w_ld = p.pack_w ? round_up(p.w_cols, 64) : p.w_cols;
     p.x_plane = (size_t)p.rows_alloc * p.x_ld;
     p.w_plane = (size_t)p.w_rows * p.w_ld;
     size_t at = 0;
@@ -1063,7 +1101,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
     k.per_block = (int)(p.N <= 16384 ? 8 : round_up((p.N + 2047) / 2048, 8));      // (a block counts the targets before its rows)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
-    k.x_vec = p.E % kPer16<T> == 0 && p.E == p.x_ld && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
     k.plane = p.x_plane;
     k.count = ints; k.row_map = ints + 1; k.c_targets = ints + 1 + p.rows_alloc;
@@ -1076,7 +1114,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
         k.w_plane = p.w_plane;
         k.w_rows = (int)p.w_rows; k.w_cols = (int)p.w_cols; k.w_ld = (int)p.w_ld;
         k.w_col_pieces = (int)((p.w_ld + kPackCols - 1) / kPackCols);
-        k.w_vec = p.w_cols % kPer16<T> == 0 && p.w_cols == p.w_ld && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+        k.w_vec = p.w_cols % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
         w_blocks = (p.w_rows * k.w_col_pieces + 7) / 8;
     }
     *w_base = p.pack_w ? static_cast<const void *>(ws + p.w_at) : w;
@@ -1107,7 +1145,7 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
 {
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout);
+    int rc = plan_call<T>(p, w, N, E, V, layout, 4096);
     if (rc != HIPGPT_OK) return rc;
     const int n_tiles = (int)((V + kTileN - 1) / kTileN), m_tiles = (int)(p.rows_alloc / kTileM);
     if ((long long)m_tiles * n_tiles > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d V=%d is beyond one call", N, V);
@@ -1147,7 +1185,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout);
+    int rc = plan_call<T>(p, w, N, E, V, layout, 1024);
     if (rc != HIPGPT_OK) return rc;
     // pieces of the vocabulary of like size
     const long long most = std::max<long long>(1024, (long long)(kPieceBytes / ((size_t)p.rows_alloc * 2 * NP)) / kTileN * kTileN);
@@ -1177,11 +1215,9 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     a.shares = reinterpret_cast<float4 *>(ws + shares_at);
     a.sum = reinterpret_cast<float4 *>(ws + sum_at);
     a.expire = take_expiry(700);
-    a.dz_ld = (size_t)width;
-    a.dz_plane = dz_plane;
     // z[n][v]; dx[n][e] = sum_v dz[n][v] w[v][e]; dW[v][e] = sum_n dz[n][v] x[n][e], or dW[e][v]
-    auto dz_map = [&](CUtensorMap *m, int piece, int box) {
-        return operand_map(m, ws + dz_at + (piece & 1) * dz_bytes, NP == 2, width, p.rows_alloc, width, dz_plane, NP, box);
+    auto dz_map = [&](CUtensorMap *m, int piece, int box, int inner = 64) {
+        return operand_map(m, ws + dz_at + (piece & 1) * dz_bytes, NP == 2, width, p.rows_alloc, width, dz_plane, NP, box, inner);
     };
     rc = x_map<T>(&a.a[kDz], p, ws, false);
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb, ev);
@@ -1208,7 +1244,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
         z.n_tiles = i < pieces ? (int)((here + kTileN - 1) / kTileN) : 0;
         if (z.n_tiles) {
             a.v0 = z.b_n0 = (int)v0;
-            a.dz = reinterpret_cast<uint16_t *>(ws + dz_at + (i & 1) * dz_bytes);
+            rc = dz_map(&a.dz_out, i, 32, 32);
         }
         if (i > 0) {
             const long long o0 = v0 - width, old = std::min<long long>(width, V - o0);
