@@ -59,12 +59,10 @@ __device__ int g_loss_status = 0;
 
 // Sizes of one product D = A B (A: M x K, B: K x N), its place in the operands and what becomes of the result.
 struct Problem {
-    int m_tiles, n_tiles, stages;            // of 256, 256 and 64; n_tiles 0: not asked for
-    int narrow;                              // the last of the n_tiles has at most 128 columns
-    int n_fast;                              // tiles in a row: n runs fastest, or m
+    int n_tiles, stages;                     // kDz: columns of 256, depth of 64; n_tiles 0: not asked for
     int a_across, b_across;                  // operand contiguous across the reduction (along M or N) instead of along it
     int b_k0, b_n0;                          // where the product begins in B
-    int m_by_count, k_by_count;              // M, or K, is the number of rows that take part
+    int m_by_count;                          // M is the number of rows that take part
     // kDx, kDw: element (row, column) of the result at row * ld + column
     void *out;
     long long ld;
@@ -83,6 +81,7 @@ struct LossArgs {
     float *z_target;
     float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
     int *arrived;                            // [tile][block of the pair][warp]: pairs that have left their share of a tile
+    const struct Cut *cut;                   // the launch's
     int first, last;                         // the launch's share of dx is that of the first, the last piece
     size_t rows_alloc;
     int v0, V;                               // first column of the piece whose logits are formed, and of all
@@ -101,7 +100,7 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 
 // ---- rows that take part, moved together ------------------------------------------------------------------------------
 
-constexpr int kAmaxBlocks = 296;
+constexpr int kAmaxBlocks = 148;
 
 // partial[which][block] = largest finite |value| that the block has seen: x (rows that take part), w, g
 __global__ void __launch_bounds__(256)
@@ -353,16 +352,13 @@ __device__ __forceinline__ void put_columns(T *dst, const float (&v)[32], int co
 // How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
 // side by side read the same stages of it), as many whole rounds as leave every pair something over are dealt out tile by tile; the stages of the rest are cut into a length for
 // each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in half stages: a narrow tile's stages count half.
+struct Place { int tile, k; };               // tile: kDx's, then kDw's
 constexpr int kMostPairs = 128;
 struct Cut {
-    long long total[2], all;                 // of kDx, of both
     int m_tiles[2], n_tiles[2], stages[2], tiles[2], narrow[2], n_fast[2];
     int dealt;                               // tiles that are dealt out whole
-    long long begin[kMostPairs + 1];         // each pair's length of the rest
-    long long scan[4];
-    int fits;
+    Place begin[kMostPairs + 1];             // each pair's length of the rest
 };
-struct Place { int tile, k; };               // tile: kDx's, then kDw's
 
 // Tile u of problem i: its row and column of tiles, and what a stage of it counts
 struct TileOf { int m, n, unit; };
@@ -372,21 +368,29 @@ __device__ __forceinline__ TileOf tile_of(const Cut &c, int i, int u)
     const int m = c.n_fast[i] ? u / nt : u % mt, n = c.n_fast[i] ? u % nt : u / mt;
     return {m, n, c.narrow[i] && n == nt - 1 ? 1 : 2};
 }
+// Half stages of kDx, of both
+struct Lengths { long long first, all; };
+__device__ __forceinline__ Lengths lengths_of(const Cut &c)
+{
+    long long total[2];
+    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * c.stages[i] * max(0, 2 * c.n_tiles[i] - c.narrow[i]);
+    return {total[0], total[0] + total[1]};
+}
 // Half stages before tile t
-__device__ __forceinline__ long long place_before(const Cut &c, int t)
+__device__ __forceinline__ long long place_before(const Cut &c, const Lengths &len, int t)
 {
     const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
-    if (u >= c.tiles[i]) return c.all;
+    if (u >= c.tiles[i]) return len.all;
     const TileOf x = tile_of(c, i, u);
     const long long stages = c.stages[i];
     const long long here = c.n_fast[i] ? stages * ((long long)x.m * (2 * c.n_tiles[i] - c.narrow[i]) + 2 * x.n) : stages * (2LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
-    return (i ? c.total[0] : 0) + here;
+    return (i ? len.first : 0) + here;
 }
-__device__ __forceinline__ Place place_of(const Cut &c, long long at)
+__device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long long at)
 {
-    if (at >= c.all) return {c.tiles[0] + c.tiles[1], 0};
-    const int i = at >= c.total[0];
-    if (i) at -= c.total[0];
+    if (at >= len.all) return {c.tiles[0] + c.tiles[1], 0};
+    const int i = at >= len.first;
+    if (i) at -= len.first;
     const long long stages = c.stages[i];
     int u, unit;
     if (c.n_fast[i]) {
@@ -410,20 +414,54 @@ __device__ __forceinline__ Place place_of(const Cut &c, long long at)
 }
 __device__ __forceinline__ bool before(const Place &a, const Place &b) { return a.tile < b.tile || (a.tile == b.tile && a.k < b.k); }
 
-// By the first kMostPairs threads of a block (four warps): the pairs' lengths.  Tiles of kDz are dealt out one by one from pair 0 on and cost dz_cost each.
-__device__ __forceinline__ void cut_tiles(Cut &c, int pairs, int dz_tiles, int dz_cost)
+// What a call's launches are cut from
+struct PlanArgs {
+    int pieces, width, V, E, pairs, dz_stages, dz_extra;
+    int ev, with_x, with_w;
+};
+
+// A block for each launch of the backward, kMostPairs threads.  Tiles of kDz are dealt out one by one from pair 0 on.
+__global__ void __launch_bounds__(kMostPairs)
+loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
 {
-    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, tiles = c.tiles[0] + c.tiles[1];
-    const long long both = c.all + (long long)dz_cost * dz_tiles;
+    dependency_wait();
+    dependents_may_start();
+    __shared__ Cut c;
+    __shared__ Lengths len;
+    __shared__ long long scan[kMostPairs / 32];
+    __shared__ int all_fit;
+    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, launch = blockIdx.x, pairs = a.pairs, count = *count_at;
+    const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep), e_tiles = (a.E + kTileN - 1) / kTileN;
+    auto columns = [&](int piece) { return piece < 0 || piece >= a.pieces ? 0 : (int)min((long long)a.width, a.V - (long long)piece * a.width); };
+    auto narrow = [](int n) { return n && (n - 1) % kTileN < kTileN / 2 ? 1 : 0; };
+    const int old = columns(launch - 1), v_tiles = (old + kTileN - 1) / kTileN;
+    if (q == 0) {
+        c.m_tiles[0] = count_tiles;
+        c.n_tiles[0] = a.with_x && old ? e_tiles : 0;
+        c.stages[0] = (old + kDeep - 1) / kDeep;
+        c.narrow[0] = narrow(a.E);
+        c.n_fast[0] = 1;
+        c.m_tiles[1] = a.ev ? e_tiles : v_tiles;
+        c.n_tiles[1] = a.with_w && old ? (a.ev ? v_tiles : e_tiles) : 0;
+        c.stages[1] = count_stages;
+        c.narrow[1] = narrow(a.ev ? old : a.E);
+        c.n_fast[1] = !a.ev;
+        for (int i = 0; i < 2; ++i) c.tiles[i] = c.m_tiles[i] * c.n_tiles[i];
+        len = lengths_of(c);
+    }
+    __syncthreads();
+    const int tiles = c.tiles[0] + c.tiles[1], dz_tiles = count_tiles * ((columns(launch) + kTileN - 1) / kTileN);
+    const long long dz_cost = 2 * a.dz_stages + a.dz_extra, both = len.all + dz_cost * dz_tiles;
     for (int rounds = tiles / pairs;; --rounds) {
         const int dealt = max(0, rounds) * pairs;
-        long long load = 0, rest = c.all - place_before(c, dealt);
+        const long long rest = len.all - place_before(c, len, dealt);
+        long long load = 0;
         if (q < pairs) {
             for (int t = q; t < dealt; t += pairs) {
                 const int i = t >= c.tiles[0];
                 load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * c.stages[i];
             }
-            load += (long long)dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
+            load += dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
         }
         long long incl = load;
 #pragma unroll
@@ -431,28 +469,31 @@ __device__ __forceinline__ void cut_tiles(Cut &c, int pairs, int dz_tiles, int d
             const long long up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += up;
         }
-        if (lane == 31) c.scan[warp] = incl;
-        if (q == 0) c.fits = 1;
-        asm volatile("bar.sync 15, 128;" ::: "memory");
-        for (int w = 0; w < warp; ++w) incl += c.scan[w];
+        if (lane == 31) scan[warp] = incl;
+        if (q == 0) all_fit = 1;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) incl += scan[w];
         // what is left for the pairs before this one when each has an equal part of everything; a length of at least four stages each
-        const long long begin = both * q / pairs - (incl - load);
-        const long long mine = both * (q + 1) / pairs - incl - begin;
-        if (q < pairs && mine < 8 && (rest > 0 || dealt > 0)) c.fits = 0;
-        asm volatile("bar.sync 15, 128;" ::: "memory");
-        const bool fits = c.fits != 0;
+        const long long begin = both * q / pairs - (incl - load), mine = both * (q + 1) / pairs - incl - begin;
+        if (q < pairs && mine < 8) all_fit = 0;
+        __syncthreads();
+        const bool fits = all_fit != 0;
         if (!fits && rounds > 0) continue;
         if (q == 0) c.dealt = dealt;
         if (q <= pairs) {
+            long long at;
             if (fits) {
-                c.begin[q] = (c.all - rest) + (q < pairs ? begin : rest);
+                at = (len.all - rest) + (q < pairs ? begin : rest);
             } else {                         // too little for equal parts beside kDz's tiles: equal lengths of eight stages or more, for as many pairs as that gives
-                const int active = (int)max(1LL, min((long long)pairs, c.all / 16));
-                c.begin[q] = q >= active ? c.all : c.all * q / active;
+                const int active = (int)max(1LL, min((long long)pairs, len.all / 16));
+                at = q >= active ? len.all : len.all * q / active;
             }
+            c.begin[q] = place_of(c, len, at);
         }
-        return;
+        break;
     }
+    __syncthreads();
+    for (int i = q; i < (int)(sizeof(Cut) / sizeof(int)); i += kMostPairs) reinterpret_cast<int *>(cuts + launch)[i] = reinterpret_cast<const int *>(&c)[i];
 }
 
 // What a pair does, one after the other: its tiles of kDx and kDw, its length of the rest of them, its tiles of kDz
@@ -521,38 +562,12 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
     __shared__ Cut cut;
-    __shared__ Walk first;
-    if (threadIdx.x == 0) {
-        first = {0, {0, 0}, {0, 0}, pair, 0, count_tiles};
-        if (args.p[kDz].n_tiles) first.dz_tiles = count_tiles * args.p[kDz].n_tiles;
-        cut = {};
-        if constexpr (FORM == kBackward) {
-            for (int i = 0; i < 2; ++i) {
-                const Problem &p = args.p[i];
-                cut.m_tiles[i] = p.m_by_count ? count_tiles : p.m_tiles;
-                cut.n_tiles[i] = p.n_tiles;
-                cut.stages[i] = p.k_by_count ? count_stages : p.stages;
-                cut.tiles[i] = cut.m_tiles[i] * p.n_tiles;
-                cut.narrow[i] = p.narrow;
-                cut.n_fast[i] = p.n_fast;
-                cut.total[i] = (long long)cut.m_tiles[i] * cut.stages[i] * max(0, 2 * p.n_tiles - p.narrow);
-            }
-            cut.all = cut.total[0] + cut.total[1];
-        }
-    }
-    __syncthreads();
     if constexpr (FORM == kBackward) {
-        if (cut.all) {
-            if (threadIdx.x < kMostPairs) cut_tiles(cut, pairs, first.dz_tiles, 2 * args.p[kDz].stages + kDzExtra<NP>);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                first.dealt = pair < cut.dealt ? pair : cut.dealt;
-                first.at = place_of(cut, cut.begin[pair]);
-                first.end = place_of(cut, cut.begin[pair + 1]);
-            }
-            __syncthreads();
-        }
+        for (int i = threadIdx.x; i < (int)(sizeof(Cut) / sizeof(int)); i += kThreads) reinterpret_cast<int *>(&cut)[i] = reinterpret_cast<const int *>(args.cut)[i];
+        __syncthreads();
     }
+    Walk first = {0, {0, 0}, {0, 0}, pair, count_tiles * args.p[kDz].n_tiles, count_tiles};
+    if constexpr (FORM == kBackward) first = {min(pair, cut.dealt), cut.begin[pair], cut.begin[pair + 1], pair, count_tiles * args.p[kDz].n_tiles, count_tiles};
     auto next = [&](Walk &w, Work &x) {
         if constexpr (FORM == kBackward) {
             const bool deal = w.dealt < cut.dealt;
@@ -594,7 +609,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 for (int k = KIND == kDz ? 0 : x.k0; k < end; ++k) {
                     if (round) wait(&empty[s], (uint32_t)((round - 1) & 1), 2);
                     if (elect_one() && seen) {
-                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(x.narrow ? 2 * STAGE - NP * kOperand : 2 * STAGE));
                         const uint32_t bar = full_of_first + (uint32_t)(s * sizeof(uint64_t));
                         uint8_t *at = ring + s * STAGE;
 #pragma unroll
@@ -607,12 +622,9 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                             } else {
                                 tma_load_pair(a, ma, ka, m0, pl, bar);
                             }
-                            if (p.b_across) {
-                                tma_load_pair(b, mb, n0, kb, pl, bar);
-                                tma_load_pair(b + kOperand / 2, mb, n0 + 64, kb, pl, bar);
-                            } else {
-                                tma_load_pair(b, mb, kb, n0, pl, bar);
-                            }
+                            // (64 columns at a time either way: a narrow tile has no more)
+                            tma_load_pair(b, mb, p.b_across ? n0 : kb, p.b_across ? kb : n0, pl, bar);
+                            if (!x.narrow) tma_load_pair(b + kOperand / 2, mb, p.b_across ? n0 + 64 : kb, p.b_across ? kb : n0 + 64, pl, bar);
                         }
                     }
                     __syncwarp();
@@ -646,7 +658,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                         tc_fence_after();
                         const uint32_t at = smem_u32(ring + s * STAGE);
                         const uint64_t a = make_desc(at, a_lbo, 1024, 2), b = make_desc(at + NP * kOperand, b_lbo, 1024, 2);
-                        constexpr uint64_t lo = kOperand >> 4;
+                        [[maybe_unused]] constexpr uint64_t lo = kOperand >> 4;
 #pragma unroll
                         for (int j = 0; j < kDeep / 16; ++j) {
                             if constexpr (NP == 2) {
@@ -850,8 +862,8 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             if (FORM == kBackward && x.kind != kDz) {
                 if (!whole) {
                     const Place tile_begin = {x.tile, 0}, tile_end = {x.tile, x.stages};
-                    while (p0 > 0 && before(tile_begin, place_of(cut, cut.begin[p0]))) --p0;
-                    while (before(place_of(cut, cut.begin[p1 + 1]), tile_end)) ++p1;
+                    while (p0 > 0 && before(tile_begin, cut.begin[p0])) --p0;
+                    while (before(cut.begin[p1 + 1], tile_end)) ++p1;
                     arrived = args.arrived + ((size_t)x.tile * 2 + rank) * kEpiWarps + warp;
                     if (pair == p0) {
                         int there = 0;
@@ -1099,7 +1111,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.amax = amax;
     k.targets = targets; k.lse = lse; k.g = g;
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
-    k.per_block = (int)(p.N <= 16384 ? 8 : round_up((p.N + 2047) / 2048, 8));      // (a block counts the targets before its rows)
+    k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
@@ -1128,16 +1140,16 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     return check_launch("loss_pack_kernel");
 }
 
-// Maps of the operands of one problem: `across`: contiguous across the reduction, boxes of 64 x 64; along it: boxes of 64 x 128 rows
+// Maps of the operands of one problem, in boxes of 64 x 64; A contiguous along the reduction: of 64 x 128 rows
 template <typename T>
-int x_map(CUtensorMap *m, const Plan &p, const uint8_t *ws, bool across)
+int x_map(CUtensorMap *m, const Plan &p, const uint8_t *ws, int box)
 {
-    return operand_map(m, ws + p.x_at, sizeof(T) == 4, p.E, p.rows_alloc, p.x_ld, p.x_plane, sizeof(T) == 4 ? 2 : 1, across ? kDeep : kHalfM);
+    return operand_map(m, ws + p.x_at, sizeof(T) == 4, p.E, p.rows_alloc, p.x_ld, p.x_plane, sizeof(T) == 4 ? 2 : 1, box);
 }
 template <typename T>
-int w_map(CUtensorMap *m, const Plan &p, const void *w, bool across)
+int w_map(CUtensorMap *m, const Plan &p, const void *w)
 {
-    return operand_map(m, w, sizeof(T) == 4, p.w_cols, p.w_rows, p.w_ld, p.w_plane, sizeof(T) == 4 ? 2 : 1, across ? kDeep : kHalfM);
+    return operand_map(m, w, sizeof(T) == 4, p.w_cols, p.w_rows, p.w_ld, p.w_plane, sizeof(T) == 4 ? 2 : 1, 64);
 }
 
 template <typename T>
@@ -1160,8 +1172,8 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     int pairs = 1;
     rc = loss_pairs(p.dev, (long long)m_tiles * n_tiles, &pairs);
     if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, st, &wb);
-    if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, false);
-    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb, ev);
+    if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, kHalfM);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
     if (rc != HIPGPT_OK) return rc;
     Problem &q = a.p[kDz];
     q.n_tiles = n_tiles;
@@ -1193,7 +1205,6 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     const int pieces = (int)((V + width - 1) / width);
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
     const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM), piece_tiles = (int)(width / kTileN);
-    const bool e_narrow = (E - 1) % kTileN < kTileN / 2;
     const long long dx_tiles = grad_x ? (long long)m_tiles * e_tiles : 0, dw_tiles = grad_w ? (long long)piece_tiles * e_tiles : 0;
     if (dx_tiles + dw_tiles > 1 << 26 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
     int pairs = 1;
@@ -1203,8 +1214,9 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     const size_t tile_bytes = (size_t)kTileM * kTileN * sizeof(float), dz_plane = (size_t)p.rows_alloc * width, dz_bytes = padded(NP * dz_plane * 2);
     const size_t dz_at = p.end, shares_at = dz_at + (pieces > 1 ? 2 : 1) * dz_bytes, sum_at = shares_at + 2 * pairs * tile_bytes, arrived_at = sum_at + (pieces > 1 ? dx_tiles * tile_bytes : 0);
     const int arrived = (int)(dx_tiles + dw_tiles) * 2 * kEpiWarps;
+    const size_t cuts_at = arrived_at + padded((size_t)arrived * sizeof(int));
     StreamWorkspace::Lease lease;
-    rc = g_loss_ws.enter(st, arrived_at + padded((size_t)arrived * sizeof(int)), &lease);
+    rc = g_loss_ws.enter(st, cuts_at + padded((size_t)(pieces + 1) * sizeof(Cut)), &lease);
     if (rc != HIPGPT_OK) return rc;
     uint8_t *ws = lease.get();
     LossArgs a = {};
@@ -1212,6 +1224,10 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     a.arrived = reinterpret_cast<int *>(ws + arrived_at);
     rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, st, &wb);
     if (rc != HIPGPT_OK) return rc;
+    Cut *cuts = reinterpret_cast<Cut *>(ws + cuts_at);
+    const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr};
+    const cudaError_t e = launch_overlapped(loss_plan_kernel, dim3((unsigned)(pieces + 1)), dim3(kMostPairs), 0, st, plan, a.count, cuts);
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_plan_kernel: %s", cudaGetErrorString(e));
     a.shares = reinterpret_cast<float4 *>(ws + shares_at);
     a.sum = reinterpret_cast<float4 *>(ws + sum_at);
     a.expire = take_expiry(700);
@@ -1219,28 +1235,25 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     auto dz_map = [&](CUtensorMap *m, int piece, int box, int inner = 64) {
         return operand_map(m, ws + dz_at + (piece & 1) * dz_bytes, NP == 2, width, p.rows_alloc, width, dz_plane, NP, box, inner);
     };
-    rc = x_map<T>(&a.a[kDz], p, ws, false);
-    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb, ev);
-    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDx], p, wb, !ev);
-    if (rc == HIPGPT_OK) rc = x_map<T>(ev ? &a.a[kDw] : &a.b[kDw], p, ws, true);
+    rc = x_map<T>(&a.a[kDz], p, ws, kHalfM);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
+    if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDx], p, wb);
+    if (rc == HIPGPT_OK) rc = x_map<T>(ev ? &a.a[kDw] : &a.b[kDw], p, ws, 64);
     if (rc != HIPGPT_OK) return rc;
     a.p[kDz].stages = (E + kDeep - 1) / kDeep;
     a.p[kDz].b_across = ev;
     a.p[kDz].m_by_count = 1;
-    a.p[kDx].narrow = e_narrow;
-    a.p[kDx].n_fast = 1;                             // (the tiles of E next to one another, in both)
-    a.p[kDw].n_fast = !ev;
     a.p[kDx].b_across = !ev;
     a.p[kDx].m_by_count = 1;
     a.p[kDx].out = grad_x;
     a.p[kDx].ld = a.p[kDx].cols = E;
     a.p[kDw].a_across = a.p[kDw].b_across = 1;
-    a.p[kDw].k_by_count = 1;
     a.p[kDw].accumulate = accumulate_w;
     a.p[kDw].ld = ev ? V : E;
     for (int i = 0; i <= pieces; ++i) {              // the logits' gradient of piece i, the products with that of piece i - 1
         Problem &z = a.p[kDz], &dx = a.p[kDx], &dw = a.p[kDw];
         const long long v0 = i * width, here = std::min<long long>(width, V - v0);
+        a.cut = cuts + i;
         z.n_tiles = i < pieces ? (int)((here + kTileN - 1) / kTileN) : 0;
         if (z.n_tiles) {
             a.v0 = z.b_n0 = (int)v0;
@@ -1248,19 +1261,13 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
         }
         if (i > 0) {
             const long long o0 = v0 - width, old = std::min<long long>(width, V - o0);
-            const int v_tiles = (int)((old + kTileN - 1) / kTileN);
             a.first = i == 1;
             a.last = i == pieces;
             if (grad_x) {
-                dx.n_tiles = e_tiles;
-                dx.stages = (int)((old + kDeep - 1) / kDeep);
                 dx.b_k0 = (int)o0;
                 if (rc == HIPGPT_OK) rc = dz_map(&a.a[kDx], i - 1, kHalfM);
             }
             if (grad_w) {
-                dw.m_tiles = ev ? e_tiles : v_tiles;
-                dw.n_tiles = ev ? v_tiles : e_tiles;
-                dw.narrow = ev ? (old - 1) % kTileN < kTileN / 2 : e_narrow;
                 dw.rows = ev ? E : (int)old;
                 dw.cols = ev ? (int)old : E;
                 dw.out = static_cast<T *>(grad_w) + (ev ? o0 : o0 * E);
