@@ -46,8 +46,8 @@ constexpr int kTmemColumns = 512;
 constexpr int kPromote = 4;
 constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
-// What a tile of kDz costs a pair beside its stages, in half stages
-template <int NP> constexpr int kDzExtra = 4;
+// What a tile of kDz costs a pair beside its stages, in quarter stages
+template <int NP> constexpr int kDzExtra = 8;
 template <int NP> constexpr int kRing = NP == 1 ? 6 : 3;
 constexpr int kRingBytes = 6 * 2 * kOperand;
 enum Form { kForward, kBackward };
@@ -351,7 +351,8 @@ __device__ __forceinline__ void put_columns(T *dst, const float (&v)[32], int co
 
 // How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
 // side by side read the same stages of it), as many whole rounds as leave every pair something over are dealt out tile by tile; the stages of the rest are cut into a length for
-// each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in half stages: a narrow tile's stages count half.
+// each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in quarter stages: a narrow
+// tile's stages count three (they fetch three quarters, and that is what bounds them).
 struct Place { int tile, k; };               // tile: kDx's, then kDw's
 constexpr int kMostPairs = 128;
 struct Cut {
@@ -366,24 +367,24 @@ __device__ __forceinline__ TileOf tile_of(const Cut &c, int i, int u)
 {
     const int nt = c.n_tiles[i], mt = c.m_tiles[i];
     const int m = c.n_fast[i] ? u / nt : u % mt, n = c.n_fast[i] ? u % nt : u / mt;
-    return {m, n, c.narrow[i] && n == nt - 1 ? 1 : 2};
+    return {m, n, c.narrow[i] && n == nt - 1 ? 3 : 4};
 }
-// Half stages of kDx, of both
+// Quarter stages of kDx, of both
 struct Lengths { long long first, all; };
 __device__ __forceinline__ Lengths lengths_of(const Cut &c)
 {
     long long total[2];
-    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * c.stages[i] * max(0, 2 * c.n_tiles[i] - c.narrow[i]);
+    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * c.stages[i] * max(0, 4 * c.n_tiles[i] - c.narrow[i]);
     return {total[0], total[0] + total[1]};
 }
-// Half stages before tile t
+// Quarter stages before tile t
 __device__ __forceinline__ long long place_before(const Cut &c, const Lengths &len, int t)
 {
     const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
     if (u >= c.tiles[i]) return len.all;
     const TileOf x = tile_of(c, i, u);
     const long long stages = c.stages[i];
-    const long long here = c.n_fast[i] ? stages * ((long long)x.m * (2 * c.n_tiles[i] - c.narrow[i]) + 2 * x.n) : stages * (2LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
+    const long long here = c.n_fast[i] ? stages * ((long long)x.m * (4 * c.n_tiles[i] - c.narrow[i]) + 4 * x.n) : stages * (4LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
     return (i ? len.first : 0) + here;
 }
 __device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long long at)
@@ -394,18 +395,18 @@ __device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long
     const long long stages = c.stages[i];
     int u, unit;
     if (c.n_fast[i]) {
-        const long long row = stages * (2 * c.n_tiles[i] - c.narrow[i]);
+        const long long row = stages * (4 * c.n_tiles[i] - c.narrow[i]);
         const long long m = at / row;
         at -= m * row;
-        const int n = (int)min(at / (2 * stages), (long long)c.n_tiles[i] - 1);
-        at -= n * 2 * stages;
-        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 1 : 2;
+        const int n = (int)min(at / (4 * stages), (long long)c.n_tiles[i] - 1);
+        at -= n * 4 * stages;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
         u = (int)m * c.n_tiles[i] + n;
     } else {
-        const long long column = 2 * stages * c.m_tiles[i];
+        const long long column = 4 * stages * c.m_tiles[i];
         const int n = (int)min(at / column, (long long)c.n_tiles[i] - 1);
         at -= n * column;
-        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 1 : 2;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
         const int m = (int)(at / (unit * stages));
         at -= m * unit * stages;
         u = n * c.m_tiles[i] + m;
@@ -451,7 +452,7 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
     }
     __syncthreads();
     const int tiles = c.tiles[0] + c.tiles[1], dz_tiles = count_tiles * ((columns(launch) + kTileN - 1) / kTileN);
-    const long long dz_cost = 2 * a.dz_stages + a.dz_extra, both = len.all + dz_cost * dz_tiles;
+    const long long dz_cost = 4 * a.dz_stages + a.dz_extra, both = len.all + dz_cost * dz_tiles;
     for (int rounds = tiles / pairs;; --rounds) {
         const int dealt = max(0, rounds) * pairs;
         const long long rest = len.all - place_before(c, len, dealt);
@@ -475,7 +476,7 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
         for (int w = 0; w < warp; ++w) incl += scan[w];
         // what is left for the pairs before this one when each has an equal part of everything; a length of at least four stages each
         const long long begin = both * q / pairs - (incl - load), mine = both * (q + 1) / pairs - incl - begin;
-        if (q < pairs && mine < 8) all_fit = 0;
+        if (q < pairs && mine < 16) all_fit = 0;
         __syncthreads();
         const bool fits = all_fit != 0;
         if (!fits && rounds > 0) continue;
@@ -485,7 +486,7 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
             if (fits) {
                 at = (len.all - rest) + (q < pairs ? begin : rest);
             } else {                         // too little for equal parts beside kDz's tiles: equal lengths of eight stages or more, for as many pairs as that gives
-                const int active = (int)max(1LL, min((long long)pairs, len.all / 16));
+                const int active = (int)max(1LL, min((long long)pairs, len.all / 32));
                 at = q >= active ? len.all : len.all * q / active;
             }
             c.begin[q] = place_of(c, len, at);
@@ -574,7 +575,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             if (deal || before(w.at, w.end)) {
                 const int t = deal ? w.dealt : w.at.tile, i = t >= cut.tiles[0];
                 const TileOf place = tile_of(cut, i, t - (i ? cut.tiles[0] : 0));
-                x = {i, place.m, place.n, deal ? 0 : w.at.k, deal || t != w.end.tile ? cut.stages[i] : w.end.k, cut.stages[i], t, place.unit == 1};
+                x = {i, place.m, place.n, deal ? 0 : w.at.k, deal || t != w.end.tile ? cut.stages[i] : w.end.k, cut.stages[i], t, place.unit == 3};
                 if (deal) w.dealt += pairs; else w.at = {t + 1, 0};
                 return true;
             }
@@ -865,14 +866,6 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     while (p0 > 0 && before(tile_begin, cut.begin[p0])) --p0;
                     while (before(cut.begin[p1 + 1], tile_end)) ++p1;
                     arrived = args.arrived + ((size_t)x.tile * 2 + rank) * kEpiWarps + warp;
-                    if (pair == p0) {
-                        int there = 0;
-                        if (lane == 0) there = *reinterpret_cast<volatile int *>(arrived);
-                        there = __shfl_sync(0xffffffffu, there, 0);
-                        __threadfence();
-                        complete = there == p1 - p0;
-                        if (complete && lane == 0) *arrived = 0;         // for the next launch
-                    }
                 }
                 sources = (p1 - p0) + (x.kind == kDx && !args.first);
             }
@@ -924,6 +917,14 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 tmem_wait_ld();
                 release(unit & 1);
                 ++unit;
+            }
+            if (FORM == kBackward && !whole && pair == p0) {
+                int there = 0;
+                if (lane == 0) there = *reinterpret_cast<volatile int *>(arrived);
+                there = __shfl_sync(0xffffffffu, there, 0);
+                __threadfence();
+                complete = there == p1 - p0;
+                if (complete && lane == 0) *arrived = 0;                 // for the next launch
             }
 #pragma unroll
             for (int c = 0; c < kWarpChunks; ++c) {
