@@ -9,12 +9,17 @@
 // The scale belongs to the probability that is used (a multiple of 2^-16), so the expected value is the input's.  A dropped
 // element is 0 whatever it held, NaN and infinities too.  fp32 arithmetic, rounded once.
 //
-// Bound: HBM.  16 bits a value, not 32, because the generator's ten rounds would otherwise cost more than the copy of
-// 16-bit values: about 80 instructions for each counter, 10 a value at eight values.
+// Bound: HBM (4 M fp32 values and more); for 16-bit values the generator's ten rounds, about 80 instructions for each counter, come near it: 5.4 TB/s at 67 M
+// values without a residual, 6.4 TB/s with one, 6.8 TB/s for 33 M fp32 values with one.  16 bits a value, not 32, because that would be twice the rounds.
 #include "elem_types.cuh"
 
 namespace hipgpt {
 namespace {
+
+// Counters a thread: more 16-byte words on their way for it, which 16-bit values need (67 M of them: one 59.8 us, two 55.2, four 49.4; with a residual 68.6,
+// 63.2, 63.1) and 32-bit ones do not (33 M with a residual: 59.3, 59.3, 60.0); one where that would leave SMs without a block
+template <typename T> constexpr int kPer = sizeof(T) == 2 ? 4 : 1;
+constexpr long long kManyValues = 1 << 22;
 
 struct Words { uint32_t w[4]; };
 
@@ -35,41 +40,50 @@ __device__ __forceinline__ Words philox(unsigned long long counter, unsigned lon
     return {{c0, c1, c2, c3}};
 }
 
-// One thread: eight values, one counter.  in, residual and out may be one buffer: a thread reads what it writes.
-template <typename T, bool RES, bool VEC>
+// One thread: PER counters, eight values each, 256 counters apart; all its values are asked for before the first counter is worked on.  in, residual and out may be
+// one buffer: a thread reads what it writes.
+template <typename T, bool RES, bool VEC, int PER>
 __global__ void __launch_bounds__(256)
 dropout_counter_kernel(const T *in, const T *res, T *out, unsigned long long seed, unsigned long long offset, const unsigned long long *counter,
                        uint32_t thr, float scale, long long n)
 {
     dependency_wait();
     dependents_may_start();
-    const long long blk = (long long)blockIdx.x * 256 + threadIdx.x, i0 = blk * 8;
-    if (i0 >= n) return;
-    const unsigned long long c = offset + (counter ? *counter : 0ull) + (unsigned long long)blk;
-    float x[8], y[8];
-    const bool whole = VEC && i0 + 8 <= n;
-    if (whole) {
-        load_values<T, 8>(in + i0, x);
-        if constexpr (RES) load_values<T, 8>(res + i0, y);
-    } else {
+    const long long first = (long long)blockIdx.x * (256 * PER) + threadIdx.x;
+    if (first * 8 >= n) return;
+    const unsigned long long base = offset + (counter ? *counter : 0ull);
+    float x[PER][8], y[PER][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = i0 + j < n ? to_float(in[i0 + j]) : 0.0f;
-            if constexpr (RES) y[j] = i0 + j < n ? to_float(res[i0 + j]) : 0.0f;
+    for (int u = 0; u < PER; ++u) {
+        const long long i0 = (first + 256 * u) * 8;
+        if (VEC && i0 + 8 <= n) {
+            load_values<T, 8>(in + i0, x[u]);
+            if constexpr (RES) load_values<T, 8>(res + i0, y[u]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[u][j] = i0 + j < n ? to_float(in[i0 + j]) : 0.0f;
+                if constexpr (RES) y[u][j] = i0 + j < n ? to_float(res[i0 + j]) : 0.0f;
+            }
         }
     }
-    const Words r = philox(c, seed);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t bits = j & 1 ? r.w[j / 2] >> 16 : r.w[j / 2] & 0xFFFFu;
-        x[j] = bits >= thr ? __fmul_rn(x[j], scale) : 0.0f;
-        if constexpr (RES) x[j] = __fadd_rn(y[j], x[j]);
-    }
-    if (whole) {
-        store_values<T, 8>(out + i0, x);
-    } else {
+    for (int u = 0; u < PER; ++u) {
+        const long long i0 = (first + 256 * u) * 8;
+        if (i0 >= n) return;
+        const Words r = philox(base + (unsigned long long)(first + 256 * u), seed);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (i0 + j < n) out[i0 + j] = from_float<T>(x[j]);
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t bits = j & 1 ? r.w[j / 2] >> 16 : r.w[j / 2] & 0xFFFFu;
+            x[u][j] = bits >= thr ? __fmul_rn(x[u][j], scale) : 0.0f;
+            if constexpr (RES) x[u][j] = __fadd_rn(y[u][j], x[u][j]);
+        }
+        if (VEC && i0 + 8 <= n) {
+            store_values<T, 8>(out + i0, x[u]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (i0 + j < n) out[i0 + j] = from_float<T>(x[u][j]);
+        }
     }
 }
 
@@ -78,9 +92,12 @@ int launch_dropout_counter(const void *in, const void *res, void *out, unsigned 
                            uint32_t thr, long long n, cudaStream_t st)
 {
     const bool vec = all_aligned16({in, res, out});
-    const auto kern = res ? (vec ? dropout_counter_kernel<T, true, true> : dropout_counter_kernel<T, true, false>)
-                          : (vec ? dropout_counter_kernel<T, false, true> : dropout_counter_kernel<T, false, false>);
-    const long long blocks = (n + 2047) / 2048;
+    constexpr int PER = kPer<T>;
+    const bool few = n < kManyValues;
+    const auto kern = !vec ? (res ? dropout_counter_kernel<T, true, false, 1> : dropout_counter_kernel<T, false, false, 1>)
+                      : few ? (res ? dropout_counter_kernel<T, true, true, 1> : dropout_counter_kernel<T, false, true, 1>)
+                            : (res ? dropout_counter_kernel<T, true, true, PER> : dropout_counter_kernel<T, false, true, PER>);
+    const long long block = 2048LL * (!vec || few ? 1 : PER), blocks = (n + block - 1) / block;
     const cudaError_t e = launch_overlapped(kern, dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const T *>(in), static_cast<const T *>(res), static_cast<T *>(out),
                                             seed, offset, counter, thr, 65536.0f / (float)(65536u - thr), n);
     return e == cudaSuccess ? check_launch("dropout_counter_kernel") : fail(HIPGPT_ERR_CUDA, "dropout_counter_kernel: %s", cudaGetErrorString(e));

@@ -43,7 +43,7 @@ constexpr int kOperand = kHalfM * kDeep * 2;            // bytes of one block's 
 constexpr int kEpiWarps = 16, kThreads = 32 * (kEpiWarps + 2);      // four warps share a row's columns
 constexpr int kWarpChunks = kTileN / 4 / 32;              // 32-column chunks of a warp
 constexpr int kTmemColumns = 512;
-constexpr int kPromote = 4;
+constexpr int kPromote = 2;
 constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
 // What a tile of kDz costs a pair beside its stages, in quarter stages
@@ -322,31 +322,6 @@ __device__ __noinline__ bool loss_wait_slow(uint64_t *bar, uint32_t parity, int 
     atomicCAS(&g_loss_status, 0, site);
     linger();
     return false;
-}
-
-template <typename T>
-__device__ __forceinline__ void put_columns(T *dst, const float (&v)[32], int cols, bool accumulate, bool vec)
-{
-    if (vec && cols >= 32) {
-        constexpr int W = kPer16<T>;
-#pragma unroll
-        for (int j = 0; j < 32; j += W) {
-            float x[W];
-#pragma unroll
-            for (int k = 0; k < W; ++k) x[k] = v[j + k];
-            if (accumulate) {
-                float old[W];
-                load_values<T, W>(dst + j, old);
-#pragma unroll
-                for (int k = 0; k < W; ++k) x[k] += old[k];
-            }
-            store_values<T, W>(dst + j, x);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < cols) dst[j] = from_float<T>(accumulate ? to_float(dst[j]) + v[j] : v[j]);
-    }
 }
 
 // How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
@@ -660,16 +635,16 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                         const uint32_t at = smem_u32(ring + s * STAGE);
                         const uint64_t a = make_desc(at, a_lbo, 1024, 2), b = make_desc(at + NP * kOperand, b_lbo, 1024, 2);
                         [[maybe_unused]] constexpr uint64_t lo = kOperand >> 4;
+                        if constexpr (NP == 2) {     // the small products before the large ones: less of them is cut off
 #pragma unroll
-                        for (int j = 0; j < kDeep / 16; ++j) {
-                            if constexpr (NP == 2) {
+                            for (int j = 0; j < kDeep / 16; ++j) {
                                 if (elect_one()) mma_pair(acc, a + lo + j * a_step, b + j * b_step, idesc, (k > k0 || j) ? 1u : 0u);
                                 if (elect_one()) mma_pair(acc, a + j * a_step, b + lo + j * b_step, idesc, 1u);
-                                if (elect_one()) mma_pair(acc, a + j * a_step, b + j * b_step, idesc, 1u);
-                            } else {
-                                if (elect_one()) mma_pair(acc, a + j * a_step, b + j * b_step, idesc, (k > k0 || j) ? 1u : 0u);
                             }
                         }
+#pragma unroll
+                        for (int j = 0; j < kDeep / 16; ++j)
+                            if (elect_one()) mma_pair(acc, a + j * a_step, b + j * b_step, idesc, (NP == 2 || k > k0 || j) ? 1u : 0u);
                         if (elect_one()) commit_pair(&empty[s]);
                         if (++s == RING) { s = 0; ++round; }
                     }
@@ -752,10 +727,13 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) *stage_at(lane, j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             };
+            auto out_free = [&] {                 // what lay there is out
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+            };
             // kDz: 32 columns of a plane by a bulk copy out of there
             auto put_dz = [&](int c, int plane, const uint32_t (&o)[16]) {
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // what lay there is out
-                __syncwarp();
+                out_free();
                 stage(o);
                 proxy_fence();
                 __syncwarp();
@@ -822,7 +800,26 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 }
                 const unsigned rows_here = __ballot_sync(0xffffffffu, out_here);
                 if (p.accumulate || !out_vec || left < 32) {
-                    if (out_here) put_columns<T>(static_cast<T *>(p.out) + out_row + col0 + 32 * c, v, left, p.accumulate != 0, out_vec);
+                    // added to what is there, rows of any alignment, or the last columns: 16 fp32 values of each row at a time, half a warp a row, a value a lane
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16) {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(v[h + j]);
+                        out_free();
+                        stage(o);
+                        __syncwarp();
+                        const int col = lane & 15;
+#pragma unroll 4
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = 2 * i + (lane >> 4);
+                            T *to = static_cast<T *>(p.out) + __shfl_sync(0xffffffffu, out_row, r) + col0 + 32 * c + h + col;
+                            if ((rows_here >> r & 1) && h + col < left) {
+                                const float y = reinterpret_cast<const float *>(stage_at(r, col >> 2))[col & 3];
+                                *to = from_float<T>(p.accumulate ? to_float(*to) + y : y);
+                            }
+                        }
+                    }
                     return;
                 }
                 // 64 bytes of each row at a time, four lanes a row: whole sectors, where a thread's own row by itself would be stored 16 bytes here and 16 there
@@ -835,8 +832,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                         if constexpr (NP == 1) o[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
                         else o[j] = __float_as_uint(v[h + j]);
                     }
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    __syncwarp();
+                    out_free();
                     stage(o);
                     __syncwarp();
 #pragma unroll
