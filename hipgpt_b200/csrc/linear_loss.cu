@@ -330,6 +330,8 @@ __device__ __noinline__ bool loss_wait_slow(uint64_t *bar, uint32_t parity, int 
 // tile's stages count three (they fetch three quarters, and that is what bounds them).
 struct Place { int tile, k; };               // tile: kDx's, then kDw's
 constexpr int kMostPairs = 128;
+// A tile counts so many stages more: what becomes of its accumulator is not hidden by the products of a short one (24 stages of 24 + 8: 12 us)
+constexpr int kTileExtra = 8;
 struct Cut {
     int m_tiles[2], n_tiles[2], stages[2], tiles[2], narrow[2], n_fast[2];
     int dealt;                               // tiles that are dealt out whole
@@ -349,7 +351,7 @@ struct Lengths { long long first, all; };
 __device__ __forceinline__ Lengths lengths_of(const Cut &c)
 {
     long long total[2];
-    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * c.stages[i] * max(0, 4 * c.n_tiles[i] - c.narrow[i]);
+    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * (c.stages[i] + kTileExtra) * max(0, 4 * c.n_tiles[i] - c.narrow[i]);
     return {total[0], total[0] + total[1]};
 }
 // Quarter stages before tile t
@@ -358,7 +360,7 @@ __device__ __forceinline__ long long place_before(const Cut &c, const Lengths &l
     const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
     if (u >= c.tiles[i]) return len.all;
     const TileOf x = tile_of(c, i, u);
-    const long long stages = c.stages[i];
+    const long long stages = c.stages[i] + kTileExtra;
     const long long here = c.n_fast[i] ? stages * ((long long)x.m * (4 * c.n_tiles[i] - c.narrow[i]) + 4 * x.n) : stages * (4LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
     return (i ? len.first : 0) + here;
 }
@@ -367,7 +369,7 @@ __device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long
     if (at >= len.all) return {c.tiles[0] + c.tiles[1], 0};
     const int i = at >= len.first;
     if (i) at -= len.first;
-    const long long stages = c.stages[i];
+    const long long stages = c.stages[i] + kTileExtra;
     int u, unit;
     if (c.n_fast[i]) {
         const long long row = stages * (4 * c.n_tiles[i] - c.narrow[i]);
@@ -386,7 +388,8 @@ __device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long
         at -= m * unit * stages;
         u = n * c.m_tiles[i] + m;
     }
-    return {(i ? c.tiles[0] : 0) + u, (int)(at / unit)};
+    const int k = (int)(at / unit), tile = (i ? c.tiles[0] : 0) + u;
+    return k < c.stages[i] ? Place{tile, k} : Place{tile + 1, 0};             // (a tile's last stages are what it costs otherwise)
 }
 __device__ __forceinline__ bool before(const Place &a, const Place &b) { return a.tile < b.tile || (a.tile == b.tile && a.k < b.k); }
 
@@ -435,7 +438,7 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
         if (q < pairs) {
             for (int t = q; t < dealt; t += pairs) {
                 const int i = t >= c.tiles[0];
-                load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * c.stages[i];
+                load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * (c.stages[i] + kTileExtra);
             }
             load += dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
         }
