@@ -74,6 +74,7 @@ struct LossArgs {
     CUtensorMap a[3], b[3], dz_out;
     Problem p[3];
     const int *count;                        // rows that take part
+    int *failed;                             // a wait of this call has run out: its later launches do nothing
     const int *row_map, *targets;            // of the rows that take part
     const float *lse, *g;
     const float *amax;                       // fp32: the largest |x|, |w|, |g|
@@ -212,7 +213,7 @@ struct Pack {
     int N, E, V, ld, per_block, x_blocks, x_vec;
     uint16_t *xp;
     size_t plane;
-    int *count, *row_map, *c_targets;
+    int *count, *failed, *row_map, *c_targets;
     float *c_lse, *c_g;
     float *zero_loss, *zero_lse;             // forward: what rows that take no part get
     uint8_t *zero_grad;                      // backward: their rows of the gradient
@@ -250,6 +251,7 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
         scale = pow2_scale(most[0]);
         gscale = grad_scale(most);
     }
+    if (blockIdx.x == 0 && tid == 0) *p.failed = 0;
     for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
     const int from = blockIdx.x * p.per_block, to = min(p.N, from + p.per_block);
     auto inside = [&](int t) { return t >= 0 && t < p.V; };
@@ -314,12 +316,13 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar)
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-__device__ __noinline__ bool loss_wait_slow(uint64_t *bar, uint32_t parity, int site, volatile int *abort_flag, uint32_t peer_flag, int expire)
+__device__ __noinline__ bool loss_wait_slow(uint64_t *bar, uint32_t parity, int site, volatile int *abort_flag, uint32_t peer_flag, int *failed, int expire)
 {
     if (!expires_now(expire, site) && mbar_wait(bar, parity)) return true;
     *abort_flag = 1;
     asm volatile("st.volatile.shared::cluster.u32 [%0], %1;" ::"r"(peer_flag), "r"(1) : "memory");      // the other block's rows of the tile are not stored either
     atomicCAS(&g_loss_status, 0, site);
+    atomicExch(failed, 1);
     linger();
     return false;
 }
@@ -534,10 +537,11 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         const int gone = abort_flag;
         const bool done = mbar_test(bar, parity);
         seen = !gone;
-        if (!gone && !done) seen = loss_wait_slow(bar, parity, site, &abort_flag, peer_flag, args.expire);
+        if (!gone && !done) seen = loss_wait_slow(bar, parity, site, &abort_flag, peer_flag, args.failed, args.expire);
     };
 
     // No row may take part: one tile of rows of zeros, and one stage, are then worked on (so gradients of zero are written)
+    const bool failed = *args.failed != 0;
     const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
     __shared__ Cut cut;
@@ -545,8 +549,12 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         for (int i = threadIdx.x; i < (int)(sizeof(Cut) / sizeof(int)); i += kThreads) reinterpret_cast<int *>(&cut)[i] = reinterpret_cast<const int *>(args.cut)[i];
         __syncthreads();
     }
-    Walk first = {0, {0, 0}, {0, 0}, pair, count_tiles * args.p[kDz].n_tiles, count_tiles};
-    if constexpr (FORM == kBackward) first = {min(pair, cut.dealt), cut.begin[pair], cut.begin[pair + 1], pair, count_tiles * args.p[kDz].n_tiles, count_tiles};
+    Walk first = {0, {0, 0}, {0, 0}, pair, failed ? 0 : count_tiles * args.p[kDz].n_tiles, count_tiles};
+    if constexpr (FORM == kBackward) {
+        first.dealt = failed ? cut.dealt : min(pair, cut.dealt);
+        first.at = cut.begin[pair];
+        first.end = failed ? first.at : cut.begin[pair + 1];
+    }
     auto next = [&](Walk &w, Work &x) {
         if constexpr (FORM == kBackward) {
             const bool deal = w.dealt < cut.dealt;
@@ -988,12 +996,12 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 // Forward: a block joins the parts of 32 rows, each of its warps every eighth part in order, then the eight in order
 __global__ void __launch_bounds__(256)
 loss_join_kernel(const float2 *__restrict__ part, int parts, size_t rows_alloc, const float *__restrict__ z_target, const int *__restrict__ row_map, const int *__restrict__ count,
-                 float *loss, float *lse)
+                 const int *__restrict__ failed, float *loss, float *lse)
 {
     dependency_wait();
     dependents_may_start();
     __shared__ float2 sh[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *count;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = *failed ? 0 : *count;
     for (int r0 = blockIdx.x * 32; r0 < n; r0 += gridDim.x * 32) {
         const int row = r0 + lane;
         float2 all = make_float2(-INFINITY, 0.0f);
@@ -1086,7 +1094,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth
     auto take = [&](size_t bytes) { const size_t r = at; at += padded(bytes); return r; };
     p.x_at = take(NP * p.x_plane * 2);
     p.w_at = take(p.pack_w ? NP * p.w_plane * 2 : 0);
-    p.ints_at = take((1 + 2 * (size_t)p.rows_alloc) * sizeof(int));
+    p.ints_at = take((2 + 2 * (size_t)p.rows_alloc) * sizeof(int));
     p.floats_at = take(2 * (size_t)p.rows_alloc * sizeof(float));
     p.amax_at = take((3 + 3 * kAmaxBlocks) * sizeof(float));
     p.end = at;
@@ -1116,7 +1124,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
     k.plane = p.x_plane;
-    k.count = ints; k.row_map = ints + 1; k.c_targets = ints + 1 + p.rows_alloc;
+    k.count = ints; k.failed = ints + 1; k.row_map = ints + 2; k.c_targets = ints + 2 + p.rows_alloc;
     k.c_lse = floats; k.c_g = floats + p.rows_alloc;
     k.zero_loss = zero_loss; k.zero_lse = zero_lse; k.zero_grad = static_cast<uint8_t *>(zero_grad);
     k.zero_ints = zero_ints; k.zeros = zeros;
@@ -1133,7 +1141,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     if (k.x_blocks + w_blocks > 2147483647LL) return fail(HIPGPT_ERR_UNSUPPORTED, "weights of %lld rows of %lld values are beyond one call", p.w_rows, p.w_cols);
     e = launch_overlapped(loss_pack_kernel<T>, dim3((unsigned)(k.x_blocks + w_blocks)), dim3(256), 0, st, x, w, k);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
-    a.count = k.count; a.row_map = k.row_map; a.targets = k.c_targets;
+    a.count = k.count; a.failed = k.failed; a.row_map = k.row_map; a.targets = k.c_targets;
     a.lse = k.c_lse; a.g = k.c_g; a.amax = amax;
     a.rows_alloc = (size_t)p.rows_alloc;
     a.V = p.V;
@@ -1186,7 +1194,7 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     rc = launch_loss_gemm<kForward, T>(a, pairs, p.dev, st);
     if (rc != HIPGPT_OK) return rc;
     const cudaError_t e = launch_overlapped(loss_join_kernel, dim3((unsigned)std::min<long long>((N + 31) / 32, 148 * 8)), dim3(256), 0, st, (const float2 *)a.part, n_tiles, a.rows_alloc,
-                                            (const float *)a.z_target, a.row_map, a.count, loss, lse);
+                                            (const float *)a.z_target, a.row_map, a.count, (const int *)a.failed, loss, lse);
     return e == cudaSuccess ? check_launch("loss_join_kernel") : fail(HIPGPT_ERR_CUDA, "loss_join_kernel: %s", cudaGetErrorString(e));
 }
 

@@ -122,8 +122,6 @@ def test_dropout(dtype, n, p):
     seed, offset = 0xF123456789ABCDEF, (1 << 40) + 17
     keep, inv = tu.kept(n, p, seed, offset)
     keep = keep.cuda()
-    if n > 3:
-        x[int((~keep).nonzero()[0])] if not keep.all() else None
     bad = ~keep
     x[bad] = float("nan")                        # a dropped value is zero whatever it was
     zero = torch.zeros((), dtype=torch.float64, device="cuda")
@@ -235,3 +233,168 @@ def test_loss_gradient_over_several_pieces_of_the_vocabulary(dtype, by_token):
         tu.within(gx, dx, ex, "grad_x")
         tu.within(gw if by_token else gw.t(), dw, ew, "grad_w")
     assert _status() == 0
+
+
+# ---- the calls together, captured, side by side -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_step_with_tied_weights(dtype):
+    """ids -> embedding -> dropout -> loss and all the way back, both gradients into one table, against float64 with the mask given."""
+    B, S, V, E, p, seed = 3, 50, 700, 72, 0.25, 99
+    gen, N, scale = _gen(4), B * S, 2.5
+    tok, pos = _normal(gen, V, E, dtype=dtype, scale=0.3), _normal(gen, S, E, dtype=dtype, scale=0.3)
+    ids, targets = _ids(gen, N, V), _ids(gen, N, V)
+    targets[7:20] = -1
+    x, y, loss, lse = _nan(N, E, dtype=dtype), _nan(N, E, dtype=dtype), _nan(N), _nan(N)
+    g = torch.where(targets >= 0, 1.0 / float((targets >= 0).sum()), 0.0).float()
+    gy, gx, gtok, gpos = _nan(N, E, dtype=dtype), _nan(N, E, dtype=dtype), _nan(V, E, dtype=dtype), _nan(S, E, dtype=dtype)
+    training.embedding_scaled(ids, tok, pos, x, B, S, V, E, scale=scale)
+    training.dropout_counter(x, None, y, p, seed=seed, offset=3)
+    training.linear_cross_entropy(y, tok, targets, loss, lse, N, E, V)
+    training.linear_cross_entropy_backward(y, tok, targets, lse, g, gy, gtok, N, E, V)
+    training.dropout_counter(gy, None, gx, p, seed=seed, offset=3)
+    gtok0 = gtok.clone()
+    training.embedding_backward(gx, ids, gtok, None, B, S, V, E, scale=scale, accumulate=True)
+    training.embedding_backward(gx, ids, None, gpos, B, S, V, E, scale=scale)
+    keep, inv = tu.kept(N * E, p, seed, 3)
+    mask = keep.cuda().view(N, E).double() * inv
+    t64, p64 = tok.double().requires_grad_(), pos.double().requires_grad_()
+    h = (t64[ids.long()] * scale + p64.repeat(B, 1)) * mask
+    ok = targets >= 0
+    l64 = torch.nn.functional.cross_entropy(h @ t64.t(), torch.where(ok, targets, torch.zeros_like(targets)).long(), reduction="none") * ok
+    (l64 * g.double()).sum().backward()
+    # three roundings of the storage type on the way to a loss, six to the table's gradient, each relative to what is there; halves of them add up at most
+    eps = 2 * tu.HALF[dtype] + 2e-6
+    assert float((loss.double() - l64.detach()).abs().max()) <= 8 * eps * float(l64.detach().max())
+    for got, want in ((gtok, t64.grad), (gpos, p64.grad)):
+        assert float((got.double() - want).norm() / want.norm()) <= 8 * eps
+    assert not torch.equal(gtok, gtok0) and _status() == 0
+
+
+def _calls(gen, dtype, B, S, V, E):
+    """The five calls on tensors of their own: [(call, outputs)]."""
+    N = B * S
+    tok, pos, g = _normal(gen, V, E, dtype=dtype), _normal(gen, S, E, dtype=dtype), _normal(gen, N, E, dtype=dtype)
+    ids, targets, grad = _ids(gen, N, V, -1), _ids(gen, N, V, -1), torch.rand(N, generator=gen, device="cuda")
+    x = _normal(gen, N, E, dtype=dtype, scale=E ** -0.5)
+    out, drop, loss, lse = _nan(N, E, dtype=dtype), _nan(N, E, dtype=dtype), _nan(N), _nan(N)
+    gt, gp, gx, gw = _nan(V, E, dtype=dtype), _nan(S, E, dtype=dtype), _nan(N, E, dtype=dtype), _nan(V, E, dtype=dtype)
+    w = tok
+    return (lambda: (training.embedding_scaled(ids, tok, pos, out, B, S, V, E, scale=1.5),
+                     training.dropout_counter(x, g, drop, 0.2, seed=1),
+                     training.embedding_backward(g, ids, gt, gp, B, S, V, E),
+                     training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V),
+                     training.linear_cross_entropy_backward(x, w, targets, lse, grad, gx, gw, N, E, V))), [out, drop, gt, gp, loss, lse, gx, gw], [tok, pos, g, x, grad]
+
+
+def _snapshot(outs):
+    torch.cuda.synchronize()
+    return [o.clone() for o in outs]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_calls_replay_on_new_inputs_and_graphs_do_not_meet(dtype):
+    gen = _gen(8)
+    jobs = [_calls(gen, dtype, 2, 130, 900, 136), _calls(gen, dtype, 5, 17, 333, 64)]
+    graphs = []
+    for call, _, _ in jobs:
+        call()                                   # what a first call sets up is no part of a graph
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graphs.append(graph)
+    for _ in range(2):
+        want = []
+        for call, outs, ins in jobs:
+            for t in ins[:4]:
+                t.copy_(_normal(gen, *t.shape, dtype=dtype, scale=0.2))
+            call()
+            want.append(_snapshot(outs))
+            for o in outs:
+                o.fill_(float("nan"))
+        _capi.lib().hipgpt_release_workspace()   # a graph has buffers of its own
+        streams = [torch.cuda.Stream() for _ in jobs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs, _), w in zip(jobs, want):
+            for o, e in zip(outs, w):
+                assert torch.equal(o, e)
+    assert _status() == 0
+
+
+def test_streams_and_threads_side_by_side_give_the_bits_of_one_alone():
+    import threading
+    gen = _gen(12)
+    jobs = [_calls(gen, F32, 3, 200, 1500, 96), _calls(gen, BF16, 4, 128, 2000, 200), _calls(gen, BF16, 1, 40, 5000, 72), _calls(gen, F32, 7, 9, 50, 33)]
+    want = []
+    for call, outs, _ in jobs:
+        call()
+        want.append(_snapshot(outs))
+        for o in outs:
+            o.fill_(float("nan"))
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(job):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    job[0]()
+        except Exception as e:                   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for (_, outs, _), w in zip(jobs, want):
+        for o, e in zip(outs, w):
+            assert torch.equal(o, e)
+    assert _status() == 0
+
+
+def test_python_refusals_on_the_gpu():
+    x, w, t, f = torch.zeros(4, 8, device="cuda"), torch.zeros(16, 8, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
+    with pytest.raises(ValueError, match="values"):
+        training.linear_cross_entropy(x, w, t, f, f.clone(), 5, 8, 16)
+    with pytest.raises(ValueError, match="contiguous"):
+        training.linear_cross_entropy(x.t(), w, t, f, f.clone(), 4, 8, 16)
+    with pytest.raises(ValueError, match="targets"):
+        training.linear_cross_entropy(x, w, t.long(), f, f.clone(), 4, 8, 16)
+    with pytest.raises(ValueError, match="w"):
+        training.linear_cross_entropy(x, w.bfloat16(), t, f, f.clone(), 4, 8, 16)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        training.dropout_counter(x.half(), None, x.half(), 0.1, seed=1)
+    with pytest.raises(_capi.HipGPTError, match="outside"):
+        training.dropout_counter(x, None, x.clone(), 1.0, seed=1)
+    with pytest.raises(_capi.HipGPTError, match="not summed"):
+        training.embedding_backward(x, t, w.bfloat16(), None, 2, 2, 16, 8)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("code,block", [(701, 0), (702, 1), (703, 2), (703, 3), (704, 0)])
+def test_an_expired_wait_of_the_loss_stores_no_loss(dtype, code, block):
+    """The parts of one block are missing, so no row's loss is stored; the status names the wait; the next call is as ever."""
+    N, E, V = 600, 520, 40000
+    x, w, targets, _ = _loss_case(N, E, V, dtype, 3)
+    loss, lse = _nan(N), _nan(N)
+    run = lambda: training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V)  # noqa: E731
+    run()
+    want = _snapshot([loss, lse])
+    for _ in range(20):                          # what is waited for may have come before, so that nothing has to wait: then once more
+        loss.fill_(-7.0)
+        _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
+        run()
+        torch.cuda.synchronize()
+        status = _status()
+        if status:
+            break
+    assert status == code and bool((loss == -7.0).all())
+    run()
+    assert torch.equal(loss, want[0]) and torch.equal(lse, want[1]) and _status() == 0
