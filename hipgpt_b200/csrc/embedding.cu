@@ -85,7 +85,7 @@ struct SortShared {
 __device__ __forceinline__ int read_peer_int(const int *p, int rank)
 {
     int v;
-    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(peer_addr(smem_u32(p), rank)) : "memory");
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(peer_addr(smem_u32(p), rank)));
     return v;
 }
 
@@ -174,14 +174,16 @@ sort_ids_kernel(const int *__restrict__ ids, int n, int V, int blocks, int bits,
         cluster_sync();
         // digit d = tid: keys of smaller digits anywhere, and of this digit in the blocks before
         int total = 0, before = 0;
-        if (tid < bins)
+        if (tid < bins) {
+            int h[kMostSortBlocks];              // (all of them on their way before the first is used)
+#pragma unroll
+            for (int r = 0; r < kMostSortBlocks; ++r) h[r] = read_peer_int(&s.hist[tid], r < blocks ? r : rank);
 #pragma unroll
             for (int r = 0; r < kMostSortBlocks; ++r) {
-                if (r >= blocks) break;
-                const int h = read_peer_int(&s.hist[tid], r);
-                total += h;
-                before += r < rank ? h : 0;
+                total += r < blocks ? h[r] : 0;
+                before += r < rank ? h[r] : 0;
             }
+        }
         int incl = total;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -464,8 +466,20 @@ embed_sum_kernel(const T *__restrict__ g, const int *__restrict__ ids, const int
                 for (int j = 0; j < W; ++j) if (t >= 0 && j < left) to[j] = g[(size_t)t * p.E + e + j];
             }
         }
+        // (an entry's values are read while the one before it is added)
+        int2 ahead = entry_s[group][0];
+        float x_ahead[W];
+        auto read = [&](int k) { load_values<T, W>(reinterpret_cast<const T *>(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16) + sub * W, x_ahead); };
+        read(0);
+#pragma unroll 1
         for (int k = 0; k < here && !gone; ++k) {
-            const int2 en = entry_s[group][k];
+            const int2 en = ahead;
+            float x[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) x[j] = x_ahead[j];
+            const int behind = min(k + 1, kRound - 1);
+            ahead = entry_s[group][behind];
+            read(behind);
             if (en.y < 0 && !pos) continue;
             if (en.x != v) {
                 if (v >= 0) flush(v);
@@ -473,8 +487,6 @@ embed_sum_kernel(const T *__restrict__ g, const int *__restrict__ ids, const int
                 clear();
             }
             if (en.y < 0) continue;
-            float x[W];
-            load_values<T, W>(reinterpret_cast<const T *>(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16) + sub * W, x);
 #pragma unroll
             for (int j = 0; j < W; ++j) acc[j] = __fadd_rn(acc[j], x[j]);
         }
