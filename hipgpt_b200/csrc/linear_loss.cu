@@ -509,6 +509,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     __shared__ uint64_t full[RING], empty[RING], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
+    __shared__ float scales_s[3];             // fp32: what takes the operands' scales out of the logits, dx, dW
     __shared__ float2 part_s[FORM == kForward ? 2 : 1][4][kHalfM];
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
@@ -541,14 +542,19 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     };
 
     // No row may take part: one tile of rows of zeros, and one stage, are then worked on (so gradients of zero are written)
+    if (NP == 2 && threadIdx.x == 0) {
+        const float x_inv = pow2_inverse(operand_scale(args.amax, 0)), w_inv = pow2_inverse(operand_scale(args.amax, 1)), g_inv = FORM == kBackward ? pow2_inverse(grad_scale(args.amax)) : 1.0f;
+        scales_s[0] = x_inv * w_inv;
+        scales_s[1] = g_inv * w_inv;
+        scales_s[2] = g_inv * x_inv;
+    }
     const bool failed = *args.failed != 0;
     const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
     __shared__ Cut cut;
-    if constexpr (FORM == kBackward) {
+    if constexpr (FORM == kBackward)
         for (int i = threadIdx.x; i < (int)(sizeof(Cut) / sizeof(int)); i += kThreads) reinterpret_cast<int *>(&cut)[i] = reinterpret_cast<const int *>(args.cut)[i];
-        __syncthreads();
-    }
+    __syncthreads();
     Walk first = {0, {0, 0}, {0, 0}, pair, failed ? 0 : count_tiles * args.p[kDz].n_tiles, count_tiles};
     if constexpr (FORM == kBackward) {
         first.dealt = failed ? cut.dealt : min(pair, cut.dealt);
@@ -670,36 +676,30 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         // ---- what becomes of an accumulator: thread = row = TMEM lane; four warps share a row's columns ----
         const int quarter = warp & 3, fourth = warp >> 2, row_in_tile = rank * kHalfM + quarter * 32 + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t drained[2] = {peer_addr(smem_u32(&acc_empty[0]), 0), peer_addr(smem_u32(&acc_empty[1]), 0)};
-        const float x_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 0)) : 1.0f, w_inv = NP == 2 ? pow2_inverse(operand_scale(args.amax, 1)) : 1.0f;
-        const float z_scale = x_inv * w_inv;
+        const uint32_t drained = peer_addr(smem_u32(&acc_empty[0]), 0);
+        const float z_scale = NP == 2 ? scales_s[0] : 1.0f;
         uint8_t *out_s = ring + kRingBytes + warp * kOutBytes;           // (kBackward)
         int unit = 0, part_at = 0;
         while (next(walk, x)) {
             const Problem &p = args.p[x.kind];
             const int row = x.m * kTileM + row_in_tile;
             const int chunks = x.narrow ? kWarpChunks / 2 : kWarpChunks, mine0 = fourth * 32 * chunks, col0 = x.n * kTileN + mine0;      // its 32-column chunks
+            // The reads of TMEM have completed and nothing in memory goes with it, so the arrival need not wait for the stores that are on their way
             auto release = [&](int buf) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(buf ? drained[1] : drained[0]) : "memory");
+                if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(drained + (uint32_t)(buf * sizeof(uint64_t))) : "memory");
             };
             const bool whole = x.kind == kDz || (x.k0 == 0 && x.k1 == x.stages);
 
-            // per row
-            const bool here = row < count;
-            int target = -1;
-            float lse = 0.0f, g = 0.0f, out_scale = 1.0f, run_max = -INFINITY, run_sum = 0.0f;
-            size_t out_row = 0;
-            bool out_here = false, out_vec = false;
-            if (FORM == kForward || x.kind == kDz) {
-                if (here) target = __ldg(args.targets + row) - args.v0;
-                if constexpr (FORM == kBackward) if (here) { lse = __ldg(args.lse + row); g = __ldg(args.g + row); }
-            } else {
-                out_here = row < (p.m_by_count ? count : p.rows);
-                if (out_here) out_row = (size_t)(x.kind == kDx ? __ldg(args.row_map + row) : row) * p.ld;
-                if constexpr (NP == 2) out_scale = pow2_inverse(grad_scale(args.amax)) * (x.kind == kDx ? w_inv : x_inv);
-                out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+            // per row: whether it is there, and its target (of the logits), or its row of the result
+            const bool here = row < (FORM == kForward || x.kind != kDw ? count : p.rows);
+            int of_row = -1;
+            float lse = 0.0f, g = 0.0f, run_max = -INFINITY, run_sum = 0.0f;
+            if (here) {
+                if (FORM == kForward || x.kind == kDz) of_row = __ldg(args.targets + row) - args.v0;
+                else of_row = x.kind == kDx ? __ldg(args.row_map + row) : row;
+                if (FORM == kBackward && x.kind == kDz) { lse = __ldg(args.lse + row); g = __ldg(args.g + row); }
             }
             const int left_all = (FORM == kForward || x.kind == kDz ? args.V - args.v0 : p.cols) - col0;           // columns from col0 on
 
@@ -714,9 +714,9 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) if (j >= left) v[j] = -INFINITY;
                 }
-                if (target >= col && target < col + 32 && !abort_flag) {
+                if (of_row >= col && of_row < col + 32 && !abort_flag) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) if (target - col == j) args.z_target[row] = v[j] * z_scale;
+                    for (int j = 0; j < 32; ++j) if (of_row - col == j) args.z_target[row] = v[j] * z_scale;
                 }
                 float m = run_max;
 #pragma unroll
@@ -762,9 +762,9 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     v[j] = ex2_approx(d.x);
                     v[j + 1] = ex2_approx(d.y);
                 }
-                if (target >= col && target < col + 32) {
+                if (of_row >= col && of_row < col + 32) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] -= target - col == j ? 1.0f : 0.0f;
+                    for (int j = 0; j < 32; ++j) v[j] -= of_row - col == j ? 1.0f : 0.0f;
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
@@ -806,10 +806,12 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     return;
                 }
                 if constexpr (NP == 2) {
+                    const float out_scale = scales_s[x.kind == kDx ? 1 : 2];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= out_scale;
                 }
-                const unsigned rows_here = __ballot_sync(0xffffffffu, out_here);
+                const unsigned rows_here = __ballot_sync(0xffffffffu, here);
+                const bool out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
                 if (p.accumulate || !out_vec || left < 32) {
                     // added to what is there, rows of any alignment, or the last columns: 16 fp32 values of each row at a time, half a warp a row, a value a lane
 #pragma unroll
@@ -824,7 +826,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 #pragma unroll 4
                         for (int i = 0; i < 16; ++i) {
                             const int r = 2 * i + (lane >> 4);
-                            T *to = static_cast<T *>(p.out) + __shfl_sync(0xffffffffu, out_row, r) + col0 + 32 * c + h + col;
+                            T *to = static_cast<T *>(p.out) + __shfl_sync(0xffffffffu, of_row, r) * p.ld + col0 + 32 * c + h + col;
                             if ((rows_here >> r & 1) && h + col < left) {
                                 const float y = reinterpret_cast<const float *>(stage_at(r, col >> 2))[col & 3];
                                 *to = from_float<T>(p.accumulate ? to_float(*to) + y : y);
@@ -849,7 +851,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = 8 * i + (lane >> 2);
-                        const size_t at = __shfl_sync(0xffffffffu, out_row, r);
+                        const long long at = __shfl_sync(0xffffffffu, of_row, r) * p.ld;
                         const uint4 u = *stage_at(r, lane & 3);
                         if (rows_here >> r & 1) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at + col0 + 32 * c + h + (lane & 3) * kPer16<T>) = u;
                     }
@@ -891,9 +893,29 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 }
             };
 
-            // Everything leaves TMEM before anything is stored: the arrival that gives an accumulator back would wait for stores before it.
-            float acc[kWarpChunks][32];
+            // whether the others' shares of a tile that this pair is the first of are there
+            auto others_there = [&] {
+                int there = 0;
+                if (lane == 0) there = *reinterpret_cast<volatile int *>(arrived);
+                there = __shfl_sync(0xffffffffu, there, 0);
+                __threadfence();
+                if (there == p1 - p0 && lane == 0) *arrived = 0;         // for the next launch
+                return there == p1 - p0;
+            };
+            auto take = [&](int c, float (&v)[32]) {
+                if constexpr (FORM == kForward) {
+                    log_sum(c, v);
+                } else if (x.kind == kDz) {
+                    logit_gradient(c, v);
+                } else if (complete) {
+                    add_sources(c, v);
+                    finish(c, v);
+                } else {
+                    leave(c, v);
+                }
+            };
             if constexpr (NP == 2) {
+                float acc[kWarpChunks][32];
 #pragma unroll
                 for (int c = 0; c < kWarpChunks; ++c)
 #pragma unroll
@@ -915,38 +937,23 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     }
                     release(unit & 1);
                 }
+                if (FORM == kBackward && !whole && pair == p0) complete = others_there();
+#pragma unroll
+                for (int c = 0; c < kWarpChunks; ++c)
+                    if (FORM == kForward || c < chunks) take(c, acc[c]);
             } else {
                 wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
                 tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < kWarpChunks; ++c)        // (of a narrow tile the last one is not looked at)
-                    tmem_ld32(lane_base + (uint32_t)((unit & 1) * kTileN + (mine0 + 32 * c) % kTileN), acc[c]);
-                tmem_wait_ld();
-                release(unit & 1);
-                ++unit;
-            }
-            if (FORM == kBackward && !whole && pair == p0) {
-                int there = 0;
-                if (lane == 0) there = *reinterpret_cast<volatile int *>(arrived);
-                there = __shfl_sync(0xffffffffu, there, 0);
-                __threadfence();
-                complete = there == p1 - p0;
-                if (complete && lane == 0) *arrived = 0;                 // for the next launch
-            }
-#pragma unroll
-            for (int c = 0; c < kWarpChunks; ++c) {
-                if constexpr (FORM == kForward) {
-                    log_sum(c, acc[c]);
-                } else if (x.kind == kDz) {
-                    logit_gradient(c, acc[c]);
-                } else if (c < chunks) {
-                    if (complete) {
-                        add_sources(c, acc[c]);
-                        finish(c, acc[c]);
-                    } else {
-                        leave(c, acc[c]);
-                    }
+                if (FORM == kBackward && !whole && pair == p0) complete = others_there();
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    float v[32];
+                    tmem_ld32(lane_base + (uint32_t)((unit & 1) * kTileN + mine0 + 32 * c), v);
+                    tmem_wait_ld();
+                    if (c == chunks - 1) release(unit & 1);
+                    take(c, v);
                 }
+                ++unit;
             }
             if constexpr (FORM == kForward) {
                 // the four warps that share these rows meet; one joins what they have (two buffers: a warp is at most a tile ahead)

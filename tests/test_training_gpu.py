@@ -380,14 +380,15 @@ def test_python_refusals_on_the_gpu():
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("code,block", [(701, 0), (702, 1), (703, 2), (703, 3), (704, 0)])
 def test_an_expired_wait_of_the_loss_stores_no_loss(dtype, code, block):
-    """The parts of one block are missing, so no row's loss is stored; the status names the wait; the next call is as ever."""
-    N, E, V = 600, 520, 40000
-    x, w, targets, _ = _loss_case(N, E, V, dtype, 3)
-    loss, lse = _nan(N), _nan(N)
-    run = lambda: training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V)  # noqa: E731
-    run()
-    want = _snapshot([loss, lse])
-    for _ in range(20):                          # what is waited for may have come before, so that nothing has to wait: then once more
+    """The parts of one block are missing, so no row's loss is stored; the status names the wait; the next call is as ever.  What is waited for may have come before, so
+    that nothing has to wait: then once more, in the end with one stage a tile, where the products wait for what becomes of their sums."""
+    for E in (520,) * 10 + (64,) * 20:
+        N, V = 600, 40000
+        x, w, targets, _ = _loss_case(N, E, V, dtype, 3)
+        loss, lse = _nan(N), _nan(N)
+        run = lambda: training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V)  # noqa: E731, B023
+        run()
+        want = _snapshot([loss, lse])
         loss.fill_(-7.0)
         _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
         run()
