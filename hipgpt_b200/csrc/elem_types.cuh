@@ -79,6 +79,17 @@ inline bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb)
     return a0 < b0 + nb && b0 < a0 + na;
 }
 
+// A call's arrays; the first `outputs` of them are written
+struct Extent { const void *at; size_t bytes; };
+inline int refuse_overlaps(int outputs, std::initializer_list<Extent> arrays)
+{
+    int i = 0;
+    for (const Extent *a = arrays.begin(); a != arrays.end() && i < outputs; ++a, ++i)
+        for (const Extent *b = a + 1; b != arrays.end(); ++b)
+            if (a->at && b->at && a->bytes && b->bytes && ranges_overlap(a->at, a->bytes, b->at, b->bytes)) return fail(HIPGPT_ERR_BAD_ARG, "an output overlaps another of the call's arrays");
+    return HIPGPT_OK;
+}
+
 inline bool all_aligned16(std::initializer_list<const void *> ps)
 {
     uintptr_t all = 0;

@@ -452,8 +452,8 @@ embed_sum_kernel(const T *__restrict__ g, const int *__restrict__ ids, const int
                 if (t >= 0) bulk_load(rows_s + ((size_t)(group * kRound + k) << p.row_log) * 16, g + (size_t)t * p.E + at, (uint32_t)(cols * sizeof(T)), &landed);
             }
             __syncthreads();                 // the entries
-            if (!mbar_wait(&landed, (uint32_t)(round & 1))) {
-                gone = true;
+            gone = !__all_sync(0xffffffffu, mbar_wait(&landed, (uint32_t)(round & 1)));        // (a warp as a whole: its lanes meet again in last_of)
+            if (gone) {
                 atomicCAS(&g_embed_status, 0, 1);
                 linger();
             }
@@ -584,6 +584,7 @@ int check_embedding_sizes(int B, int S, int V, int E, int type)
 {
     if (type != HIPGPT_TYPE_F32 && type != HIPGPT_TYPE_BF16) return fail(HIPGPT_ERR_BAD_ARG, "unknown type %d", type);
     if (B < 0 || S < 0 || V < 0 || E < 0) return fail(HIPGPT_ERR_BAD_ARG, "negative size: B=%d S=%d V=%d E=%d", B, S, V, E);
+    if (V >= 1 << 30 || E >= 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "tables of %d rows of %d values are beyond one call", V, E);
     if ((long long)B * S > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "%lld tokens are beyond one call", (long long)B * S);
     return HIPGPT_OK;
 }
@@ -614,6 +615,9 @@ int hipgpt_embedding_scaled(const int *d_ids, const void *d_tok, const void *d_p
     if (rc != HIPGPT_OK) return rc;
     if (B == 0 || S == 0 || E == 0) return HIPGPT_OK;
     if (!d_ids || !d_out || (V > 0 && !d_tok)) return fail(HIPGPT_ERR_NULL, "ids, tok and out must not be NULL");
+    const size_t ts = type == HIPGPT_TYPE_F32 ? 4 : 2, row = (size_t)E * ts, n = (size_t)B * S;
+    const int clear = refuse_overlaps(1, {{d_out, n * row}, {d_ids, n * sizeof(int)}, {d_tok, V * row}, {d_pos, S * row}});
+    if (clear != HIPGPT_OK) return clear;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return type == HIPGPT_TYPE_F32 ? launch_embedding_scaled<float>(d_ids, d_tok, d_pos, d_out, scale, (long long)B * S, S, V, E, st)
                                    : launch_embedding_scaled<__nv_bfloat16>(d_ids, d_tok, d_pos, d_out, scale, (long long)B * S, S, V, E, st);
@@ -636,6 +640,9 @@ int hipgpt_embedding_backward(const void *d_grad_out, const int *d_ids, void *d_
         return e == cudaSuccess ? HIPGPT_OK : fail(HIPGPT_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
     }
     if (!d_grad_out || !d_ids) return fail(HIPGPT_ERR_NULL, "grad_out and ids must not be NULL");
+    const size_t n = (size_t)B * S, row = (size_t)E * gs;
+    const int clear = refuse_overlaps(2, {{d_grad_tok, V * row}, {d_grad_pos, S * row}, {d_grad_out, n * E * (type == HIPGPT_TYPE_F32 ? 4 : 2)}, {d_ids, n * sizeof(int)}});
+    if (clear != HIPGPT_OK) return clear;
     if (type == HIPGPT_TYPE_F32) return launch_embedding_backward<float, float>(d_grad_out, d_ids, d_grad_tok, d_grad_pos, scale, accumulate, B, S, V, E, st);
     return grad_type == HIPGPT_TYPE_F32 ? launch_embedding_backward<__nv_bfloat16, float>(d_grad_out, d_ids, d_grad_tok, d_grad_pos, scale, accumulate, B, S, V, E, st)
                                         : launch_embedding_backward<__nv_bfloat16, __nv_bfloat16>(d_grad_out, d_ids, d_grad_tok, d_grad_pos, scale, accumulate, B, S, V, E, st);

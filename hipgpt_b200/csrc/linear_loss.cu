@@ -1221,7 +1221,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
     const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM), piece_tiles = (int)(width / kTileN);
     const long long dx_tiles = grad_x ? (long long)m_tiles * e_tiles : 0, dw_tiles = grad_w ? (long long)piece_tiles * e_tiles : 0;
-    if (dx_tiles + dw_tiles > 1 << 26 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
+    if (dx_tiles + dw_tiles > 1 << 25 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
     int pairs = 1;
     rc = loss_pairs(p.dev, 1 << 30, &pairs);
     if (rc != HIPGPT_OK) return rc;
@@ -1330,6 +1330,9 @@ int hipgpt_linear_cross_entropy(const void *d_x, const void *d_w, const int *d_t
     if (rc != HIPGPT_OK) return rc;
     if (N == 0) return HIPGPT_OK;
     if (!d_x || !d_w || !d_targets || !d_loss || !d_lse) return fail(HIPGPT_ERR_NULL, "x, w, targets, loss and lse must not be NULL");
+    const size_t ts = type == HIPGPT_TYPE_F32 ? 4 : 2, rows = (size_t)N * 4;
+    const int clear = refuse_overlaps(2, {{d_loss, rows}, {d_lse, rows}, {d_x, (size_t)N * E * ts}, {d_w, (size_t)V * E * ts}, {d_targets, rows}});
+    if (clear != HIPGPT_OK) return clear;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return type == HIPGPT_TYPE_F32 ? forward<float>(d_x, d_w, d_targets, d_loss, d_lse, N, E, V, layout, st)
                                    : forward<__nv_bfloat16>(d_x, d_w, d_targets, d_loss, d_lse, N, E, V, layout, st);
@@ -1348,6 +1351,9 @@ int hipgpt_linear_cross_entropy_backward(const void *d_x, const void *d_w, const
     }
     if (!d_grad_x && !d_grad_w) return HIPGPT_OK;
     if (!d_x || !d_w || !d_targets || !d_lse || !d_grad_loss) return fail(HIPGPT_ERR_NULL, "x, w, targets, lse and grad_loss must not be NULL");
+    const size_t ts = type == HIPGPT_TYPE_F32 ? 4 : 2, rows = (size_t)N * 4, xb = (size_t)N * E * ts, wb = (size_t)V * E * ts;
+    const int clear = refuse_overlaps(2, {{d_grad_x, xb}, {d_grad_w, wb}, {d_x, xb}, {d_w, wb}, {d_targets, rows}, {d_lse, rows}, {d_grad_loss, rows}});
+    if (clear != HIPGPT_OK) return clear;
     return type == HIPGPT_TYPE_F32
                ? backward<float>(d_x, d_w, d_targets, d_lse, d_grad_loss, d_grad_x, d_grad_w, accumulate_w, N, E, V, layout, st)
                : backward<__nv_bfloat16>(d_x, d_w, d_targets, d_lse, d_grad_loss, d_grad_x, d_grad_w, accumulate_w, N, E, V, layout, st);

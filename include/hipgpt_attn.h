@@ -229,8 +229,10 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
 /*
  * The two ends of a training step, in fp32 or with 16-bit storage (`type`; sums and softmax in fp32 either way, each result rounded once).
  * Buffers of the library (per device and stream, at most eight; hipgpt_release_workspace() frees them; a captured call gets buffers of
- * its graph) hold what a call keeps between its kernels.  Nothing depends on the order in which blocks run: results are the same bits run
- * to run.
+ * its graph) hold what a call keeps between its kernels: the operands as the tensor core takes them, and for the gradient of the loss two pieces
+ * of the logits' gradient of at most 192 MB each (or of 1024 columns, if that is more) and the sums.  Nothing depends on the order in which blocks run: results are
+ * the same bits run to run.  Except in hipgpt_dropout_counter no output may overlap another array of the call (HIPGPT_ERR_BAD_ARG).  Should a wait inside a kernel run out
+ * (hipgpt_kernel_status), the call's results are not all stored.
  *   hipgpt_embedding_scaled    out[t] = scale tok[id_t] + pos[t mod S], zeros for an id outside [0, V); tok [V][E], pos [S][E] or NULL,
  *                              out [B*S][E], all of `type`.  (hipgpt_embedding_lookup with a scale, without positions, in either type.)
  *   hipgpt_embedding_backward  grad_tok[v] = scale * sum of grad_out[t] over the tokens with id v, grad_pos[s] = sum of grad_out over the

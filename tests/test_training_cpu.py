@@ -78,3 +78,41 @@ def test_the_python_calls_refuse_what_is_no_gpu_tensor():
 def test_an_expiring_wait_can_be_asked_for_in_the_loss():
     assert _lib().hipgpt_debug_expire_wait(700, 0) == BAD
     assert _lib().hipgpt_debug_expire_wait(801, 0) == BAD
+
+
+G = 1 << 32                              # addresses this far apart hold arrays that do not meet
+
+
+@pytest.mark.parametrize("V,E", [((1 << 31) - 1, 1), (1 << 30, 8), (1, (1 << 31) - 1), (5, 1 << 30)])
+def test_embedding_tables_beyond_the_index_range(V, E):
+    assert _lib().hipgpt_embedding_scaled(P, P + G, None, P + 2 * G, 1.0, 1, 1, V, E, 1, None) == UNSUPPORTED
+    assert _lib().hipgpt_embedding_backward(P, P + G, P + 2 * G, None, 1.0, 0, 1, 1, V, E, 1, 1, None) == UNSUPPORTED
+
+
+def _with(arrays, which, at):
+    return [at if i == which else a for i, a in enumerate(arrays)]
+
+
+@pytest.mark.parametrize("which,size", [(0, 6 * 4), (1, 5 * 32), (2, 3 * 32)])
+def test_embedding_into_its_own_inputs(which, size):
+    for at in (P + 9 * G, P + 9 * G - size + 4, P + 9 * G + 6 * 32 - 4):
+        ptrs = _with([P, P + G, P + 2 * G], which, at)
+        assert _lib().hipgpt_embedding_scaled(*ptrs, P + 9 * G, 1.0, 2, 3, 5, 8, 0, None) == BAD
+
+
+@pytest.mark.parametrize("out,other", [(2, 0), (2, 1), (3, 0), (3, 1), (2, 3)])
+def test_embedding_gradient_into_its_own_inputs(out, other):
+    ptrs = [P, P + G, P + 2 * G, P + 3 * G]
+    assert _lib().hipgpt_embedding_backward(*_with(ptrs, out, ptrs[other]), 1.0, 0, 2, 3, 5, 8, 0, 0, None) == BAD
+
+
+@pytest.mark.parametrize("out,other", [(3, 0), (3, 1), (3, 2), (4, 0), (4, 1), (4, 2), (3, 4)])
+def test_loss_into_its_own_inputs(out, other):
+    ptrs = [P + i * G for i in range(5)]
+    assert _lib().hipgpt_linear_cross_entropy(*_with(ptrs, out, ptrs[other]), 4, 8, 16, 0, 0, None) == BAD
+
+
+@pytest.mark.parametrize("out,other", [(5, i) for i in range(5)] + [(6, i) for i in range(6)])
+def test_loss_gradient_into_its_own_inputs(out, other):
+    ptrs = [P + i * G for i in range(7)]
+    assert _lib().hipgpt_linear_cross_entropy_backward(*_with(ptrs, out, ptrs[other]), 0, 4, 8, 16, 0, 0, None) == BAD
