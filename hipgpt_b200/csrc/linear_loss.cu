@@ -22,7 +22,7 @@
 //
 // Products: tcgen05.mma.cta_group::2, 256 x 256 tiles of two blocks, 64 deep stages by TMA in a ring, two accumulators in TMEM: the products of a
 // tile run while eight warps take the tile before it out.  Any operand may be contiguous along the reduction or across it (a descriptor
-// bit), so neither x, W nor dz is ever transposed.  bf16: operands as they are, dz rounded to bf16.  fp32: each operand as two fp16 numbers
+// bit), so neither x, W nor dz is ever transposed.  bf16: operands as they are, dz / (largest |g|) rounded to bf16.  fp32: each operand as two fp16 numbers
 // hi + lo of the value times a power of two (one per matrix; 2^-22 of the value), three products a pair: lo hi + hi lo + hi hi.  The tensor
 // core's fp32 sums are cut off, not rounded, so fp32 sums leave TMEM every kPromote stages and go on in registers.
 #include "elem_types.cuh"
@@ -77,7 +77,7 @@ struct LossArgs {
     int *failed;                             // a wait of this call has run out: its later launches do nothing
     const int *row_map, *targets;            // of the rows that take part
     const float *lse, *g;
-    const float *amax;                       // fp32: the largest |x|, |w|, |g|
+    const float *amax;                       // the largest |x|, |w| (fp32), |g|
     float2 *part;                            // kForward: [tile of the vocabulary][row] maximum and sum
     float *z_target;
     float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
@@ -89,6 +89,8 @@ struct LossArgs {
     int expire;
 };
 
+// bf16: the gradient of the logits is rounded in units of the largest |g|.  With one g for all rows (a mean) the target's element then is p - 1, all but exact where p is small;
+// rounded as it is, -g would be off by the same half step of bf16 in every row, and that element is most of the row's gradient.
 // fp32 operands: x = (hi + lo) / scale.  The gradient of the logits is |dz| <= 2 |g|: 2^14 / (power of two above the largest |g|) leaves room
 __device__ __forceinline__ float operand_scale(const float *amax, int which) { return pow2_scale(amax[which]); }
 __device__ __forceinline__ float grad_scale(const float *amax) { return operand_scale(amax, 2) * 0.5f; }
@@ -101,7 +103,7 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 
 // ---- rows that take part, moved together ------------------------------------------------------------------------------
 
-constexpr int kAmaxBlocks = 148;
+constexpr int kAmaxBlocks = 148, kMostPackBlocks = 512;       // (of loss_pack_kernel: those that have rows of x)
 
 // partial[which][block] = largest finite |value| that the block has seen: x (rows that take part), w, g
 __global__ void __launch_bounds__(256)
@@ -215,6 +217,7 @@ struct Pack {
     size_t plane;
     int *count, *failed, *row_map, *c_targets;
     float *c_lse, *c_g;
+    float *g_most;                           // bf16, backward: the largest finite |g| that each block has seen
     float *zero_loss, *zero_lse;             // forward: what rows that take no part get
     uint8_t *zero_grad;                      // backward: their rows of the gradient
     int *zero_ints;
@@ -253,6 +256,7 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
     }
     if (blockIdx.x == 0 && tid == 0) *p.failed = 0;
     for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
+    float g_most = 0.0f;
     const int from = blockIdx.x * p.per_block, to = min(p.N, from + p.per_block);
     auto inside = [&](int t) { return t >= 0 && t < p.V; };
     int before = 0;
@@ -275,7 +279,12 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
                 if (lane == j) {
                     p.row_map[i] = n;
                     p.c_targets[i] = t;
-                    if (p.g) { p.c_g[i] = p.g[n] * gscale; p.c_lse[i] = p.lse[n]; }
+                    if (p.g) {
+                        const float g = p.g[n];
+                        if (fabsf(g) <= 3.0e38f) g_most = fmaxf(g_most, fabsf(g));
+                        p.c_g[i] = g * gscale;
+                        p.c_lse[i] = p.lse[n];
+                    }
                 }
                 pack_row<T>(x + (size_t)n * p.E, p.xp + (size_t)i * p.ld, p.plane, 0, p.ld, p.E, scale, lane, p.x_vec != 0);
             } else {
@@ -287,6 +296,17 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
             }
         }
         base += __popc(mask);
+    }
+    if (sizeof(T) == 2 && p.g) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) g_most = fmaxf(g_most, __shfl_xor_sync(0xffffffffu, g_most, o));
+        if (lane == 0) warp_max[warp] = g_most;
+        __syncthreads();
+        if (tid == 0) {
+#pragma unroll
+            for (int w8 = 1; w8 < 8; ++w8) g_most = fmaxf(g_most, warp_max[w8]);
+            p.g_most[blockIdx.x] = g_most;
+        }
     }
     if (to == p.N && from < p.N) {           // the last block that has rows: their number, and zeros up to a whole stage (one at least) of the products that sum over them
         if (tid == 0) *p.count = base;
@@ -400,6 +420,9 @@ __device__ __forceinline__ bool before(const Place &a, const Place &b) { return 
 struct PlanArgs {
     int pieces, width, V, E, pairs, dz_stages, dz_extra;
     int ev, with_x, with_w;
+    const float *g_most;                     // bf16: loss_pack_kernel's, of so many blocks, and where the largest goes
+    int g_blocks;
+    float *most;
 };
 
 // A block for each launch of the backward, kMostPairs threads.  Tiles of kDz are dealt out one by one from pair 0 on.
@@ -412,11 +435,24 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
     __shared__ Lengths len;
     __shared__ long long scan[kMostPairs / 32];
     __shared__ int all_fit;
+    __shared__ float warp_most[kMostPairs / 32];
     const int q = threadIdx.x, lane = q & 31, warp = q >> 5, launch = blockIdx.x, pairs = a.pairs, count = *count_at;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep), e_tiles = (a.E + kTileN - 1) / kTileN;
     auto columns = [&](int piece) { return piece < 0 || piece >= a.pieces ? 0 : (int)min((long long)a.width, a.V - (long long)piece * a.width); };
     auto narrow = [](int n) { return n && (n - 1) % kTileN < kTileN / 2 ? 1 : 0; };
     const int old = columns(launch - 1), v_tiles = (old + kTileN - 1) / kTileN;
+    if (a.g_blocks && launch == 0) {
+        float m = 0.0f;
+        for (int i = q; i < a.g_blocks; i += kMostPairs) m = fmaxf(m, __ldg(a.g_most + i));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) warp_most[warp] = m;
+        __syncthreads();
+        if (q == 0) {
+            for (int w = 1; w < kMostPairs / 32; ++w) m = fmaxf(m, warp_most[w]);
+            *a.most = m > 0.0f ? m : 1.0f;
+        }
+    }
     if (q == 0) {
         c.m_tiles[0] = count_tiles;
         c.n_tiles[0] = a.with_x && old ? e_tiles : 0;
@@ -509,7 +545,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     __shared__ uint64_t full[RING], empty[RING], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    __shared__ float scales_s[3];             // fp32: what takes the operands' scales out of the logits, dx, dW
+    __shared__ float scales_s[3];             // what takes the operands' scales out of the logits (fp32), dx, dW
     __shared__ float2 part_s[FORM == kForward ? 2 : 1][4][kHalfM];
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
@@ -548,6 +584,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         scales_s[1] = g_inv * w_inv;
         scales_s[2] = g_inv * x_inv;
     }
+    if (NP == 1 && FORM == kBackward && threadIdx.x == 0) scales_s[1] = scales_s[2] = args.amax[2];
     const bool failed = *args.failed != 0;
     const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
@@ -699,7 +736,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             if (here) {
                 if (FORM == kForward || x.kind == kDz) of_row = __ldg(args.targets + row) - args.v0;
                 else of_row = x.kind == kDx ? __ldg(args.row_map + row) : row;
-                if (FORM == kBackward && x.kind == kDz) { lse = __ldg(args.lse + row); g = __ldg(args.g + row); }
+                if (FORM == kBackward && x.kind == kDz) { lse = __ldg(args.lse + row); g = NP == 2 ? __ldg(args.g + row) : __fdiv_rn(__ldg(args.g + row), scales_s[1]); }
             }
             const int left_all = (FORM == kForward || x.kind == kDz ? args.V - args.v0 : p.cols) - col0;           // columns from col0 on
 
@@ -805,11 +842,9 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     for (int j = 0; j < 8; ++j) __stcg(sum + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
                     return;
                 }
-                if constexpr (NP == 2) {
-                    const float out_scale = scales_s[x.kind == kDx ? 1 : 2];
+                const float out_scale = scales_s[x.kind == kDx ? 1 : 2];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] *= out_scale;
-                }
+                for (int j = 0; j < 32; ++j) v[j] *= out_scale;
                 const unsigned rows_here = __ballot_sync(0xffffffffu, here);
                 const bool out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
                 if (p.accumulate || !out_vec || left < 32) {
@@ -1103,7 +1138,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth
     p.w_at = take(p.pack_w ? NP * p.w_plane * 2 : 0);
     p.ints_at = take((2 + 2 * (size_t)p.rows_alloc) * sizeof(int));
     p.floats_at = take(2 * (size_t)p.rows_alloc * sizeof(float));
-    p.amax_at = take((3 + 3 * kAmaxBlocks) * sizeof(float));
+    p.amax_at = take((3 + std::max(3 * kAmaxBlocks, kMostPackBlocks)) * sizeof(float));
     p.end = at;
     return HIPGPT_OK;
 }
@@ -1111,7 +1146,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth
 // Fills what the plan has in the workspace, and of `a` what every form reads
 template <typename T>
 int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, const int *targets, const float *lse, const float *g, float *zero_loss, float *zero_lse, void *zero_grad,
-              int *zero_ints, int zeros, cudaStream_t st, const void **w_base)
+              int *zero_ints, int zeros, cudaStream_t st, const void **w_base, int *x_blocks)
 {
     int *ints = reinterpret_cast<int *>(ws + p.ints_at);
     float *floats = reinterpret_cast<float *>(ws + p.floats_at), *amax = reinterpret_cast<float *>(ws + p.amax_at);
@@ -1123,10 +1158,11 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_amax_kernel: %s", cudaGetErrorString(e));
     }
     k.partial = amax + 3;
+    k.g_most = amax + 3;
     k.amax = amax;
     k.targets = targets; k.lse = lse; k.g = g;
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
-    k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows)
+    k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + kMostPackBlocks - 1) / kMostPackBlocks, 32));      // (a block counts the targets before its rows)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
@@ -1150,6 +1186,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
     a.count = k.count; a.failed = k.failed; a.row_map = k.row_map; a.targets = k.c_targets;
     a.lse = k.c_lse; a.g = k.c_g; a.amax = amax;
+    *x_blocks = k.x_blocks;
     a.rows_alloc = (size_t)p.rows_alloc;
     a.V = p.V;
     return check_launch("loss_pack_kernel");
@@ -1184,9 +1221,9 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     LossArgs a = {};
     const void *wb = nullptr;
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
-    int pairs = 1;
+    int pairs = 1, x_blocks = 0;
     rc = loss_pairs(p.dev, (long long)m_tiles * n_tiles, &pairs);
-    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, st, &wb);
+    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, st, &wb, &x_blocks);
     if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, kHalfM);
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
     if (rc != HIPGPT_OK) return rc;
@@ -1222,7 +1259,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM), piece_tiles = (int)(width / kTileN);
     const long long dx_tiles = grad_x ? (long long)m_tiles * e_tiles : 0, dw_tiles = grad_w ? (long long)piece_tiles * e_tiles : 0;
     if (dx_tiles + dw_tiles > 1 << 25 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
-    int pairs = 1;
+    int pairs = 1, x_blocks = 0;
     rc = loss_pairs(p.dev, 1 << 30, &pairs);
     if (rc != HIPGPT_OK) return rc;
 
@@ -1237,10 +1274,11 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     LossArgs a = {};
     const void *wb = nullptr;
     a.arrived = reinterpret_cast<int *>(ws + arrived_at);
-    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, st, &wb);
+    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, st, &wb, &x_blocks);
     if (rc != HIPGPT_OK) return rc;
     Cut *cuts = reinterpret_cast<Cut *>(ws + cuts_at);
-    const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr};
+    const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr,
+                           a.amax + 3, NP == 1 ? x_blocks : 0, const_cast<float *>(a.amax) + 2};
     const cudaError_t e = launch_overlapped(loss_plan_kernel, dim3((unsigned)(pieces + 1)), dim3(kMostPairs), 0, st, plan, a.count, cuts);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_plan_kernel: %s", cudaGetErrorString(e));
     a.shares = reinterpret_cast<float4 *>(ws + shares_at);

@@ -254,7 +254,7 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
  *                              is zero.
  *                              Products run on the tensor pipe with fp32 accumulation.  fp32: from two fp16 pieces of each operand under one
  *                              power of two per matrix (2^-22 of a value down to 2^-17 of the matrix's largest, 2^-40 of that one below).
- *                              bf16: the gradient of the logits is rounded to bf16 before the second product.
+ *                              bf16: the gradient of the logits, in units of the largest |grad_loss|, is rounded to bf16 before the second product.
  */
 #define HIPGPT_TYPE_F32   0
 #define HIPGPT_TYPE_BF16  1

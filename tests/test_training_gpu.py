@@ -220,7 +220,7 @@ def test_loss_and_gradient(dtype, by_token, N, E, V):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("by_token", [True, False])
 def test_loss_gradient_over_several_pieces_of_the_vocabulary(dtype, by_token):
-    N, E, V = 4500, 72, 11000                    # the logits' gradient would be 100 (bf16) or 200 MB in one piece
+    N, E, V = 4500, 72, 26000                    # the logits' gradient would be 240 (bf16) or 480 MB in one piece
     x, w, targets, g = _loss_case(N, E, V, dtype, 1, 0.1)
     ref = tu.Loss(x, w, targets, g, dtype)
     wl = _lay(w, by_token)
@@ -233,6 +233,28 @@ def test_loss_gradient_over_several_pieces_of_the_vocabulary(dtype, by_token):
         tu.within(gx, dx, ex, "grad_x")
         tu.within(gw if by_token else gw.t(), dw, ew, "grad_w")
     assert _status() == 0
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+def test_a_common_weight_of_the_rows_is_not_rounded_into_the_gradient(by_token):
+    """All rows weigh the same, by a number that bf16 would round by nearly half a step (2^-8): with p near 1 / V, -g w[t] is nearly all of a row's gradient, and must not come out
+    smaller than it is throughout.  The share of the wanted gradient that is missing: p - 1 is rounded by at most p < 2^-10 and the results' own roundings go either way (2^-9 / sqrt(N E) < 2^-15
+    of it), so less than 2^-9 with room; g rounded would be 2^-8 - 2^-11."""
+    N, E, V = 300, 64, 4096
+    x, w, targets, g = _loss_case(N, E, V, BF16, 9)
+    x.mul_(2.0 ** -4)                            # (powers of two: still bf16 values)
+    w.mul_(0.25)
+    g.fill_(1.0 + 2.0 ** -8 - 2.0 ** -11)
+    ref = tu.Loss(x, w, targets, g, BF16)
+    assert float(ref.z.abs().max()) < 0.69       # p < 4 / V = 2^-10
+    wl = _lay(w, by_token)
+    loss, lse, gx, gw = _nan(N), _nan(N), _nan(N, E, dtype=BF16), _nan(*wl.shape, dtype=BF16)
+    training.linear_cross_entropy(x, wl, targets, loss, lse, N, E, V, by_token=by_token)
+    training.linear_cross_entropy_backward(x, wl, targets, lse, g, gx, gw, N, E, V, by_token=by_token)
+    (dx, dw), _ = ref.gradients(lse)
+    for got, want in ((gx, dx), (gw if by_token else gw.t(), dw)):
+        missing = 1.0 - float((got.double() * want).sum() / (want * want).sum())
+        assert abs(missing) < 2.0 ** -9
 
 
 # ---- the calls together, captured, side by side -----------------------------------------------------------------------
