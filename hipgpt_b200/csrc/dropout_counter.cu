@@ -17,9 +17,10 @@ namespace hipgpt {
 namespace {
 
 // Counters a thread: more 16-byte words on their way for it, which 16-bit values need (67 M of them: one 59.8 us, two 55.2, four 49.4; with a residual 68.6,
-// 63.2, 63.1) and 32-bit ones do not (33 M with a residual: 59.3, 59.3, 60.0); one where that would leave SMs without a block
+// 63.2, 63.1) and 32-bit ones do not (33 M with a residual: 59.3, 59.3, 60.0).  Fewer values are better spread over more blocks: one against four, 0.5 M 1.7 and 2.3 us, 4 M 4.4 and
+// 5.5, 8 M 8.3 and 8.3, 16 M 16.2 and 14.4
 template <typename T> constexpr int kPer = sizeof(T) == 2 ? 4 : 1;
-constexpr long long kManyValues = 1 << 22;
+constexpr long long kManyValues = 1 << 23;
 
 struct Words { uint32_t w[4]; };
 

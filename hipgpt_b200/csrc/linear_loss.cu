@@ -1116,7 +1116,7 @@ struct Plan {
 };
 
 template <typename T>
-int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth)
+int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
 {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     p.N = N; p.E = E; p.V = V; p.layout = layout;
@@ -1126,9 +1126,10 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, int worth
     p.rows_alloc = round_up(N, kTileM);
     p.w_rows = layout == HIPGPT_WEIGHTS_VE ? V : E;
     p.w_cols = layout == HIPGPT_WEIGHTS_VE ? E : V;
-    // 16-bit weights are read where they lie if TMA can (rows of whole 16-byte words); others are copied once per call, and so are those whose rows do not
-    // begin on lines where there are `worth` rows of x or more: the products then read two lines for each
-    p.pack_w = NP == 2 || p.w_cols % 8 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0 || (p.w_cols % 64 != 0 && N >= worth);
+    // 16-bit weights are read where they lie if TMA can (rows of whole 16-byte words).  Others are copied once per call.  (Where rows do not begin on lines the products
+    // read two lines for each, but a copy gains nothing by that: forward, E = 776 and 1544, V = 20011: 1024 rows 40.5 -> 36.3 and 69 -> 56 us without it, 8192 rows 185 -> 186 and 343 -> 336;
+    // gradient, 776 and 1544: 1024 rows 134 -> 129 and 209 -> 198, 4096 and 8192 rows the same.)
+    p.pack_w = NP == 2 || p.w_cols % 8 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0;
     p.w_ld = p.pack_w ? round_up(p.w_cols, 64) : p.w_cols;
     p.x_plane = (size_t)p.rows_alloc * p.x_ld;
     p.w_plane = (size_t)p.w_rows * p.w_ld;
@@ -1209,7 +1210,7 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
 {
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout, 4096);
+    int rc = plan_call<T>(p, w, N, E, V, layout);
     if (rc != HIPGPT_OK) return rc;
     const int n_tiles = (int)((V + kTileN - 1) / kTileN), m_tiles = (int)(p.rows_alloc / kTileM);
     if ((long long)m_tiles * n_tiles > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d V=%d is beyond one call", N, V);
@@ -1249,7 +1250,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout, 1024);
+    int rc = plan_call<T>(p, w, N, E, V, layout);
     if (rc != HIPGPT_OK) return rc;
     // pieces of the vocabulary of like size
     const long long most = std::max<long long>(1024, (long long)(kPieceBytes / ((size_t)p.rows_alloc * 2 * NP)) / kTileN * kTileN);
