@@ -103,13 +103,13 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 
 // ---- rows that take part, moved together ------------------------------------------------------------------------------
 
-constexpr int kAmaxBlocks = 148, kMostPackBlocks = 512;       // (of loss_pack_kernel: those that have rows of x)
+constexpr int kAmaxBlocks = 4 * 148;
 
 // partial[which][block] = largest finite |value| that the block has seen: x (rows that take part), w, g
 __global__ void __launch_bounds__(256)
-loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial)
+loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial, int early)
 {
-    dependency_wait();
+    if (!early) dependency_wait();
     dependents_may_start();
     __shared__ float warp_max[8];
     const int which = blockIdx.y, lane = threadIdx.x & 31;
@@ -134,16 +134,19 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
         }
     } else {
         const bool vec = E % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-        for (long long n = at >> 5; n < N; n += step >> 5) {
-            const int t = __ldg(targets + n);
-            if (t < 0 || t >= V) continue;
-            const float *row = x + (size_t)n * E;
-            if (vec) {
+        const long long warps = step >> 5;
+        for (long long n0 = at >> 5; n0 < N; n0 += 32 * warps) {             // a warp's next 32 rows: their targets at once
+            const int t = n0 + lane * warps < N ? __ldg(targets + n0 + lane * warps) : -1;
+            unsigned inside = __ballot_sync(0xffffffffu, t >= 0 && t < V);
+            for (; inside; inside &= inside - 1) {
+                const float *row = x + (size_t)(n0 + (__ffs(inside) - 1) * warps) * E;
+                if (vec) {
 #pragma unroll 4
-                for (int e = lane * 4; e < E; e += 128) take4(__ldg(reinterpret_cast<const float4 *>(row + e)));
-            } else {
+                    for (int e = lane * 4; e < E; e += 128) take4(__ldg(reinterpret_cast<const float4 *>(row + e)));
+                } else {
 #pragma unroll 4
-                for (int e = lane; e < E; e += 32) take(__ldg(row + e));
+                    for (int e = lane; e < E; e += 32) take(__ldg(row + e));
+                }
             }
         }
     }
@@ -156,21 +159,28 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
         for (int i = 1; i < 8; ++i) m = fmaxf(m, warp_max[i]);
         partial[which * kAmaxBlocks + blockIdx.x] = m;
     }
+    if (early) dependency_wait();
 }
 
-// The largest of a block's `count` values; every thread of 256 gets it
-__device__ __forceinline__ float block_max(const float *v, int count, float (&sh)[8])
+// The largest of each row of `count` of loss_amax_kernel's; every thread of 256 gets them
+__device__ __forceinline__ void block_max(const float *partial, int rows, int count, float (&sh)[3][8], float (&most)[3])
 {
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < count; i += 256) m = fmaxf(m, v[i]);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+    for (int r = 0; r < 3; ++r) most[r] = 0.0f;
+    for (int i = threadIdx.x; i < count; i += 256)
+#pragma unroll
+        for (int r = 0; r < 3; ++r) if (r < rows) most[r] = fmaxf(most[r], partial[r * kAmaxBlocks + i]);
+#pragma unroll
+    for (int r = 0; r < 3; ++r) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], o));
+        if ((threadIdx.x & 31) == 0) sh[r][threadIdx.x >> 5] = most[r];
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, sh[i]);
-    return m;
+    for (int r = 0; r < 3; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most[r] = fmaxf(most[r], sh[r][i]);
 }
 
 // The values of a row of `cols` from `begin` to `end` -> 16-bit ones in each plane, by one warp.  (What lies between `cols` and the next row is never read.)
@@ -217,7 +227,6 @@ struct Pack {
     size_t plane;
     int *count, *failed, *row_map, *c_targets;
     float *c_lse, *c_g;
-    float *g_most;                           // bf16, backward: the largest finite |g| that each block has seen
     float *zero_loss, *zero_lse;             // forward: what rows that take no part get
     uint8_t *zero_grad;                      // backward: their rows of the gradient
     int *zero_ints;
@@ -226,6 +235,7 @@ struct Pack {
     uint16_t *wp;
     size_t w_plane;
     int w_rows, w_cols, w_ld, w_col_pieces, w_vec;
+    int early, targets_vec;
 };
 constexpr int kPackCols = 1024;
 
@@ -233,35 +243,42 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
 {
-    dependency_wait();
+    if (!p.early) dependency_wait();
     dependents_may_start();
     __shared__ int warp_sum[8];
-    __shared__ float warp_max[8];
+    __shared__ float warp_max[3][8];
+    float most[3];
+    if constexpr (sizeof(T) == 4) block_max(p.partial, p.g ? 3 : 2, p.amax_blocks, warp_max, most);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x >= p.x_blocks) {     // eight pieces of rows of the weights a block
-        const float scale = sizeof(T) == 4 ? pow2_scale(block_max(p.partial + kAmaxBlocks, p.amax_blocks, warp_max)) : 1.0f;
+        const float scale = sizeof(T) == 4 ? pow2_scale(most[1]) : 1.0f;
         const long long job = (long long)(blockIdx.x - p.x_blocks) * 8 + warp;
         const int r = (int)(job / p.w_col_pieces), c = (int)(job % p.w_col_pieces) * kPackCols;
         if (r < p.w_rows) pack_row<T>(w + (size_t)r * p.w_cols, p.wp + (size_t)r * p.w_ld, p.w_plane, c, min(p.w_ld, c + kPackCols), p.w_cols, scale, lane, p.w_vec != 0);
+        if (p.early) dependency_wait();
         return;
     }
     float scale = 1.0f, gscale = 1.0f;
     if constexpr (sizeof(T) == 4) {
-        float most[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) most[i] = i < 2 || p.g ? block_max(p.partial + i * kAmaxBlocks, p.amax_blocks, warp_max) : 0.0f;
-        if (blockIdx.x == 0 && tid < 3) p.amax[tid] = most[tid];
+        if (blockIdx.x == 0 && tid == 0) { p.amax[0] = most[0]; p.amax[1] = most[1]; p.amax[2] = most[2]; }
         scale = pow2_scale(most[0]);
         gscale = grad_scale(most);
     }
     if (blockIdx.x == 0 && tid == 0) *p.failed = 0;
     for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
-    float g_most = 0.0f;
     const int from = blockIdx.x * p.per_block, to = min(p.N, from + p.per_block);
     auto inside = [&](int t) { return t >= 0 && t < p.V; };
-    int before = 0;
+    int before = 0, done = 0;
+    if (p.targets_vec) {
+        done = from / 4 * 4;
 #pragma unroll 8
-    for (int i = tid; i < from; i += 256) before += inside(__ldg(p.targets + i));
+        for (int i = tid; i < done / 4; i += 256) {
+            const int4 t = __ldg(reinterpret_cast<const int4 *>(p.targets) + i);
+            before += inside(t.x) + inside(t.y) + inside(t.z) + inside(t.w);
+        }
+    }
+#pragma unroll 8
+    for (int i = done + tid; i < from; i += 256) before += inside(__ldg(p.targets + i));
 #pragma unroll
     for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     if (lane == 0) warp_sum[warp] = before;
@@ -280,9 +297,7 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
                     p.row_map[i] = n;
                     p.c_targets[i] = t;
                     if (p.g) {
-                        const float g = p.g[n];
-                        if (fabsf(g) <= 3.0e38f) g_most = fmaxf(g_most, fabsf(g));
-                        p.c_g[i] = g * gscale;
+                        p.c_g[i] = p.g[n] * gscale;
                         p.c_lse[i] = p.lse[n];
                     }
                 }
@@ -297,17 +312,6 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
         }
         base += __popc(mask);
     }
-    if (sizeof(T) == 2 && p.g) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) g_most = fmaxf(g_most, __shfl_xor_sync(0xffffffffu, g_most, o));
-        if (lane == 0) warp_max[warp] = g_most;
-        __syncthreads();
-        if (tid == 0) {
-#pragma unroll
-            for (int w8 = 1; w8 < 8; ++w8) g_most = fmaxf(g_most, warp_max[w8]);
-            p.g_most[blockIdx.x] = g_most;
-        }
-    }
     if (to == p.N && from < p.N) {           // the last block that has rows: their number, and zeros up to a whole stage (one at least) of the products that sum over them
         if (tid == 0) *p.count = base;
         const int end = max(kDeep, (base + kDeep - 1) / kDeep * kDeep);
@@ -315,6 +319,7 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
             for (int c = lane * 4; c < p.ld; c += 128)
                 for (int pl = 0; pl < (sizeof(T) == 4 ? 2 : 1); ++pl) *reinterpret_cast<uint2 *>(p.xp + pl * p.plane + (size_t)i * p.ld + c) = make_uint2(0u, 0u);
     }
+    if (p.early) dependency_wait();
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------------
@@ -420,39 +425,54 @@ __device__ __forceinline__ bool before(const Place &a, const Place &b) { return 
 struct PlanArgs {
     int pieces, width, V, E, pairs, dz_stages, dz_extra;
     int ev, with_x, with_w;
-    const float *g_most;                     // bf16: loss_pack_kernel's, of so many blocks, and where the largest goes
-    int g_blocks;
+    const int *targets;
+    const float *g;                          // bf16: where the largest finite |g| goes, of rows that take part; 1 if there is none
+    int N;
     float *most;
 };
+constexpr int kPlanThreads = 512;
 
-// A block for each launch of the backward, kMostPairs threads.  Tiles of kDz are dealt out one by one from pair 0 on.
-__global__ void __launch_bounds__(kMostPairs)
-loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
+// A block for each launch of the backward.  Tiles of kDz are dealt out one by one from pair 0 on.  It counts the rows that take part by itself, and what is launched
+// behind it runs beside it: that starts once this kernel has seen the work before it complete, and waits for this one at its own end (`early`).
+__global__ void __launch_bounds__(kPlanThreads)
+loss_plan_kernel(PlanArgs a, Cut *cuts)
 {
     dependency_wait();
     dependents_may_start();
     __shared__ Cut c;
     __shared__ Lengths len;
-    __shared__ long long scan[kMostPairs / 32];
-    __shared__ int all_fit;
-    __shared__ float warp_most[kMostPairs / 32];
-    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, launch = blockIdx.x, pairs = a.pairs, count = *count_at;
+    __shared__ long long scan[kPlanThreads / 32];
+    __shared__ int warp_count[kPlanThreads / 32];
+    __shared__ float warp_most[kPlanThreads / 32];
+    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, launch = blockIdx.x, pairs = a.pairs;
+    int count = 0;
+    float most = 0.0f;
+    const bool find_most = a.most && launch == 0;
+#pragma unroll 8
+    for (int n = q; n < a.N; n += kPlanThreads) {
+        const int t = __ldg(a.targets + n);
+        const bool inside = t >= 0 && t < a.V;
+        count += inside;
+        if (find_most && inside) {
+            const float g = fabsf(__ldg(a.g + n));
+            if (g <= 3.0e38f) most = fmaxf(most, g);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if (lane == 0) { warp_count[warp] = count; warp_most[warp] = most; }
+    __syncthreads();
+    count = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) { count += warp_count[w]; most = fmaxf(most, warp_most[w]); }
+    if (find_most && q == 0) *a.most = most > 0.0f ? most : 1.0f;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep), e_tiles = (a.E + kTileN - 1) / kTileN;
     auto columns = [&](int piece) { return piece < 0 || piece >= a.pieces ? 0 : (int)min((long long)a.width, a.V - (long long)piece * a.width); };
     auto narrow = [](int n) { return n && (n - 1) % kTileN < kTileN / 2 ? 1 : 0; };
     const int old = columns(launch - 1), v_tiles = (old + kTileN - 1) / kTileN;
-    if (a.g_blocks && launch == 0) {
-        float m = 0.0f;
-        for (int i = q; i < a.g_blocks; i += kMostPairs) m = fmaxf(m, __ldg(a.g_most + i));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) warp_most[warp] = m;
-        __syncthreads();
-        if (q == 0) {
-            for (int w = 1; w < kMostPairs / 32; ++w) m = fmaxf(m, warp_most[w]);
-            *a.most = m > 0.0f ? m : 1.0f;
-        }
-    }
     if (q == 0) {
         c.m_tiles[0] = count_tiles;
         c.n_tiles[0] = a.with_x && old ? e_tiles : 0;
@@ -488,14 +508,11 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
             if (lane >= o) incl += up;
         }
         if (lane == 31) scan[warp] = incl;
-        if (q == 0) all_fit = 1;
         __syncthreads();
         for (int w = 0; w < warp; ++w) incl += scan[w];
         // what is left for the pairs before this one when each has an equal part of everything; a length of at least four stages each
         const long long begin = both * q / pairs - (incl - load), mine = both * (q + 1) / pairs - incl - begin;
-        if (q < pairs && mine < 16) all_fit = 0;
-        __syncthreads();
-        const bool fits = all_fit != 0;
+        const bool fits = __syncthreads_and(q >= pairs || mine >= 16) != 0;
         if (!fits && rounds > 0) continue;
         if (q == 0) c.dealt = dealt;
         if (q <= pairs) {
@@ -511,7 +528,7 @@ loss_plan_kernel(PlanArgs a, const int *__restrict__ count_at, Cut *cuts)
         break;
     }
     __syncthreads();
-    for (int i = q; i < (int)(sizeof(Cut) / sizeof(int)); i += kMostPairs) reinterpret_cast<int *>(cuts + launch)[i] = reinterpret_cast<const int *>(&c)[i];
+    for (int i = q; i < (int)(sizeof(Cut) / sizeof(int)); i += kPlanThreads) reinterpret_cast<int *>(cuts + launch)[i] = reinterpret_cast<const int *>(&c)[i];
 }
 
 // What a pair does, one after the other: its tiles of kDx and kDw, its length of the rest of them, its tiles of kDz
@@ -1139,7 +1156,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
     p.w_at = take(p.pack_w ? NP * p.w_plane * 2 : 0);
     p.ints_at = take((2 + 2 * (size_t)p.rows_alloc) * sizeof(int));
     p.floats_at = take(2 * (size_t)p.rows_alloc * sizeof(float));
-    p.amax_at = take((3 + std::max(3 * kAmaxBlocks, kMostPackBlocks)) * sizeof(float));
+    p.amax_at = take((3 + 3 * kAmaxBlocks) * sizeof(float));
     p.end = at;
     return HIPGPT_OK;
 }
@@ -1147,7 +1164,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
 // Fills what the plan has in the workspace, and of `a` what every form reads
 template <typename T>
 int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, const int *targets, const float *lse, const float *g, float *zero_loss, float *zero_lse, void *zero_grad,
-              int *zero_ints, int zeros, cudaStream_t st, const void **w_base, int *x_blocks)
+              int *zero_ints, int zeros, bool early, cudaStream_t st, const void **w_base)
 {
     int *ints = reinterpret_cast<int *>(ws + p.ints_at);
     float *floats = reinterpret_cast<float *>(ws + p.floats_at), *amax = reinterpret_cast<float *>(ws + p.amax_at);
@@ -1155,15 +1172,16 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     cudaError_t e;
     if constexpr (sizeof(T) == 4) {
         k.amax_blocks = (int)std::min<long long>(kAmaxBlocks, std::max<long long>(((long long)p.V * p.E + 4095) / 4096, ((long long)p.N + 7) / 8));
-        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, g ? 3 : 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, amax + 3);
+        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, g ? 3 : 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, amax + 3, (int)early);
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_amax_kernel: %s", cudaGetErrorString(e));
     }
     k.partial = amax + 3;
-    k.g_most = amax + 3;
     k.amax = amax;
     k.targets = targets; k.lse = lse; k.g = g;
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
-    k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + kMostPackBlocks - 1) / kMostPackBlocks, 32));      // (a block counts the targets before its rows)
+    k.early = early && sizeof(T) == 2;                     // (fp32: loss_amax_kernel is)
+    k.targets_vec = (reinterpret_cast<uintptr_t>(targets) & 15) == 0;
+    k.per_block = (int)(p.N <= 8192 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
@@ -1187,7 +1205,6 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
     a.count = k.count; a.failed = k.failed; a.row_map = k.row_map; a.targets = k.c_targets;
     a.lse = k.c_lse; a.g = k.c_g; a.amax = amax;
-    *x_blocks = k.x_blocks;
     a.rows_alloc = (size_t)p.rows_alloc;
     a.V = p.V;
     return check_launch("loss_pack_kernel");
@@ -1222,9 +1239,9 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     LossArgs a = {};
     const void *wb = nullptr;
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
-    int pairs = 1, x_blocks = 0;
+    int pairs = 1;
     rc = loss_pairs(p.dev, (long long)m_tiles * n_tiles, &pairs);
-    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, st, &wb, &x_blocks);
+    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, false, st, &wb);
     if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, kHalfM);
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
     if (rc != HIPGPT_OK) return rc;
@@ -1260,7 +1277,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     const int e_tiles = (E + kTileN - 1) / kTileN, m_tiles = (int)(p.rows_alloc / kTileM), piece_tiles = (int)(width / kTileN);
     const long long dx_tiles = grad_x ? (long long)m_tiles * e_tiles : 0, dw_tiles = grad_w ? (long long)piece_tiles * e_tiles : 0;
     if (dx_tiles + dw_tiles > 1 << 25 || (long long)m_tiles * piece_tiles > 1 << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d E=%d V=%d is beyond one call", N, E, V);
-    int pairs = 1, x_blocks = 0;
+    int pairs = 1;
     rc = loss_pairs(p.dev, 1 << 30, &pairs);
     if (rc != HIPGPT_OK) return rc;
 
@@ -1275,13 +1292,13 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     LossArgs a = {};
     const void *wb = nullptr;
     a.arrived = reinterpret_cast<int *>(ws + arrived_at);
-    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, st, &wb, &x_blocks);
-    if (rc != HIPGPT_OK) return rc;
     Cut *cuts = reinterpret_cast<Cut *>(ws + cuts_at);
-    const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr,
-                           a.amax + 3, NP == 1 ? x_blocks : 0, const_cast<float *>(a.amax) + 2};
-    const cudaError_t e = launch_overlapped(loss_plan_kernel, dim3((unsigned)(pieces + 1)), dim3(kMostPairs), 0, st, plan, a.count, cuts);
+    const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr, targets, grad_loss, N,
+                           NP == 1 ? reinterpret_cast<float *>(ws + p.amax_at) + 2 : nullptr};
+    const cudaError_t e = launch_overlapped(loss_plan_kernel, dim3((unsigned)(pieces + 1)), dim3(kPlanThreads), 0, st, plan, cuts);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_plan_kernel: %s", cudaGetErrorString(e));
+    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, true, st, &wb);
+    if (rc != HIPGPT_OK) return rc;
     a.shares = reinterpret_cast<float4 *>(ws + shares_at);
     a.sum = reinterpret_cast<float4 *>(ws + sum_at);
     a.expire = take_expiry(700);
