@@ -25,6 +25,11 @@
 // bit), so neither x, W nor dz is ever transposed.  bf16: operands as they are, dz / (largest |g|) rounded to bf16.  fp32: each operand as two fp16 numbers
 // hi + lo of the value times a power of two (one per matrix; 2^-22 of the value), three products a pair: lo hi + hi lo + hi hi.  The tensor
 // core's fp32 sums are cut off, not rounded, so fp32 sums leave TMEM every kPromote stages and go on in registers.
+//
+// Bound, on one B200: the tensor pipe and the power it draws.  8192 x 1024 x 65536 bf16: loss 672 us in a short run (1640 TFLOP/s), 775 where the power cap sets the clock (1.37 GHz); a stage takes
+// 521 cycles, 512 of them products.  Its gradient 2670 - 2850 (1160 - 1240): 620 - 740 cycles a stage, because the operands of a 256 x 256 tile come at the 64 bytes a cycle that an SM takes from L2
+// while the logits' gradient goes out the same way.  8192 x 256 x 5000 fp32 (three products): loss 60 us, 47 of them products (30 at the full rate: 9 rounds of tiles where 8.65 are needed, the last epilogue, the launch),
+// gradient 193, 70 + 100 in its two launches of products (113 at the full rate).  64 x 256 x 5000: 20 us, a chain of four launches.
 #include "elem_types.cuh"
 #include "stream_workspace.hpp"
 #include "tma_host.cuh"
@@ -43,10 +48,14 @@ constexpr int kOperand = kHalfM * kDeep * 2;            // bytes of one block's 
 constexpr int kEpiWarps = 16, kThreads = 32 * (kEpiWarps + 2);      // four warps share a row's columns
 constexpr int kWarpChunks = kTileN / 4 / 32;              // 32-column chunks of a warp
 constexpr int kTmemColumns = 512;
+// Stages that TMEM sums by itself, and what the sums lose: default model's gradient 281 us and 2.2e-7 (of the largest value) with one, 229 and 4.6e-7 with two, 209 and 1.1e-6 with four
+// (sizes as below, before the accumulators were given back earlier)
 constexpr int kPromote = 2;
+// What a piece's gradient of the logits takes.  Longer pieces mean fewer launches and joins, and lie in HBM instead of L2: 8192 x 1024 x 65536 bf16 in pieces of 64 MB 3190 us, 128 MB 2850, 192 MB
+// 2800, 256 MB 2750; 8192 x 256 x 5000 fp32 226 us in two pieces (128 MB), 201 in one
 constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
-// What a tile of kDz costs a pair beside its stages, in quarter stages
+// What a tile of kDz costs a pair beside its stages, in quarter stages (8 and 24 measure alike)
 template <int NP> constexpr int kDzExtra = 8;
 template <int NP> constexpr int kRing = NP == 1 ? 6 : 3;
 constexpr int kRingBytes = 6 * 2 * kOperand;
@@ -1181,7 +1190,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
     k.early = early && sizeof(T) == 2;                     // (fp32: loss_amax_kernel is)
     k.targets_vec = (reinterpret_cast<uintptr_t>(targets) & 15) == 0;
-    k.per_block = (int)(p.N <= 8192 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows)
+    k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows; of 8192, 8 and 32 are alike)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
