@@ -261,8 +261,9 @@ zero_table_kernel(G *table, long long count)
 
 // A block has kSumThreads threads, each 16 bytes of a row of gradients; they form groups of 2^row_log threads that cover a slice of a row (at most kSliceBytes).  A
 // group's task: a piece of the sorted entries, or of the batch at one position.  The rows of kRound entries at a time come into shared memory by
-// one bulk copy each, so that a group has all of them on their way at once without a register.
-constexpr int kSumThreads = 128, kSliceBytes = 16 * kSumThreads, kRound = 16, kSuper = 32;
+// one bulk copy each, so that a group has all of them on their way at once without a register.  (kRound 8, 16, 32: 32768 tokens and a table of 50021 x 1024 92, 88, 87 us; 20 x 1024 89, 64, 67; 8192 tokens,
+// 5000 x 256 fp32 25.6, 25.2, 26.5.)
+constexpr int kSumThreads = 128, kSliceBytes = 16 * kSumThreads, kRound = 16, kSuper = 64;
 constexpr size_t kSumRows = (size_t)kSumThreads * 16 * kRound;          // bytes of a round's rows; behind them the entries
 
 __device__ int g_embed_status = 0;            // 1: a round's copies did not come
@@ -503,8 +504,9 @@ int launch_embedding_backward(const void *grad_out, const int *ids, void *grad_t
     p.slices = ceil_div(E, p.slice);
     while ((1 << p.row_log) * kPer16<T> < p.slice) ++p.row_log;
     p.units = p.slices * std::max(1, (1 << p.row_log) / 32);
-    // a piece: one round of copies, or as many as leave 2048 pieces (so that joining twice is enough)
-    p.piece = kRound * std::max(1, ceil_div(n, 2048 * kRound));
+    // a piece: one round of copies, or as many as leave 65536 threads at work (2048 to 8192 pieces, so that joining twice is enough).  131072 rows of 256 bf16 values: 111 us in 2048 pieces,
+    // 114 in 4096, 120 in 8192; 262144 rows of 64 values: 163, 128, 110
+    p.piece = kRound * std::max(1, ceil_div(n, (long long)std::max(2048, std::min(8192, 65536 >> p.row_log)) * kRound));
     p.pieces = ceil_div(n, p.piece);
     p.pos_piece = kRound * std::max(1, ceil_div(B, 2048 * kRound));
     p.pos_pieces = grad_pos ? ceil_div(B, p.pos_piece) : 0;
