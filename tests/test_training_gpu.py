@@ -50,7 +50,8 @@ def test_embedding(dtype, B, S, V, E, pos):
     assert bool((out[(ids < 0) | (ids >= V)] == 0).all())
 
 
-BACKWARD_SIZES = [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 5), (5, 13, 40, 64), (4, 256, 5000, 256), (3, 700, 90, 200), (300, 7, 1500, 48), (1, 4500, 3, 33), (9, 2000, 70000, 16), (200, 1, 17, 520)]
+BACKWARD_SIZES = [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 5), (5, 13, 40, 64), (4, 256, 5000, 256), (3, 700, 90, 200), (300, 7, 1500, 48), (1, 4500, 3, 33), (9, 2000, 70000, 16), (200, 1, 17, 520),
+                  (20, 2000, 300, 1024), (70, 2000, 50000, 8)]         # several rounds of copies a piece; several tiles a block of the sort
 
 
 @pytest.mark.parametrize("dtype,gt", [(F32, F32), (BF16, BF16), (BF16, F32)])
