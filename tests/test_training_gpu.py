@@ -258,6 +258,42 @@ def test_a_common_weight_of_the_rows_is_not_rounded_into_the_gradient(by_token):
         assert abs(missing) < 2.0 ** -9
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,E,V", [(1, 8, 2), (300, 72, 1001)])
+def test_loss_of_no_row_that_takes_part(dtype, N, E, V):
+    x, w, targets, g = _nan(N, E, dtype=dtype), _normal(_gen(1), V, E, dtype=dtype), torch.full((N,), V, dtype=torch.int32, device="cuda"), _nan(N)
+    loss, lse, gx, gw = _nan(N), _nan(N), _nan(N, E, dtype=dtype), _nan(V, E, dtype=dtype)
+    training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V)
+    training.linear_cross_entropy_backward(x, w, targets, lse, g, gx, gw, N, E, V)
+    assert all(bool((t == 0).all()) for t in (loss, lse, gx, gw))
+    old = _normal(_gen(2), V, E, dtype=dtype)
+    gw = old.clone()
+    training.linear_cross_entropy_backward(x, w, targets, lse, g, None, gw, N, E, V, accumulate=True)
+    assert torch.equal(gw, old) and _status() == 0
+
+
+def test_the_calls_through_ctypes_give_the_same_bits(monkeypatch):
+    from hipgpt_b200 import launchers
+    N, E, V = 40, 72, 300
+    x, w, targets, g = _loss_case(N, E, V, BF16, 4, 0.2)
+    ids = _ids(_gen(6), N, V, -1, V + 1)
+    pos = _normal(_gen(7), 8, E, dtype=BF16)
+
+    def calls():
+        out, y, loss, lse = _nan(N, E, dtype=BF16), _nan(N, E, dtype=BF16), _nan(N), _nan(N)
+        gx, gw, gt, gp = _nan(N, E, dtype=BF16), _nan(V, E, dtype=BF16), _nan(V, E), _nan(8, E)
+        training.embedding_scaled(ids, w, pos, out, 5, 8, V, E, scale=2.0)
+        training.dropout_counter(x, out, y, 0.3, seed=-5, offset=1 << 40)
+        training.linear_cross_entropy(x, w, targets, loss, lse, N, E, V)
+        training.linear_cross_entropy_backward(x, w, targets, lse, g, gx, gw, N, E, V)
+        training.embedding_backward(gx, ids, gt, gp, 5, 8, V, E)
+        return [out, y, loss, lse, gx, gw, gt, gp]
+
+    first = calls()
+    monkeypatch.setattr(launchers, "_native", launchers._ThroughCtypes)
+    assert all(torch.equal(a, b) for a, b in zip(first, calls()))
+
+
 # ---- the calls together, captured, side by side -----------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
