@@ -23,7 +23,7 @@
 // Products: tcgen05.mma.cta_group::2, 256 x 256 tiles of two blocks, 64 deep stages by TMA in a ring, two accumulators in TMEM: the products of a
 // tile run while eight warps take the tile before it out.  Any operand may be contiguous along the reduction or across it (a descriptor
 // bit), so neither x, W nor dz is ever transposed.  bf16: operands as they are, dz / (largest |g|) rounded to bf16.  fp32: each operand as two fp16 numbers
-// hi + lo of the value times a power of two (one per matrix; 2^-22 of the value), three products a pair: lo hi + hi lo + hi hi.  The tensor
+// hi + lo of the value times a power of two (2^-22 of the value; row_scales), three products a pair: lo hi + hi lo + hi hi.  The tensor
 // core's fp32 sums are cut off, not rounded, so fp32 sums leave TMEM every kPromote stages and go on in registers.
 //
 // Bound, on one B200: the tensor pipe and the power it draws.  8192 x 1024 x 65536 bf16: loss 672 us in a short run (1640 TFLOP/s), 775 where the power cap sets the clock (1.37 GHz); a stage takes
@@ -35,6 +35,7 @@
 #include "tma_host.cuh"
 
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -80,13 +81,14 @@ struct Problem {
 };
 
 struct LossArgs {
-    CUtensorMap a[3], b[3], dz_out;
+    CUtensorMap a[3], b[3], dz_out, xq;      // xq: takes the place of x in dW where scales[3] says so (fp32)
     Problem p[3];
     const int *count;                        // rows that take part
     int *failed;                             // a wait of this call has run out: its later launches do nothing
     const int *row_map, *targets;            // of the rows that take part
     const float *lse, *g;
-    const float *amax;                       // the largest |x|, |w| (fp32), |g|
+    const float *x_inv, *row_unit;           // fp32: what takes a row's scale out of its logits, and out of its row of dx
+    const float *scales;                     // fp32: what takes W's scale out; two whose product takes the scales of dz and x out of dW; 1: dW takes xq.  bf16: [2] the largest |g|
     float2 *part;                            // kForward: [tile of the vocabulary][row] maximum and sum
     float *z_target;
     float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
@@ -95,14 +97,37 @@ struct LossArgs {
     int first, last;                         // the launch's share of dx is that of the first, the last piece
     size_t rows_alloc;
     int v0, V;                               // first column of the piece whose logits are formed, and of all
+    int x_is_a;                              // dW's first operand is x
     int expire;
 };
 
 // bf16: the gradient of the logits is rounded in units of the largest |g|.  With one g for all rows (a mean) the target's element then is p - 1, all but exact where p is small;
 // rounded as it is, -g would be off by the same half step of bf16 in every row, and that element is most of the row's gradient.
-// fp32 operands: x = (hi + lo) / scale.  The gradient of the logits is |dz| <= 2 |g|: 2^14 / (power of two above the largest |g|) leaves room
-__device__ __forceinline__ float operand_scale(const float *amax, int which) { return pow2_scale(amax[which]); }
-__device__ __forceinline__ float grad_scale(const float *amax) { return operand_scale(amax, 2) * 0.5f; }
+//
+// fp32: an operand is hi + lo, two fp16 numbers of the value times a power of two that brings the largest of its row (x) or of the matrix (W) into [2^14, 2^15); nothing is kept below 2^-39 of that one.
+// The gradient of the logits, of at most a few times |g| (p may pass 1 a little where lse is the caller's), is scaled row by row to [2^13, 2^14) at |g|, so a row that weighs little keeps its bits; what takes
+// that out multiplies its row of dx.  In dW, a sum over the rows, |g| max|x| of all rows lie under one scale.  A row h binades below the largest of these leaves up to 8 of them to its dz, of which its
+// row of dx can spare that many (2^-30 of g is left, and the errors of 65536 columns add up to 2^-24).  Only where a row lies deeper does dW take a second copy of x, whose rows are smaller by the rest.
+constexpr int kMostShift = 8;
+// floor(log2 a) of a finite a > 0, at least -112
+__device__ __forceinline__ int exponent_of(float a) { return max((int)(__float_as_uint(a) >> 23) - 127, -112); }
+// 2^e; zero below the normal numbers
+__device__ __forceinline__ float pow2(int e) { return e < -126 ? 0.0f : __uint_as_float((uint32_t)(127 + min(e, 127)) << 23); }
+
+struct RowScales {
+    float x, x_inv;                          // of a row of x in the logits, and its inverse
+    float x_dw;                              // ... in dW
+    float dz, dz_inv;                        // of the row's gradient of the logits
+};
+// m: the row's largest finite |x|; most: the largest exponent_of(|g|) + exponent_of(m) of all rows
+__device__ __forceinline__ RowScales row_scales(float m, float g, int most)
+{
+    const float ga = fabsf(g);
+    const bool weighs = ga > 0.0f && ga <= FLT_MAX;
+    const int ex = m > 0.0f ? exponent_of(m) : 14, eg = weighs ? exponent_of(ga) : 0;
+    const int below = weighs && m > 0.0f ? most - ex - eg : 0, shift = min(below, kMostShift);
+    return {pow2(14 - ex), pow2(ex - 14), pow2(14 - ex - (below - shift)), pow2(13 - eg - shift), pow2(eg + shift - 13)};
+}
 
 __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 {
@@ -114,17 +139,23 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
 
 constexpr int kAmaxBlocks = 4 * 148;
 
-// partial[which][block] = largest finite |value| that the block has seen: x (rows that take part), w, g
+// partial[1][block] = the largest finite |w| that the block has seen; row_max[n] = that of row n of x, of the rows that take part.  Backward: partial[0][block] = the largest exponent_of(|g_n|) +
+// exponent_of(row_max[n]) of the rows that have both, partial[2][block] = minus the smallest.
 __global__ void __launch_bounds__(256)
-loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial, int early)
+loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial, float *row_max, int early)
 {
     if (!early) dependency_wait();
     dependents_may_start();
-    __shared__ float warp_max[8];
+    __shared__ float warp_max[2][8];
     const int which = blockIdx.y, lane = threadIdx.x & 31;
-    float m = 0.0f;
-    auto take = [&](float v) { v = fabsf(v); m = v <= 3.0e38f ? fmaxf(m, v) : m; };      // (not of infinities and NaN: they stay what they are)
+    float m = 0.0f, minus_least = -INFINITY;
+    auto take = [&](float v) { v = fabsf(v); m = v <= FLT_MAX ? fmaxf(m, v) : m; };      // (not of infinities and NaN: they stay what they are)
     auto take4 = [&](const float4 &v) { take(v.x); take(v.y); take(v.z); take(v.w); };
+    auto over_warp = [](float v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    };
     const long long step = (long long)gridDim.x * 256, at = (long long)blockIdx.x * 256 + threadIdx.x;
     if (which == 1) {
         const long long total = (long long)V * E, words = (reinterpret_cast<uintptr_t>(w) & 15) == 0 ? total / 4 : 0;
@@ -136,19 +167,20 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
         }
         for (; i < words; i += step) take4(__ldg(w4 + i));
         for (i = words * 4 + at; i < total; i += step) take(__ldg(w + i));
-    } else if (which == 2) {
-        for (long long n = at; n < N; n += step) {
-            const int t = __ldg(targets + n);
-            if (t >= 0 && t < V) take(__ldg(g + n));
-        }
     } else {
         const bool vec = E % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
         const long long warps = step >> 5;
+        float most = -INFINITY;
         for (long long n0 = at >> 5; n0 < N; n0 += 32 * warps) {             // a warp's next 32 rows: their targets at once
-            const int t = n0 + lane * warps < N ? __ldg(targets + n0 + lane * warps) : -1;
+            const long long mine = n0 + lane * warps;
+            const int t = mine < N ? __ldg(targets + mine) : -1;
+            const float weight = g && t >= 0 && t < V ? fabsf(__ldg(g + mine)) : 0.0f;
             unsigned inside = __ballot_sync(0xffffffffu, t >= 0 && t < V);
             for (; inside; inside &= inside - 1) {
-                const float *row = x + (size_t)(n0 + (__ffs(inside) - 1) * warps) * E;
+                const int from = __ffs(inside) - 1;
+                const long long n = n0 + from * warps;
+                const float *row = x + (size_t)n * E;
+                m = 0.0f;
                 if (vec) {
 #pragma unroll 4
                     for (int e = lane * 4; e < E; e += 128) take4(__ldg(reinterpret_cast<const float4 *>(row + e)));
@@ -156,29 +188,41 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
 #pragma unroll 4
                     for (int e = lane; e < E; e += 32) take(__ldg(row + e));
                 }
+                m = over_warp(m);
+                if (lane == 0) row_max[n] = m;
+                const float ga = __shfl_sync(0xffffffffu, weight, from);
+                if (m > 0.0f && ga > 0.0f && ga <= FLT_MAX) {
+                    const float e = (float)(exponent_of(m) + exponent_of(ga));
+                    most = fmaxf(most, e);
+                    minus_least = fmaxf(minus_least, -e);
+                }
             }
         }
+        m = most;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) warp_max[threadIdx.x >> 5] = m;
+    m = over_warp(m);
+    if (lane == 0) {                         // (the least is the same in all lanes)
+        warp_max[0][threadIdx.x >> 5] = m;
+        warp_max[1][threadIdx.x >> 5] = minus_least;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 2 - which) {
+        m = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, warp_max[i]);
-        partial[which * kAmaxBlocks + blockIdx.x] = m;
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, warp_max[threadIdx.x][i]);
+        partial[(which + 2 * threadIdx.x) * kAmaxBlocks + blockIdx.x] = m;
     }
     if (early) dependency_wait();
 }
 
-// The largest of each row of `count` of loss_amax_kernel's; every thread of 256 gets them
-__device__ __forceinline__ void block_max(const float *partial, int rows, int count, float (&sh)[3][8], float (&most)[3])
+// The largest of each of loss_amax_kernel's rows (backward: all three, forward: the second); every thread of 256 gets them
+__device__ __forceinline__ void block_max(const float *partial, bool backward, int count, float (&sh)[3][8], float (&most)[3])
 {
 #pragma unroll
-    for (int r = 0; r < 3; ++r) most[r] = 0.0f;
+    for (int r = 0; r < 3; ++r) most[r] = -INFINITY;
     for (int i = threadIdx.x; i < count; i += 256)
 #pragma unroll
-        for (int r = 0; r < 3; ++r) if (r < rows) most[r] = fmaxf(most[r], partial[r * kAmaxBlocks + i]);
+        for (int r = 0; r < 3; ++r) if (backward || r == 1) most[r] = fmaxf(most[r], partial[r * kAmaxBlocks + i]);
 #pragma unroll
     for (int r = 0; r < 3; ++r) {
 #pragma unroll
@@ -225,17 +269,17 @@ __device__ __forceinline__ void pack_row(const T *src, uint16_t *dst, size_t pla
 }
 
 struct Pack {
-    const float *partial;                    // fp32: loss_amax_kernel's
+    const float *partial, *row_max;          // fp32: loss_amax_kernel's
     int amax_blocks;
-    float *amax;
+    float *scales;
     // the rows of x
     const int *targets;
     const float *lse, *g;                    // backward
     int N, E, V, ld, per_block, x_blocks, x_vec;
-    uint16_t *xp;
+    uint16_t *xp, *xq;                       // xq: the rows as dW takes them (fp32), or NULL
     size_t plane;
     int *count, *failed, *row_map, *c_targets;
-    float *c_lse, *c_g;
+    float *c_lse, *c_g, *c_x_inv, *c_unit;
     float *zero_loss, *zero_lse;             // forward: what rows that take no part get
     uint8_t *zero_grad;                      // backward: their rows of the gradient
     int *zero_ints;
@@ -256,22 +300,30 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
     dependents_may_start();
     __shared__ int warp_sum[8];
     __shared__ float warp_max[3][8];
-    float most[3];
-    if constexpr (sizeof(T) == 4) block_max(p.partial, p.g ? 3 : 2, p.amax_blocks, warp_max, most);
+    int w_exp = 14, most = 27;                // (scales of 1)
+    bool deep = false;                       // a row lies more than kMostShift below the largest
+    if constexpr (sizeof(T) == 4) {
+        float largest[3];
+        block_max(p.partial, p.g != nullptr, p.amax_blocks, warp_max, largest);
+        if (largest[1] > 0.0f) w_exp = exponent_of(largest[1]);
+        if (largest[0] > -INFINITY) most = (int)largest[0];
+        deep = largest[0] + largest[2] > (float)kMostShift;
+    }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x >= p.x_blocks) {     // eight pieces of rows of the weights a block
-        const float scale = sizeof(T) == 4 ? pow2_scale(most[1]) : 1.0f;
+        const float scale = pow2(14 - w_exp);
         const long long job = (long long)(blockIdx.x - p.x_blocks) * 8 + warp;
         const int r = (int)(job / p.w_col_pieces), c = (int)(job % p.w_col_pieces) * kPackCols;
         if (r < p.w_rows) pack_row<T>(w + (size_t)r * p.w_cols, p.wp + (size_t)r * p.w_ld, p.w_plane, c, min(p.w_ld, c + kPackCols), p.w_cols, scale, lane, p.w_vec != 0);
         if (p.early) dependency_wait();
         return;
     }
-    float scale = 1.0f, gscale = 1.0f;
-    if constexpr (sizeof(T) == 4) {
-        if (blockIdx.x == 0 && tid == 0) { p.amax[0] = most[0]; p.amax[1] = most[1]; p.amax[2] = most[2]; }
-        scale = pow2_scale(most[0]);
-        gscale = grad_scale(most);
+    if (sizeof(T) == 4 && blockIdx.x == 0 && tid == 0) {
+        p.scales[0] = pow2(w_exp - 14);
+        const int e = most - 27;              // (one power of two could pass the range of fp32)
+        p.scales[1] = pow2(e / 2);
+        p.scales[2] = pow2(e - e / 2);
+        p.scales[3] = deep ? 1.0f : 0.0f;
     }
     if (blockIdx.x == 0 && tid == 0) *p.failed = 0;
     for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
@@ -296,21 +348,38 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
 #pragma unroll
     for (int w8 = 0; w8 < 8; ++w8) base += warp_sum[w8];
     for (int r0 = from; r0 < to; r0 += 32) {
-        const int t = r0 + lane < to ? __ldg(p.targets + r0 + lane) : -1;
+        // each lane looks at one row; what belongs to it is stored by the first warp
+        const bool there = r0 + lane < to;
+        const int t = there ? __ldg(p.targets + r0 + lane) : -1;
+        const float g = p.g && there ? __ldg(p.g + r0 + lane) : 0.0f;
         const unsigned mask = __ballot_sync(0xffffffffu, inside(t));
-        for (int j = warp; j < 32 && r0 + j < to; j += 8) {
-            const int n = r0 + j;
+        RowScales scale = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+        if (sizeof(T) == 4 && there) scale = row_scales(p.row_max[r0 + lane], g, most);       // (of a row that takes no part: not used)
+        if (warp == 0 && inside(t)) {
+            const int i = base + __popc(mask & ((1u << lane) - 1));
+            p.row_map[i] = r0 + lane;
+            p.c_targets[i] = t;
+            if (sizeof(T) == 4) p.c_x_inv[i] = scale.x_inv;
+            if (p.g) {
+                p.c_g[i] = g * scale.dz;
+                p.c_lse[i] = p.lse[r0 + lane];
+                if (sizeof(T) == 4) p.c_unit[i] = scale.dz_inv;
+            }
+        }
+        float x_scale[4], x_dw_scale[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x_scale[k] = __shfl_sync(0xffffffffu, scale.x, warp + 8 * k);
+            x_dw_scale[k] = __shfl_sync(0xffffffffu, scale.x_dw, warp + 8 * k);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int j = warp + 8 * k, n = r0 + j;
+            if (n >= to) break;
             if (mask >> j & 1) {
-                const int i = base + __popc(mask & ((1u << j) - 1));
-                if (lane == j) {
-                    p.row_map[i] = n;
-                    p.c_targets[i] = t;
-                    if (p.g) {
-                        p.c_g[i] = p.g[n] * gscale;
-                        p.c_lse[i] = p.lse[n];
-                    }
-                }
-                pack_row<T>(x + (size_t)n * p.E, p.xp + (size_t)i * p.ld, p.plane, 0, p.ld, p.E, scale, lane, p.x_vec != 0);
+                const size_t at = (size_t)(base + __popc(mask & ((1u << j) - 1))) * p.ld;
+                pack_row<T>(x + (size_t)n * p.E, p.xp + at, p.plane, 0, p.ld, p.E, x_scale[k], lane, p.x_vec != 0);
+                if (sizeof(T) == 4 && deep && p.xq) pack_row<T>(x + (size_t)n * p.E, p.xq + at, p.plane, 0, p.ld, p.E, x_dw_scale[k], lane, p.x_vec != 0);
             } else {
                 if (p.zero_loss && lane == 0) p.zero_loss[n] = p.zero_lse[n] = 0.0f;
                 if (p.zero_grad) {
@@ -324,9 +393,10 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
     if (to == p.N && from < p.N) {           // the last block that has rows: their number, and zeros up to a whole stage (one at least) of the products that sum over them
         if (tid == 0) *p.count = base;
         const int end = max(kDeep, (base + kDeep - 1) / kDeep * kDeep);
+        uint16_t *rows = p.xq && deep ? p.xq : p.xp;
         for (int i = base + warp; i < end; i += 8)
             for (int c = lane * 4; c < p.ld; c += 128)
-                for (int pl = 0; pl < (sizeof(T) == 4 ? 2 : 1); ++pl) *reinterpret_cast<uint2 *>(p.xp + pl * p.plane + (size_t)i * p.ld + c) = make_uint2(0u, 0u);
+                for (int pl = 0; pl < (sizeof(T) == 4 ? 2 : 1); ++pl) *reinterpret_cast<uint2 *>(rows + pl * p.plane + (size_t)i * p.ld + c) = make_uint2(0u, 0u);
     }
     if (p.early) dependency_wait();
 }
@@ -572,7 +642,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     __shared__ uint64_t full[RING], empty[RING], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    __shared__ float scales_s[3];             // what takes the operands' scales out of the logits (fp32), dx, dW
+    __shared__ float scales_s[4];             // LossArgs::scales
     __shared__ float2 part_s[FORM == kForward ? 2 : 1][4][kHalfM];
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
@@ -605,13 +675,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
     };
 
     // No row may take part: one tile of rows of zeros, and one stage, are then worked on (so gradients of zero are written)
-    if (NP == 2 && threadIdx.x == 0) {
-        const float x_inv = pow2_inverse(operand_scale(args.amax, 0)), w_inv = pow2_inverse(operand_scale(args.amax, 1)), g_inv = FORM == kBackward ? pow2_inverse(grad_scale(args.amax)) : 1.0f;
-        scales_s[0] = x_inv * w_inv;
-        scales_s[1] = g_inv * w_inv;
-        scales_s[2] = g_inv * x_inv;
-    }
-    if (NP == 1 && FORM == kBackward && threadIdx.x == 0) scales_s[1] = scales_s[2] = args.amax[2];
+    if (threadIdx.x < 4 && (NP == 2 || FORM == kBackward)) scales_s[threadIdx.x] = args.scales[threadIdx.x];
     const bool failed = *args.failed != 0;
     const int count = *args.count, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
     const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep);
@@ -661,6 +725,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 constexpr int KIND = decltype(kind)::value;
                 const Problem &p = args.p[KIND];
                 const CUtensorMap *ma = &args.a[KIND], *mb = &args.b[KIND];
+                if (NP == 2 && KIND == kDw && scales_s[3] != 0.0f) (args.x_is_a ? ma : mb) = &args.xq;
                 const int m0 = x.m * kTileM + rank * kHalfM, n0 = p.b_n0 + x.n * kTileN + rank * (x.narrow ? kHalfM / 2 : kHalfM);
                 const int end = KIND == kDz ? p.stages : x.k1;
                 for (int k = KIND == kDz ? 0 : x.k0; k < end; ++k) {
@@ -741,7 +806,6 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
         const int quarter = warp & 3, fourth = warp >> 2, row_in_tile = rank * kHalfM + quarter * 32 + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t drained = peer_addr(smem_u32(&acc_empty[0]), 0);
-        const float z_scale = NP == 2 ? scales_s[0] : 1.0f;
         uint8_t *out_s = ring + kRingBytes + warp * kOutBytes;           // (kBackward)
         int unit = 0, part_at = 0;
         while (next(walk, x)) {
@@ -759,11 +823,16 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             // per row: whether it is there, and its target (of the logits), or its row of the result
             const bool here = row < (FORM == kForward || x.kind != kDw ? count : p.rows);
             int of_row = -1;
-            float lse = 0.0f, g = 0.0f, run_max = -INFINITY, run_sum = 0.0f;
+            float lse = 0.0f, g = 0.0f, z_scale = 1.0f, run_max = -INFINITY, run_sum = 0.0f;
             if (here) {
-                if (FORM == kForward || x.kind == kDz) of_row = __ldg(args.targets + row) - args.v0;
-                else of_row = x.kind == kDx ? __ldg(args.row_map + row) : row;
-                if (FORM == kBackward && x.kind == kDz) { lse = __ldg(args.lse + row); g = NP == 2 ? __ldg(args.g + row) : __fdiv_rn(__ldg(args.g + row), scales_s[1]); }
+                if (FORM == kForward || x.kind == kDz) {
+                    of_row = __ldg(args.targets + row) - args.v0;
+                    if constexpr (NP == 2) z_scale = __ldg(args.x_inv + row);          // (W's joins it behind the waits, so that they begin before this has come)
+                } else {
+                    of_row = x.kind == kDx ? __ldg(args.row_map + row) : row;
+                    if (NP == 2 && x.kind == kDx) g = __ldg(args.row_unit + row);
+                }
+                if (FORM == kBackward && x.kind == kDz) { lse = __ldg(args.lse + row); g = NP == 2 ? __ldg(args.g + row) : __fdiv_rn(__ldg(args.g + row), scales_s[2]); }
             }
             const int left_all = (FORM == kForward || x.kind == kDz ? args.V - args.v0 : p.cols) - col0;           // columns from col0 on
 
@@ -869,9 +938,10 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     for (int j = 0; j < 8; ++j) __stcg(sum + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
                     return;
                 }
-                const float out_scale = scales_s[x.kind == kDx ? 1 : 2];
+                // fp32: both powers of two that go into an operand (their product may pass the range of fp32)
+                const float s0 = NP == 1 ? scales_s[2] : scales_s[x.kind == kDx ? 0 : 1], s1 = NP == 1 ? 1.0f : x.kind == kDx ? g : scales_s[2];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= out_scale;
+                for (int j = 0; j < 32; ++j) v[j] = NP == 1 ? v[j] * s0 : v[j] * s0 * s1;
                 const unsigned rows_here = __ballot_sync(0xffffffffu, here);
                 const bool out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
                 if (p.accumulate || !out_vec || left < 32) {
@@ -1000,6 +1070,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     release(unit & 1);
                 }
                 if (FORM == kBackward && !whole && pair == p0) complete = others_there();
+                z_scale = fminf(z_scale * scales_s[0], FLT_MAX);           // (an infinite one would make NaN of a logit of zero)
 #pragma unroll
                 for (int c = 0; c < kWarpChunks; ++c)
                     if (FORM == kForward || c < chunks) take(c, acc[c]);
@@ -1139,11 +1210,12 @@ struct Plan {
     bool pack_w;
     size_t x_plane, w_plane;
     // places in the workspace
-    size_t x_at, w_at, ints_at, floats_at, amax_at, end;
+    size_t x_at, xq_at, w_at, ints_at, floats_at, amax_at, end;
+    bool with_xq;                                    // room for a second copy of the rows
 };
 
 template <typename T>
-int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
+int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, bool with_w_grad)
 {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     p.N = N; p.E = E; p.V = V; p.layout = layout;
@@ -1162,11 +1234,13 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout)
     p.w_plane = (size_t)p.w_rows * p.w_ld;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += padded(bytes); return r; };
+    p.with_xq = with_w_grad && NP == 2;
     p.x_at = take(NP * p.x_plane * 2);
+    p.xq_at = take(p.with_xq ? NP * p.x_plane * 2 : 0);
     p.w_at = take(p.pack_w ? NP * p.w_plane * 2 : 0);
     p.ints_at = take((2 + 2 * (size_t)p.rows_alloc) * sizeof(int));
-    p.floats_at = take(2 * (size_t)p.rows_alloc * sizeof(float));
-    p.amax_at = take((3 + 3 * kAmaxBlocks) * sizeof(float));
+    p.floats_at = take((NP == 2 ? 5 : 2) * (size_t)p.rows_alloc * sizeof(float));
+    p.amax_at = take((4 + 3 * kAmaxBlocks) * sizeof(float));
     p.end = at;
     return HIPGPT_OK;
 }
@@ -1177,16 +1251,17 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
               int *zero_ints, int zeros, bool early, cudaStream_t st, const void **w_base)
 {
     int *ints = reinterpret_cast<int *>(ws + p.ints_at);
-    float *floats = reinterpret_cast<float *>(ws + p.floats_at), *amax = reinterpret_cast<float *>(ws + p.amax_at);
+    float *floats = reinterpret_cast<float *>(ws + p.floats_at), *scales = reinterpret_cast<float *>(ws + p.amax_at), *partial = scales + 4, *row_max = floats + 4 * p.rows_alloc;
     Pack k = {};
     cudaError_t e;
     if constexpr (sizeof(T) == 4) {
         k.amax_blocks = (int)std::min<long long>(kAmaxBlocks, std::max<long long>(((long long)p.V * p.E + 4095) / 4096, ((long long)p.N + 7) / 8));
-        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, g ? 3 : 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, amax + 3, (int)early);
+        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, partial, row_max, (int)early);
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_amax_kernel: %s", cudaGetErrorString(e));
     }
-    k.partial = amax + 3;
-    k.amax = amax;
+    k.partial = partial;
+    k.row_max = row_max;
+    k.scales = scales;
     k.targets = targets; k.lse = lse; k.g = g;
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
     k.early = early && sizeof(T) == 2;                     // (fp32: loss_amax_kernel is)
@@ -1195,9 +1270,10 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
     k.x_vec = p.E % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     k.xp = reinterpret_cast<uint16_t *>(ws + p.x_at);
+    k.xq = p.with_xq ? reinterpret_cast<uint16_t *>(ws + p.xq_at) : nullptr;
     k.plane = p.x_plane;
     k.count = ints; k.failed = ints + 1; k.row_map = ints + 2; k.c_targets = ints + 2 + p.rows_alloc;
-    k.c_lse = floats; k.c_g = floats + p.rows_alloc;
+    k.c_lse = floats; k.c_g = floats + p.rows_alloc; k.c_x_inv = floats + 2 * p.rows_alloc; k.c_unit = floats + 3 * p.rows_alloc;       // (the last two in fp32 only)
     k.zero_loss = zero_loss; k.zero_lse = zero_lse; k.zero_grad = static_cast<uint8_t *>(zero_grad);
     k.zero_ints = zero_ints; k.zeros = zeros;
     long long w_blocks = 0;
@@ -1214,7 +1290,7 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     e = launch_overlapped(loss_pack_kernel<T>, dim3((unsigned)(k.x_blocks + w_blocks)), dim3(256), 0, st, x, w, k);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
     a.count = k.count; a.failed = k.failed; a.row_map = k.row_map; a.targets = k.c_targets;
-    a.lse = k.c_lse; a.g = k.c_g; a.amax = amax;
+    a.lse = k.c_lse; a.g = k.c_g; a.x_inv = k.c_x_inv; a.row_unit = k.c_unit; a.scales = scales;
     a.rows_alloc = (size_t)p.rows_alloc;
     a.V = p.V;
     return check_launch("loss_pack_kernel");
@@ -1222,9 +1298,9 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
 
 // Maps of the operands of one problem, in boxes of 64 x 64; A contiguous along the reduction: of 64 x 128 rows
 template <typename T>
-int x_map(CUtensorMap *m, const Plan &p, const uint8_t *ws, int box)
+int x_map(CUtensorMap *m, const Plan &p, const uint8_t *ws, int box, bool second = false)
 {
-    return operand_map(m, ws + p.x_at, sizeof(T) == 4, p.E, p.rows_alloc, p.x_ld, p.x_plane, sizeof(T) == 4 ? 2 : 1, box);
+    return operand_map(m, ws + (second ? p.xq_at : p.x_at), sizeof(T) == 4, p.E, p.rows_alloc, p.x_ld, p.x_plane, sizeof(T) == 4 ? 2 : 1, box);
 }
 template <typename T>
 int w_map(CUtensorMap *m, const Plan &p, const void *w)
@@ -1237,7 +1313,7 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
 {
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout);
+    int rc = plan_call<T>(p, w, N, E, V, layout, false);
     if (rc != HIPGPT_OK) return rc;
     const int n_tiles = (int)((V + kTileN - 1) / kTileN), m_tiles = (int)(p.rows_alloc / kTileM);
     if ((long long)m_tiles * n_tiles > 1LL << 30) return fail(HIPGPT_ERR_UNSUPPORTED, "N=%d V=%d is beyond one call", N, V);
@@ -1277,7 +1353,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv);
     Plan p;
-    int rc = plan_call<T>(p, w, N, E, V, layout);
+    int rc = plan_call<T>(p, w, N, E, V, layout, grad_w != nullptr);
     if (rc != HIPGPT_OK) return rc;
     // pieces of the vocabulary of like size
     const long long most = std::max<long long>(1024, (long long)(kPieceBytes / ((size_t)p.rows_alloc * 2 * NP)) / kTileN * kTileN);
@@ -1320,6 +1396,8 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDx], p, wb);
     if (rc == HIPGPT_OK) rc = x_map<T>(ev ? &a.a[kDw] : &a.b[kDw], p, ws, 64);
+    if (rc == HIPGPT_OK && p.with_xq) rc = x_map<T>(&a.xq, p, ws, 64, true);
+    a.x_is_a = ev;
     if (rc != HIPGPT_OK) return rc;
     a.p[kDz].stages = (E + kDeep - 1) / kDeep;
     a.p[kDz].b_across = ev;

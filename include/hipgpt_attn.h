@@ -252,8 +252,11 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
  *   hipgpt_linear_cross_entropy_backward  gradients of x and the weights from grad_loss[N] (each row's; read only where the target is inside) and the
  *                              forward's lse; either may be NULL; accumulate_w != 0: added to what grad_w holds.  grad_x of a row that takes no part
  *                              is zero.
- *                              Products run on the tensor pipe with fp32 accumulation.  fp32: from two fp16 pieces of each operand under one
- *                              power of two per matrix (2^-22 of a value down to 2^-17 of the matrix's largest, 2^-40 of that one below).
+ *                              Products run on the tensor pipe with fp32 accumulation.  fp32: from two fp16 pieces of each operand under a
+ *                              power of two per row of x, per row of the logits' gradient and for the weights (2^-22 of a value down to 2^-17 of the largest
+ *                              of its row, or of the weights; 2^-39 of that one below), so a row keeps its digits however little it weighs or measures
+ *                              beside others.  In grad_w, a sum over the rows, a row's share keeps 2^-38 of the largest |grad_loss| max|x| of all rows, 2^8
+ *                              finer for rows that lie deeper.  An infinity in x or the weights makes NaN of the fp32 logits that it meets.
  *                              bf16: the gradient of the logits, in units of the largest |grad_loss|, is rounded to bf16 before the second product.
  */
 #define HIPGPT_TYPE_F32   0

@@ -1,0 +1,151 @@
+"""The loss and its gradient over the whole range of values: rows that weigh or measure very differently, values next to the type's largest, infinities and NaN
+in rows that take part, sums of many terms of one sign."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from hipgpt_b200 import training  # noqa: E402
+from tests import training_util as tu  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _case(N, E, V, dtype, seed):
+    gen = _gen(seed)
+    w = torch.randn(V, E, generator=gen, device="cuda") * (1.5 / E ** 0.5)
+    targets = torch.randint(0, V, (N,), generator=gen, device="cuda", dtype=torch.int32)
+    x = torch.randn(N, E, generator=gen, device="cuda") + 1.5 * w[targets.long()]
+    return x.to(dtype), w.to(dtype), targets
+
+
+def _nan_like(t):
+    return torch.full_like(t, NAN)
+
+
+def _forward(x, w, targets, by_token):
+    N, (V, E) = x.shape[0], w.shape
+    wl = w if by_token else w.t().contiguous()
+    loss, lse = torch.full((N,), NAN, device="cuda"), torch.full((N,), NAN, device="cuda")
+    training.linear_cross_entropy(x, wl, targets, loss, lse, N, E, V, by_token=by_token)
+    return loss, lse
+
+
+def _backward(x, w, targets, lse, g, by_token):
+    N, (V, E) = x.shape[0], w.shape
+    wl = w if by_token else w.t().contiguous()
+    gx, gw = _nan_like(x), _nan_like(wl)
+    training.linear_cross_entropy_backward(x, wl, targets, lse, g, gx, gw, N, E, V, by_token=by_token)
+    return gx, gw if by_token else gw.t()
+
+
+class _Fp32:
+    """float64 results for fp32 calls and bounds that go row by row.
+
+    An operand is two fp16 numbers, 2^-22 of the value, and the product of the two low ones is left out (2^-22); below 2^-39 of the largest value of
+    its row (x) or of the matrix (W) nothing is kept.  TMEM adds up 24 instructions that may each cut off a step (2^-23), then fp32 additions follow, one for
+    128 inner indices and one for each of at most 74 pairs that share a tile.  A row's gradient of the logits keeps 2^-29 of its weight at least; a row of x in the
+    weights' gradient 2^-38 of the largest |g| max|x| of all rows, made 2^a finer for a row that is a (at most 8) binades and some more below that."""
+
+    def __init__(self, x, w, targets, g, lse):
+        x, w, g, lse = x.double(), w.double(), g.double(), lse.double()
+        (N, E), V = x.shape, w.shape[0]
+        step, half = 2.0 ** -23, 2.0 ** -24
+        run = lambda k: 24 * step + (-(-k // 128) + 76) * half  # noqa: E731
+        xa, wa, xmax, wmax = x.abs(), w.abs(), x.abs().max(1, keepdim=True).values, w.abs().max()
+        z, at = x @ w.t(), targets.long()
+        ez = xa @ wa.t() * (3 * 2.0 ** -22 + run(E)) + 2.0 ** -38 * E * xmax * wmax
+        rows = torch.arange(N, device=x.device)
+        self.lse, self.e_lse = torch.logsumexp(z, 1), ez.max(1).values + (64 + V / 1024 + 40) * half + 2.0 ** -21 + 2.0 ** -22 * torch.logsumexp(z, 1).abs()
+        self.loss, self.e_loss = self.lse - z[rows, at], 2 * self.e_lse + half * z[rows, at].abs()
+        p = torch.exp(z - lse[:, None])
+        dz, ga = p.clone(), g.abs()[:, None]
+        dz[rows, at] -= 1
+        edz = p * (2 * ez + (z - lse[:, None]).abs() * 2.0 ** -22 + 2.0 ** -21)
+        edz[rows, at] += 2.0 ** -23
+        edz = (edz + (2.0 ** -22 + 2.0 ** -22) * dz.abs() + 2.0 ** -29) * ga
+        dz = dz * g[:, None]
+        self.dx, self.dw = dz @ w, dz.t() @ x
+        da = dz.abs() + edz
+        self.e_dx = edz @ wa + da @ wa * (3 * 2.0 ** -22 + run(V)) + 2.0 ** -39 * wmax * da.sum(1, keepdim=True) + 2 * half * self.dx.abs() + 1e-38
+        most = (ga * xmax).max()
+        a = torch.log2(most / (ga * xmax).clamp(min=1e-300)).sub(6).floor().clamp(0, 8)
+        floor = 2.0 ** -38 * most * 2.0 ** -a / ga.clamp(min=1e-300) * (ga > 0)
+        self.e_dw = edz.t() @ xa + da.t() @ xa * (3 * 2.0 ** -22 + run(N)) + da.t() @ floor.expand(N, E) + 2 * half * self.dw.abs() + 1e-38
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+@pytest.mark.parametrize("light", [1.0, 1e-4, 1e-6, 1e-8, 1e-12, 1e-20])
+def test_fp32_gradient_of_rows_that_weigh_little(by_token, light):
+    """One row of weight 1, the others of `light`: the gradient of every row is as good as if it were alone."""
+    N, E, V = 300, 256, 5000
+    x, w, targets = _case(N, E, V, F32, 5)
+    g = torch.full((N,), light, device="cuda")
+    g[17], g[200] = 1.0, -light / 3
+    _, lse = _forward(x, w, targets, by_token)
+    gx, gw = _backward(x, w, targets, lse, g, by_token)
+    ref = _Fp32(x, w, targets, g, lse)
+    tu.within(gx, ref.dx, ref.e_dx, "grad_x")
+    tu.within(gw, ref.dw, ref.e_dw, "grad_w")
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+@pytest.mark.parametrize("large,small", [(1e8, 1.0), (1.0, 1e-10), (1e30, 1e-30)])
+def test_fp32_rows_of_unequal_magnitude(by_token, large, small):
+    N, E, V = 200, 128, 1500
+    x, w, targets = _case(N, E, V, F32, 6)
+    x[::3] *= small
+    x[7] *= large
+    g = torch.ones(N, device="cuda")
+    loss, lse = _forward(x, w, targets, by_token)
+    gx, gw = _backward(x, w, targets, lse, g, by_token)
+    ref = _Fp32(x, w, targets, g, lse)
+    others = torch.arange(N, device="cuda") != 7           # (row 7's own logits are so large that its p is 0 or 1; an lse of 1e30 has no digits for it)
+    tu.within(loss[others], ref.loss[others], ref.e_loss[others], "loss")
+    tu.within(lse, ref.lse, ref.e_lse, "lse")
+    tu.within(gx[others], ref.dx[others], ref.e_dx[others], "grad_x")
+    g[7] = 0.0                                             # its gradients left out, the others' show in the weights' too
+    gx, gw = _backward(x, w, targets, lse, g, by_token)
+    ref = _Fp32(torch.where(others[:, None], x, torch.zeros_like(x)), w, targets, g, torch.where(others, lse, torch.full_like(lse, math.log(V))))
+    tu.within(gw, ref.dw, ref.e_dw, "grad_w")
+    assert bool((gx[7] == 0).all())
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+def test_fp32_values_next_to_the_largest(by_token):
+    """3.3e38 in x or in W: finite values, so finite logits where the other factor is small."""
+    N, E, V = 40, 64, 300
+    x, w, targets = _case(N, E, V, F32, 7)
+    g = torch.ones(N, device="cuda")
+    for which in (0, 1):
+        xs, ws = (x * 1e33, w * 1e-32) if which == 0 else (x * 1e-32, w * 1e33)
+        big = xs if which == 0 else ws
+        big[3, 5] = 3.3e38
+        loss, lse = _forward(xs, ws, targets, by_token)
+        ref = _Fp32(xs, ws, targets, g, lse)
+        tu.within(lse, ref.lse, ref.e_lse, "lse")
+        tu.within(loss, ref.loss, ref.e_loss, "loss")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("by_token", [True, False])
+def test_nan_in_a_row_that_takes_part_stays_in_it(dtype, by_token):
+    N, E, V = 300, 72, 900
+    x, w, targets = _case(N, E, V, dtype, 9)
+    g = torch.rand(N, generator=_gen(1), device="cuda") + 0.5
+    loss0, lse0 = _forward(x, w, targets, by_token)
+    gx0, _ = _backward(x, w, targets, lse0, g, by_token)
+    x[5, 3], x[290] = NAN, NAN
+    loss, lse = _forward(x, w, targets, by_token)
+    bad = torch.zeros(N, dtype=torch.bool, device="cuda")
+    bad[[5, 290]] = True
+    assert bool(torch.isnan(loss[bad]).all() and torch.isnan(lse[bad]).all())
+    assert torch.equal(loss[~bad], loss0[~bad]) and torch.equal(lse[~bad], lse0[~bad])
+    gx, gw = _backward(x, w, targets, lse, g, by_token)
+    assert torch.equal(gx[~bad], gx0[~bad]) and bool(torch.isnan(gx[bad]).all()) and bool(torch.isnan(gw).all())
