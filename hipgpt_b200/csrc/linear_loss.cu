@@ -52,6 +52,10 @@ constexpr int kTmemColumns = 512;
 // Stages that TMEM sums by itself, and what the sums lose: default model's gradient 281 us and 2.2e-7 (of the largest value) with one, 229 and 4.6e-7 with two, 209 and 1.1e-6 with four
 // (sizes as below, before the accumulators were given back earlier)
 constexpr int kPromote = 2;
+// bf16: a sum that stays in TMEM is cut off by up to 2^-23 of itself for each 16 terms, always towards zero (262144 terms of one sign in one sum: 1.6e-3 short, 65536: 3e-4).  The loss adds its logits up in registers
+// every 16 stages (64 instructions: within 2^-17).  The backward, whose results are rounded to bf16, stores a tile's sum every 128 (512: within 2^-14, a 64th of a rounding) and adds it to the next one's: accumulators
+// kept in registers there cost every tile (8192 x 256 x 5000 93 -> 106 us, by what else then leaves the registers).
+constexpr int kLossStages = 16, kGradStages = 128;
 // What a piece's gradient of the logits takes.  Longer pieces mean fewer launches and joins, and lie in HBM instead of L2: 8192 x 1024 x 65536 bf16 in pieces of 64 MB 3190 us, 128 MB 2850, 192 MB
 // 2800, 256 MB 2750; 8192 x 256 x 5000 fp32 226 us in two pieces (128 MB), 201 in one
 constexpr size_t kPieceBytes = 192u << 20;
@@ -63,6 +67,7 @@ constexpr int kRingBytes = 6 * 2 * kOperand;
 enum Form { kForward, kBackward };
 constexpr int kOutBytes = 32 * 64;                      // a warp's 32 rows of 64 bytes on their way out
 template <Form FORM> constexpr size_t kGemmSmem = kRingBytes + (FORM == kBackward ? kEpiWarps * kOutBytes : 0) + 1024;
+template <Form FORM, int NP> constexpr int kSumStages = NP == 2 ? kPromote : FORM == kForward ? kLossStages : kGradStages;
 enum Kind { kDx, kDw, kDz };                            // problems of kBackward; kForward's one problem lies at kDz's place
 
 __device__ int g_loss_status = 0;
@@ -91,7 +96,7 @@ struct LossArgs {
     const float *scales;                     // fp32: what takes W's scale out; two whose product takes the scales of dz and x out of dW; 1: dW takes xq.  bf16: [2] the largest |g|
     float2 *part;                            // kForward: [tile of the vocabulary][row] maximum and sum
     float *z_target;
-    float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
+    float4 *shares, *sum;                    // kBackward: tiles left by several pairs, [2 a pair], and (bf16) long ones so far, [1 a pair]; dx so far, [tile].  Of a tile: [column / 4][row]
     int *arrived;                            // [tile][block of the pair][warp]: pairs that have left their share of a tile
     const struct Cut *cut;                   // the launch's
     int first, last;                         // the launch's share of dx is that of the first, the last piece
@@ -629,6 +634,33 @@ __device__ __forceinline__ float2 join_parts(float2 a, float2 b)
     return make_float2(m, a.y * ex2_approx((a.x - ref) * kLog2e) + b.y * ex2_approx((b.x - ref) * kLog2e));
 }
 
+// 32 columns of a thread's row, four of them at `to`, the next kTileM further on
+__device__ __forceinline__ void put_tile(float4 *to, const float (&v)[32])
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) __stcg(to + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+}
+__device__ __forceinline__ void add_tile(const float4 *from, float (&v)[32])
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float4 o = __ldcg(from + j * kTileM);
+        v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
+    }
+}
+// A sum of TMEM's, added to what a thread has stored at `so_far` if `more`, and stored there.  (Not inline: few calls come here, and those that do not keep their registers.)
+__device__ __noinline__ void put_by(uint32_t tmem, float4 *so_far, int chunks, bool more)
+{
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+        float v[32];
+        tmem_ld32(tmem + (uint32_t)(32 * c), v);
+        tmem_wait_ld();
+        if (more) add_tile(so_far + c * 8 * kTileM, v);
+        put_tile(so_far + c * 8 * kTileM, v);
+    }
+}
+
 // T: the storage type; operands have one plane (bf16) or two (fp32 as fp16 hi and lo).  site codes in the status word: 1 stage landed, 2 stage free,
 // 3 accumulator complete, 4 accumulator drained
 template <Form FORM, typename T>
@@ -769,7 +801,8 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                                        ((uint32_t)((x.narrow ? kTileN / 2 : kTileN) >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
                 const uint32_t a_lbo = p.a_across ? kOperand / 2 : 16, b_lbo = p.b_across ? kOperand / 2 : 16;
                 const uint64_t a_step = p.a_across ? 128 : 2, b_step = p.b_across ? 128 : 2;
-                const int begin = KIND == kDz ? 0 : x.k0, end = KIND == kDz ? p.stages : x.k1, unit_stages = NP == 1 ? end - begin : kPromote;
+                constexpr int unit_stages = kSumStages<FORM, NP>;
+                const int begin = KIND == kDz ? 0 : x.k0, end = KIND == kDz ? p.stages : x.k1;
                 for (int k0 = begin; k0 < end; k0 += unit_stages, ++unit) {
                     const uint32_t acc = tmem + (uint32_t)((unit & 1) * kTileN);
                     if (unit >= 2) wait(&acc_empty[unit & 1], (uint32_t)((unit / 2 - 1) & 1), 4);
@@ -838,6 +871,9 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 
             // where 32 columns of this thread's row begin in a tile of `shares` or `sum`
             auto tile_at = [&](int tile, int c) { return ((size_t)tile * (kTileN / 4) + (size_t)((mine0 + 32 * c) / 4)) * kTileM + row_in_tile; };
+
+            // the sum of a long tile's stages so far, behind the pairs' shares
+            auto so_far = [&](int c) { return args.shares + tile_at(2 * pairs + pair, c); };
 
             // kForward: 32 columns from col0 + 32 c on
             auto log_sum = [&](int c, float (&v)[32]) {
@@ -933,9 +969,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 const int left = left_all - 32 * c;
                 if (left <= 0 || __any_sync(0xffffffffu, abort_flag)) return;
                 if (x.kind == kDx && !args.last) {
-                    float4 *sum = args.sum + tile_at(x.tile, c);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) __stcg(sum + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    put_tile(args.sum + tile_at(x.tile, c), v);
                     return;
                 }
                 // fp32: both powers of two that go into an operand (their product may pass the range of fp32)
@@ -991,9 +1025,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
             };
             // ... and of one that is not: into this pair's share
             auto leave = [&](int c, const float (&v)[32]) {
-                float4 *share = args.shares + tile_at(2 * pair + (x.k0 == 0), c);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) __stcg(share + j * kTileM, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                put_tile(args.shares + tile_at(2 * pair + (x.k0 == 0), c), v);
             };
 
             // A tile that falls to several pairs (they follow one another, each with a part of its stages): the first of them is usually the last to come to it,
@@ -1015,14 +1047,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
 
             auto add_sources = [&](int c, float (&v)[32]) {
 #pragma unroll 1
-                for (int i = 0; i < sources; ++i) {
-                    const float4 *from = source(i, c);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float4 o = __ldcg(from + j * kTileM);
-                        v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
-                    }
-                }
+                for (int i = 0; i < sources; ++i) add_tile(source(i, c), v);
             };
 
             // whether the others' shares of a tile that this pair is the first of are there
@@ -1046,15 +1071,20 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     leave(c, v);
                 }
             };
-            if constexpr (NP == 2) {
+            constexpr int unit_stages = kSumStages<FORM, NP>;
+            auto await_sum = [&] {
+                wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
+                tc_fence_after();
+            };
+            if (NP == 2 || (FORM == kForward && x.k1 - x.k0 > unit_stages)) {
+                // TMEM's sums are added up in registers
                 float acc[kWarpChunks][32];
 #pragma unroll
                 for (int c = 0; c < kWarpChunks; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
-                for (int k0 = x.k0; k0 < x.k1; k0 += kPromote, ++unit) {
-                    wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
-                    tc_fence_after();
+                for (int k0 = x.k0; k0 < x.k1; k0 += unit_stages, ++unit) {
+                    await_sum();
 #pragma unroll
                     for (int c = 0; c < kWarpChunks; ++c) {
                         if (c >= chunks) continue;
@@ -1070,13 +1100,17 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     release(unit & 1);
                 }
                 if (FORM == kBackward && !whole && pair == p0) complete = others_there();
-                z_scale = fminf(z_scale * scales_s[0], FLT_MAX);           // (an infinite one would make NaN of a logit of zero)
+                if constexpr (NP == 2) z_scale = fminf(z_scale * scales_s[0], FLT_MAX);           // (an infinite one would make NaN of a logit of zero)
 #pragma unroll
                 for (int c = 0; c < kWarpChunks; ++c)
                     if (FORM == kForward || c < chunks) take(c, acc[c]);
             } else {
-                wait(&acc_full[unit & 1], (uint32_t)((unit / 2) & 1), 3);
-                tc_fence_after();
+                for (int k0 = x.k0; FORM == kBackward && k0 + unit_stages < x.k1; k0 += unit_stages, ++unit) {
+                    await_sum();
+                    put_by(lane_base + (uint32_t)((unit & 1) * kTileN + mine0), so_far(0), chunks, k0 > x.k0);
+                    release(unit & 1);
+                }
+                await_sum();
                 if (FORM == kBackward && !whole && pair == p0) complete = others_there();
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
@@ -1084,6 +1118,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     tmem_ld32(lane_base + (uint32_t)((unit & 1) * kTileN + mine0 + 32 * c), v);
                     tmem_wait_ld();
                     if (c == chunks - 1) release(unit & 1);
+                    if (FORM == kBackward && x.k1 - x.k0 > unit_stages) add_tile(so_far(c), v);
                     take(c, v);
                 }
                 ++unit;
@@ -1368,7 +1403,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     if (rc != HIPGPT_OK) return rc;
 
     const size_t tile_bytes = (size_t)kTileM * kTileN * sizeof(float), dz_plane = (size_t)p.rows_alloc * width, dz_bytes = padded(NP * dz_plane * 2);
-    const size_t dz_at = p.end, shares_at = dz_at + (pieces > 1 ? 2 : 1) * dz_bytes, sum_at = shares_at + 2 * pairs * tile_bytes, arrived_at = sum_at + (pieces > 1 ? dx_tiles * tile_bytes : 0);
+    const size_t dz_at = p.end, shares_at = dz_at + (pieces > 1 ? 2 : 1) * dz_bytes, sum_at = shares_at + (NP == 1 ? 3 : 2) * pairs * tile_bytes, arrived_at = sum_at + (pieces > 1 ? dx_tiles * tile_bytes : 0);
     const int arrived = (int)(dx_tiles + dw_tiles) * 2 * kEpiWarps;
     const size_t cuts_at = arrived_at + padded((size_t)arrived * sizeof(int));
     StreamWorkspace::Lease lease;

@@ -257,7 +257,9 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
  *                              of its row, or of the weights; 2^-39 of that one below), so a row keeps its digits however little it weighs or measures
  *                              beside others.  In grad_w, a sum over the rows, a row's share keeps 2^-38 of the largest |grad_loss| max|x| of all rows, 2^8
  *                              finer for rows that lie deeper.  An infinity in x or the weights makes NaN of the fp32 logits that it meets.
- *                              bf16: the gradient of the logits, in units of the largest |grad_loss|, is rounded to bf16 before the second product.
+ *                              bf16: the gradient of the logits, in units of the largest |grad_loss|, is rounded to bf16 before the second product (so
+ *                              is the weight of a row that weighs less, alike in all rows of its weight); no sum stays on the tensor pipe, which cuts off
+ *                              where others round, for more than 8192 terms.
  */
 #define HIPGPT_TYPE_F32   0
 #define HIPGPT_TYPE_BF16  1

@@ -149,3 +149,55 @@ def test_nan_in_a_row_that_takes_part_stays_in_it(dtype, by_token):
     assert torch.equal(loss[~bad], loss0[~bad]) and torch.equal(lse[~bad], lse0[~bad])
     gx, gw = _backward(x, w, targets, lse, g, by_token)
     assert torch.equal(gx[~bad], gx0[~bad]) and bool(torch.isnan(gx[bad]).all()) and bool(torch.isnan(gw).all())
+
+
+def test_bf16_weight_gradient_over_many_rows_of_one_sign():
+    """262144 terms of one sign.  The tensor core's sums are cut off, up to 2^-23 of what they come to for each 16 terms and always downwards; a sum of at most 128 stages (512 instructions) stays within
+    2^-14 of itself, however many rows there are, and what follows is rounded either way, as are p and the results.  A result is off by up to 2^-8 of itself (evenly spread: 2^-8 / sqrt(3) at one sigma),
+    alike in the columns of a row, whose sums are nearly the same; over 1023 rows that leaves 2^-8 / sqrt(3 * 1023) < 2^-13.7 at one sigma.  Four of them, and 2^-14."""
+    N, E, V = 262144, 4864, 1024
+    gen = _gen(2)
+    x = torch.rand(N, E, generator=gen, device="cuda", dtype=BF16).add_(1.0)
+    w, targets, g = torch.zeros(V, E, dtype=BF16, device="cuda"), torch.zeros(N, dtype=torch.int32, device="cuda"), torch.ones(N, device="cuda")
+    w[:, 0] = (torch.randn(V, generator=gen, device="cuda") * 0.5).to(BF16)
+    p = torch.softmax(x[:, :1].double() * w[:, 0].double(), 1)
+    lse = -torch.log(p[:, 0] / torch.exp(x[:, 0].double() * w[0, 0].double())).float()
+    gw = _nan_like(w)
+    training.linear_cross_entropy_backward(x, w, targets, lse, g, None, gw, N, E, V)
+    want = torch.zeros(V, E, dtype=torch.float64, device="cuda")
+    for a in range(0, N, 16384):
+        want += p[a:a + 16384].t() @ x[a:a + 16384].double()
+    short = 1.0 - gw[1:].double() / want[1:]               # (row 0 is every row's target)
+    assert abs(float(short.mean())) < 2.0 ** -14 + 4 * 2.0 ** -13.7, float(short.mean())
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+def test_bf16_loss_of_wide_rows_of_one_sign(by_token):
+    """Logits of 65536 terms of one sign: cut off at most 64 times (16 stages) before they leave the tensor core's sums."""
+    N, E, V = 70, 65536, 300
+    gen = _gen(4)
+    x = (torch.rand(N, E, generator=gen, device="cuda") + 0.5).to(BF16)
+    w = ((torch.rand(V, E, generator=gen, device="cuda") + 0.5) * torch.linspace(0, 8, V, device="cuda")[:, None] / E).to(BF16)
+    targets = torch.randint(0, V, (N,), generator=gen, device="cuda", dtype=torch.int32)
+    loss, lse = _forward(x, w, targets, by_token)
+    z = x.double() @ w.double().t()
+    cut = float(z.max()) * (64 * 2.0 ** -23 + (E // 1024 + 2) * 2.0 ** -24)
+    want = torch.logsumexp(z, 1)
+    assert float((lse.double() - want).abs().max()) < cut + 2.0 ** -20
+    assert float((loss.double() - (want - z.gather(1, targets.long()[:, None])[:, 0])).abs().max()) < 2 * cut + 2.0 ** -20
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+def test_bf16_gradient_of_wide_rows(by_token):
+    """Logits over 257 stages: their sums are put by on the way, in the backward too."""
+    N, E, V = 70, 16400, 300
+    x, w, targets = _case(N, E, V, BF16, 11)
+    g = torch.rand(N, generator=_gen(12), device="cuda") - 0.3
+    ref = tu.Loss(x, w, targets, g, BF16)
+    loss, lse = _forward(x, w, targets, by_token)
+    tu.within(lse, ref.lse, ref.e_lse, "lse")
+    tu.within(loss, ref.loss, ref.e_loss, "loss")
+    gx, gw = _backward(x, w, targets, lse, g, by_token)
+    (dx, dw), (ex, ew) = ref.gradients(lse)
+    tu.within(gx, dx, ex, "grad_x")
+    tu.within(gw, dw, ew, "grad_w")
