@@ -627,10 +627,13 @@ struct Walk {
     int dz, dz_tiles, dz_m_tiles;
 };
 
-// Two parts of a row: (maximum, sum of exponentials relative to it)
+// What exponentials are taken relative to: the maximum, or the next finite number.  (So beside a logit of +infinity the others count for nothing and the sum is infinite, and infinity - infinity is met nowhere.)
+__device__ __forceinline__ float reference(float m) { return fminf(fmaxf(m, -FLT_MAX), FLT_MAX); }
+
+// Two parts of a row: (maximum, sum of exponentials relative to its reference)
 __device__ __forceinline__ float2 join_parts(float2 a, float2 b)
 {
-    const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.0f : m;
+    const float m = fmaxf(a.x, b.x), ref = reference(m);
     return make_float2(m, a.y * ex2_approx((a.x - ref) * kLog2e) + b.y * ex2_approx((b.x - ref) * kLog2e));
 }
 
@@ -890,7 +893,7 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                 float m = run_max;
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) m = max3(m, v[j] * z_scale, v[j + 1] * z_scale);
-                const float ref = m == -INFINITY ? 0.0f : m;
+                const float ref = reference(m);
                 float s0 = run_sum * ex2_approx((run_max - ref) * kLog2e), s1 = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {

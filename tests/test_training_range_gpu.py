@@ -135,6 +135,31 @@ def test_fp32_values_next_to_the_largest(by_token):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("by_token", [True, False])
+def test_logits_that_are_infinite(dtype, by_token):
+    """A logit that overflows to +infinity: log-sum-exp and loss are infinite (a target of +infinity itself: inf - inf).  To -infinity: it counts for nothing.  The other rows are as ever."""
+    N, E, V = 70, 64, 700
+    x, w, targets = _case(N, E, V, dtype, 8)
+    targets[:] = 1
+    w[650], w[651] = 0, 0
+    x[:, 0], w[:, 0] = 0, 0                                # column 0 meets only these
+    want = _forward(x, w, targets, by_token)
+    w[650, 0], w[651, 0] = 2.0, -2.0
+    x[3, 0], x[68, 0] = 2e38, -2e38                        # one logit of such a row is +infinity, one -infinity
+    loss, lse = _forward(x, w, targets, by_token)
+    hit = torch.zeros(N, dtype=torch.bool, device="cuda")
+    hit[[3, 68]] = True
+    assert bool((lse[hit] == INF).all()) and bool((loss[hit] == INF).all()), (lse[hit], loss[hit])
+    assert torch.equal(loss[~hit], want[0][~hit]) and torch.equal(lse[~hit], want[1][~hit]) if dtype == BF16 else float((loss[~hit] - want[0][~hit]).abs().max()) < 1e-5
+    targets[3] = 650
+    loss, lse = _forward(x, w, targets, by_token)
+    assert float(lse[3]) == INF and math.isnan(float(loss[3])) and float(loss[68]) == INF
+    targets[3], x[68, 0] = 651, 0                          # the target's logit is -infinity
+    loss, lse = _forward(x, w, targets, by_token)
+    assert float(lse[3]) == INF and float(loss[3]) == INF and math.isfinite(float(loss[68]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("by_token", [True, False])
 def test_nan_in_a_row_that_takes_part_stays_in_it(dtype, by_token):
     N, E, V = 300, 72, 900
     x, w, targets = _case(N, E, V, dtype, 9)
