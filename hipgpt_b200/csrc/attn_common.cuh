@@ -24,6 +24,8 @@ int check_launch(const char *what);
 // (barriers, TMEM, roles), while the last blocks of the kernel before it on the stream are still running, once those
 // have let their dependents go.  Such a kernel must execute dependency_wait() before its first access to global
 // memory; the wait returns when the kernel before it has completed and its writes are visible.
+// One exception: stores alone, of a kernel that reads nothing (zero_table_kernel in embedding.cu), may come before its wait if the kernel before it waits in every block before it
+// lets its dependents go: whatever touched that memory has then completed.  What a kernel reads may have been written by another; that it sees those writes is promised behind its own wait only.
 // HIPGPT_NO_OVERLAPPED_LAUNCH=1 launches the plain way.
 // `cluster` > 1: that many consecutive blocks form a cluster.
 template <typename... KArgs, typename... Args>

@@ -140,19 +140,199 @@ __device__ __forceinline__ void split_half(float x, __half &hi, __half &lo)
     lo = __float2half_rn(x - __half2float(hi));
 }
 
+// ---- what the backward's launches do -----------------------------------------------------------------------------------
+
+// How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
+// side by side read the same stages of it), as many whole rounds as leave every pair something over are dealt out tile by tile; the stages of the rest are cut into a length for
+// each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in quarter stages: a narrow
+// tile's stages count three (they fetch three quarters, and that is what bounds them).
+constexpr int kPackThreads = 256;            // of a block of the kernels before the products
+struct Place { int tile, k; };               // tile: kDx's, then kDw's
+constexpr int kMostPairs = 128;
+// A tile counts so many stages more: what becomes of its accumulator is not hidden by the products of a short one (24 stages of 24 + 8: 12 us)
+constexpr int kTileExtra = 8;
+struct Cut {
+    int m_tiles[2], n_tiles[2], stages[2], tiles[2], narrow[2], n_fast[2];
+    int dealt;                               // tiles that are dealt out whole
+    Place begin[kMostPairs + 1];             // each pair's length of the rest
+};
+
+// Tile u of problem i: its row and column of tiles, and what a stage of it counts
+struct TileOf { int m, n, unit; };
+__device__ __forceinline__ TileOf tile_of(const Cut &c, int i, int u)
+{
+    const int nt = c.n_tiles[i], mt = c.m_tiles[i];
+    const int m = c.n_fast[i] ? u / nt : u % mt, n = c.n_fast[i] ? u % nt : u / mt;
+    return {m, n, c.narrow[i] && n == nt - 1 ? 3 : 4};
+}
+// Quarter stages of kDx, of both
+struct Lengths { long long first, all; };
+__device__ __forceinline__ Lengths lengths_of(const Cut &c)
+{
+    long long total[2];
+    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * (c.stages[i] + kTileExtra) * max(0, 4 * c.n_tiles[i] - c.narrow[i]);
+    return {total[0], total[0] + total[1]};
+}
+// Quarter stages before tile t
+__device__ __forceinline__ long long place_before(const Cut &c, const Lengths &len, int t)
+{
+    const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
+    if (u >= c.tiles[i]) return len.all;
+    const TileOf x = tile_of(c, i, u);
+    const long long stages = c.stages[i] + kTileExtra;
+    const long long here = c.n_fast[i] ? stages * ((long long)x.m * (4 * c.n_tiles[i] - c.narrow[i]) + 4 * x.n) : stages * (4LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
+    return (i ? len.first : 0) + here;
+}
+__device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long long at)
+{
+    if (at >= len.all) return {c.tiles[0] + c.tiles[1], 0};
+    const int i = at >= len.first;
+    if (i) at -= len.first;
+    const long long stages = c.stages[i] + kTileExtra;
+    int u, unit;
+    if (c.n_fast[i]) {
+        const long long row = stages * (4 * c.n_tiles[i] - c.narrow[i]);
+        const long long m = at / row;
+        at -= m * row;
+        const int n = (int)min(at / (4 * stages), (long long)c.n_tiles[i] - 1);
+        at -= n * 4 * stages;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
+        u = (int)m * c.n_tiles[i] + n;
+    } else {
+        const long long column = 4 * stages * c.m_tiles[i];
+        const int n = (int)min(at / column, (long long)c.n_tiles[i] - 1);
+        at -= n * column;
+        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
+        const int m = (int)(at / (unit * stages));
+        at -= m * unit * stages;
+        u = n * c.m_tiles[i] + m;
+    }
+    const int k = (int)(at / unit), tile = (i ? c.tiles[0] : 0) + u;
+    return k < c.stages[i] ? Place{tile, k} : Place{tile + 1, 0};             // (a tile's last stages are what it costs otherwise)
+}
+__device__ __forceinline__ bool before(const Place &a, const Place &b) { return a.tile < b.tile || (a.tile == b.tile && a.k < b.k); }
+
+// What a call's launches are cut from
+struct PlanArgs {
+    int pieces, width, V, E, pairs, dz_stages, dz_extra;
+    int ev, with_x, with_w;
+    const int *targets;
+    const float *g;                          // bf16: where the largest finite |g| goes, of rows that take part; 1 if there is none
+    int N;
+    float *most;
+};
+
+// By a block of kPackThreads for each launch of the backward, among the first kernel's.  Tiles of kDz are dealt out one by one from pair 0 on.
+__device__ __forceinline__ void plan_launch(const PlanArgs &a, int launch, Cut *cuts)
+{
+    __shared__ Cut c;
+    __shared__ Lengths len;
+    __shared__ long long scan[kPackThreads / 32];
+    __shared__ int warp_count[kPackThreads / 32];
+    __shared__ float warp_most[kPackThreads / 32];
+    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, pairs = a.pairs;
+    int count = 0;
+    float most = 0.0f;
+    const bool find_most = a.most && launch == 0;
+#pragma unroll 8
+    for (int n = q; n < a.N; n += kPackThreads) {
+        const int t = __ldg(a.targets + n);
+        const bool inside = t >= 0 && t < a.V;
+        count += inside;
+        if (find_most && inside) {
+            const float g = fabsf(__ldg(a.g + n));
+            if (g <= 3.0e38f) most = fmaxf(most, g);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if (lane == 0) { warp_count[warp] = count; warp_most[warp] = most; }
+    __syncthreads();
+    count = 0;
+#pragma unroll
+    for (int w = 0; w < kPackThreads / 32; ++w) { count += warp_count[w]; most = fmaxf(most, warp_most[w]); }
+    if (find_most && q == 0) *a.most = most > 0.0f ? most : 1.0f;
+    const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep), e_tiles = (a.E + kTileN - 1) / kTileN;
+    auto columns = [&](int piece) { return piece < 0 || piece >= a.pieces ? 0 : (int)min((long long)a.width, a.V - (long long)piece * a.width); };
+    auto narrow = [](int n) { return n && (n - 1) % kTileN < kTileN / 2 ? 1 : 0; };
+    const int old = columns(launch - 1), v_tiles = (old + kTileN - 1) / kTileN;
+    if (q == 0) {
+        c.m_tiles[0] = count_tiles;
+        c.n_tiles[0] = a.with_x && old ? e_tiles : 0;
+        c.stages[0] = (old + kDeep - 1) / kDeep;
+        c.narrow[0] = narrow(a.E);
+        c.n_fast[0] = 1;
+        c.m_tiles[1] = a.ev ? e_tiles : v_tiles;
+        c.n_tiles[1] = a.with_w && old ? (a.ev ? v_tiles : e_tiles) : 0;
+        c.stages[1] = count_stages;
+        c.narrow[1] = narrow(a.ev ? old : a.E);
+        c.n_fast[1] = !a.ev;
+        for (int i = 0; i < 2; ++i) c.tiles[i] = c.m_tiles[i] * c.n_tiles[i];
+        len = lengths_of(c);
+    }
+    __syncthreads();
+    const int tiles = c.tiles[0] + c.tiles[1], dz_tiles = count_tiles * ((columns(launch) + kTileN - 1) / kTileN);
+    const long long dz_cost = 4 * a.dz_stages + a.dz_extra, both = len.all + dz_cost * dz_tiles;
+    for (int rounds = tiles / pairs;; --rounds) {
+        const int dealt = max(0, rounds) * pairs;
+        const long long rest = len.all - place_before(c, len, dealt);
+        long long load = 0;
+        if (q < pairs) {
+            for (int t = q; t < dealt; t += pairs) {
+                const int i = t >= c.tiles[0];
+                load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * (c.stages[i] + kTileExtra);
+            }
+            load += dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
+        }
+        long long incl = load;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) incl += scan[w];
+        // what is left for the pairs before this one when each has an equal part of everything; a length of at least eight stages each (four: 90 x 256 x 6163 fp32 58 us instead
+        // of 55, 300 x 256 x 5000 56 instead of 54, longer ones alike)
+        const long long begin = both * q / pairs - (incl - load), mine = both * (q + 1) / pairs - incl - begin;
+        const bool fits = __syncthreads_and(q >= pairs || mine >= 32) != 0;
+        if (!fits && rounds > 0) continue;
+        if (q == 0) c.dealt = dealt;
+        if (q <= pairs) {
+            long long at;
+            if (fits) {
+                at = (len.all - rest) + (q < pairs ? begin : rest);
+            } else {                         // too little for equal parts beside kDz's tiles: equal lengths of eight stages or more, for as many pairs as that gives
+                const int active = (int)max(1LL, min((long long)pairs, len.all / 32));
+                at = q >= active ? len.all : len.all * q / active;
+            }
+            c.begin[q] = place_of(c, len, at);
+        }
+        break;
+    }
+    __syncthreads();
+    for (int i = q; i < (int)(sizeof(Cut) / sizeof(int)); i += kPackThreads) reinterpret_cast<int *>(cuts + launch)[i] = reinterpret_cast<const int *>(&c)[i];
+}
+
 // ---- rows that take part, moved together ------------------------------------------------------------------------------
 
 constexpr int kAmaxBlocks = 4 * 148;
 
 // partial[1][block] = the largest finite |w| that the block has seen; row_max[n] = that of row n of x, of the rows that take part.  Backward: partial[0][block] = the largest exponent_of(|g_n|) +
 // exponent_of(row_max[n]) of the rows that have both, partial[2][block] = minus the smallest.
-__global__ void __launch_bounds__(256)
-loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial, float *row_max, int early)
+__global__ void __launch_bounds__(kPackThreads)
+loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ g, const int *__restrict__ targets, int N, int E, int V, float *partial, float *row_max, int blocks,
+                 PlanArgs plan, int launches, Cut *cuts)
 {
-    if (!early) dependency_wait();
+    dependency_wait();
     dependents_may_start();
+    if ((int)blockIdx.x < launches) { plan_launch(plan, blockIdx.x, cuts); return; }
     __shared__ float warp_max[2][8];
-    const int which = blockIdx.y, lane = threadIdx.x & 31;
+    const int which = ((int)blockIdx.x - launches) / blocks, block = ((int)blockIdx.x - launches) % blocks, lane = threadIdx.x & 31;
     float m = 0.0f, minus_least = -INFINITY;
     auto take = [&](float v) { v = fabsf(v); m = v <= FLT_MAX ? fmaxf(m, v) : m; };      // (not of infinities and NaN: they stay what they are)
     auto take4 = [&](const float4 &v) { take(v.x); take(v.y); take(v.z); take(v.w); };
@@ -161,7 +341,7 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
         for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
         return v;
     };
-    const long long step = (long long)gridDim.x * 256, at = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long step = (long long)blocks * 256, at = (long long)block * 256 + threadIdx.x;
     if (which == 1) {
         const long long total = (long long)V * E, words = (reinterpret_cast<uintptr_t>(w) & 15) == 0 ? total / 4 : 0;
         const float4 *w4 = reinterpret_cast<const float4 *>(w);
@@ -215,9 +395,8 @@ loss_amax_kernel(const float *__restrict__ x, const float *__restrict__ w, const
         m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, warp_max[threadIdx.x][i]);
-        partial[(which + 2 * threadIdx.x) * kAmaxBlocks + blockIdx.x] = m;
+        partial[(which + 2 * threadIdx.x) * kAmaxBlocks + block] = m;
     }
-    if (early) dependency_wait();
 }
 
 // The largest of each of loss_amax_kernel's rows (backward: all three, forward: the second); every thread of 256 gets them
@@ -293,16 +472,19 @@ struct Pack {
     uint16_t *wp;
     size_t w_plane;
     int w_rows, w_cols, w_ld, w_col_pieces, w_vec;
-    int early, targets_vec;
+    int targets_vec;
 };
 constexpr int kPackCols = 1024;
 
 template <typename T>
-__global__ void __launch_bounds__(256)
-loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
+__global__ void __launch_bounds__(kPackThreads)
+loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p, PlanArgs plan, int launches, Cut *cuts)
 {
-    if (!p.early) dependency_wait();
+    dependency_wait();
     dependents_may_start();
+    if constexpr (sizeof(T) == 2)            // (fp32: among loss_amax_kernel's blocks)
+        if ((int)blockIdx.x < launches) { plan_launch(plan, blockIdx.x, cuts); return; }
+    const int block = sizeof(T) == 2 ? (int)blockIdx.x - launches : (int)blockIdx.x;
     __shared__ int warp_sum[8];
     __shared__ float warp_max[3][8];
     int w_exp = 14, most = 27;                // (scales of 1)
@@ -315,24 +497,23 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
         deep = largest[0] + largest[2] > (float)kMostShift;
     }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if ((int)blockIdx.x >= p.x_blocks) {     // eight pieces of rows of the weights a block
+    if (block >= p.x_blocks) {               // eight pieces of rows of the weights a block
         const float scale = pow2(14 - w_exp);
-        const long long job = (long long)(blockIdx.x - p.x_blocks) * 8 + warp;
+        const long long job = (long long)(block - p.x_blocks) * 8 + warp;
         const int r = (int)(job / p.w_col_pieces), c = (int)(job % p.w_col_pieces) * kPackCols;
         if (r < p.w_rows) pack_row<T>(w + (size_t)r * p.w_cols, p.wp + (size_t)r * p.w_ld, p.w_plane, c, min(p.w_ld, c + kPackCols), p.w_cols, scale, lane, p.w_vec != 0);
-        if (p.early) dependency_wait();
         return;
     }
-    if (sizeof(T) == 4 && blockIdx.x == 0 && tid == 0) {
+    if (sizeof(T) == 4 && block == 0 && tid == 0) {
         p.scales[0] = pow2(w_exp - 14);
         const int e = most - 27;              // (one power of two could pass the range of fp32)
         p.scales[1] = pow2(e / 2);
         p.scales[2] = pow2(e - e / 2);
         p.scales[3] = deep ? 1.0f : 0.0f;
     }
-    if (blockIdx.x == 0 && tid == 0) *p.failed = 0;
-    for (int i = blockIdx.x * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
-    const int from = blockIdx.x * p.per_block, to = min(p.N, from + p.per_block);
+    if (block == 0 && tid == 0) *p.failed = 0;
+    for (int i = block * 256 + tid; i < p.zeros; i += p.x_blocks * 256) p.zero_ints[i] = 0;
+    const int from = block * p.per_block, to = min(p.N, from + p.per_block);
     auto inside = [&](int t) { return t >= 0 && t < p.V; };
     int before = 0, done = 0;
     if (p.targets_vec) {
@@ -403,7 +584,6 @@ loss_pack_kernel(const T *__restrict__ x, const T *__restrict__ w, Pack p)
             for (int c = lane * 4; c < p.ld; c += 128)
                 for (int pl = 0; pl < (sizeof(T) == 4 ? 2 : 1); ++pl) *reinterpret_cast<uint2 *>(rows + pl * p.plane + (size_t)i * p.ld + c) = make_uint2(0u, 0u);
     }
-    if (p.early) dependency_wait();
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------------
@@ -434,186 +614,6 @@ __device__ __noinline__ bool loss_wait_slow(uint64_t *bar, uint32_t parity, int 
     atomicExch(failed, 1);
     linger();
     return false;
-}
-
-// How the tiles of kDx and kDw fall to the pairs.  In a row (kDx's first; the tiles that share rows or columns of dz next to one another, so that pairs that run
-// side by side read the same stages of it), as many whole rounds as leave every pair something over are dealt out tile by tile; the stages of the rest are cut into a length for
-// each pair such that all pairs have the same to do, the whole tiles of kDz counted in.  Places are in quarter stages: a narrow
-// tile's stages count three (they fetch three quarters, and that is what bounds them).
-struct Place { int tile, k; };               // tile: kDx's, then kDw's
-constexpr int kMostPairs = 128;
-// A tile counts so many stages more: what becomes of its accumulator is not hidden by the products of a short one (24 stages of 24 + 8: 12 us)
-constexpr int kTileExtra = 8;
-struct Cut {
-    int m_tiles[2], n_tiles[2], stages[2], tiles[2], narrow[2], n_fast[2];
-    int dealt;                               // tiles that are dealt out whole
-    Place begin[kMostPairs + 1];             // each pair's length of the rest
-};
-
-// Tile u of problem i: its row and column of tiles, and what a stage of it counts
-struct TileOf { int m, n, unit; };
-__device__ __forceinline__ TileOf tile_of(const Cut &c, int i, int u)
-{
-    const int nt = c.n_tiles[i], mt = c.m_tiles[i];
-    const int m = c.n_fast[i] ? u / nt : u % mt, n = c.n_fast[i] ? u % nt : u / mt;
-    return {m, n, c.narrow[i] && n == nt - 1 ? 3 : 4};
-}
-// Quarter stages of kDx, of both
-struct Lengths { long long first, all; };
-__device__ __forceinline__ Lengths lengths_of(const Cut &c)
-{
-    long long total[2];
-    for (int i = 0; i < 2; ++i) total[i] = (long long)c.m_tiles[i] * (c.stages[i] + kTileExtra) * max(0, 4 * c.n_tiles[i] - c.narrow[i]);
-    return {total[0], total[0] + total[1]};
-}
-// Quarter stages before tile t
-__device__ __forceinline__ long long place_before(const Cut &c, const Lengths &len, int t)
-{
-    const int i = t >= c.tiles[0], u = t - (i ? c.tiles[0] : 0);
-    if (u >= c.tiles[i]) return len.all;
-    const TileOf x = tile_of(c, i, u);
-    const long long stages = c.stages[i] + kTileExtra;
-    const long long here = c.n_fast[i] ? stages * ((long long)x.m * (4 * c.n_tiles[i] - c.narrow[i]) + 4 * x.n) : stages * (4LL * x.n * c.m_tiles[i] + (long long)x.m * x.unit);
-    return (i ? len.first : 0) + here;
-}
-__device__ __forceinline__ Place place_of(const Cut &c, const Lengths &len, long long at)
-{
-    if (at >= len.all) return {c.tiles[0] + c.tiles[1], 0};
-    const int i = at >= len.first;
-    if (i) at -= len.first;
-    const long long stages = c.stages[i] + kTileExtra;
-    int u, unit;
-    if (c.n_fast[i]) {
-        const long long row = stages * (4 * c.n_tiles[i] - c.narrow[i]);
-        const long long m = at / row;
-        at -= m * row;
-        const int n = (int)min(at / (4 * stages), (long long)c.n_tiles[i] - 1);
-        at -= n * 4 * stages;
-        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
-        u = (int)m * c.n_tiles[i] + n;
-    } else {
-        const long long column = 4 * stages * c.m_tiles[i];
-        const int n = (int)min(at / column, (long long)c.n_tiles[i] - 1);
-        at -= n * column;
-        unit = c.narrow[i] && n == c.n_tiles[i] - 1 ? 3 : 4;
-        const int m = (int)(at / (unit * stages));
-        at -= m * unit * stages;
-        u = n * c.m_tiles[i] + m;
-    }
-    const int k = (int)(at / unit), tile = (i ? c.tiles[0] : 0) + u;
-    return k < c.stages[i] ? Place{tile, k} : Place{tile + 1, 0};             // (a tile's last stages are what it costs otherwise)
-}
-__device__ __forceinline__ bool before(const Place &a, const Place &b) { return a.tile < b.tile || (a.tile == b.tile && a.k < b.k); }
-
-// What a call's launches are cut from
-struct PlanArgs {
-    int pieces, width, V, E, pairs, dz_stages, dz_extra;
-    int ev, with_x, with_w;
-    const int *targets;
-    const float *g;                          // bf16: where the largest finite |g| goes, of rows that take part; 1 if there is none
-    int N;
-    float *most;
-};
-constexpr int kPlanThreads = 512;
-
-// A block for each launch of the backward.  Tiles of kDz are dealt out one by one from pair 0 on.  It counts the rows that take part by itself, and what is launched
-// behind it runs beside it: that starts once this kernel has seen the work before it complete, and waits for this one at its own end (`early`).
-__global__ void __launch_bounds__(kPlanThreads)
-loss_plan_kernel(PlanArgs a, Cut *cuts)
-{
-    dependency_wait();
-    dependents_may_start();
-    __shared__ Cut c;
-    __shared__ Lengths len;
-    __shared__ long long scan[kPlanThreads / 32];
-    __shared__ int warp_count[kPlanThreads / 32];
-    __shared__ float warp_most[kPlanThreads / 32];
-    const int q = threadIdx.x, lane = q & 31, warp = q >> 5, launch = blockIdx.x, pairs = a.pairs;
-    int count = 0;
-    float most = 0.0f;
-    const bool find_most = a.most && launch == 0;
-#pragma unroll 8
-    for (int n = q; n < a.N; n += kPlanThreads) {
-        const int t = __ldg(a.targets + n);
-        const bool inside = t >= 0 && t < a.V;
-        count += inside;
-        if (find_most && inside) {
-            const float g = fabsf(__ldg(a.g + n));
-            if (g <= 3.0e38f) most = fmaxf(most, g);
-        }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        count += __shfl_xor_sync(0xffffffffu, count, o);
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    }
-    if (lane == 0) { warp_count[warp] = count; warp_most[warp] = most; }
-    __syncthreads();
-    count = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanThreads / 32; ++w) { count += warp_count[w]; most = fmaxf(most, warp_most[w]); }
-    if (find_most && q == 0) *a.most = most > 0.0f ? most : 1.0f;
-    const int count_tiles = max(1, (count + kTileM - 1) / kTileM), count_stages = max(1, (count + kDeep - 1) / kDeep), e_tiles = (a.E + kTileN - 1) / kTileN;
-    auto columns = [&](int piece) { return piece < 0 || piece >= a.pieces ? 0 : (int)min((long long)a.width, a.V - (long long)piece * a.width); };
-    auto narrow = [](int n) { return n && (n - 1) % kTileN < kTileN / 2 ? 1 : 0; };
-    const int old = columns(launch - 1), v_tiles = (old + kTileN - 1) / kTileN;
-    if (q == 0) {
-        c.m_tiles[0] = count_tiles;
-        c.n_tiles[0] = a.with_x && old ? e_tiles : 0;
-        c.stages[0] = (old + kDeep - 1) / kDeep;
-        c.narrow[0] = narrow(a.E);
-        c.n_fast[0] = 1;
-        c.m_tiles[1] = a.ev ? e_tiles : v_tiles;
-        c.n_tiles[1] = a.with_w && old ? (a.ev ? v_tiles : e_tiles) : 0;
-        c.stages[1] = count_stages;
-        c.narrow[1] = narrow(a.ev ? old : a.E);
-        c.n_fast[1] = !a.ev;
-        for (int i = 0; i < 2; ++i) c.tiles[i] = c.m_tiles[i] * c.n_tiles[i];
-        len = lengths_of(c);
-    }
-    __syncthreads();
-    const int tiles = c.tiles[0] + c.tiles[1], dz_tiles = count_tiles * ((columns(launch) + kTileN - 1) / kTileN);
-    const long long dz_cost = 4 * a.dz_stages + a.dz_extra, both = len.all + dz_cost * dz_tiles;
-    for (int rounds = tiles / pairs;; --rounds) {
-        const int dealt = max(0, rounds) * pairs;
-        const long long rest = len.all - place_before(c, len, dealt);
-        long long load = 0;
-        if (q < pairs) {
-            for (int t = q; t < dealt; t += pairs) {
-                const int i = t >= c.tiles[0];
-                load += (long long)tile_of(c, i, t - (i ? c.tiles[0] : 0)).unit * (c.stages[i] + kTileExtra);
-            }
-            load += dz_cost * (dz_tiles / pairs + (q < dz_tiles % pairs));
-        }
-        long long incl = load;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        if (lane == 31) scan[warp] = incl;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) incl += scan[w];
-        // what is left for the pairs before this one when each has an equal part of everything; a length of at least eight stages each (four: 90 x 256 x 6163 fp32 58 us instead
-        // of 55, 300 x 256 x 5000 56 instead of 54, longer ones alike)
-        const long long begin = both * q / pairs - (incl - load), mine = both * (q + 1) / pairs - incl - begin;
-        const bool fits = __syncthreads_and(q >= pairs || mine >= 32) != 0;
-        if (!fits && rounds > 0) continue;
-        if (q == 0) c.dealt = dealt;
-        if (q <= pairs) {
-            long long at;
-            if (fits) {
-                at = (len.all - rest) + (q < pairs ? begin : rest);
-            } else {                         // too little for equal parts beside kDz's tiles: equal lengths of eight stages or more, for as many pairs as that gives
-                const int active = (int)max(1LL, min((long long)pairs, len.all / 32));
-                at = q >= active ? len.all : len.all * q / active;
-            }
-            c.begin[q] = place_of(c, len, at);
-        }
-        break;
-    }
-    __syncthreads();
-    for (int i = q; i < (int)(sizeof(Cut) / sizeof(int)); i += kPlanThreads) reinterpret_cast<int *>(cuts + launch)[i] = reinterpret_cast<const int *>(&c)[i];
 }
 
 // What a pair does, one after the other: its tiles of kDx and kDw, its length of the rest of them, its tiles of kDz
@@ -1286,7 +1286,7 @@ int plan_call(Plan &p, const void *w, int N, int E, int V, int layout, bool with
 // Fills what the plan has in the workspace, and of `a` what every form reads
 template <typename T>
 int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, const int *targets, const float *lse, const float *g, float *zero_loss, float *zero_lse, void *zero_grad,
-              int *zero_ints, int zeros, bool early, cudaStream_t st, const void **w_base)
+              int *zero_ints, int zeros, const PlanArgs &plan, int launches, Cut *cuts, cudaStream_t st, const void **w_base)
 {
     int *ints = reinterpret_cast<int *>(ws + p.ints_at);
     float *floats = reinterpret_cast<float *>(ws + p.floats_at), *scales = reinterpret_cast<float *>(ws + p.amax_at), *partial = scales + 4, *row_max = floats + 4 * p.rows_alloc;
@@ -1294,7 +1294,9 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     cudaError_t e;
     if constexpr (sizeof(T) == 4) {
         k.amax_blocks = (int)std::min<long long>(kAmaxBlocks, std::max<long long>(((long long)p.V * p.E + 4095) / 4096, ((long long)p.N + 7) / 8));
-        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)k.amax_blocks, 2), dim3(256), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, partial, row_max, (int)early);
+        e = launch_overlapped(loss_amax_kernel, dim3((unsigned)(launches + 2 * k.amax_blocks)), dim3(kPackThreads), 0, st, (const float *)x, (const float *)w, g, targets, p.N, p.E, p.V, partial, row_max,
+                              k.amax_blocks, plan, launches, cuts);
+        launches = 0;
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_amax_kernel: %s", cudaGetErrorString(e));
     }
     k.partial = partial;
@@ -1302,7 +1304,6 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
     k.scales = scales;
     k.targets = targets; k.lse = lse; k.g = g;
     k.N = p.N; k.E = p.E; k.V = p.V; k.ld = (int)p.x_ld;
-    k.early = early && sizeof(T) == 2;                     // (fp32: loss_amax_kernel is)
     k.targets_vec = (reinterpret_cast<uintptr_t>(targets) & 15) == 0;
     k.per_block = (int)(p.N <= 2048 ? 8 : p.N <= 16384 ? 32 : round_up((p.N + 511) / 512, 32));      // (a block counts the targets before its rows; of 8192, 8 and 32 are alike)
     k.x_blocks = (p.N + k.per_block - 1) / k.per_block;
@@ -1324,8 +1325,8 @@ int pack_call(const Plan &p, uint8_t *ws, LossArgs &a, const T *x, const T *w, c
         w_blocks = (p.w_rows * k.w_col_pieces + 7) / 8;
     }
     *w_base = p.pack_w ? static_cast<const void *>(ws + p.w_at) : w;
-    if (k.x_blocks + w_blocks > 2147483647LL) return fail(HIPGPT_ERR_UNSUPPORTED, "weights of %lld rows of %lld values are beyond one call", p.w_rows, p.w_cols);
-    e = launch_overlapped(loss_pack_kernel<T>, dim3((unsigned)(k.x_blocks + w_blocks)), dim3(256), 0, st, x, w, k);
+    if (launches + k.x_blocks + w_blocks > 2147483647LL) return fail(HIPGPT_ERR_UNSUPPORTED, "weights of %lld rows of %lld values are beyond one call", p.w_rows, p.w_cols);
+    e = launch_overlapped(loss_pack_kernel<T>, dim3((unsigned)(launches + k.x_blocks + w_blocks)), dim3(kPackThreads), 0, st, x, w, k, plan, launches, cuts);
     if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_pack_kernel: %s", cudaGetErrorString(e));
     a.count = k.count; a.failed = k.failed; a.row_map = k.row_map; a.targets = k.c_targets;
     a.lse = k.c_lse; a.g = k.c_g; a.x_inv = k.c_x_inv; a.row_unit = k.c_unit; a.scales = scales;
@@ -1365,7 +1366,7 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     const bool ev = layout == HIPGPT_WEIGHTS_EV;
     int pairs = 1;
     rc = loss_pairs(p.dev, (long long)m_tiles * n_tiles, &pairs);
-    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, false, st, &wb);
+    if (rc == HIPGPT_OK) rc = pack_call<T>(p, ws, a, x, w, targets, nullptr, nullptr, loss, lse, nullptr, nullptr, 0, PlanArgs(), 0, nullptr, st, &wb);
     if (rc == HIPGPT_OK) rc = x_map<T>(&a.a[kDz], p, ws, kHalfM);
     if (rc == HIPGPT_OK) rc = w_map<T>(&a.b[kDz], p, wb);
     if (rc != HIPGPT_OK) return rc;
@@ -1419,9 +1420,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     Cut *cuts = reinterpret_cast<Cut *>(ws + cuts_at);
     const PlanArgs plan = {pieces, (int)width, V, E, pairs, (E + kDeep - 1) / kDeep, kDzExtra<NP>, ev, grad_x != nullptr, grad_w != nullptr, targets, grad_loss, N,
                            NP == 1 ? reinterpret_cast<float *>(ws + p.amax_at) + 2 : nullptr};
-    const cudaError_t e = launch_overlapped(loss_plan_kernel, dim3((unsigned)(pieces + 1)), dim3(kPlanThreads), 0, st, plan, cuts);
-    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "loss_plan_kernel: %s", cudaGetErrorString(e));
-    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, true, st, &wb);
+    rc = pack_call<T>(p, ws, a, x, w, targets, lse, grad_loss, nullptr, nullptr, grad_x, a.arrived, arrived, plan, pieces + 1, cuts, st, &wb);
     if (rc != HIPGPT_OK) return rc;
     a.shares = reinterpret_cast<float4 *>(ws + shares_at);
     a.sum = reinterpret_cast<float4 *>(ws + sum_at);
