@@ -123,18 +123,20 @@ PyObject *decode(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 // ---- training.py ------------------------------------------------------------------------------------------------------
 
-// The tensors of one call of training.py: contiguous, on the current device, of at least `count` values; None gives NULL.  The first failure stands.
+// The tensors of one call of training.py: contiguous, on the current device, of at least `count` values; None gives NULL.  Tables and weights of two or more dimensions: of rows of `row` values
+// (weights by token given as [E][V], or the other way round, are no others than these to the count).  The first failure stands.
 struct Tensors {
     PyObject *const *a;
     bool ok = true;
 
-    void *at(int i, const char *name, at::ScalarType type, int64_t count)
+    void *at(int i, const char *name, at::ScalarType type, int64_t count, int64_t row = -1)
     {
         if (!ok || a[i] == Py_None) return nullptr;
         ok = false;
         if (!THPVariable_Check(a[i])) { PyErr_Format(PyExc_ValueError, "%s: expected a contiguous CUDA %s tensor", name, c10::toString(type)); return nullptr; }
         const at::Tensor &t = THPVariable_Unpack(a[i]);
-        if (!(t.is_cuda() && t.scalar_type() == type && t.is_contiguous())) PyErr_Format(PyExc_ValueError, "%s: expected a contiguous CUDA %s tensor", name, c10::toString(type));
+        if (row >= 0 && t.dim() >= 2 && t.size(-1) != row) PyErr_Format(PyExc_ValueError, "%s has rows of %lld values, %lld are expected", name, (long long)t.size(-1), (long long)row);
+        else if (!(t.is_cuda() && t.scalar_type() == type && t.is_contiguous())) PyErr_Format(PyExc_ValueError, "%s: expected a contiguous CUDA %s tensor", name, c10::toString(type));
         else if (t.get_device() != c10::cuda::current_device()) PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, another is the current device", name, (int)t.get_device());
         else if (t.numel() < count) PyErr_Format(PyExc_ValueError, "%s holds %lld values, %lld are needed", name, (long long)t.numel(), (long long)count);
         else { ok = true; return t.data_ptr(); }
@@ -165,7 +167,7 @@ PyObject *embedding_scaled(PyObject *, PyObject *const *a, Py_ssize_t n)
     const int64_t B = i[0], S = i[1], V = i[2], E = i[3];
     Tensors t{a};
     const at::ScalarType k = t.kind(3, "out", &type);
-    const void *ids = t.at(0, "ids", at::kInt, B * S), *tok = t.at(1, "tok", k, V * E), *pos = t.at(2, "pos", k, S * E);
+    const void *tok = t.at(1, "tok", k, V * E, E), *pos = t.at(2, "pos", k, S * E, E), *ids = t.at(0, "ids", at::kInt, B * S);
     void *out = t.at(3, "out", k, B * S * E);
     if (!t.ok) return nullptr;
     return status_of([&](void *st) { return hipgpt_embedding_scaled(static_cast<const int *>(ids), tok, pos, out, (float)scale, i[0], i[1], i[2], i[3], type, st); });
@@ -183,8 +185,8 @@ PyObject *embedding_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
     const int64_t B = i[1], S = i[2], V = i[3], E = i[4];
     Tensors t{a};
     const at::ScalarType k = t.kind(0, "grad_out", &type), gk = t.kind(a[2] == Py_None ? 3 : 2, "grad_tok", &grad_type);
+    void *tok = t.at(2, "grad_tok", gk, V * E, E), *pos = t.at(3, "grad_pos", gk, S * E, E);
     const void *g = t.at(0, "grad_out", k, B * S * E), *ids = t.at(1, "ids", at::kInt, B * S);
-    void *tok = t.at(2, "grad_tok", gk, V * E), *pos = t.at(3, "grad_pos", gk, S * E);
     if (!t.ok) return nullptr;
     return status_of([&](void *st) { return hipgpt_embedding_backward(g, static_cast<const int *>(ids), tok, pos, (float)scale, i[0], i[1], i[2], i[3], i[4], type, grad_type, st); });
     END_HANDLE_TH_ERRORS
@@ -216,10 +218,10 @@ PyObject *linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
     HANDLE_TH_ERRORS
     int i[4], type = 0;
     if (!count(n, 9) || !ints(a + 5, 4, i)) return nullptr;
-    const int64_t N = i[0], E = i[1], V = i[2];
+    const int64_t N = i[0], E = i[1], V = i[2], row = i[3] == HIPGPT_WEIGHTS_EV ? V : E;
     Tensors t{a};
     const at::ScalarType k = t.kind(0, "x", &type);
-    const void *x = t.at(0, "x", k, N * E), *w = t.at(1, "w", k, V * E), *targets = t.at(2, "targets", at::kInt, N);
+    const void *w = t.at(1, "w", k, V * E, row), *x = t.at(0, "x", k, N * E), *targets = t.at(2, "targets", at::kInt, N);
     void *loss = t.at(3, "loss", at::kFloat, N), *lse = t.at(4, "lse", at::kFloat, N);
     if (!t.ok) return nullptr;
     return status_of([&](void *st) {
@@ -234,11 +236,11 @@ PyObject *linear_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize
     HANDLE_TH_ERRORS
     int i[5], type = 0;
     if (!count(n, 12) || !ints(a + 7, 5, i)) return nullptr;
-    const int64_t N = i[1], E = i[2], V = i[3];
+    const int64_t N = i[1], E = i[2], V = i[3], row = i[4] == HIPGPT_WEIGHTS_EV ? V : E;
     Tensors t{a};
     const at::ScalarType k = t.kind(0, "x", &type);
-    const void *x = t.at(0, "x", k, N * E), *w = t.at(1, "w", k, V * E), *targets = t.at(2, "targets", at::kInt, N), *lse = t.at(3, "lse", at::kFloat, N), *g = t.at(4, "grad_loss", at::kFloat, N);
-    void *gx = t.at(5, "grad_x", k, N * E), *gw = t.at(6, "grad_w", k, V * E);
+    const void *w = t.at(1, "w", k, V * E, row), *x = t.at(0, "x", k, N * E), *targets = t.at(2, "targets", at::kInt, N), *lse = t.at(3, "lse", at::kFloat, N), *g = t.at(4, "grad_loss", at::kFloat, N);
+    void *gx = t.at(5, "grad_x", k, N * E), *gw = t.at(6, "grad_w", k, V * E, row);
     if (!t.ok) return nullptr;
     return status_of([&](void *st) {
         return hipgpt_linear_cross_entropy_backward(x, w, static_cast<const int *>(targets), static_cast<const float *>(lse), static_cast<const float *>(g), gx, gw, i[0], i[1], i[2], i[3], i[4], type, st);

@@ -42,10 +42,12 @@ def _storage(t):
         raise ValueError(f"expected float32 or bfloat16, not {t.dtype}") from None
 
 
-def _ptr_of(name, t, dtype, count):
-    """The address of a tensor of at least `count` values on the current device, None for None."""
+def _ptr_of(name, t, dtype, count, row=None):
+    """The address of a tensor of at least `count` values on the current device, None for None; row: of two or more dimensions, the last of so many."""
     if t is None:
         return None
+    if row is not None and t.dim() >= 2 and t.shape[-1] != row:
+        raise ValueError(f"{name} has rows of {t.shape[-1]} values, {row} are expected")
     if not (t.is_cuda and t.is_contiguous() and t.dtype == dtype):
         raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor")
     if t.device.index != torch.cuda.current_device():
@@ -106,15 +108,16 @@ class _ThroughCtypes:
     @staticmethod
     def embedding_scaled(ids, tok, pos, out, scale, B, S, V, E):
         n, dt = B * S, out.dtype
-        return _capi.lib().hipgpt_embedding_scaled(_ptr_of("ids", ids, torch.int32, n), _ptr_of("tok", tok, dt, V * E), _ptr_of("pos", pos, dt, S * E), _ptr_of("out", out, dt, n * E),
-                                                   scale, B, S, V, E, _storage(out), _stream())
+        tables = _ptr_of("tok", tok, dt, V * E, E), _ptr_of("pos", pos, dt, S * E, E)
+        return _capi.lib().hipgpt_embedding_scaled(_ptr_of("ids", ids, torch.int32, n), *tables, _ptr_of("out", out, dt, n * E), scale, B, S, V, E, _storage(out), _stream())
 
     @staticmethod
     def embedding_backward(grad_out, ids, grad_tok, grad_pos, scale, accumulate, B, S, V, E):
         n, table = B * S, grad_tok if grad_tok is not None else grad_pos
         gt = table.dtype
-        return _capi.lib().hipgpt_embedding_backward(_ptr_of("grad_out", grad_out, grad_out.dtype, n * E), _ptr_of("ids", ids, torch.int32, n), _ptr_of("grad_tok", grad_tok, gt, V * E),
-                                                     _ptr_of("grad_pos", grad_pos, gt, S * E), scale, accumulate, B, S, V, E, _storage(grad_out), _storage(table), _stream())
+        tables = _ptr_of("grad_tok", grad_tok, gt, V * E, E), _ptr_of("grad_pos", grad_pos, gt, S * E, E)
+        return _capi.lib().hipgpt_embedding_backward(_ptr_of("grad_out", grad_out, grad_out.dtype, n * E), _ptr_of("ids", ids, torch.int32, n), *tables, scale, accumulate, B, S, V, E,
+                                                     _storage(grad_out), _storage(table), _stream())
 
     @staticmethod
     def dropout_counter(x, residual, out, counter, p, seed, offset):
@@ -124,16 +127,18 @@ class _ThroughCtypes:
 
     @staticmethod
     def linear_cross_entropy(x, w, targets, loss, lse, N, E, V, layout):
-        dt, f = x.dtype, _FLOAT32
-        return _capi.lib().hipgpt_linear_cross_entropy(_ptr_of("x", x, dt, N * E), _ptr_of("w", w, dt, V * E), _ptr_of("targets", targets, torch.int32, N), _ptr_of("loss", loss, f, N),
+        dt, f, row = x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
+        weights = _ptr_of("w", w, dt, V * E, row)
+        return _capi.lib().hipgpt_linear_cross_entropy(_ptr_of("x", x, dt, N * E), weights, _ptr_of("targets", targets, torch.int32, N), _ptr_of("loss", loss, f, N),
                                                        _ptr_of("lse", lse, f, N), N, E, V, layout, _storage(x), _stream())
 
     @staticmethod
     def linear_cross_entropy_backward(x, w, targets, lse, grad_loss, grad_x, grad_w, accumulate, N, E, V, layout):
-        dt, f = x.dtype, _FLOAT32
+        dt, f, row = x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
+        weights = _ptr_of("w", w, dt, V * E, row)
         return _capi.lib().hipgpt_linear_cross_entropy_backward(
-            _ptr_of("x", x, dt, N * E), _ptr_of("w", w, dt, V * E), _ptr_of("targets", targets, torch.int32, N), _ptr_of("lse", lse, f, N), _ptr_of("grad_loss", grad_loss, f, N),
-            _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E), accumulate, N, E, V, layout, _storage(x), _stream())
+            _ptr_of("x", x, dt, N * E), weights, _ptr_of("targets", targets, torch.int32, N), _ptr_of("lse", lse, f, N), _ptr_of("grad_loss", grad_loss, f, N),
+            _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E, row), accumulate, N, E, V, layout, _storage(x), _stream())
 
 
 class _AtFirstCall:

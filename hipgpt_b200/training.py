@@ -3,7 +3,8 @@ counter, the loss and its gradient (the C entry points of the same names in incl
 
 Like launchers.py: outputs are given by the caller, calls are asynchronous on torch's current stream, torch holds the memory and
 nothing else.  Activations and weights are contiguous float32 or bfloat16 tensors, one type per call; ids and targets int32.  All
-tensors are on the current device.  Sizes beyond what a tensor holds are refused.
+tensors are on the current device.  Sizes beyond what a tensor holds are refused, and tables and weights of two dimensions whose
+rows have another length than the sizes say.
 """
 from __future__ import annotations
 
