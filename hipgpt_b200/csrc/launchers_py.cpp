@@ -123,6 +123,25 @@ PyObject *decode(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 // ---- training.py ------------------------------------------------------------------------------------------------------
 
+// Like ints, but what an int does not hold is refused (its low bits alone could pass for a size that the tensors have)
+bool sizes(PyObject *const *args, int n, int *out)
+{
+    for (int i = 0; i < n; ++i) {
+        PyObject *x = PyLong_Check(args[i]) ? Py_NewRef(args[i]) : PyObject_CallOneArg(g_any_int, args[i]);
+        if (!x) return false;
+        int over = 0;
+        const long v = PyLong_AsLongAndOverflow(x, &over);
+        Py_DECREF(x);
+        if (v == -1 && PyErr_Occurred()) return false;
+        out[i] = static_cast<int>(v);
+        if (over || out[i] != v) {
+            PyErr_Format(PyExc_ValueError, "%R is beyond one call", args[i]);
+            return false;
+        }
+    }
+    return true;
+}
+
 // The tensors of one call of training.py: contiguous, on the current device, of at least `count` values; None gives NULL.  Tables and weights of two or more dimensions: of rows of `row` values
 // (weights by token given as [E][V], or the other way round, are no others than these to the count).  The first failure stands.
 struct Tensors {
@@ -161,7 +180,7 @@ PyObject *embedding_scaled(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     int i[4], type = 0;
-    if (!count(n, 9) || !ints(a + 5, 4, i)) return nullptr;
+    if (!count(n, 9) || !sizes(a + 5, 4, i)) return nullptr;
     const double scale = PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) return nullptr;
     const int64_t B = i[0], S = i[1], V = i[2], E = i[3];
@@ -179,7 +198,7 @@ PyObject *embedding_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     int i[5], type = 0, grad_type = 0;
-    if (!count(n, 10) || !ints(a + 5, 5, i)) return nullptr;
+    if (!count(n, 10) || !sizes(a + 5, 5, i)) return nullptr;
     const double scale = PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) return nullptr;
     const int64_t B = i[1], S = i[2], V = i[3], E = i[4];
@@ -217,7 +236,7 @@ PyObject *linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     int i[4], type = 0;
-    if (!count(n, 9) || !ints(a + 5, 4, i)) return nullptr;
+    if (!count(n, 9) || !sizes(a + 5, 4, i)) return nullptr;
     const int64_t N = i[0], E = i[1], V = i[2], row = i[3] == HIPGPT_WEIGHTS_EV ? V : E;
     Tensors t{a};
     const at::ScalarType k = t.kind(0, "x", &type);
@@ -235,7 +254,7 @@ PyObject *linear_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize
 {
     HANDLE_TH_ERRORS
     int i[5], type = 0;
-    if (!count(n, 12) || !ints(a + 7, 5, i)) return nullptr;
+    if (!count(n, 12) || !sizes(a + 7, 5, i)) return nullptr;
     const int64_t N = i[1], E = i[2], V = i[3], row = i[4] == HIPGPT_WEIGHTS_EV ? V : E;
     Tensors t{a};
     const at::ScalarType k = t.kind(0, "x", &type);

@@ -35,11 +35,21 @@ def _ptr_bf16(t):
 _TYPES = {torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16}
 
 
-def _storage(t):
+def _storage(name, t):
+    """The library's code of a tensor's type: float32 or bfloat16."""
     try:
         return _TYPES[t.dtype]
     except KeyError:
         raise ValueError(f"expected float32 or bfloat16, not {t.dtype}") from None
+
+
+def _sizes(*values):
+    """Ints as the library takes them; more than one holds is refused (ctypes would pass its low bits)."""
+    out = tuple(_int(v) for v in values)
+    for v in out:
+        if not -(1 << 31) <= v < 1 << 31:
+            raise ValueError(f"{v} is beyond one call")
+    return out
 
 
 def _ptr_of(name, t, dtype, count, row=None):
@@ -107,38 +117,43 @@ class _ThroughCtypes:
     # training.py's
     @staticmethod
     def embedding_scaled(ids, tok, pos, out, scale, B, S, V, E):
-        n, dt = B * S, out.dtype
+        B, S, V, E = _sizes(B, S, V, E)
+        type_, n, dt = _storage("out", out), B * S, out.dtype
         tables = _ptr_of("tok", tok, dt, V * E, E), _ptr_of("pos", pos, dt, S * E, E)
-        return _capi.lib().hipgpt_embedding_scaled(_ptr_of("ids", ids, torch.int32, n), *tables, _ptr_of("out", out, dt, n * E), scale, B, S, V, E, _storage(out), _stream())
+        return _capi.lib().hipgpt_embedding_scaled(_ptr_of("ids", ids, torch.int32, n), *tables, _ptr_of("out", out, dt, n * E), scale, B, S, V, E, type_, _stream())
 
     @staticmethod
     def embedding_backward(grad_out, ids, grad_tok, grad_pos, scale, accumulate, B, S, V, E):
+        accumulate, B, S, V, E = _sizes(accumulate, B, S, V, E)
         n, table = B * S, grad_tok if grad_tok is not None else grad_pos
-        gt = table.dtype
+        type_, grad_type, gt = _storage("grad_out", grad_out), _storage("grad_tok", table), table.dtype
         tables = _ptr_of("grad_tok", grad_tok, gt, V * E, E), _ptr_of("grad_pos", grad_pos, gt, S * E, E)
         return _capi.lib().hipgpt_embedding_backward(_ptr_of("grad_out", grad_out, grad_out.dtype, n * E), _ptr_of("ids", ids, torch.int32, n), *tables, scale, accumulate, B, S, V, E,
-                                                     _storage(grad_out), _storage(table), _stream())
+                                                     type_, grad_type, _stream())
 
     @staticmethod
     def dropout_counter(x, residual, out, counter, p, seed, offset):
+        type_ = _storage("out", out)
         n, dt, most = out.numel(), out.dtype, (1 << 64) - 1
         return _capi.lib().hipgpt_dropout_counter(_ptr_of("x", x, dt, n), _ptr_of("residual", residual, dt, n), _ptr_of("out", out, dt, n), p, seed & most, offset & most,
-                                                  _ptr_of("counter", counter, torch.int64, 1), n, _storage(out), _stream())
+                                                  _ptr_of("counter", counter, torch.int64, 1), n, type_, _stream())
 
     @staticmethod
     def linear_cross_entropy(x, w, targets, loss, lse, N, E, V, layout):
-        dt, f, row = x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
+        N, E, V, layout = _sizes(N, E, V, layout)
+        type_, dt, f, row = _storage("x", x), x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
         weights = _ptr_of("w", w, dt, V * E, row)
         return _capi.lib().hipgpt_linear_cross_entropy(_ptr_of("x", x, dt, N * E), weights, _ptr_of("targets", targets, torch.int32, N), _ptr_of("loss", loss, f, N),
-                                                       _ptr_of("lse", lse, f, N), N, E, V, layout, _storage(x), _stream())
+                                                       _ptr_of("lse", lse, f, N), N, E, V, layout, type_, _stream())
 
     @staticmethod
     def linear_cross_entropy_backward(x, w, targets, lse, grad_loss, grad_x, grad_w, accumulate, N, E, V, layout):
-        dt, f, row = x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
+        accumulate, N, E, V, layout = _sizes(accumulate, N, E, V, layout)
+        type_, dt, f, row = _storage("x", x), x.dtype, _FLOAT32, V if layout == _capi.WEIGHTS_EV else E
         weights = _ptr_of("w", w, dt, V * E, row)
         return _capi.lib().hipgpt_linear_cross_entropy_backward(
             _ptr_of("x", x, dt, N * E), weights, _ptr_of("targets", targets, torch.int32, N), _ptr_of("lse", lse, f, N), _ptr_of("grad_loss", grad_loss, f, N),
-            _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E, row), accumulate, N, E, V, layout, _storage(x), _stream())
+            _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E, row), accumulate, N, E, V, layout, type_, _stream())
 
 
 class _AtFirstCall:

@@ -40,3 +40,28 @@ def test_tables_the_other_way_round(calls):
         calls.embedding_scaled(ids, torch.zeros(8, 5), None, out, 2, 3, 5, 8)
     with refused:
         calls.embedding_backward(out, ids, torch.zeros(8, 5), None, 2, 3, 5, 8)
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("size", [(1 << 32) + 4, -(1 << 32) + 4, 1 << 31, 1 << 70])
+def test_sizes_that_an_int_does_not_hold(calls, which, size):
+    """(1 << 32) + 4 is not 4."""
+    x, w, t, loss, lse = _loss_tensors(4, (4, 4))
+    sizes = [4, 4, 4, 4]
+    sizes[which] = size
+    refused = pytest.raises(ValueError, match="beyond one call")
+    with refused:
+        calls.embedding_scaled(t, w, None, x, *sizes)
+    with refused:
+        calls.embedding_backward(x, t, w, None, *sizes)
+    if which < 3:
+        with refused:
+            calls.linear_cross_entropy(x, w, t, loss, lse, *sizes[:3])
+        with refused:
+            calls.linear_cross_entropy_backward(x, w, t, lse, loss, x.clone(), w.clone(), *sizes[:3])
+
+
+def test_sizes_that_are_no_integers(calls):
+    x, w, t, loss, lse = _loss_tensors(4, (16, 8))
+    with pytest.raises(TypeError):
+        calls.linear_cross_entropy(x, w, t, loss, lse, 4.0, 8, 16)
