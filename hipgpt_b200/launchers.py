@@ -37,6 +37,8 @@ _TYPES = {torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16}
 
 def _storage(name, t):
     """The library's code of a tensor's type: float32 or bfloat16."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a CUDA tensor")
     try:
         return _TYPES[t.dtype]
     except KeyError:
@@ -56,6 +58,8 @@ def _ptr_of(name, t, dtype, count, row=None):
     """The address of a tensor of at least `count` values on the current device, None for None; row: of two or more dimensions, the last of so many."""
     if t is None:
         return None
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor")
     if row is not None and t.dim() >= 2 and t.shape[-1] != row:
         raise ValueError(f"{name} has rows of {t.shape[-1]} values, {row} are expected")
     if not (t.is_cuda and t.is_contiguous() and t.dtype == dtype):

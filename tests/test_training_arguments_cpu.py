@@ -61,6 +61,23 @@ def test_sizes_that_an_int_does_not_hold(calls, which, size):
             calls.linear_cross_entropy_backward(x, w, t, lse, loss, x.clone(), w.clone(), *sizes[:3])
 
 
+def test_what_is_no_tensor_is_named(calls):
+    x, w, t, loss, lse = _loss_tensors(4, (16, 8))
+    for bad in (None, 7, "x", [1.0]):
+        with pytest.raises(ValueError, match="out"):
+            calls.embedding_scaled(t, w, None, bad, 1, 4, 16, 8)
+        with pytest.raises(ValueError, match="grad_out"):
+            calls.embedding_backward(bad, t, w, None, 1, 4, 16, 8)
+        with pytest.raises(ValueError, match="out"):
+            calls.dropout_counter(x, None, bad, 0.1, seed=1)
+        with pytest.raises(ValueError, match="x"):
+            calls.linear_cross_entropy(bad, w, t, loss, lse, 4, 8, 16)
+        with pytest.raises(ValueError, match="x"):
+            calls.linear_cross_entropy_backward(bad, w, t, lse, loss, None, w.clone(), 4, 8, 16)
+    with pytest.raises(ValueError, match="w"):
+        calls.linear_cross_entropy(x, 3.0, t, loss, lse, 4, 8, 16)
+
+
 def test_sizes_that_are_no_integers(calls):
     x, w, t, loss, lse = _loss_tensors(4, (16, 8))
     with pytest.raises(TypeError):
