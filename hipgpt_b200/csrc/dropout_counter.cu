@@ -120,6 +120,7 @@ extern "C" int hipgpt_dropout_counter(const void *d_in, const void *d_residual, 
     const size_t bytes = (size_t)n * (type == HIPGPT_TYPE_F32 ? 4 : 2);
     for (const void *src : {d_in, d_residual})
         if (src && src != d_out && ranges_overlap(src, bytes, d_out, bytes)) return fail(HIPGPT_ERR_BAD_ARG, "out overlaps an input without being it");
+    if (d_counter && ranges_overlap(d_counter, sizeof(*d_counter), d_out, bytes)) return fail(HIPGPT_ERR_BAD_ARG, "out overlaps the counter");
     double t = (double)p * 65536.0 + 0.5;                // (exact: p has 24 bits)
     const uint32_t thr = t >= 65535.0 ? 65535u : (uint32_t)t;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -244,7 +244,7 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
  *                              (offset + *d_counter) + i / 8, key `seed`, kept if bits >= floor(65536 p + 1/2); 1 - p is that of the
  *                              16 bits.  The mask is not stored: the backward pass is the same call on the gradient.  d_residual may be NULL, d_out
  *                              may be d_in or d_residual; a call uses ceil(n / 8) counters.  d_counter: a 64-bit device word added to `offset`
- *                              (a captured call draws a new mask at each replay if the word has moved on), or NULL.  0 <= p < 1.
+ *                              (a captured call draws a new mask at each replay if the word has moved on), or NULL; not a part of d_out.  0 <= p < 1.
  *   hipgpt_linear_cross_entropy           z = x W^T, lse[n] = log sum_v exp z[n][v], loss[n] = lse[n] - z[n][target_n], without storing z.  x
  *                              [N][E]; weights [V][E] (HIPGPT_WEIGHTS_VE: a token embedding used twice) or [E][V] (HIPGPT_WEIGHTS_EV: the
  *                              reference's output projection, src/gpt_model.cpp).  A row whose target is outside [0, V) takes no

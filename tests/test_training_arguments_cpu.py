@@ -82,3 +82,11 @@ def test_sizes_that_are_no_integers(calls):
     x, w, t, loss, lse = _loss_tensors(4, (16, 8))
     with pytest.raises(TypeError):
         calls.linear_cross_entropy(x, w, t, loss, lse, 4.0, 8, 16)
+
+
+@pytest.mark.parametrize("at", [0, 8, 248])
+def test_dropout_into_its_own_counter(at):
+    """Blocks read the counter while others store."""
+    from hipgpt_b200 import _capi
+    P = 0x7F0000000000
+    assert _capi.lib().hipgpt_dropout_counter(P + (1 << 32), None, P, 0.1, 1, 0, P + at, 64, 0, None) == _capi.ERR_BAD_ARG
