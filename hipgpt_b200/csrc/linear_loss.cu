@@ -975,10 +975,10 @@ loss_gemm_kernel(const __grid_constant__ LossArgs args)
                     put_tile(args.sum + tile_at(x.tile, c), v);
                     return;
                 }
-                // fp32: both powers of two that go into an operand (their product may pass the range of fp32)
-                const float s0 = NP == 1 ? scales_s[2] : scales_s[x.kind == kDx ? 0 : 1], s1 = NP == 1 ? 1.0f : x.kind == kDx ? g : scales_s[2];
+                // fp32: two powers of two whose product may pass the range of fp32; the smaller one first, so that no result is lost on the way that is not too large itself
+                const float a = NP == 1 ? scales_s[2] : scales_s[x.kind == kDx ? 0 : 1], b = NP == 1 ? 1.0f : x.kind == kDx ? g : scales_s[2], s0 = fminf(a, b), s1 = fmaxf(a, b);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = NP == 1 ? v[j] * s0 : v[j] * s0 * s1;
+                for (int j = 0; j < 32; ++j) v[j] = NP == 1 ? v[j] * a : v[j] * s0 * s1;
                 const unsigned rows_here = __ballot_sync(0xffffffffu, here);
                 const bool out_vec = p.ld % kPer16<T> == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
                 if (p.accumulate || !out_vec || left < 32) {

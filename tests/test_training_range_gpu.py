@@ -226,3 +226,25 @@ def test_bf16_gradient_of_wide_rows(by_token):
     (dx, dw), (ex, ew) = ref.gradients(lse)
     tu.within(gx, dx, ex, "grad_x")
     tu.within(gw, dw, ew, "grad_w")
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+@pytest.mark.parametrize("sw,sg", [(1e37, 1e-36), (1e-36, 1e37)])
+def test_fp32_scales_that_undo_one_another(by_token, sw, sg):
+    """Weights of 1e37 and gradients of 1e-36, or the other way round: grad_x is of ordinary size."""
+    N, E, V = 60, 64, 500
+    x, w, targets = _case(N, E, V, F32, 13)
+    x, w, g = x / sw, w * sw, torch.full((N,), sg, device="cuda")
+    _, lse = _forward(x, w, targets, by_token)
+    gx, _ = _backward(x, w, targets, lse, g, by_token)     # (grad_w passes the range of fp32 in one of them)
+    ref = _Fp32(x, w, targets, g, lse)
+    tu.within(gx, ref.dx, ref.e_dx + 2.0 ** -20 * ref.dx.abs().max(), "grad_x")           # (values of 1e-37 are scaled by 2^126 at most)
+
+
+def test_gradients_of_another_shape_are_refused():
+    x, w, t = torch.zeros(4, 8, device="cuda"), torch.zeros(16, 8, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    f = torch.zeros(4, device="cuda")
+    with pytest.raises(ValueError, match="grad_w has rows"):
+        training.linear_cross_entropy_backward(x, w, t, f, f.clone(), None, torch.zeros(8, 16, device="cuda"), 4, 8, 16)
+    with pytest.raises(ValueError, match="grad_pos has rows"):
+        training.embedding_backward(x, t, None, torch.zeros(8, 2, device="cuda"), 2, 2, 16, 8)
