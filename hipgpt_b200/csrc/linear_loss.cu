@@ -1,4 +1,4 @@
-// Softmax cross entropy of a linear layer's logits, and its gradient, without the logits in memory (HipGPT multiplies by its output
+// Softmax cross entropy of a linear layer's logits, and its gradient, without stored logits (HipGPT multiplies by its output
 // projection, stores [N][V] logits and their gradient, and multiplies twice more: src/gpt_model.cpp, softmax_loss_kernel
 // src/hip_kernels.cpp:606-657).
 //
@@ -9,27 +9,29 @@
 //   kForward    a row's maximum and sum of exponentials over 256 columns, kept for loss_join_kernel; the target's logit
 //   kBackward   the vocabulary in pieces.  Of one piece the logits are formed again and their gradient stored as 16-bit numbers (kDz); the
 //               same launch forms, from the gradient of the piece before, that piece's share of dx (kDx, summed over the pieces in fp32) and its rows of
-//               dW (kDw).  Two pieces' gradients exist at a time and stay within L2 (kPieceBytes each).
-// The backward pass costs 6 N E V operations instead of 4, and no [N][V] array exists in either.
+//               dW (kDw).  Two pieces' gradients exist at a time (kPieceBytes each at most, or 1024 columns); where one piece takes the whole vocabulary, so much is stored of the
+//               gradient of the logits as a whole.
+// The backward pass costs 6 N E V operations instead of 4; the forward stores nothing of size [N][V].
 //
-// The two large sums of a launch have few tiles and long reductions (default model, a piece of 1024 columns: 32 tiles of 16 stages and 4 of 128), so the tiles that
-// do not come out even are not dealt out whole: their stages in a row are cut into a length for each pair of blocks (cut_tiles).  A tile that falls to several pairs
+// The two large sums of a launch have few tiles and long reductions (default model, one piece: 32 tiles of 79 stages and 20 of 128), so the tiles that
+// do not come out even are not dealt out whole: their stages in a row are cut into a length for each pair of blocks (plan_launch).  A tile that falls to several pairs
 // is left by each as a sum in fp32; the one that comes last adds them up, in the order of their stages.  Nothing waits for another pair, and the order of a sum depends on the
 // sizes alone.
 //
-// Rows whose target lies outside the vocabulary are left out at the start: loss_pack_x_kernel moves the others together, so they cost
+// Rows whose target lies outside the vocabulary are left out at the start: loss_pack_kernel moves the others together, so they cost
 // nothing and what they hold (NaN from padding) meets no product.
 //
 // Products: tcgen05.mma.cta_group::2, 256 x 256 tiles of two blocks, 64 deep stages by TMA in a ring, two accumulators in TMEM: the products of a
-// tile run while eight warps take the tile before it out.  Any operand may be contiguous along the reduction or across it (a descriptor
+// tile run while sixteen warps take the tile before it out.  Any operand may be contiguous along the reduction or across it (a descriptor
 // bit), so neither x, W nor dz is ever transposed.  bf16: operands as they are, dz / (largest |g|) rounded to bf16.  fp32: each operand as two fp16 numbers
 // hi + lo of the value times a power of two (2^-22 of the value; row_scales), three products a pair: lo hi + hi lo + hi hi.  The tensor
-// core's fp32 sums are cut off, not rounded, so fp32 sums leave TMEM every kPromote stages and go on in registers.
+// core's fp32 sums are cut off, not rounded, so sums leave TMEM every kSumStages stages.
 //
-// Bound, on one B200: the tensor pipe and the power it draws.  8192 x 1024 x 65536 bf16: loss 672 us in a short run (1640 TFLOP/s), 775 where the power cap sets the clock (1.37 GHz); a stage takes
-// 521 cycles, 512 of them products.  Its gradient 2670 - 2850 (1160 - 1240): 620 - 740 cycles a stage, because the operands of a 256 x 256 tile come at the 64 bytes a cycle that an SM takes from L2
-// while the logits' gradient goes out the same way.  8192 x 256 x 5000 fp32 (three products): loss 60 us, 47 of them products (30 at the full rate: 9 rounds of tiles where 8.65 are needed, the last epilogue, the launch),
-// gradient 193, 70 + 100 in its two launches of products (113 at the full rate).  64 x 256 x 5000: 20 us, a chain of four launches.
+// Bound, on one B200 (profiles/loss_gemm_kernel.md).  Loss: the tensor pipe and the power it draws: 8192 x 1024 x 65536 bf16 673 us in a short run (1634 TFLOP/s), 775 where the power cap sets the clock (1.37 GHz); a stage takes
+// 521 cycles, 512 of them products.  8192 x 256 x 5000 fp32 (three products) 64 us, 48 of them products at 0.73 of the pipe (9 rounds of tiles where 8.65 are needed, the last one's way out).
+// Gradient, bf16, large: 2370 in the best short run, 2500 - 2850 in longer ones; its sums keep the pipe 0.88 busy with operands at 57 of the 64 bytes a cycle that an SM takes from L2, the launches that also store dz 0.72.
+// Gradient, fp32, 8192 x 256 x 5000: 194, 70 + 100 in its two launches of products.  There the operands take 22 and 31 bytes a cycle: the first waits for dz's way out (one place of 2 KB a warp; 0.46 of the pipe), the second reads
+// dz out of HBM twice (168 MB in one piece: 0.3 GB) and joins shares (0.69).  64 x 256 x 5000: 21 us, a chain of four launches.
 #include "elem_types.cuh"
 #include "stream_workspace.hpp"
 #include "tma_host.cuh"
@@ -50,13 +52,13 @@ constexpr int kEpiWarps = 16, kThreads = 32 * (kEpiWarps + 2);      // four warp
 constexpr int kWarpChunks = kTileN / 4 / 32;              // 32-column chunks of a warp
 constexpr int kTmemColumns = 512;
 // Stages that TMEM sums by itself, and what the sums lose: default model's gradient 281 us and 2.2e-7 (of the largest value) with one, 229 and 4.6e-7 with two, 209 and 1.1e-6 with four
-// (sizes as below, before the accumulators were given back earlier)
+// (8192 x 256 x 5000, before the accumulators were given back earlier)
 constexpr int kPromote = 2;
 // bf16: a sum that stays in TMEM is cut off by up to 2^-23 of itself for each 16 terms, always towards zero (262144 terms of one sign in one sum: 1.6e-3 short, 65536: 3e-4).  The loss adds its logits up in registers
 // every 16 stages (64 instructions: within 2^-17).  The backward, whose results are rounded to bf16, stores a tile's sum every 128 (512: within 2^-14, a 64th of a rounding) and adds it to the next one's: accumulators
 // kept in registers there cost every tile (8192 x 256 x 5000 93 -> 106 us, by what else then leaves the registers).
 constexpr int kLossStages = 16, kGradStages = 128;
-// What a piece's gradient of the logits takes.  Longer pieces mean fewer launches and joins, and lie in HBM instead of L2: 8192 x 1024 x 65536 bf16 in pieces of 64 MB 3190 us, 128 MB 2850, 192 MB
+// What a piece's gradient of the logits takes at most.  Longer pieces mean fewer launches and joins, and lie in HBM instead of L2 (which 64 MB would leave room for): 8192 x 1024 x 65536 bf16 in pieces of 64 MB 3190 us, 128 MB 2850, 192 MB
 // 2800, 256 MB 2750; 8192 x 256 x 5000 fp32 226 us in two pieces (128 MB), 201 in one
 constexpr size_t kPieceBytes = 192u << 20;
 template <int NP> constexpr int kStageBytes = 2 * NP * kOperand;
@@ -77,7 +79,6 @@ struct Problem {
     int n_tiles, stages;                     // kDz: columns of 256, depth of 64; n_tiles 0: not asked for
     int a_across, b_across;                  // operand contiguous across the reduction (along M or N) instead of along it
     int b_k0, b_n0;                          // where the product begins in B
-    int m_by_count;                          // M is the number of rows that take part
     // kDx, kDw: element (row, column) of the result at row * ld + column
     void *out;
     long long ld;
@@ -1374,7 +1375,6 @@ int forward(const void *xv, const void *wv, const int *targets, float *loss, flo
     q.n_tiles = n_tiles;
     q.stages = (E + kDeep - 1) / kDeep;
     q.b_across = ev;
-    q.m_by_count = 1;
     a.part = reinterpret_cast<float2 *>(ws + part_at);
     a.z_target = reinterpret_cast<float *>(ws + zt_at);
     a.expire = take_expiry(700);
@@ -1438,9 +1438,7 @@ int backward(const void *xv, const void *wv, const int *targets, const float *ls
     if (rc != HIPGPT_OK) return rc;
     a.p[kDz].stages = (E + kDeep - 1) / kDeep;
     a.p[kDz].b_across = ev;
-    a.p[kDz].m_by_count = 1;
     a.p[kDx].b_across = !ev;
-    a.p[kDx].m_by_count = 1;
     a.p[kDx].out = grad_x;
     a.p[kDx].ld = a.p[kDx].cols = E;
     a.p[kDw].a_across = a.p[kDw].b_across = 1;
