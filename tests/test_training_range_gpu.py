@@ -76,7 +76,7 @@ class _Fp32:
         self.e_dx = edz @ wa + da @ wa * (3 * 2.0 ** -22 + run(V)) + 2.0 ** -39 * wmax * da.sum(1, keepdim=True) + 2 * half * self.dx.abs() + 1e-38
         most = (ga * xmax).max()
         a = torch.log2(most / (ga * xmax).clamp(min=1e-300)).sub(6).floor().clamp(0, 8)
-        floor = 2.0 ** -38 * most * 2.0 ** -a / ga.clamp(min=1e-300) * (ga > 0)
+        floor = 2.0 ** -38 * most * 2.0 ** -a / ga.clamp(min=1e-200) * (ga > 0)
         self.e_dw = edz.t() @ xa + da.t() @ xa * (3 * 2.0 ** -22 + run(N)) + da.t() @ floor.expand(N, E) + 2 * half * self.dw.abs() + 1e-38
 
 
