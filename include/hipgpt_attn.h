@@ -234,7 +234,7 @@ HIPGPT_API int hipgpt_embedding_lookup(const int *d_ids, const float *d_tok, con
  * the same bits run to run.  Except in hipgpt_dropout_counter no output may overlap another array of the call (HIPGPT_ERR_BAD_ARG).  Should a wait inside a kernel run out
  * (hipgpt_kernel_status), the call's results are not all stored.
  *   hipgpt_embedding_scaled    out[t] = scale tok[id_t] + pos[t mod S], zeros for an id outside [0, V); tok [V][E], pos [S][E] or NULL,
- *                              out [B*S][E], all of `type`.  (hipgpt_embedding_lookup with a scale, without positions, in either type.)
+ *                              out [B*S][E], all of `type`.  (hipgpt_embedding_lookup with a scale, positions or none, in either type.)
  *   hipgpt_embedding_backward  grad_tok[v] = scale * sum of grad_out[t] over the tokens with id v, grad_pos[s] = sum of grad_out over the
  *                              tokens at position s whose id is inside [0, V); either may be NULL.  Rows of tok that no token has get
  *                              zeros.  accumulate != 0: added to what the tables hold (and those rows are left as they are).  `type`: of
