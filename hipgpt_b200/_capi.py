@@ -17,9 +17,11 @@ ERR_BAD_ARG, ERR_NULL, ERR_UNSUPPORTED, ERR_CUDA, ERR_SCRATCH = -1, -2, -3, -4, 
 ALGO_AUTO, ALGO_GENERIC, ALGO_ROWS, ALGO_TENSOR = 0, 1, 2, 3
 TYPE_F32, TYPE_BF16 = 0, 1
 WEIGHTS_VE, WEIGHTS_EV = 0, 1
+CACHE_PLAIN, CACHE_E4M3, CACHE_INT8 = 0, 1, 2
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_BASE, ROTARY_RAMP = 0, 1, 2, 3
 TENSOR_DEFAULT, TENSOR_SPLIT_TF32, TENSOR_TILED, TENSOR_WHOLE_HEAD = 0, 1, 5, 6
 
-_vp, _i, _sz, _f, _ull = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_ulonglong
+_vp, _i, _sz, _f, _ull, _ll, _d = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_ulonglong, C.c_longlong, C.c_double
 
 # name -> (restype, argtypes); one entry per declaration in include/hipgpt_attn.h
 SIGNATURES = {
@@ -55,6 +57,12 @@ SIGNATURES = {
     "hipgpt_dropout_counter": (_i, [_vp, _vp, _vp, _f, _ull, _ull, _vp, C.c_longlong, _i, _vp]),
     "hipgpt_linear_cross_entropy": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "hipgpt_linear_cross_entropy_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "hipgpt_rotary_frequencies": (_i, [_vp, _i, _d, _i, _d, _d, _d, _d]),
+    "hipgpt_rotary_words": (_i, [_vp, _vp, _i]),
+    "hipgpt_rotary": (_i, [_vp, _ll, _vp, _vp, _vp, _ll, _f, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "hipgpt_cache_write": (_i, [_vp, _vp, _vp, _ll, _vp, _ll, _vp]),
+    "hipgpt_cache_read": (_i, [_vp, _vp, _vp, _ll, _vp, _ll, _vp]),
+    "hipgpt_paged_attention": (_i, [_vp, _vp, _vp, _ll, _vp, _ll, _i, _i, _f, _vp]),
     "hipgpt_mha_decode_scratch_bytes": (_sz, [_i, _i, _i, _i]),
     "hipgpt_mha_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _vp]),
     "hipgpt_mha_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),

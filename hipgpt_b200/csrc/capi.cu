@@ -332,6 +332,7 @@ void hipgpt_release_workspace(void)
     mha_backward_tc_release();
     embedding_release_scratch();
     loss_release_scratch();
+    paged_release_scratch();
     g_bwd_rows_ws.release();
     std::lock_guard<std::mutex> lock(g_ws.mu);
     if (g_ws.dev) cudaFree(g_ws.dev);

@@ -1,4 +1,4 @@
-// The Python mirror's hot calls (hipgpt_b200/launchers.py, training.py) as a CPython extension: tensors are looked at and their addresses taken in C++.  Through
+// The Python mirror's hot calls (hipgpt_b200/launchers.py, training.py, serving.py) as a CPython extension: tensors are looked at and their addresses taken in C++.  Through
 // attribute look-ups and ctypes a call of decode attention cost 3.4 us of the host beside the launch's own 2.6, more than the kernel takes
 // (2.6 us at B=8 H=8 D=32 ctx=77): 6.2 -> 3.1 us per call, attention at B=2 H=8 S=64 D=32 5.6 -> 4.8 (the kernel 4.4).
 // Every function returns the library's status; launchers.py raises.
@@ -267,6 +267,112 @@ PyObject *linear_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize
     END_HANDLE_TH_ERRORS
 }
 
+// ---- serving.py -------------------------------------------------------------------------------------------------------
+
+// A tensor of T rows of H * D values, contiguous or its first dimension alone spread: its address, and the values between its rows
+void *rows_at(Tensors &t, int i, const char *name, at::ScalarType type, int64_t T, int64_t H, int64_t D, long long *stride)
+{
+    if (!t.ok) return nullptr;
+    t.ok = false;
+    const char *kind = c10::toString(type);
+    if (!THPVariable_Check(t.a[i])) { PyErr_Format(PyExc_ValueError, "%s: expected a CUDA %s tensor", name, kind); return nullptr; }
+    const at::Tensor &x = THPVariable_Unpack(t.a[i]);
+    const int64_t width = H * D;
+    const bool whole = x.is_contiguous();
+    int64_t inner = 1;
+    bool rows = x.dim() >= 2 && x.size(0) > 0;
+    for (int64_t d = x.dim() - 1; d >= 1; --d) {
+        rows = rows && (x.size(d) == 1 || x.stride(d) == inner);
+        inner *= x.size(d);
+    }
+    if (x.dim() >= 2 && !(inner == width || (whole && (x.size(-1) == D || x.size(-1) == width)))) PyErr_Format(PyExc_ValueError, "%s has rows of %lld values, %lld are expected", name, (long long)inner, (long long)width);
+    else if (!(x.is_cuda() && x.scalar_type() == type && (whole || rows))) PyErr_Format(PyExc_ValueError, "%s: expected a CUDA %s tensor, contiguous but for its first dimension", name, kind);
+    else if (x.get_device() != c10::cuda::current_device()) PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, another is the current device", name, (int)x.get_device());
+    else if (x.numel() < T * width) PyErr_Format(PyExc_ValueError, "%s holds %lld values, %lld are needed", name, (long long)x.numel(), (long long)(T * width));
+    else { t.ok = true; *stride = whole ? width : x.stride(0); return x.data_ptr(); }
+    return nullptr;
+}
+
+// x, positions, words, out, T, H, D, R, interleaved, inverse, magnitude
+PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int i[6], type = 0;
+    if (!count(n, 11) || !sizes(a + 4, 6, i)) return nullptr;
+    const double magnitude = PyFloat_AsDouble(a[10]);
+    if (PyErr_Occurred()) return nullptr;
+    const int64_t T = i[0], H = i[1], D = i[2], R = i[3];
+    Tensors t{a};
+    long long sx = 0, so = 0;
+    const at::ScalarType k = t.kind(3, "out", &type);
+    const void *x = rows_at(t, 0, "x", k, T, H, D, &sx);
+    void *out = rows_at(t, 3, "out", k, T, H, D, &so);
+    const void *positions = t.at(1, "positions", at::kInt, T), *words = t.at(2, "words", at::kLong, R / 2);
+    if (!t.ok) return nullptr;
+    return status_of([&](void *st) {
+        return hipgpt_rotary(x, sx, static_cast<const int *>(positions), static_cast<const unsigned long long *>(words), out, so, (float)magnitude, i[4], i[5], i[0], i[1], i[2], i[3], type, st);
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// A cache's address and device, then (at 4) offsets, lengths, pages, T, B
+const hipgpt_paged_cache *cache_at(PyObject *const *a)
+{
+    const auto *c = static_cast<const hipgpt_paged_cache *>(PyLong_AsVoidPtr(a[0]));
+    const long device = PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    if (device != c10::cuda::current_device()) { PyErr_Format(PyExc_ValueError, "the cache is on cuda:%ld, another is the current device", device); return nullptr; }
+    return c;
+}
+bool batch_at(Tensors &t, int64_t T, int64_t B, hipgpt_paged_batch *out)
+{
+    if (!t.ok) return false;
+    if (!THPVariable_Check(t.a[6]) || THPVariable_Unpack(t.a[6]).dim() != 2) { PyErr_SetString(PyExc_ValueError, "pages: expected a contiguous CUDA int32 tensor of two dimensions"); return t.ok = false; }
+    const int64_t most = THPVariable_Unpack(t.a[6]).size(1);
+    if (most > 2147483647LL) { PyErr_Format(PyExc_ValueError, "%lld is beyond one call", (long long)most); return t.ok = false; }
+    *out = {static_cast<const int *>(t.at(4, "offsets", at::kInt, B + 1)), static_cast<const int *>(t.at(5, "lengths", at::kInt, B)), static_cast<const int *>(t.at(6, "pages", at::kInt, B * most)),
+            (int)B, (int)T, (int)most};
+    return t.ok;
+}
+at::ScalarType type_of(const hipgpt_paged_cache *c) { return c->type == HIPGPT_TYPE_F32 ? at::kFloat : at::kBFloat16; }
+
+// cache, device, k, v, offsets, lengths, pages, T, B, write
+PyObject *cache_move(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int i[3];
+    if (!count(n, 10) || !sizes(a + 7, 3, i)) return nullptr;
+    Tensors t{a};
+    const hipgpt_paged_cache *c = reinterpret_cast<const hipgpt_paged_cache *>(PyLong_AsVoidPtr(a[0]));
+    if (PyErr_Occurred()) return nullptr;
+    long long sk = 0, sv = 0;
+    hipgpt_paged_batch batch;
+    void *k = rows_at(t, 2, "k", type_of(c), i[0], c->heads, c->head_dim, &sk), *v = rows_at(t, 3, "v", type_of(c), i[0], c->heads, c->head_dim, &sv);
+    if (!t.ok || !cache_at(a) || !batch_at(t, i[0], i[1], &batch)) return nullptr;
+    return status_of([&](void *st) { return i[2] ? hipgpt_cache_write(c, &batch, k, sk, v, sv, st) : hipgpt_cache_read(c, &batch, k, sk, v, sv, st); });
+    END_HANDLE_TH_ERRORS
+}
+
+// cache, device, q, out, offsets, lengths, pages, T, B, H, causal, scale
+PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int i[4];
+    if (!count(n, 12) || !sizes(a + 7, 4, i)) return nullptr;
+    const double scale = PyFloat_AsDouble(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensors t{a};
+    const hipgpt_paged_cache *c = reinterpret_cast<const hipgpt_paged_cache *>(PyLong_AsVoidPtr(a[0]));
+    if (PyErr_Occurred()) return nullptr;
+    long long sq = 0, so = 0;
+    hipgpt_paged_batch batch;
+    const void *q = rows_at(t, 2, "q", type_of(c), i[0], i[2], c->head_dim, &sq);
+    void *out = rows_at(t, 3, "out", type_of(c), i[0], i[2], c->head_dim, &so);
+    if (!t.ok || !cache_at(a) || !batch_at(t, i[0], i[1], &batch)) return nullptr;
+    return status_of([&](void *st) { return hipgpt_paged_attention(c, &batch, q, sq, out, so, i[2], i[3], (float)scale, st); });
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     if (!count(n, 3)) return nullptr;
@@ -284,6 +390,9 @@ PyMethodDef methods[] = {{"attention", reinterpret_cast<PyCFunction>(reinterpret
                          {"dropout_counter", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(dropout_counter)), METH_FASTCALL, nullptr},
                          {"linear_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(linear_cross_entropy)), METH_FASTCALL, nullptr},
                          {"linear_cross_entropy_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(linear_cross_entropy_backward)), METH_FASTCALL, nullptr},
+                         {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rotary)), METH_FASTCALL, nullptr},
+                         {"cache_move", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(cache_move)), METH_FASTCALL, nullptr},
+                         {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_attention)), METH_FASTCALL, nullptr},
                          {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(bind)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hipgpt_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

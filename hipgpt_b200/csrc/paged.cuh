@@ -1,0 +1,110 @@
+// A cache in pages and the ragged batch that works on it: what the kernels of rotary.cu's neighbours share (paged_cache.cu, attn_paged.cu,
+// attn_paged_tc.cu).
+//
+//   cache   k, v [pages][heads][page size][D] of the activations' type, or of 8-bit codes with one fp32 scale per row ([pages][heads][page size])
+//   batch   sequence b's new tokens are the rows offsets[b] .. offsets[b+1] of the call's tensors; they are the last of the lengths[b] tokens that the
+//           sequence has with them; position p of it lies in page table[b][p / page size], at p % page size
+//
+// What the device holds is not known to the host and is not trusted: offsets are cut to [0, T], lengths to what a row of the table can hold, and a page
+// number outside the cache is a page without tokens.
+#pragma once
+
+#include "elem_types.cuh"
+
+namespace hipgpt {
+
+struct PagedView {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    const int *offsets, *lengths, *table;
+    int B, T, most_pages, pages, shift, heads, D;
+};
+
+struct Sequence { int first, n, len; };          // first row, new tokens, length with them
+__device__ __forceinline__ Sequence sequence_of(const PagedView &c, int b)
+{
+    const int a = min(max(__ldg(c.offsets + b), 0), c.T), e = min(max(__ldg(c.offsets + b + 1), 0), c.T);
+    const long long room = (long long)c.most_pages << c.shift;
+    return {a, max(e - a, 0), (int)min((long long)max(__ldg(c.lengths + b), 0), room)};
+}
+
+// The row of position p (>= 0, below the sequence's length) of sequence b in units of rows of the cache, -1 where its page is none
+__device__ __forceinline__ long long row_of(const PagedView &c, int b, int head, int p)
+{
+    const int page = __ldg(c.table + (size_t)b * c.most_pages + (p >> c.shift));
+    if (page < 0 || page >= c.pages) return -1;
+    return ((((long long)page * c.heads) + head) << c.shift) + (p & ((1 << c.shift) - 1));
+}
+
+// ---- 8-bit codes: four of one word as the bf16 values that they are (exact), in two words ----
+// `x` holds two codes in the upper bytes (e4m3) or lower bytes (int8) of its halves; the other bytes may hold anything.
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// sign, 4 bits of exponent and 3 of mantissa at bf16's place stand for 2^-120 of the value, subnormals included
+__device__ __forceinline__ uint32_t e4m3_to_bf16x2(uint32_t x) { return mul_bf16x2((x & 0x80008000u) | ((x >> 4) & 0x07F007F0u), 0x7B807B80u); }
+// 0x43uu with seven bits u is 128 + u; 0x4300 is 128 and 0x4380 is 256: the low bits less what the sign bit says
+__device__ __forceinline__ uint32_t int8_to_bf16x2(uint32_t x) { return sub_bf16x2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) | 0x43004300u); }
+template <int FMT>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w0, uint32_t w1, int byte0, int byte1)      // byte0 of w0 in the low half, byte1 of w1 in the high one
+{
+    if constexpr (FMT == HIPGPT_CACHE_E4M3) return e4m3_to_bf16x2(__byte_perm(w0, w1, (byte0 << 4) | ((4 + byte1) << 12)));
+    else return int8_to_bf16x2(__byte_perm(w0, w1, byte0 | ((4 + byte1) << 8)));
+}
+
+// What the host checks of a cache and a batch (0: go on, 1: nothing to do, < 0: refused)
+inline int check_paged(const hipgpt_paged_cache *c, const hipgpt_paged_batch *b, PagedView *out)
+{
+    if (!c || !b) return fail(HIPGPT_ERR_NULL, "cache and batch must not be NULL");
+    if (c->type != HIPGPT_TYPE_F32 && c->type != HIPGPT_TYPE_BF16) return fail(HIPGPT_ERR_BAD_ARG, "unknown type %d", c->type);
+    if (c->format != HIPGPT_CACHE_PLAIN && c->format != HIPGPT_CACHE_E4M3 && c->format != HIPGPT_CACHE_INT8) return fail(HIPGPT_ERR_BAD_ARG, "unknown cache format %d", c->format);
+    if (c->pages < 0 || c->heads <= 0 || c->head_dim <= 0 || b->sequences < 0 || b->tokens < 0 || b->most_pages < 0)
+        return fail(HIPGPT_ERR_BAD_ARG, "bad size: pages=%d heads=%d head_dim=%d sequences=%d tokens=%d most_pages=%d", c->pages, c->heads, c->head_dim, b->sequences, b->tokens, b->most_pages);
+    if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return fail(HIPGPT_ERR_BAD_ARG, "page size %d is no power of two from 16 to 1024", c->page_size);
+    if (c->head_dim % 16 || c->head_dim > 128) return fail(HIPGPT_ERR_UNSUPPORTED, "head_dim %d is no multiple of 16 up to 128", c->head_dim);
+    if ((long long)c->heads * c->head_dim > 1 << 24) return fail(HIPGPT_ERR_BAD_ARG, "rows of %d heads of %d values are too long", c->heads, c->head_dim);
+    if ((long long)b->most_pages * c->page_size > 2147483647LL) return fail(HIPGPT_ERR_BAD_ARG, "%d pages of %d tokens are beyond what a length can say", b->most_pages, c->page_size);
+    if ((long long)c->pages * c->heads * c->page_size > 1LL << 40) return fail(HIPGPT_ERR_BAD_ARG, "a cache of %d pages is too large", c->pages);
+    if (b->tokens == 0 || b->sequences == 0) return 1;
+    if (!b->offsets || !b->lengths || (!b->page_table && b->most_pages > 0)) return fail(HIPGPT_ERR_NULL, "offsets, lengths and the page table must not be NULL");
+    const bool coded = c->format != HIPGPT_CACHE_PLAIN;
+    if (c->pages > 0 && (!c->k || !c->v || (coded && (!c->k_scale || !c->v_scale)))) return fail(HIPGPT_ERR_NULL, "the cache's arrays must not be NULL");
+    if (!all_aligned16({c->k, c->v, c->k_scale, c->v_scale})) return fail(HIPGPT_ERR_BAD_ARG, "the cache's arrays must start on 16-byte boundaries");
+    int shift = 0;
+    while ((1 << shift) < c->page_size) ++shift;
+    *out = {static_cast<const uint8_t *>(c->k), static_cast<const uint8_t *>(c->v), c->k_scale, c->v_scale, b->offsets, b->lengths, b->page_table,
+            b->sequences, b->tokens, b->most_pages, c->pages, shift, c->heads, c->head_dim};
+    return HIPGPT_OK;
+}
+
+inline size_t cache_element_bytes(const hipgpt_paged_cache *c) { return c->format != HIPGPT_CACHE_PLAIN ? 1 : c->type == HIPGPT_TYPE_F32 ? 4 : 2; }
+inline size_t cache_rows(const hipgpt_paged_cache *c) { return (size_t)c->pages * c->heads * c->page_size; }
+
+// Rows of `width` bytes, `stride` bytes apart
+struct Rows { const void *at; size_t stride, width; long long n; };
+inline size_t extent_of(const Rows &r) { return r.n > 0 ? (size_t)(r.n - 1) * r.stride + r.width : 0; }
+// Columns of one wider array (the same stride) may lie beside each other; otherwise what is between the rows counts as theirs
+inline bool rows_overlap(const Rows &a, const Rows &b)
+{
+    if (!a.at || !b.at || a.n <= 0 || b.n <= 0 || !ranges_overlap(a.at, extent_of(a), b.at, extent_of(b))) return false;
+    if (a.stride != b.stride) return true;
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.at), pb = reinterpret_cast<uintptr_t>(b.at);
+    const size_t d = pb >= pa ? (pb - pa) % a.stride : (a.stride - (pa - pb) % a.stride) % a.stride;
+    return !(d >= a.width && d + b.width <= a.stride);
+}
+inline int check_stride(const char *what, long long stride, long long width)
+{
+    if (stride < width || stride > 1LL << 40) return fail(HIPGPT_ERR_BAD_ARG, "%s: rows of %lld values cannot be %lld apart", what, width, stride);
+    return HIPGPT_OK;
+}
+// A written array against the batch's and the cache's
+inline int refuse_rows_over(const Rows &out, std::initializer_list<Rows> others, const hipgpt_paged_cache *c, const hipgpt_paged_batch *b)
+{
+    for (const Rows &o : others) if (rows_overlap(out, o)) return fail(HIPGPT_ERR_BAD_ARG, "an output overlaps another of the call's arrays");
+    const size_t rows = cache_rows(c), bytes = rows * c->head_dim * cache_element_bytes(c);
+    for (const Extent &e : {Extent{c->k, bytes}, Extent{c->v, bytes}, Extent{c->k_scale, rows * 4}, Extent{c->v_scale, rows * 4}, Extent{b->offsets, 4 * ((size_t)b->sequences + 1)},
+                            Extent{b->lengths, 4 * (size_t)b->sequences}, Extent{b->page_table, 4 * (size_t)b->sequences * b->most_pages}})
+        if (e.at && e.bytes && out.at && ranges_overlap(out.at, extent_of(out), e.at, e.bytes)) return fail(HIPGPT_ERR_BAD_ARG, "an output overlaps another of the call's arrays");
+    return HIPGPT_OK;
+}
+
+}  // namespace hipgpt

@@ -71,6 +71,49 @@ def _ptr_of(name, t, dtype, count, row=None):
     return t.data_ptr()
 
 
+_TYPE_OF = {code: dtype for dtype, code in _TYPES.items()}
+
+
+class _PagedCache(ctypes.Structure):
+    """hipgpt_paged_cache"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [(n, ctypes.c_int) for n in ("pages", "page_size", "heads", "head_dim", "type", "format")]
+
+
+class _PagedBatch(ctypes.Structure):
+    """hipgpt_paged_batch"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("offsets", "lengths", "page_table")] + [(n, ctypes.c_int) for n in ("sequences", "tokens", "most_pages")]
+
+
+def _rows_of(name, t, dtype, T, H, D):
+    """(address, values between rows) of a tensor of T rows of H * D values: contiguous, or its first dimension alone spread."""
+    width = H * D
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a CUDA {dtype} tensor")
+    inner = 1
+    for n in t.shape[1:]:
+        inner *= n
+    whole = t.is_contiguous()
+    if t.dim() >= 2 and not (inner == width or (whole and t.shape[-1] in (D, width))):
+        raise ValueError(f"{name} has rows of {inner} values, {width} are expected")
+    if not (t.is_cuda and t.dtype == dtype and (whole or (t.dim() >= 2 and t.shape[0] and t[0].is_contiguous()))):
+        raise ValueError(f"{name}: expected a CUDA {dtype} tensor, contiguous but for its first dimension")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
+    if t.numel() < T * width:
+        raise ValueError(f"{name} holds {t.numel()} values, {T * width} are needed")
+    return t.data_ptr(), width if whole else t.stride(0)
+
+
+def _batch_of(device, offsets, lengths, pages, T, B):
+    if device != torch.cuda.current_device():
+        raise ValueError(f"the cache is on cuda:{device}, the current device is {torch.cuda.current_device()}")
+    if not isinstance(pages, torch.Tensor) or pages.dim() != 2:
+        raise ValueError("pages: expected a contiguous CUDA int32 tensor of two dimensions")
+    most = pages.shape[1]
+    at = _ptr_of("offsets", offsets, torch.int32, B + 1), _ptr_of("lengths", lengths, torch.int32, B), _ptr_of("pages", pages, torch.int32, B * most)
+    return _PagedBatch(*at, B, T, *_sizes(most))
+
+
 # the current stream's handle without the Stream object around it (3.2 us of host time per call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = torch.cuda.current_device
@@ -158,6 +201,34 @@ class _ThroughCtypes:
         return _capi.lib().hipgpt_linear_cross_entropy_backward(
             _ptr_of("x", x, dt, N * E), weights, _ptr_of("targets", targets, torch.int32, N), _ptr_of("lse", lse, f, N), _ptr_of("grad_loss", grad_loss, f, N),
             _ptr_of("grad_x", grad_x, dt, N * E), _ptr_of("grad_w", grad_w, dt, V * E, row), accumulate, N, E, V, layout, type_, _stream())
+
+    # serving.py's
+    @staticmethod
+    def rotary(x, positions, words, out, T, H, D, R, interleaved, inverse, magnitude):
+        T, H, D, R, interleaved, inverse = _sizes(T, H, D, R, interleaved, inverse)
+        type_ = _storage("out", out)
+        src, dst = _rows_of("x", x, out.dtype, T, H, D), _rows_of("out", out, out.dtype, T, H, D)
+        return _capi.lib().hipgpt_rotary(*src, _ptr_of("positions", positions, torch.int32, T), _ptr_of("words", words, torch.int64, R // 2), *dst, magnitude, interleaved, inverse,
+                                         T, H, D, R, type_, _stream())
+
+    @staticmethod
+    def cache_move(cache, device, k, v, offsets, lengths, pages, T, B, write):
+        T, B = _sizes(T, B)
+        c = _PagedCache.from_address(cache)
+        dt = _TYPE_OF[c.type]
+        rows = *_rows_of("k", k, dt, T, c.heads, c.head_dim), *_rows_of("v", v, dt, T, c.heads, c.head_dim)
+        batch = _batch_of(device, offsets, lengths, pages, T, B)
+        call = _capi.lib().hipgpt_cache_write if write else _capi.lib().hipgpt_cache_read
+        return call(cache, ctypes.byref(batch), *rows, _stream())
+
+    @staticmethod
+    def paged_attention(cache, device, q, out, offsets, lengths, pages, T, B, H, causal, scale):
+        T, B, H = _sizes(T, B, H)
+        c = _PagedCache.from_address(cache)
+        dt = _TYPE_OF[c.type]
+        rows = *_rows_of("q", q, dt, T, H, c.head_dim), *_rows_of("out", out, dt, T, H, c.head_dim)
+        batch = _batch_of(device, offsets, lengths, pages, T, B)
+        return _capi.lib().hipgpt_paged_attention(cache, ctypes.byref(batch), *rows, H, causal, scale, _stream())
 
 
 class _AtFirstCall:

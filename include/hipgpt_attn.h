@@ -308,6 +308,69 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
                               int B, int H, int D, int ctx, int cap, void *stream);
 
 /*
+ * Serving a ragged batch from a cache in pages (extension; the reference re-runs the whole window for each token, src/gpt_model.cpp:261-280).
+ * Activations in fp32 or bf16 (`type`), sums and softmax in fp32.
+ *
+ *   hipgpt_paged_cache   k, v [pages][heads][page_size][head_dim]: values of `type` (HIPGPT_CACHE_PLAIN) or 8-bit codes, whose scales k_scale, v_scale
+ *                        [pages][heads][page_size] fp32 belong to one row of a head each (NULL for plain caches).  page_size a power of two from 16 to
+ *                        1024, head_dim a multiple of 16 up to 128, the arrays on 16-byte boundaries.
+ *     HIPGPT_CACHE_E4M3  scale = the smallest power of two (2^-126 at least) with max|row| <= 448 scale; codes rounded to nearest, ties to even: four significant bits
+ *                        of a value down to 2^-13 of its row's largest
+ *     HIPGPT_CACHE_INT8  scale = max|row| / 127 in fp32 (2^-126 at least), code = value / scale to nearest, ties to even
+ *     A row that holds an infinity or NaN gets codes 0 and the scale NaN: all of it reads as NaN.
+ *   hipgpt_paged_batch   `tokens` new tokens of `sequences` sequences, rows of the call's tensors: sequence b's are offsets[b] .. offsets[b+1]-1
+ *                        (offsets [sequences + 1], ascending), the last ones of the lengths[b] tokens that it has with them; position p of sequence b lies in page
+ *                        page_table[b][p / page_size] ([sequences][most_pages]) at p % page_size.  All three on the device, read when the kernels run (a captured
+ *                        call sees what they hold at its replay), so bad values cannot be refused: offsets are cut to [0, tokens], lengths to most_pages *
+ *                        page_size, a page number outside [0, pages) is a page without tokens.  Rows of no sequence are left as they are.
+ *   Tensors of tokens have rows of heads * head_dim values, *_stride values apart (a part of a wider row, as of a packed projection, is one).  No output may overlap
+ *   another array of the call (HIPGPT_ERR_BAD_ARG), but for columns of one wider array beside each other and where noted.
+ *
+ *   hipgpt_rotary_frequencies  radians per position (float64, host) of the R / 2 pairs of a rotation: base^(-2i/R), for long contexts slowed down:
+ *                              HIPGPT_ROTARY_LINEAR all by `factor`; _BASE the base raised to base * factor^(R / (R - 2)), which slows the last pair by the factor and
+ *                              the first not at all; _RAMP by the factor where a pair turns less than `low` times in `original` positions, not where more than `high`
+ *                              times, on a straight line in the number of turns in between.
+ *   hipgpt_rotary_words        n such frequencies as the kernel takes them: 64-bit fractions of a turn (host to host; the caller copies them to the device).
+ *   hipgpt_rotary              out = magnitude * R(position) x on the first R values of each head, the others copied; pairs (i, i + R/2), or (2i, 2i + 1) with
+ *                              interleaved != 0.  inverse != 0: the rotation backwards, which is the backward pass.  Position times frequency is taken exactly modulo
+ *                              a turn, so far positions lose nothing.  x may be out (the same stride).  R even, R <= D; any D up to 1024.
+ *   hipgpt_cache_write         rows of k and v [tokens][heads * head_dim] to their places in the cache, in its format.  Positions below 0 (more new tokens than the length) and
+ *                              pages without number are left out.  Two tokens must not share a place.
+ *   hipgpt_cache_read          the other way round: the values that the cache holds for the batch's tokens, zeros where it has no place for one.
+ *   hipgpt_paged_attention     out[t][h] = softmax(scale q k^T) v over the keys of t's sequence: causal != 0 those up to t's position, 0 all lengths[b].
+ *                              q, out [tokens][H * head_dim], H a multiple of the cache's heads: H / heads query heads in a row share one.  A row that sees no key gets zeros
+ *                              (as one whose scores are all minus infinity).  What lies in masked places, NaN too, does not matter.  scale > 0.
+ *                              fp32: products from three bf16 pieces of each fp32 operand on the tensor pipe, sums in fp32; an infinity in q or a plain cache makes NaN of
+ *                              the scores that it meets.  bf16: probabilities are rounded to bf16 before the second product.
+ *                              Keys are split over blocks where rows are few; buffers of the library (per device and stream, at most eight; hipgpt_release_workspace()
+ *                              frees them; a captured call gets buffers of its graph) hold the parts.  The same bits run to run on the same GPU.
+ */
+#define HIPGPT_CACHE_PLAIN 0
+#define HIPGPT_CACHE_E4M3  1
+#define HIPGPT_CACHE_INT8  2
+#define HIPGPT_ROTARY_UNSCALED 0
+#define HIPGPT_ROTARY_LINEAR   1
+#define HIPGPT_ROTARY_BASE     2
+#define HIPGPT_ROTARY_RAMP     3
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int pages, page_size, heads, head_dim, type, format;
+} hipgpt_paged_cache;
+typedef struct {
+    const int *offsets, *lengths, *page_table;
+    int sequences, tokens, most_pages;
+} hipgpt_paged_batch;
+HIPGPT_API int hipgpt_rotary_frequencies(double *h_freq, int R, double base, int scaling, double factor, double original, double low, double high);
+HIPGPT_API int hipgpt_rotary_words(const double *h_freq, unsigned long long *h_words, int n);
+HIPGPT_API int hipgpt_rotary(const void *d_x, long long x_stride, const int *d_positions, const unsigned long long *d_words, void *d_out, long long out_stride,
+                  float magnitude, int interleaved, int inverse, int T, int H, int D, int R, int type, void *stream);
+HIPGPT_API int hipgpt_cache_write(const hipgpt_paged_cache *cache, const hipgpt_paged_batch *batch, const void *d_k, long long k_stride, const void *d_v, long long v_stride, void *stream);
+HIPGPT_API int hipgpt_cache_read(const hipgpt_paged_cache *cache, const hipgpt_paged_batch *batch, void *d_k, long long k_stride, void *d_v, long long v_stride, void *stream);
+HIPGPT_API int hipgpt_paged_attention(const hipgpt_paged_cache *cache, const hipgpt_paged_batch *batch, const void *d_q, long long q_stride, void *d_out, long long out_stride,
+                           int H, int causal, float scale, void *stream);
+
+/*
  * Greedy generation with a HipGPT-shaped model on one GPU, KV-cache form: the host driver that
  * stands where GPTModel::generate's loop stands (src/gpt_model.cpp:248-353) for the benchmark's
  * whole-model shape.  Every token runs once, at its own position, against cached keys and
