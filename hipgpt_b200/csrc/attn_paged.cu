@@ -20,6 +20,9 @@
 #include <math.h>
 
 namespace hipgpt {
+
+StreamWorkspace g_paged_ws;                      // parts of tiles (attn_paged_tc.cu's too)
+
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
@@ -425,9 +428,9 @@ paged_rows_kernel(const AttnArgs a)
                 }
                 if (dst) {
                     if (lane == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[r] = make_float2(top, sum);
-                } else if (!C::CODED && __any_sync(0xffffffffu, wild)) {
+                } else if (__any_sync(0xffffffffu, wild)) {
                     __syncwarp();
-                    mend_row<T>(a, w.b, w.head, s, (int)row, keys);
+                    mend_row<T, FMT>(a, w.b, w.head, s, (int)row, keys);
                 }
             }
         } else {
@@ -461,28 +464,27 @@ paged_rows_kernel(const AttnArgs a)
                             }
                     if (dst && there && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[mt][r], sum);
                 }
-            if constexpr (!C::CODED) {
-                if (!dst) {
+            if (!dst) {
 #pragma unroll
-                    for (int mt = 0; mt < C::MT; ++mt)
+                for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            unsigned some = __ballot_sync(0xffffffffu, wild[mt][r]);
-                            __syncwarp();
-                            while (some) {
-                                const int who = (__ffs((int)some) - 1) >> 2;     // its row in the tile's eight
-                                some &= ~(0xFu << (4 * who));
-                                mend_row<T>(a, w.b, w.head, s, row0 + (warp * C::MT + mt) * 16 + who + 8 * r, keys);
-                            }
+                    for (int r = 0; r < 2; ++r) {
+                        unsigned some = __ballot_sync(0xffffffffu, wild[mt][r]);
+                        __syncwarp();
+                        while (some) {
+                            const int who = (__ffs((int)some) - 1) >> 2;         // its row in the tile's eight
+                            some &= ~(0xFu << (4 * who));
+                            mend_row<T, FMT>(a, w.b, w.head, s, row0 + (warp * C::MT + mt) * 16 + who + 8 * r, keys);
                         }
-                }
+                    }
             }
         }
     }
-    if (a.cuts && tid == 0) a.cuts[blockIdx.x] = cut;
+    if (a.cuts && tid == 0) {
+        a.cuts[blockIdx.x] = cut;
+        a.whole[blockIdx.x] = 1;
+    }
 }
-
-StreamWorkspace g_paged_ws;
 
 template <typename T, int FMT, int DP, bool SPLITROWS>
 int launch_rows(AttnArgs a, cudaStream_t st)
@@ -512,10 +514,11 @@ int launch_rows(AttnArgs a, cudaStream_t st)
     StreamWorkspace::Lease ws;
     if (cuts) {
         const size_t parts = (size_t)2 * grid * C::ROWS * (DP + 2) * sizeof(float);
-        const int rc = g_paged_ws.enter(st, parts + (size_t)grid * sizeof(int4), &ws);
+        const int rc = g_paged_ws.enter(st, parts + (size_t)grid * (sizeof(int4) + sizeof(int)), &ws);
         if (rc != HIPGPT_OK) return rc;
         a.parts = reinterpret_cast<float *>(ws.get());
         a.cuts = reinterpret_cast<int4 *>(ws.get() + parts);
+        a.whole = reinterpret_cast<int *>(a.cuts + grid);
     }
     e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), C::kSmem, st, a);
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<T, FMT, C::ROWS, DP>, dim3((unsigned)grid, (unsigned)(C::ROWS + 15) / 16), dim3(256), 0, st, a);
@@ -532,9 +535,15 @@ template <typename T>
 int launch_paged(int format, const AttnArgs &a, cudaStream_t st)
 {
     const bool few = (long long)a.c.T * a.group <= 32LL * a.c.B;
-    if (format == HIPGPT_CACHE_PLAIN) return few ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_PLAIN, true>(a, st);
-    if (format == HIPGPT_CACHE_E4M3) return few ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_E4M3, true>(a, st);
-    return few ? launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, true>(a, st);
+    if constexpr (sizeof(T) == 2) {
+        if (!few) return launch_paged_tc(format, a, st);
+        return format == HIPGPT_CACHE_PLAIN ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st)
+             : format == HIPGPT_CACHE_E4M3  ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st);
+    } else {
+        if (format == HIPGPT_CACHE_PLAIN) return few ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_PLAIN, true>(a, st);
+        if (format == HIPGPT_CACHE_E4M3) return few ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_E4M3, true>(a, st);
+        return few ? launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, true>(a, st);
+    }
 }
 
 }  // namespace

@@ -21,6 +21,7 @@ struct AttnArgs {
     int least;                           // units a block takes at least
     float *parts;                        // [2 * blocks][ROWS][DP + 2]: sums, then maximum (log2 domain) and sum of exponentials of each row
     int4 *cuts;                          // [blocks]: the tile that begins here and goes on: sequence, head, tile, last block (w < 0: none)
+    int *whole;                          // [blocks]: 0 where a wait ran out
 };
 
 // One tile's run of units in a block
@@ -173,10 +174,18 @@ struct Run {
 };
 
 // ---- rows worked out key by key ----------------------------------------------------------------------------------------
-// A product over a tile of keys takes every row's probabilities times every key's values, zero times what a row must not see.  Where that is an infinity or NaN in a
-// plain cache (codes are finite, and a masked scale is left out) the sum is NaN.  Such a row is found by its result, and is worked out again without the keys that it does not see.
+// A product over a tile of keys takes every row's probabilities times every key's values, zero times what a row must not see.  Where that is an infinity or NaN the
+// sum is NaN.  Such a row is found by its result, and is worked out again without the keys that it does not see.
 
-template <typename T>
+// One value of a row of the cache
+template <typename T, int FMT>
+__device__ __forceinline__ float cached(const uint8_t *base, const float *scale, long long row, int D, int d)
+{
+    if constexpr (FMT == HIPGPT_CACHE_PLAIN) return to_float(reinterpret_cast<const T *>(base)[row * D + d]);
+    else return __uint_as_float(code_pair<FMT>(base[row * D + d], 0u, 0, 0) << 16) * scale[row];
+}
+
+template <typename T, int FMT>
 __device__ __forceinline__ bool any_wild(const AttnArgs &a, int b, int head, int from, int to)
 {
     const int lane = threadIdx.x & 31;
@@ -185,14 +194,14 @@ __device__ __forceinline__ bool any_wild(const AttnArgs &a, int b, int head, int
         const long long row = row_of(a.c, b, head, p);
         bool w = false;
         if (row >= 0)
-            for (int d = lane; d < a.c.D; d += 32) w = w || !(fabsf(to_float(reinterpret_cast<const T *>(a.c.v)[row * a.c.D + d])) <= 3.402823466e38f);
+            for (int d = lane; d < a.c.D; d += 32) w = w || !(fabsf(cached<T, FMT>(a.c.v, a.c.vs, row, a.c.D, d)) <= 3.402823466e38f);
         wild = __any_sync(0xffffffffu, w);
     }
     return wild;
 }
 
-// One warp: row `row` of (sequence b, head of the cache); only for plain caches
-template <typename T>
+// One warp: row `row` of (sequence b, head of the cache)
+template <typename T, int FMT>
 __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row)
 {
     const int lane = threadIdx.x & 31, D = a.c.D, limit = limit_of(a, s, row);
@@ -208,10 +217,9 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
     for (int p = 0; p < limit; ++p) {
         const long long r = row_of(a.c, b, head, p);
         if (r < 0) continue;
-        const T *k = reinterpret_cast<const T *>(a.c.k) + r * D, *v = reinterpret_cast<const T *>(a.c.v) + r * D;
         float z = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) z = fmaf(qv[i], to_float(k[lane + 32 * i]), z);
+        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) z = fmaf(qv[i], cached<T, FMT>(a.c.k, a.c.ks, r, D, lane + 32 * i), z);
 #pragma unroll
         for (int off = 16; off; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
         z *= a.cscale;
@@ -220,7 +228,7 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
         m = mn;
         l = fmaf(l, alpha, e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) o[i] = fmaf(e, to_float(v[lane + 32 * i]), o[i] * alpha);
+        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) o[i] = fmaf(e, cached<T, FMT>(a.c.v, a.c.vs, r, D, lane + 32 * i), o[i] * alpha);
     }
     T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
 #pragma unroll
@@ -228,11 +236,11 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
 }
 
 // Whether a row whose result is not finite was touched by keys that it does not see (its tile's keys go up to `keys`)
-template <typename T>
+template <typename T, int FMT>
 __device__ __forceinline__ void mend_row(const AttnArgs &a, int b, int head, const Sequence &s, int row, int keys)
 {
     const int limit = limit_of(a, s, row);
-    if (limit < keys && any_wild<T>(a, b, head, limit, keys)) row_again<T>(a, b, head, s, row);
+    if (limit < keys && any_wild<T, FMT>(a, b, head, limit, keys)) row_again<T, FMT>(a, b, head, s, row);
 }
 
 // ---- joining the parts ----------------------------------------------------------------------------------------------------
@@ -245,6 +253,7 @@ paged_join_kernel(const AttnArgs a)
     dependents_may_start();
     const int4 cut = a.cuts[blockIdx.x];
     if (cut.w < 0) return;
+    for (int blk = blockIdx.x; blk <= cut.w; ++blk) if (!a.whole[blk]) return;
     const Sequence s = sequence_of(a.c, cut.x);
     const int lane = threadIdx.x & 31, D = a.c.D;
     constexpr int E = DP / 32;
@@ -275,13 +284,13 @@ paged_join_kernel(const AttnArgs a)
             wild = wild || !(fabsf(y) <= 3.402823466e38f);
             if (lane + 32 * i < D) out[lane + 32 * i] = from_float<T>(y);
         }
-        if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-            if (__any_sync(0xffffffffu, wild)) {
-                __syncwarp();
-                mend_row<T>(a, cut.x, cut.y, s, (int)row, tile_keys<ROWS>(a, s, cut.z));
-            }
+        if (__any_sync(0xffffffffu, wild)) {
+            __syncwarp();
+            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)row, tile_keys<ROWS>(a, s, cut.z));
         }
     }
 }
+
+int launch_paged_tc(int format, const AttnArgs &a, cudaStream_t st);
 
 }  // namespace hipgpt

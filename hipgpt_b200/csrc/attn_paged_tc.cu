@@ -1,0 +1,535 @@
+// Attention of new tokens over a paged cache on the tensor pipe (tcgen05 + TMEM): 16-bit activations with many rows a sequence, every cache format.
+//
+// A block takes 256 rows (two tiles of 128, a row a TMEM lane) of one sequence and head of the cache, so the keys and values that it fetches serve both; one block an SM, which
+// goes from one run of units of 128 keys to the next (attn_paged.cuh).  Roles:
+//   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: scores are read from TMEM twice, for their maximum and for P = exp2(s - m) goes over them
+//                    in bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
+//                    sums in fp32 do not care).  P V is summed in TMEM.
+//   warps 8-11       bring keys and values into shared memory in the layout of the operands, two tiles of each ahead: plain rows by cp.async, codes by way of registers, widened to
+//                    bf16.  e4m3's scales are powers of two and go into the values (exact); int8's multiply scores and probabilities.
+//   warp 12          issues the products.  Those of one tile run while the other's softmax does: P V of a tile, then Q K^T of its next, over the same columns of TMEM (products of one thread
+//                    run in the order of their issue, so a commit behind the second covers the first).
+// Bound: the special-function unit (16 exponentials a clock) and the tensor pipe alike at D = 128.
+// Every wait is bounded: on expiry the block raises a flag that cuts all later waits short, records a status code, skips its stores, lets what is on its way land,
+// frees its TMEM and returns.
+#include "attn_paged.cuh"
+#include "stream_workspace.hpp"
+
+#include <math.h>
+
+#include <type_traits>
+
+namespace hipgpt {
+
+extern StreamWorkspace g_paged_ws;
+
+namespace {
+
+constexpr int kRows = 256, kKeys = 128, kStages = 2;
+constexpr int kTables = 4;            // a tile's scales and pages are read until its scores have been: the products of the tile after the next say so
+constexpr int kSoft = 256, kProducers = 128, kThreads = kSoft + kProducers + 32;
+constexpr float kRescaleStep = 8.0f;
+constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
+
+__device__ int g_paged_status = 0;
+
+__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int site, volatile int *abort_flag)
+{
+    if (mbar_wait(bar, parity)) return true;
+    *abort_flag = 1;
+    atomicCAS(&g_paged_status, 0, site);
+    linger();
+    return false;
+}
+
+template <int DP>
+struct TcCfg {
+    static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2;
+    static constexpr size_t kBytes = 2 * (size_t)kQTile + 2 * kStages * (size_t)kTile + 1024;
+};
+
+template <int FMT, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_tc_kernel(const AttnArgs a, int expire)
+{
+    using C = TcCfg<DP>;
+    using T = __nv_bfloat16;
+    constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN, SCALED = FMT == HIPGPT_CACHE_INT8;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *q_s = base;                             // [tile][block of 64 columns][128 rows][128 B], swizzled
+    uint8_t *k_s = q_s + 2 * C::kQTile;              // [stage][block][128 keys][128 B], K-major operand
+    uint8_t *v_s = k_s + kStages * C::kTile;         // the same bytes, read as an N-major operand
+    __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys], vs_s[SCALED ? kTables : 1][kKeys];
+    __shared__ uint32_t there_s[kTables];            // whether each 16 keys of a tile have a page
+    __shared__ long long sums[kThreads / 32 + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&k_full[i], kProducers / 32);
+            mbar_init(&v_full[i], kProducers / 32);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_free[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 4);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    dependency_wait();
+    dependents_may_start();
+
+    // site codes in the status word: 1 keys landed, 2 values landed, 3 queries there, 4 scores ready, 5 probabilities written, 6 sums complete, 7 key stage free, 8 value stage free
+    bool seen = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        const int gone = abort_flag;
+        const bool done = mbar_test(bar, parity);
+        seen = !gone;
+        if (!gone && expires_now(expire, site)) {
+            abort_flag = 1;
+            atomicCAS(&g_paged_status, 0, site);
+            linger();
+            seen = false;
+        } else if (!gone && !done) {
+            seen = wait_slow(bar, parity, site, &abort_flag);
+        }
+    };
+    auto arrive = [&](uint64_t *bar) {
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    };
+
+    Run<kRows, kKeys, kThreads> run(a);
+    bool more = run.begin(sums);
+    // units of each of the two tiles of rows within the block's run of the tile: [from, to) cut to what the tile's rows see (the second has no rows where there are none)
+    auto units_of = [&](const Tile &w, int half) {
+        const long long rows = (long long)w.s.n * a.group, first = (long long)w.tile * kRows + 128 * half;
+        if (first >= rows) return 0;
+        const long long last = min(first + 128, rows) - 1;
+        const int u = max(1, (limit_of(a, w.s, (int)last) + kKeys - 1) / kKeys);
+        return max(min(w.to, u) - w.from, 0);
+    };
+
+    if (warp >= 8 && warp < 12) {
+        // ================= keys and values ======================================================================
+        const int pt = tid - kSoft, D = a.c.D;
+        uint32_t n = 0;                              // tiles of keys so far
+        for (; more; more = run.next()) {
+            const Tile w = run.at();
+            const int units = max(units_of(w, 0), units_of(w, 1)), keys = tile_keys<kRows>(a, w.s, w.tile);
+            for (int u = w.from; u < w.from + units; ++u, ++n) {
+                const int st = n % kStages;
+                const uint32_t ph = (n / kStages) & 1;
+                // pages of the tile's eight times sixteen keys
+                const int p0 = u * kKeys;
+                int page = -1;
+                if (lane < 8 && p0 + 16 * lane < keys) {
+                    page = __ldg(a.c.table + (size_t)w.b * a.c.most_pages + ((p0 + 16 * lane) >> a.c.shift));
+                    if (page >= a.c.pages) page = -1;
+                }
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 255u;
+                auto row_at = [&](int key) {         // the row in the cache, -1: none
+                    const int pg = __shfl_sync(0xffffffffu, page, key >> 4);
+                    return pg < 0 || p0 + key >= keys ? -1LL : ((((long long)pg * a.c.heads) + w.head) << a.c.shift) + ((p0 + key) & ((1 << a.c.shift) - 1));
+                };
+                if constexpr (!CODED) {
+                    constexpr int CH = DP / 8, PER = kProducers / CH;        // chunks of 16 bytes a key; keys at a time
+                    const int c = pt % CH, k0 = pt / CH;
+                    const int off = (c / 8) * (kKeys * 128) + sw128(k0, c % 8);
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
+                        uint8_t *dst = (which ? v_s : k_s) + st * C::kTile + off;
+                        const uint8_t *src = which ? a.c.v : a.c.k;
+#pragma unroll 8
+                        for (int i = 0; i < kKeys / PER; ++i) {
+                            const long long row = row_at(k0 + PER * i);
+                            const bool ok = row >= 0 && c * 8 < D && seen;
+                            cp_async16(dst + i * PER * 128, ok ? src + (row * D + c * 8) * 2 : src, ok);
+                        }
+                        cp_async_commit();
+                    }
+                    if (pt == 0) there_s[n % kTables] = there;
+                    cp_async_wait<1>();
+                    proxy_fence();
+                    arrive(&k_full[st]);
+                    cp_async_wait<0>();
+                    proxy_fence();
+                    arrive(&v_full[st]);
+                } else {
+                    constexpr int CH = DP / 16, PER = kProducers / CH, N = kKeys / PER;      // chunks of 16 codes a key; keys at a time; rounds
+                    const int c = pt % CH, k0 = pt / CH;
+                    uint4 raw[2][N];
+                    float scale[2][SCALED ? 1 : N];
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        const uint8_t *src = which ? a.c.v : a.c.k;
+                        const float *sc = which ? a.c.vs : a.c.ks;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const long long row = row_at(k0 + PER * i);
+                            raw[which][i] = make_uint4(0u, 0u, 0u, 0u);
+                            if (row >= 0 && c * 16 < D) raw[which][i] = __ldg(reinterpret_cast<const uint4 *>(src + row * D + c * 16));
+                            if constexpr (!SCALED) scale[which][i] = row >= 0 ? __ldg(sc + row) : 0.0f;
+                        }
+                        if constexpr (SCALED) {
+                            const long long row = row_at(pt);
+                            scale[which][0] = row >= 0 ? __ldg(sc + row) : 0.0f;
+                        }
+                    }
+                    // the two halves of a chunk's 32 bytes; where two threads of a row would meet in a bank, one takes them the other way round
+                    const int c0 = 2 * c, turn = DP == 128 ? c >> 2 : 0;
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
+                        uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const uint32_t in[4] = {raw[which][i].x, raw[which][i].y, raw[which][i].z, raw[which][i].w};
+                            uint32_t out[8];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                out[2 * x] = code_pair<FMT>(in[x], in[x], 0, 1);
+                                out[2 * x + 1] = code_pair<FMT>(in[x], in[x], 2, 3);
+                            }
+                            if constexpr (!SCALED) {
+                                const uint32_t s2 = pack_bf16(scale[which][i], scale[which][i]);
+#pragma unroll
+                                for (int x = 0; x < 8; ++x) out[x] = mul_bf16x2(out[x], s2);
+                            }
+                            const int key = k0 + PER * i;
+                            const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
+                            *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + turn) % 8)) = turn ? hi : lo;
+                            *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + 1 - turn) % 8)) = turn ? lo : hi;
+                        }
+                        if constexpr (SCALED) (which ? vs_s : ks_s)[n % kTables][pt] = which ? scale[which][0] : scale[which][0] * a.cscale;
+                        if (which == 0 && pt == 0) there_s[n % kTables] = there;
+                        proxy_fence();
+                        arrive(which ? &v_full[st] : &k_full[st]);
+                    }
+                }
+            }
+        }
+    } else if (warp == 12) {
+        // ================= the products =========================================================================
+        constexpr uint32_t idesc_qk = idesc_bf16(128, kKeys, 0), idesc_pv = idesc_bf16(128, DP, 1);
+        uint32_t n = 0, np[2] = {0, 0}, items = 0;   // tiles of keys, of probabilities; tiles of rows
+        for (; more; more = run.next(), ++items) {
+            const Tile w = run.at();
+            const int u[2] = {units_of(w, 0), units_of(w, 1)}, units = max(u[0], u[1]);
+            auto qk = [&](int half, int t) {
+                const int st = (n + t) % kStages;
+                const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2), dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint64_t off = (uint64_t)((k / 4) * (128 * 128 / 16) + (k % 4) * 2);
+                    if (elect_one()) mma_h_ss(tmem + kColS + half * 128, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
+                }
+                if (elect_one()) tc_commit(&s_full[half]);
+            };
+            auto pv = [&](int half, int t) {
+                const int st = (n + t) % kStages;
+                const uint64_t dv = make_desc(smem_u32(v_s + st * C::kTile), kKeys * 128, 1024, 2);
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                    if (elect_one()) mma_h_ts(tmem + kColO + half * 128, tmem + kColS + half * 128 + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
+            };
+            // the last of the two to read a stage gives it back
+            auto free_k = [&](int half, int t) { if (half == (t < u[1] ? 1 : 0) && elect_one()) tc_commit(&k_free[(n + t) % kStages]); };
+            auto free_v = [&](int half, int t) { if (half == (t < u[1] ? 1 : 0) && elect_one()) tc_commit(&v_free[(n + t) % kStages]); };
+            auto ph = [&](int t) { return ((n + t) / kStages) & 1u; };
+            for (int half = 0; half < 2; ++half) wait(&q_full[half], items & 1, 3);     // (both every time: a phase must not be passed over)
+            wait(&k_full[n % kStages], ph(0), 1);
+            tc_fence_after();
+            for (int half = 0; half < 2; ++half) {
+                if (u[half]) { qk(half, 0); free_k(half, 0); }
+                else if (elect_one()) tc_commit(&o_done[half]);      // (whoever has no units of this tile must not run ahead into the next)
+            }
+            for (int t = 0; t < units; ++t) {
+                if (t + 1 < units) wait(&k_full[(n + t + 1) % kStages], ph(t + 1), 1);
+                wait(&v_full[(n + t) % kStages], ph(t), 2);
+                for (int half = 0; half < 2; ++half) {
+                    if (t >= u[half]) continue;
+                    wait(&p_full[half], np[half]++ & 1, 5);
+                    tc_fence_after();
+                    pv(half, t);
+                    free_v(half, t);
+                    if (t + 1 < u[half]) { qk(half, t + 1); free_k(half, t + 1); }
+                    else if (elect_one()) tc_commit(&o_done[half]);
+                }
+            }
+            n += units;
+        }
+        __syncwarp();
+        if (abort_flag) linger();
+    } else {
+        // ================= softmax ===============================================================================
+        const int half = warp >> 2, quad = warp & 3, D = a.c.D;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t s_addr = tmem + kColS + half * 128 + lanes, o_addr = tmem + kColO + half * 128 + lanes;
+        uint32_t n = 0, ns = 0, no = 0;              // tiles of keys, of scores; tiles of rows
+        int4 cut = make_int4(0, 0, 0, -1);
+        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.q_stride * 2) | (uintptr_t)(a.out_stride * 2)) & 15) == 0;
+        for (; more; more = run.next()) {
+            const Tile w = run.at();
+            const long long rows = (long long)w.s.n * a.group;
+            const int r = half * 128 + quad * 32 + lane;                     // row of the block's tile
+            const long long row = (long long)w.tile * kRows + r;
+            const bool mine = row < rows;
+            const long long t = w.s.first + row / a.group;
+            const long long col = (long long)(w.head * a.group + (int)(row % a.group)) * D;
+            const int u0 = units_of(w, 0), u1 = units_of(w, 1), units = half ? u1 : u0;
+            const bool tile_there = (long long)w.tile * kRows + 128 * half < rows;
+            // ---- the row of Q ---------------------------------------------------------------------------------
+            if (tile_there) {
+                const T *src = static_cast<const T *>(a.q) + t * a.q_stride + col;
+                uint8_t *dst = q_s + half * C::kQTile;
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c) {
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (mine && c * 8 < D) {
+                        if (vec) {
+                            x = *reinterpret_cast<const uint4 *>(src + c * 8);
+                        } else {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] = __bfloat16_as_ushort(src[c * 8 + 2 * i]) | (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * i + 1]) << 16;
+                            x = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(dst + (c / 8) * (128 * 128) + sw128(quad * 32 + lane, c % 8)) = x;
+                }
+                proxy_fence();
+            }
+            arrive(&q_full[half]);
+            const int limit = mine ? limit_of(a, w.s, (int)row) : 0;
+            const long long wfirst = (long long)w.tile * kRows + half * 128 + quad * 32;
+            const int least_limit = wfirst < rows ? limit_of(a, w.s, (int)wfirst) : 1 << 30;       // (rows behind the last: their results are not looked at)
+            float m = -INFINITY, l = 0.0f;
+            for (int i = 0; i < units; ++i) {
+                const int st = (n + i) % kStages, tb = (n + i) % kTables, p0 = (w.from + i) * kKeys;
+                wait(&s_full[half], ns++ & 1, 4);
+                tc_fence_after();
+                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
+                const bool masked = p0 + kKeys > least_limit || there != 255u;
+                const float cscale = a.cscale;
+                // a pass over the scores: their maximum (STORE: P in their place, and its sum)
+                float mx = -INFINITY, part = 0.0f;
+                auto pass = [&](auto mask_c, auto store_c, float ref) {
+                    constexpr bool MASK = decltype(mask_c)::value, STORE = decltype(store_c)::value;
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    float top[2] = {-INFINITY, -INFINITY};
+                    const float2 nref = make_float2(-ref, -ref);
+#pragma unroll
+                    for (int ch = 0; ch < 4; ++ch) {
+                        float v[32];
+                        uint32_t pk[16];
+                        tmem_ld32(s_addr + ch * 32, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const int k = ch * 32 + c;
+                            float2 x = make_float2(v[c], v[c + 1]), f = make_float2(cscale, cscale);
+                            if constexpr (SCALED) f = *reinterpret_cast<const float2 *>(&ks_s[tb][k]);
+                            bool v0 = true, v1 = true;
+                            if constexpr (MASK) {
+                                const bool g = (there >> (k >> 4)) & 1;
+                                v0 = g && p0 + k < limit;
+                                v1 = g && p0 + k + 1 < limit;
+                            }
+                            if constexpr (!STORE) {
+                                if constexpr (SCALED) x = fmul2(x, f);       // (else the maximum is scaled)
+                                top[(c >> 1) & 1] = max3(top[(c >> 1) & 1], v0 ? x.x : -INFINITY, v1 ? x.y : -INFINITY);
+                            } else {
+                                x = ffma2(x, f, nref);
+                                float2 y = make_float2(ex2_approx(v0 ? x.x : -INFINITY), ex2_approx(v1 ? x.y : -INFINITY));
+                                sum[(c >> 1) & 1] = fadd2(sum[(c >> 1) & 1], y);
+                                if constexpr (SCALED) {
+                                    y = fmul2(y, *reinterpret_cast<const float2 *>(&vs_s[tb][k]));
+                                    if constexpr (MASK) {
+                                        y.x = v0 ? y.x : 0.0f;
+                                        y.y = v1 ? y.y : 0.0f;
+                                    }
+                                }
+                                pk[c / 2] = pack_bf16(y.x, y.y);
+                            }
+                        }
+                        if constexpr (STORE) tmem_st16_u32(s_addr + ch * 16, pk);       // (over scores that are read already)
+                    }
+                    if constexpr (!STORE) mx = SCALED ? fmaxf(top[0], top[1]) : fmaxf(top[0], top[1]) * cscale;
+                    else part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                };
+                using Yes = std::integral_constant<bool, true>;
+                using No = std::integral_constant<bool, false>;
+                if (masked) pass(Yes(), No(), 0.0f); else pass(No(), No(), 0.0f);
+                if (i == 0) {
+                    m = mx;
+                } else {
+                    const bool grow = m == -INFINITY ? mx > m : mx > m + kRescaleStep;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
+                        if (grow) m = mx;
+                        l *= alpha;
+                        // what was summed before has come: its products were issued before those of these scores
+#pragma unroll 1
+                        for (int hh = 0; hh < DP / 16; ++hh) {
+                            float x[16];
+                            tmem_ld16(o_addr + hh * 16, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) x[c] *= alpha;
+                            tmem_st16(o_addr + hh * 16, x);
+                        }
+                    }
+                }
+                if constexpr (SCALED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);     // the scales of the values
+                const float ref = m == -INFINITY ? 0.0f : m;
+                if (masked) pass(Yes(), Yes(), ref); else pass(No(), Yes(), ref);
+                l += part;
+                tmem_wait_st();
+                tc_fence_before();
+                arrive(&p_full[half]);
+            }
+            n += max(u0, u1);
+            // ---- the tile's end ---------------------------------------------------------------------------------
+            const int part = run.part();
+            if (part >= 0 && (part & 1)) cut = run.cut();
+            wait(&o_done[half], no++ & 1, 6);
+            tc_fence_after();
+            if (!tile_there) continue;
+            const bool store = mine && !abort_flag;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            float *dst = part < 0 ? nullptr : a.parts + (size_t)part * kRows * (DP + 2);
+            bool wild = false;
+            T *out = static_cast<T *>(a.out) + t * a.out_stride + col;
+#pragma unroll 1
+            for (int hh = 0; hh < DP / 16; ++hh) {
+                float x[16];
+                if (units > 0) {
+                    tmem_ld16(o_addr + hh * 16, x);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) x[c] = 0.0f;
+                }
+                if (dst) {
+                    if (store) {
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) *reinterpret_cast<float2 *>(dst + (size_t)r * DP + hh * 16 + c) = make_float2(x[c], x[c + 1]);
+                    }
+                } else {
+                    uint32_t y[8];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        x[c] = l == 0.0f ? 0.0f : x[c] * inv;
+                        wild = wild || !(fabsf(x[c]) <= 3.402823466e38f);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) y[c] = pack_bf16(x[2 * c], x[2 * c + 1]);
+                    if (store && hh * 16 < D) {
+                        if (vec) {
+                            *reinterpret_cast<uint4 *>(out + hh * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<uint4 *>(out + hh * 16 + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) out[hh * 16 + c] = __ushort_as_bfloat16((unsigned short)(y[c / 2] >> (c & 1) * 16));
+                        }
+                    }
+                }
+            }
+            if (dst) {
+                if (store) *reinterpret_cast<float2 *>(dst + (size_t)kRows * DP + 2 * r) = make_float2(m, l);
+            } else {
+                unsigned some = __ballot_sync(0xffffffffu, wild && store);
+                __syncwarp();
+                while (some) {
+                    const int who = __ffs((int)some) - 1;
+                    some &= some - 1;
+                    mend_row<T, FMT>(a, w.b, w.head, w.s, (int)(wfirst + who), tile_keys<kRows>(a, w.s, w.tile));
+                }
+            }
+            tc_fence_before();                       // (these columns are read before the next products write them)
+        }
+        if (tid == 0 && a.cuts) a.cuts[blockIdx.x] = cut;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && a.whole) a.whole[blockIdx.x] = !abort_flag;
+    tc_fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <int FMT, int DP>
+int launch_tc(AttnArgs a, cudaStream_t st)
+{
+    using C = TcCfg<DP>;
+    const auto kern = paged_tc_kernel<FMT, DP>;
+    // more than half of an SM's shared memory: one block an SM, for its TMEM
+    constexpr size_t smem = C::kBytes > 120 * 1024 ? C::kBytes : 120 * 1024;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    static std::atomic<unsigned long long> done{0};
+    if (e == cudaSuccess) e = once_per_device(done, dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
+    const long long room = (long long)a.c.most_pages << a.c.shift;
+    const long long most = (room + kKeys - 1) / kKeys > 1 ? (room + kKeys - 1) / kKeys : 1;
+    const long long tiles = ((long long)a.c.T * a.group / kRows + (a.c.T < a.c.B ? a.c.T : a.c.B)) * a.c.heads;
+    int grid = sms;
+    a.least = 1;
+    if (tiles < (1LL << 40) / most && tiles * most < grid) grid = (int)(tiles * most);
+    const bool cuts = most > 1;
+    StreamWorkspace::Lease ws;
+    if (cuts) {
+        const size_t parts = (size_t)2 * grid * kRows * (DP + 2) * sizeof(float);
+        const int rc = g_paged_ws.enter(st, parts + (size_t)grid * (sizeof(int4) + sizeof(int)), &ws);
+        if (rc != HIPGPT_OK) return rc;
+        a.parts = reinterpret_cast<float *>(ws.get());
+        a.cuts = reinterpret_cast<int4 *>(ws.get() + parts);
+        a.whole = reinterpret_cast<int *>(a.cuts + grid);
+    }
+    e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, a, take_expiry(1000));
+    if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<__nv_bfloat16, FMT, kRows, DP>, dim3((unsigned)grid, 4), dim3(256), 0, st, a);
+    return e == cudaSuccess ? check_launch("paged_tc_kernel") : fail(HIPGPT_ERR_CUDA, "paged_tc_kernel: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+
+int launch_paged_tc(int format, const AttnArgs &a, cudaStream_t st)
+{
+    const bool narrow = a.c.D <= 64;
+    if (format == HIPGPT_CACHE_PLAIN) return narrow ? launch_tc<HIPGPT_CACHE_PLAIN, 64>(a, st) : launch_tc<HIPGPT_CACHE_PLAIN, 128>(a, st);
+    if (format == HIPGPT_CACHE_E4M3) return narrow ? launch_tc<HIPGPT_CACHE_E4M3, 64>(a, st) : launch_tc<HIPGPT_CACHE_E4M3, 128>(a, st);
+    return narrow ? launch_tc<HIPGPT_CACHE_INT8, 64>(a, st) : launch_tc<HIPGPT_CACHE_INT8, 128>(a, st);
+}
+
+int paged_status_fetch(int *status)
+{
+    int s = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&s, g_paged_status, sizeof(int));
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
+    if (s != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_paged_status, &zero, sizeof(int));
+    }
+    *status = s;
+    return HIPGPT_OK;
+}
+
+}  // namespace hipgpt

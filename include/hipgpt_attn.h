@@ -488,8 +488,8 @@ HIPGPT_API int hipgpt_probe_fma(float *d_sink, int blocks, int iters, double *fl
  * waits on hardware barriers are bounded; a block whose wait runs out stores nothing and records
  * which wait it was: 1..8 for the split-TF32 kernel, 100 + site for the bf16 kernel, 300 + site
  * for the tiled fp32 kernel, 400 + site for the whole-head kernel, 500 + site for the tensor-core projections,
- * 600 + site for the attention backward, 700 + site for the loss, 801 for the embedding's gradient, 900 + site for the test hook
- * hipgpt_debug_wait_expiry.  This call waits for the whole
+ * 600 + site for the attention backward, 700 + site for the loss, 801 for the embedding's gradient, 1000 + site for
+ * attention over a paged cache, 900 + site for the test hook hipgpt_debug_wait_expiry.  This call waits for the whole
  * device (cudaDeviceSynchronize), stores the status word in *status and clears it.  0 means every
  * launch since the last call completed normally.  Callers of the device-pointer entry points
  * that need to know must poll this; hipgpt_mha_forward_host does it itself and returns
@@ -518,7 +518,7 @@ HIPGPT_API int hipgpt_set_full_range(int on);
  *       arrives, with a limit of `limit_cycles` SM cycles (at most 2^24, a few milliseconds).  Afterwards
  *       hipgpt_kernel_status() reports 907 and d_canary[0..n) is untouched.
  *   hipgpt_debug_expire_wait  in the calling thread's next call of a tensor-core projection (code 501 ... 504) or of a tensor-core
- *       backward (601 ... 627) or loss, forward or backward (701 ... 704), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
+ *       backward (601 ... 627) or loss, forward or backward (701 ... 704), or of attention of many rows over a paged cache (1001 ... 1008), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
  *       each of the call's launches that has it, if it has to wait at all.
  *   hipgpt_gpt_debug_stall_barrier  makes the NEXT hipgpt_gpt_generate call give up: in the persistent mode it starts with a
  *       grid-barrier counter that cannot complete, and every block gives up at its first barrier; by clusters the first block's

@@ -205,7 +205,8 @@ CHUNKS = [(100, 100), (1, 40), (0, 0), (64, 500), (7, 3), (33, 1031), (129, 129)
 @pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("heads,H,D,page", [(1, 1, 16, 16), (2, 8, 128, 64), (3, 3, 32, 16), (1, 20, 64, 128), (2, 2, 80, 32), (4, 8, 48, 1024)])
-@pytest.mark.parametrize("seqs", [DECODE, CHUNKS, [(3, 700), (2, 2)], [(700, 900)]], ids=["tokens", "chunks", "few", "long"])
+@pytest.mark.parametrize("seqs", [DECODE, CHUNKS, [(3, 700), (2, 2)], [(700, 900)], [(300, 8000), (129, 129), (40, 900), (33, 34), (1, 3000)]],
+                         ids=["tokens", "chunks", "few", "long", "far"])
 def test_attention(fmt, dtype, heads, H, D, page, seqs):
     batch = Batch(seqs, page, seed=D, before=1, behind=2)
     for causal in (True, False):
@@ -230,9 +231,10 @@ def test_attention_peaked_scaled_and_strided(dtype, fmt):
     assert torch.equal(wide[:, 2:2 + H * D], out.view(batch.T, -1)) and bool((wide[:, :2] == 2).all()) and bool((wide[:, 2 + H * D:] == 2).all())
 
 
+@pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("seqs", [[(1, 200), (40, 300)], [(4, 60), (3, 200)], [(300, 400)]])
-def test_what_a_row_does_not_see_does_not_matter(dtype, seqs):
+@pytest.mark.parametrize("seqs", [[(1, 200), (40, 300)], [(4, 60), (3, 200)], [(300, 400)], [(1, 2), (300, 5000)]])
+def test_what_a_row_does_not_see_does_not_matter(fmt, dtype, seqs):
     """NaN and infinities in keys and values of the sequence's later tokens: the rows before them are as they were without."""
     batch = Batch(seqs, 16, seed=3)
     heads, H, D = 2, 4, 32
@@ -243,9 +245,9 @@ def test_what_a_row_does_not_see_does_not_matter(dtype, seqs):
     def wild(name, x):
         x[page, 1, slot, 3] = float("nan") if name == "k" else float("inf")
     first = batch.first[-2]
-    _, _, out, want, bound, _ = _attend(batch, heads, H, D, dtype, "plain", wild=wild)
+    _, _, out, want, bound, _ = _attend(batch, heads, H, D, dtype, fmt, wild=wild)
     clean = torch.ones(batch.T, H, dtype=torch.bool, device="cuda")
-    clean[first + n - 2:, 2:] = False
+    clean[first + n - 2:, H // heads:] = False
     within(out[clean], want[clean], bound[clean], "rows that do not see it")
     assert not bool(torch.isfinite(out[~clean]).all(-1).any()), "rows that do"
 
@@ -434,3 +436,25 @@ def test_through_ctypes(monkeypatch):
         results.append((turned, *back, o))
         monkeypatch.setattr(launchers, "_native", launchers._ThroughCtypes)
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("fmt", ["plain", "int8"])
+@pytest.mark.parametrize("code,block", [(1001, 0), (1002, 3), (1003, 1), (1004, 2), (1005, 0), (1006, 5), (1007, 4), (1008, 1)])
+def test_an_expired_wait_stores_no_part_of_a_value(fmt, code, block):
+    """Every row of the result is as ever, or nothing was stored there; the next call is as ever."""
+    batch = Batch([(300, 8000), (129, 129), (40, 900)], 64, seed=3)          # five units of 128 keys a block
+    cache, q, out, want, bound, mine = _attend(batch, 2, 8, 128, BF16, fmt)
+    within(out, want, bound)
+    for _ in range(20):
+        got = torch.full_like(out, -7.0)
+        _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
+        serving.paged_attention(cache, q, got, *batch.args, 8)
+        torch.cuda.synchronize()
+        status = _status()
+        if status:
+            break
+    assert status == code and _status() == 0
+    same, left = (got == out).all(-1), (got == -7.0).all(-1)
+    assert bool((same | left).all()) and bool(left.any()) and bool(same.any())
+    serving.paged_attention(cache, q, got, *batch.args, 8)
+    assert torch.equal(got, out)
