@@ -536,7 +536,7 @@ int launch_paged(int format, const AttnArgs &a, cudaStream_t st)
 {
     const bool few = (long long)a.c.T * a.group <= 32LL * a.c.B;
     if constexpr (sizeof(T) == 2) {
-        if (!few) return launch_paged_tc(format, a, st);
+        if (!few && a.c.pages > 0) return launch_paged_tc(format, a, st);          // (without pages there is nothing to copy)
         return format == HIPGPT_CACHE_PLAIN ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st)
              : format == HIPGPT_CACHE_E4M3  ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st);
     } else {

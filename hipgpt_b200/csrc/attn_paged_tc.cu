@@ -5,15 +5,19 @@
 //   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: scores are read from TMEM twice, for their maximum and for P = exp2(s - m) goes over them
 //                    in bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
 //                    sums in fp32 do not care).  P V is summed in TMEM.
-//   warps 8-11       bring keys and values into shared memory in the layout of the operands, two tiles of each ahead: plain rows by cp.async, codes by way of registers, widened to
-//                    bf16.  e4m3's scales are powers of two and go into the values (exact); int8's multiply scores and probabilities.
+//   warps 8-11       codes: widen them to bf16 in the layout of the operands, two tiles of keys and of values ahead.  e4m3's scales are powers of two and go into
+//                    the values (exact); int8's multiply scores and probabilities.  Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
 //   warp 12          issues the products.  Those of one tile run while the other's softmax does: P V of a tile, then Q K^T of its next, over the same columns of TMEM (products of one thread
 //                    run in the order of their issue, so a commit behind the second covers the first).
+//   warp 13          asks for the copies, a lane a run of keys in one page: boxes of 64 columns, swizzled, straight into the operands (plain; a page that is none lies
+//                    outside the tensor and comes as zeros), or codes and scales as they lie into a ring of half tiles.  (Loads by the threads themselves, 16 KB on their way, brought
+//                    6 bytes a clock; bulk copies bring 24.)
 // Bound: the special-function unit (16 exponentials a clock) and the tensor pipe alike at D = 128.
 // Every wait is bounded: on expiry the block raises a flag that cuts all later waits short, records a status code, skips its stores, lets what is on its way land,
 // frees its TMEM and returns.
 #include "attn_paged.cuh"
 #include "stream_workspace.hpp"
+#include "tma_host.cuh"
 
 #include <math.h>
 
@@ -27,7 +31,8 @@ namespace {
 
 constexpr int kRows = 256, kKeys = 128, kStages = 2;
 constexpr int kTables = 4;            // a tile's scales and pages are read until its scores have been: the products of the tile after the next say so
-constexpr int kSoft = 256, kProducers = 128, kThreads = kSoft + kProducers + 32;
+constexpr int kSoft = 256, kWideners = 128, kThreads = kSoft + kWideners + 64;
+constexpr int kHalf = 64, kSlots = 3;  // keys of a half tile of codes, half tiles in the ring
 constexpr float kRescaleStep = 8.0f;
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
 
@@ -42,17 +47,17 @@ __device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int site,
     return false;
 }
 
-template <int DP>
+template <int FMT, int DP>
 struct TcCfg {
-    static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2;
-    static constexpr size_t kBytes = 2 * (size_t)kQTile + 2 * kStages * (size_t)kTile + 1024;
+    static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2, kSlot = kHalf * DP;
+    static constexpr size_t kBytes = 2 * (size_t)kQTile + 2 * kStages * (size_t)kTile + (FMT == HIPGPT_CACHE_PLAIN ? 0 : kSlots * (size_t)kSlot) + 1024;
 };
 
 template <int FMT, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_tc_kernel(const AttnArgs a, int expire)
+paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a, int expire)
 {
-    using C = TcCfg<DP>;
+    using C = TcCfg<FMT, DP>;
     using T = __nv_bfloat16;
     constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN, SCALED = FMT == HIPGPT_CACHE_INT8;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -60,7 +65,10 @@ paged_tc_kernel(const AttnArgs a, int expire)
     uint8_t *q_s = base;                             // [tile][block of 64 columns][128 rows][128 B], swizzled
     uint8_t *k_s = q_s + 2 * C::kQTile;              // [stage][block][128 keys][128 B], K-major operand
     uint8_t *v_s = k_s + kStages * C::kTile;         // the same bytes, read as an N-major operand
+    uint8_t *raw_s = v_s + kStages * C::kTile;       // [slot][64 keys][D] codes as they lie in their pages
     __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2], o_done[2];
+    __shared__ uint64_t landed[CODED ? kSlots : kStages], raw_free[kSlots];
+    __shared__ __align__(16) float scale_s[CODED ? kSlots : 1][kHalf];
     __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys], vs_s[SCALED ? kTables : 1][kKeys];
     __shared__ uint32_t there_s[kTables];            // whether each 16 keys of a tile have a page
     __shared__ long long sums[kThreads / 32 + 2];
@@ -72,8 +80,8 @@ paged_tc_kernel(const AttnArgs a, int expire)
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&k_full[i], kProducers / 32);
-            mbar_init(&v_full[i], kProducers / 32);
+            mbar_init(&k_full[i], CODED ? kWideners / 32 : 1);
+            mbar_init(&v_full[i], CODED ? kWideners / 32 : 1);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_free[i], 1);
         }
@@ -83,6 +91,8 @@ paged_tc_kernel(const AttnArgs a, int expire)
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
+        for (int i = 0; i < (CODED ? kSlots : kStages); ++i) mbar_init(&landed[i], 1);
+        for (int i = 0; i < kSlots; ++i) mbar_init(&raw_free[i], kWideners / 32);
     }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
@@ -95,7 +105,8 @@ paged_tc_kernel(const AttnArgs a, int expire)
     dependency_wait();
     dependents_may_start();
 
-    // site codes in the status word: 1 keys landed, 2 values landed, 3 queries there, 4 scores ready, 5 probabilities written, 6 sums complete, 7 key stage free, 8 value stage free
+    // site codes in the status word: 1 keys landed, 2 values landed, 3 queries there, 4 scores ready, 5 probabilities written, 6 sums complete, 7 key stage free, 8 value stage free, 9 copies landed,
+    // 10 half tile free
     bool seen = true;
     auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
         const int gone = abort_flag;
@@ -126,82 +137,120 @@ paged_tc_kernel(const AttnArgs a, int expire)
         return max(min(w.to, u) - w.from, 0);
     };
 
-    if (warp >= 8 && warp < 12) {
-        // ================= keys and values ======================================================================
+    if (warp == 13) {
+        // ================= the copies ============================================================================
+        uint32_t n = 0, slot = 0;                    // tiles of keys so far; half tiles of codes
+        const int page_keys = 1 << a.c.shift, D = a.c.D;
+        for (; more; more = run.next()) {
+            const Tile w = run.at();
+            const int units = max(units_of(w, 0), units_of(w, 1)), keys = tile_keys<kRows>(a, w.s, w.tile);
+            // the pages of a tile's eight times sixteen keys, a lane each; asked for a tile ahead
+            auto look = [&](int u) {
+                const int p = u * kKeys + 16 * lane;
+                const int pg = lane < 8 && p < keys ? __ldg(a.c.table + (size_t)w.b * a.c.most_pages + (p >> a.c.shift)) : -1;
+                return pg < a.c.pages ? pg : -1;
+            };
+            int page = look(w.from);
+            for (int u = w.from; u < w.from + units; ++u, ++n) {
+                const int st = n % kStages, p0 = u * kKeys;
+                const uint32_t ph = (n / kStages) & 1;
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 255u;
+                const int next_page = u + 1 < w.from + units ? look(u + 1) : -1;
+                if (lane == 0) there_s[n % kTables] = there;         // (before the arrivals below)
+                if constexpr (!CODED) {
+                    constexpr int NB = DP / 64;
+                    const int run_keys = min(page_keys, kKeys), runs = kKeys / run_keys;
+                    const int at = lane / NB * run_keys, x = lane % NB * 64;                    // this lane's box
+                    const int pg = __shfl_sync(0xffffffffu, page, (at >> 4) & 7);
+                    const int z = pg < 0 ? a.c.pages * a.c.heads : pg * a.c.heads + w.head;
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
+                        uint64_t *bar = which ? &landed[st] : &k_full[st];
+                        __syncwarp();
+                        if (lane == 0 && seen) mbar_arrive_expect_tx(bar, (uint32_t)C::kTile);
+                        __syncwarp();
+                        if (lane < runs * NB && seen)
+                            tma_load_3d((which ? v_s : k_s) + st * C::kTile + (x / 64) * (kKeys * 128) + at * 128, which ? &vmap : &kmap, x, (p0 + at) & (page_keys - 1), z, bar);
+                    }
+                } else {
+                    const int run_keys = min(page_keys, kHalf), runs = kHalf / run_keys;
+#pragma unroll
+                    for (int part = 0; part < 4; ++part, slot = slot + 1) {
+                        const int which = part >> 1, sl = slot % kSlots, at = (part & 1) * kHalf + lane * run_keys;
+                        const int pg = __shfl_sync(0xffffffffu, page, (at >> 4) & 7);
+                        const int count = lane < runs && pg >= 0 ? min(run_keys, keys - (p0 + at)) : 0;             // (a page that is none lies behind the last key)
+                        const int scales = (count + 3) & ~3;         // whole 16 bytes, within the page
+                        int bytes = count * D + scales * 4;
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);             // (runs are four at most)
+                        if (slot >= kSlots) wait(&raw_free[sl], ((slot / kSlots) & 1) ^ 1, 10);
+                        __syncwarp();
+                        if (lane == 0 && seen) mbar_arrive_expect_tx(&landed[sl], (uint32_t)bytes);
+                        __syncwarp();
+                        if (count > 0 && seen) {
+                            const long long row = ((((long long)pg * a.c.heads) + w.head) << a.c.shift) + ((p0 + at) & (page_keys - 1));
+                            bulk_load(raw_s + sl * C::kSlot + lane * run_keys * D, (which ? a.c.v : a.c.k) + row * D, (uint32_t)(count * D), &landed[sl]);
+                            bulk_load(&scale_s[sl][lane * run_keys], (which ? a.c.vs : a.c.ks) + row, (uint32_t)(scales * 4), &landed[sl]);
+                        }
+                    }
+                }
+                page = next_page;
+            }
+        }
+        __syncwarp();
+        if (abort_flag) linger();
+    } else if (warp >= 8 && warp < 12) {
+        // ================= codes to operands; rows behind the last key ===========================================
         const int pt = tid - kSoft, D = a.c.D;
-        uint32_t n = 0;                              // tiles of keys so far
+        uint32_t n = 0, slot = 0;
+        if constexpr (!CODED) more = more && warp == 8;
         for (; more; more = run.next()) {
             const Tile w = run.at();
             const int units = max(units_of(w, 0), units_of(w, 1)), keys = tile_keys<kRows>(a, w.s, w.tile);
             for (int u = w.from; u < w.from + units; ++u, ++n) {
-                const int st = n % kStages;
+                const int st = n % kStages, p0 = u * kKeys;
                 const uint32_t ph = (n / kStages) & 1;
-                // pages of the tile's eight times sixteen keys
-                const int p0 = u * kKeys;
-                int page = -1;
-                if (lane < 8 && p0 + 16 * lane < keys) {
-                    page = __ldg(a.c.table + (size_t)w.b * a.c.most_pages + ((p0 + 16 * lane) >> a.c.shift));
-                    if (page >= a.c.pages) page = -1;
-                }
-                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 255u;
-                auto row_at = [&](int key) {         // the row in the cache, -1: none
-                    const int pg = __shfl_sync(0xffffffffu, page, key >> 4);
-                    return pg < 0 || p0 + key >= keys ? -1LL : ((((long long)pg * a.c.heads) + w.head) << a.c.shift) + ((p0 + key) & ((1 << a.c.shift) - 1));
-                };
                 if constexpr (!CODED) {
-                    constexpr int CH = DP / 8, PER = kProducers / CH;        // chunks of 16 bytes a key; keys at a time
-                    const int c = pt % CH, k0 = pt / CH;
-                    const int off = (c / 8) * (kKeys * 128) + sw128(k0, c % 8);
+                    wait(&landed[st], ph, 9);
+                    const int first = keys - p0;
+                    if (first < kKeys) {
+                        for (int i = max(first, 0) * 8 + lane; i < kKeys * 8; i += 32)
 #pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
-                        uint8_t *dst = (which ? v_s : k_s) + st * C::kTile + off;
-                        const uint8_t *src = which ? a.c.v : a.c.k;
-#pragma unroll 8
-                        for (int i = 0; i < kKeys / PER; ++i) {
-                            const long long row = row_at(k0 + PER * i);
-                            const bool ok = row >= 0 && c * 8 < D && seen;
-                            cp_async16(dst + i * PER * 128, ok ? src + (row * D + c * 8) * 2 : src, ok);
-                        }
-                        cp_async_commit();
+                            for (int nb = 0; nb < DP / 64; ++nb) *reinterpret_cast<uint4 *>(v_s + st * C::kTile + nb * (kKeys * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        proxy_fence();
                     }
-                    if (pt == 0) there_s[n % kTables] = there;
-                    cp_async_wait<1>();
-                    proxy_fence();
-                    arrive(&k_full[st]);
-                    cp_async_wait<0>();
-                    proxy_fence();
                     arrive(&v_full[st]);
                 } else {
-                    constexpr int CH = DP / 16, PER = kProducers / CH, N = kKeys / PER;      // chunks of 16 codes a key; keys at a time; rounds
+                    constexpr int CH = DP / 16, PER = kWideners / CH, N = kHalf / PER;       // chunks of 16 codes a key; keys at a time; rounds
                     const int c = pt % CH, k0 = pt / CH;
-                    uint4 raw[2][N];
-                    float scale[2][SCALED ? 1 : N];
-#pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        const uint8_t *src = which ? a.c.v : a.c.k;
-                        const float *sc = which ? a.c.vs : a.c.ks;
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const long long row = row_at(k0 + PER * i);
-                            raw[which][i] = make_uint4(0u, 0u, 0u, 0u);
-                            if (row >= 0 && c * 16 < D) raw[which][i] = __ldg(reinterpret_cast<const uint4 *>(src + row * D + c * 16));
-                            if constexpr (!SCALED) scale[which][i] = row >= 0 ? __ldg(sc + row) : 0.0f;
-                        }
-                        if constexpr (SCALED) {
-                            const long long row = row_at(pt);
-                            scale[which][0] = row >= 0 ? __ldg(sc + row) : 0.0f;
-                        }
-                    }
                     // the two halves of a chunk's 32 bytes; where two threads of a row would meet in a bank, one takes them the other way round
                     const int c0 = 2 * c, turn = DP == 128 ? c >> 2 : 0;
-#pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
-                        uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128);
+                    uint32_t there = 0;
+#pragma unroll 1
+                    for (int part = 0; part < 4; ++part, ++slot) {
+                        const int which = part >> 1, sl = slot % kSlots, base_key = (part & 1) * kHalf;
+                        wait(&landed[sl], (slot / kSlots) & 1, 9);
+                        if (part == 0) there = *reinterpret_cast<volatile uint32_t *>(&there_s[n % kTables]);
+                        uint4 raw[N];
+                        float scale[SCALED ? 1 : N];
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
-                            const uint32_t in[4] = {raw[which][i].x, raw[which][i].y, raw[which][i].z, raw[which][i].w};
+                            const int key = k0 + PER * i, tile_key = base_key + key;
+                            const bool ok = p0 + tile_key < keys && (there >> (tile_key >> 4) & 1) && c * 16 < D;
+                            raw[i] = ok ? *reinterpret_cast<const uint4 *>(raw_s + sl * C::kSlot + key * D + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+                            if constexpr (!SCALED) scale[i] = ok ? scale_s[sl][key] : 0.0f;
+                        }
+                        if constexpr (SCALED) {
+                            const int tile_key = base_key + pt;
+                            scale[0] = pt < kHalf && p0 + tile_key < keys && (there >> (tile_key >> 4) & 1) ? scale_s[sl][pt] : 0.0f;
+                        }
+                        arrive(&raw_free[sl]);
+                        if (n >= kStages && (part & 1) == 0) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
+                        uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128) + base_key * 128;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                             uint32_t out[8];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
@@ -209,7 +258,7 @@ paged_tc_kernel(const AttnArgs a, int expire)
                                 out[2 * x + 1] = code_pair<FMT>(in[x], in[x], 2, 3);
                             }
                             if constexpr (!SCALED) {
-                                const uint32_t s2 = pack_bf16(scale[which][i], scale[which][i]);
+                                const uint32_t s2 = pack_bf16(scale[i], scale[i]);
 #pragma unroll
                                 for (int x = 0; x < 8; ++x) out[x] = mul_bf16x2(out[x], s2);
                             }
@@ -218,10 +267,12 @@ paged_tc_kernel(const AttnArgs a, int expire)
                             *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + turn) % 8)) = turn ? hi : lo;
                             *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + 1 - turn) % 8)) = turn ? lo : hi;
                         }
-                        if constexpr (SCALED) (which ? vs_s : ks_s)[n % kTables][pt] = which ? scale[which][0] : scale[which][0] * a.cscale;
-                        if (which == 0 && pt == 0) there_s[n % kTables] = there;
-                        proxy_fence();
-                        arrive(which ? &v_full[st] : &k_full[st]);
+                        if constexpr (SCALED)
+                            if (pt < kHalf) (which ? vs_s : ks_s)[n % kTables][base_key + pt] = which ? scale[0] : scale[0] * a.cscale;
+                        if (part & 1) {
+                            proxy_fence();
+                            arrive(which ? &v_full[st] : &k_full[st]);
+                        }
                     }
                 }
             }
@@ -262,7 +313,6 @@ paged_tc_kernel(const AttnArgs a, int expire)
                 else if (elect_one()) tc_commit(&o_done[half]);      // (whoever has no units of this tile must not run ahead into the next)
             }
             for (int t = 0; t < units; ++t) {
-                if (t + 1 < units) wait(&k_full[(n + t + 1) % kStages], ph(t + 1), 1);
                 wait(&v_full[(n + t) % kStages], ph(t), 2);
                 for (int half = 0; half < 2; ++half) {
                     if (t >= u[half]) continue;
@@ -270,8 +320,14 @@ paged_tc_kernel(const AttnArgs a, int expire)
                     tc_fence_after();
                     pv(half, t);
                     free_v(half, t);
-                    if (t + 1 < u[half]) { qk(half, t + 1); free_k(half, t + 1); }
-                    else if (elect_one()) tc_commit(&o_done[half]);
+                    if (t + 1 < u[half]) {
+                        if (half == (t + 1 < u[0] ? 0 : 1)) {                // (the first to need it)
+                            wait(&k_full[(n + t + 1) % kStages], ph(t + 1), 1);
+                            tc_fence_after();
+                        }
+                        qk(half, t + 1);
+                        free_k(half, t + 1);
+                    } else if (elect_one()) tc_commit(&o_done[half]);
                 }
             }
             n += units;
@@ -336,16 +392,17 @@ paged_tc_kernel(const AttnArgs a, int expire)
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                     float top[2] = {-INFINITY, -INFINITY};
                     const float2 nref = make_float2(-ref, -ref);
-#pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        float v[32];
-                        uint32_t pk[16];
-                        tmem_ld32(s_addr + ch * 32, v);
+#pragma unroll 1
+                    for (int ch = 0; ch < 2; ++ch) {
+                        float v[2][32];
+                        uint32_t pk[2][16];
+                        tmem_ld32(s_addr + ch * 64, v[0]);
+                        tmem_ld32(s_addr + ch * 64 + 32, v[1]);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const int k = ch * 32 + c;
-                            float2 x = make_float2(v[c], v[c + 1]), f = make_float2(cscale, cscale);
+                        for (int c = 0; c < 64; c += 2) {
+                            const int k = ch * 64 + c;
+                            float2 x = make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), f = make_float2(cscale, cscale);
                             if constexpr (SCALED) f = *reinterpret_cast<const float2 *>(&ks_s[tb][k]);
                             bool v0 = true, v1 = true;
                             if constexpr (MASK) {
@@ -367,10 +424,13 @@ paged_tc_kernel(const AttnArgs a, int expire)
                                         y.y = v1 ? y.y : 0.0f;
                                     }
                                 }
-                                pk[c / 2] = pack_bf16(y.x, y.y);
+                                pk[c / 32][c / 2 % 16] = pack_bf16(y.x, y.y);
                             }
                         }
-                        if constexpr (STORE) tmem_st16_u32(s_addr + ch * 16, pk);       // (over scores that are read already)
+                        if constexpr (STORE) {                       // (over scores that are read already)
+                            tmem_st16_u32(s_addr + ch * 32, pk[0]);
+                            tmem_st16_u32(s_addr + ch * 32 + 16, pk[1]);
+                        }
                     }
                     if constexpr (!STORE) mx = SCALED ? fmaxf(top[0], top[1]) : fmaxf(top[0], top[1]) * cscale;
                     else part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -475,10 +535,27 @@ paged_tc_kernel(const AttnArgs a, int expire)
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
+// Rank-3 map {D, page size, pages * heads} over the rows of a plain 16-bit cache; a box is [1][keys of one page, 128 at most][64 values] = rows of 128 bytes, 128-byte swizzled.  What is
+// outside (values from D on, a page that is none) comes as zeros.
+int page_map(CUtensorMap *m, const void *rows, const PagedView &c)
+{
+    EncodeTiledFn enc = tma_encode_fn();
+    if (!enc) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t size = 1ull << c.shift;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.D, size, (cuuint64_t)c.pages * c.heads};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, size * c.D * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(size < kKeys ? size : kKeys), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(rows), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return HIPGPT_OK;
+}
+
 template <int FMT, int DP>
 int launch_tc(AttnArgs a, cudaStream_t st)
 {
-    using C = TcCfg<DP>;
+    using C = TcCfg<FMT, DP>;
     const auto kern = paged_tc_kernel<FMT, DP>;
     // more than half of an SM's shared memory: one block an SM, for its TMEM
     constexpr size_t smem = C::kBytes > 120 * 1024 ? C::kBytes : 120 * 1024;
@@ -504,7 +581,13 @@ int launch_tc(AttnArgs a, cudaStream_t st)
         a.cuts = reinterpret_cast<int4 *>(ws.get() + parts);
         a.whole = reinterpret_cast<int *>(a.cuts + grid);
     }
-    e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, a, take_expiry(1000));
+    CUtensorMap kmap = {}, vmap = {};
+    if (FMT == HIPGPT_CACHE_PLAIN) {
+        int rc = page_map(&kmap, a.c.k, a.c);
+        if (rc == HIPGPT_OK) rc = page_map(&vmap, a.c.v, a.c);
+        if (rc != HIPGPT_OK) return rc;
+    }
+    e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, kmap, vmap, a, take_expiry(1000));
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<__nv_bfloat16, FMT, kRows, DP>, dim3((unsigned)grid, 4), dim3(256), 0, st, a);
     return e == cudaSuccess ? check_launch("paged_tc_kernel") : fail(HIPGPT_ERR_CUDA, "paged_tc_kernel: %s", cudaGetErrorString(e));
 }

@@ -439,12 +439,14 @@ def test_through_ctypes(monkeypatch):
 
 
 @pytest.mark.parametrize("fmt", ["plain", "int8"])
-@pytest.mark.parametrize("code,block", [(1001, 0), (1002, 3), (1003, 1), (1004, 2), (1005, 0), (1006, 5), (1007, 4), (1008, 1)])
+@pytest.mark.parametrize("code,block", [(1001, 0), (1002, 3), (1003, 1), (1004, 2), (1005, 0), (1006, 5), (1007, 4), (1008, 1), (1009, 6), (1010, 2)])
 def test_an_expired_wait_stores_no_part_of_a_value(fmt, code, block):
     """Every row of the result is as ever, or nothing was stored there; the next call is as ever."""
     batch = Batch([(300, 8000), (129, 129), (40, 900)], 64, seed=3)          # five units of 128 keys a block
     cache, q, out, want, bound, mine = _attend(batch, 2, 8, 128, BF16, fmt)
     within(out, want, bound)
+    if code == 1010 and fmt == "plain":
+        pytest.skip("plain rows have no ring")
     for _ in range(20):
         got = torch.full_like(out, -7.0)
         _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
