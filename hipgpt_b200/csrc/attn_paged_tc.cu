@@ -2,8 +2,8 @@
 //
 // A block takes 256 rows (two tiles of 128, a row a TMEM lane) of one sequence and head of the cache, so the keys and values that it fetches serve both; one block an SM, which
 // goes from one run of units of 128 keys to the next (attn_paged.cuh).  Roles:
-//   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: scores are read from TMEM twice, for their maximum and for P = exp2(s - m) goes over them
-//                    in bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
+//   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: its scores are read from TMEM into registers, P = exp2(s - m) goes over them in
+//                    bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
 //                    sums in fp32 do not care).  P V is summed in TMEM.
 //   warps 8-11       codes: widen them to bf16 in the layout of the operands, two tiles of keys and of values ahead.  e4m3's scales are powers of two and go into
 //                    the values (exact); int8's multiply scores and probabilities.  Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
@@ -21,8 +21,6 @@
 
 #include <math.h>
 
-#include <type_traits>
-
 namespace hipgpt {
 
 extern StreamWorkspace g_paged_ws;
@@ -31,14 +29,17 @@ namespace {
 
 constexpr int kRows = 256, kKeys = 128, kStages = 2;
 constexpr int kTables = 4;            // a tile's scales and pages are read until its scores have been: the products of the tile after the next say so
-constexpr int kSoft = 256, kWideners = 128, kThreads = kSoft + kWideners + 64;
+constexpr int kSoft = 256, kWideners = 128, kThreads = 512;
+// Registers a thread of each warpgroup: 128 at launch; 184 + 184 + 88 + 56 = 4 x 128
+constexpr int kSoftRegs = 184, kWidenRegs = 88, kIssueRegs = 56;
 constexpr int kHalf = 64, kSlots = 3;  // keys of a half tile of codes, half tiles in the ring
 constexpr float kRescaleStep = 8.0f;
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
 
 __device__ int g_paged_status = 0;
 
-__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int site, volatile int *abort_flag)
+// (in line: with calls inside them the roles' registers cannot be shared out)
+__device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int site, volatile int *abort_flag)
 {
     if (mbar_wait(bar, parity)) return true;
     *abort_flag = 1;
@@ -101,7 +102,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = 0;                         // all 512 columns are this block's
     dependency_wait();
     dependents_may_start();
 
@@ -137,7 +138,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         return max(min(w.to, u) - w.from, 0);
     };
 
-    if (warp == 13) {
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        more = more && warp < 14;                    // (registers are given back by whole warpgroups)
+    }
+    if (warp >= 13) {
         // ================= the copies ============================================================================
         uint32_t n = 0, slot = 0;                    // tiles of keys so far; half tiles of codes
         const int page_keys = 1 << a.c.shift, D = a.c.D;
@@ -201,6 +206,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         __syncwarp();
         if (abort_flag) linger();
     } else if (warp >= 8 && warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
         // ================= codes to operands; rows behind the last key ===========================================
         const int pt = tid - kSoft, D = a.c.D;
         uint32_t n = 0, slot = 0;
@@ -245,7 +251,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             const int tile_key = base_key + pt;
                             scale[0] = pt < kHalf && p0 + tile_key < keys && (there >> (tile_key >> 4) & 1) ? scale_s[sl][pt] : 0.0f;
                         }
-                        arrive(&raw_free[sl]);
                         if (n >= kStages && (part & 1) == 0) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
                         uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128) + base_key * 128;
 #pragma unroll
@@ -269,6 +274,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
                         if constexpr (SCALED)
                             if (pt < kHalf) (which ? vs_s : ks_s)[n % kTables][base_key + pt] = which ? scale[0] : scale[0] * a.cscale;
+                        arrive(&raw_free[sl]);       // (not before the codes have been used: an arrival does not wait for loads)
                         if (part & 1) {
                             proxy_fence();
                             arrive(which ? &v_full[st] : &k_full[st]);
@@ -283,23 +289,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         uint32_t n = 0, np[2] = {0, 0}, items = 0;   // tiles of keys, of probabilities; tiles of rows
         for (; more; more = run.next(), ++items) {
             const Tile w = run.at();
-            const int u[2] = {units_of(w, 0), units_of(w, 1)}, units = max(u[0], u[1]);
+            // (read from one lane: every address below is then known to be the warp's, not a lane's)
+            const int u[2] = {__shfl_sync(0xffffffffu, units_of(w, 0), 0), __shfl_sync(0xffffffffu, units_of(w, 1), 0)}, units = max(u[0], u[1]);
             auto qk = [&](int half, int t) {
                 const int st = (n + t) % kStages;
                 const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2), dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint64_t off = (uint64_t)((k / 4) * (128 * 128 / 16) + (k % 4) * 2);
-                    if (elect_one()) mma_h_ss(tmem + kColS + half * 128, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint64_t off = (uint64_t)((k / 4) * (128 * 128 / 16) + (k % 4) * 2);
+                        mma_h_ss(tmem + kColS + half * 128, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
+                    }
+                    tc_commit(&s_full[half]);
                 }
-                if (elect_one()) tc_commit(&s_full[half]);
             };
             auto pv = [&](int half, int t) {
                 const int st = (n + t) % kStages;
                 const uint64_t dv = make_desc(smem_u32(v_s + st * C::kTile), kKeys * 128, 1024, 2);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    if (elect_one()) mma_h_ts(tmem + kColO + half * 128, tmem + kColS + half * 128 + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        mma_h_ts(tmem + kColO + half * 128, tmem + kColS + half * 128 + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
+                }
             };
             // the last of the two to read a stage gives it back
             auto free_k = [&](int half, int t) { if (half == (t < u[1] ? 1 : 0) && elect_one()) tc_commit(&k_free[(n + t) % kStages]); };
@@ -336,6 +347,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (abort_flag) linger();
     } else {
         // ================= softmax ===============================================================================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int half = warp >> 2, quad = warp & 3, D = a.c.D;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + kColS + half * 128 + lanes, o_addr = tmem + kColO + half * 128 + lanes;
@@ -384,60 +396,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 tc_fence_after();
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
                 const bool masked = p0 + kKeys > least_limit || there != 255u;
-                const float cscale = a.cscale;
-                // a pass over the scores: their maximum (STORE: P in their place, and its sum)
-                float mx = -INFINITY, part = 0.0f;
-                auto pass = [&](auto mask_c, auto store_c, float ref) {
-                    constexpr bool MASK = decltype(mask_c)::value, STORE = decltype(store_c)::value;
-                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    float top[2] = {-INFINITY, -INFINITY};
-                    const float2 nref = make_float2(-ref, -ref);
-#pragma unroll 1
-                    for (int ch = 0; ch < 2; ++ch) {
-                        float v[2][32];
-                        uint32_t pk[2][16];
-                        tmem_ld32(s_addr + ch * 64, v[0]);
-                        tmem_ld32(s_addr + ch * 64 + 32, v[1]);
-                        tmem_wait_ld();
+                float v[4][32];
 #pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const int k = ch * 64 + c;
-                            float2 x = make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), f = make_float2(cscale, cscale);
-                            if constexpr (SCALED) f = *reinterpret_cast<const float2 *>(&ks_s[tb][k]);
-                            bool v0 = true, v1 = true;
-                            if constexpr (MASK) {
-                                const bool g = (there >> (k >> 4)) & 1;
-                                v0 = g && p0 + k < limit;
-                                v1 = g && p0 + k + 1 < limit;
-                            }
-                            if constexpr (!STORE) {
-                                if constexpr (SCALED) x = fmul2(x, f);       // (else the maximum is scaled)
-                                top[(c >> 1) & 1] = max3(top[(c >> 1) & 1], v0 ? x.x : -INFINITY, v1 ? x.y : -INFINITY);
-                            } else {
-                                x = ffma2(x, f, nref);
-                                float2 y = make_float2(ex2_approx(v0 ? x.x : -INFINITY), ex2_approx(v1 ? x.y : -INFINITY));
-                                sum[(c >> 1) & 1] = fadd2(sum[(c >> 1) & 1], y);
-                                if constexpr (SCALED) {
-                                    y = fmul2(y, *reinterpret_cast<const float2 *>(&vs_s[tb][k]));
-                                    if constexpr (MASK) {
-                                        y.x = v0 ? y.x : 0.0f;
-                                        y.y = v1 ? y.y : 0.0f;
-                                    }
-                                }
-                                pk[c / 32][c / 2 % 16] = pack_bf16(y.x, y.y);
-                            }
-                        }
-                        if constexpr (STORE) {                       // (over scores that are read already)
-                            tmem_st16_u32(s_addr + ch * 32, pk[0]);
-                            tmem_st16_u32(s_addr + ch * 32 + 16, pk[1]);
-                        }
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
+                tmem_wait_ld();
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int c = 0; c < kKeys; c += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(&ks_s[tb][c]);
+                        const float2 lo = fmul2(make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), make_float2(f.x, f.y));
+                        const float2 hi = fmul2(make_float2(v[c / 32][c % 32 + 2], v[c / 32][c % 32 + 3]), make_float2(f.z, f.w));
+                        v[c / 32][c % 32] = lo.x; v[c / 32][c % 32 + 1] = lo.y; v[c / 32][c % 32 + 2] = hi.x; v[c / 32][c % 32 + 3] = hi.y;
                     }
-                    if constexpr (!STORE) mx = SCALED ? fmaxf(top[0], top[1]) : fmaxf(top[0], top[1]) * cscale;
-                    else part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                };
-                using Yes = std::integral_constant<bool, true>;
-                using No = std::integral_constant<bool, false>;
-                if (masked) pass(Yes(), No(), 0.0f); else pass(No(), No(), 0.0f);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < kKeys; ++c) v[c / 32][c % 32] = p0 + c < limit && (there >> (c >> 4) & 1) ? v[c / 32][c % 32] : -INFINITY;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < kKeys; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], v[c / 32][c % 32], v[c / 32][c % 32 + 1]);
+                const float factor = SCALED ? 1.0f : a.cscale;               // (int8: among the scales)
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
                 if (i == 0) {
                     m = mx;
                 } else {
@@ -458,10 +438,40 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
                     }
                 }
-                if constexpr (SCALED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);     // the scales of the values
                 const float ref = m == -INFINITY ? 0.0f : m;
-                if (masked) pass(Yes(), Yes(), ref); else pass(No(), Yes(), ref);
-                l += part;
+                const float2 f2 = make_float2(factor, factor), nref = make_float2(-ref, -ref);
+                if constexpr (SCALED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);     // the scales of the values
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        float2 y[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float2 s2 = make_float2(v[q][c + 2 * e], v[q][c + 2 * e + 1]), x = SCALED ? fadd2(s2, nref) : ffma2(s2, f2, nref);
+                            y[e] = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                            sum[e] = fadd2(sum[e], y[e]);
+                        }
+                        if constexpr (SCALED) {
+                            // (a row that must not see a value does not see its scale either)
+                            const float4 f = *reinterpret_cast<const float4 *>(&vs_s[tb][q * 32 + c]);
+                            y[0] = fmul2(y[0], make_float2(f.x, f.y));
+                            y[1] = fmul2(y[1], make_float2(f.z, f.w));
+                            if (masked) {
+                                y[0].x = v[q][c] == -INFINITY ? 0.0f : y[0].x;
+                                y[0].y = v[q][c + 1] == -INFINITY ? 0.0f : y[0].y;
+                                y[1].x = v[q][c + 2] == -INFINITY ? 0.0f : y[1].x;
+                                y[1].y = v[q][c + 3] == -INFINITY ? 0.0f : y[1].y;
+                            }
+                        }
+                        pk[c / 2] = pack_bf16(y[0].x, y[0].y);
+                        pk[c / 2 + 1] = pack_bf16(y[1].x, y[1].y);
+                    }
+                    tmem_st16_u32(s_addr + q * 16, pk);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
                 arrive(&p_full[half]);

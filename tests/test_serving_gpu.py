@@ -460,3 +460,17 @@ def test_an_expired_wait_stores_no_part_of_a_value(fmt, code, block):
     assert bool((same | left).all()) and bool(left.any()) and bool(same.any())
     serving.paged_attention(cache, q, got, *batch.args, 8)
     assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
+@pytest.mark.parametrize("n,length", [(1024, 16000), (1, 30000)])
+def test_long_calls_give_the_same_bits_every_time(fmt, n, length):
+    """Many tiles in flight in every block: what one stage hands to the next is there when it is used, and is used before it goes."""
+    batch = Batch([(n, length), (n, length // 2)], 128, seed=4)
+    cache, q, out, want, bound, _ = _attend(batch, 4, 16, 128, BF16, fmt)
+    within(out, want, bound)
+    got = torch.empty_like(out)
+    for _ in range(60):
+        got.fill_(float("nan"))
+        serving.paged_attention(cache, q, got, *batch.args, 16)
+        assert torch.equal(got, out)
