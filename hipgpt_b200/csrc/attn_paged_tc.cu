@@ -7,8 +7,8 @@
 //                    sums in fp32 do not care).  P V is summed in TMEM.
 //   warps 8-11       codes: widen them to bf16 in the layout of the operands, two tiles of keys and of values ahead.  e4m3's scales are powers of two and go into
 //                    the values (exact); int8's multiply scores and probabilities.  Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
-//   warp 12          issues the products.  Those of one tile run while the other's softmax does: P V of a tile, then Q K^T of its next, over the same columns of TMEM (products of one thread
-//                    run in the order of their issue, so a commit behind the second covers the first).
+//   warps 12, 14     issue the products of the first and of the second tile: P V, 64 keys as soon as the softmax has them, then Q K^T of the next keys over the same columns of TMEM
+//                    (products of one thread run in the order of their issue, so a commit behind the second covers the first); the other tile's softmax runs meanwhile.
 //   warp 13          asks for the copies, a lane a run of keys in one page: boxes of 64 columns, swizzled, straight into the operands (plain; a page that is none lies
 //                    outside the tensor and comes as zeros), or codes and scales as they lie into a ring of half tiles.  (Loads by the threads themselves, 16 KB on their way, brought
 //                    6 bytes a clock; bulk copies bring 24.)
@@ -67,7 +67,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t *k_s = q_s + 2 * C::kQTile;              // [stage][block][128 keys][128 B], K-major operand
     uint8_t *v_s = k_s + kStages * C::kTile;         // the same bytes, read as an N-major operand
     uint8_t *raw_s = v_s + kStages * C::kTile;       // [slot][64 keys][D] codes as they lie in their pages
-    __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2], o_done[2];
+    __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2][2], o_done[2];
     __shared__ uint64_t landed[CODED ? kSlots : kStages], raw_free[kSlots];
     __shared__ __align__(16) float scale_s[CODED ? kSlots : 1][kHalf];
     __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys], vs_s[SCALED ? kTables : 1][kKeys];
@@ -83,13 +83,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], CODED ? kWideners / 32 : 1);
             mbar_init(&v_full[i], CODED ? kWideners / 32 : 1);
-            mbar_init(&k_free[i], 1);
-            mbar_init(&v_free[i], 1);
+            mbar_init(&k_free[i], 2);
+            mbar_init(&v_free[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i][0], 4);
+            mbar_init(&p_full[i][1], 4);
             mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < (CODED ? kSlots : kStages); ++i) mbar_init(&landed[i], 1);
@@ -140,9 +141,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        more = more && warp < 14;                    // (registers are given back by whole warpgroups)
+        more = more && warp != 15;                   // (registers are given back by whole warpgroups)
     }
-    if (warp >= 13) {
+    if (warp == 13 || warp == 15) {
         // ================= the copies ============================================================================
         uint32_t n = 0, slot = 0;                    // tiles of keys so far; half tiles of codes
         const int page_keys = 1 << a.c.shift, D = a.c.D;
@@ -283,64 +284,61 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
             }
         }
-    } else if (warp == 12) {
-        // ================= the products =========================================================================
+    } else if (warp >= 12) {
+        // ================= the products, a warp for each tile of rows ===========================================
         constexpr uint32_t idesc_qk = idesc_bf16(128, kKeys, 0), idesc_pv = idesc_bf16(128, DP, 1);
-        uint32_t n = 0, np[2] = {0, 0}, items = 0;   // tiles of keys, of probabilities; tiles of rows
+        const int half = (warp - 12) >> 1;
+        const uint32_t s_col = tmem + kColS + half * 128, o_col = tmem + kColO + half * 128;
+        const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2);
+        uint32_t n = 0, np = 0, items = 0;           // tiles of keys, of probabilities; tiles of rows
         for (; more; more = run.next(), ++items) {
             const Tile w = run.at();
             // (read from one lane: every address below is then known to be the warp's, not a lane's)
-            const int u[2] = {__shfl_sync(0xffffffffu, units_of(w, 0), 0), __shfl_sync(0xffffffffu, units_of(w, 1), 0)}, units = max(u[0], u[1]);
-            auto qk = [&](int half, int t) {
+            const int u = __shfl_sync(0xffffffffu, units_of(w, half), 0), units = __shfl_sync(0xffffffffu, max(units_of(w, 0), units_of(w, 1)), 0);
+            auto ph = [&](int t) { return ((n + t) / kStages) & 1u; };
+            auto qk = [&](int t) {
                 const int st = (n + t) % kStages;
-                const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2), dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
+                const uint64_t dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
+                wait(&k_full[st], ph(t), 1);
+                tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint64_t off = (uint64_t)((k / 4) * (128 * 128 / 16) + (k % 4) * 2);
-                        mma_h_ss(tmem + kColS + half * 128, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
+                        mma_h_ss(s_col, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
                     }
                     tc_commit(&s_full[half]);
+                    tc_commit(&k_free[st]);
                 }
             };
-            auto pv = [&](int half, int t) {
+            wait(&q_full[half], items & 1, 3);
+            tc_fence_after();
+            if (u > 0) qk(0);
+            for (int t = 0; t < u; ++t, ++np) {
                 const int st = (n + t) % kStages;
                 const uint64_t dv = make_desc(smem_u32(v_s + st * C::kTile), kKeys * 128, 1024, 2);
-                if (elect_one()) {
+                wait(&v_full[st], ph(t), 2);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        mma_h_ts(tmem + kColO + half * 128, tmem + kColS + half * 128 + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
-                }
-            };
-            // the last of the two to read a stage gives it back
-            auto free_k = [&](int half, int t) { if (half == (t < u[1] ? 1 : 0) && elect_one()) tc_commit(&k_free[(n + t) % kStages]); };
-            auto free_v = [&](int half, int t) { if (half == (t < u[1] ? 1 : 0) && elect_one()) tc_commit(&v_free[(n + t) % kStages]); };
-            auto ph = [&](int t) { return ((n + t) / kStages) & 1u; };
-            for (int half = 0; half < 2; ++half) wait(&q_full[half], items & 1, 3);     // (both every time: a phase must not be passed over)
-            wait(&k_full[n % kStages], ph(0), 1);
-            tc_fence_after();
-            for (int half = 0; half < 2; ++half) {
-                if (u[half]) { qk(half, 0); free_k(half, 0); }
-                else if (elect_one()) tc_commit(&o_done[half]);      // (whoever has no units of this tile must not run ahead into the next)
-            }
-            for (int t = 0; t < units; ++t) {
-                wait(&v_full[(n + t) % kStages], ph(t), 2);
-                for (int half = 0; half < 2; ++half) {
-                    if (t >= u[half]) continue;
-                    wait(&p_full[half], np[half]++ & 1, 5);
+                for (int part = 0; part < 2; ++part) {               // (the first 64 keys while the softmax takes the others)
+                    wait(&p_full[half][part], np & 1, 5);
                     tc_fence_after();
-                    pv(half, t);
-                    free_v(half, t);
-                    if (t + 1 < u[half]) {
-                        if (half == (t + 1 < u[0] ? 0 : 1)) {                // (the first to need it)
-                            wait(&k_full[(n + t + 1) % kStages], ph(t + 1), 1);
-                            tc_fence_after();
-                        }
-                        qk(half, t + 1);
-                        free_k(half, t + 1);
-                    } else if (elect_one()) tc_commit(&o_done[half]);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = part * (kKeys / 32); k < (part + 1) * (kKeys / 32); ++k) mma_h_ts(o_col, s_col + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
+                        if (part) tc_commit(&v_free[st]);
+                    }
                 }
+                if (t + 1 < u) qk(t + 1);
             }
+            // what this tile of rows does not see is given back all the same, when it has come
+            for (int t = u; t < units; ++t) {
+                const int st = (n + t) % kStages;
+                wait(&k_full[st], ph(t), 1);
+                if (elect_one()) tc_commit(&k_free[st]);
+                wait(&v_full[st], ph(t), 2);
+                if (elect_one()) tc_commit(&v_free[st]);
+            }
+            if (elect_one()) tc_commit(&o_done[half]);       // (without units too: whoever has none must not run ahead into the next)
             n += units;
         }
         __syncwarp();
@@ -470,11 +468,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         pk[c / 2 + 1] = pack_bf16(y[1].x, y[1].y);
                     }
                     tmem_st16_u32(s_addr + q * 16, pk);
+                    if (q == 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        arrive(&p_full[half][0]);
+                    }
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
-                arrive(&p_full[half]);
+                arrive(&p_full[half][1]);
             }
             n += max(u0, u1);
             // ---- the tile's end ---------------------------------------------------------------------------------
