@@ -19,7 +19,7 @@ struct AttnArgs {
     int group, causal;
     float scale, cscale;                 // and scale * log2 e
     int least;                           // units a block takes at least
-    float *parts;                        // [2 * blocks][ROWS][DP + 2]: sums, then maximum (log2 domain) and sum of exponentials of each row
+    float *parts;                        // [2 * blocks][ROWS][DP + 2]: sums, then reference maximum (log2 domain) and sum of exponentials of each row
     int4 *cuts;                          // [blocks]: the tile that begins here and goes on: sequence, head, tile, last block (w < 0: none)
     int *whole;                          // [blocks]: 0 where a wait ran out
 };
@@ -77,24 +77,37 @@ struct Run {
     Sequence s;
     int units;
 
-    // units of a sequence, for one head: the tiles are gone through by a warp where there are many
-    __device__ __forceinline__ long long sequence_units(const Sequence &q) const
+    // units of one head of the sequences b0 ...: of one in each thread, or, where there are no more sequences than warps, of one in the first lane of each warp (its lanes
+    // share the tiles); `i`: which sequence
+    __device__ __forceinline__ long long count(int b0, int &i) const
     {
-        const int tiles = tiles_of<ROWS>(a, q);
+        const bool few = a.c.B <= THREADS / 32;
+        const int lane = threadIdx.x & 31;
+        i = few ? (int)(threadIdx.x >> 5) : b0 + (int)threadIdx.x;
         long long n = 0;
-        for (int i = 0; i < tiles; ++i) n += tile_units<ROWS, UNIT>(a, q, i);
-        return n;
+        if (i < a.c.B) {
+            const Sequence q = sequence_of(a.c, i);
+            const int tiles = tiles_of<ROWS>(a, q);
+            for (int t = few ? lane : 0; t < tiles; t += few ? 32 : 1) n += tile_units<ROWS, UNIT>(a, q, t);
+        }
+        if (few) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+            if (lane) n = 0;
+        }
+        return n * a.c.heads;
     }
 
     __device__ __forceinline__ explicit Run(const AttnArgs &args) : a(args) {}
 
     __device__ __forceinline__ bool begin(long long *shared)
     {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x, lane = tid & 31;
         // all units
-        long long mine = 0;
-        for (int i = tid; i < a.c.B; i += THREADS) mine += sequence_units(sequence_of(a.c, i));
-        const long long total = block_sum<THREADS>(mine, shared) * a.c.heads;
+        int i = 0;
+        long long n = count(0, i), mine = n;
+        for (int b0 = THREADS; b0 < a.c.B; b0 += THREADS) { int x; mine += count(b0, x); }
+        const long long total = block_sum<THREADS>(mine, shared);
         per = max((total + gridDim.x - 1) / gridDim.x, (long long)a.least);
         u = start = (long long)blockIdx.x * per;
         end = min(total, u + per);
@@ -102,17 +115,16 @@ struct Run {
         // the sequence that holds the first
         long long before = 0;
         for (int b0 = 0;; b0 += THREADS) {
-            const int i = b0 + tid;
-            const long long n = i < a.c.B ? sequence_units(sequence_of(a.c, i)) * a.c.heads : 0;
+            if (b0) n = count(b0, i);
             // running sums over the block
             long long upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                if ((tid & 31) >= o) upto += x;
+                if (lane >= o) upto += x;
             }
             __syncthreads();
-            if ((tid & 31) == 31) shared[tid >> 5] = upto;
+            if (lane == 31) shared[tid >> 5] = upto;
             if (tid == 0) shared[THREADS / 32 + 1] = -1;
             __syncthreads();
             long long chunk = 0;
@@ -131,12 +143,25 @@ struct Run {
             if (b0 + THREADS >= a.c.B) return false;                  // (not reached: u < total)
         }
         s = sequence_of(a.c, b);
-        // tile after tile, all heads of one before the next
-        for (tile = 0;; ++tile) {
-            units = tile_units<ROWS, UNIT>(a, s, tile);
-            const long long all = (long long)units * a.c.heads;
-            if (u < base + all) break;
-            base += all;
+        // tile after tile, all heads of one before the next; 32 tiles at a time
+        const int tiles = tiles_of<ROWS>(a, s);
+        for (tile = 0;; tile += 32) {
+            const int mine_units = tile + lane < tiles ? tile_units<ROWS, UNIT>(a, s, tile + lane) : 0;
+            long long upto = (long long)mine_units * a.c.heads;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned behind = __ballot_sync(0xffffffffu, u < base + upto);
+            if (behind) {
+                const int at = __ffs((int)behind) - 1;
+                units = __shfl_sync(0xffffffffu, mine_units, at);
+                base += __shfl_sync(0xffffffffu, upto, at) - (long long)units * a.c.heads;
+                tile += at;
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, upto, 31);
         }
         head = (int)((u - base) / units);
         base += (long long)head * units;
@@ -200,9 +225,9 @@ __device__ __forceinline__ bool any_wild(const AttnArgs &a, int b, int head, int
     return wild;
 }
 
-// One warp: row `row` of (sequence b, head of the cache)
+// One warp: values c0 .. c1 of row `row` of (sequence b, head of the cache)
 template <typename T, int FMT>
-__device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row)
+__device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row, int c0, int c1)
 {
     const int lane = threadIdx.x & 31, D = a.c.D, limit = limit_of(a, s, row);
     const long long t = s.first + row / a.group;
@@ -232,15 +257,15 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
     }
     T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) out[lane + 32 * i] = from_float<T>(l == 0.0f ? 0.0f : o[i] / l);
+    for (int i = 0; i < 4; ++i) if (lane + 32 * i >= c0 && lane + 32 * i < min(c1, D)) out[lane + 32 * i] = from_float<T>(l == 0.0f ? 0.0f : o[i] / l);
 }
 
 // Whether a row whose result is not finite was touched by keys that it does not see (its tile's keys go up to `keys`)
 template <typename T, int FMT>
-__device__ __forceinline__ void mend_row(const AttnArgs &a, int b, int head, const Sequence &s, int row, int keys)
+__device__ __forceinline__ void mend_row(const AttnArgs &a, int b, int head, const Sequence &s, int row, int keys, int c0 = 0, int c1 = 128)
 {
     const int limit = limit_of(a, s, row);
-    if (limit < keys && any_wild<T, FMT>(a, b, head, limit, keys)) row_again<T, FMT>(a, b, head, s, row);
+    if (limit < keys && any_wild<T, FMT>(a, b, head, limit, keys)) row_again<T, FMT>(a, b, head, s, row, c0, c1);
 }
 
 // ---- joining the parts ----------------------------------------------------------------------------------------------------

@@ -5,10 +5,11 @@
 //   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: its scores are read from TMEM into registers, P = exp2(s - m) goes over them in
 //                    bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
 //                    sums in fp32 do not care).  P V is summed in TMEM.
-//   warps 8-11       codes: widen them to bf16 in the layout of the operands, two tiles of keys and of values ahead.  e4m3's scales are powers of two and go into
-//                    the values (exact); int8's multiply scores and probabilities.  Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
-//   warps 12, 14     issue the products of the first and of the second tile: P V, 64 keys as soon as the softmax has them, then Q K^T of the next keys over the same columns of TMEM
-//                    (products of one thread run in the order of their issue, so a commit behind the second covers the first); the other tile's softmax runs meanwhile.
+//   warps 8-11       codes: widen them to fp16 in the layout of the operands, two tiles of keys and of values ahead, times their scales over a power of two of each 64 keys, which goes
+//                    into the scores' factor, and for V into the exponent of P.  (e4m3: exact; int8: values are rounded to fp16, as P is, scores multiplied by the keys' scales instead.)
+//                    Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
+//   warp 12          issues the products: P V of a tile, 64 keys as soon as the softmax has them, then Q K^T of its next keys over the same columns of TMEM (products of one thread run in
+//                    the order of their issue, so a commit behind the second covers the first); the other tile's softmax runs meanwhile.
 //   warp 13          asks for the copies, a lane a run of keys in one page: boxes of 64 columns, swizzled, straight into the operands (plain; a page that is none lies
 //                    outside the tensor and comes as zeros), or codes and scales as they lie into a ring of half tiles.  (Loads by the threads themselves, 16 KB on their way, brought
 //                    6 bytes a clock; bulk copies bring 24.)
@@ -29,7 +30,7 @@ namespace {
 
 constexpr int kRows = 256, kKeys = 128, kStages = 2;
 constexpr int kTables = 4;            // a tile's scales and pages are read until its scores have been: the products of the tile after the next say so
-constexpr int kSoft = 256, kWideners = 128, kThreads = 512;
+constexpr int kWideners = 128, kThreads = 512;
 // Registers a thread of each warpgroup: 128 at launch; 184 + 184 + 88 + 56 = 4 x 128
 constexpr int kSoftRegs = 184, kWidenRegs = 88, kIssueRegs = 56;
 constexpr int kHalf = 64, kSlots = 3;  // keys of a half tile of codes, half tiles in the ring
@@ -48,6 +49,24 @@ __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int si
     return false;
 }
 
+// The largest scale of 64 keys goes to [2^k, 2^(k + 1)) in fp16: 128 * 2^8 and 448 * 2^7 are still numbers there, and rows whose scale is 2^-21 of it keep their digits
+template <int FMT> constexpr int kUp = FMT == HIPGPT_CACHE_E4M3 ? 6 : 7;
+
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// Four codes as fp16 (exact), in two words
+template <int FMT>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    if constexpr (FMT == HIPGPT_CACHE_E4M3) {
+        asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        w ^= 0x80808080u;                            // 128 more, without sign; 0x64 above a byte u is 1024 + u
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
+    }
+}
+
 template <int FMT, int DP>
 struct TcCfg {
     static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2, kSlot = kHalf * DP;
@@ -61,6 +80,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     using C = TcCfg<FMT, DP>;
     using T = __nv_bfloat16;
     constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN, SCALED = FMT == HIPGPT_CACHE_INT8;
+    constexpr float kBias = CODED ? 6.0f : 0.0f;
+    constexpr int kIssuers = CODED ? 2 : 1;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *q_s = base;                             // [tile][block of 64 columns][128 rows][128 B], swizzled
@@ -70,7 +91,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2][2], o_done[2];
     __shared__ uint64_t landed[CODED ? kSlots : kStages], raw_free[kSlots];
     __shared__ __align__(16) float scale_s[CODED ? kSlots : 1][kHalf];
-    __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys], vs_s[SCALED ? kTables : 1][kKeys];
+    __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys];       // int8: the scales of the keys
+    __shared__ float k_unit[kTables][2], v_exp[kTables][2];          // codes: the power of two that each 64 keys of a tile were divided by, the exponent of that of the values
+    __shared__ float q_unit[CODED ? 2 * 128 : 1];                    // and that of a row of Q
     __shared__ uint32_t there_s[kTables];            // whether each 16 keys of a tile have a page
     __shared__ long long sums[kThreads / 32 + 2];
     __shared__ uint32_t tmem_slot;
@@ -83,8 +106,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], CODED ? kWideners / 32 : 1);
             mbar_init(&v_full[i], CODED ? kWideners / 32 : 1);
-            mbar_init(&k_free[i], 2);
-            mbar_init(&v_free[i], 2);
+            mbar_init(&k_free[i], kIssuers);
+            mbar_init(&v_free[i], kIssuers);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
@@ -109,18 +132,17 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     // site codes in the status word: 1 keys landed, 2 values landed, 3 queries there, 4 scores ready, 5 probabilities written, 6 sums complete, 7 key stage free, 8 value stage free, 9 copies landed,
     // 10 half tile free
-    bool seen = true;
+    // (what has come costs one test and no look at the flag: there are seven waits for each 128 keys in the warp that issues the products)
+    bool seen = true;                                // what this thread waited for last has come (for who asks for copies then)
     auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
-        const int gone = abort_flag;
-        const bool done = mbar_test(bar, parity);
-        seen = !gone;
-        if (!gone && expires_now(expire, site)) {
+        seen = true;
+        if (expire != 0 && expires_now(expire, site) && !abort_flag) {
             abort_flag = 1;
             atomicCAS(&g_paged_status, 0, site);
             linger();
             seen = false;
-        } else if (!gone && !done) {
-            seen = wait_slow(bar, parity, site, &abort_flag);
+        } else if (!mbar_test(bar, parity)) {
+            seen = !abort_flag && wait_slow(bar, parity, site, &abort_flag);
         }
     };
     auto arrive = [&](uint64_t *bar) {
@@ -141,7 +163,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        more = more && warp != 15;                   // (registers are given back by whole warpgroups)
+        more = more && (warp < 14 || (warp == 14 && kIssuers == 2));             // (registers are given back by whole warpgroups)
     }
     if (warp == 13 || warp == 15) {
         // ================= the copies ============================================================================
@@ -209,12 +231,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     } else if (warp >= 8 && warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
         // ================= codes to operands; rows behind the last key ===========================================
-        const int pt = tid - kSoft, D = a.c.D;
+        const int pt = tid - 256, D = a.c.D;
         uint32_t n = 0, slot = 0;
+        int v_most = 0;                              // the largest exponent of values so far
         if constexpr (!CODED) more = more && warp == 8;
         for (; more; more = run.next()) {
             const Tile w = run.at();
             const int units = max(units_of(w, 0), units_of(w, 1)), keys = tile_keys<kRows>(a, w.s, w.tile);
+            v_most = -200;
             for (int u = w.from; u < w.from + units; ++u, ++n) {
                 const int st = n % kStages, p0 = u * kKeys;
                 const uint32_t ph = (n / kStages) & 1;
@@ -234,47 +258,69 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     // the two halves of a chunk's 32 bytes; where two threads of a row would meet in a bank, one takes them the other way round
                     const int c0 = 2 * c, turn = DP == 128 ? c >> 2 : 0;
                     uint32_t there = 0;
+                    bool all = false;
 #pragma unroll 1
                     for (int part = 0; part < 4; ++part, ++slot) {
                         const int which = part >> 1, sl = slot % kSlots, base_key = (part & 1) * kHalf;
                         wait(&landed[sl], (slot / kSlots) & 1, 9);
-                        if (part == 0) there = *reinterpret_cast<volatile uint32_t *>(&there_s[n % kTables]);
+                        if (part == 0) {
+                            there = *reinterpret_cast<volatile uint32_t *>(&there_s[n % kTables]);
+                            all = p0 + kKeys <= keys && there == 255u && D == DP;
+                        }
+                        auto holds = [&](int key) { return all || (p0 + base_key + key < keys && (there >> ((base_key + key) >> 4) & 1)); };
                         uint4 raw[N];
-                        float scale[SCALED ? 1 : N];
+                        float scale[N];
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
-                            const int key = k0 + PER * i, tile_key = base_key + key;
-                            const bool ok = p0 + tile_key < keys && (there >> (tile_key >> 4) & 1) && c * 16 < D;
+                            const int key = k0 + PER * i;
+                            const bool ok = holds(key) && c * 16 < D;
                             raw[i] = ok ? *reinterpret_cast<const uint4 *>(raw_s + sl * C::kSlot + key * D + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-                            if constexpr (!SCALED) scale[i] = ok ? scale_s[sl][key] : 0.0f;
+                            scale[i] = ok ? scale_s[sl][key] : 0.0f;
                         }
-                        if constexpr (SCALED) {
-                            const int tile_key = base_key + pt;
-                            scale[0] = pt < kHalf && p0 + tile_key < keys && (there >> (tile_key >> 4) & 1) ? scale_s[sl][pt] : 0.0f;
+                        int e = 0;
+                        float key_scale = 0.0f;
+                        if (!SCALED || which) {
+                            uint32_t most = 0;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t bits = holds(lane + 32 * i) ? __float_as_uint(scale_s[sl][lane + 32 * i]) : 0u;
+                                most = max(most, bits < 0x7F800000u ? bits : 0u);
+                            }
+                            most = __reduce_max_sync(0xffffffffu, most);
+                            e = (int)(most >> 23) - 127 - kUp<FMT>;
+                            if (which) {
+                                // Values far below those before them need not fill fp16, and all of one size with P: a tile of zeros must not carry the sum of exponentials out of fp32
+                                e = max(max(e, v_most - 20), -96);
+                                v_most = max(v_most, e);
+                            }
+                            e = min(max(e, -126), 120);
+                        } else if (pt < kHalf) {
+                            key_scale = holds(pt) ? scale_s[sl][pt] : 0.0f;
                         }
                         if (n >= kStages && (part & 1) == 0) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
+                        if (pt == 0) {
+                            if (which) v_exp[n % kTables][part & 1] = (float)e;
+                            else k_unit[n % kTables][part & 1] = SCALED ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
+                        }
+                        if constexpr (SCALED)
+                            if (which == 0 && pt < kHalf) ks_s[n % kTables][base_key + pt] = key_scale;
+                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
                         uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128) + base_key * 128;
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
-                            const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                            const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, s2 = SCALED && !which ? 0x3C003C00u : half2_of(scale[i] * down, scale[i] * down);
                             uint32_t out[8];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                out[2 * x] = code_pair<FMT>(in[x], in[x], 0, 1);
-                                out[2 * x + 1] = code_pair<FMT>(in[x], in[x], 2, 3);
-                            }
-                            if constexpr (!SCALED) {
-                                const uint32_t s2 = pack_bf16(scale[i], scale[i]);
-#pragma unroll
-                                for (int x = 0; x < 8; ++x) out[x] = mul_bf16x2(out[x], s2);
+                                codes_to_half<FMT>(in[x], out[2 * x], out[2 * x + 1]);
+                                out[2 * x] = mul_f16x2(out[2 * x], s2);
+                                out[2 * x + 1] = mul_f16x2(out[2 * x + 1], s2);
                             }
                             const int key = k0 + PER * i;
                             const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
                             *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + turn) % 8)) = turn ? hi : lo;
                             *reinterpret_cast<uint4 *>(tile + sw128(key, (c0 + 1 - turn) % 8)) = turn ? lo : hi;
                         }
-                        if constexpr (SCALED)
-                            if (pt < kHalf) (which ? vs_s : ks_s)[n % kTables][base_key + pt] = which ? scale[0] : scale[0] * a.cscale;
                         arrive(&raw_free[sl]);       // (not before the codes have been used: an arrival does not wait for loads)
                         if (part & 1) {
                             proxy_fence();
@@ -285,60 +331,74 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
         }
     } else if (warp >= 12) {
-        // ================= the products, a warp for each tile of rows ===========================================
-        constexpr uint32_t idesc_qk = idesc_bf16(128, kKeys, 0), idesc_pv = idesc_bf16(128, DP, 1);
-        const int half = (warp - 12) >> 1;
-        const uint32_t s_col = tmem + kColS + half * 128, o_col = tmem + kColO + half * 128;
-        const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2);
-        uint32_t n = 0, np = 0, items = 0;           // tiles of keys, of probabilities; tiles of rows
+        // ================= the products =========================================================================
+        // Plain rows: one warp issues those of both tiles, one tile's after the other's, so that one tile's softmax runs beside the other's products.  (Two warps' products share the pipe, and
+        // both tiles' scores come late, at the same time: 442 against 422 us.)  Codes: a warp for each tile, because they wait for the values to be widened and must not wait for each other too.
+        constexpr uint32_t kHalfTypes = CODED ? ~((1u << 7) | (1u << 10)) : ~0u;         // fp16 operands instead of bf16
+        constexpr uint32_t idesc_qk = idesc_bf16(128, kKeys, 0) & kHalfTypes, idesc_pv = idesc_bf16(128, DP, 1) & kHalfTypes;
+        const int h0 = kIssuers == 2 ? (warp - 12) >> 1 : 0, h1 = kIssuers == 2 ? h0 + 1 : 2;      // the tiles of this warp
+        uint32_t n = 0, np[2] = {0, 0}, items = 0;   // tiles of keys, of probabilities; tiles of rows
         for (; more; more = run.next(), ++items) {
             const Tile w = run.at();
             // (read from one lane: every address below is then known to be the warp's, not a lane's)
-            const int u = __shfl_sync(0xffffffffu, units_of(w, half), 0), units = __shfl_sync(0xffffffffu, max(units_of(w, 0), units_of(w, 1)), 0);
+            const int u[2] = {__shfl_sync(0xffffffffu, units_of(w, 0), 0), __shfl_sync(0xffffffffu, units_of(w, 1), 0)}, units = max(u[0], u[1]);
+            const int mine = kIssuers == 2 ? u[h0] : units;
             auto ph = [&](int t) { return ((n + t) / kStages) & 1u; };
-            auto qk = [&](int t) {
+            // the last of this warp's to read a stage gives it back
+            auto last = [&](int half, int t) { return kIssuers == 2 || half == (t < u[1] ? 1 : 0); };
+            auto qk = [&](int half, int t) {
                 const int st = (n + t) % kStages;
-                const uint64_t dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
-                wait(&k_full[st], ph(t), 1);
-                tc_fence_after();
+                const uint64_t dq = make_desc(smem_u32(q_s + half * C::kQTile), 16, 1024, 2), dk = make_desc(smem_u32(k_s + st * C::kTile), 16, 1024, 2);
+                if (kIssuers == 2 || half == (t < u[0] ? 0 : 1)) {           // (the first to need it)
+                    wait(&k_full[st], ph(t), 1);
+                    tc_fence_after();
+                }
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint64_t off = (uint64_t)((k / 4) * (128 * 128 / 16) + (k % 4) * 2);
-                        mma_h_ss(s_col, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
+                        mma_h_ss(tmem + kColS + half * 128, dq + off, dk + off, idesc_qk, k ? 1u : 0u);
                     }
                     tc_commit(&s_full[half]);
-                    tc_commit(&k_free[st]);
+                    if (last(half, t)) tc_commit(&k_free[st]);
                 }
             };
-            wait(&q_full[half], items & 1, 3);
+            for (int half = h0; half < h1; ++half) wait(&q_full[half], items & 1, 3);       // (without units too: a phase must not be passed over)
             tc_fence_after();
-            if (u > 0) qk(0);
-            for (int t = 0; t < u; ++t, ++np) {
+            for (int half = h0; half < h1; ++half) {
+                if (u[half]) qk(half, 0);
+                else if (elect_one()) tc_commit(&o_done[half]);      // (whoever has no units of this tile must not run ahead into the next)
+            }
+            for (int t = 0; t < mine; ++t) {
                 const int st = (n + t) % kStages;
                 const uint64_t dv = make_desc(smem_u32(v_s + st * C::kTile), kKeys * 128, 1024, 2);
                 wait(&v_full[st], ph(t), 2);
+                for (int half = h0; half < h1; ++half) {
+                    if (t >= u[half]) continue;
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {               // (the first 64 keys while the softmax takes the others)
-                    wait(&p_full[half][part], np & 1, 5);
-                    tc_fence_after();
-                    if (elect_one()) {
+                    for (int part = 0; part < 2; ++part) {               // (the first 64 keys while the softmax takes the others)
+                        wait(&p_full[half][part], np[half] & 1, 5);
+                        tc_fence_after();
+                        if (elect_one()) {
 #pragma unroll
-                        for (int k = part * (kKeys / 32); k < (part + 1) * (kKeys / 32); ++k) mma_h_ts(o_col, s_col + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
-                        if (part) tc_commit(&v_free[st]);
+                            for (int k = part * (kKeys / 32); k < (part + 1) * (kKeys / 32); ++k)
+                                mma_h_ts(tmem + kColO + half * 128, tmem + kColS + half * 128 + (uint32_t)(k * 8), dv + (uint64_t)(k * 128), idesc_pv, t || k ? 1u : 0u);
+                            if (part && last(half, t)) tc_commit(&v_free[st]);
+                        }
                     }
+                    ++np[half];
+                    if (t + 1 < u[half]) qk(half, t + 1);
+                    else if (elect_one()) tc_commit(&o_done[half]);
                 }
-                if (t + 1 < u) qk(t + 1);
             }
-            // what this tile of rows does not see is given back all the same, when it has come
-            for (int t = u; t < units; ++t) {
+            // what this warp's tile does not see is given back all the same, when it has come
+            for (int t = mine; t < units; ++t) {
                 const int st = (n + t) % kStages;
                 wait(&k_full[st], ph(t), 1);
                 if (elect_one()) tc_commit(&k_free[st]);
                 wait(&v_full[st], ph(t), 2);
                 if (elect_one()) tc_commit(&v_free[st]);
             }
-            if (elect_one()) tc_commit(&o_done[half]);       // (without units too: whoever has none must not run ahead into the next)
             n += units;
         }
         __syncwarp();
@@ -358,34 +418,59 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int r = half * 128 + quad * 32 + lane;                     // row of the block's tile
             const long long row = (long long)w.tile * kRows + r;
             const bool mine = row < rows;
+            const long long wfirst = row - lane;
             const long long t = w.s.first + row / a.group;
             const long long col = (long long)(w.head * a.group + (int)(row % a.group)) * D;
             const int u0 = units_of(w, 0), u1 = units_of(w, 1), units = half ? u1 : u0;
             const bool tile_there = (long long)w.tile * kRows + 128 * half < rows;
-            // ---- the row of Q ---------------------------------------------------------------------------------
+            // ---- the rows of Q: DP / 8 lanes a row ------------------------------------------------------------
+            constexpr int CH = DP / 8, PER = 32 / CH;
+            const int c = lane % CH;
+            uint8_t *q_at = q_s + half * C::kQTile + (c / 8) * (128 * 128);
+            const long long q_off = t * a.q_stride + col, out_off = t * a.out_stride + col;
             if (tile_there) {
-                const T *src = static_cast<const T *>(a.q) + t * a.q_stride + col;
-                uint8_t *dst = q_s + half * C::kQTile;
+                uint4 in[32 / PER];                                          // (all on their way at once)
 #pragma unroll
-                for (int c = 0; c < DP / 8; ++c) {
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (mine && c * 8 < D) {
+                for (int i = 0; i < 32 / PER; ++i) {
+                    const int rr = lane / CH + PER * i;                      // row of the warp
+                    const T *src = static_cast<const T *>(a.q) + __shfl_sync(0xffffffffu, q_off, rr) + c * 8;
+                    in[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (wfirst + rr < rows && c * 8 < D) {
                         if (vec) {
-                            x = *reinterpret_cast<const uint4 *>(src + c * 8);
+                            in[i] = __ldg(reinterpret_cast<const uint4 *>(src));
                         } else {
                             uint32_t y[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) y[i] = __bfloat16_as_ushort(src[c * 8 + 2 * i]) | (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * i + 1]) << 16;
-                            x = make_uint4(y[0], y[1], y[2], y[3]);
+                            for (int e = 0; e < 4; ++e) y[e] = __bfloat16_as_ushort(src[2 * e]) | (uint32_t)__bfloat16_as_ushort(src[2 * e + 1]) << 16;
+                            in[i] = make_uint4(y[0], y[1], y[2], y[3]);
                         }
                     }
-                    *reinterpret_cast<uint4 *>(dst + (c / 8) * (128 * 128) + sw128(quad * 32 + lane, c % 8)) = x;
+                }
+#pragma unroll
+                for (int i = 0; i < 32 / PER; ++i) {
+                    const int rr = lane / CH + PER * i;
+                    uint4 x = in[i];
+                    if constexpr (CODED) {
+                        // to fp16, the largest of the row to [2^14, 2^15): exact down to 2^-28 of it
+                        float v[8];
+                        unpack(x, v, T());
+                        float most = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+                        for (int o = 1; o < CH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        const float up = pow2_scale(most);
+                        x = make_uint4(half2_of(v[0] * up, v[1] * up), half2_of(v[2] * up, v[3] * up), half2_of(v[4] * up, v[5] * up), half2_of(v[6] * up, v[7] * up));
+                        if (c == 0) q_unit[half * 128 + quad * 32 + rr] = pow2_inverse(up);
+                    }
+                    *reinterpret_cast<uint4 *>(q_at + sw128(quad * 32 + rr, c % 8)) = x;
                 }
                 proxy_fence();
             }
+            __syncwarp();
+            const float row_factor = CODED && tile_there ? a.cscale * q_unit[CODED ? half * 128 + quad * 32 + lane : 0] : a.cscale;
             arrive(&q_full[half]);
             const int limit = mine ? limit_of(a, w.s, (int)row) : 0;
-            const long long wfirst = (long long)w.tile * kRows + half * 128 + quad * 32;
             const int least_limit = wfirst < rows ? limit_of(a, w.s, (int)wfirst) : 1 << 30;       // (rows behind the last: their results are not looked at)
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < units; ++i) {
@@ -395,27 +480,48 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
                 const bool masked = p0 + kKeys > least_limit || there != 255u;
                 float v[4][32];
+                if constexpr (!SCALED) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
-                tmem_wait_ld();
-                if constexpr (SCALED) {
+                    for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, v[q]);
+                    tmem_wait_ld();
+                } else {
+                    // times the scales of their keys; those of 32 come while the scores do
 #pragma unroll
-                    for (int c = 0; c < kKeys; c += 4) {
-                        const float4 f = *reinterpret_cast<const float4 *>(&ks_s[tb][c]);
-                        const float2 lo = fmul2(make_float2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), make_float2(f.x, f.y));
-                        const float2 hi = fmul2(make_float2(v[c / 32][c % 32 + 2], v[c / 32][c % 32 + 3]), make_float2(f.z, f.w));
-                        v[c / 32][c % 32] = lo.x; v[c / 32][c % 32 + 1] = lo.y; v[c / 32][c % 32 + 2] = hi.x; v[c / 32][c % 32 + 3] = hi.y;
+                    for (int q = 0; q < 4; ++q) {
+                        float4 f[8];
+                        tmem_ld32(s_addr + q * 32, v[q]);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) f[c] = *reinterpret_cast<const float4 *>(&ks_s[tb][q * 32 + c * 4]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const float2 lo = fmul2(make_float2(v[q][4 * c], v[q][4 * c + 1]), make_float2(f[c].x, f[c].y)), hi = fmul2(make_float2(v[q][4 * c + 2], v[q][4 * c + 3]), make_float2(f[c].z, f[c].w));
+                            v[q][4 * c] = lo.x; v[q][4 * c + 1] = lo.y; v[q][4 * c + 2] = hi.x; v[q][4 * c + 3] = hi.y;
+                        }
                     }
                 }
                 if (masked) {
 #pragma unroll
                     for (int c = 0; c < kKeys; ++c) v[c / 32][c % 32] = p0 + c < limit && (there >> (c >> 4) & 1) ? v[c / 32][c % 32] : -INFINITY;
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // what the scores of each 64 keys are multiplied by, and (codes) the exponent that their values were divided by: P takes it
+                float factor[2] = {row_factor, row_factor}, up[2] = {0.0f, 0.0f};
+                if constexpr (CODED) {
+                    wait(&v_full[st], ((n + i) / kStages) & 1, 2);
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], v[c / 32][c % 32], v[c / 32][c % 32 + 1]);
-                const float factor = SCALED ? 1.0f : a.cscale;               // (int8: among the scales)
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
+                    for (int h = 0; h < 2; ++h) {    // (a masked score times 0 would be NaN)
+                        factor[h] = fminf(fmaxf(factor[h] * *reinterpret_cast<volatile float *>(&k_unit[tb][h]), 1.17549435e-38f), 3.402823466e38f);
+                        up[h] = *reinterpret_cast<volatile float *>(&v_exp[tb][h]);
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 64 * h; c < 64 * h + 64; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], v[c / 32][c % 32], v[c / 32][c % 32 + 1]);
+                    mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), factor[h], up[h]));
+                }
                 if (i == 0) {
                     m = mx;
                 } else {
@@ -436,37 +542,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const float2 f2 = make_float2(factor, factor), nref = make_float2(-ref, -ref);
-                if constexpr (SCALED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);     // the scales of the values
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                // (fp16: P up to 2^14, its small values too)
+                const float ref = m == -INFINITY ? 0.0f : m - kBias;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t pk[16];
+                    const float2 f2 = make_float2(factor[q >> 1], factor[q >> 1]), nref = make_float2(up[q >> 1] - ref, up[q >> 1] - ref);
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        float2 y[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float2 s2 = make_float2(v[q][c + 2 * e], v[q][c + 2 * e + 1]), x = SCALED ? fadd2(s2, nref) : ffma2(s2, f2, nref);
-                            y[e] = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                            sum[e] = fadd2(sum[e], y[e]);
-                        }
-                        if constexpr (SCALED) {
-                            // (a row that must not see a value does not see its scale either)
-                            const float4 f = *reinterpret_cast<const float4 *>(&vs_s[tb][q * 32 + c]);
-                            y[0] = fmul2(y[0], make_float2(f.x, f.y));
-                            y[1] = fmul2(y[1], make_float2(f.z, f.w));
-                            if (masked) {
-                                y[0].x = v[q][c] == -INFINITY ? 0.0f : y[0].x;
-                                y[0].y = v[q][c + 1] == -INFINITY ? 0.0f : y[0].y;
-                                y[1].x = v[q][c + 2] == -INFINITY ? 0.0f : y[1].x;
-                                y[1].y = v[q][c + 3] == -INFINITY ? 0.0f : y[1].y;
-                            }
-                        }
-                        pk[c / 2] = pack_bf16(y[0].x, y[0].y);
-                        pk[c / 2 + 1] = pack_bf16(y[1].x, y[1].y);
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 x = ffma2(make_float2(v[q][c], v[q][c + 1]), f2, nref), y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        sum[c / 2 % 2] = fadd2(sum[c / 2 % 2], y);
+                        pk[c / 2] = CODED ? half2_of(y.x, y.y) : pack_bf16(y.x, y.y);
                     }
+                    const float part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    l = CODED ? fmaf(part, __uint_as_float((uint32_t)(127 - (int)up[q >> 1]) << 23), l) : l + part;
                     tmem_st16_u32(s_addr + q * 16, pk);
                     if (q == 1) {
                         tmem_wait_st();
@@ -474,7 +564,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         arrive(&p_full[half][0]);
                     }
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
                 arrive(&p_full[half][1]);
@@ -486,50 +575,61 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             wait(&o_done[half], no++ & 1, 6);
             tc_fence_after();
             if (!tile_there) continue;
-            const bool store = mine && !abort_flag;
+            const bool store = !abort_flag;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            float *dst = part < 0 ? nullptr : a.parts + (size_t)part * kRows * (DP + 2);
             bool wild = false;
-            T *out = static_cast<T *>(a.out) + t * a.out_stride + col;
+            if (part >= 0) {
+                // a part: column after column, so that the lanes' rows lie beside each other
+                float *dst = a.parts + (size_t)part * kRows * (DP + 2) + r;
 #pragma unroll 1
-            for (int hh = 0; hh < DP / 16; ++hh) {
-                float x[16];
-                if (units > 0) {
+                for (int hh = 0; hh < DP / 16; ++hh) {
+                    float x[16];
                     tmem_ld16(o_addr + hh * 16, x);
                     tmem_wait_ld();
-                } else {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) x[c] = 0.0f;
+                    for (int e = 0; e < 16; ++e) if (store) dst[(hh * 16 + e) * kRows] = units > 0 ? x[e] : 0.0f;
                 }
-                if (dst) {
-                    if (store) {
-#pragma unroll
-                        for (int c = 0; c < 16; c += 2) *reinterpret_cast<float2 *>(dst + (size_t)r * DP + hh * 16 + c) = make_float2(x[c], x[c + 1]);
-                    }
-                } else {
+                if (store) {
+                    dst[DP * kRows] = m == -INFINITY ? m : m - kBias;
+                    dst[(DP + 1) * kRows] = l;
+                }
+            } else {
+                // whole rows leave by way of the tile of Q, which the last Q K^T has read
+                uint8_t *turn = q_s + half * C::kQTile;
+#pragma unroll 1
+                for (int hh = 0; hh < DP / 16; ++hh) {
+                    float x[16];
+                    tmem_ld16(o_addr + hh * 16, x);
+                    tmem_wait_ld();
                     uint32_t y[8];
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        x[c] = l == 0.0f ? 0.0f : x[c] * inv;
-                        wild = wild || !(fabsf(x[c]) <= 3.402823466e38f);
+                    for (int e = 0; e < 16; ++e) {
+                        x[e] = l == 0.0f ? 0.0f : x[e] * inv;
+                        wild = wild || !(fabsf(x[e]) <= 3.402823466e38f);
                     }
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) y[c] = pack_bf16(x[2 * c], x[2 * c + 1]);
-                    if (store && hh * 16 < D) {
+                    for (int e = 0; e < 8; ++e) y[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                    uint8_t *at = turn + (hh / 4) * (128 * 128);
+                    *reinterpret_cast<uint4 *>(at + sw128(quad * 32 + lane, hh % 4 * 2)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4 *>(at + sw128(quad * 32 + lane, hh % 4 * 2 + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < 32 / PER; ++i) {
+                    const int rr = lane / CH + PER * i;
+                    T *out = static_cast<T *>(a.out) + __shfl_sync(0xffffffffu, out_off, rr) + c * 8;
+                    if (store && wfirst + rr < rows && c * 8 < D) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(q_at + sw128(quad * 32 + rr, c % 8));
                         if (vec) {
-                            *reinterpret_cast<uint4 *>(out + hh * 16) = make_uint4(y[0], y[1], y[2], y[3]);
-                            *reinterpret_cast<uint4 *>(out + hh * 16 + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                            *reinterpret_cast<uint4 *>(out) = x;
                         } else {
+                            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) out[hh * 16 + c] = __ushort_as_bfloat16((unsigned short)(y[c / 2] >> (c & 1) * 16));
+                            for (int e = 0; e < 8; ++e) out[e] = __ushort_as_bfloat16((unsigned short)(y[e / 2] >> (e & 1) * 16));
                         }
                     }
                 }
-            }
-            if (dst) {
-                if (store) *reinterpret_cast<float2 *>(dst + (size_t)kRows * DP + 2 * r) = make_float2(m, l);
-            } else {
-                unsigned some = __ballot_sync(0xffffffffu, wild && store);
+                unsigned some = __ballot_sync(0xffffffffu, wild && store && mine);
                 __syncwarp();
                 while (some) {
                     const int who = __ffs((int)some) - 1;
@@ -563,6 +663,68 @@ int page_map(CUtensorMap *m, const void *rows, const PagedView &c)
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
     return HIPGPT_OK;
+}
+
+// Joins the parts of the tile that began in this block of the kernel before and went on; a thread a row and sixteen columns, parts in ascending order.
+template <int FMT, int DP>
+__global__ void __launch_bounds__(256)
+paged_tc_join_kernel(const AttnArgs a)
+{
+    using T = __nv_bfloat16;
+    dependency_wait();
+    dependents_may_start();
+    const int4 cut = a.cuts[blockIdx.x];
+    if (cut.w < 0) return;
+    for (int blk = blockIdx.x; blk <= cut.w; ++blk) if (!a.whole[blk]) return;
+    const Sequence s = sequence_of(a.c, cut.x);
+    const int r = threadIdx.x, D = a.c.D, c0 = blockIdx.y * 16;
+    const long long row = (long long)cut.z * kRows + r, rows = (long long)s.n * a.group;
+    float m = -INFINITY, l = 0.0f, o[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+    if (row < rows) {
+        for (int blk = blockIdx.x; blk <= cut.w; ++blk) {
+            const float *p = a.parts + (size_t)(2 * blk + (blk == (int)blockIdx.x)) * kRows * (DP + 2) + r;
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = p[(c0 + e) * kRows];
+            const float m2 = p[DP * kRows], l2 = p[(DP + 1) * kRows], mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.0f : mn;
+            const float f1 = ex2_approx(m - base), f2 = ex2_approx(m2 - base);
+            m = mn;
+            l = fmaf(l, f1, l2 * f2);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(o[e], f1, x[e] * f2);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *out = static_cast<T *>(a.out) + (s.first + row / a.group) * a.out_stride + (long long)(cut.y * a.group + (int)(row % a.group)) * D + c0;
+    bool wild = false;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+        wild = wild || !(fabsf(o[e]) <= 3.402823466e38f);
+    }
+    if (row < rows && c0 < D) {
+        if (((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * 2)) & 15) == 0) {
+            float x[8], y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { x[e] = o[e]; y[e] = o[8 + e]; }
+            store_values<T, 8>(out, x);
+            store_values<T, 8>(out + 8, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) out[e] = from_float<T>(o[e]);
+        }
+    }
+    if (__syncthreads_or(row < rows && wild)) {
+        const int keys = tile_keys<kRows>(a, s, cut.z);
+        unsigned some = __ballot_sync(0xffffffffu, row < rows && wild);
+        while (some) {
+            const int who = __ffs((int)some) - 1;
+            some &= some - 1;
+            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)(row - (r & 31)) + who, keys, c0, c0 + 16);
+        }
+    }
 }
 
 template <int FMT, int DP>
@@ -601,7 +763,7 @@ int launch_tc(AttnArgs a, cudaStream_t st)
         if (rc != HIPGPT_OK) return rc;
     }
     e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, kmap, vmap, a, take_expiry(1000));
-    if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<__nv_bfloat16, FMT, kRows, DP>, dim3((unsigned)grid, 4), dim3(256), 0, st, a);
+    if (e == cudaSuccess && cuts) e = launch_overlapped(paged_tc_join_kernel<FMT, DP>, dim3((unsigned)grid, DP / 16), dim3(kRows), 0, st, a);
     return e == cudaSuccess ? check_launch("paged_tc_kernel") : fail(HIPGPT_ERR_CUDA, "paged_tc_kernel: %s", cudaGetErrorString(e));
 }
 
