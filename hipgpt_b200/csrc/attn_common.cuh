@@ -181,6 +181,7 @@ int loss_status_fetch(int *status);
 // attention over a paged cache (attn_paged.cu, attn_paged_tc.cu)
 void paged_release_scratch();
 int paged_status_fetch(int *status);
+int paged_rows_status_fetch(int *status);
 int launch_mha_generic(const float *q, const float *k, const float *v, float *out, float *probs,
                        int B, int S, int E, int H, int causal, cudaStream_t st);
 int launch_sdp(const float *Q, const float *K, float *scores, int B, int S, int D, cudaStream_t st);

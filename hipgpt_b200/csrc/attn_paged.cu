@@ -1,19 +1,17 @@
-// Attention of new tokens over a paged cache, in registers: the kernel for single tokens and for fp32.
+// Attention of new tokens over a paged cache on mma.sync: the kernel for single tokens and for fp32.
 //
 //   out = softmax(scale q K^T) V per row, one pass over the keys with the running maximum and sum
 //
-// Bound for single tokens: HBM, the cache is read once (the group's rows share it).  So K and V go from global memory straight to the registers of the warp that
-// multiplies them (mma.sync: sixteen rows by eight keys; what tcgen05 adds is not needed where the bytes decide, and its operands would have to lie in
-// shared memory first):
+// Bound for single tokens: HBM, the cache is read once (the group's rows share it).  One warp brings K and V as they lie in their pages into a ring in shared memory by bulk copies, a lane a
+// run of keys in one page; four warps multiply (sixteen rows by eight keys an instruction; what tcgen05 adds is not needed where the bytes decide, and its operands would have to be
+// laid out once more).  (Loads straight into registers read 2.2 TB/s at 32 sequences of 8192 to 32768 tokens, 8 heads of 128 codes: too few bytes on their way; copies LATER.)
 //   * which 16 values of a row an instruction sums over does not matter as long as Q's are the same, so a thread of the four that share a key takes 16
 //     consecutive bytes of its row, and Q is laid out to match;
 //   * P's layout as a result (keys 2t, 2t+1, 8+2t, 9+2t of sixteen) is its layout as an operand, so a thread takes 16 consecutive bytes of each of those four rows of V, and the
-//     column of V^T that an instruction needs is one byte (or half) picked from each of two registers by the permutation that widening the codes takes anyway.
-// Shared memory holds Q (a block's warps take the same rows and different keys) and the warps' results at the end.  Each warp has a block of V on its way while it works on
-// K, and the next block of K while it works on V.
-// Codes are widened to bf16 (exact); a key's scale multiplies its scores, a value's scale its probabilities.
-// fp32 operands are three bf16 pieces (24 bits); products of pieces whose orders add up to more than two are left out.  The tensor core cuts off where others round, so no fp32 sum
-// stays in it for more than a block of keys.
+//     column of V^T that an instruction needs is one byte (or half) picked from each of two registers.
+// Codes become fp16 (exact), and so does Q, a power of two for each row; a key's scale multiplies its scores, a value's scale its probabilities, all of one power of two that follows the largest.
+// fp32 operands are two fp16 pieces (22 bits) against codes, three bf16 pieces (24 bits) against each other, without the products whose orders add up to more than two.  The tensor core cuts off
+// where others round, so no fp32 sum stays in it for more than a block of keys.
 #include "attn_paged.cuh"
 #include "stream_workspace.hpp"
 
@@ -25,126 +23,256 @@ StreamWorkspace g_paged_ws;                      // parts of tiles (attn_paged_t
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kWarps = 4, kThreads = 32 * (kWarps + 1);
 
-// D += A B: 16 rows, 8 columns, 16 summed over; bf16
+__device__ int g_rows_status = 0;
+
+// D += A B: 16 rows, 8 columns, 16 summed over; fp16 or bf16
+template <bool HALF>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-// Piece i of N of two fp32 values as bf16 pairs; what is left in the values
+// The next piece of two fp32 values; what is left in the values
+template <bool HALF>
 __device__ __forceinline__ uint32_t next_piece(float &lo, float &hi)
 {
-    const uint32_t w = pack_bf16(lo, hi);
-    lo -= __uint_as_float(w << 16);
-    hi -= __uint_as_float(w & 0xFFFF0000u);
-    return w;
-}
-
-template <int BYTES>
-__device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *p, bool there)
-{
-    if constexpr (BYTES == 16) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (there) u = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (BYTES == 8) {
-        uint2 u = make_uint2(0u, 0u);
-        if (there) u = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = u.x; w[1] = u.y;
+    if constexpr (HALF) {
+        const uint32_t w = half2_of(lo, hi);
+        float a, b;
+        asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;}" : "=f"(a), "=f"(b) : "r"(w));
+        lo -= a;
+        hi -= b;
+        return w;
     } else {
-        static_assert(BYTES == 4, "a word at least");
-        w[0] = there ? __ldg(reinterpret_cast<const uint32_t *>(p)) : 0u;
+        const uint32_t w = pack_bf16(lo, hi);
+        lo -= __uint_as_float(w << 16);
+        hi -= __uint_as_float(w & 0xFFFF0000u);
+        return w;
     }
 }
 
-constexpr int least_of(int a, int b) { return a < b ? a : b; }
+template <int BYTES>
+__device__ __forceinline__ void read_words(uint32_t *w, const uint8_t *p)
+{
+    if constexpr (BYTES == 16) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else if constexpr (BYTES == 8) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        w[0] = u.x; w[1] = u.y;
+    } else {
+        static_assert(BYTES == 4, "a word at least");
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+__host__ __device__ constexpr int least_of(int a, int b) { return a < b ? a : b; }
+__host__ __device__ constexpr int most_of(int a, int b) { return a > b ? a : b; }
 
 template <typename T, int FMT, int DP, bool SPLITROWS>
 struct Shape {
     static constexpr bool F32 = sizeof(T) == 4, CODED = FMT != HIPGPT_CACHE_PLAIN;
     static constexpr int EB = CODED ? 1 : (int)sizeof(T);               // bytes of an element of the cache
-    static constexpr int NQ = F32 ? 3 : 1, NK = F32 && !CODED ? 3 : 1;  // pieces of Q and P, of K and V
+    static constexpr int NQ = !F32 ? 1 : CODED ? 2 : 3, NK = F32 && !CODED ? 3 : 1;  // pieces of Q and P, of K and V
     static constexpr int MT = SPLITROWS && DP <= 64 ? 2 : 1;            // tiles of 16 rows a warp
     static constexpr int ROWS = 16 * MT * (SPLITROWS ? kWarps : 1);
-    // keys a warp takes at a time: 32 registers of K and as many of V
-    static constexpr int KB = 4096 / (DP * EB) >= 32 ? 32 : 16;
-    static constexpr int UNIT = SPLITROWS ? 64 : kWarps * KB;
+    static constexpr int KB = 4096 / (DP * EB) >= 32 ? 32 : 16;         // keys a warp takes at a time
+    static constexpr int UNIT = SPLITROWS ? 64 : kWarps * KB;           // keys of a place in the ring
     static constexpr int EC = least_of(16 / EB, DP / 4), NC = DP / 4 / EC;       // K: elements of a chunk, chunks a thread
     static constexpr int EV = least_of(16 / EB, DP / 8), NV = DP / 8 / EV;       // V: the same
     static constexpr int STEPS = DP / 16, TILES = DP / 8;
-    static constexpr size_t kQBytes = (size_t)NQ * (ROWS / 16) * STEPS * 32 * 16;
+    static constexpr int kQBytes = NQ * (ROWS / 16) * STEPS * 32 * 16;
     static constexpr int kPad = DP + 4;
-    static constexpr size_t kOBytes = SPLITROWS ? 0 : (size_t)kWarps * ROWS * kPad * 4;
-    static constexpr size_t kSmem = kQBytes + kOBytes;
+    static constexpr int kOBytes = SPLITROWS ? 0 : 2 * 16 * kPad * 4;   // two warps' results
+    static constexpr int kSlotBytes = UNIT * DP * EB + (CODED ? UNIT * 4 : 0);
+    static constexpr int kFixed = kQBytes + kOBytes + 1024;
+    // places of the ring: as many as leave room for two blocks an SM, four at least
+    static constexpr int kSlots = most_of(4, least_of(12, (112 * 1024 - kFixed) / kSlotBytes));
+    static constexpr size_t kSmem = (size_t)kQBytes + kOBytes + (size_t)kSlots * kSlotBytes;
+    static constexpr int kBlocks = kSmem <= 112 * 1024 ? 2 : 1;         // an SM
 };
 
 template <typename T, int FMT, int DP, bool SPLITROWS>
-__global__ void __launch_bounds__(kThreads, SPLITROWS || (sizeof(T) == 4 && DP == 128) ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, Shape<T, FMT, DP, SPLITROWS>::kBlocks)
 paged_rows_kernel(const AttnArgs a)
 {
     using C = Shape<T, FMT, DP, SPLITROWS>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint4 *q_s = reinterpret_cast<uint4 *>(smem);
-    float *o_s = reinterpret_cast<float *>(smem + C::kQBytes);
-    __shared__ long long sums[kWarps + 2];
-    __shared__ float2 ml_s[kWarps][16];
-    dependency_wait();
-    dependents_may_start();
+    constexpr bool HALF = C::CODED;
+    constexpr int SLOTS = C::kSlots;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *ring = smem;                            // [slot][UNIT keys][D] as in the pages, then their scales
+    uint4 *q_s = reinterpret_cast<uint4 *>(smem + SLOTS * C::kSlotBytes);
+    float *o_s = reinterpret_cast<float *>(smem + SLOTS * C::kSlotBytes + C::kQBytes);
+    __shared__ uint64_t full[SLOTS], empty[SLOTS];
+    __shared__ uint32_t there_s[SLOTS];              // whether each 16 keys of a place have a page
+    __shared__ long long sums[kWarps + 3];
+    __shared__ float2 ml_s[2][16];
+    __shared__ float q_unit[C::ROWS];
+    __shared__ volatile int abort_flag;
 
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int D = a.c.D;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kWarps);
+        }
+    }
+    __syncthreads();
+    dependency_wait();
+    dependents_may_start();
+
+    // sites: 11 keys or values landed, 12 place free
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        if (mbar_test(bar, parity)) return true;
+        if (!abort_flag) {
+            if (mbar_wait(bar, parity)) return true;
+            abort_flag = 1;
+            atomicCAS(&g_rows_status, 0, site);
+            linger();
+        }
+        return false;
+    };
     Run<C::ROWS, C::UNIT, kThreads> run(a);
-    int4 cut = make_int4(0, 0, 0, -1);
     bool more = run.begin(sums);
+
+    if (warp == kWarps) {
+        // ================= the copies ============================================================================
+        uint32_t slot = 0;
+        const int page_keys = 1 << a.c.shift, run_keys = min(page_keys, C::UNIT), runs = C::UNIT / run_keys;
+        bool alive = true;
+        for (; more; more = run.next()) {
+            const Tile w = run.at();
+            const int keys = tile_keys<C::ROWS>(a, w.s, w.tile);
+            auto look = [&](int u) {                 // a page for each run of keys, asked for a unit ahead
+                const int p = u * C::UNIT + lane * run_keys;
+                const int pg = lane < runs && p < keys ? __ldg(a.c.table + (size_t)w.b * a.c.most_pages + (p >> a.c.shift)) : -1;
+                return pg < a.c.pages ? pg : -1;
+            };
+            int page = look(w.from);
+            for (int u = w.from; u < w.to; ++u) {
+                const int p = u * C::UNIT + lane * run_keys;
+                const int count = page >= 0 ? min(run_keys, keys - p) : 0, scales = C::CODED ? (count + 3) & ~3 : 0;
+                const long long row = ((((long long)page * a.c.heads) + w.head) << a.c.shift) + (p & (page_keys - 1));
+                int bytes = count * D * C::EB + scales * 4;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
+                // one bit for each sixteen keys
+                const uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
+                uint32_t there = 0;
+#pragma unroll
+                for (int i = 0; i < C::UNIT / 16; ++i) there |= (some >> (16 * i / run_keys) & 1u) << i;
+                page = u + 1 < w.to ? look(u + 1) : -1;
+#pragma unroll
+                for (int which = 0; which < 2; ++which, ++slot) {
+                    const int sl = slot % SLOTS;
+                    if (slot >= SLOTS) alive = wait(&empty[sl], ((slot / SLOTS) & 1) ^ 1, 12) && alive;
+                    alive = __all_sync(0xffffffffu, alive);
+                    if (lane == 0 && alive) {
+                        there_s[sl] = there;
+                        mbar_arrive_expect_tx(&full[sl], (uint32_t)bytes);
+                    }
+                    __syncwarp();
+                    if (count > 0 && alive) {
+                        uint8_t *dst = ring + sl * C::kSlotBytes;
+                        bulk_load(dst + lane * run_keys * D * C::EB, (which ? a.c.v : a.c.k) + row * D * C::EB, (uint32_t)(count * D * C::EB), &full[sl]);
+                        if constexpr (C::CODED) bulk_load(dst + C::UNIT * DP + lane * run_keys * 4, (which ? a.c.vs : a.c.ks) + row, (uint32_t)(scales * 4), &full[sl]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (abort_flag) linger();
+        return;
+    }
+
+    // ===================== the products =====================================================================
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); };       // of the four warps
+    auto leave = [&](int sl) {
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
+    };
+    uint32_t slot = 0;
+    int4 cut = make_int4(0, 0, 0, -1);
     for (; more; more = run.next()) {
         const Tile w = run.at();
         const Sequence &s = w.s;
-        const long long rows = (long long)s.n * a.group;
+        const int rows = (int)min((long long)s.n * a.group, 2147483647LL);
         const int row0 = w.tile * C::ROWS;
 
         // ---- Q as operands ----------------------------------------------------------------------------------------
-        __syncthreads();                         // (the tile before has been read)
-        for (int i = tid; i < (C::ROWS / 16) * C::STEPS * 32; i += kThreads) {
+        meet();                                      // (the tile before has been read)
+        if constexpr (HALF) {
+            // a power of two for each row brings its largest value to [2^14, 2^15)
+            for (int r = warp; r < C::ROWS; r += kWarps) {
+                const int row = row0 + r;
+                float most = 0.0f;
+                if (row < rows) {
+                    const T *src = static_cast<const T *>(a.q) + (long long)(s.first + row / a.group) * a.q_stride + (long long)(w.head * a.group + row % a.group) * D;
+                    for (int d = lane; d < D; d += 32) most = fmaxf(most, fabsf(to_float(src[d])));
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (lane == 0) q_unit[r] = pow2_scale(most);
+            }
+            meet();
+        }
+        for (int i = tid; i < (C::ROWS / 16) * C::STEPS * 32; i += 32 * kWarps) {
             const int l = i & 31, ks = (i >> 5) % C::STEPS, mt = (i >> 5) / C::STEPS;
             const int d = ((l & 3) + 4 * (ks / (C::EC / 4))) * C::EC + 4 * (ks % (C::EC / 4));
             float x[2][4];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const long long row = row0 + mt * 16 + (l >> 2) + 8 * r;
-                const bool there = row < rows && d < D;
-                const T *src = static_cast<const T *>(a.q) + (s.first + row / a.group) * a.q_stride + (long long)(w.head * a.group + (int)(row % a.group)) * D + d;
+                const int rr = mt * 16 + (l >> 2) + 8 * r, row = row0 + rr;
+                const bool here = row < rows && d < D;
+                const T *src = static_cast<const T *>(a.q) + (long long)(s.first + row / a.group) * a.q_stride + (long long)(w.head * a.group + row % a.group) * D + d;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[r][e] = there ? to_float(src[e]) : 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    x[r][e] = here ? to_float(src[e]) : 0.0f;
+                    if constexpr (HALF) x[r][e] *= q_unit[rr];
+                }
             }
 #pragma unroll
             for (int n = 0; n < C::NQ; ++n) {
                 uint4 f;
-                f.x = next_piece(x[0][0], x[0][1]);
-                f.y = next_piece(x[1][0], x[1][1]);
-                f.z = next_piece(x[0][2], x[0][3]);
-                f.w = next_piece(x[1][2], x[1][3]);
+                f.x = next_piece<HALF>(x[0][0], x[0][1]);
+                f.y = next_piece<HALF>(x[1][0], x[1][1]);
+                f.z = next_piece<HALF>(x[0][2], x[0][3]);
+                f.w = next_piece<HALF>(x[1][2], x[1][3]);
                 q_s[n * (C::ROWS / 16) * C::STEPS * 32 + i] = f;
             }
         }
-        __syncthreads();
+        meet();
         const uint4 *q_w = q_s + (SPLITROWS ? warp * C::MT * C::STEPS * 32 : 0) + lane;
 
         int limit[C::MT][2];
+        float factor[C::MT][2];                      // of the scores, to the logarithm to base two
         const int wrow = row0 + (SPLITROWS ? warp * 16 * C::MT : 0);
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) limit[mt][r] = limit_of(a, s, wrow + mt * 16 + g + 8 * r);
-        const int least_limit = limit_of(a, s, wrow);
+            for (int r = 0; r < 2; ++r) {
+                const int rr = mt * 16 + g + 8 * r;
+                limit[mt][r] = wrow + rr < rows ? limit_of(a, s, wrow + rr) : 0;
+                factor[mt][r] = a.cscale;
+                // (a masked score times 0 would be NaN)
+                if constexpr (HALF) factor[mt][r] = fmaxf(a.cscale * pow2_inverse(q_unit[wrow - row0 + rr]), 1.17549435e-38f);
+            }
+        const int least_limit = wrow < rows ? limit_of(a, s, wrow) : 0;
         const int keys = tile_keys<C::ROWS>(a, s, w.tile);
-        const long long wlast = min((long long)wrow + 16 * C::MT, rows) - 1;             // this warp's rows end here, and their keys
-        const int wkeys = !SPLITROWS ? keys : wlast < wrow ? 0 : limit_of(a, s, (int)wlast);
+        const int wlast = min(wrow + 16 * C::MT, rows) - 1;              // this warp's rows end here, and their keys
+        const int wkeys = !SPLITROWS ? keys : wlast < wrow ? 0 : limit_of(a, s, wlast);
 
         float o[C::MT][C::TILES][4], m[C::MT][2], l[C::MT][2];
+        int unit = -126;                             // codes: o is divided by 2^unit, which follows the largest scale of the values
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
@@ -156,281 +284,333 @@ paged_rows_kernel(const AttnArgs a)
         }
 
         // ---- blocks of KB keys ------------------------------------------------------------------------------------
-        constexpr int NG = C::KB / 16, NJ = C::KB / 8, PER_UNIT = C::UNIT / C::KB, STEP = SPLITROWS ? 1 : kWarps;
-        const int blk_end = min(w.to * PER_UNIT, (wkeys + C::KB - 1) / C::KB);
-        uint32_t kreg[NJ][C::NC][C::EC * C::EB / 4], vreg[NG][4][C::NV][C::EV * C::EB / 4];
-        float2 kscale[C::CODED ? NJ : 1], vscale[C::CODED ? NJ : 1];
-        long long at[NG], next_at[NG];           // the first row of each 16 keys in the cache
-        auto find = [&](long long (&where)[NG], int blk) {
+        constexpr int NG = C::KB / 16, NJ = C::KB / 8, BLOCKS = SPLITROWS ? C::UNIT / C::KB : 1;
+        const int pitch = D * C::EB;
+        for (int u = w.from; u < w.to; ++u, slot += 2) {
+            const int ksl = slot % SLOTS, vsl = (slot + 1) % SLOTS;
+            const uint8_t *k_at = ring + ksl * C::kSlotBytes, *v_at = ring + vsl * C::kSlotBytes;
+            wait(&full[ksl], (slot / SLOTS) & 1, 11);
+            const uint32_t there_all = *reinterpret_cast<volatile uint32_t *>(&there_s[ksl]);
+            bool v_here = false;
+#pragma unroll 1
+            for (int blk = 0; blk < BLOCKS; ++blk) {
+                const int k0 = (SPLITROWS ? blk : warp) * C::KB, p0 = u * C::UNIT + k0;      // the block's first key in its place, and in the sequence
+                if (p0 >= wkeys) break;
+                const uint32_t there = there_all >> (k0 / 16) & ((1u << NG) - 1);
+                const bool partial = p0 + C::KB > wkeys || there != (1u << NG) - 1;          // places without keys
+                const bool masked = p0 + C::KB > least_limit || there != (1u << NG) - 1;
+                // scores: the main products, and apart from them those of the smaller pieces
+                float z[C::MT][NJ][4], zc[C::NQ > 1 ? C::MT : 1][C::NQ > 1 ? NJ : 1][4];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int p = blk * C::KB + 16 * i;
-                where[i] = blk < blk_end && p < wkeys ? row_of(a.c, w.b, w.head, p) : -1;
-            }
-        };
-        auto load_k = [&](const long long (&where)[NG], int blk) {
+                for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int in = 8 * (j & 1) + g;
-                const bool there = where[j / 2] >= 0 && blk * C::KB + 16 * (j / 2) + in < wkeys;
-                const uint8_t *row = a.c.k + (where[j / 2] + in) * D * C::EB;
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            z[mt][j][e] = 0.0f;
+                            if constexpr (C::NQ > 1) zc[mt][j][e] = 0.0f;
+                        }
+                constexpr int PER = C::EC / 4;       // instructions a chunk
 #pragma unroll
                 for (int i = 0; i < C::NC; ++i) {
-                    const int d = (t4 + 4 * i) * C::EC;
-                    load_words<C::EC * C::EB>(kreg[j][i], row + d * C::EB, there && d < D);
-                }
-                if constexpr (C::CODED) kscale[j] = where[j / 2] >= 0 ? __ldg(reinterpret_cast<const float2 *>(a.c.ks + where[j / 2] + 8 * (j & 1) + 2 * t4)) : make_float2(0.0f, 0.0f);
-            }
-        };
-        auto load_v = [&](int blk) {
+                    uint32_t kw[NJ][C::EC * C::EB / 4];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
+                    for (int j = 0; j < NJ; ++j) {
+                        const int d = (t4 + 4 * i) * C::EC;
+                        if (d < D) read_words<C::EC * C::EB>(kw[j], k_at + (k0 + 8 * j + g) * pitch + d * C::EB);
+                        else
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int in = 8 * (x >> 1) + 2 * t4 + (x & 1);
-                    const bool there = at[i] >= 0 && blk * C::KB + 16 * i + in < wkeys;
-                    const uint8_t *row = a.c.v + (at[i] + in) * D * C::EB;
-#pragma unroll
-                    for (int c = 0; c < C::NV; ++c) {
-                        const int d = (g + 8 * c) * C::EV;
-                        load_words<C::EV * C::EB>(vreg[i][x][c], row + d * C::EB, there && d < D);
-                    }
-                }
-            }
-            if constexpr (C::CODED)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) vscale[j] = at[j / 2] >= 0 ? __ldg(reinterpret_cast<const float2 *>(a.c.vs + at[j / 2] + 8 * (j & 1) + 2 * t4)) : make_float2(0.0f, 0.0f);
-        };
-        const int blk0 = w.from * PER_UNIT + (SPLITROWS ? 0 : warp);
-        find(at, blk0);
-        load_k(at, blk0);
-        for (int blk = blk0; blk < blk_end; blk += STEP) {
-            load_v(blk);
-            find(next_at, blk + STEP);
-            // scores: the main products, and apart from them those of the smaller pieces
-            float z[C::MT][NJ][4], zc[C::F32 ? C::MT : 1][C::F32 ? NJ : 1][4];
-#pragma unroll
-            for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        z[mt][j][e] = 0.0f;
-                        if constexpr (C::F32) zc[mt][j][e] = 0.0f;
+                            for (int x = 0; x < C::EC * C::EB / 4; ++x) kw[j][x] = 0u;
                     }
 #pragma unroll
-            for (int ks = 0; ks < C::STEPS; ++ks) {
-                uint4 q[C::NQ][C::MT];
+                    for (int x = 0; x < PER; ++x) {
+                        uint4 q[C::NQ][C::MT];
 #pragma unroll
-                for (int n = 0; n < C::NQ; ++n)
+                        for (int n = 0; n < C::NQ; ++n)
 #pragma unroll
-                    for (int mt = 0; mt < C::MT; ++mt) q[n][mt] = q_w[(n * (C::ROWS / 16) + mt) * C::STEPS * 32 + ks * 32];
-                constexpr int PER = C::EC / 4;
+                            for (int mt = 0; mt < C::MT; ++mt) q[n][mt] = q_w[(n * (C::ROWS / 16) + mt) * C::STEPS * 32 + (i * PER + x) * 32];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const uint32_t *kw = kreg[j][ks / PER];
-                    uint32_t b[C::NK][2];
-                    if constexpr (C::CODED) {
-                        const uint32_t x = kw[ks % PER];
-                        b[0][0] = code_pair<FMT>(x, x, 0, 1);
-                        b[0][1] = code_pair<FMT>(x, x, 2, 3);
-                    } else if constexpr (!C::F32) {
-                        b[0][0] = kw[2 * (ks % PER)];
-                        b[0][1] = kw[2 * (ks % PER) + 1];
-                    } else {
-                        float x[4] = {__uint_as_float(kw[0]), __uint_as_float(kw[1]), __uint_as_float(kw[2]), __uint_as_float(kw[3])};
+                        for (int j = 0; j < NJ; ++j) {
+                            uint32_t b[C::NK][2];
+                            if constexpr (C::CODED) {
+                                codes_to_half<FMT>(kw[j][x], b[0][0], b[0][1]);
+                            } else if constexpr (!C::F32) {
+                                b[0][0] = kw[j][2 * x];
+                                b[0][1] = kw[j][2 * x + 1];
+                            } else {
+                                float y[4] = {__uint_as_float(kw[j][0]), __uint_as_float(kw[j][1]), __uint_as_float(kw[j][2]), __uint_as_float(kw[j][3])};
 #pragma unroll
-                        for (int n = 0; n < 3; ++n) {
-                            b[n][0] = next_piece(x[0], x[1]);
-                            b[n][1] = next_piece(x[2], x[3]);
+                                for (int n = 0; n < 3; ++n) {
+                                    b[n][0] = next_piece<false>(y[0], y[1]);
+                                    b[n][1] = next_piece<false>(y[2], y[3]);
+                                }
+                            }
+#pragma unroll
+                            for (int mt = 0; mt < C::MT; ++mt) {
+#pragma unroll
+                                for (int order = C::NQ - 1; order >= 1; --order)
+#pragma unroll
+                                    for (int n = 0; n <= order && n < C::NK; ++n) mma16<HALF>(zc[mt][j], q[order - n][mt], b[n][0], b[n][1]);
+                                mma16<HALF>(z[mt][j], q[0][mt], b[0][0], b[0][1]);
+                            }
                         }
                     }
-#pragma unroll
-                    for (int mt = 0; mt < C::MT; ++mt) {
-                        if constexpr (C::F32) {
-#pragma unroll
-                            for (int order = 2; order >= 1; --order)
-#pragma unroll
-                                for (int n = 0; n <= order && n < C::NK; ++n) mma16(zc[mt][j], q[order - n][mt], b[n][0], b[n][1]);
-                        }
-                        mma16(z[mt][j], q[0][mt], b[0][0], b[0][1]);
-                    }
                 }
-            }
-            float2 ks2[C::CODED ? NJ : 1];
-            if constexpr (C::CODED)
+                float2 ks2[C::CODED ? NJ : 1], vs2[C::CODED ? NJ : 1];
+                if constexpr (C::CODED)
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) ks2[j] = kscale[j];
-            load_k(next_at, blk + STEP);
+                    for (int j = 0; j < NJ; ++j) ks2[j] = *reinterpret_cast<const float2 *>(k_at + C::UNIT * DP + (k0 + 8 * j + 2 * t4) * 4);
+                if (!v_here) {
+                    wait(&full[vsl], ((slot + 1) / SLOTS) & 1, 11);
+                    v_here = true;
+                }
 
-            // ---- softmax ----------------------------------------------------------------------------------------------
-            const int p0 = blk * C::KB;
-            bool masked = p0 + C::KB > least_limit;
+                // ---- softmax ----------------------------------------------------------------------------------------------
+                auto seen = [&](int mt, int j, int e) { return p0 + 8 * j + 2 * t4 + (e & 1) < limit[mt][e >> 1] && (there >> (j >> 1) & 1); };
+                float shrink = 1.0f;
+                if constexpr (C::CODED) {
+                    // P times the scales of the values, over 2^unit: at most 2^15
+                    uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) masked = masked || at[i] < 0;
-            uint4 p[C::NQ][C::MT][NG];
-#pragma unroll
-            for (int mt = 0; mt < C::MT; ++mt) {
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = z[mt][j][e];
-                        if constexpr (C::F32) x += zc[mt][j][e];
-                        if constexpr (C::CODED) x *= (e & 1) ? ks2[j].y : ks2[j].x;
-                        x *= a.cscale;
-                        if (masked && !(p0 + 8 * j + 2 * t4 + (e & 1) < limit[mt][e >> 1] && at[j / 2] >= 0)) x = -INFINITY;
-                        z[mt][j][e] = x;
-                        top[e >> 1] = fmaxf(top[e >> 1], x);
-                    }
-                float base[2], alpha[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    const float now = fmaxf(m[mt][r], top[r]);
-                    base[r] = now == -INFINITY ? 0.0f : now;
-                    alpha[r] = ex2_approx(m[mt][r] - base[r]);
-                    m[mt][r] = now;
-                    l[mt][r] *= alpha[r];
-                }
-                if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-                    for (int j = 0; j < C::TILES; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[e >> 1];
-                }
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = z[mt][j][e];
-                        float y = ex2_approx(x - base[e >> 1]);
-                        l[mt][e >> 1] += y;
-                        if constexpr (C::CODED) {
-                            y *= (e & 1) ? vscale[j].y : vscale[j].x;
-                            if (masked && x == -INFINITY) y = 0.0f;              // (the scale of a place that holds nothing may be anything)
+                    for (int j = 0; j < NJ; ++j) {
+                        vs2[j] = *reinterpret_cast<const float2 *>(v_at + C::UNIT * DP + (k0 + 8 * j + 2 * t4) * 4);
+                        if (partial) {
+                            const int p = p0 + 8 * j + 2 * t4;
+                            vs2[j].x = p < wkeys && (there >> (j >> 1) & 1) ? vs2[j].x : 0.0f;
+                            vs2[j].y = p + 1 < wkeys && (there >> (j >> 1) & 1) ? vs2[j].y : 0.0f;
                         }
-                        z[mt][j][e] = y;
+                        const uint32_t bx = __float_as_uint(vs2[j].x), by = __float_as_uint(vs2[j].y);
+                        most = max(most, max(bx < 0x7F800000u ? bx : 0u, by < 0x7F800000u ? by : 0u));
+                    }
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    const int e = max((int)(most >> 23) - 127 - 13, -126);       // (p <= 1, the scale < 2 * 2^13 then)
+                    if (e > unit) {
+                        shrink = ex2_approx((float)max(unit - e, -126));
+                        unit = e;
+                    }
+                    const float down = __uint_as_float((uint32_t)(127 - min(unit, 126)) << 23);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        vs2[j].x *= down;
+                        vs2[j].y *= down;
+                    }
+                }
+                uint4 p[C::NQ][C::MT][NG];
+#pragma unroll
+                for (int mt = 0; mt < C::MT; ++mt) {
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = z[mt][j][e];
+                            if constexpr (C::NQ > 1) x += zc[mt][j][e];
+                            if constexpr (C::CODED) x *= (e & 1) ? ks2[j].y : ks2[j].x;
+                            x *= factor[mt][e >> 1];
+                            if (masked && !seen(mt, j, e)) x = -INFINITY;
+                            z[mt][j][e] = x;
+                            top[e >> 1] = fmaxf(top[e >> 1], x);
+                        }
+                    float base[2], alpha[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                        const float now = fmaxf(m[mt][r], top[r]);
+                        base[r] = now == -INFINITY ? 0.0f : now;
+                        alpha[r] = ex2_approx(m[mt][r] - base[r]);
+                        m[mt][r] = now;
+                        l[mt][r] *= alpha[r];
+                        alpha[r] *= shrink;
+                    }
+                    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                        for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[e >> 1];
                     }
 #pragma unroll
-                for (int i = 0; i < NG; ++i)
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int n = 0; n < C::NQ; ++n) {
-                        p[n][mt][i].x = next_piece(z[mt][2 * i][0], z[mt][2 * i][1]);
-                        p[n][mt][i].y = next_piece(z[mt][2 * i][2], z[mt][2 * i][3]);
-                        p[n][mt][i].z = next_piece(z[mt][2 * i + 1][0], z[mt][2 * i + 1][1]);
-                        p[n][mt][i].w = next_piece(z[mt][2 * i + 1][2], z[mt][2 * i + 1][3]);
-                    }
-            }
-
-            // ---- P V --------------------------------------------------------------------------------------------------
-#pragma unroll
-            for (int c = 0; c < C::NV; ++c)
-#pragma unroll
-                for (int e = 0; e < C::EV; ++e) {
-                    const int j = c * C::EV + e;
-                    uint32_t b[NG][C::NK][2];
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = z[mt][j][e];
+                            float y = ex2_approx(x - base[e >> 1]);
+                            l[mt][e >> 1] += y;
+                            if constexpr (C::CODED) {
+                                y *= (e & 1) ? vs2[j].y : vs2[j].x;
+                                if (masked && x == -INFINITY) y = 0.0f;      // (the scale of a value that a row does not see may be anything)
+                            }
+                            z[mt][j][e] = y;
+                        }
 #pragma unroll
                     for (int i = 0; i < NG; ++i)
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const uint32_t *w0 = vreg[i][2 * hf][c], *w1 = vreg[i][2 * hf + 1][c];
-                            if constexpr (C::CODED) {
-                                b[i][0][hf] = code_pair<FMT>(w0[e / 4], w1[e / 4], e & 3, e & 3);
-                            } else if constexpr (!C::F32) {
-                                b[i][0][hf] = __byte_perm(w0[e / 2], w1[e / 2], e & 1 ? 0x7632 : 0x5410);
-                            } else {
-                                float x = __uint_as_float(w0[e]), y = __uint_as_float(w1[e]);
+                        for (int n = 0; n < C::NQ; ++n) {
+                            p[n][mt][i].x = next_piece<HALF>(z[mt][2 * i][0], z[mt][2 * i][1]);
+                            p[n][mt][i].y = next_piece<HALF>(z[mt][2 * i][2], z[mt][2 * i][3]);
+                            p[n][mt][i].z = next_piece<HALF>(z[mt][2 * i + 1][0], z[mt][2 * i + 1][1]);
+                            p[n][mt][i].w = next_piece<HALF>(z[mt][2 * i + 1][2], z[mt][2 * i + 1][3]);
+                        }
+                }
+
+                if (blk == BLOCKS - 1 || p0 + C::KB >= wkeys) leave(ksl);        // (what was read of it has been used: an arrival does not wait for loads)
+
+                // ---- P V --------------------------------------------------------------------------------------------------
 #pragma unroll
-                                for (int n = 0; n < 3; ++n) b[i][n][hf] = next_piece(x, y);
+                for (int c = 0; c < C::NV; ++c) {
+                    const int d = (g + 8 * c) * C::EV;
+                    uint32_t vw[NG][4][C::EV * C::EB / 4];
+#pragma unroll
+                    for (int i = 0; i < NG; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int in = 16 * i + 8 * (x >> 1) + 2 * t4 + (x & 1);
+                            // what lies in places without keys may be anything
+                            if (d < D && (!partial || (p0 + in < wkeys && (there >> i & 1)))) read_words<C::EV * C::EB>(vw[i][x], v_at + (k0 + in) * pitch + d * C::EB);
+                            else
+#pragma unroll
+                                for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[i][x][y] = 0u;
+                        }
+                    constexpr int W = C::CODED ? least_of(C::EV, 4) : 1;         // columns at a time: those of one word of codes
+#pragma unroll
+                    for (int e = 0; e < C::EV; e += W) {
+                        uint32_t b[NG][W][C::NK][2];
+#pragma unroll
+                        for (int i = 0; i < NG; ++i)
+#pragma unroll
+                            for (int hf = 0; hf < 2; ++hf) {
+                                const uint32_t *w0 = vw[i][2 * hf], *w1 = vw[i][2 * hf + 1];
+                                if constexpr (C::CODED) {
+                                    codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x5140), b[i][0][0][hf], b[i][1][0][hf]);
+                                    codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x7362), b[i][2][0][hf], b[i][3][0][hf]);
+                                } else if constexpr (!C::F32) {
+                                    b[i][0][0][hf] = __byte_perm(w0[e / 2], w1[e / 2], e & 1 ? 0x7632 : 0x5410);
+                                } else {
+                                    float x = __uint_as_float(w0[e]), y = __uint_as_float(w1[e]);
+#pragma unroll
+                                    for (int n = 0; n < 3; ++n) b[i][0][n][hf] = next_piece<false>(x, y);
+                                }
                             }
-                        }
 #pragma unroll
-                    for (int mt = 0; mt < C::MT; ++mt) {
-                        if constexpr (C::F32) {
-                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int x = 0; x < W; ++x)
 #pragma unroll
-                            for (int order = 2; order >= 0; --order)
+                            for (int mt = 0; mt < C::MT; ++mt) {
+                                const int j = c * C::EV + e + x;
+                                if constexpr (C::F32) {
+                                    float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                                for (int n = 0; n <= order && n < C::NK; ++n)
+                                    for (int order = C::NQ - 1; order >= 0; --order)
 #pragma unroll
-                                    for (int i = 0; i < NG; ++i) mma16(d, p[order - n][mt][i], b[i][n][0], b[i][n][1]);
+                                        for (int n = 0; n <= order && n < C::NK; ++n)
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) o[mt][j][x] += d[x];
-                        } else {
+                                            for (int i = 0; i < NG; ++i) mma16<HALF>(d4, p[order - n][mt][i], b[i][x][n][0], b[i][x][n][1]);
 #pragma unroll
-                            for (int i = 0; i < NG; ++i) mma16(o[mt][j], p[0][mt][i], b[i][0][0], b[i][0][1]);
-                        }
+                                    for (int y = 0; y < 4; ++y) o[mt][j][y] += d4[y];
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < NG; ++i) mma16<HALF>(o[mt][j], p[0][mt][i], b[i][x][0][0], b[i][x][0][1]);
+                                }
+                            }
                     }
                 }
-#pragma unroll
-            for (int i = 0; i < NG; ++i) at[i] = next_at[i];
+            }
+            // (a warp without keys here gives the places back when they have come)
+            if ((SPLITROWS ? 0 : warp * C::KB) + u * C::UNIT >= wkeys) leave(ksl);
+            if (!v_here) wait(&full[vsl], ((slot + 1) / SLOTS) & 1, 11);
+            leave(vsl);
         }
+        const float grown = C::CODED ? __uint_as_float((uint32_t)(127 + min(unit, 126)) << 23) : 1.0f;
 #pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt)
+        for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 1);
                 l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 2);
             }
+            if constexpr (C::CODED)
+#pragma unroll
+                for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[mt][j][e] *= grown;
+        }
 
         // ---- the tile's end ---------------------------------------------------------------------------------------
         const int part = run.part();
         if (part >= 0 && (part & 1)) cut = run.cut();
+        const bool store = !abort_flag;
         float *dst = part < 0 ? nullptr : a.parts + (size_t)part * C::ROWS * (DP + 2);
         // columns of TILES' tile c * EV + e: values (2 t4 + 8 c) EV + e and (2 t4 + 1 + 8 c) EV + e
         if constexpr (!SPLITROWS) {
-            // the warps' sums by way of shared memory; a warp joins four rows
+            // the warps' sums by way of shared memory: two of them leave theirs, the others add their own, then a warp joins four rows
+            auto row_at = [&](int buf, int r) { return o_s + (buf * 16 + g + 8 * r) * C::kPad; };
+            auto put = [&](int buf) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float *row = o_s + (warp * 16 + g + 8 * r) * C::kPad;
+                for (int r = 0; r < 2; ++r) {
+                    float *row = row_at(buf, r);
 #pragma unroll
-                for (int c = 0; c < C::NV; ++c)
+                    for (int c = 0; c < C::NV; ++c)
 #pragma unroll
-                    for (int e = 0; e < C::EV; ++e) {
-                        row[(2 * t4 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r];
-                        row[(2 * t4 + 1 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r + 1];
-                    }
-                if (t4 == 0) ml_s[warp][g + 8 * r] = make_float2(m[0][r], l[0][r]);
-            }
-            __syncthreads();
-            for (int r = warp; r < 16; r += kWarps) {
-                const long long row = row0 + r;
-                if (row >= rows) break;
-                float top = -INFINITY, sum = 0.0f, f[kWarps];
-#pragma unroll
-                for (int x = 0; x < kWarps; ++x) top = fmaxf(top, ml_s[x][r].x);
-                const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-                for (int x = 0; x < kWarps; ++x) {
-                    f[x] = ex2_approx(ml_s[x][r].x - base);
-                    sum = fmaf(ml_s[x][r].y, f[x], sum);
+                        for (int e = 0; e < C::EV; ++e) {
+                            row[(2 * t4 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r];
+                            row[(2 * t4 + 1 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r + 1];
+                        }
+                    if (t4 == 0) ml_s[buf][g + 8 * r] = make_float2(m[0][r], l[0][r]);
                 }
+            };
+            if (warp >= 2) put(warp - 2);
+            meet();
+            if (warp < 2) {
+                float2 other[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) other[r] = ml_s[warp][g + 8 * r];
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float now = fmaxf(m[0][r], other[r].x), base = now == -INFINITY ? 0.0f : now;
+                    const float f0 = ex2_approx(m[0][r] - base), f1 = ex2_approx(other[r].x - base);
+                    const float *row = row_at(warp, r);
+                    m[0][r] = now;
+                    l[0][r] = fmaf(l[0][r], f0, other[r].y * f1);
+#pragma unroll
+                    for (int c = 0; c < C::NV; ++c)
+#pragma unroll
+                        for (int e = 0; e < C::EV; ++e) {
+                            float *x = &o[0][c * C::EV + e][2 * r];
+                            x[0] = fmaf(x[0], f0, row[(2 * t4 + 8 * c) * C::EV + e] * f1);
+                            x[1] = fmaf(x[1], f0, row[(2 * t4 + 1 + 8 * c) * C::EV + e] * f1);
+                        }
+                }
+                put(warp);                           // (a thread reads and writes the same places)
+            }
+            meet();
+            for (int r = warp; r < 16; r += kWarps) {
+                const int row = row0 + r;
+                if (row >= rows) break;
+                const float2 x0 = ml_s[0][r], x1 = ml_s[1][r];
+                const float top = fmaxf(x0.x, x1.x), base = top == -INFINITY ? 0.0f : top;
+                const float f0 = ex2_approx(x0.x - base), f1 = ex2_approx(x1.x - base), sum = fmaf(x0.y, f0, x1.y * f1);
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const long long t = s.first + row / a.group;
-                T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + (int)(row % a.group)) * D;
+                T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + row % a.group) * D;
                 bool wild = false;
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) {
                     const int d = lane + 32 * i;
-                    float y = 0.0f;
-#pragma unroll
-                    for (int x = 0; x < kWarps; ++x) y = fmaf(o_s[(x * 16 + r) * C::kPad + d], f[x], y);
+                    float y = fmaf(o_s[r * C::kPad + d], f0, o_s[(16 + r) * C::kPad + d] * f1);
                     if (dst) {
-                        dst[(size_t)r * DP + d] = y;
+                        if (store) dst[(size_t)r * DP + d] = y;
                     } else {
                         y = sum == 0.0f ? 0.0f : y * inv;
                         wild = wild || !(fabsf(y) <= 3.402823466e38f);
-                        if (d < D) out[d] = from_float<T>(y);
+                        if (d < D && store) out[d] = from_float<T>(y);
                     }
                 }
                 if (dst) {
-                    if (lane == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[r] = make_float2(top, sum);
-                } else if (__any_sync(0xffffffffu, wild)) {
+                    if (lane == 0 && store) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[r] = make_float2(top, sum);
+                } else if (__any_sync(0xffffffffu, wild) && store) {
                     __syncwarp();
-                    mend_row<T, FMT>(a, w.b, w.head, s, (int)row, keys);
+                    mend_row<T, FMT>(a, w.b, w.head, s, row, keys);
                 }
             }
         } else {
@@ -440,29 +620,28 @@ paged_rows_kernel(const AttnArgs a)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     wild[mt][r] = false;
-                    const int rr = (warp * C::MT + mt) * 16 + g + 8 * r;
-                    const long long row = row0 + rr;
+                    const int rr = (warp * C::MT + mt) * 16 + g + 8 * r, row = row0 + rr;
                     const float sum = l[mt][r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const bool there = row < rows;
+                    const bool here = row < rows && store;
                     const long long t = s.first + row / a.group;
-                    T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + (int)(row % a.group)) * D;
+                    T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + row % a.group) * D;
 #pragma unroll
                     for (int c = 0; c < C::NV; ++c)
 #pragma unroll
-                        for (int e = 0; e < C::EV; ++e)
+                        for (int x = 0; x < 2; ++x)
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
+                            for (int e = 0; e < C::EV; ++e) {
                                 const int d = (2 * t4 + x + 8 * c) * C::EV + e;
                                 const float y = o[mt][c * C::EV + e][2 * r + x];
                                 if (dst) {
-                                    if (there) dst[(size_t)rr * DP + d] = y;
+                                    if (here) dst[(size_t)rr * DP + d] = y;
                                 } else {
                                     const float v = sum == 0.0f ? 0.0f : y * inv;
-                                    wild[mt][r] = wild[mt][r] || (there && !(fabsf(v) <= 3.402823466e38f));
-                                    if (there && d < D) out[d] = from_float<T>(v);
+                                    wild[mt][r] = wild[mt][r] || (here && !(fabsf(v) <= 3.402823466e38f));
+                                    if (here && d < D) out[d] = from_float<T>(v);
                                 }
                             }
-                    if (dst && there && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[mt][r], sum);
+                    if (dst && here && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[mt][r], sum);
                 }
             if (!dst) {
 #pragma unroll
@@ -480,9 +659,10 @@ paged_rows_kernel(const AttnArgs a)
             }
         }
     }
+    meet();
     if (a.cuts && tid == 0) {
         a.cuts[blockIdx.x] = cut;
-        a.whole[blockIdx.x] = 1;
+        a.whole[blockIdx.x] = !abort_flag;
     }
 }
 
@@ -549,6 +729,19 @@ int launch_paged(int format, const AttnArgs &a, cudaStream_t st)
 }  // namespace
 
 void paged_release_scratch() { g_paged_ws.release(); }
+
+int paged_rows_status_fetch(int *status)
+{
+    int s = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&s, g_rows_status, sizeof(int));
+    if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
+    if (s != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_rows_status, &zero, sizeof(int));
+    }
+    *status = s;
+    return HIPGPT_OK;
+}
 
 }  // namespace hipgpt
 

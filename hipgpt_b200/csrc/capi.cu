@@ -167,6 +167,7 @@ static int fetch_status_words(int *status)
     if (rc == HIPGPT_OK) rc = loss_status_fetch(&ls);
     if (rc == HIPGPT_OK) rc = embedding_status_fetch(&em);
     if (rc == HIPGPT_OK) rc = paged_status_fetch(&pg);
+    if (rc == HIPGPT_OK && !pg) rc = paged_rows_status_fetch(&pg);
     if (rc != HIPGPT_OK) return rc;
     *status = a ? a : (b ? 100 + b : (d ? 300 + d : (h ? 400 + h : (gm ? 500 + gm : (bw ? 600 + bw : (ls ? 700 + ls : (em ? 800 + em : (pr ? 900 + pr : (pg ? 1000 + pg : 0)))))))));
     return HIPGPT_OK;

@@ -51,6 +51,22 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w0, uint32_t w1, int byte
     else return int8_to_bf16x2(__byte_perm(w0, w1, byte0 | ((4 + byte1) << 8)));
 }
 
+// ... and as fp16, for products
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// Four codes as fp16 (exact), in two words
+template <int FMT>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    if constexpr (FMT == HIPGPT_CACHE_E4M3) {
+        asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        w ^= 0x80808080u;                            // 128 more, without sign; 0x64 above a byte u is 1024 + u
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
+    }
+}
+
 // What the host checks of a cache and a batch (0: go on, 1: nothing to do, < 0: refused)
 inline int check_paged(const hipgpt_paged_cache *c, const hipgpt_paged_batch *b, PagedView *out)
 {

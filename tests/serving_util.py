@@ -145,6 +145,11 @@ def attention(batch, k, v, q, H, causal, scale, dtype, fmt):
             keys = len(kk)
             rel = rel + (keys / 16 + 32) * step                             # sums of probabilities and of P V
             pv = torch.einsum("ngk,kd->ngd", p * rel, vv.abs()) + o.abs() * (p * rel).sum(-1, keepdim=True)
+            if fmt != "plain":
+                # Codes: a probability times its value's scale is held in fp16 pieces, divided by a power of two that brings the largest such product to 2^13 at least.  Below fp16's normal numbers
+                # the pieces stop at its smallest step, 2^-24: half of one, 2^-25, of a code, that is 2^-38 of the largest scale times the code, for each key.  A scale times its code is less than
+                # twice the largest value of a row (e4m3: the largest is above 224 scales, of 448).
+                pv = pv + keys * 2.0 ** -37 * vv.abs().max()
             o = o.masked_fill((seen & wild[None]).any(-1)[:, None, None], float("nan"))
             out[f:f + n, h * G:(h + 1) * G] = o
             bound[f:f + n, h * G:(h + 1) * G] = pv + HALF[dtype] * (o.abs() + pv) + 1e-37
