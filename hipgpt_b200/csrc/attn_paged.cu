@@ -98,6 +98,56 @@ struct Shape {
     static constexpr int kBlocks = kSmem <= 112 * 1024 ? 2 : 1;         // an SM
 };
 
+// The warp that asks for the copies: a place of the ring takes UNIT keys or values as they lie in their pages, then their scales; a lane a run of keys in one page
+template <typename C, int THREADS, typename Wait>
+__device__ __forceinline__ void bring(const AttnArgs &a, Run<C::ROWS, C::UNIT, THREADS> &run, bool more, uint8_t *ring, uint64_t *full, uint64_t *empty, uint32_t *there_s, Wait wait)
+{
+    const int lane = threadIdx.x & 31, D = a.c.D;
+    uint32_t slot = 0;
+    const int page_keys = 1 << a.c.shift, run_keys = min(page_keys, C::UNIT), runs = C::UNIT / run_keys;
+    bool alive = true;
+    for (; more; more = run.next()) {
+        const Tile w = run.at();
+        const int keys = tile_keys<C::ROWS>(a, w.s, w.tile);
+        auto look = [&](int u) {                     // a page for each run of keys, asked for a unit ahead
+            const int p = u * C::UNIT + lane * run_keys;
+            const int pg = lane < runs && p < keys ? __ldg(a.c.table + (size_t)w.b * a.c.most_pages + (p >> a.c.shift)) : -1;
+            return pg < a.c.pages ? pg : -1;
+        };
+        int page = look(w.from);
+        for (int u = w.from; u < w.to; ++u) {
+            const int p = u * C::UNIT + lane * run_keys;
+            const int count = page >= 0 ? min(run_keys, keys - p) : 0, scales = C::CODED ? (count + 3) & ~3 : 0;         // (whole 16 bytes of scales)
+            const long long row = ((((long long)page * a.c.heads) + w.head) << a.c.shift) + (p & (page_keys - 1));
+            int bytes = count * D * C::EB + scales * 4;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
+            // one bit for each sixteen keys
+            const uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
+            uint32_t there = 0;
+#pragma unroll
+            for (int i = 0; i < C::UNIT / 16; ++i) there |= (some >> (16 * i / run_keys) & 1u) << i;
+            page = u + 1 < w.to ? look(u + 1) : -1;
+#pragma unroll
+            for (int which = 0; which < 2; ++which, ++slot) {
+                const int sl = slot % C::kSlots;
+                if (slot >= C::kSlots) alive = wait(&empty[sl], ((slot / C::kSlots) & 1) ^ 1, 12) && alive;
+                alive = __all_sync(0xffffffffu, alive);
+                if (lane == 0 && alive) {
+                    there_s[sl] = there;
+                    mbar_arrive_expect_tx(&full[sl], (uint32_t)bytes);
+                }
+                __syncwarp();
+                if (count > 0 && alive) {
+                    uint8_t *dst = ring + sl * C::kSlotBytes;
+                    bulk_load(dst + lane * run_keys * D * C::EB, (which ? a.c.v : a.c.k) + row * D * C::EB, (uint32_t)(count * D * C::EB), &full[sl]);
+                    if constexpr (C::CODED) bulk_load(dst + C::UNIT * C::STEPS * 16 + lane * run_keys * 4, (which ? a.c.vs : a.c.ks) + row, (uint32_t)(scales * 4), &full[sl]);
+                }
+            }
+        }
+    }
+}
+
 template <typename T, int FMT, int DP, bool SPLITROWS>
 __global__ void __launch_bounds__(kThreads, Shape<T, FMT, DP, SPLITROWS>::kBlocks)
 paged_rows_kernel(const AttnArgs a)
@@ -145,50 +195,7 @@ paged_rows_kernel(const AttnArgs a)
     bool more = run.begin(sums);
 
     if (warp == kWarps) {
-        // ================= the copies ============================================================================
-        uint32_t slot = 0;
-        const int page_keys = 1 << a.c.shift, run_keys = min(page_keys, C::UNIT), runs = C::UNIT / run_keys;
-        bool alive = true;
-        for (; more; more = run.next()) {
-            const Tile w = run.at();
-            const int keys = tile_keys<C::ROWS>(a, w.s, w.tile);
-            auto look = [&](int u) {                 // a page for each run of keys, asked for a unit ahead
-                const int p = u * C::UNIT + lane * run_keys;
-                const int pg = lane < runs && p < keys ? __ldg(a.c.table + (size_t)w.b * a.c.most_pages + (p >> a.c.shift)) : -1;
-                return pg < a.c.pages ? pg : -1;
-            };
-            int page = look(w.from);
-            for (int u = w.from; u < w.to; ++u) {
-                const int p = u * C::UNIT + lane * run_keys;
-                const int count = page >= 0 ? min(run_keys, keys - p) : 0, scales = C::CODED ? (count + 3) & ~3 : 0;
-                const long long row = ((((long long)page * a.c.heads) + w.head) << a.c.shift) + (p & (page_keys - 1));
-                int bytes = count * D * C::EB + scales * 4;
-#pragma unroll
-                for (int o = 16; o; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
-                // one bit for each sixteen keys
-                const uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
-                uint32_t there = 0;
-#pragma unroll
-                for (int i = 0; i < C::UNIT / 16; ++i) there |= (some >> (16 * i / run_keys) & 1u) << i;
-                page = u + 1 < w.to ? look(u + 1) : -1;
-#pragma unroll
-                for (int which = 0; which < 2; ++which, ++slot) {
-                    const int sl = slot % SLOTS;
-                    if (slot >= SLOTS) alive = wait(&empty[sl], ((slot / SLOTS) & 1) ^ 1, 12) && alive;
-                    alive = __all_sync(0xffffffffu, alive);
-                    if (lane == 0 && alive) {
-                        there_s[sl] = there;
-                        mbar_arrive_expect_tx(&full[sl], (uint32_t)bytes);
-                    }
-                    __syncwarp();
-                    if (count > 0 && alive) {
-                        uint8_t *dst = ring + sl * C::kSlotBytes;
-                        bulk_load(dst + lane * run_keys * D * C::EB, (which ? a.c.v : a.c.k) + row * D * C::EB, (uint32_t)(count * D * C::EB), &full[sl]);
-                        if constexpr (C::CODED) bulk_load(dst + C::UNIT * DP + lane * run_keys * 4, (which ? a.c.vs : a.c.ks) + row, (uint32_t)(scales * 4), &full[sl]);
-                    }
-                }
-            }
-        }
+        bring<C, kThreads>(a, run, more, ring, full, empty, there_s, wait);
         __syncwarp();
         if (abort_flag) linger();
         return;
@@ -666,11 +673,442 @@ paged_rows_kernel(const AttnArgs a)
     }
 }
 
-template <typename T, int FMT, int DP, bool SPLITROWS>
-int launch_rows(AttnArgs a, cudaStream_t st)
+// ---- eight rows at most: single tokens -------------------------------------------------------------------------------------
+// The products the other way round, S^T = K Q^T and O^T = V^T P^T: sixteen keys (or columns of V) by eight rows an instruction, so no half of it is empty, and half the registers hold the sums.  A thread
+// takes its bytes of K and V as before; P^T as a result has its keys where the operand has its rows, and eight by eight of them are turned by one instruction.
+
+template <typename T, int FMT, int DP>
+struct TokenShape {
+    using R = Shape<T, FMT, DP, false>;
+    static constexpr bool F32 = R::F32, CODED = R::CODED;
+    static constexpr int EB = R::EB, NQ = R::NQ, NK = R::NK, ROWS = 8, KB = R::KB, UNIT = kWarps * KB;
+    static constexpr int EC = R::EC, NC = R::NC, EV = R::EV, NV = R::NV, STEPS = DP / 16, TILES = DP / 16;
+    static constexpr int kQBytes = NQ * STEPS * 32 * 8, kPad = DP + 4, kOBytes = kWarps * 8 * kPad * 4;
+    static constexpr int kSlotBytes = R::kSlotBytes;
+    static constexpr int kBudget = (F32 && DP == 128 ? 112 : 74) * 1024;         // three blocks an SM (two where the sums of wide fp32 rows take the registers)
+    static constexpr int kSlots = most_of(3, least_of(12, (kBudget - kQBytes - kOBytes - 1024) / kSlotBytes));
+    static constexpr size_t kSmem = (size_t)kQBytes + kOBytes + (size_t)kSlots * kSlotBytes;
+    static constexpr int kBlocks = kSmem > 112 * 1024 ? 1 : F32 && DP == 128 ? 2 : 3;
+};
+
+__device__ __forceinline__ uint32_t turned8(uint32_t x)
 {
-    using C = Shape<T, FMT, DP, SPLITROWS>;
-    const auto kern = paged_rows_kernel<T, FMT, DP, SPLITROWS>;
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+template <typename T, int FMT, int DP>
+__global__ void __launch_bounds__(kThreads, TokenShape<T, FMT, DP>::kBlocks)
+paged_token_kernel(const AttnArgs a)
+{
+    using C = TokenShape<T, FMT, DP>;
+    constexpr bool HALF = C::CODED;
+    constexpr int SLOTS = C::kSlots;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *ring = smem;
+    uint2 *q_s = reinterpret_cast<uint2 *>(smem + SLOTS * C::kSlotBytes);
+    float *o_s = reinterpret_cast<float *>(smem + SLOTS * C::kSlotBytes + C::kQBytes);
+    __shared__ uint64_t full[SLOTS], empty[SLOTS];
+    __shared__ uint32_t there_s[SLOTS];
+    __shared__ long long sums[kWarps + 3];
+    __shared__ float2 ml_s[kWarps][8];
+    __shared__ float q_unit[8];
+    __shared__ volatile int abort_flag;
+
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int D = a.c.D;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kWarps);
+        }
+    }
+    __syncthreads();
+    dependency_wait();
+    dependents_may_start();
+
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        if (mbar_test(bar, parity)) return true;
+        if (!abort_flag) {
+            if (mbar_wait(bar, parity)) return true;
+            abort_flag = 1;
+            atomicCAS(&g_rows_status, 0, site);
+            linger();
+        }
+        return false;
+    };
+    Run<C::ROWS, C::UNIT, kThreads> run(a);
+    bool more = run.begin(sums);
+    if (warp == kWarps) {
+        bring<C, kThreads>(a, run, more, ring, full, empty, there_s, wait);
+        __syncwarp();
+        if (abort_flag) linger();
+        return;
+    }
+
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); };
+    auto leave = [&](int sl) {
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
+    };
+    uint32_t slot = 0;
+    int4 cut = make_int4(0, 0, 0, -1);
+    for (; more; more = run.next()) {
+        const Tile w = run.at();
+        const Sequence &s = w.s;
+        const int rows = (int)min((long long)s.n * a.group, 2147483647LL);
+        const int row0 = w.tile * 8;
+
+        // ---- Q as operands: a row's values by two warps' lanes, two rows a warp --------------------------------------------
+        meet();                                      // (the tile before has been read)
+        if constexpr (HALF) {
+            for (int r = warp; r < 8; r += kWarps) {
+                const int row = row0 + r;
+                float most = 0.0f;
+                if (row < rows) {
+                    const T *src = static_cast<const T *>(a.q) + (long long)(s.first + row / a.group) * a.q_stride + (long long)(w.head * a.group + row % a.group) * D;
+                    for (int d = lane; d < D; d += 32) most = fmaxf(most, fabsf(to_float(src[d])));
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (lane == 0) q_unit[r] = pow2_scale(most);
+            }
+            meet();
+        }
+        for (int i = tid; i < C::STEPS * 32; i += 32 * kWarps) {
+            const int l = i & 31, ks = i >> 5, r = l >> 2, row = row0 + r;
+            const int d = ((l & 3) + 4 * (ks / (C::EC / 4))) * C::EC + 4 * (ks % (C::EC / 4));
+            const bool here = row < rows && d < D;
+            const T *src = static_cast<const T *>(a.q) + (long long)(s.first + row / a.group) * a.q_stride + (long long)(w.head * a.group + row % a.group) * D + d;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = here ? to_float(src[e]) : 0.0f;
+                if constexpr (HALF) x[e] *= q_unit[r];
+            }
+#pragma unroll
+            for (int n = 0; n < C::NQ; ++n) {
+                uint2 f;
+                f.x = next_piece<HALF>(x[0], x[1]);
+                f.y = next_piece<HALF>(x[2], x[3]);
+                q_s[n * C::STEPS * 32 + i] = f;
+            }
+        }
+        meet();
+
+        // this thread's rows: 2 t4 and 2 t4 + 1
+        int limit[2];
+        float factor[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[C::TILES][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = row0 + 2 * t4 + r;
+            limit[r] = row < rows ? limit_of(a, s, row) : 0;
+            factor[r] = a.cscale;
+            if constexpr (HALF) factor[r] = fmaxf(a.cscale * pow2_inverse(q_unit[2 * t4 + r]), 1.17549435e-38f);       // (a masked score times 0 would be NaN)
+        }
+        const int least_limit = limit_of(a, s, row0), keys = tile_keys<8>(a, s, w.tile);
+        int unit = -126;                             // codes: o is divided by 2^unit, which follows the largest scale of the values
+#pragma unroll
+        for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+
+        constexpr int NG = C::KB / 16;
+        const int pitch = D * C::EB, k0 = warp * C::KB;
+        for (int u = w.from; u < w.to; ++u, slot += 2) {
+            const int ksl = slot % SLOTS, vsl = (slot + 1) % SLOTS;
+            const uint8_t *k_at = ring + ksl * C::kSlotBytes, *v_at = ring + vsl * C::kSlotBytes;
+            const int p0 = u * C::UNIT + k0;         // the warp's first key in the sequence
+            wait(&full[ksl], (slot / SLOTS) & 1, 11);
+            if (p0 >= keys) {
+                leave(ksl);
+                wait(&full[vsl], ((slot + 1) / SLOTS) & 1, 11);
+                leave(vsl);
+                continue;
+            }
+            const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[ksl]) >> (k0 / 16) & ((1u << NG) - 1);
+            const bool partial = p0 + C::KB > keys || there != (1u << NG) - 1;
+            const bool masked = p0 + C::KB > least_limit || there != (1u << NG) - 1;
+            float z[NG][4], zc[C::NQ > 1 ? NG : 1][4];
+#pragma unroll
+            for (int i = 0; i < NG; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[i][e] = 0.0f;
+                    if constexpr (C::NQ > 1) zc[i][e] = 0.0f;
+                }
+            constexpr int PER = C::EC / 4;           // instructions a chunk
+#pragma unroll
+            for (int i = 0; i < C::NC; ++i) {
+                uint32_t kw[NG][2][C::EC * C::EB / 4];
+                const int d = (t4 + 4 * i) * C::EC;
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        if (d < D) read_words<C::EC * C::EB>(kw[j][hf], k_at + (k0 + 16 * j + 8 * hf + g) * pitch + d * C::EB);
+                        else
+#pragma unroll
+                            for (int x = 0; x < C::EC * C::EB / 4; ++x) kw[j][hf][x] = 0u;
+                    }
+#pragma unroll
+                for (int x = 0; x < PER; ++x) {
+                    uint2 q[C::NQ];
+#pragma unroll
+                    for (int n = 0; n < C::NQ; ++n) q[n] = q_s[(n * C::STEPS + i * PER + x) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) {
+                        uint4 f[C::NK];
+                        if constexpr (C::CODED) {
+                            codes_to_half<FMT>(kw[j][0][x], f[0].x, f[0].z);
+                            codes_to_half<FMT>(kw[j][1][x], f[0].y, f[0].w);
+                        } else if constexpr (!C::F32) {
+                            f[0] = make_uint4(kw[j][0][2 * x], kw[j][1][2 * x], kw[j][0][2 * x + 1], kw[j][1][2 * x + 1]);
+                        } else {
+                            float y[2][4];
+#pragma unroll
+                            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[hf][e] = __uint_as_float(kw[j][hf][e]);
+#pragma unroll
+                            for (int n = 0; n < 3; ++n) {
+                                f[n].x = next_piece<false>(y[0][0], y[0][1]);
+                                f[n].y = next_piece<false>(y[1][0], y[1][1]);
+                                f[n].z = next_piece<false>(y[0][2], y[0][3]);
+                                f[n].w = next_piece<false>(y[1][2], y[1][3]);
+                            }
+                        }
+#pragma unroll
+                        for (int order = C::NQ - 1; order >= 1; --order)
+#pragma unroll
+                            for (int n = 0; n <= order && n < C::NK; ++n) mma16<HALF>(zc[j], f[n], q[order - n].x, q[order - n].y);
+                        mma16<HALF>(z[j], f[0], q[0].x, q[0].y);
+                    }
+                }
+            }
+            float ks[C::CODED ? NG : 1][2], vs[C::CODED ? NG : 1][2];
+            if constexpr (C::CODED)
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) ks[j][hf] = *reinterpret_cast<const float *>(k_at + C::UNIT * DP + (k0 + 16 * j + 8 * hf + g) * 4);
+            wait(&full[vsl], ((slot + 1) / SLOTS) & 1, 11);
+
+            // ---- softmax: element e of a tile is key g + 8 (e / 2) and row 2 t4 + e % 2 ---------------------------------
+            float shrink = 1.0f;
+            if constexpr (C::CODED) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int in = 16 * j + 8 * hf + g;
+                        float x = *reinterpret_cast<const float *>(v_at + C::UNIT * DP + (k0 + in) * 4);
+                        if (partial && !(p0 + in < keys && (there >> j & 1))) x = 0.0f;
+                        vs[j][hf] = x;
+                        const uint32_t bits = __float_as_uint(x);
+                        most = max(most, bits < 0x7F800000u ? bits : 0u);
+                    }
+                most = __reduce_max_sync(0xffffffffu, most);
+                const int e = max((int)(most >> 23) - 127 - 13, -126);           // (p <= 1, the scale < 2 * 2^13 then)
+                if (e > unit) {
+                    shrink = ex2_approx((float)max(unit - e, -126));
+                    unit = e;
+                }
+                const float down = __uint_as_float((uint32_t)(127 - min(unit, 126)) << 23);
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) vs[j][hf] *= down;
+            }
+            float top[2] = {-INFINITY, -INFINITY}, base[2], alpha[2];
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = z[j][e];
+                    if constexpr (C::NQ > 1) x += zc[j][e];
+                    if constexpr (C::CODED) x *= ks[j][e >> 1];
+                    x *= factor[e & 1];
+                    if (masked && !(p0 + 16 * j + 8 * (e >> 1) + g < limit[e & 1] && (there >> j & 1))) x = -INFINITY;
+                    z[j][e] = x;
+                    top[e & 1] = fmaxf(top[e & 1], x);
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], off));
+                const float now = fmaxf(m[r], top[r]);
+                base[r] = now == -INFINITY ? 0.0f : now;
+                alpha[r] = ex2_approx(m[r] - base[r]);
+                m[r] = now;
+                l[r] *= alpha[r];
+                alpha[r] *= shrink;
+            }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e & 1];
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = z[j][e];
+                    float y = ex2_approx(x - base[e & 1]);
+                    l[e & 1] += y;
+                    if constexpr (C::CODED) {
+                        y *= vs[j][e >> 1];
+                        if (masked && x == -INFINITY) y = 0.0f;              // (the scale of a value that a row does not see may be anything)
+                    }
+                    z[j][e] = y;
+                }
+            uint2 p[C::NQ][NG];
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int n = 0; n < C::NQ; ++n) {
+                    p[n][j].x = turned8(next_piece<HALF>(z[j][0], z[j][1]));
+                    p[n][j].y = turned8(next_piece<HALF>(z[j][2], z[j][3]));
+                }
+            leave(ksl);                              // (what was read of it has been used: an arrival does not wait for loads)
+
+            // ---- O^T += V^T P^T: a tile is values 2 x and 2 x + 1 of each thread's chunk -----------------------------------
+#pragma unroll
+            for (int c = 0; c < C::NV; ++c) {
+                const int d = (g + 8 * c) * C::EV;
+                uint32_t vw[NG][4][C::EV * C::EB / 4];
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int in = 16 * i + 8 * (x >> 1) + 2 * t4 + (x & 1);
+                        // what lies in places without keys may be anything
+                        if (d < D && (!partial || (p0 + in < keys && (there >> i & 1)))) read_words<C::EV * C::EB>(vw[i][x], v_at + (k0 + in) * pitch + d * C::EB);
+                        else
+#pragma unroll
+                            for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[i][x][y] = 0u;
+                    }
+#pragma unroll
+                for (int x = 0; x < C::EV / 2; ++x) {
+                    const int j = c * (C::EV / 2) + x;
+                    float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint4 f[NG][C::NK];
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        if constexpr (C::CODED) {
+                            const int word = x / 2, pick = x & 1 ? 0x7362 : 0x5140;
+                            codes_to_half<FMT>(__byte_perm(vw[i][0][word], vw[i][1][word], pick), f[i][0].x, f[i][0].y);
+                            codes_to_half<FMT>(__byte_perm(vw[i][2][word], vw[i][3][word], pick), f[i][0].z, f[i][0].w);
+                        } else if constexpr (!C::F32) {
+                            f[i][0] = make_uint4(__byte_perm(vw[i][0][x], vw[i][1][x], 0x5410), __byte_perm(vw[i][0][x], vw[i][1][x], 0x7632),
+                                                 __byte_perm(vw[i][2][x], vw[i][3][x], 0x5410), __byte_perm(vw[i][2][x], vw[i][3][x], 0x7632));
+                        } else {
+                            float y[4][2];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) y[k][e] = __uint_as_float(vw[i][k][2 * x + e]);
+#pragma unroll
+                            for (int n = 0; n < 3; ++n) {
+                                f[i][n].x = next_piece<false>(y[0][0], y[1][0]);
+                                f[i][n].y = next_piece<false>(y[0][1], y[1][1]);
+                                f[i][n].z = next_piece<false>(y[2][0], y[3][0]);
+                                f[i][n].w = next_piece<false>(y[2][1], y[3][1]);
+                            }
+                        }
+                    }
+                    if constexpr (C::F32) {
+#pragma unroll
+                        for (int order = C::NQ - 1; order >= 0; --order)
+#pragma unroll
+                            for (int n = 0; n <= order && n < C::NK; ++n)
+#pragma unroll
+                                for (int i = 0; i < NG; ++i) mma16<HALF>(d4, f[i][n], p[order - n][i].x, p[order - n][i].y);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][e] += d4[e];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) mma16<HALF>(o[j], f[i][0], p[0][i].x, p[0][i].y);
+                    }
+                }
+            }
+            leave(vsl);
+        }
+        const float grown = C::CODED ? __uint_as_float((uint32_t)(127 + min(unit, 126)) << 23) : 1.0f;
+
+        // ---- the tile's end: the warps' sums by way of shared memory, two rows a warp --------------------------------------
+        const int part = run.part();
+        if (part >= 0 && (part & 1)) cut = run.cut();
+        const bool store = !abort_flag;
+        float *dst = part < 0 ? nullptr : a.parts + (size_t)part * 8 * (DP + 2);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+            if (g == 0) ml_s[warp][2 * t4 + r] = make_float2(m[r], l[r]);
+            float *row = o_s + (warp * 8 + 2 * t4 + r) * C::kPad;
+#pragma unroll
+            for (int c = 0; c < C::NV; ++c)
+#pragma unroll
+                for (int x = 0; x < C::EV / 2; ++x) {
+                    const int j = c * (C::EV / 2) + x;
+                    *reinterpret_cast<float2 *>(row + (g + 8 * c) * C::EV + 2 * x) = make_float2(o[j][r] * grown, o[j][2 + r] * grown);
+                }
+        }
+        meet();
+        for (int r = warp; r < 8; r += kWarps) {
+            const int row = row0 + r;
+            if (row >= rows) break;
+            float top = -INFINITY, sum = 0.0f, f[kWarps];
+#pragma unroll
+            for (int x = 0; x < kWarps; ++x) top = fmaxf(top, ml_s[x][r].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int x = 0; x < kWarps; ++x) {
+                f[x] = ex2_approx(ml_s[x][r].x - base);
+                sum = fmaf(ml_s[x][r].y, f[x], sum);
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const long long t = s.first + row / a.group;
+            T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + row % a.group) * D;
+            bool wild = false;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                const int d = lane + 32 * i;
+                float y = 0.0f;
+#pragma unroll
+                for (int x = 0; x < kWarps; ++x) y = fmaf(o_s[(x * 8 + r) * C::kPad + d], f[x], y);
+                if (dst) {
+                    if (store) dst[(size_t)r * DP + d] = y;
+                } else {
+                    y = sum == 0.0f ? 0.0f : y * inv;
+                    wild = wild || !(fabsf(y) <= 3.402823466e38f);
+                    if (d < D && store) out[d] = from_float<T>(y);
+                }
+            }
+            if (dst) {
+                if (lane == 0 && store) reinterpret_cast<float2 *>(dst + 8 * DP)[r] = make_float2(top, sum);
+            } else if (__any_sync(0xffffffffu, wild) && store) {
+                __syncwarp();
+                mend_row<T, FMT>(a, w.b, w.head, s, row, keys);
+            }
+        }
+    }
+    meet();
+    if (a.cuts && tid == 0) {
+        a.cuts[blockIdx.x] = cut;
+        a.whole[blockIdx.x] = !abort_flag;
+    }
+}
+
+template <typename T, int FMT, int DP, typename C>
+int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
+{
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     static std::atomic<unsigned long long> done{0};
@@ -702,28 +1140,33 @@ int launch_rows(AttnArgs a, cudaStream_t st)
     }
     e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), C::kSmem, st, a);
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<T, FMT, C::ROWS, DP>, dim3((unsigned)grid, (unsigned)(C::ROWS + 15) / 16), dim3(256), 0, st, a);
-    return e == cudaSuccess ? check_launch("paged_rows_kernel") : fail(HIPGPT_ERR_CUDA, "paged_rows_kernel: %s", cudaGetErrorString(e));
+    return e == cudaSuccess ? check_launch("paged attention") : fail(HIPGPT_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int FMT, bool SPLITROWS>
-int launch_rows_of(const AttnArgs &a, cudaStream_t st)
+// Rows a sequence, on the average: eight at most (single tokens of a small group), some, many
+enum { kTokens, kSome, kMany };
+template <typename T, int FMT, int DP>
+int launch_width(int rows, const AttnArgs &a, cudaStream_t st)
 {
-    return a.c.D <= 32 ? launch_rows<T, FMT, 32, SPLITROWS>(a, st) : a.c.D <= 64 ? launch_rows<T, FMT, 64, SPLITROWS>(a, st) : launch_rows<T, FMT, 128, SPLITROWS>(a, st);
+    if (rows == kTokens) return launch_kernel<T, FMT, DP, TokenShape<T, FMT, DP>>(paged_token_kernel<T, FMT, DP>, a, st);
+    if constexpr (sizeof(T) == 4)
+        if (rows == kMany) return launch_kernel<T, FMT, DP, Shape<T, FMT, DP, true>>(paged_rows_kernel<T, FMT, DP, true>, a, st);
+    return launch_kernel<T, FMT, DP, Shape<T, FMT, DP, false>>(paged_rows_kernel<T, FMT, DP, false>, a, st);
+}
+template <typename T, int FMT>
+int launch_format(int rows, const AttnArgs &a, cudaStream_t st)
+{
+    return a.c.D <= 32 ? launch_width<T, FMT, 32>(rows, a, st) : a.c.D <= 64 ? launch_width<T, FMT, 64>(rows, a, st) : launch_width<T, FMT, 128>(rows, a, st);
 }
 
 template <typename T>
 int launch_paged(int format, const AttnArgs &a, cudaStream_t st)
 {
-    const bool few = (long long)a.c.T * a.group <= 32LL * a.c.B;
-    if constexpr (sizeof(T) == 2) {
-        if (!few && a.c.pages > 0) return launch_paged_tc(format, a, st);          // (without pages there is nothing to copy)
-        return format == HIPGPT_CACHE_PLAIN ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st)
-             : format == HIPGPT_CACHE_E4M3  ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st);
-    } else {
-        if (format == HIPGPT_CACHE_PLAIN) return few ? launch_rows_of<T, HIPGPT_CACHE_PLAIN, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_PLAIN, true>(a, st);
-        if (format == HIPGPT_CACHE_E4M3) return few ? launch_rows_of<T, HIPGPT_CACHE_E4M3, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_E4M3, true>(a, st);
-        return few ? launch_rows_of<T, HIPGPT_CACHE_INT8, false>(a, st) : launch_rows_of<T, HIPGPT_CACHE_INT8, true>(a, st);
-    }
+    const long long all = (long long)a.c.T * a.group;
+    const int rows = all <= 8LL * a.c.B ? kTokens : all <= 32LL * a.c.B ? kSome : kMany;
+    if (sizeof(T) == 2 && rows == kMany && a.c.pages > 0) return launch_paged_tc(format, a, st);         // (without pages there is nothing to copy)
+    return format == HIPGPT_CACHE_PLAIN ? launch_format<T, HIPGPT_CACHE_PLAIN>(rows, a, st)
+         : format == HIPGPT_CACHE_E4M3  ? launch_format<T, HIPGPT_CACHE_E4M3>(rows, a, st) : launch_format<T, HIPGPT_CACHE_INT8>(rows, a, st);
 }
 
 }  // namespace

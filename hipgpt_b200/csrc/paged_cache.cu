@@ -5,31 +5,27 @@
 //   int8  scale max|x| / 127 (rounded to fp32); the code is the whole number nearest to x / scale, ties to even, of the exact quotient: the rounded product
 //         with 1 / scale may be one off beside a border, and the remainder x - code * scale, which one multiply-add gives exactly, says so
 //
-// Bound: HBM for prompts; the launch for single tokens.  A row is read 16 bytes a thread by as many neighbouring threads as it needs (a power of two of them), the
-// largest magnitude goes round by shuffles, each thread has its part of K and of V on its way at once.
+// Bound: HBM for prompts; the launch for single tokens.  A block takes some tokens; where each goes is looked up once for all its heads.  A row is read 16 bytes a thread by as many neighbouring
+// threads as it needs (a power of two of them), the largest magnitude goes round by shuffles, and a thread has kAhead parts of K and of V on their way at once.
 #include "paged.cuh"
 
 namespace hipgpt {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kMostTokens = 32;
 
 struct MoveArgs {
     PagedView c;
     const void *k, *v;                   // rows of tokens (written for reading the cache)
     long long k_stride, v_stride;
-    int lanes, log_lanes, vec;           // threads a row
+    int lanes, log_lanes, tokens;        // threads a row; tokens a block
+    uint32_t per_head;                   // 2^32 / heads, rounded up: r * per_head >> 32 is r / heads for r * heads < 2^32
 };
 
-// (token, head) of this thread's row, and where it lies in the cache: row < 0: nowhere; token < 0: no such row, or no sequence's
-struct Place { long long token; int head; long long row; };
-
-// The sequence of the block's first token is found by all threads together; a thread goes on from there.
-__device__ __forceinline__ Place place_of(const MoveArgs &a)
+// Where the block's tokens lie in the cache: the row of head 0 (the others 1 << shift apart), -1: nowhere, -2: no such token, or no sequence's.  The sequence of the first is found
+// by all threads together; a thread for each token goes on from there.
+__device__ __forceinline__ void places_of(const MoveArgs &a, int t0, long long (&places)[kMostTokens])
 {
-    const long long rows = (long long)a.c.T * a.c.heads;
-    const long long first = (long long)blockIdx.x << (8 - a.log_lanes);
-    const int t0 = (int)(first / a.c.heads);
     int below = 0;                       // sequences that end at or before t0
     for (int b0 = 0; b0 < a.c.B; b0 += kThreads) {
         const int b = b0 + threadIdx.x;
@@ -37,16 +33,23 @@ __device__ __forceinline__ Place place_of(const MoveArgs &a)
         below += some;
         if (some < min(kThreads, a.c.B - b0)) break;
     }
-    const long long r = first + (threadIdx.x >> a.log_lanes);
-    if (r >= rows) return {-1, 0, -1};
-    const int t = (int)(r / a.c.heads), head = (int)(r - (long long)t * a.c.heads);
-    int b = below;
-    while (b < a.c.B && __ldg(a.c.offsets + b + 1) <= t) ++b;
-    if (b >= a.c.B) return {-1, 0, -1};
-    const Sequence s = sequence_of(a.c, b);
-    if (t < s.first || t >= s.first + s.n) return {-1, 0, -1};
-    const int p = s.len - s.n + (t - s.first);
-    return {t, head, p < 0 ? -1 : row_of(a.c, b, head, p)};
+    if ((int)threadIdx.x < a.tokens) {
+        const int t = t0 + threadIdx.x;
+        long long place = -2;
+        if (t < a.c.T) {
+            int b = below;
+            while (b < a.c.B && __ldg(a.c.offsets + b + 1) <= t) ++b;
+            if (b < a.c.B) {
+                const Sequence s = sequence_of(a.c, b);
+                if (t >= s.first && t < s.first + s.n) {
+                    const int p = s.len - s.n + (t - s.first);
+                    place = p < 0 ? -1 : row_of(a.c, b, 0, p);
+                }
+            }
+        }
+        places[threadIdx.x] = place;
+    }
+    __syncthreads();
 }
 
 __device__ __forceinline__ float row_max(float m, int lanes)
@@ -78,6 +81,8 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Four codes of a word.  x * inv + 1.5 * 2^23 rounds to the nearest whole number in the low bits; where a remainder comes within 2^-10 of half a scale, which is seldom, all four
+// are looked at again.
 __device__ __forceinline__ int int8_code(float x, float s, float inv)
 {
     float q = rintf(x * inv);
@@ -87,84 +92,98 @@ __device__ __forceinline__ int int8_code(float x, float s, float inv)
     else if (r < -half || (r == -half && odd)) q -= 1.0f;
     return (int)q;
 }
+__device__ __forceinline__ uint32_t int8_word(const float *x, float s, float inv)
+{
+    constexpr float kMagic = 12582912.0f;
+    float t[4], far = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        t[e] = fmaf(x[e], inv, kMagic);
+        far = fmaxf(far, fabsf(fmaf(kMagic - t[e], s, x[e])));
+    }
+    uint32_t w = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+    if (far > 0.4990234375f * s) w = (int8_code(x[0], s, inv) & 255) | (int8_code(x[1], s, inv) & 255) << 8 | (int8_code(x[2], s, inv) & 255) << 16 | (uint32_t)int8_code(x[3], s, inv) << 24;
+    return w;
+}
 
+constexpr int kAhead = 2;
+
+// W: values of 16 bytes, or 1 for rows that do not start on 16 bytes (value by value, four a thread)
 template <typename T, int FMT, int W>
 __global__ void __launch_bounds__(kThreads)
 cache_write_kernel(const MoveArgs a)
 {
     dependency_wait();
     dependents_may_start();
-    const Place at = place_of(a);
-    const int lane = threadIdx.x & (a.lanes - 1), D = a.c.D;
-    const bool there = at.token >= 0 && at.row >= 0;
-    // every thread of the warp takes part in the shuffles: those without a row have zeros
-    if constexpr (W > 1) {
-        const int d = lane * W;
-        const bool mine = there && d < D;
-        float x[2][W];
+    __shared__ long long places[kMostTokens];
+    const int t0 = blockIdx.x * a.tokens, D = a.c.D;
+    places_of(a, t0, places);
+    constexpr int N = W > 1 ? W : 4;                 // values a thread
+    const int all = a.tokens * a.c.heads << a.log_lanes;
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < all; i0 += kThreads * kAhead) {
+        float x[kAhead][2][N];
+        long long row[kAhead];
+        // (every thread of the warp takes part in the shuffles: those without a row have zeros)
+        const int d = (i0 & (a.lanes - 1)) * N;
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[0][i] = x[1][i] = 0.0f;
-        if (mine) {
-            load_values<T, W>(static_cast<const T *>(a.k) + at.token * a.k_stride + at.head * D + d, x[0]);
-            load_values<T, W>(static_cast<const T *>(a.v) + at.token * a.v_stride + at.head * D + d, x[1]);
-        }
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + kThreads * u, r = i >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
+            row[u] = i < all ? places[t] : -2;
+            const bool mine = row[u] >= 0 && d < D;
+            row[u] = mine ? row[u] + ((long long)head << a.c.shift) : -1;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);
-            if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                if (mine) store_values<T, W>(reinterpret_cast<T *>(base) + at.row * D + d, x[w]);
-            } else {
-                float m = 0.0f;
-                bool fine = true;
+            for (int w = 0; w < 2; ++w) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    m = fmaxf(m, fabsf(x[w][i]));
-                    fine = fine && fabsf(x[w][i]) <= 3.402823466e38f;
-                }
-                m = row_max(fine ? m : INFINITY, a.lanes);
-                float inv, s = scale_of<FMT>(m, inv);
-                const bool whole = m <= 3.402823466e38f;
-                uint32_t code[W / 4];
-#pragma unroll
-                for (int i = 0; i < W / 4; ++i) {
-                    const float *y = x[w] + 4 * i;
-                    if constexpr (FMT == HIPGPT_CACHE_E4M3) code[i] = e4m3_pair(y[0] * inv, y[1] * inv) | e4m3_pair(y[2] * inv, y[3] * inv) << 16;
-                    else code[i] = (int8_code(y[0], s, inv) & 255) | (int8_code(y[1], s, inv) & 255) << 8 | (int8_code(y[2], s, inv) & 255) << 16 | (uint32_t)int8_code(y[3], s, inv) << 24;
-                    if (!whole) code[i] = 0u;
-                }
+                for (int e = 0; e < N; ++e) x[u][w][e] = 0.0f;
                 if (mine) {
-                    uint8_t *dst = base + at.row * D + d;
-                    if constexpr (W == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(code[0], code[1]);
-                    else *reinterpret_cast<uint32_t *>(dst) = code[0];
-                    if (lane == 0) const_cast<float *>(w ? a.c.vs : a.c.ks)[at.row] = whole ? s : __uint_as_float(0x7FFFFFFFu);
+                    const T *src = static_cast<const T *>(w ? a.v : a.k) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D + d;
+                    if constexpr (W > 1) load_values<T, W>(src, x[u][w]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < N; ++e) x[u][w][e] = to_float(src[e]);
                 }
             }
         }
-    } else {
-        // rows that do not start on 16 bytes: value by value, twice
-        for (int w = 0; w < 2; ++w) {
-            const T *src = static_cast<const T *>(w ? a.v : a.k) + at.token * (w ? a.v_stride : a.k_stride) + at.head * D;
-            uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);
-            if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                if (there) for (int d = lane; d < D; d += a.lanes) reinterpret_cast<T *>(base)[at.row * D + d] = src[d];
-            } else {
-                float m = 0.0f;
-                if (there) for (int d = lane; d < D; d += a.lanes) {
-                    const float x = fabsf(to_float(src[d]));
-                    m = x <= 3.402823466e38f ? fmaxf(m, x) : INFINITY;
-                }
-                m = row_max(m, a.lanes);
-                float inv, s = scale_of<FMT>(m, inv);
-                const bool whole = m <= 3.402823466e38f;
-                if (there) {
-                    for (int d = lane; d < D; d += a.lanes) {
-                        const float x = to_float(src[d]);
-                        base[at.row * D + d] = !whole ? 0 : FMT == HIPGPT_CACHE_E4M3 ? (uint8_t)e4m3_pair(x * inv, 0.0f) : (uint8_t)int8_code(x, s, inv);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);
+                if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
+                    if (row[u] >= 0) {
+                        T *dst = reinterpret_cast<T *>(base) + row[u] * D + d;
+                        if constexpr (W > 1) store_values<T, W>(dst, x[u][w]);
+                        else
+#pragma unroll
+                            for (int e = 0; e < N; ++e) dst[e] = from_float<T>(x[u][w][e]);
                     }
-                    if (lane == 0) const_cast<float *>(w ? a.c.vs : a.c.ks)[at.row] = whole ? s : __uint_as_float(0x7FFFFFFFu);
+                } else {
+                    float m = 0.0f;
+                    bool fine = true;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        m = fmaxf(m, fabsf(x[u][w][e]));
+                        fine = fine && fabsf(x[u][w][e]) <= 3.402823466e38f;
+                    }
+                    m = row_max(fine ? m : INFINITY, a.lanes);
+                    float inv, s = scale_of<FMT>(m, inv);
+                    const bool whole = m <= 3.402823466e38f;
+                    uint32_t code[N / 4];
+#pragma unroll
+                    for (int e = 0; e < N / 4; ++e) {
+                        const float *y = x[u][w] + 4 * e;
+                        if constexpr (FMT == HIPGPT_CACHE_E4M3) code[e] = e4m3_pair(y[0] * inv, y[1] * inv) | e4m3_pair(y[2] * inv, y[3] * inv) << 16;
+                        else code[e] = int8_word(y, s, inv);
+                        if (!whole) code[e] = 0u;
+                    }
+                    if (row[u] >= 0) {
+                        uint8_t *dst = base + row[u] * D + d;
+                        if constexpr (N == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(code[0], code[1]);
+                        else *reinterpret_cast<uint32_t *>(dst) = code[0];
+                        if (d == 0) const_cast<float *>(w ? a.c.vs : a.c.ks)[row[u]] = whole ? s : __uint_as_float(0x7FFFFFFFu);
+                    }
                 }
             }
-        }
     }
 }
 
@@ -174,44 +193,62 @@ cache_read_kernel(const MoveArgs a)
 {
     dependency_wait();
     dependents_may_start();
-    const Place at = place_of(a);
-    if (at.token < 0) return;
-    const int D = a.c.D;
-    const bool there = at.row >= 0;
-    constexpr int STEP = W > 1 ? W : 1;
+    __shared__ long long places[kMostTokens];
+    const int t0 = blockIdx.x * a.tokens, D = a.c.D;
+    places_of(a, t0, places);
+    constexpr int N = W > 1 ? W : 4;
+    const int all = a.tokens * a.c.heads << a.log_lanes;
+    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kAhead) {
+        float x[kAhead][2][N], s[kAhead][2];
+        uint32_t word[kAhead][2][2];
+        long long place[kAhead];
+        const int d = (i0 & (a.lanes - 1)) * N;
+        if (d >= D) continue;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const uint8_t *base = w ? a.c.v : a.c.k;
-        T *dst = static_cast<T *>(const_cast<void *>(w ? a.v : a.k)) + at.token * (w ? a.v_stride : a.k_stride) + at.head * D;
-        float s = 0.0f;
-        if constexpr (FMT != HIPGPT_CACHE_PLAIN) if (there) s = __ldg((w ? a.c.vs : a.c.ks) + at.row);
-        for (int d = (threadIdx.x & (a.lanes - 1)) * STEP; d < D; d += a.lanes * STEP) {
-            float x[STEP];
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + kThreads * u, r = i >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
+            place[u] = i < all ? places[t] : -2;
+            const long long row = place[u] + ((long long)head << a.c.shift);
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) x[i] = 0.0f;
-            if (there) {
+            for (int w = 0; w < 2; ++w) {
+                const uint8_t *base = w ? a.c.v : a.c.k;
+                s[u][w] = 0.0f;
+                word[u][w][0] = word[u][w][1] = 0u;
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[u][w][e] = 0.0f;
+                if (place[u] < 0) continue;
                 if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                    load_values<T, STEP>(reinterpret_cast<const T *>(base) + at.row * D + d, x);
-                } else if constexpr (W == 1) {
-                    const uint32_t two = code_pair<FMT>(base[at.row * D + d], 0u, 0, 0);
-                    x[0] = __uint_as_float(two << 16) * s;
+                    load_values<T, N>(reinterpret_cast<const T *>(base) + row * D + d, x[u][w]);
                 } else {
-                    uint32_t word[W / 4];
-                    if constexpr (W == 8) {
-                        const uint2 u = *reinterpret_cast<const uint2 *>(base + at.row * D + d);
-                        word[0] = u.x; word[1] = u.y;
+                    s[u][w] = __ldg((w ? a.c.vs : a.c.ks) + row);
+                    if constexpr (N == 8) {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(base + row * D + d);
+                        word[u][w][0] = y.x; word[u][w][1] = y.y;
                     } else {
-                        word[0] = *reinterpret_cast<const uint32_t *>(base + at.row * D + d);
-                    }
-#pragma unroll
-                    for (int i = 0; i < W / 2; ++i) {
-                        const uint32_t two = code_pair<FMT>(word[i / 2], word[i / 2], (i & 1) * 2, (i & 1) * 2 + 1);
-                        x[2 * i] = __uint_as_float(two << 16) * s;
-                        x[2 * i + 1] = __uint_as_float(two & 0xFFFF0000u) * s;
+                        word[u][w][0] = *reinterpret_cast<const uint32_t *>(base + row * D + d);
                     }
                 }
             }
-            store_values<T, STEP>(dst + d, x);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (place[u] == -2) continue;
+            const int r = (i0 + kThreads * u) >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                if constexpr (FMT != HIPGPT_CACHE_PLAIN)
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) {
+                        const uint32_t two = code_pair<FMT>(word[u][w][e / 2], word[u][w][e / 2], (e & 1) * 2, (e & 1) * 2 + 1);
+                        x[u][w][2 * e] = __uint_as_float(two << 16) * s[u][w];
+                        x[u][w][2 * e + 1] = __uint_as_float(two & 0xFFFF0000u) * s[u][w];
+                    }
+                T *dst = static_cast<T *>(const_cast<void *>(w ? a.v : a.k)) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D + d;
+                if constexpr (W > 1) store_values<T, W>(dst, x[u][w]);
+                else
+#pragma unroll
+                    for (int e = 0; e < N; ++e) dst[e] = from_float<T>(x[u][w][e]);
+            }
         }
     }
 }
@@ -221,12 +258,17 @@ int launch_move(MoveArgs a, bool write, cudaStream_t st)
 {
     constexpr int W = kPer16<T>;
     const bool vec = all_aligned16({a.k, a.v}) && a.k_stride % W == 0 && a.v_stride % W == 0;
-    // D / W threads of 16 bytes, rounded up to a power of two; without them as many as a warp
+    // D / W threads of 16 bytes, rounded up to a power of two; without them four values each
     a.log_lanes = 0;
-    while (a.log_lanes < 5 && (vec ? W : 4) << a.log_lanes < a.c.D) ++a.log_lanes;
+    while ((vec ? W : 4) << a.log_lanes < a.c.D) ++a.log_lanes;
     a.lanes = 1 << a.log_lanes;
-    const long long rows = (long long)a.c.T * a.c.heads, per = kThreads >> a.log_lanes, blocks = (rows + per - 1) / per;
-    if (blocks > 2147483647LL) return fail(HIPGPT_ERR_BAD_ARG, "%d tokens of %d heads are beyond one call", a.c.T, a.c.heads);
+    // Tokens a block: one where there are few, 32 (whose places are looked up side by side) where there are enough for four blocks an SM
+    const long long each = (long long)a.c.heads << a.log_lanes;
+    a.tokens = 1;
+    while (a.tokens < kMostTokens && (a.tokens * each < kThreads * kAhead || a.c.T / (2 * a.tokens) >= 148 * 4) && a.c.T >= 2 * a.tokens * 148) a.tokens *= 2;
+    const long long blocks = ((long long)a.c.T + a.tokens - 1) / a.tokens;
+    a.per_head = (uint32_t)(((1ull << 32) + a.c.heads - 1) / a.c.heads);             // (of one head: not used)
+    if (each * a.tokens > 1LL << 30 || ((long long)a.tokens * a.c.heads + kThreads * kAhead) * a.c.heads >= 1LL << 32) return fail(HIPGPT_ERR_BAD_ARG, "rows of %d heads are beyond one call", a.c.heads);
     const auto kern = write ? (vec ? cache_write_kernel<T, FMT, W> : cache_write_kernel<T, FMT, 1>) : (vec ? cache_read_kernel<T, FMT, W> : cache_read_kernel<T, FMT, 1>);
     const cudaError_t e = launch_overlapped(kern, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
     const char *what = write ? "cache_write_kernel" : "cache_read_kernel";

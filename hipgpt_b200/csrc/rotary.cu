@@ -42,12 +42,16 @@ rotary_kernel(const RotaryArgs a, bool inverse)
     T *out = static_cast<T *>(a.out) + t * a.out_stride;
     constexpr int PAIRS = HALVES ? W : (W > 1 ? W / 2 : 1);            // (W == 1: one pair, value by value)
     const int turning = a.R / 2 / PAIRS;
+    // (U heads at a time: the next loads must not wait for these stores, and the compiler cannot know that x and out, which may be one, have no element of two heads in common)
+    constexpr int U = 4;
     if (lane >= turning) {
         const int d = a.R + (lane - turning) * W;
-        for (int h = h0; h < h1; ++h) {
-            float v[W];
-            load_values<T, W>(x + h * a.D + d, v);
-            store_values<T, W>(out + h * a.D + d, v);
+        for (int h = h0; h < h1; h += U) {
+            float v[U][W];
+#pragma unroll
+            for (int u = 0; u < U; ++u) if (h + u < h1) load_values<T, W>(x + (h + u) * a.D + d, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) if (h + u < h1) store_values<T, W>(out + (h + u) * a.D + d, v[u]);
         }
         return;
     }
@@ -66,31 +70,49 @@ rotary_kernel(const RotaryArgs a, bool inverse)
     };
     if constexpr (HALVES) {
         const int d = lane * W, e = d + a.R / 2;
-#pragma unroll 2
-        for (int h = h0; h < h1; ++h) {
-            float p[W], q[W];
-            load_values<T, W>(x + h * a.D + d, p);
-            load_values<T, W>(x + h * a.D + e, q);
+        if constexpr (W > 1) {
+            uint4 p4[U], q4[U];
+            for (int h = h0; h < h1; h += U) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) turn(i, p[i], q[i], p[i], q[i]);
-            store_values<T, W>(out + h * a.D + d, p);
-            store_values<T, W>(out + h * a.D + e, q);
+                for (int u = 0; u < U; ++u) if (h + u < h1) {
+                    p4[u] = *reinterpret_cast<const uint4 *>(x + (h + u) * a.D + d);
+                    q4[u] = *reinterpret_cast<const uint4 *>(x + (h + u) * a.D + e);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) if (h + u < h1) {
+                    float p[W], q[W];
+                    unpack(p4[u], p, T());
+                    unpack(q4[u], q, T());
+#pragma unroll
+                    for (int i = 0; i < W; ++i) turn(i, p[i], q[i], p[i], q[i]);
+                    store_values<T, W>(out + (h + u) * a.D + d, p);
+                    store_values<T, W>(out + (h + u) * a.D + e, q);
+                }
+            }
+        } else {
+            for (int h = h0; h < h1; ++h) {
+                float p = to_float(x[h * a.D + d]), q = to_float(x[h * a.D + e]);
+                turn(0, p, q, p, q);
+                out[h * a.D + d] = from_float<T>(p);
+                out[h * a.D + e] = from_float<T>(q);
+            }
         }
     } else {
         const int d = lane * PAIRS * 2;
-#pragma unroll 4
-        for (int h = h0; h < h1; ++h) {
-            if constexpr (W == 1) {
-                float p = to_float(x[h * a.D + d]), q = to_float(x[h * a.D + d + 1]);
-                turn(0, p, q, p, q);
-                out[h * a.D + d] = from_float<T>(p);
-                out[h * a.D + d + 1] = from_float<T>(q);
-            } else {
-                float v[W];
-                load_values<T, W>(x + h * a.D + d, v);
+        constexpr int V = W > 1 ? W : 2;             // values of a head
+        for (int h = h0; h < h1; h += U) {
+            float v[U][V];
 #pragma unroll
-                for (int i = 0; i < PAIRS; ++i) turn(i, v[2 * i], v[2 * i + 1], v[2 * i], v[2 * i + 1]);
-                store_values<T, W>(out + h * a.D + d, v);
+            for (int u = 0; u < U; ++u) if (h + u < h1) {
+                if constexpr (W > 1) load_values<T, W>(x + (h + u) * a.D + d, v[u]);
+                else for (int i = 0; i < 2; ++i) v[u][i] = to_float(x[(h + u) * a.D + d + i]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) if (h + u < h1) {
+#pragma unroll
+                for (int i = 0; i < PAIRS; ++i) turn(i, v[u][2 * i], v[u][2 * i + 1], v[u][2 * i], v[u][2 * i + 1]);
+                if constexpr (W > 1) store_values<T, W>(out + (h + u) * a.D + d, v[u]);
+                else for (int i = 0; i < 2; ++i) out[(h + u) * a.D + d + i] = from_float<T>(v[u][i]);
             }
         }
     }
