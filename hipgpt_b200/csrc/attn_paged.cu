@@ -80,7 +80,7 @@ struct Shape {
     static constexpr bool F32 = sizeof(T) == 4, CODED = FMT != HIPGPT_CACHE_PLAIN;
     static constexpr int EB = CODED ? 1 : (int)sizeof(T);               // bytes of an element of the cache
     static constexpr int NQ = !F32 ? 1 : CODED ? 2 : 3, NK = F32 && !CODED ? 3 : 1;  // pieces of Q and P, of K and V
-    static constexpr int MT = SPLITROWS && DP <= 64 ? 2 : 1;            // tiles of 16 rows a warp
+    static constexpr int MT = 1;                                        // tiles of 16 rows a warp
     static constexpr int ROWS = 16 * MT * (SPLITROWS ? kWarps : 1);
     static constexpr int KB = 4096 / (DP * EB) >= 32 ? 32 : 16;         // keys a warp takes at a time
     static constexpr int UNIT = SPLITROWS ? 64 : kWarps * KB;           // keys of a place in the ring
@@ -92,10 +92,11 @@ struct Shape {
     static constexpr int kOBytes = SPLITROWS ? 0 : 2 * 16 * kPad * 4;   // two warps' results
     static constexpr int kSlotBytes = UNIT * DP * EB + (CODED ? UNIT * 4 : 0);
     static constexpr int kFixed = kQBytes + kOBytes + 1024;
-    // places of the ring: as many as leave room for two blocks an SM, four at least
-    static constexpr int kSlots = most_of(4, least_of(12, (112 * 1024 - kFixed) / kSlotBytes));
+    // places of the ring: four at least
+    static constexpr int kBudget = (DP == 128 ? 112 : 74) * 1024;       // two or three blocks an SM
+    static constexpr int kSlots = most_of(4, least_of(12, (kBudget - kFixed) / kSlotBytes));
     static constexpr size_t kSmem = (size_t)kQBytes + kOBytes + (size_t)kSlots * kSlotBytes;
-    static constexpr int kBlocks = kSmem <= 112 * 1024 ? 2 : 1;         // an SM
+    static constexpr int kBlocks = kSmem > 112 * 1024 ? 1 : DP == 128 || kSmem > 74 * 1024 ? 2 : 3;           // an SM
 };
 
 // The warp that asks for the copies: a place of the ring takes UNIT keys or values as they lie in their pages, then their scales; a lane a run of keys in one page
