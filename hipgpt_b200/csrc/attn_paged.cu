@@ -322,13 +322,17 @@ paged_rows_kernel(const AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < C::NC; ++i) {
                     uint32_t kw[NJ][C::EC * C::EB / 4];
+                    const int d = (t4 + 4 * i) * C::EC;
+                    if (D == DP) {
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        const int d = (t4 + 4 * i) * C::EC;
-                        if (d < D) read_words<C::EC * C::EB>(kw[j], k_at + (k0 + 8 * j + g) * pitch + d * C::EB);
-                        else
+                        for (int j = 0; j < NJ; ++j) read_words<C::EC * C::EB>(kw[j], k_at + (k0 + 8 * j + g) * (DP * C::EB) + d * C::EB);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) {
 #pragma unroll
                             for (int x = 0; x < C::EC * C::EB / 4; ++x) kw[j][x] = 0u;
+                            if (d < D) read_words<C::EC * C::EB>(kw[j], k_at + (k0 + 8 * j + g) * pitch + d * C::EB);
+                        }
                     }
 #pragma unroll
                     for (int x = 0; x < PER; ++x) {
@@ -415,11 +419,18 @@ paged_rows_kernel(const AttnArgs a)
                             float x = z[mt][j][e];
                             if constexpr (C::NQ > 1) x += zc[mt][j][e];
                             if constexpr (C::CODED) x *= (e & 1) ? ks2[j].y : ks2[j].x;
-                            x *= factor[mt][e >> 1];
-                            if (masked && !seen(mt, j, e)) x = -INFINITY;
-                            z[mt][j][e] = x;
-                            top[e >> 1] = fmaxf(top[e >> 1], x);
+                            z[mt][j][e] = x * factor[mt][e >> 1];
                         }
+                    if (masked) {
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[mt][j][e] = seen(mt, j, e) ? z[mt][j][e] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], z[mt][j][e]);
                     float base[2], alpha[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
@@ -442,15 +453,24 @@ paged_rows_kernel(const AttnArgs a)
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = z[mt][j][e];
-                            float y = ex2_approx(x - base[e >> 1]);
+                            const float y = ex2_approx(z[mt][j][e] - base[e >> 1]);
                             l[mt][e >> 1] += y;
-                            if constexpr (C::CODED) {
-                                y *= (e & 1) ? vs2[j].y : vs2[j].x;
-                                if (masked && x == -INFINITY) y = 0.0f;      // (the scale of a value that a row does not see may be anything)
-                            }
                             z[mt][j][e] = y;
                         }
+                    if constexpr (C::CODED) {
+                        if (!masked) {
+#pragma unroll
+                            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) z[mt][j][e] *= (e & 1) ? vs2[j].y : vs2[j].x;
+                        } else {
+                            // (the scale of a value that a row does not see may be anything)
+#pragma unroll
+                            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) z[mt][j][e] = seen(mt, j, e) ? z[mt][j][e] * ((e & 1) ? vs2[j].y : vs2[j].x) : 0.0f;
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < NG; ++i)
 #pragma unroll
@@ -469,17 +489,19 @@ paged_rows_kernel(const AttnArgs a)
                 for (int c = 0; c < C::NV; ++c) {
                     const int d = (g + 8 * c) * C::EV;
                     uint32_t vw[NG][4][C::EV * C::EB / 4];
+                    if (D == DP && !partial) {
 #pragma unroll
-                    for (int i = 0; i < NG; ++i)
+                        for (int x = 0; x < 4 * NG; ++x) read_words<C::EV * C::EB>(vw[x / 4][x % 4], v_at + (k0 + 8 * (x >> 1) + 2 * t4 + (x & 1)) * (DP * C::EB) + d * C::EB);
+                    } else {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int in = 16 * i + 8 * (x >> 1) + 2 * t4 + (x & 1);
-                            // what lies in places without keys may be anything
-                            if (d < D && (!partial || (p0 + in < wkeys && (there >> i & 1)))) read_words<C::EV * C::EB>(vw[i][x], v_at + (k0 + in) * pitch + d * C::EB);
-                            else
+                        for (int x = 0; x < 4 * NG; ++x) {
+                            const int in = 8 * (x >> 1) + 2 * t4 + (x & 1);
 #pragma unroll
-                                for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[i][x][y] = 0u;
+                            for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[x / 4][x % 4][y] = 0u;
+                            // (what lies in places without keys may be anything)
+                            if (d < D && p0 + in < wkeys && (there >> (x / 4) & 1)) read_words<C::EV * C::EB>(vw[x / 4][x % 4], v_at + (k0 + in) * pitch + d * C::EB);
                         }
+                    }
                     constexpr int W = C::CODED ? least_of(C::EV, 4) : 1;         // columns at a time: those of one word of codes
 #pragma unroll
                     for (int e = 0; e < C::EV; e += W) {
@@ -846,15 +868,17 @@ paged_token_kernel(const AttnArgs a)
             for (int i = 0; i < C::NC; ++i) {
                 uint32_t kw[NG][2][C::EC * C::EB / 4];
                 const int d = (t4 + 4 * i) * C::EC;
+                if (D == DP) {
 #pragma unroll
-                for (int j = 0; j < NG; ++j)
+                    for (int j = 0; j < 2 * NG; ++j) read_words<C::EC * C::EB>(kw[j / 2][j % 2], k_at + (k0 + 8 * j + g) * (DP * C::EB) + d * C::EB);
+                } else {
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        if (d < D) read_words<C::EC * C::EB>(kw[j][hf], k_at + (k0 + 16 * j + 8 * hf + g) * pitch + d * C::EB);
-                        else
+                    for (int j = 0; j < 2 * NG; ++j) {
 #pragma unroll
-                            for (int x = 0; x < C::EC * C::EB / 4; ++x) kw[j][hf][x] = 0u;
+                        for (int x = 0; x < C::EC * C::EB / 4; ++x) kw[j / 2][j % 2][x] = 0u;
+                        if (d < D) read_words<C::EC * C::EB>(kw[j / 2][j % 2], k_at + (k0 + 8 * j + g) * pitch + d * C::EB);
                     }
+                }
 #pragma unroll
                 for (int x = 0; x < PER; ++x) {
                     uint2 q[C::NQ];
@@ -933,11 +957,19 @@ paged_token_kernel(const AttnArgs a)
                     float x = z[j][e];
                     if constexpr (C::NQ > 1) x += zc[j][e];
                     if constexpr (C::CODED) x *= ks[j][e >> 1];
-                    x *= factor[e & 1];
-                    if (masked && !(p0 + 16 * j + 8 * (e >> 1) + g < limit[e & 1] && (there >> j & 1))) x = -INFINITY;
-                    z[j][e] = x;
-                    top[e & 1] = fmaxf(top[e & 1], x);
+                    z[j][e] = x * factor[e & 1];
                 }
+            auto seen = [&](int j, int e) { return p0 + 16 * j + 8 * (e >> 1) + g < limit[e & 1] && (there >> j & 1); };
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[j][e] = seen(j, e) ? z[j][e] : -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], z[j][e]);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -959,15 +991,22 @@ paged_token_kernel(const AttnArgs a)
             for (int j = 0; j < NG; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = z[j][e];
-                    float y = ex2_approx(x - base[e & 1]);
+                    const float y = ex2_approx(z[j][e] - base[e & 1]);
                     l[e & 1] += y;
-                    if constexpr (C::CODED) {
-                        y *= vs[j][e >> 1];
-                        if (masked && x == -INFINITY) y = 0.0f;              // (the scale of a value that a row does not see may be anything)
-                    }
                     z[j][e] = y;
                 }
+            if constexpr (C::CODED) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[j][e] *= vs[j][e >> 1];
+                if (masked) {                        // (the scale of a value that a row does not see may be anything)
+#pragma unroll
+                    for (int j = 0; j < NG; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) z[j][e] = seen(j, e) ? z[j][e] : 0.0f;
+                }
+            }
             uint2 p[C::NQ][NG];
 #pragma unroll
             for (int j = 0; j < NG; ++j)
@@ -983,17 +1022,19 @@ paged_token_kernel(const AttnArgs a)
             for (int c = 0; c < C::NV; ++c) {
                 const int d = (g + 8 * c) * C::EV;
                 uint32_t vw[NG][4][C::EV * C::EB / 4];
+                if (D == DP && !partial) {
 #pragma unroll
-                for (int i = 0; i < NG; ++i)
+                    for (int x = 0; x < 4 * NG; ++x) read_words<C::EV * C::EB>(vw[x / 4][x % 4], v_at + (k0 + 8 * (x >> 1) + 2 * t4 + (x & 1)) * (DP * C::EB) + d * C::EB);
+                } else {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int in = 16 * i + 8 * (x >> 1) + 2 * t4 + (x & 1);
-                        // what lies in places without keys may be anything
-                        if (d < D && (!partial || (p0 + in < keys && (there >> i & 1)))) read_words<C::EV * C::EB>(vw[i][x], v_at + (k0 + in) * pitch + d * C::EB);
-                        else
+                    for (int x = 0; x < 4 * NG; ++x) {
+                        const int in = 8 * (x >> 1) + 2 * t4 + (x & 1);
 #pragma unroll
-                            for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[i][x][y] = 0u;
+                        for (int y = 0; y < C::EV * C::EB / 4; ++y) vw[x / 4][x % 4][y] = 0u;
+                        // (what lies in places without keys may be anything)
+                        if (d < D && p0 + in < keys && (there >> (x / 4) & 1)) read_words<C::EV * C::EB>(vw[x / 4][x % 4], v_at + (k0 + in) * pitch + d * C::EB);
                     }
+                }
 #pragma unroll
                 for (int x = 0; x < C::EV / 2; ++x) {
                     const int j = c * (C::EV / 2) + x;

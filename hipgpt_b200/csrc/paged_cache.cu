@@ -81,8 +81,8 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Four codes of a word.  x * inv + 1.5 * 2^23 rounds to the nearest whole number in the low bits; where a remainder comes within 2^-10 of half a scale, which is seldom, all four
-// are looked at again.
+// Four codes of a word.  x * inv + 1.5 * 2^23 rounds to the nearest whole number in the low bits; x * inv is off by 127 * 2^-24 of a code at most, so only where a remainder
+// comes within 2 * 10^-5 of half a scale, which is seldom, the four are looked at again.
 __device__ __forceinline__ int int8_code(float x, float s, float inv)
 {
     float q = rintf(x * inv);
@@ -102,7 +102,7 @@ __device__ __forceinline__ uint32_t int8_word(const float *x, float s, float inv
         far = fmaxf(far, fabsf(fmaf(kMagic - t[e], s, x[e])));
     }
     uint32_t w = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
-    if (far > 0.4990234375f * s) w = (int8_code(x[0], s, inv) & 255) | (int8_code(x[1], s, inv) & 255) << 8 | (int8_code(x[2], s, inv) & 255) << 16 | (uint32_t)int8_code(x[3], s, inv) << 24;
+    if (far > 0.49998f * s) w = (int8_code(x[0], s, inv) & 255) | (int8_code(x[1], s, inv) & 255) << 8 | (int8_code(x[2], s, inv) & 255) << 16 | (uint32_t)int8_code(x[3], s, inv) << 24;
     return w;
 }
 
