@@ -6,7 +6,7 @@
 //         with 1 / scale may be one off beside a border, and the remainder x - code * scale, which one multiply-add gives exactly, says so
 //
 // Bound: HBM for prompts; the launch for single tokens.  A block takes some tokens; where each goes is looked up once for all its heads.  A row is read 16 bytes a thread by as many neighbouring
-// threads as it needs (a power of two of them), the largest magnitude goes round by shuffles, and a thread has kAhead parts of K and of V on their way at once.
+// threads as it needs (a power of two of them), the largest magnitude goes round by shuffles, and a thread has its parts of K and of V on their way at once.
 #include "paged.cuh"
 
 namespace hipgpt {
@@ -52,9 +52,10 @@ __device__ __forceinline__ void places_of(const MoveArgs &a, int t0, long long (
     __syncthreads();
 }
 
-__device__ __forceinline__ float row_max(float m, int lanes)
+// Magnitudes as their bits: of numbers in their order, infinities and NaN above all of them
+__device__ __forceinline__ uint32_t row_max(uint32_t m, int lanes)
 {
-    for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 1; o < lanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
 
@@ -71,7 +72,7 @@ __device__ __forceinline__ float scale_of(float amax, float &inv)
         return __uint_as_float((uint32_t)(127 + k) << 23);
     } else {
         const float s = fmaxf(__fdiv_rn(amax, 127.0f), 0x1p-126f);
-        inv = __frcp_rn(s);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));        // (2^-23 of it: a guess)
         return s;
     }
 }
@@ -81,8 +82,8 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Four codes of a word.  x * inv + 1.5 * 2^23 rounds to the nearest whole number in the low bits; x * inv is off by 127 * 2^-24 of a code at most, so only where a remainder
-// comes within 2 * 10^-5 of half a scale, which is seldom, the four are looked at again.
+// Four codes of a word.  x * inv + 1.5 * 2^23 rounds to the nearest whole number in the low bits; x * inv is off by 127 * 2^-23 of a code at most, so only where a remainder
+// comes within 4 * 10^-5 of half a scale, which is seldom, the four are looked at again.
 __device__ __forceinline__ int int8_code(float x, float s, float inv)
 {
     float q = rintf(x * inv);
@@ -102,13 +103,22 @@ __device__ __forceinline__ uint32_t int8_word(const float *x, float s, float inv
         far = fmaxf(far, fabsf(fmaf(kMagic - t[e], s, x[e])));
     }
     uint32_t w = __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
-    if (far > 0.49998f * s) w = (int8_code(x[0], s, inv) & 255) | (int8_code(x[1], s, inv) & 255) << 8 | (int8_code(x[2], s, inv) & 255) << 16 | (uint32_t)int8_code(x[3], s, inv) << 24;
+    if (far > 0.49996f * s) w = (int8_code(x[0], s, inv) & 255) | (int8_code(x[1], s, inv) & 255) << 8 | (int8_code(x[2], s, inv) & 255) << 16 | (uint32_t)int8_code(x[3], s, inv) << 24;
     return w;
 }
 
-constexpr int kAhead = 2;
+// A thread takes two chunks of a row of K and of V (what a row takes for itself, its scale and its place, is then for twice the values), `lanes` chunks apart.
+// W: values of a chunk, 16 bytes, or 1 for rows that do not start on 16 bytes (chunks of four values, one by one)
+constexpr int kChunks = 2;
+template <typename T, int W> constexpr int kChunk = W > 1 ? W : 4;
 
-// W: values of 16 bytes, or 1 for rows that do not start on 16 bytes (value by value, four a thread)
+// Row i of the block's rows: its token and head
+__device__ __forceinline__ void row_at(const MoveArgs &a, int i, int &t, int &head)
+{
+    t = a.c.heads == 1 ? i : (int)__umulhi((uint32_t)i, a.per_head);
+    head = i - t * a.c.heads;
+}
+
 template <typename T, int FMT, int W>
 __global__ void __launch_bounds__(kThreads)
 cache_write_kernel(const MoveArgs a)
@@ -116,74 +126,73 @@ cache_write_kernel(const MoveArgs a)
     dependency_wait();
     dependents_may_start();
     __shared__ long long places[kMostTokens];
-    const int t0 = blockIdx.x * a.tokens, D = a.c.D;
+    const int t0 = blockIdx.x * a.tokens, D = a.c.D, lane = threadIdx.x & (a.lanes - 1);
     places_of(a, t0, places);
-    constexpr int N = W > 1 ? W : 4;                 // values a thread
+    constexpr int N = kChunk<T, W>;
     const int all = a.tokens * a.c.heads << a.log_lanes;
-    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < all; i0 += kThreads * kAhead) {
-        float x[kAhead][2][N];
-        long long row[kAhead];
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < all; i0 += kThreads) {
         // (every thread of the warp takes part in the shuffles: those without a row have zeros)
-        const int d = (i0 & (a.lanes - 1)) * N;
+        int t, head;
+        row_at(a, i0 >> a.log_lanes, t, head);
+        long long row = i0 < all ? places[t] : -2;
+        const bool mine = row >= 0;
+        row += (long long)head << a.c.shift;
+        float x[2][kChunks][N];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + kThreads * u, r = i >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
-            row[u] = i < all ? places[t] : -2;
-            const bool mine = row[u] >= 0 && d < D;
-            row[u] = mine ? row[u] + ((long long)head << a.c.shift) : -1;
+        for (int w = 0; w < 2; ++w) {
+            const T *src = static_cast<const T *>(w ? a.v : a.k) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = (lane + c * a.lanes) * N;
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[u][w][e] = 0.0f;
-                if (mine) {
-                    const T *src = static_cast<const T *>(w ? a.v : a.k) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D + d;
-                    if constexpr (W > 1) load_values<T, W>(src, x[u][w]);
+                for (int e = 0; e < N; ++e) x[w][c][e] = 0.0f;
+                if (mine && d < D) {
+                    if constexpr (W > 1) load_values<T, W>(src + d, x[w][c]);
                     else
 #pragma unroll
-                        for (int e = 0; e < N; ++e) x[u][w][e] = to_float(src[e]);
+                        for (int e = 0; e < N; ++e) x[w][c][e] = to_float(src[d + e]);
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
+        for (int w = 0; w < 2; ++w) {
+            uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);
+            if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
+                T *dst = reinterpret_cast<T *>(base) + row * D;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);
-                if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                    if (row[u] >= 0) {
-                        T *dst = reinterpret_cast<T *>(base) + row[u] * D + d;
-                        if constexpr (W > 1) store_values<T, W>(dst, x[u][w]);
-                        else
+                for (int c = 0; c < kChunks; ++c) {
+                    const int d = (lane + c * a.lanes) * N;
+                    if (mine && d < D) store_values<T, N>(dst + d, x[w][c]);
+                }
+            } else {
+                uint32_t most = 0;
 #pragma unroll
-                            for (int e = 0; e < N; ++e) dst[e] = from_float<T>(x[u][w][e]);
-                    }
-                } else {
-                    float m = 0.0f;
-                    bool fine = true;
+                for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        m = fmaxf(m, fabsf(x[u][w][e]));
-                        fine = fine && fabsf(x[u][w][e]) <= 3.402823466e38f;
-                    }
-                    m = row_max(fine ? m : INFINITY, a.lanes);
-                    float inv, s = scale_of<FMT>(m, inv);
-                    const bool whole = m <= 3.402823466e38f;
+                    for (int e = 0; e < N; ++e) most = max(most, __float_as_uint(x[w][c][e]) & 0x7FFFFFFFu);
+                most = row_max(most, a.lanes);
+                const bool whole = most < 0x7F800000u;
+                float inv, s = scale_of<FMT>(__uint_as_float(most), inv);
+                uint8_t *dst = base + row * D;
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    const int d = (lane + c * a.lanes) * N;
                     uint32_t code[N / 4];
 #pragma unroll
                     for (int e = 0; e < N / 4; ++e) {
-                        const float *y = x[u][w] + 4 * e;
+                        const float *y = x[w][c] + 4 * e;
                         if constexpr (FMT == HIPGPT_CACHE_E4M3) code[e] = e4m3_pair(y[0] * inv, y[1] * inv) | e4m3_pair(y[2] * inv, y[3] * inv) << 16;
                         else code[e] = int8_word(y, s, inv);
                         if (!whole) code[e] = 0u;
                     }
-                    if (row[u] >= 0) {
-                        uint8_t *dst = base + row[u] * D + d;
-                        if constexpr (N == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(code[0], code[1]);
-                        else *reinterpret_cast<uint32_t *>(dst) = code[0];
-                        if (d == 0) const_cast<float *>(w ? a.c.vs : a.c.ks)[row[u]] = whole ? s : __uint_as_float(0x7FFFFFFFu);
+                    if (mine && d < D) {
+                        if constexpr (N == 8) *reinterpret_cast<uint2 *>(dst + d) = make_uint2(code[0], code[1]);
+                        else *reinterpret_cast<uint32_t *>(dst + d) = code[0];
                     }
                 }
+                if (mine && lane == 0) const_cast<float *>(w ? a.c.vs : a.c.ks)[row] = whole ? s : __uint_as_float(0x7FFFFFFFu);
             }
+        }
     }
 }
 
@@ -194,60 +203,56 @@ cache_read_kernel(const MoveArgs a)
     dependency_wait();
     dependents_may_start();
     __shared__ long long places[kMostTokens];
-    const int t0 = blockIdx.x * a.tokens, D = a.c.D;
+    const int t0 = blockIdx.x * a.tokens, D = a.c.D, lane = threadIdx.x & (a.lanes - 1);
     places_of(a, t0, places);
-    constexpr int N = W > 1 ? W : 4;
+    constexpr int N = kChunk<T, W>;
     const int all = a.tokens * a.c.heads << a.log_lanes;
-    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kAhead) {
-        float x[kAhead][2][N], s[kAhead][2];
-        uint32_t word[kAhead][2][2];
-        long long place[kAhead];
-        const int d = (i0 & (a.lanes - 1)) * N;
-        if (d >= D) continue;
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+        int t, head;
+        row_at(a, i >> a.log_lanes, t, head);
+        const long long place = places[t], row = place + ((long long)head << a.c.shift);
+        if (place == -2) continue;
+        float x[2][kChunks][N], s[2] = {0.0f, 0.0f};
+        uint32_t word[2][kChunks][2];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + kThreads * u, r = i >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
-            place[u] = i < all ? places[t] : -2;
-            const long long row = place[u] + ((long long)head << a.c.shift);
+        for (int w = 0; w < 2; ++w) {
+            const uint8_t *base = w ? a.c.v : a.c.k;
+            if constexpr (FMT != HIPGPT_CACHE_PLAIN) if (place >= 0) s[w] = __ldg((w ? a.c.vs : a.c.ks) + row);
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const uint8_t *base = w ? a.c.v : a.c.k;
-                s[u][w] = 0.0f;
-                word[u][w][0] = word[u][w][1] = 0u;
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = (lane + c * a.lanes) * N;
+                word[w][c][0] = word[w][c][1] = 0u;
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[u][w][e] = 0.0f;
-                if (place[u] < 0) continue;
+                for (int e = 0; e < N; ++e) x[w][c][e] = 0.0f;
+                if (place < 0 || d >= D) continue;
                 if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                    load_values<T, N>(reinterpret_cast<const T *>(base) + row * D + d, x[u][w]);
+                    load_values<T, N>(reinterpret_cast<const T *>(base) + row * D + d, x[w][c]);
+                } else if constexpr (N == 8) {
+                    const uint2 y = *reinterpret_cast<const uint2 *>(base + row * D + d);
+                    word[w][c][0] = y.x; word[w][c][1] = y.y;
                 } else {
-                    s[u][w] = __ldg((w ? a.c.vs : a.c.ks) + row);
-                    if constexpr (N == 8) {
-                        const uint2 y = *reinterpret_cast<const uint2 *>(base + row * D + d);
-                        word[u][w][0] = y.x; word[u][w][1] = y.y;
-                    } else {
-                        word[u][w][0] = *reinterpret_cast<const uint32_t *>(base + row * D + d);
-                    }
+                    word[w][c][0] = *reinterpret_cast<const uint32_t *>(base + row * D + d);
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (place[u] == -2) continue;
-            const int r = (i0 + kThreads * u) >> a.log_lanes, t = a.c.heads == 1 ? r : (int)__umulhi((uint32_t)r, a.per_head), head = r - t * a.c.heads;
+        for (int w = 0; w < 2; ++w) {
+            T *dst = static_cast<T *>(const_cast<void *>(w ? a.v : a.k)) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
+            for (int c = 0; c < kChunks; ++c) {
+                const int d = (lane + c * a.lanes) * N;
+                if (d >= D) continue;
                 if constexpr (FMT != HIPGPT_CACHE_PLAIN)
 #pragma unroll
                     for (int e = 0; e < N / 2; ++e) {
-                        const uint32_t two = code_pair<FMT>(word[u][w][e / 2], word[u][w][e / 2], (e & 1) * 2, (e & 1) * 2 + 1);
-                        x[u][w][2 * e] = __uint_as_float(two << 16) * s[u][w];
-                        x[u][w][2 * e + 1] = __uint_as_float(two & 0xFFFF0000u) * s[u][w];
+                        const uint32_t two = code_pair<FMT>(word[w][c][e / 2], word[w][c][e / 2], (e & 1) * 2, (e & 1) * 2 + 1);
+                        x[w][c][2 * e] = __uint_as_float(two << 16) * s[w];
+                        x[w][c][2 * e + 1] = __uint_as_float(two & 0xFFFF0000u) * s[w];
                     }
-                T *dst = static_cast<T *>(const_cast<void *>(w ? a.v : a.k)) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D + d;
-                if constexpr (W > 1) store_values<T, W>(dst, x[u][w]);
+                if constexpr (W > 1) store_values<T, W>(dst + d, x[w][c]);
                 else
 #pragma unroll
-                    for (int e = 0; e < N; ++e) dst[e] = from_float<T>(x[u][w][e]);
+                    for (int e = 0; e < N; ++e) dst[d + e] = from_float<T>(x[w][c][e]);
             }
         }
     }
@@ -258,17 +263,17 @@ int launch_move(MoveArgs a, bool write, cudaStream_t st)
 {
     constexpr int W = kPer16<T>;
     const bool vec = all_aligned16({a.k, a.v}) && a.k_stride % W == 0 && a.v_stride % W == 0;
-    // D / W threads of 16 bytes, rounded up to a power of two; without them four values each
+    // As many threads as take D values two chunks each, rounded up to a power of two
     a.log_lanes = 0;
-    while ((vec ? W : 4) << a.log_lanes < a.c.D) ++a.log_lanes;
+    while (kChunks * (vec ? W : 4) << a.log_lanes < a.c.D) ++a.log_lanes;
     a.lanes = 1 << a.log_lanes;
-    // Tokens a block: one where there are few, 32 (whose places are looked up side by side) where there are enough for four blocks an SM
+    // Tokens a block: one where there are few, 32 (whose places are looked up side by side) where there are enough for eight blocks an SM
     const long long each = (long long)a.c.heads << a.log_lanes;
     a.tokens = 1;
-    while (a.tokens < kMostTokens && (a.tokens * each < kThreads * kAhead || a.c.T / (2 * a.tokens) >= 148 * 4) && a.c.T >= 2 * a.tokens * 148) a.tokens *= 2;
+    while (a.tokens < kMostTokens && (a.tokens * each < kThreads || a.c.T / (2 * a.tokens) >= 148 * 8) && a.c.T >= 2 * a.tokens * 148) a.tokens *= 2;
     const long long blocks = ((long long)a.c.T + a.tokens - 1) / a.tokens;
     a.per_head = (uint32_t)(((1ull << 32) + a.c.heads - 1) / a.c.heads);             // (of one head: not used)
-    if (each * a.tokens > 1LL << 30 || ((long long)a.tokens * a.c.heads + kThreads * kAhead) * a.c.heads >= 1LL << 32) return fail(HIPGPT_ERR_BAD_ARG, "rows of %d heads are beyond one call", a.c.heads);
+    if (each * a.tokens > 1LL << 30 || ((long long)a.tokens * a.c.heads + kThreads) * a.c.heads >= 1LL << 32) return fail(HIPGPT_ERR_BAD_ARG, "rows of %d heads are beyond one call", a.c.heads);
     const auto kern = write ? (vec ? cache_write_kernel<T, FMT, W> : cache_write_kernel<T, FMT, 1>) : (vec ? cache_read_kernel<T, FMT, W> : cache_read_kernel<T, FMT, 1>);
     const cudaError_t e = launch_overlapped(kern, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
     const char *what = write ? "cache_write_kernel" : "cache_read_kernel";
