@@ -108,7 +108,9 @@ struct Run {
         long long n = count(0, i), mine = n;
         for (int b0 = THREADS; b0 < a.c.B; b0 += THREADS) { int x; mine += count(b0, x); }
         const long long total = block_sum<THREADS>(mine, shared);
-        per = max((total + gridDim.x - 1) / gridDim.x, (long long)a.least);
+        // (64-bit divisions take a hundred instructions)
+        per = total < 1 << 30 ? (int)(((unsigned)total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
+        per = max(per, (long long)a.least);
         u = start = (long long)blockIdx.x * per;
         end = min(total, u + per);
         if (u >= end) return false;
@@ -163,7 +165,7 @@ struct Run {
             }
             base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        head = (int)((u - base) / units);
+        head = u - base < 1 << 30 ? (int)((unsigned)(u - base) / (unsigned)units) : (int)((u - base) / units);
         base += (long long)head * units;
         return true;
     }
@@ -254,6 +256,11 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
         l = fmaf(l, alpha, e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) o[i] = fmaf(e, cached<T, FMT>(a.c.v, a.c.vs, r, D, lane + 32 * i), o[i] * alpha);
+        // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
+        bool number = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) number = number || (lane + 32 * i < D && o[i] == o[i]);
+        if (l != l || !__any_sync(0xffffffffu, number)) break;
     }
     T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
 #pragma unroll

@@ -8,12 +8,14 @@
 //   warps 8-11       codes: widen them to fp16 in the layout of the operands, two tiles of keys and of values ahead, times their scales over a power of two of each 64 keys, which goes
 //                    into the scores' factor, and for V into the exponent of P.  (e4m3: exact; int8: values are rounded to fp16, as P is, scores multiplied by the keys' scales instead.)
 //                    Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
-//   warp 12          issues the products: P V of a tile, 64 keys as soon as the softmax has them, then Q K^T of its next keys over the same columns of TMEM (products of one thread run in
+//   warp 12          (codes: and 14, one for each tile) issues the products: P V of a tile, 64 keys as soon as the softmax has them, then Q K^T of its next keys over the same columns of TMEM (products of one thread run in
 //                    the order of their issue, so a commit behind the second covers the first); the other tile's softmax runs meanwhile.
 //   warp 13          asks for the copies, a lane a run of keys in one page: boxes of 64 columns, swizzled, straight into the operands (plain; a page that is none lies
 //                    outside the tensor and comes as zeros), or codes and scales as they lie into a ring of half tiles.  (Loads by the threads themselves, 16 KB on their way, brought
 //                    6 bytes a clock; bulk copies bring 24.)
-// Bound: the special-function unit (16 exponentials a clock) and the tensor pipe alike at D = 128.
+// Bound: neither pipe yet.  At D = 128 a unit's products are 2048 clocks of the tensor pipe and its exponentials as many of the special-function unit; plain rows take 4150, the chain from P to the next scores
+// (P V's second half, Q K^T, two commits: 1750) and the softmax (2300) of a tile one after the other, the two tiles half a turn apart; int8 takes 6500, widening the codes (four half tiles of
+// 1600).  32 heads over 8 of 128: five ragged sequences of 1100 new tokens in 8000, plain: 487 us (420 with the cache in L2: 911 TFLOP/s); 4096 new tokens in 32768, int8: 3.05 ms, 676 TFLOP/s.
 // Every wait is bounded: on expiry the block raises a flag that cuts all later waits short, records a status code, skips its stores, lets what is on its way land,
 // frees its TMEM and returns.
 #include "attn_paged.cuh"

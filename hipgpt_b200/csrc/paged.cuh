@@ -1,5 +1,4 @@
-// A cache in pages and the ragged batch that works on it: what the kernels of rotary.cu's neighbours share (paged_cache.cu, attn_paged.cu,
-// attn_paged_tc.cu).
+// A cache in pages and the ragged batch that works on it: what rotary.cu, paged_cache.cu, attn_paged.cu and attn_paged_tc.cu share.
 //
 //   cache   k, v [pages][heads][page size][D] of the activations' type, or of 8-bit codes with one fp32 scale per row ([pages][heads][page size])
 //   batch   sequence b's new tokens are the rows offsets[b] .. offsets[b+1] of the call's tensors; they are the last of the lengths[b] tokens that the
@@ -78,7 +77,7 @@ inline int check_paged(const hipgpt_paged_cache *c, const hipgpt_paged_batch *b,
     if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return fail(HIPGPT_ERR_BAD_ARG, "page size %d is no power of two from 16 to 1024", c->page_size);
     if (c->head_dim % 16 || c->head_dim > 128) return fail(HIPGPT_ERR_UNSUPPORTED, "head_dim %d is no multiple of 16 up to 128", c->head_dim);
     if ((long long)c->heads * c->head_dim > 1 << 24) return fail(HIPGPT_ERR_BAD_ARG, "rows of %d heads of %d values are too long", c->heads, c->head_dim);
-    if ((long long)b->most_pages * c->page_size > 2147483647LL) return fail(HIPGPT_ERR_BAD_ARG, "%d pages of %d tokens are beyond what a length can say", b->most_pages, c->page_size);
+    if ((long long)b->most_pages * c->page_size > 1 << 30) return fail(HIPGPT_ERR_BAD_ARG, "%d pages of %d tokens are beyond one sequence", b->most_pages, c->page_size);
     if ((long long)c->pages * c->heads > 2147483646LL || (long long)c->pages * c->heads * c->page_size > 1LL << 40) return fail(HIPGPT_ERR_BAD_ARG, "a cache of %d pages is too large", c->pages);
     if (b->tokens == 0 || b->sequences == 0) return 1;
     if (!b->offsets || !b->lengths || (!b->page_table && b->most_pages > 0)) return fail(HIPGPT_ERR_NULL, "offsets, lengths and the page table must not be NULL");

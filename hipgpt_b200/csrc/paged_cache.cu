@@ -127,17 +127,14 @@ cache_write_kernel(const MoveArgs a)
     dependents_may_start();
     __shared__ long long places[kMostTokens];
     const int t0 = blockIdx.x * a.tokens, D = a.c.D, lane = threadIdx.x & (a.lanes - 1);
-    places_of(a, t0, places);
     constexpr int N = kChunk<T, W>;
     const int all = a.tokens * a.c.heads << a.log_lanes;
-    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < all; i0 += kThreads) {
-        // (every thread of the warp takes part in the shuffles: those without a row have zeros)
-        int t, head;
+    float x[2][kChunks][N];
+    int t, head;
+    // (every thread of the warp takes part in the shuffles: those without a row have zeros)
+    auto fetch = [&](int i0) {
         row_at(a, i0 >> a.log_lanes, t, head);
-        long long row = i0 < all ? places[t] : -2;
-        const bool mine = row >= 0;
-        row += (long long)head << a.c.shift;
-        float x[2][kChunks][N];
+        const bool here = i0 < all && t0 + t < a.c.T;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const T *src = static_cast<const T *>(w ? a.v : a.k) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D;
@@ -146,7 +143,7 @@ cache_write_kernel(const MoveArgs a)
                 const int d = (lane + c * a.lanes) * N;
 #pragma unroll
                 for (int e = 0; e < N; ++e) x[w][c][e] = 0.0f;
-                if (mine && d < D) {
+                if (here && d < D) {
                     if constexpr (W > 1) load_values<T, W>(src + d, x[w][c]);
                     else
 #pragma unroll
@@ -154,6 +151,14 @@ cache_write_kernel(const MoveArgs a)
                 }
             }
         }
+    };
+    fetch(threadIdx.x);                              // (on their way while the places are looked up)
+    places_of(a, t0, places);
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < all; i0 += kThreads) {
+        if (i0 != (int)threadIdx.x) fetch(i0);
+        long long row = i0 < all ? places[t] : -2;
+        const bool mine = row >= 0;
+        row += (long long)head << a.c.shift;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             uint8_t *base = const_cast<uint8_t *>(w ? a.c.v : a.c.k);

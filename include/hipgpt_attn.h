@@ -320,7 +320,7 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *     A row that holds an infinity or NaN gets codes 0 and the scale NaN: all of it reads as NaN.
  *   hipgpt_paged_batch   `tokens` new tokens of `sequences` sequences, rows of the call's tensors: sequence b's are offsets[b] .. offsets[b+1]-1
  *                        (offsets [sequences + 1], ascending), the last ones of the lengths[b] tokens that it has with them; position p of sequence b lies in page
- *                        page_table[b][p / page_size] ([sequences][most_pages]) at p % page_size.  All three on the device, read when the kernels run (a captured
+ *                        page_table[b][p / page_size] ([sequences][most_pages], most_pages * page_size <= 2^30) at p % page_size.  All three on the device, read when the kernels run (a captured
  *                        call sees what they hold at its replay), so bad values cannot be refused: offsets are cut to [0, tokens], lengths to most_pages *
  *                        page_size, a page number outside [0, pages) is a page without tokens.  Rows of no sequence are left as they are.
  *   Tensors of tokens have rows of heads * head_dim values, *_stride values apart (a part of a wider row, as of a packed projection, is one).  No output may overlap
@@ -340,8 +340,11 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *   hipgpt_paged_attention     out[t][h] = softmax(scale q k^T) v over the keys of t's sequence: causal != 0 those up to t's position, 0 all lengths[b].
  *                              q, out [tokens][H * head_dim], H a multiple of the cache's heads: H / heads query heads in a row share one.  A row that sees no key gets zeros
  *                              (as one whose scores are all minus infinity).  What lies in masked places, NaN too, does not matter.  scale > 0.
- *                              fp32: products from three bf16 pieces of each fp32 operand on the tensor pipe, sums in fp32; an infinity in q or a plain cache makes NaN of
- *                              the scores that it meets.  bf16: probabilities are rounded to bf16 before the second product.
+ *                              Products on the tensor pipe, sums in fp32.  fp32: of three bf16 pieces of each operand (24 bits), against codes of two fp16 pieces (22 bits, a power of
+ *                              two for each row of q); an infinity in q or a plain cache makes NaN of the scores that it meets.  bf16, plain cache: probabilities are rounded to bf16 before
+ *                              the second product.  8-bit caches: probabilities times their values' scales are held in fp16 over a power of two that follows the largest: a value whose scale is
+ *                              below 2^-38 of its sequence's largest is lost.  bf16 with many rows a sequence: in int8 a value times its scale is rounded to fp16, and values share a power of two
+ *                              with the 63 keys beside them: scales down to 2^-21 of their largest keep all digits.
  *                              Keys are split over blocks where rows are few; buffers of the library (per device and stream, at most eight; hipgpt_release_workspace()
  *                              frees them; a captured call gets buffers of its graph) hold the parts.  The same bits run to run on the same GPU.
  */
@@ -518,7 +521,7 @@ HIPGPT_API int hipgpt_set_full_range(int on);
  *       arrives, with a limit of `limit_cycles` SM cycles (at most 2^24, a few milliseconds).  Afterwards
  *       hipgpt_kernel_status() reports 907 and d_canary[0..n) is untouched.
  *   hipgpt_debug_expire_wait  in the calling thread's next call of a tensor-core projection (code 501 ... 504) or of a tensor-core
- *       backward (601 ... 627) or loss, forward or backward (701 ... 704), or of attention of many rows over a paged cache (1001 ... 1008), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
+ *       backward (601 ... 627) or loss, forward or backward (701 ... 704), or of attention of many rows over a paged cache (1001 ... 1010), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
  *       each of the call's launches that has it, if it has to wait at all.
  *   hipgpt_gpt_debug_stall_barrier  makes the NEXT hipgpt_gpt_generate call give up: in the persistent mode it starts with a
  *       grid-barrier counter that cannot complete, and every block gives up at its first barrier; by clusters the first block's

@@ -474,3 +474,59 @@ def test_long_calls_give_the_same_bits_every_time(fmt, n, length):
         got.fill_(float("nan"))
         serving.paged_attention(cache, q, got, *batch.args, 16)
         assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("seqs", [[(300, 900), (70, 80)], [(1, 900), (4, 500)], [(20, 700)]], ids=["many", "tokens", "some"])
+def test_rows_of_any_magnitude(fmt, dtype, seqs):
+    """Values of zeros, tiny and large ones page beside page, keys and queries far from one: the powers of two that rows and tiles share follow them."""
+    batch = Batch(seqs, 64, seed=13)
+    heads, H, D = 2, 4, 64
+
+    def wild(name, x):
+        if name == "k":
+            x *= 2.0 ** -30
+        else:
+            for page in range(len(x)):
+                x[page] *= (0.0, 2.0 ** -20, 1.0, 2.0 ** 10)[page % 4]
+    _, _, out, want, bound, _ = _attend(batch, heads, H, D, dtype, fmt, wild=wild, spread=2.0 ** 31)
+    within(out, want, bound)
+
+    def tiny(name, x):
+        x *= 2.0 ** -100                                            # scores of zero, values near the smallest numbers
+    _, _, out, want, bound, _ = _attend(batch, heads, H, D, dtype, fmt, wild=tiny, spread=2.0 ** -100)
+    within(out, want, bound)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_nothing_but_nan(fmt, dtype):
+    """Every value NaN: every row that sees one is NaN, and the call comes back."""
+    batch = Batch([(600, 20000), (1, 20000), (3, 3)], 64, seed=1)
+
+    def wild(name, x):
+        if name == "v":
+            x.fill_(float("nan"))
+    cache, _, _ = su.filled_cache(batch, 2, 64, dtype, fmt, wild=wild)
+    q = _normal(_gen(1), batch.T, 4, 64, dtype=dtype)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, *batch.args, 4)
+    assert bool(torch.isnan(out).all()) and _status() == 0
+
+
+def test_many_short_sequences():
+    """More sequences than a block has threads, some empty, of one token and more."""
+    gen = torch.Generator().manual_seed(5)
+    seqs = [(int(n), int(n) + int(m)) for n, m in zip(torch.randint(0, 3, (700,), generator=gen), torch.randint(0, 40, (700,), generator=gen))]
+    for dtype, fmt in ((F32, "plain"), (BF16, "e4m3")):
+        for group in (2, 40):                                       # few rows a sequence, and many
+            batch = Batch(seqs, 16, seed=6)
+            _, _, out, want, bound, mine = _attend(batch, 1, group, 32, dtype, fmt)
+            within(out[mine], want[mine], bound[mine])
+    x = _normal(_gen(3), batch.T, 1, 32, dtype=BF16)
+    cache = serving.PagedCache(batch.num_pages, 16, 1, 32, dtype=BF16, format="plain")
+    back = [torch.full_like(x, float("nan")) for _ in range(2)]
+    serving.cache_write(cache, x, x, *batch.args)
+    serving.cache_read(cache, *back, *batch.args)
+    assert torch.equal(back[0], x) and torch.equal(back[1], x)
