@@ -5,17 +5,18 @@
 //   warps 0-3, 4-7   softmax of the first and of the second tile, a thread a row: its scores are read from TMEM into registers, P = exp2(s - m) goes over them in
 //                    bf16.  The reference maximum m moves, and the sums so far are scaled, when a row of the warp has outgrown it by more than 2^8 (P in bf16 and
 //                    sums in fp32 do not care).  P V is summed in TMEM.
-//   warps 8-11       codes: widen them to fp16 in the layout of the operands, two tiles of keys and of values ahead, times their scales over a power of two of each 64 keys, which goes
+//   warps 8-11       codes that were not widened before the kernel: widen them to fp16 in the layout of the operands, two tiles of keys and of values ahead, times their scales over a power of two of each 64 keys, which goes
 //                    into the scores' factor, and for V into the exponent of P.  (e4m3: exact; int8: values are rounded to fp16, as P is, scores multiplied by the keys' scales instead.)
-//                    Plain rows: one warp clears the rows of V behind the last key, which may hold anything.
-//   warp 12          (codes: and 14, one for each tile) issues the products: P V of a tile, 64 keys as soon as the softmax has them, then Q K^T of its next keys over the same columns of TMEM (products of one thread run in
+//                    Plain and widened rows: one warp clears the rows of V behind the last key, which may hold anything.
+//   warp 12          (codes widened here: and 14, one for each tile) issues the products: P V of a tile, 64 keys as soon as the softmax has them, then Q K^T of its next keys over the same columns of TMEM (products of one thread run in
 //                    the order of their issue, so a commit behind the second covers the first); the other tile's softmax runs meanwhile.
 //   warp 13          asks for the copies, a lane a run of keys in one page: boxes of 64 columns, swizzled, straight into the operands (plain; a page that is none lies
 //                    outside the tensor and comes as zeros), or codes and scales as they lie into a ring of half tiles.  (Loads by the threads themselves, 16 KB on their way, brought
 //                    6 bytes a clock; bulk copies bring 24.)
 // Bound: neither pipe yet.  At D = 128 a unit's products are 2048 clocks of the tensor pipe and its exponentials as many of the special-function unit; plain rows take 4150, the chain from P to the next scores
-// (P V's second half, Q K^T, two commits: 1750) and the softmax (2300) of a tile one after the other, the two tiles half a turn apart; int8 takes 6500, widening the codes (four half tiles of
-// 1600).  32 heads over 8 of 128: five ragged sequences of 1100 new tokens in 8000, plain: 487 us (420 with the cache in L2: 911 TFLOP/s); 4096 new tokens in 32768, int8: 3.05 ms, 676 TFLOP/s.
+// (P V's second half, Q K^T, two commits: 1750) and the softmax (2300) of a tile one after the other, the two tiles half a turn apart.  Widening codes here takes 6500 (four half
+// tiles of 1600).  32 heads over 8 of 128: five ragged sequences of 1100 new tokens in 8000, plain: 446 us, 857 TFLOP/s; 4096 new tokens in 32768, int8: 2.12 ms, 972 TFLOP/s, widened before;
+// 3.03 ms, widened here.
 // Every wait is bounded: on expiry the block raises a flag that cuts all later waits short, records a status code, skips its stores, lets what is on its way land,
 // frees its TMEM and returns.
 #include "attn_paged.cuh"
@@ -54,21 +55,29 @@ __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int si
 // The largest scale of 64 keys goes to [2^k, 2^(k + 1)) in fp16: 128 * 2^8 and 448 * 2^7 are still numbers there, and rows whose scale is 2^-21 of it keep their digits
 template <int FMT> constexpr int kUp = FMT == HIPGPT_CACHE_E4M3 ? 6 : 7;
 
-template <int FMT, int DP>
-struct TcCfg {
-    static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2, kSlot = kHalf * DP;
-    static constexpr size_t kBytes = 2 * (size_t)kQTile + 2 * kStages * (size_t)kTile + (FMT == HIPGPT_CACHE_PLAIN ? 0 : kSlots * (size_t)kSlot) + 1024;
+// Codes that were widened before the call's attention: rows of fp16 of each sequence and head, one behind the other
+struct Wide {
+    void *k, *v;                         // [sequence][head][room][D]
+    float *scale;                        // [sequence][head][room]: int8, the scales of the keys
+    float *k_unit, *v_exp;               // [sequence][head][room / 64]
+    int room;                            // keys, a multiple of 128
 };
 
-template <int FMT, int DP>
+template <int FMT, int DP, bool WIDENED>
+struct TcCfg {
+    static constexpr int kQTile = 128 * DP * 2, kTile = kKeys * DP * 2, kSlot = kHalf * DP;
+    static constexpr size_t kBytes = 2 * (size_t)kQTile + 2 * kStages * (size_t)kTile + (FMT == HIPGPT_CACHE_PLAIN || WIDENED ? 0 : kSlots * (size_t)kSlot) + 1024;
+};
+
+template <int FMT, int DP, bool WIDENED>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a, int expire)
+paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a, const Wide wide, int expire)
 {
-    using C = TcCfg<FMT, DP>;
+    using C = TcCfg<FMT, DP, WIDENED>;
     using T = __nv_bfloat16;
-    constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN, SCALED = FMT == HIPGPT_CACHE_INT8;
+    constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN, SCALED = FMT == HIPGPT_CACHE_INT8, WIDENS = CODED && !WIDENED;
     constexpr float kBias = CODED ? 6.0f : 0.0f;
-    constexpr int kIssuers = CODED ? 2 : 1;
+    constexpr int kIssuers = WIDENS ? 2 : 1;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *q_s = base;                             // [tile][block of 64 columns][128 rows][128 B], swizzled
@@ -76,8 +85,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t *v_s = k_s + kStages * C::kTile;         // the same bytes, read as an N-major operand
     uint8_t *raw_s = v_s + kStages * C::kTile;       // [slot][64 keys][D] codes as they lie in their pages
     __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2][2], o_done[2];
-    __shared__ uint64_t landed[CODED ? kSlots : kStages], raw_free[kSlots];
-    __shared__ __align__(16) float scale_s[CODED ? kSlots : 1][kHalf];
+    __shared__ uint64_t landed[WIDENS ? kSlots : kStages], raw_free[kSlots];
+    __shared__ __align__(16) float scale_s[WIDENS ? kSlots : 1][kHalf];
     __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys];       // int8: the scales of the keys
     __shared__ float k_unit[kTables][2], v_exp[kTables][2];          // codes: the power of two that each 64 keys of a tile were divided by, the exponent of that of the values
     __shared__ float q_unit[CODED ? 2 * 128 : 1];                    // and that of a row of Q
@@ -91,8 +100,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&k_full[i], CODED ? kWideners / 32 : 1);
-            mbar_init(&v_full[i], CODED ? kWideners / 32 : 1);
+            mbar_init(&k_full[i], WIDENS ? kWideners / 32 : 1);
+            mbar_init(&v_full[i], WIDENS ? kWideners / 32 : 1);
             mbar_init(&k_free[i], kIssuers);
             mbar_init(&v_free[i], kIssuers);
         }
@@ -103,7 +112,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             mbar_init(&p_full[i][1], 4);
             mbar_init(&o_done[i], 1);
         }
-        for (int i = 0; i < (CODED ? kSlots : kStages); ++i) mbar_init(&landed[i], 1);
+        for (int i = 0; i < (WIDENS ? kSlots : kStages); ++i) mbar_init(&landed[i], 1);
         for (int i = 0; i < kSlots; ++i) mbar_init(&raw_free[i], kWideners / 32);
     }
     if (warp == 12) {
@@ -172,12 +181,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 255u;
                 const int next_page = u + 1 < w.from + units ? look(u + 1) : -1;
                 if (lane == 0) there_s[n % kTables] = there;         // (before the arrivals below)
-                if constexpr (!CODED) {
+                if constexpr (!WIDENS) {
                     constexpr int NB = DP / 64;
-                    const int run_keys = min(page_keys, kKeys), runs = kKeys / run_keys;
+                    const int run_keys = WIDENED ? kKeys : min(page_keys, kKeys), runs = kKeys / run_keys;
                     const int at = lane / NB * run_keys, x = lane % NB * 64;                    // this lane's box
                     const int pg = __shfl_sync(0xffffffffu, page, (at >> 4) & 7);
-                    const int z = pg < 0 ? a.c.pages * a.c.heads : pg * a.c.heads + w.head;
+                    const int z = WIDENED ? w.b * a.c.heads + w.head : pg < 0 ? a.c.pages * a.c.heads : pg * a.c.heads + w.head;
+                    const int y = WIDENED ? p0 : (p0 + at) & (page_keys - 1);
 #pragma unroll
                     for (int which = 0; which < 2; ++which) {
                         if (n >= kStages) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
@@ -186,7 +196,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         if (lane == 0 && seen) mbar_arrive_expect_tx(bar, (uint32_t)C::kTile);
                         __syncwarp();
                         if (lane < runs * NB && seen)
-                            tma_load_3d((which ? v_s : k_s) + st * C::kTile + (x / 64) * (kKeys * 128) + at * 128, which ? &vmap : &kmap, x, (p0 + at) & (page_keys - 1), z, bar);
+                            tma_load_3d((which ? v_s : k_s) + st * C::kTile + (x / 64) * (kKeys * 128) + at * 128, which ? &vmap : &kmap, x, y, z, bar);
                     }
                 } else {
                     const int run_keys = min(page_keys, kHalf), runs = kHalf / run_keys;
@@ -221,16 +231,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int pt = tid - 256, D = a.c.D;
         uint32_t n = 0, slot = 0;
         int v_most = 0;                              // the largest exponent of values so far
-        if constexpr (!CODED) more = more && warp == 8;
+        if constexpr (!WIDENS) more = more && warp == 8;
         for (; more; more = run.next()) {
             const Tile w = run.at();
             const int units = max(units_of(w, 0), units_of(w, 1)), keys = tile_keys<kRows>(a, w.s, w.tile);
             v_most = -200;
+            // (widened: the scales of a tile's keys, and the two powers of two of its keys and of its values, a tile ahead)
+            float4 scales = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float unit = 0.0f;
+            auto fetch = [&](int u) {
+                const size_t bh = (size_t)w.b * a.c.heads + w.head;
+                if constexpr (SCALED) scales = *reinterpret_cast<const float4 *>(wide.scale + bh * wide.room + u * kKeys + lane * 4);
+                if (lane < 4) unit = (lane < 2 ? wide.k_unit : wide.v_exp)[bh * (wide.room / kHalf) + u * 2 + (lane & 1)];
+            };
+            if constexpr (WIDENED) if (units > 0) fetch(w.from);
             for (int u = w.from; u < w.from + units; ++u, ++n) {
                 const int st = n % kStages, p0 = u * kKeys;
                 const uint32_t ph = (n / kStages) & 1;
-                if constexpr (!CODED) {
+                if constexpr (!WIDENS) {
                     wait(&landed[st], ph, 9);
+                    if constexpr (WIDENED) {
+                        if constexpr (SCALED) *reinterpret_cast<float4 *>(&ks_s[n % kTables][lane * 4]) = scales;
+                        if (lane < 4) (lane < 2 ? k_unit : v_exp)[n % kTables][lane & 1] = unit;
+                        if (u + 1 < w.from + units) fetch(u + 1);
+                    }
                     const int first = keys - p0;
                     if (first < kKeys) {
                         for (int i = max(first, 0) * 8 + lane; i < kKeys * 8; i += 32)
@@ -319,7 +343,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
     } else if (warp >= 12) {
         // ================= the products =========================================================================
-        // Plain rows: one warp issues those of both tiles, one tile's after the other's, so that one tile's softmax runs beside the other's products.  (Two warps' products share the pipe, and
+        // Plain and widened rows: one warp issues those of both tiles, one tile's after the other's, so that one tile's softmax runs beside the other's products.  (Two warps' products share the pipe, and
         // both tiles' scores come late, at the same time: 442 against 422 us.)  Codes: a warp for each tile, because they wait for the values to be widened and must not wait for each other too.
         constexpr uint32_t kHalfTypes = CODED ? ~((1u << 7) | (1u << 10)) : ~0u;         // fp16 operands instead of bf16
         constexpr uint32_t idesc_qk = idesc_bf16(128, kKeys, 0) & kHalfTypes, idesc_pv = idesc_bf16(128, DP, 1) & kHalfTypes;
@@ -467,6 +491,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
                 const bool masked = p0 + kKeys > least_limit || there != 255u;
                 float v[4][32];
+                if constexpr (WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);                  // (what was divided out comes with the values)
                 if constexpr (!SCALED) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, v[q]);
@@ -494,7 +519,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 // what the scores of each 64 keys are multiplied by, and (codes) the exponent that their values were divided by: P takes it
                 float factor[2] = {row_factor, row_factor}, up[2] = {0.0f, 0.0f};
                 if constexpr (CODED) {
-                    wait(&v_full[st], ((n + i) / kStages) & 1, 2);
+                    if constexpr (!WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {    // (a masked score times 0 would be NaN)
                         factor[h] = fminf(fmaxf(factor[h] * *reinterpret_cast<volatile float *>(&k_unit[tb][h]), 1.17549435e-38f), 3.402823466e38f);
@@ -635,21 +660,106 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// Rank-3 map {D, page size, pages * heads} over the rows of a plain 16-bit cache; a box is [1][keys of one page, 128 at most][64 values] = rows of 128 bytes, 128-byte swizzled.  What is
-// outside (values from D on, a page that is none) comes as zeros.
-int page_map(CUtensorMap *m, const void *rows, const PagedView &c)
+int encode(CUtensorMap *m, const void *rows, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3])
 {
     EncodeTiledFn enc = tma_encode_fn();
     if (!enc) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t size = 1ull << c.shift;
-    const cuuint64_t dims[3] = {(cuuint64_t)c.D, size, (cuuint64_t)c.pages * c.heads};
-    const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, size * c.D * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)(size < kKeys ? size : kKeys), 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(rows), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(HIPGPT_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
     return HIPGPT_OK;
+}
+
+// Rank-3 map {D, page size, pages * heads} over the rows of a plain 16-bit cache; a box is [1][keys of one page, 128 at most][64 values] = rows of 128 bytes, 128-byte swizzled.  What is
+// outside (values from D on, a page that is none) comes as zeros.
+int page_map(CUtensorMap *m, const void *rows, const PagedView &c)
+{
+    const cuuint64_t size = 1ull << c.shift;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.D, size, (cuuint64_t)c.pages * c.heads};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, size * c.D * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(size < kKeys ? size : kKeys), 1};
+    return encode(m, rows, dims, strides, box);
+}
+
+// ... and over widened rows
+int wide_map(CUtensorMap *m, const void *rows, const Wide &wide, const PagedView &c)
+{
+    const cuuint64_t dims[3] = {(cuuint64_t)c.D, (cuuint64_t)wide.room, (cuuint64_t)c.B * c.heads};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, (cuuint64_t)wide.room * c.D * 2};
+    const cuuint32_t box[3] = {64, kKeys, 1};
+    return encode(m, rows, dims, strides, box);
+}
+
+// Codes of 64 keys of a sequence and head to fp16, as the widening warps of the kernel above do it: one read of the codes instead of one for each 256 rows of queries.  What lies behind the
+// last key or in a page that is none becomes zeros; a sequence's first 128 keys are always written (a tile without keys has one unit all the same).
+// Bound: memory (a byte read, two written for each code).
+template <int FMT>
+__global__ void __launch_bounds__(256)
+paged_widen_kernel(const PagedView c, const Wide wide)
+{
+    constexpr bool SCALED = FMT == HIPGPT_CACHE_INT8;
+    __shared__ float scale_s[2][kHalf], down_s[2];
+    dependency_wait();
+    dependents_may_start();
+    const int tid = threadIdx.x, lane = tid & 31, groups = wide.room / kHalf;
+    const int g = blockIdx.x % groups, bh = blockIdx.x / groups, b = bh / c.heads, head = bh % c.heads, p0 = g * kHalf;
+    const Sequence s = sequence_of(c, b);
+    if (s.n == 0 || p0 >= max((s.len + kKeys - 1) / kKeys, 1) * kKeys) return;
+    auto row = [&](int key) { return p0 + key < s.len ? row_of(c, b, head, p0 + key) : -1LL; };
+    if (tid < 64) {
+        const int which = tid >> 5;
+        uint32_t most = 0;
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long long at = row(lane + 32 * i);
+            f[i] = at >= 0 ? (which ? c.vs : c.ks)[at] : 0.0f;
+            const uint32_t bits = __float_as_uint(f[i]);
+            most = max(most, bits < 0x7F800000u ? bits : 0u);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        // (values: a tile of zeros must not carry the sum of exponentials out of fp32)
+        const int e = SCALED && !which ? 0 : min(max((int)(most >> 23) - 127 - kUp<FMT>, which ? -96 : -126), 120);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            scale_s[which][lane + 32 * i] = SCALED && !which ? 1.0f : f[i];
+            if (SCALED && !which) wide.scale[(size_t)bh * wide.room + p0 + lane + 32 * i] = f[i];
+        }
+        if (lane == 0) {
+            down_s[which] = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (which) wide.v_exp[(size_t)bh * groups + g] = (float)e;
+            else wide.k_unit[(size_t)bh * groups + g] = __uint_as_float((uint32_t)(127 + e) << 23);
+        }
+    }
+    __syncthreads();
+    const int chunks = c.D / 16, all = 2 * kHalf * chunks;           // of 16 codes
+    uint4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = tid + 256 * i, j = x % (all / 2), which = x / (all / 2);
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (x >= all) continue;
+        const long long at = row(j / chunks);
+        if (at >= 0) raw[i] = __ldg(reinterpret_cast<const uint4 *>((which ? c.v : c.k) + at * c.D) + j % chunks);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = tid + 256 * i, j = x % (all / 2), which = x / (all / 2);
+        if (x >= all) continue;
+        const float f = scale_s[which][j / chunks] * down_s[which];
+        const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, f2 = half2_of(f, f);
+        uint32_t out[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            codes_to_half<FMT>(in[q], out[2 * q], out[2 * q + 1]);
+            out[2 * q] = mul_f16x2(out[2 * q], f2);
+            out[2 * q + 1] = mul_f16x2(out[2 * q + 1], f2);
+        }
+        uint4 *dst = static_cast<uint4 *>(which ? wide.v : wide.k) + (((size_t)bh * wide.room + p0) * chunks + j) * 2;
+        dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+        dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    }
 }
 
 // Joins the parts of the tile that began in this block of the kernel before and went on; a thread a row and sixteen columns, parts in ascending order.
@@ -714,11 +824,21 @@ paged_tc_join_kernel(const AttnArgs a)
     }
 }
 
-template <int FMT, int DP>
+// Codes are widened before the attention, into a buffer, where the keys serve many tiles of rows and that takes at most kMostWide bytes; without the memory, in the kernel as ever.
+// 16 heads over 4 of 128 in 32768 keys, int8, before / in the kernel: 512 rows a sequence 124 / 103 us, 1024 154 / 149, 2048 217 / 252, 4096 348 / 447, 16384 1069 / 1552; e4m3: 108 / 96,
+// 132 / 136, 188 / 224, 297 / 399, 920 / 1393; four sequences of up to 4096 keys, int8: 1024 rows 90 / 79, 2048 121 / 125, 4096 174 / 201, 16384 551 / 637.
+constexpr size_t kMostWide = (size_t)1 << 30;
+constexpr long long kWideRows = 1536;
+constexpr int kNoMemory = 1;             // (no status code of the library)
+size_t wide_bytes(const PagedView &c, long long room) { return (size_t)c.B * c.heads * room * (4 * (size_t)c.D + 4) + (size_t)c.B * c.heads * (room / kHalf) * 8; }
+// rows of the table, to whole tiles of keys
+long long wide_room(const PagedView &c) { return ((((long long)c.most_pages << c.shift) + kKeys - 1) / kKeys) * kKeys; }
+
+template <int FMT, int DP, bool WIDENED>
 int launch_tc(AttnArgs a, cudaStream_t st)
 {
-    using C = TcCfg<FMT, DP>;
-    const auto kern = paged_tc_kernel<FMT, DP>;
+    using C = TcCfg<FMT, DP, WIDENED>;
+    const auto kern = paged_tc_kernel<FMT, DP, WIDENED>;
     // more than half of an SM's shared memory: one block an SM, for its TMEM
     constexpr size_t smem = C::kBytes > 120 * 1024 ? C::kBytes : 120 * 1024;
     int dev = 0, sms = 0;
@@ -735,21 +855,43 @@ int launch_tc(AttnArgs a, cudaStream_t st)
     if (tiles < (1LL << 40) / most && tiles * most < grid) grid = (int)(tiles * most);
     const bool cuts = most > 1;
     StreamWorkspace::Lease ws;
-    if (cuts) {
-        const size_t parts = (size_t)2 * grid * kRows * (DP + 2) * sizeof(float);
-        const int rc = g_paged_ws.enter(st, parts + (size_t)grid * (sizeof(int4) + sizeof(int)), &ws);
+    Wide wide = {};
+    const size_t parts = cuts ? (size_t)2 * grid * kRows * (DP + 2) * sizeof(float) : 0, lists = cuts ? ((size_t)grid * (sizeof(int4) + sizeof(int)) + 255) / 256 * 256 : 0;
+    if (cuts || WIDENED) {
+        wide.room = WIDENED ? (int)wide_room(a.c) : 0;
+        const int rc = g_paged_ws.enter(st, parts + lists + (WIDENED ? wide_bytes(a.c, wide.room) : 0), &ws);
+        if (rc != HIPGPT_OK && WIDENED) {
+            cudaGetLastError();
+            return kNoMemory;
+        }
         if (rc != HIPGPT_OK) return rc;
+    }
+    if (cuts) {
         a.parts = reinterpret_cast<float *>(ws.get());
         a.cuts = reinterpret_cast<int4 *>(ws.get() + parts);
         a.whole = reinterpret_cast<int *>(a.cuts + grid);
     }
     CUtensorMap kmap = {}, vmap = {};
-    if (FMT == HIPGPT_CACHE_PLAIN) {
+    if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
         int rc = page_map(&kmap, a.c.k, a.c);
         if (rc == HIPGPT_OK) rc = page_map(&vmap, a.c.v, a.c);
         if (rc != HIPGPT_OK) return rc;
     }
-    e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, kmap, vmap, a, take_expiry(1000));
+    if constexpr (WIDENED) {
+        const size_t lots = (size_t)a.c.B * a.c.heads, each = lots * wide.room * a.c.D * 2;
+        uint8_t *at = ws.get() + parts + lists;
+        wide.k = at;
+        wide.v = at + each;
+        wide.scale = reinterpret_cast<float *>(at + 2 * each);
+        wide.k_unit = wide.scale + lots * wide.room;
+        wide.v_exp = wide.k_unit + lots * (wide.room / kHalf);
+        int rc = wide_map(&kmap, wide.k, wide, a.c);
+        if (rc == HIPGPT_OK) rc = wide_map(&vmap, wide.v, wide, a.c);
+        if (rc != HIPGPT_OK) return rc;
+        e = launch_overlapped(paged_widen_kernel<FMT>, dim3((unsigned)(lots * (wide.room / kHalf))), dim3(256), 0, st, a.c, wide);
+        if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "paged_widen_kernel: %s", cudaGetErrorString(e));
+    }
+    e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, kmap, vmap, a, wide, take_expiry(1000));
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_tc_join_kernel<FMT, DP>, dim3((unsigned)grid, DP / 16), dim3(kRows), 0, st, a);
     return e == cudaSuccess ? check_launch("paged_tc_kernel") : fail(HIPGPT_ERR_CUDA, "paged_tc_kernel: %s", cudaGetErrorString(e));
 }
@@ -759,9 +901,16 @@ int launch_tc(AttnArgs a, cudaStream_t st)
 int launch_paged_tc(int format, const AttnArgs &a, cudaStream_t st)
 {
     const bool narrow = a.c.D <= 64;
-    if (format == HIPGPT_CACHE_PLAIN) return narrow ? launch_tc<HIPGPT_CACHE_PLAIN, 64>(a, st) : launch_tc<HIPGPT_CACHE_PLAIN, 128>(a, st);
-    if (format == HIPGPT_CACHE_E4M3) return narrow ? launch_tc<HIPGPT_CACHE_E4M3, 64>(a, st) : launch_tc<HIPGPT_CACHE_E4M3, 128>(a, st);
-    return narrow ? launch_tc<HIPGPT_CACHE_INT8, 64>(a, st) : launch_tc<HIPGPT_CACHE_INT8, 128>(a, st);
+    if (format == HIPGPT_CACHE_PLAIN) return narrow ? launch_tc<HIPGPT_CACHE_PLAIN, 64, false>(a, st) : launch_tc<HIPGPT_CACHE_PLAIN, 128, false>(a, st);
+    const long long room = wide_room(a.c);
+    const bool wide = room > 0 && (long long)a.c.T * a.group >= kWideRows * a.c.B && (long long)a.c.heads * a.c.B <= (long long)(kMostWide / 64) / room && wide_bytes(a.c, room) <= kMostWide;
+    if (wide) {
+        const int rc = format == HIPGPT_CACHE_E4M3 ? (narrow ? launch_tc<HIPGPT_CACHE_E4M3, 64, true>(a, st) : launch_tc<HIPGPT_CACHE_E4M3, 128, true>(a, st))
+                                                   : (narrow ? launch_tc<HIPGPT_CACHE_INT8, 64, true>(a, st) : launch_tc<HIPGPT_CACHE_INT8, 128, true>(a, st));
+        if (rc != kNoMemory) return rc;
+    }
+    if (format == HIPGPT_CACHE_E4M3) return narrow ? launch_tc<HIPGPT_CACHE_E4M3, 64, false>(a, st) : launch_tc<HIPGPT_CACHE_E4M3, 128, false>(a, st);
+    return narrow ? launch_tc<HIPGPT_CACHE_INT8, 64, false>(a, st) : launch_tc<HIPGPT_CACHE_INT8, 128, false>(a, st);
 }
 
 int paged_status_fetch(int *status)

@@ -347,6 +347,8 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *                              with the 63 keys beside them: scales down to 2^-21 of their largest keep all digits.
  *                              Keys are split over blocks where rows are few; buffers of the library (per device and stream, at most eight; hipgpt_release_workspace()
  *                              frees them; a captured call gets buffers of its graph) hold the parts.  The same bits run to run on the same GPU.
+ *                              bf16 with 1536 rows (tokens * H / heads) a sequence and more on average: where it takes at most 2^30 bytes, the buffer also holds the 8-bit cache's rows in
+ *                              16 bits, sequences * most_pages * page_size * heads * (4 head_dim + 4) bytes.
  */
 #define HIPGPT_CACHE_PLAIN 0
 #define HIPGPT_CACHE_E4M3  1

@@ -530,3 +530,120 @@ def test_many_short_sequences():
     serving.cache_write(cache, x, x, *batch.args)
     serving.cache_read(cache, *back, *batch.args)
     assert torch.equal(back[0], x) and torch.equal(back[1], x)
+
+
+# Sequences of many rows: 8-bit rows are widened before the attention
+WIDE = [(700, 2100), (0, 0), (900, 900), (1, 5), (1200, 1000)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("heads,H,D,page", [(1, 4, 128, 16), (2, 8, 64, 1024), (1, 8, 48, 128), (2, 8, 80, 64), (1, 3, 16, 32)])
+def test_codes_widened_before(fmt, heads, H, D, page):
+    batch = Batch(WIDE, page, seed=D, before=1, behind=2)
+    assert batch.T * (H // heads) >= 1536 * batch.B
+    for causal in (True, False):
+        _, _, out, want, bound, mine = _attend(batch, heads, H, D, BF16, fmt, causal=causal)
+        within(out[mine], want[mine], bound[mine], f"causal={causal}")
+        assert bool(torch.isnan(out[~mine]).all())
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_codes_widened_before_of_any_magnitude(fmt):
+    batch = Batch([(1000, 1300), (700, 800)], 64, seed=13)
+
+    def wild(name, x):
+        if name == "k":
+            x *= 2.0 ** -30
+        else:
+            for page in range(len(x)):
+                x[page] *= (0.0, 2.0 ** -20, 1.0, 2.0 ** 10)[page % 4]
+    _, _, out, want, bound, _ = _attend(batch, 2, 8, 64, BF16, fmt, wild=wild, spread=2.0 ** 31)
+    within(out, want, bound)
+
+    def tiny(name, x):
+        x *= 2.0 ** -100
+    _, _, out, want, bound, _ = _attend(batch, 2, 8, 64, BF16, fmt, wild=tiny, spread=2.0 ** -100)
+    within(out, want, bound)
+
+    def zeros(name, x):
+        if name == "v":
+            x.zero_()
+    _, _, out, want, bound, _ = _attend(batch, 2, 8, 64, BF16, fmt, wild=zeros)
+    assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_codes_widened_before_what_is_not_seen_and_no_pages(fmt):
+    batch = Batch([(700, 900), (1000, 1200)], 16, seed=3)
+    heads, H, D = 2, 8, 32
+    p = 1200 - 2
+    page, slot = int(batch.table[-1, p // 16]), p % 16
+
+    def wild(name, x):
+        x[page, 1, slot, 3] = float("nan") if name == "k" else float("inf")
+    _, _, out, want, bound, _ = _attend(batch, heads, H, D, BF16, fmt, wild=wild)
+    clean = torch.ones(batch.T, H, dtype=torch.bool, device="cuda")
+    clean[700 + 1000 - 2:, H // heads:] = False
+    within(out[clean], want[clean], bound[clean], "rows that do not see it")
+    assert not bool(torch.isfinite(out[~clean]).all(-1).any()), "rows that do"
+    batch.table[0, 3], batch.table[0, 55], batch.table[1, 10:40] = 1 << 30, -7, batch.num_pages
+    batch.pages.copy_(batch.table)
+    _, _, out, want, bound, mine = _attend(batch, heads, H, D, BF16, fmt)
+    within(out, want, bound, "pages that are none")
+    q, out = _normal(_gen(2), batch.T, H, D, dtype=BF16), torch.zeros(batch.T, H, D, device="cuda", dtype=BF16)
+    cache = su.filled_cache(batch, heads, D, BF16, fmt)[0]
+    for offsets, lengths in (([-3, 1500, 1 << 30], [1 << 30, -5]), ([0, 1700, 400], [(1 << 31) - 1, 0]), ([900, 100, 1600], [7, 1200])):
+        serving.paged_attention(cache, q, out, torch.tensor(offsets, dtype=torch.int32).cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), batch.pages, batch.T, batch.B, H)
+        torch.cuda.synchronize()
+        assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_codes_widened_before_in_graphs_on_streams_and_every_time(fmt):
+    batch = Batch([(900, 5000), (900, 901)], 64, seed=6)
+    cache, q, out, want, bound, _ = _attend(batch, 2, 8, 128, BF16, fmt)
+    within(out, want, bound)
+    graphs = [(torch.cuda.CUDAGraph(), torch.empty_like(out)) for _ in range(2)]
+    for graph, got in graphs:
+        with torch.cuda.graph(graph):
+            serving.paged_attention(cache, q, got, *batch.args, 8)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.zeros_like(out) for _ in range(30)]
+    torch.cuda.synchronize()
+    for i, got in enumerate(outs):
+        with torch.cuda.stream(streams[i % 3]):
+            serving.paged_attention(cache, q, got, *batch.args, 8)
+    for graph, _ in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in outs + [got for _, got in graphs]:
+        assert torch.equal(got, out)
+    batch.seqs = [(900, 3000), (900, 950)]                           # a replay sees what the lengths hold then
+    batch.lengths.copy_(torch.tensor([3000, 950], dtype=torch.int32))
+    serving.paged_attention(cache, q, out, *batch.args, 8)
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    seen_nan = torch.isnan(out)                                      # (the second sequence's keys from 901 on were never written)
+    assert torch.equal(torch.isnan(graphs[0][1]), seen_nan) and torch.equal(graphs[0][1].nan_to_num(), out.nan_to_num())
+    assert not bool(seen_nan[:900].any()) and bool(seen_nan[-1].all())
+
+
+@pytest.mark.parametrize("code,block", [(1001, 0), (1002, 3), (1003, 1), (1004, 2), (1005, 0), (1006, 5), (1007, 4), (1008, 1), (1009, 6)])
+def test_codes_widened_before_an_expired_wait(code, block):
+    batch = Batch([(900, 5000), (900, 901)], 64, seed=6)
+    cache, q, out, want, bound, _ = _attend(batch, 2, 8, 128, BF16, "int8")
+    within(out, want, bound)
+    for _ in range(20):
+        got = torch.full_like(out, -7.0)
+        _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
+        serving.paged_attention(cache, q, got, *batch.args, 8)
+        torch.cuda.synchronize()
+        status = _status()
+        if status:
+            break
+    assert status == code and _status() == 0
+    same, left = (got == out).all(-1), (got == -7.0).all(-1)
+    assert bool((same | left).all()) and bool(left.any()) and bool(same.any())
+    serving.paged_attention(cache, q, got, *batch.args, 8)
+    assert torch.equal(got, out)
