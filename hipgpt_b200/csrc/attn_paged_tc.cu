@@ -693,7 +693,7 @@ int wide_map(CUtensorMap *m, const void *rows, const Wide &wide, const PagedView
 
 // Codes of 64 keys of a sequence and head to fp16, as the widening warps of the kernel above do it: one read of the codes instead of one for each 256 rows of queries.  What lies behind the
 // last key or in a page that is none becomes zeros; a sequence's first 128 keys are always written (a tile without keys has one unit all the same).
-// Bound: memory (a byte read, two written for each code).
+// Bound: memory (a byte read, two written for each code), and the chain page -> row before it: 32768 keys of 8 heads of 128, K and V: 55 us, 3.7 TB/s.
 template <int FMT>
 __global__ void __launch_bounds__(256)
 paged_widen_kernel(const PagedView c, const Wide wide)
