@@ -76,22 +76,23 @@ __device__ __forceinline__ void read_words(uint32_t *w, const uint8_t *p)
 __host__ __device__ constexpr int least_of(int a, int b) { return a < b ? a : b; }
 __host__ __device__ constexpr int most_of(int a, int b) { return a > b ? a : b; }
 
-template <typename T, int FMT, int DP, bool SPLITROWS>
+// CUT: K and V come as pieces that were cut before the kernel
+template <typename T, int FMT, int DP, bool SPLITROWS, bool CUT_ = false>
 struct Shape {
-    static constexpr bool F32 = sizeof(T) == 4, CODED = FMT != HIPGPT_CACHE_PLAIN;
+    static constexpr bool F32 = sizeof(T) == 4, CODED = FMT != HIPGPT_CACHE_PLAIN, CUT = CUT_;
     static constexpr int EB = CODED ? 1 : (int)sizeof(T);               // bytes of an element of the cache
     static constexpr int NQ = !F32 ? 1 : CODED ? 2 : 3, NK = F32 && !CODED ? 3 : 1;  // pieces of Q and P, of K and V
     static constexpr int MT = 1;                                        // tiles of 16 rows a warp
     static constexpr int ROWS = 16 * MT * (SPLITROWS ? kWarps : 1);
     static constexpr int KB = 4096 / (DP * EB) >= 32 ? 32 : 16;         // keys a warp takes at a time
-    static constexpr int UNIT = SPLITROWS ? 64 : kWarps * KB;           // keys of a place in the ring
+    static constexpr int UNIT = CUT && DP > 32 ? 32 : SPLITROWS ? 64 : kWarps * KB;      // keys of a place in the ring
     static constexpr int EC = least_of(16 / EB, DP / 4), NC = DP / 4 / EC;       // K: elements of a chunk, chunks a thread
     static constexpr int EV = least_of(16 / EB, DP / 8), NV = DP / 8 / EV;       // V: the same
     static constexpr int STEPS = DP / 16, TILES = DP / 8;
     static constexpr int kQBytes = NQ * (ROWS / 16) * STEPS * 32 * 16;
     static constexpr int kPad = DP + 4;
     static constexpr int kOBytes = SPLITROWS ? 0 : 2 * 16 * kPad * 4;   // two warps' results
-    static constexpr int kSlotBytes = UNIT * DP * EB + (CODED ? UNIT * 4 : 0);
+    static constexpr int kSlotBytes = UNIT * DP * (CUT ? 6 : EB) + (CODED ? UNIT * 4 : 0);
     static constexpr int kFixed = kQBytes + kOBytes + 1024;
     // places of the ring: four at least
     static constexpr int kBudget = (DP == 128 ? 112 : 74) * 1024;       // two or three blocks an SM
@@ -122,8 +123,12 @@ __device__ __forceinline__ void bring(const AttnArgs &a, Run<C::ROWS, C::UNIT, T
             const int count = page >= 0 ? min(run_keys, keys - p) : 0, scales = C::CODED ? (count + 3) & ~3 : 0;         // (whole 16 bytes of scales)
             const long long row = ((((long long)page * a.c.heads) + w.head) << a.c.shift) + (p & (page_keys - 1));
             int bytes = count * D * C::EB + scales * 4;
+            if constexpr (C::CUT) {
+                bytes = C::kSlotBytes;
+            } else {
 #pragma unroll
-            for (int o = 16; o; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
+                for (int o = 16; o; o >>= 1) bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
+            }
             // one bit for each sixteen keys
             const uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
             uint32_t there = 0;
@@ -140,7 +145,10 @@ __device__ __forceinline__ void bring(const AttnArgs &a, Run<C::ROWS, C::UNIT, T
                     mbar_arrive_expect_tx(&full[sl], (uint32_t)bytes);
                 }
                 __syncwarp();
-                if (count > 0 && alive) {
+                if constexpr (C::CUT) {
+                    const long long place = ((long long)w.b * a.c.heads + w.head) * a.cut_units + u;
+                    if (lane == 0 && alive) bulk_load(ring + sl * C::kSlotBytes, (which ? a.cut_v : a.cut_k) + place * C::kSlotBytes, C::kSlotBytes, &full[sl]);
+                } else if (count > 0 && alive) {
                     uint8_t *dst = ring + sl * C::kSlotBytes;
                     bulk_load(dst + lane * run_keys * D * C::EB, (which ? a.c.v : a.c.k) + row * D * C::EB, (uint32_t)(count * D * C::EB), &full[sl]);
                     if constexpr (C::CODED) bulk_load(dst + C::UNIT * C::STEPS * 16 + lane * run_keys * 4, (which ? a.c.vs : a.c.ks) + row, (uint32_t)(scales * 4), &full[sl]);
@@ -150,11 +158,11 @@ __device__ __forceinline__ void bring(const AttnArgs &a, Run<C::ROWS, C::UNIT, T
     }
 }
 
-template <typename T, int FMT, int DP, bool SPLITROWS>
-__global__ void __launch_bounds__(kThreads, Shape<T, FMT, DP, SPLITROWS>::kBlocks)
+template <typename T, int FMT, int DP, bool SPLITROWS, bool CUT = false>
+__global__ void __launch_bounds__(kThreads, Shape<T, FMT, DP, SPLITROWS, CUT>::kBlocks)
 paged_rows_kernel(const AttnArgs a)
 {
-    using C = Shape<T, FMT, DP, SPLITROWS>;
+    using C = Shape<T, FMT, DP, SPLITROWS, CUT>;
     constexpr bool HALF = C::CODED;
     constexpr int SLOTS = C::kSlots;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -324,7 +332,8 @@ paged_rows_kernel(const AttnArgs a)
                 for (int i = 0; i < C::NC; ++i) {
                     uint32_t kw[NJ][C::EC * C::EB / 4];
                     const int d = (t4 + 4 * i) * C::EC;
-                    if (D == DP) {
+                    if constexpr (CUT) {
+                    } else if (D == DP) {
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) read_words<C::EC * C::EB>(kw[j], k_at + (k0 + 8 * j + g) * (DP * C::EB) + d * C::EB);
                     } else {
@@ -345,7 +354,10 @@ paged_rows_kernel(const AttnArgs a)
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) {
                             uint32_t b[C::NK][2];
-                            if constexpr (C::CODED) {
+                            if constexpr (CUT) {
+#pragma unroll
+                                for (int n = 0; n < 3; ++n) read_words<8>(b[n], k_at + (((k0 / 8 + j) * C::NC + i) * 3 + n) * 256 + lane * 8);
+                            } else if constexpr (C::CODED) {
                                 codes_to_half<FMT>(kw[j][x], b[0][0], b[0][1]);
                             } else if constexpr (!C::F32) {
                                 b[0][0] = kw[j][2 * x];
@@ -490,7 +502,8 @@ paged_rows_kernel(const AttnArgs a)
                 for (int c = 0; c < C::NV; ++c) {
                     const int d = (g + 8 * c) * C::EV;
                     uint32_t vw[NG][4][C::EV * C::EB / 4];
-                    if (D == DP && !partial) {
+                    if constexpr (CUT) {
+                    } else if (D == DP && !partial) {
 #pragma unroll
                         for (int x = 0; x < 4 * NG; ++x) read_words<C::EV * C::EB>(vw[x / 4][x % 4], v_at + (k0 + 8 * (x >> 1) + 2 * t4 + (x & 1)) * (DP * C::EB) + d * C::EB);
                     } else {
@@ -508,21 +521,27 @@ paged_rows_kernel(const AttnArgs a)
                     for (int e = 0; e < C::EV; e += W) {
                         uint32_t b[NG][W][C::NK][2];
 #pragma unroll
-                        for (int i = 0; i < NG; ++i)
+                        for (int i = 0; i < NG; ++i) {
+                            if constexpr (CUT) {
 #pragma unroll
-                            for (int hf = 0; hf < 2; ++hf) {
-                                const uint32_t *w0 = vw[i][2 * hf], *w1 = vw[i][2 * hf + 1];
-                                if constexpr (C::CODED) {
-                                    codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x5140), b[i][0][0][hf], b[i][1][0][hf]);
-                                    codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x7362), b[i][2][0][hf], b[i][3][0][hf]);
-                                } else if constexpr (!C::F32) {
-                                    b[i][0][0][hf] = __byte_perm(w0[e / 2], w1[e / 2], e & 1 ? 0x7632 : 0x5410);
-                                } else {
-                                    float x = __uint_as_float(w0[e]), y = __uint_as_float(w1[e]);
+                                for (int n = 0; n < 3; ++n) read_words<8>(b[i][0][n], v_at + (((k0 / 16 + i) * C::TILES + c * C::EV + e) * 3 + n) * 256 + lane * 8);
+                            } else {
 #pragma unroll
-                                    for (int n = 0; n < 3; ++n) b[i][0][n][hf] = next_piece<false>(x, y);
+                                for (int hf = 0; hf < 2; ++hf) {
+                                    const uint32_t *w0 = vw[i][2 * hf], *w1 = vw[i][2 * hf + 1];
+                                    if constexpr (C::CODED) {
+                                        codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x5140), b[i][0][0][hf], b[i][1][0][hf]);
+                                        codes_to_half<FMT>(__byte_perm(w0[e / 4], w1[e / 4], 0x7362), b[i][2][0][hf], b[i][3][0][hf]);
+                                    } else if constexpr (!C::F32) {
+                                        b[i][0][0][hf] = __byte_perm(w0[e / 2], w1[e / 2], e & 1 ? 0x7632 : 0x5410);
+                                    } else {
+                                        float x = __uint_as_float(w0[e]), y = __uint_as_float(w1[e]);
+#pragma unroll
+                                        for (int n = 0; n < 3; ++n) b[i][0][n][hf] = next_piece<false>(x, y);
+                                    }
                                 }
                             }
+                        }
 #pragma unroll
                         for (int x = 0; x < W; ++x)
 #pragma unroll
@@ -684,7 +703,7 @@ paged_rows_kernel(const AttnArgs a)
                         while (some) {
                             const int who = (__ffs((int)some) - 1) >> 2;         // its row in the tile's eight
                             some &= ~(0xFu << (4 * who));
-                            mend_row<T, FMT>(a, w.b, w.head, s, row0 + (warp * C::MT + mt) * 16 + who + 8 * r, keys);
+                            mend_row<T, FMT>(a, w.b, w.head, s, row0 + (warp * C::MT + mt) * 16 + who + 8 * r, keys_met(a, s, keys));
                         }
                     }
             }
@@ -704,7 +723,7 @@ paged_rows_kernel(const AttnArgs a)
 template <typename T, int FMT, int DP>
 struct TokenShape {
     using R = Shape<T, FMT, DP, false>;
-    static constexpr bool F32 = R::F32, CODED = R::CODED;
+    static constexpr bool F32 = R::F32, CODED = R::CODED, CUT = false;
     static constexpr int EB = R::EB, NQ = R::NQ, NK = R::NK, ROWS = 8, KB = R::KB, UNIT = kWarps * KB;
     static constexpr int EC = R::EC, NC = R::NC, EV = R::EV, NV = R::NV, STEPS = DP / 16, TILES = DP / 16;
     static constexpr int kQBytes = NQ * STEPS * 32 * 8, kPad = DP + 4, kOBytes = kWarps * 8 * kPad * 4;
@@ -1149,6 +1168,62 @@ paged_token_kernel(const AttnArgs a)
     }
 }
 
+// The keys and values of UNIT positions of a sequence and head, fp32, as the three bf16 pieces of each, in the order of the operands of paged_rows_kernel's lanes (a place of its ring), so that they are cut
+// once and not by each of its warps.  What lies behind the last key or in a page that is none becomes zeros; a sequence's first unit is always written.  Bound: memory (four bytes read, six written a value).
+template <typename C>
+__global__ void __launch_bounds__(128)
+paged_cut_kernel(const PagedView c, uint8_t *k_out, uint8_t *v_out, int units)
+{
+    __shared__ long long rows_s[C::UNIT];
+    dependency_wait();
+    dependents_may_start();
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3, warp = tid >> 5, D = c.D;
+    const int u = blockIdx.x % units, bh = blockIdx.x / units, b = bh / c.heads, head = bh % c.heads, p0 = u * C::UNIT;
+    const Sequence s = sequence_of(c, b);
+    if (s.n == 0 || (u > 0 && p0 >= s.len)) return;
+    if (tid < C::UNIT) rows_s[tid] = p0 + tid < s.len ? row_of(c, b, head, p0 + tid) : -1;
+    __syncthreads();
+    auto read = [&](const uint8_t *from, int key, int d) {
+        const long long at = rows_s[key];
+        return at >= 0 && d < D ? __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(from) + at * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    uint8_t *const k_to = k_out + (size_t)blockIdx.x * C::kSlotBytes + lane * 8, *const v_to = v_out + (size_t)blockIdx.x * C::kSlotBytes + lane * 8;
+#pragma unroll 4
+    for (int x = warp; x < C::UNIT / 8 * C::NC; x += 4) {
+        const int j = x / C::NC, i = x % C::NC;
+        float4 y = read(c.k, 8 * j + g, (t4 + 4 * i) * 4);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            const uint32_t lo = next_piece<false>(y.x, y.y), hi = next_piece<false>(y.z, y.w);
+            *reinterpret_cast<uint2 *>(k_to + (x * 3 + n) * 256) = make_uint2(lo, hi);
+        }
+    }
+#pragma unroll 2
+    for (int x = warp; x < C::UNIT / 16 * C::NV; x += 4) {
+        const int i = x / C::NV, cc = x % C::NV;
+        float y[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 f = read(c.v, 16 * i + 8 * (q >> 1) + 2 * t4 + (q & 1), (g + 8 * cc) * 4);
+            y[q][0] = f.x; y[q][1] = f.y; y[q][2] = f.z; y[q][3] = f.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const uint32_t lo = next_piece<false>(y[0][e], y[1][e]), hi = next_piece<false>(y[2][e], y[3][e]);
+                *reinterpret_cast<uint2 *>(v_to + ((i * C::TILES + cc * 4 + e) * 3 + n) * 256) = make_uint2(lo, hi);
+            }
+    }
+}
+
+// fp32 keys and values are cut before the attention, into a buffer, where they serve several tiles of rows and that takes at most kMostCut bytes; without the memory, by the warps as ever.
+// 16 heads over 8, before / by the warps, us: of 32, a sequence of 8192 keys, 64 rows 53 / 52, 128 57 / 59, 512 111 / 132, 2048 314 / 417, 32 sequences up to 512, 82 rows 65 / 63, 163 87 / 91, 327 127 / 149;
+// of 64, 8192 keys, 128 rows 92 / 83, 256 123 / 135, 2048 572 / 849; of 128, 8192 keys, 32 rows 101 / 60, 64 114 / 117, 128 152 / 190, 2048 1336 / 2410.
+constexpr size_t kMostCut = (size_t)1 << 30;
+constexpr long long cut_rows(int width) { return width <= 32 ? 112 : width <= 64 ? 160 : 64; }
+constexpr int kNoMemory = 1;                     // (no status code of the library)
+
 template <typename T, int FMT, int DP, typename C>
 int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
 {
@@ -1173,13 +1248,33 @@ int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
     if (tiles < (1LL << 40) / most && tiles * most < grid) grid = (int)(tiles * most);
     const bool cuts = most > 1;
     StreamWorkspace::Lease ws;
-    if (cuts) {
-        const size_t parts = (size_t)2 * grid * C::ROWS * (DP + 2) * sizeof(float);
-        const int rc = g_paged_ws.enter(st, parts + (size_t)grid * (sizeof(int4) + sizeof(int)), &ws);
+    const size_t parts = cuts ? (size_t)2 * grid * C::ROWS * (DP + 2) * sizeof(float) : 0, lists = cuts ? ((size_t)grid * (sizeof(int4) + sizeof(int)) + 255) / 256 * 256 : 0;
+    size_t pieces = 0;                           // bytes of K, and of V
+    if constexpr (C::CUT) {
+        const long long lots = (long long)a.c.B * a.c.heads;
+        if (a.c.pages == 0 || a.c.most_pages == 0 || lots > (long long)(kMostCut / (2 * C::kSlotBytes)) / most) return kNoMemory;
+        pieces = (size_t)lots * most * C::kSlotBytes;
+    }
+    if (cuts || pieces) {
+        const int rc = g_paged_ws.enter(st, parts + lists + 2 * pieces, &ws);
+        if (rc != HIPGPT_OK && pieces) {
+            cudaGetLastError();
+            return kNoMemory;
+        }
         if (rc != HIPGPT_OK) return rc;
+    }
+    if (cuts) {
         a.parts = reinterpret_cast<float *>(ws.get());
         a.cuts = reinterpret_cast<int4 *>(ws.get() + parts);
         a.whole = reinterpret_cast<int *>(a.cuts + grid);
+    }
+    if constexpr (C::CUT) {
+        a.cut_unit = C::UNIT;
+        a.cut_k = ws.get() + parts + lists;
+        a.cut_v = a.cut_k + pieces;
+        a.cut_units = (int)most;
+        e = launch_overlapped(paged_cut_kernel<C>, dim3((unsigned)(pieces / C::kSlotBytes)), dim3(128), 0, st, a.c, a.cut_k, a.cut_v, a.cut_units);
+        if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "paged_cut_kernel: %s", cudaGetErrorString(e));
     }
     e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), C::kSmem, st, a);
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<T, FMT, C::ROWS, DP>, dim3((unsigned)grid, (unsigned)(C::ROWS + 15) / 16), dim3(256), 0, st, a);
@@ -1192,6 +1287,11 @@ template <typename T, int FMT, int DP>
 int launch_width(int rows, const AttnArgs &a, cudaStream_t st)
 {
     if (rows == kTokens) return launch_kernel<T, FMT, DP, TokenShape<T, FMT, DP>>(paged_token_kernel<T, FMT, DP>, a, st);
+    if constexpr (sizeof(T) == 4 && FMT == HIPGPT_CACHE_PLAIN)
+        if ((long long)a.c.T * a.group >= cut_rows(DP) * a.c.B) {
+            const int rc = launch_kernel<T, FMT, DP, Shape<T, FMT, DP, true, true>>(paged_rows_kernel<T, FMT, DP, true, true>, a, st);
+            if (rc != kNoMemory) return rc;
+        }
     if constexpr (sizeof(T) == 4)
         if (rows == kMany) return launch_kernel<T, FMT, DP, Shape<T, FMT, DP, true>>(paged_rows_kernel<T, FMT, DP, true>, a, st);
     return launch_kernel<T, FMT, DP, Shape<T, FMT, DP, false>>(paged_rows_kernel<T, FMT, DP, false>, a, st);

@@ -22,6 +22,8 @@ struct AttnArgs {
     float *parts;                        // [2 * blocks][ROWS][DP + 2]: sums, then reference maximum (log2 domain) and sum of exponentials of each row
     int4 *cuts;                          // [blocks]: the tile that begins here and goes on: sequence, head, tile, last block (w < 0: none)
     int *whole;                          // [blocks]: 0 where a wait ran out
+    uint8_t *cut_k, *cut_v;              // [sequence][head][cut_units] places of the ring: fp32 cut into pieces before the attention
+    int cut_units, cut_unit;             // keys a place (0: keys as they lie in the cache)
 };
 
 // One tile's run of units in a block
@@ -275,6 +277,9 @@ __device__ __forceinline__ void mend_row(const AttnArgs &a, int b, int head, con
     if (limit < keys && any_wild<T, FMT>(a, b, head, limit, keys)) row_again<T, FMT>(a, b, head, s, row, c0, c1);
 }
 
+// The keys that a tile's rows have been multiplied with: those they see, and where these were cut before, to the end of the last place
+__device__ __forceinline__ int keys_met(const AttnArgs &a, const Sequence &s, int keys) { return a.cut_unit ? (int)min((long long)s.len, ((long long)keys + a.cut_unit - 1) / a.cut_unit * a.cut_unit) : keys; }
+
 // ---- joining the parts ----------------------------------------------------------------------------------------------------
 // One block a block of the kernel before it: the tile that began there, if it went on.  A warp takes a row; parts in ascending order.
 template <typename T, int FMT, int ROWS, int DP>
@@ -318,7 +323,7 @@ paged_join_kernel(const AttnArgs a)
         }
         if (__any_sync(0xffffffffu, wild)) {
             __syncwarp();
-            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)row, tile_keys<ROWS>(a, s, cut.z));
+            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)row, keys_met(a, s, tile_keys<ROWS>(a, s, cut.z)));
         }
     }
 }

@@ -348,7 +348,8 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *                              Keys are split over blocks where rows are few; buffers of the library (per device and stream, at most eight; hipgpt_release_workspace()
  *                              frees them; a captured call gets buffers of its graph) hold the parts.  The same bits run to run on the same GPU.
  *                              bf16 with 1536 rows (tokens * H / heads) a sequence and more on average: where it takes at most 2^30 bytes, the buffer also holds the 8-bit cache's rows in
- *                              16 bits, sequences * most_pages * page_size * heads * (4 head_dim + 4) bytes.
+ *                              16 bits, sequences * most_pages * page_size * heads * (4 head_dim + 4) bytes; fp32 over a plain cache with 160 rows and more (64 from head_dim 65 on): the keys and values as their
+ *                              pieces, three times the bytes of the sequences' keys and values in 16 bits, head_dim counted as 32, 64 or 128.
  */
 #define HIPGPT_CACHE_PLAIN 0
 #define HIPGPT_CACHE_E4M3  1

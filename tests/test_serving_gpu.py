@@ -647,3 +647,66 @@ def test_codes_widened_before_an_expired_wait(code, block):
     assert bool((same | left).all()) and bool(left.any()) and bool(same.any())
     serving.paged_attention(cache, q, got, *batch.args, 8)
     assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("heads,H,D,page", [(1, 4, 128, 16), (2, 4, 64, 1024), (1, 3, 48, 128), (2, 2, 80, 64), (2, 4, 16, 32), (3, 3, 32, 16)])
+def test_pieces_cut_before(heads, H, D, page):
+    """fp32 rows enough that keys and values are cut into pieces once: sequences that end inside a place, see nothing, have no rows or one."""
+    batch = Batch([(300, 700), (0, 0), (500, 500), (1, 5), (400, 333), (97, 1025)], page, seed=D, before=1, behind=2)
+    for causal in (True, False):
+        _, _, out, want, bound, mine = _attend(batch, heads, H, D, F32, "plain", causal=causal)
+        within(out[mine], want[mine], bound[mine], f"causal={causal}")
+        assert bool(torch.isnan(out[~mine]).all())
+    assert _status() == 0
+
+
+def test_pieces_cut_before_what_is_not_seen_and_no_pages():
+    batch = Batch([(200, 900), (330, 1200)], 16, seed=3)
+    heads, H, D = 2, 4, 32
+    for p in (1200 - 2, 1200 - 200, 1199):                           # in the places of tiles that do not see them, too
+        page, slot = int(batch.table[-1, p // 16]), p % 16
+
+        def wild(name, x):
+            x[page, 1, slot, 3] = float("nan") if name == "k" else float("inf")
+        _, _, out, want, bound, _ = _attend(batch, heads, H, D, F32, "plain", wild=wild)
+        clean = torch.ones(batch.T, H, dtype=torch.bool, device="cuda")
+        clean[200 + 330 - (1200 - p):, H // heads:] = False
+        within(out[clean], want[clean], bound[clean], "rows that do not see it")
+        assert not bool(torch.isfinite(out[~clean]).all(-1).any()), "rows that do"
+    batch.table[0, 3], batch.table[0, 55], batch.table[1, 10:40] = 1 << 30, -7, batch.num_pages
+    batch.pages.copy_(batch.table)
+    _, _, out, want, bound, mine = _attend(batch, heads, H, D, F32, "plain")
+    within(out, want, bound, "pages that are none")
+    q, out = _normal(_gen(2), batch.T, H, D), torch.zeros(batch.T, H, D, device="cuda")
+    cache = su.filled_cache(batch, heads, D, F32, "plain")[0]
+    for offsets, lengths in (([-3, 400, 1 << 30], [1 << 30, -5]), ([0, 500, 100], [(1 << 31) - 1, 0]), ([300, 100, 530], [7, 1200])):
+        serving.paged_attention(cache, q, out, torch.tensor(offsets, dtype=torch.int32).cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), batch.pages, batch.T, batch.B, H)
+        torch.cuda.synchronize()
+        assert _status() == 0
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_pieces_cut_before_in_graphs_on_streams_and_every_time(D):
+    batch = Batch([(300, 3000), (200, 901)], 64, seed=6)
+    cache, q, out, want, bound, _ = _attend(batch, 2, 4, D, F32, "plain")
+    within(out, want, bound)
+    graphs = [(torch.cuda.CUDAGraph(), torch.empty_like(out)) for _ in range(2)]
+    for graph, got in graphs:
+        with torch.cuda.graph(graph):
+            serving.paged_attention(cache, q, got, *batch.args, 4)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.zeros_like(out) for _ in range(30)]
+    torch.cuda.synchronize()
+    for i, got in enumerate(outs):
+        with torch.cuda.stream(streams[i % 3]):
+            serving.paged_attention(cache, q, got, *batch.args, 4)
+    for graph, _ in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in outs + [got for _, got in graphs]:
+        assert torch.equal(got, out)
+    batch.lengths.copy_(torch.tensor([2000, 900], dtype=torch.int32))
+    serving.paged_attention(cache, q, out, *batch.args, 4)
+    graphs[1][0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[1][1], out)
