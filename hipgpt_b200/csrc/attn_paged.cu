@@ -45,10 +45,9 @@ __device__ __forceinline__ uint32_t next_piece(float &lo, float &hi)
 {
     if constexpr (HALF) {
         const uint32_t w = half2_of(lo, hi);
-        float a, b;
-        asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;}" : "=f"(a), "=f"(b) : "r"(w));
-        lo -= a;
-        hi -= b;
+        const float2 f = floats_of(w);
+        lo -= f.x;
+        hi -= f.y;
         return w;
     } else {
         const uint32_t w = pack_bf16(lo, hi);

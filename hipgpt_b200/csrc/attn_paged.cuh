@@ -210,8 +210,13 @@ struct Run {
 template <typename T, int FMT>
 __device__ __forceinline__ float cached(const uint8_t *base, const float *scale, long long row, int D, int d)
 {
-    if constexpr (FMT == HIPGPT_CACHE_PLAIN) return to_float(reinterpret_cast<const T *>(base)[row * D + d]);
-    else return __uint_as_float(code_pair<FMT>(base[row * D + d], 0u, 0, 0) << 16) * scale[row];
+    if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
+        return to_float(reinterpret_cast<const T *>(base)[row * D + d]);
+    } else {
+        uint32_t lo, hi;
+        codes_to_half<FMT>(base[row * D + d], lo, hi);
+        return floats_of(lo).x * scale[row];
+    }
 }
 
 template <typename T, int FMT>

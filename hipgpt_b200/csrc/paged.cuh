@@ -35,25 +35,16 @@ __device__ __forceinline__ long long row_of(const PagedView &c, int b, int head,
     return ((((long long)page * c.heads) + head) << c.shift) + (p & ((1 << c.shift) - 1));
 }
 
-// ---- 8-bit codes: four of one word as the bf16 values that they are (exact), in two words ----
-// `x` holds two codes in the upper bytes (e4m3) or lower bytes (int8) of its halves; the other bytes may hold anything.
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-// sign, 4 bits of exponent and 3 of mantissa at bf16's place stand for 2^-120 of the value, subnormals included
-__device__ __forceinline__ uint32_t e4m3_to_bf16x2(uint32_t x) { return mul_bf16x2((x & 0x80008000u) | ((x >> 4) & 0x07F007F0u), 0x7B807B80u); }
-// 0x43uu with seven bits u is 128 + u; 0x4300 is 128 and 0x4380 is 256: the low bits less what the sign bit says
-__device__ __forceinline__ uint32_t int8_to_bf16x2(uint32_t x) { return sub_bf16x2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) | 0x43004300u); }
-template <int FMT>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w0, uint32_t w1, int byte0, int byte1)      // byte0 of w0 in the low half, byte1 of w1 in the high one
-{
-    if constexpr (FMT == HIPGPT_CACHE_E4M3) return e4m3_to_bf16x2(__byte_perm(w0, w1, (byte0 << 4) | ((4 + byte1) << 12)));
-    else return int8_to_bf16x2(__byte_perm(w0, w1, byte0 | ((4 + byte1) << 8)));
-}
-
-// ... and as fp16, for products
+// ---- 8-bit codes as fp16 (exact; NaN codes of e4m3 are NaN, in attention and when read back) ----
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+__device__ __forceinline__ float2 floats_of(uint32_t half2)
+{
+    float2 f;
+    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;}" : "=f"(f.x), "=f"(f.y) : "r"(half2));
+    return f;
+}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-// Four codes as fp16 (exact), in two words
+// Four codes of a word, in two words
 template <int FMT>
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi)
 {

@@ -250,10 +250,14 @@ cache_read_kernel(const MoveArgs a)
                 if (d >= D) continue;
                 if constexpr (FMT != HIPGPT_CACHE_PLAIN)
 #pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        const uint32_t two = code_pair<FMT>(word[w][c][e / 2], word[w][c][e / 2], (e & 1) * 2, (e & 1) * 2 + 1);
-                        x[w][c][2 * e] = __uint_as_float(two << 16) * s[w];
-                        x[w][c][2 * e + 1] = __uint_as_float(two & 0xFFFF0000u) * s[w];
+                    for (int e = 0; e < N / 4; ++e) {
+                        uint32_t lo, hi;
+                        codes_to_half<FMT>(word[w][c][e], lo, hi);
+                        const float2 a = floats_of(lo), b = floats_of(hi);
+                        x[w][c][4 * e] = a.x * s[w];
+                        x[w][c][4 * e + 1] = a.y * s[w];
+                        x[w][c][4 * e + 2] = b.x * s[w];
+                        x[w][c][4 * e + 3] = b.y * s[w];
                     }
                 if constexpr (W > 1) store_values<T, W>(dst + d, x[w][c]);
                 else

@@ -1,0 +1,72 @@
+"""Attention over a cache in pages and the cache's calls at the edges of their ranges (forms and bounds of tests/serving_util.py)."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from hipgpt_b200 import _capi, serving  # noqa: E402
+from tests import serving_util as su  # noqa: E402
+from tests.serving_util import BF16, F32, Batch, within  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _normal(gen, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def _status():
+    st = C.c_int(-1)
+    _capi.check(_capi.lib().hipgpt_kernel_status(C.byref(st)))
+    return st.value
+
+
+# ---- NaN codes --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_every_code_read_back(dtype):
+    """A cache filled elsewhere: each of the 256 codes stands for the same value as torch's type, NaN among them."""
+    for fmt, codes in su.CODES.items():
+        heads, D, page = 2, 128, 16
+        cache = serving.PagedCache(2, page, heads, D, dtype=dtype, format=fmt)
+        raw = torch.arange(256, dtype=torch.uint8, device="cuda").repeat(2 * heads * page * D // 256).view(2, heads, page, D)
+        cache.k.view(torch.uint8).copy_(raw)
+        cache.v.view(torch.uint8).copy_(raw.flip(-1))
+        cache.k_scale.fill_(0.5)
+        cache.v_scale.fill_(4.0)
+        batch = Batch([(32, 32)], page, spare=0)
+        back = [torch.zeros(32, heads, D, device="cuda", dtype=dtype) for _ in range(2)]
+        serving.cache_read(cache, *back, *batch.args)
+        at = batch.pages[0].long().repeat_interleave(page), torch.arange(page, device="cuda").repeat(2)
+        for got, held, scale in ((back[0], cache.k, 0.5), (back[1], cache.v, 4.0)):
+            want = (held.float() * scale)[at[0], :, at[1]].to(dtype)
+            assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(), want.nan_to_num())
+        assert (fmt == "e4m3") == bool(torch.isnan(back[0]).any())
+
+
+@pytest.mark.parametrize("name", ["k", "v"])
+@pytest.mark.parametrize("dtype,seqs,H", [(BF16, [(4, 60), (3, 200)], 4), (F32, [(4, 60), (3, 200)], 4), (BF16, [(12, 500)], 4), (F32, [(12, 500)], 4), (F32, [(300, 900), (70, 80)], 4),
+                                          (BF16, [(1, 2), (300, 2000)], 4), (BF16, [(700, 900), (1000, 1200)], 8)], ids=["tokens", "tokens32", "rows", "rows32", "many32", "tcgen05", "widened"])
+def test_a_nan_code_matters_to_the_rows_that_see_it(dtype, seqs, H, name):
+    """A NaN code under a finite scale: the rows before its position are as they were without, the others are NaN."""
+    batch = Batch(seqs, 16, seed=3)
+    heads, D = 2, 32
+    n, length = batch.seqs[-1]
+    cache, k, v = su.filled_cache(batch, heads, D, dtype, "e4m3")
+    p = length - 2                                                  # the last row but one sees it, the one before does not
+    page, slot = int(batch.table[-1, p // 16]), p % 16
+    getattr(cache, name).view(torch.uint8)[page, 1, slot, 3] = 0x7F if name == "k" else 0xFF
+    (k if name == "k" else v)[page, 1, slot, 3] = float("nan")
+    q = _normal(_gen(5), batch.T, H, D, dtype=dtype)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, *batch.args, H)
+    want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5)), dtype, "e4m3")
+    clean = torch.ones(batch.T, H, dtype=torch.bool, device="cuda")
+    clean[batch.first[-2] + n - 2:, H // heads:] = False
+    within(out[clean], want[clean], bound[clean], "rows that do not see it")
+    seen = out[~clean]
+    assert bool(torch.isnan(seen if name == "k" else seen[:, 3]).all()), "rows that do"
