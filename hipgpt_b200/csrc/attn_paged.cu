@@ -159,7 +159,7 @@ __device__ __forceinline__ void bring(const AttnArgs &a, Run<C::ROWS, C::UNIT, T
 
 template <typename T, int FMT, int DP, bool SPLITROWS, bool CUT = false>
 __global__ void __launch_bounds__(kThreads, Shape<T, FMT, DP, SPLITROWS, CUT>::kBlocks)
-paged_rows_kernel(const AttnArgs a)
+paged_rows_kernel(const __grid_constant__ AttnArgs a)
 {
     using C = Shape<T, FMT, DP, SPLITROWS, CUT>;
     constexpr bool HALF = C::CODED;
@@ -174,12 +174,16 @@ paged_rows_kernel(const AttnArgs a)
     __shared__ float2 ml_s[2][16];
     __shared__ float q_unit[C::ROWS];
     __shared__ volatile int abort_flag;
+    __shared__ uint32_t mend_s;                      // tiles of the run (their numbers modulo 32) with rows to look at again
+    __shared__ typename Run<C::ROWS, C::UNIT, kThreads>::Start start_s;
+    __shared__ int tops[kWarps];
 
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int D = a.c.D;
     if (tid == 0) {
         abort_flag = 0;
+        mend_s = 0;
         for (int i = 0; i < SLOTS; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kWarps);
@@ -202,6 +206,7 @@ paged_rows_kernel(const AttnArgs a)
     };
     Run<C::ROWS, C::UNIT, kThreads> run(a);
     bool more = run.begin(sums);
+    if (more) run.keep(&start_s);
 
     if (warp == kWarps) {
         bring<C, kThreads>(a, run, more, ring, full, empty, there_s, wait);
@@ -216,9 +221,9 @@ paged_rows_kernel(const AttnArgs a)
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
     };
-    uint32_t slot = 0;
+    uint32_t slot = 0, number = 0;                   // of places; of the tile in the run
     int4 cut = make_int4(0, 0, 0, -1);
-    for (; more; more = run.next()) {
+    for (; more; more = run.next(), ++number) {
         const Tile w = run.at();
         const Sequence &s = w.s;
         const int rows = (int)min((long long)s.n * a.group, 2147483647LL);
@@ -651,24 +656,22 @@ paged_rows_kernel(const AttnArgs a)
                         if (store) dst[(size_t)r * DP + d] = y;
                     } else {
                         y = sum == 0.0f ? 0.0f : y * inv;
-                        wild = wild || !(fabsf(y) <= 3.402823466e38f);
+                        wild = wild || (!finite(y) && sum == sum);
                         if (d < D && store) out[d] = from_float<T>(y);
                     }
                 }
                 if (dst) {
                     if (lane == 0 && store) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[r] = make_float2(top, sum);
-                } else if (__any_sync(0xffffffffu, wild) && store) {
-                    __syncwarp();
-                    mend_row<T, FMT>(a, w.b, w.head, s, row, keys);
+                } else if (__any_sync(0xffffffffu, wild) && lane == 0 && store) {
+                    atomicOr(&mend_s, 1u << (number & 31));
                 }
             }
         } else {
-            bool wild[C::MT][2];
+            bool wild = false;
 #pragma unroll
             for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    wild[mt][r] = false;
                     const int rr = (warp * C::MT + mt) * 16 + g + 8 * r, row = row0 + rr;
                     const float sum = l[mt][r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                     const bool here = row < rows && store;
@@ -686,29 +689,17 @@ paged_rows_kernel(const AttnArgs a)
                                     if (here) dst[(size_t)rr * DP + d] = y;
                                 } else {
                                     const float v = sum == 0.0f ? 0.0f : y * inv;
-                                    wild[mt][r] = wild[mt][r] || (here && !(fabsf(v) <= 3.402823466e38f));
+                                    wild = wild || (here && !finite(v) && sum == sum);
                                     if (here && d < D) out[d] = from_float<T>(v);
                                 }
                             }
                     if (dst && here && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[mt][r], sum);
                 }
-            if (!dst) {
-#pragma unroll
-                for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        unsigned some = __ballot_sync(0xffffffffu, wild[mt][r]);
-                        __syncwarp();
-                        while (some) {
-                            const int who = (__ffs((int)some) - 1) >> 2;         // its row in the tile's eight
-                            some &= ~(0xFu << (4 * who));
-                            mend_row<T, FMT>(a, w.b, w.head, s, row0 + (warp * C::MT + mt) * 16 + who + 8 * r, keys_met(a, s, keys));
-                        }
-                    }
-            }
+            if (__any_sync(0xffffffffu, wild) && lane == 0) atomicOr(&mend_s, 1u << (number & 31));
         }
     }
     meet();
+    if (mend_s) mend_run<T, FMT, C::ROWS, C::UNIT, kThreads>(a, &start_s, mend_s, warp, kWarps, tops, meet);
     if (a.cuts && tid == 0) {
         a.cuts[blockIdx.x] = cut;
         a.whole[blockIdx.x] = !abort_flag;
@@ -742,7 +733,7 @@ __device__ __forceinline__ uint32_t turned8(uint32_t x)
 
 template <typename T, int FMT, int DP>
 __global__ void __launch_bounds__(kThreads, TokenShape<T, FMT, DP>::kBlocks)
-paged_token_kernel(const AttnArgs a)
+paged_token_kernel(const __grid_constant__ AttnArgs a)
 {
     using C = TokenShape<T, FMT, DP>;
     constexpr bool HALF = C::CODED;
@@ -757,12 +748,16 @@ paged_token_kernel(const AttnArgs a)
     __shared__ float2 ml_s[kWarps][8];
     __shared__ float q_unit[8];
     __shared__ volatile int abort_flag;
+    __shared__ uint32_t mend_s;
+    __shared__ typename Run<C::ROWS, C::UNIT, kThreads>::Start start_s;
+    __shared__ int tops[kWarps];
 
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int D = a.c.D;
     if (tid == 0) {
         abort_flag = 0;
+        mend_s = 0;
         for (int i = 0; i < SLOTS; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kWarps);
@@ -784,6 +779,7 @@ paged_token_kernel(const AttnArgs a)
     };
     Run<C::ROWS, C::UNIT, kThreads> run(a);
     bool more = run.begin(sums);
+    if (more) run.keep(&start_s);
     if (warp == kWarps) {
         bring<C, kThreads>(a, run, more, ring, full, empty, there_s, wait);
         __syncwarp();
@@ -796,9 +792,9 @@ paged_token_kernel(const AttnArgs a)
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
     };
-    uint32_t slot = 0;
+    uint32_t slot = 0, number = 0;                   // of places; of the tile in the run
     int4 cut = make_int4(0, 0, 0, -1);
-    for (; more; more = run.next()) {
+    for (; more; more = run.next(), ++number) {
         const Tile w = run.at();
         const Sequence &s = w.s;
         const int rows = (int)min((long long)s.n * a.group, 2147483647LL);
@@ -1148,19 +1144,19 @@ paged_token_kernel(const AttnArgs a)
                     if (store) dst[(size_t)r * DP + d] = y;
                 } else {
                     y = sum == 0.0f ? 0.0f : y * inv;
-                    wild = wild || !(fabsf(y) <= 3.402823466e38f);
+                    wild = wild || (!finite(y) && sum == sum);
                     if (d < D && store) out[d] = from_float<T>(y);
                 }
             }
             if (dst) {
                 if (lane == 0 && store) reinterpret_cast<float2 *>(dst + 8 * DP)[r] = make_float2(top, sum);
-            } else if (__any_sync(0xffffffffu, wild) && store) {
-                __syncwarp();
-                mend_row<T, FMT>(a, w.b, w.head, s, row, keys);
+            } else if (__any_sync(0xffffffffu, wild) && lane == 0 && store) {
+                atomicOr(&mend_s, 1u << (number & 31));
             }
         }
     }
     meet();
+    if (mend_s) mend_run<T, FMT, C::ROWS, C::UNIT, kThreads>(a, &start_s, mend_s, warp, kWarps, tops, meet);
     if (a.cuts && tid == 0) {
         a.cuts[blockIdx.x] = cut;
         a.whole[blockIdx.x] = !abort_flag;

@@ -198,13 +198,19 @@ struct Run {
         if (base >= start && base + units <= end) return -1;
         return 2 * (int)blockIdx.x + (base >= start ? 1 : 0);
     }
+    // The run once more: thread 0 keeps in shared memory where it began (behind begin())
+    struct Start { long long start, end, per, base; int b, tile, head, units; };
+    __device__ __forceinline__ void keep(Start *to) const { if (threadIdx.x == 0) *to = {start, end, per, base, b, tile, head, units}; }
+    __device__ __forceinline__ Run(const AttnArgs &args, const Start &from)
+        : a(args), u(from.start), end(from.end), start(from.start), per(from.per), b(from.b), tile(from.tile), head(from.head), base(from.base), s(sequence_of(args.c, from.b)), units(from.units) {}
     // Noted by the block that has the first unit of a tile that goes on
     __device__ __forceinline__ int4 cut() const { return make_int4(b, head, tile, (int)((base + units - 1) / per)); }
 };
 
-// ---- rows worked out key by key ----------------------------------------------------------------------------------------
+// ---- rows worked out again ---------------------------------------------------------------------------------------------
 // A product over a tile of keys takes every row's probabilities times every key's values, zero times what a row must not see.  Where that is an infinity or NaN the
-// sum is NaN.  Such a row is found by its result, and is worked out again without the keys that it does not see.
+// sum is NaN.  Such a row is found by its result, and is worked out again over the keys that it sees: when the block's whole run is done and nobody in it waits for anything any more (a long row
+// takes longer than a wait may), or where parts are joined.
 
 // One value of a row of the cache
 template <typename T, int FMT>
@@ -219,22 +225,47 @@ __device__ __forceinline__ float cached(const uint8_t *base, const float *scale,
     }
 }
 
+// Sixteen values in a row of the cache, of codes without their scale
 template <typename T, int FMT>
-__device__ __forceinline__ bool any_wild(const AttnArgs &a, int b, int head, int from, int to)
+__device__ __forceinline__ void cached16(const uint8_t *base, long long row, int D, int d, float (&x)[16])
 {
-    const int lane = threadIdx.x & 31;
-    bool wild = false;
-    for (int p = from; p < to && !wild; ++p) {
-        const long long row = row_of(a.c, b, head, p);
-        bool w = false;
-        if (row >= 0)
-            for (int d = lane; d < a.c.D; d += 32) w = w || !(fabsf(cached<T, FMT>(a.c.v, a.c.vs, row, a.c.D, d)) <= 3.402823466e38f);
-        wild = __any_sync(0xffffffffu, w);
+    if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
+        constexpr int W = kPer16<T>;
+#pragma unroll
+        for (int i = 0; i < 16 / W; ++i) {
+            float y[W];
+            load_values<T, W>(reinterpret_cast<const T *>(base) + row * D + d + i * W, y);
+#pragma unroll
+            for (int e = 0; e < W; ++e) x[i * W + e] = y[e];
+        }
+    } else {
+        const uint4 c = *reinterpret_cast<const uint4 *>(base + row * D + d);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t lo, hi;
+            codes_to_half<FMT>(w[i], lo, hi);
+            const float2 p = floats_of(lo), q = floats_of(hi);
+            x[4 * i] = p.x; x[4 * i + 1] = p.y; x[4 * i + 2] = q.x; x[4 * i + 3] = q.y;
+        }
     }
-    return wild;
 }
 
-// One warp: values c0 .. c1 of row `row` of (sequence b, head of the cache)
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Whether a value at position p of the sequence is an infinity or NaN (all lanes of a warp)
+template <typename T, int FMT>
+__device__ __forceinline__ bool wild_at(const AttnArgs &a, int b, int head, int p)
+{
+    const long long row = row_of(a.c, b, head, p);
+    bool wild = false;
+    if (row >= 0)
+        for (int d = threadIdx.x & 31; d < a.c.D; d += 32) wild = wild || !finite(cached<T, FMT>(a.c.v, a.c.vs, row, a.c.D, d));
+    return __any_sync(0xffffffffu, wild);
+}
+
+// One warp: values c0 .. c1 of row `row` of (sequence b, head of the cache), 32 keys at a time: a lane a key for the scores (sixteen sums each), a lane every 32nd value for the sums over
+// the keys, which are added up 32 by 32.  About 40 clocks a key with eight warps an SM; one key after the other, with its look-ups and shuffles in a chain, it was several hundred.
 template <typename T, int FMT>
 __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row, int c0, int c1)
 {
@@ -248,25 +279,72 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
         qv[i] = lane + 32 * i < D ? to_float(q[lane + 32 * i]) : 0.0f;
         o[i] = 0.0f;
     }
-    for (int p = 0; p < limit; ++p) {
-        const long long r = row_of(a.c, b, head, p);
-        if (r < 0) continue;
-        float z = 0.0f;
+    for (int p0 = 0; p0 < limit; p0 += 32) {
+        const int p = p0 + lane;
+        const long long r = p < limit ? row_of(a.c, b, head, p) : -1;
+        float z[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) z = fmaf(qv[i], cached<T, FMT>(a.c.k, a.c.ks, r, D, lane + 32 * i), z);
+        for (int e = 0; e < 16; ++e) z[e] = 0.0f;
 #pragma unroll
-        for (int off = 16; off; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-        z *= a.cscale;
-        const float mn = fmaxf(m, z), base = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = exp2f(m - base), e = exp2f(z - base);
+        for (int c = 0; c < 8; ++c) {
+            if (16 * c >= D) break;
+            float k[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) k[e] = 0.0f;
+            if (r >= 0) cached16<T, FMT>(a.c.k, r, D, 16 * c, k);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z[e] = fmaf(__shfl_sync(0xffffffffu, qv[c / 2], 16 * (c % 2) + e), k[e], z[e]);
+        }
+#pragma unroll
+        for (int n = 8; n; n >>= 1)
+#pragma unroll
+            for (int e = 0; e < n; ++e) z[e] += z[e + n];
+        float score = z[0] * a.cscale, weight = 1.0f;
+        if constexpr (FMT != HIPGPT_CACHE_PLAIN)
+            if (r >= 0) {
+                score *= a.c.ks[r];
+                weight = a.c.vs[r];
+            }
+        if (r < 0) score = -INFINITY;
+        float top = score;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = exp2f(m - base), e = exp2f(score - base);
         m = mn;
-        l = fmaf(l, alpha, e);
+        float sum = e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lane + 32 * i < D) o[i] = fmaf(e, cached<T, FMT>(a.c.v, a.c.vs, r, D, lane + 32 * i), o[i] * alpha);
-        // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l = fmaf(l, alpha, sum);
+        // (one lane's scale and place after the other; a place that is none is not looked at)
+        const float f = r < 0 ? 0.0f : e * weight;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int j = 0; j < 32; ++j) {
+            const long long rj = __shfl_sync(0xffffffffu, r, j);
+            const float fj = __shfl_sync(0xffffffffu, f, j);
+            if (rj < 0) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (lane + 32 * i >= D) continue;
+                float v;
+                if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
+                    v = to_float(reinterpret_cast<const T *>(a.c.v)[rj * D + lane + 32 * i]);
+                } else {
+                    uint32_t lo, hi;
+                    codes_to_half<FMT>(a.c.v[rj * D + lane + 32 * i], lo, hi);
+                    v = floats_of(lo).x;
+                }
+                x[i] = fmaf(fj, v, x[i]);
+            }
+        }
         bool number = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) number = number || (lane + 32 * i < D && o[i] == o[i]);
+        for (int i = 0; i < 4; ++i) {
+            o[i] = fmaf(o[i], alpha, x[i]);
+            number = number || (lane + 32 * i < D && o[i] == o[i]);
+        }
+        // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
         if (l != l || !__any_sync(0xffffffffu, number)) break;
     }
     T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
@@ -274,32 +352,66 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
     for (int i = 0; i < 4; ++i) if (lane + 32 * i >= c0 && lane + 32 * i < min(c1, D)) out[lane + 32 * i] = from_float<T>(l == 0.0f ? 0.0f : o[i] / l);
 }
 
-// Whether a row whose result is not finite was touched by keys that it does not see (its tile's keys go up to `keys`)
-template <typename T, int FMT>
-__device__ __forceinline__ void mend_row(const AttnArgs &a, int b, int head, const Sequence &s, int row, int keys, int c0 = 0, int c1 = 128)
-{
-    const int limit = limit_of(a, s, row);
-    if (limit < keys && any_wild<T, FMT>(a, b, head, limit, keys)) row_again<T, FMT>(a, b, head, s, row, c0, c1);
-}
-
 // The keys that a tile's rows have been multiplied with: those they see, and where these were cut before, to the end of the last place
 __device__ __forceinline__ int keys_met(const AttnArgs &a, const Sequence &s, int keys) { return a.cut_unit ? (int)min((long long)s.len, ((long long)keys + a.cut_unit - 1) / a.cut_unit * a.cut_unit) : keys; }
+
+// The tile's rows from `first` on, every `step`th, one a warp, that hold something that is not finite in their values c0 .. c1 and were touched by keys that they do not see.  The block's `warps` warps call it
+// together (meet() is their barrier), with their rows stored.
+template <typename T, int FMT, int ROWS, typename Meet>
+__device__ __forceinline__ void mend_tile(const AttnArgs &a, int b, int head, int tile, const Sequence &s, int first, int step, int warp, int warps, int *tops, Meet meet, int c0 = 0, int c1 = 128)
+{
+    const int lane = threadIdx.x & 31, row0 = tile * ROWS;
+    const int rows = (int)min((long long)s.n * a.group - row0, (long long)ROWS), keys = keys_met(a, s, tile_keys<ROWS>(a, s, tile));
+    // the last such position: rows that see it see all of them
+    int top = -1;
+    for (int p = limit_of(a, s, row0) + warp; p < keys; p += warps) if (wild_at<T, FMT>(a, b, head, p)) top = p;
+    meet();                                          // (everybody's rows are stored, and what was there before has been read)
+    if (lane == 0) tops[warp] = top;
+    meet();
+    for (int w = 0; w < warps; ++w) top = max(top, tops[w]);
+    for (int r = first; r < rows; r += step) {
+        const int row = row0 + r;
+        if (limit_of(a, s, row) > top) break;
+        const T *out = static_cast<const T *>(a.out) + (long long)(s.first + row / a.group) * a.out_stride + (long long)(head * a.group + row % a.group) * a.c.D;
+        bool wild = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = lane + 32 * i;
+            if (d >= c0 && d < min(c1, a.c.D)) wild = wild || !finite(to_float(out[d]));
+        }
+        if (__any_sync(0xffffffffu, wild)) row_again<T, FMT>(a, b, head, s, row, c0, c1);
+    }
+}
+
+// The tiles of a block's run whose number (modulo 32) is in `which`
+template <typename T, int FMT, int ROWS, int UNIT, int THREADS, typename Meet>
+__device__ __noinline__ void mend_run(const AttnArgs &a, const typename Run<ROWS, UNIT, THREADS>::Start *from, uint32_t which, int warp, int warps, int *tops, Meet meet)
+{
+    Run<ROWS, UNIT, THREADS> run(a, *from);
+    int k = 0;
+    do {
+        if ((which >> (k & 31) & 1) && run.part() < 0) mend_tile<T, FMT, ROWS>(a, run.b, run.head, run.tile, run.s, warp, warps, warp, warps, tops, meet);
+        ++k;
+    } while (run.next());
+}
 
 // ---- joining the parts ----------------------------------------------------------------------------------------------------
 // One block a block of the kernel before it: the tile that began there, if it went on.  A warp takes a row; parts in ascending order.
 template <typename T, int FMT, int ROWS, int DP>
 __global__ void __launch_bounds__(256)
-paged_join_kernel(const AttnArgs a)
+paged_join_kernel(const __grid_constant__ AttnArgs a)
 {
     dependency_wait();
     dependents_may_start();
     const int4 cut = a.cuts[blockIdx.x];
     if (cut.w < 0) return;
     for (int blk = blockIdx.x; blk <= cut.w; ++blk) if (!a.whole[blk]) return;
+    __shared__ int tops[8];
     const Sequence s = sequence_of(a.c, cut.x);
     const int lane = threadIdx.x & 31, D = a.c.D;
     constexpr int E = DP / 32;
     const long long rows = (long long)s.n * a.group;
+    bool wild = false;
     for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < ROWS; r += 8 * gridDim.y) {
         const long long row = (long long)cut.z * ROWS + r;
         if (row >= rows) break;
@@ -319,17 +431,16 @@ paged_join_kernel(const AttnArgs a)
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const long long t = s.first + row / a.group;
         T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(cut.y * a.group + (int)(row % a.group)) * D;
-        bool wild = false;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const float y = l == 0.0f ? 0.0f : o[i] * inv;
-            wild = wild || !(fabsf(y) <= 3.402823466e38f);
+            wild = wild || (!finite(y) && l == l);
             if (lane + 32 * i < D) out[lane + 32 * i] = from_float<T>(y);
         }
-        if (__any_sync(0xffffffffu, wild)) {
-            __syncwarp();
-            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)row, keys_met(a, s, tile_keys<ROWS>(a, s, cut.z)));
-        }
+    }
+    if (__syncthreads_or(wild)) {
+        const int warp = threadIdx.x >> 5;
+        mend_tile<T, FMT, ROWS>(a, cut.x, cut.y, cut.z, s, blockIdx.y * 8 + warp, 8 * gridDim.y, warp, 8, tops, [] { __syncthreads(); });
     }
 }
 

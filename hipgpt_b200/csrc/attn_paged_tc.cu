@@ -71,7 +71,7 @@ struct TcCfg {
 
 template <int FMT, int DP, bool WIDENED>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a, const Wide wide, int expire)
+paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnArgs a, const Wide wide, int expire)
 {
     using C = TcCfg<FMT, DP, WIDENED>;
     using T = __nv_bfloat16;
@@ -94,11 +94,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ long long sums[kThreads / 32 + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
+    __shared__ uint32_t mend_s;                      // tiles of the run (their numbers modulo 32) with rows to look at again
+    __shared__ typename Run<kRows, kKeys, kThreads>::Start start_s;
+    __shared__ int tops[8];
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         abort_flag = 0;
+        mend_s = 0;
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], WIDENS ? kWideners / 32 : 1);
             mbar_init(&v_full[i], WIDENS ? kWideners / 32 : 1);
@@ -148,6 +152,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     Run<kRows, kKeys, kThreads> run(a);
     bool more = run.begin(sums);
+    if (more) run.keep(&start_s);
     // units of each of the two tiles of rows within the block's run of the tile: [from, to) cut to what the tile's rows see (the second has no rows where there are none)
     auto units_of = [&](const Tile &w, int half) {
         const long long rows = (long long)w.s.n * a.group, first = (long long)w.tile * kRows + 128 * half;
@@ -420,10 +425,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int half = warp >> 2, quad = warp & 3, D = a.c.D;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + kColS + half * 128 + lanes, o_addr = tmem + kColO + half * 128 + lanes;
-        uint32_t n = 0, ns = 0, no = 0;              // tiles of keys, of scores; tiles of rows
+        uint32_t n = 0, ns = 0, no = 0, number = 0;  // tiles of keys, of scores; tiles of rows, twice
         int4 cut = make_int4(0, 0, 0, -1);
         const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.q_stride * 2) | (uintptr_t)(a.out_stride * 2)) & 15) == 0;
-        for (; more; more = run.next()) {
+        for (; more; more = run.next(), ++number) {
             const Tile w = run.at();
             const long long rows = (long long)w.s.n * a.group;
             const int r = half * 128 + quad * 32 + lane;                     // row of the block's tile
@@ -617,7 +622,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         x[e] = l == 0.0f ? 0.0f : x[e] * inv;
-                        wild = wild || !(fabsf(x[e]) <= 3.402823466e38f);
+                        wild = wild || (!finite(x[e]) && l == l);
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
@@ -641,17 +646,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
                     }
                 }
-                unsigned some = __ballot_sync(0xffffffffu, wild && store && mine);
-                __syncwarp();
-                while (some) {
-                    const int who = __ffs((int)some) - 1;
-                    some &= some - 1;
-                    mend_row<T, FMT>(a, w.b, w.head, w.s, (int)(wfirst + who), tile_keys<kRows>(a, w.s, w.tile));
-                }
+                if (__any_sync(0xffffffffu, wild && mine) && lane == 0 && store) atomicOr(&mend_s, 1u << (number & 31));
             }
             tc_fence_before();                       // (these columns are read before the next products write them)
         }
         if (tid == 0 && a.cuts) a.cuts[blockIdx.x] = cut;
+        // (the other roles have come to their end, or need nothing more of this one to come to it)
+        auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        meet();
+        if (mend_s) mend_run<T, FMT, kRows, kKeys, kThreads>(a, &start_s, mend_s, warp, 8, tops, meet);
     }
     tc_fence_before();
     __syncthreads();
@@ -765,7 +768,7 @@ paged_widen_kernel(const PagedView c, const Wide wide)
 // Joins the parts of the tile that began in this block of the kernel before and went on; a thread a row and sixteen columns, parts in ascending order.
 template <int FMT, int DP>
 __global__ void __launch_bounds__(256)
-paged_tc_join_kernel(const AttnArgs a)
+paged_tc_join_kernel(const __grid_constant__ AttnArgs a)
 {
     using T = __nv_bfloat16;
     dependency_wait();
@@ -773,6 +776,7 @@ paged_tc_join_kernel(const AttnArgs a)
     const int4 cut = a.cuts[blockIdx.x];
     if (cut.w < 0) return;
     for (int blk = blockIdx.x; blk <= cut.w; ++blk) if (!a.whole[blk]) return;
+    __shared__ int tops[8];
     const Sequence s = sequence_of(a.c, cut.x);
     const int r = threadIdx.x, D = a.c.D, c0 = blockIdx.y * 16;
     const long long row = (long long)cut.z * kRows + r, rows = (long long)s.n * a.group;
@@ -799,7 +803,7 @@ paged_tc_join_kernel(const AttnArgs a)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         o[e] = l == 0.0f ? 0.0f : o[e] * inv;
-        wild = wild || !(fabsf(o[e]) <= 3.402823466e38f);
+        wild = wild || (!finite(o[e]) && l == l);
     }
     if (row < rows && c0 < D) {
         if (((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_stride * 2)) & 15) == 0) {
@@ -814,13 +818,8 @@ paged_tc_join_kernel(const AttnArgs a)
         }
     }
     if (__syncthreads_or(row < rows && wild)) {
-        const int keys = tile_keys<kRows>(a, s, cut.z);
-        unsigned some = __ballot_sync(0xffffffffu, row < rows && wild);
-        while (some) {
-            const int who = __ffs((int)some) - 1;
-            some &= some - 1;
-            mend_row<T, FMT>(a, cut.x, cut.y, s, (int)(row - (r & 31)) + who, keys, c0, c0 + 16);
-        }
+        const int warp = r >> 5;
+        mend_tile<T, FMT, kRows>(a, cut.x, cut.y, cut.z, s, warp, 8, warp, 8, tops, [] { __syncthreads(); }, c0, c0 + 16);
     }
 }
 

@@ -70,3 +70,30 @@ def test_a_nan_code_matters_to_the_rows_that_see_it(dtype, seqs, H, name):
     within(out[clean], want[clean], bound[clean], "rows that do not see it")
     seen = out[~clean]
     assert bool(torch.isnan(seen if name == "k" else seen[:, 3]).all()), "rows that do"
+
+
+# ---- rows touched by what they do not see -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,fmt,heads,H,D,seqs", [(BF16, "plain", 2, 4, 64, [(600, 140000), (40, 300)]), (BF16, "e4m3", 1, 2, 128, [(600, 140000), (40, 300)]), (BF16, "int8", 1, 4, 64, [(1000, 140000), (900, 950)]),
+                                                      (F32, "plain", 2, 2, 32, [(500, 140000), (40, 300)]), (F32, "int8", 1, 2, 64, [(300, 140000), (40, 300)]), (BF16, "e4m3", 2, 2, 64, [(8, 200000), (8, 200)]),
+                                                      (BF16, "plain", 8, 32, 128, [(1500, 20000), (900, 2000)]), (F32, "plain", 16, 32, 64, [(700, 9000), (300, 2000)])])
+def test_an_infinity_that_long_rows_do_not_see(dtype, fmt, heads, H, D, seqs):
+    """An infinity in the last value of a long sequence: the rows of its tile are worked out again, and no wait runs out for it in their block, so that everything else is as ever."""
+    batch = Batch(seqs, 64, seed=3)
+    n, length = seqs[0]
+    page, slot = int(batch.table[0, (length - 1) // 64]), (length - 1) % 64
+
+    def wild(name, x):
+        if name == "v":
+            x[page, :, slot, 3] = float("inf")
+    cache, k, v = su.filled_cache(batch, heads, D, dtype, fmt, wild=wild)
+    q = _normal(_gen(5), batch.T, H, D, dtype=dtype)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, *batch.args, H)
+    torch.cuda.synchronize()
+    assert _status() == 0
+    want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5)), dtype, fmt)
+    clean = torch.ones(batch.T, dtype=torch.bool, device="cuda")
+    clean[n - 1] = False
+    within(out[clean], want[clean], bound[clean])
+    assert not bool(torch.isfinite(out[n - 1, :, 3]).any()), "the row that sees it"
