@@ -39,9 +39,10 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint4 &a, uint32_t b0
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-// The next piece of two fp32 values; what is left in the values
+// The next piece of two fp32 values; what is left in the values.  bf16: a piece that others follow stays finite (values from 3.396e38 on would round to infinity, and nothing but NaN would be left),
+// so an infinity goes on to the last.
 template <bool HALF>
-__device__ __forceinline__ uint32_t next_piece(float &lo, float &hi)
+__device__ __forceinline__ uint32_t next_piece(float &lo, float &hi, bool last)
 {
     if constexpr (HALF) {
         const uint32_t w = half2_of(lo, hi);
@@ -50,7 +51,9 @@ __device__ __forceinline__ uint32_t next_piece(float &lo, float &hi)
         hi -= f.y;
         return w;
     } else {
-        const uint32_t w = pack_bf16(lo, hi);
+        uint32_t w;
+        if (last) w = pack_bf16(lo, hi);
+        else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
         lo -= __uint_as_float(w << 16);
         hi -= __uint_as_float(w & 0xFFFF0000u);
         return w;
@@ -264,10 +267,10 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
             for (int n = 0; n < C::NQ; ++n) {
                 uint4 f;
-                f.x = next_piece<HALF>(x[0][0], x[0][1]);
-                f.y = next_piece<HALF>(x[1][0], x[1][1]);
-                f.z = next_piece<HALF>(x[0][2], x[0][3]);
-                f.w = next_piece<HALF>(x[1][2], x[1][3]);
+                f.x = next_piece<HALF>(x[0][0], x[0][1], n == C::NQ - 1);
+                f.y = next_piece<HALF>(x[1][0], x[1][1], n == C::NQ - 1);
+                f.z = next_piece<HALF>(x[0][2], x[0][3], n == C::NQ - 1);
+                f.w = next_piece<HALF>(x[1][2], x[1][3], n == C::NQ - 1);
                 q_s[n * (C::ROWS / 16) * C::STEPS * 32 + i] = f;
             }
         }
@@ -370,8 +373,8 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                                 float y[4] = {__uint_as_float(kw[j][0]), __uint_as_float(kw[j][1]), __uint_as_float(kw[j][2]), __uint_as_float(kw[j][3])};
 #pragma unroll
                                 for (int n = 0; n < 3; ++n) {
-                                    b[n][0] = next_piece<false>(y[0], y[1]);
-                                    b[n][1] = next_piece<false>(y[2], y[3]);
+                                    b[n][0] = next_piece<false>(y[0], y[1], n == 2);
+                                    b[n][1] = next_piece<false>(y[2], y[3], n == 2);
                                 }
                             }
 #pragma unroll
@@ -492,10 +495,10 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                     for (int i = 0; i < NG; ++i)
 #pragma unroll
                         for (int n = 0; n < C::NQ; ++n) {
-                            p[n][mt][i].x = next_piece<HALF>(z[mt][2 * i][0], z[mt][2 * i][1]);
-                            p[n][mt][i].y = next_piece<HALF>(z[mt][2 * i][2], z[mt][2 * i][3]);
-                            p[n][mt][i].z = next_piece<HALF>(z[mt][2 * i + 1][0], z[mt][2 * i + 1][1]);
-                            p[n][mt][i].w = next_piece<HALF>(z[mt][2 * i + 1][2], z[mt][2 * i + 1][3]);
+                            p[n][mt][i].x = next_piece<HALF>(z[mt][2 * i][0], z[mt][2 * i][1], n == C::NQ - 1);
+                            p[n][mt][i].y = next_piece<HALF>(z[mt][2 * i][2], z[mt][2 * i][3], n == C::NQ - 1);
+                            p[n][mt][i].z = next_piece<HALF>(z[mt][2 * i + 1][0], z[mt][2 * i + 1][1], n == C::NQ - 1);
+                            p[n][mt][i].w = next_piece<HALF>(z[mt][2 * i + 1][2], z[mt][2 * i + 1][3], n == C::NQ - 1);
                         }
                 }
 
@@ -541,7 +544,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                                     } else {
                                         float x = __uint_as_float(w0[e]), y = __uint_as_float(w1[e]);
 #pragma unroll
-                                        for (int n = 0; n < 3; ++n) b[i][0][n][hf] = next_piece<false>(x, y);
+                                        for (int n = 0; n < 3; ++n) b[i][0][n][hf] = next_piece<false>(x, y, n == 2);
                                     }
                                 }
                             }
@@ -830,8 +833,8 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
             for (int n = 0; n < C::NQ; ++n) {
                 uint2 f;
-                f.x = next_piece<HALF>(x[0], x[1]);
-                f.y = next_piece<HALF>(x[2], x[3]);
+                f.x = next_piece<HALF>(x[0], x[1], n == C::NQ - 1);
+                f.y = next_piece<HALF>(x[2], x[3], n == C::NQ - 1);
                 q_s[n * C::STEPS * 32 + i] = f;
             }
         }
@@ -915,10 +918,10 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
                                 for (int e = 0; e < 4; ++e) y[hf][e] = __uint_as_float(kw[j][hf][e]);
 #pragma unroll
                             for (int n = 0; n < 3; ++n) {
-                                f[n].x = next_piece<false>(y[0][0], y[0][1]);
-                                f[n].y = next_piece<false>(y[1][0], y[1][1]);
-                                f[n].z = next_piece<false>(y[0][2], y[0][3]);
-                                f[n].w = next_piece<false>(y[1][2], y[1][3]);
+                                f[n].x = next_piece<false>(y[0][0], y[0][1], n == 2);
+                                f[n].y = next_piece<false>(y[1][0], y[1][1], n == 2);
+                                f[n].z = next_piece<false>(y[0][2], y[0][3], n == 2);
+                                f[n].w = next_piece<false>(y[1][2], y[1][3], n == 2);
                             }
                         }
 #pragma unroll
@@ -1027,8 +1030,8 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
             for (int j = 0; j < NG; ++j)
 #pragma unroll
                 for (int n = 0; n < C::NQ; ++n) {
-                    p[n][j].x = turned8(next_piece<HALF>(z[j][0], z[j][1]));
-                    p[n][j].y = turned8(next_piece<HALF>(z[j][2], z[j][3]));
+                    p[n][j].x = turned8(next_piece<HALF>(z[j][0], z[j][1], n == C::NQ - 1));
+                    p[n][j].y = turned8(next_piece<HALF>(z[j][2], z[j][3], n == C::NQ - 1));
                 }
             leave(ksl);                              // (what was read of it has been used: an arrival does not wait for loads)
 
@@ -1072,10 +1075,10 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
                                 for (int e = 0; e < 2; ++e) y[k][e] = __uint_as_float(vw[i][k][2 * x + e]);
 #pragma unroll
                             for (int n = 0; n < 3; ++n) {
-                                f[i][n].x = next_piece<false>(y[0][0], y[1][0]);
-                                f[i][n].y = next_piece<false>(y[0][1], y[1][1]);
-                                f[i][n].z = next_piece<false>(y[2][0], y[3][0]);
-                                f[i][n].w = next_piece<false>(y[2][1], y[3][1]);
+                                f[i][n].x = next_piece<false>(y[0][0], y[1][0], n == 2);
+                                f[i][n].y = next_piece<false>(y[0][1], y[1][1], n == 2);
+                                f[i][n].z = next_piece<false>(y[2][0], y[3][0], n == 2);
+                                f[i][n].w = next_piece<false>(y[2][1], y[3][1], n == 2);
                             }
                         }
                     }
@@ -1189,7 +1192,7 @@ paged_cut_kernel(const PagedView c, uint8_t *k_out, uint8_t *v_out, int units)
         float4 y = read(c.k, 8 * j + g, (t4 + 4 * i) * 4);
 #pragma unroll
         for (int n = 0; n < 3; ++n) {
-            const uint32_t lo = next_piece<false>(y.x, y.y), hi = next_piece<false>(y.z, y.w);
+            const uint32_t lo = next_piece<false>(y.x, y.y, n == 2), hi = next_piece<false>(y.z, y.w, n == 2);
             *reinterpret_cast<uint2 *>(k_to + (x * 3 + n) * 256) = make_uint2(lo, hi);
         }
     }
@@ -1206,7 +1209,7 @@ paged_cut_kernel(const PagedView c, uint8_t *k_out, uint8_t *v_out, int units)
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-                const uint32_t lo = next_piece<false>(y[0][e], y[1][e]), hi = next_piece<false>(y[2][e], y[3][e]);
+                const uint32_t lo = next_piece<false>(y[0][e], y[1][e], n == 2), hi = next_piece<false>(y[2][e], y[3][e], n == 2);
                 *reinterpret_cast<uint2 *>(v_to + ((i * C::TILES + cc * 4 + e) * 3 + n) * 256) = make_uint2(lo, hi);
             }
     }

@@ -97,3 +97,56 @@ def test_an_infinity_that_long_rows_do_not_see(dtype, fmt, heads, H, D, seqs):
     clean[n - 1] = False
     within(out[clean], want[clean], bound[clean])
     assert not bool(torch.isfinite(out[n - 1, :, 3]).any()), "the row that sees it"
+
+
+# ---- the largest numbers ------------------------------------------------------------------------------------------------
+
+# Each kernel of fp32 over a plain cache: single tokens, some rows, many cut by the warps, many cut before
+FP32 = [([(1, 700), (2, 90)], 4, 64), ([(9, 300), (12, 77)], 2, 128), ([(40, 300), (25, 77)], 2, 32), ([(150, 300), (170, 400)], 2, 32), ([(200, 300), (170, 400)], 2, 128)]
+
+
+@pytest.mark.parametrize("seqs,H,D", FP32, ids=["tokens", "some", "many", "cut32", "cut128"])
+def test_fp32_next_to_its_largest_number(seqs, H, D):
+    """Values, keys and queries beyond bf16's largest number, 3.39e38, are numbers; an infinite value makes infinities."""
+    most = torch.finfo(F32).max
+    batch, heads = Batch(seqs, 16, seed=5), 2
+    n, length = batch.seqs[-1]
+    page, slot = int(batch.table[-1, (length - 2) // 16]), (length - 2) % 16
+
+    def run(wild, scale=None, spread=1.0, turn=None):
+        cache, k, v = su.filled_cache(batch, heads, D, F32, "plain", wild=wild)
+        q = _normal(_gen(5), batch.T, H, D, scale=spread)
+        if turn is not None:
+            turn(q)
+        out = torch.zeros_like(q)
+        serving.paged_attention(cache, q, out, *batch.args, H, scale=scale)
+        want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5 if scale is None else scale)), F32, "plain")
+        return out, want, bound
+
+    def values(name, x):
+        if name == "v":
+            x[page, :, slot, 3], x[page, :, slot, 4], x[page, :, slot, 5] = most, -3.4e38, 3.397e38
+    within(*run(values), "values")
+
+    def keys(name, x):
+        if name == "k":
+            x *= 1e-3
+            x[page, :, slot, 3], x[page, :, slot, 7] = most, -3.398e38
+    within(*run(keys, scale=1e-10, spread=1e-28), "keys")
+
+    def small(name, x):
+        if name == "k":
+            x *= 1e-28
+
+    def queries(q):
+        q[-2:, :, 3], q[-1:, :, 7] = most, -3.398e38
+    within(*run(small, scale=1e-10, turn=queries), "queries")
+
+    def infinite(name, x):
+        if name == "v":
+            x[page, :, slot, 3], x[page, :, slot, 4] = float("inf"), float("-inf")
+    out, want, bound = run(infinite)
+    sees = torch.zeros(batch.T, dtype=torch.bool, device="cuda")
+    sees[-2:] = True
+    within(out[~sees], want[~sees], bound[~sees], "rows that do not see it")
+    assert bool((out[sees][..., 3] == float("inf")).all()) and bool((out[sees][..., 4] == float("-inf")).all()) and bool(torch.isfinite(out[sees][..., 5:]).all())
