@@ -209,7 +209,8 @@ struct Run {
 
 // ---- rows worked out again ---------------------------------------------------------------------------------------------
 // A product over a tile of keys takes every row's probabilities times every key's values, zero times what a row must not see.  Where that is an infinity or NaN the
-// sum is NaN.  Such a row is found by its result, and is worked out again over the keys that it sees: when the block's whole run is done and nobody in it waits for anything any more (a long row
+// sum is NaN.  Sums over the keys are divided by the probabilities' sum at their end, so they also pass fp32's range where the values come near its largest number.  Such a row is found by its result, and is
+// worked out again over the keys that it sees: when the block's whole run is done and nobody in it waits for anything any more (a long row
 // takes longer than a wait may), or where parts are joined.
 
 // One value of a row of the cache
@@ -253,19 +254,33 @@ __device__ __forceinline__ void cached16(const uint8_t *base, long long row, int
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// Whether a value at position p of the sequence is an infinity or NaN (all lanes of a warp)
+// The last position of [from, to) with a value that is not finite, -1: none.  A lane a position, 32 after 32 of them for each of the block's warps.
 template <typename T, int FMT>
-__device__ __forceinline__ bool wild_at(const AttnArgs &a, int b, int head, int p)
+__device__ __forceinline__ int last_wild(const AttnArgs &a, int b, int head, int from, int to, int warp, int warps)
 {
-    const long long row = row_of(a.c, b, head, p);
-    bool wild = false;
-    if (row >= 0)
-        for (int d = threadIdx.x & 31; d < a.c.D; d += 32) wild = wild || !finite(cached<T, FMT>(a.c.v, a.c.vs, row, a.c.D, d));
-    return __any_sync(0xffffffffu, wild);
+    int top = -1;
+    for (int p0 = from + 32 * warp; p0 < to; p0 += 32 * warps) {
+        const int p = p0 + (threadIdx.x & 31);
+        const long long row = p < to ? row_of(a.c, b, head, p) : -1;
+        bool wild = false;
+        if (row >= 0) {
+            const float unit = FMT == HIPGPT_CACHE_PLAIN ? 1.0f : a.c.vs[row];
+#pragma unroll 4
+            for (int d = 0; d < a.c.D; d += 16) {
+                float x[16];
+                cached16<T, FMT>(a.c.v, row, a.c.D, d, x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) wild = wild || !finite(x[e] * unit);
+            }
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, wild);
+        if (who) top = p0 + 31 - __clz((int)who);
+    }
+    return top;
 }
 
 // One warp: values c0 .. c1 of row `row` of (sequence b, head of the cache), 32 keys at a time: a lane a key for the scores (sixteen sums each), a lane every 32nd value for the sums over
-// the keys, which are added up 32 by 32.  About 40 clocks a key with eight warps an SM; one key after the other, with its look-ups and shuffles in a chain, it was several hundred.
+// the keys, which are added up 32 by 32 and kept as half of their average so far: nothing passes fp32's range that does not end outside it.  About 40 clocks a key with eight warps an SM; one key after the other, with its look-ups and shuffles in a chain, it was several hundred.
 template <typename T, int FMT>
 __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row, int c0, int c1)
 {
@@ -315,9 +330,11 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
         float sum = e;
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        l = fmaf(l, alpha, sum);
+        const float before = l * alpha;
+        l = before + sum;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         // (one lane's scale and place after the other; a place that is none is not looked at)
-        const float f = r < 0 ? 0.0f : e * weight;
+        const float f = r < 0 ? 0.0f : 0.5f * (e * inv) * weight;
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int j = 0; j < 32; ++j) {
@@ -341,7 +358,7 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
         bool number = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            o[i] = fmaf(o[i], alpha, x[i]);
+            o[i] = fmaf(o[i], before * inv, x[i]);
             number = number || (lane + 32 * i < D && o[i] == o[i]);
         }
         // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
@@ -349,29 +366,36 @@ __device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const
     }
     T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (lane + 32 * i >= c0 && lane + 32 * i < min(c1, D)) out[lane + 32 * i] = from_float<T>(l == 0.0f ? 0.0f : o[i] / l);
+    for (int i = 0; i < 4; ++i) {
+        // (an average of finite values that rounding took beyond the largest)
+        const float y = finite(o[i]) ? fminf(fmaxf(2.0f * o[i], -3.402823466e38f), 3.402823466e38f) : o[i];
+        if (lane + 32 * i >= c0 && lane + 32 * i < min(c1, D)) out[lane + 32 * i] = from_float<T>(y);
+    }
 }
 
 // The keys that a tile's rows have been multiplied with: those they see, and where these were cut before, to the end of the last place
 __device__ __forceinline__ int keys_met(const AttnArgs &a, const Sequence &s, int keys) { return a.cut_unit ? (int)min((long long)s.len, ((long long)keys + a.cut_unit - 1) / a.cut_unit * a.cut_unit) : keys; }
 
-// The tile's rows from `first` on, every `step`th, one a warp, that hold something that is not finite in their values c0 .. c1 and were touched by keys that they do not see.  The block's `warps` warps call it
-// together (meet() is their barrier), with their rows stored.
+// The tile's rows from `first` on, every `step`th, one a warp, that hold something that is not finite in their values c0 .. c1 and were touched by keys that they do not see, or see finite values alone.  The block's
+// `warps` warps call it together (meet() is their barrier), with their rows stored.
 template <typename T, int FMT, int ROWS, typename Meet>
 __device__ __forceinline__ void mend_tile(const AttnArgs &a, int b, int head, int tile, const Sequence &s, int first, int step, int warp, int warps, int *tops, Meet meet, int c0 = 0, int c1 = 128)
 {
     const int lane = threadIdx.x & 31, row0 = tile * ROWS;
-    const int rows = (int)min((long long)s.n * a.group - row0, (long long)ROWS), keys = keys_met(a, s, tile_keys<ROWS>(a, s, tile));
-    // the last such position: rows that see it see all of them
-    int top = -1;
-    for (int p = limit_of(a, s, row0) + warp; p < keys; p += warps) if (wild_at<T, FMT>(a, b, head, p)) top = p;
-    meet();                                          // (everybody's rows are stored, and what was there before has been read)
-    if (lane == 0) tops[warp] = top;
-    meet();
-    for (int w = 0; w < warps; ++w) top = max(top, tops[w]);
+    const int rows = (int)min((long long)s.n * a.group - row0, (long long)ROWS), keys = keys_met(a, s, tile_keys<ROWS>(a, s, tile)), least = limit_of(a, s, row0);
+    auto last = [&](int from, int to) {
+        int top = last_wild<T, FMT>(a, b, head, from, to, warp, warps);
+        meet();                                      // (everybody's rows are stored, and what was there before has been read)
+        if (lane == 0) tops[warp] = top;
+        meet();
+        for (int w = 0; w < warps; ++w) top = max(top, tops[w]);
+        return top;
+    };
+    const int top = last(least, keys);               // (rows that see it see all of them)
+    if (top < 0 && last(0, least) >= 0) return;
     for (int r = first; r < rows; r += step) {
         const int row = row0 + r;
-        if (limit_of(a, s, row) > top) break;
+        if (top >= 0 && limit_of(a, s, row) > top) break;
         const T *out = static_cast<const T *>(a.out) + (long long)(s.first + row / a.group) * a.out_stride + (long long)(head * a.group + row % a.group) * a.c.D;
         bool wild = false;
 #pragma unroll

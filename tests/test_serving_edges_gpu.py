@@ -150,3 +150,26 @@ def test_fp32_next_to_its_largest_number(seqs, H, D):
     sees[-2:] = True
     within(out[~sees], want[~sees], bound[~sees], "rows that do not see it")
     assert bool((out[sees][..., 3] == float("inf")).all()) and bool((out[sees][..., 4] == float("-inf")).all()) and bool(torch.isfinite(out[sees][..., 5:]).all())
+
+
+@pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("seqs,H", [([(1, 700), (2, 90)], 4), ([(12, 300), (9, 3000)], 4), ([(200, 500), (170, 400)], 4), ([(700, 5000), (900, 950)], 8)], ids=["tokens", "some", "many", "wide"])
+def test_averages_of_the_largest_numbers(dtype, fmt, seqs, H):
+    """Values of which a few pass fp32's range together: their average does not."""
+    batch, heads, D = Batch(seqs, 64, seed=5), 2, 64
+
+    def wild(name, x):
+        if name == "v":
+            x.clamp_(-1, 1)
+            x[..., 3].fill_(3.0e38)
+            x[..., 5].fill_(-2.9e38)
+            x[..., 7] *= 3.0e38
+    _cache, k, v = su.filled_cache(batch, heads, D, dtype, fmt, wild=wild)
+    assert bool(torch.isfinite(v).all())
+    q = _normal(_gen(5), batch.T, H, D, dtype=dtype, scale=0.25)
+    out = torch.zeros_like(q)
+    serving.paged_attention(_cache, q, out, *batch.args, H)
+    want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5)), dtype, fmt)
+    within(out, want, bound)
+    assert _status() == 0
