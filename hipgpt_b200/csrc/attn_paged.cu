@@ -12,7 +12,7 @@
 //     column of V^T that an instruction needs is one byte (or half) picked from each of two registers.
 // Codes become fp16 (exact), and so does Q, a power of two for each row; a key's scale multiplies its scores, a value's scale its probabilities, all of one power of two that follows the largest.
 // fp32 operands are two fp16 pieces (22 bits) against codes, three bf16 pieces (24 bits) against each other, without the products whose orders add up to more than two.  The tensor core cuts off
-// where others round, so no fp32 sum stays in it for more than a block of keys.
+// where others round, so no sum stays in it for more than a block of keys, or (kKeptUnits) for too many of them.
 #include "attn_paged.cuh"
 #include "stream_workspace.hpp"
 
@@ -27,6 +27,9 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * (kWarps + 1);
 
 __device__ int g_rows_status = 0;
+// The tensor core cuts sums off towards zero, about 2^-24 of a sum for each sixteen keys.  Where they stay in it from one block of keys to the next (single tokens), they are put aside after this many units: 8192
+// keys of a warp at most, so 2^-15.
+constexpr int kKeptUnits = 256;
 
 // D += A B: 16 rows, 8 columns, 16 summed over; fp16 or bf16
 template <bool HALF>
@@ -554,20 +557,15 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                             for (int mt = 0; mt < C::MT; ++mt) {
                                 const int j = c * C::EV + e + x;
-                                if constexpr (C::F32) {
-                                    float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                                    for (int order = C::NQ - 1; order >= 0; --order)
+                                for (int order = C::NQ - 1; order >= 0; --order)
 #pragma unroll
-                                        for (int n = 0; n <= order && n < C::NK; ++n)
+                                    for (int n = 0; n <= order && n < C::NK; ++n)
 #pragma unroll
-                                            for (int i = 0; i < NG; ++i) mma16<HALF>(d4, p[order - n][mt][i], b[i][x][n][0], b[i][x][n][1]);
+                                        for (int i = 0; i < NG; ++i) mma16<HALF>(d4, p[order - n][mt][i], b[i][x][n][0], b[i][x][n][1]);
 #pragma unroll
-                                    for (int y = 0; y < 4; ++y) o[mt][j][y] += d4[y];
-                                } else {
-#pragma unroll
-                                    for (int i = 0; i < NG; ++i) mma16<HALF>(o[mt][j], p[0][mt][i], b[i][x][0][0], b[i][x][0][1]);
-                                }
+                                for (int y = 0; y < 4; ++y) o[mt][j][y] += d4[y];
                             }
                     }
                 }
@@ -856,10 +854,40 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
         for (int j = 0; j < C::TILES; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+        // this thread's sums go to its places in shared memory, on top of what was put there before; `kept_m`: the reference maximum of that
+        float kept_m[2] = {-INFINITY, -INFINITY};
+        bool some = false;
+        auto put = [&] {
+            const float grown = C::CODED ? __uint_as_float((uint32_t)(127 + min(unit, 126)) << 23) : 1.0f;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float f = kept_m[r] == -INFINITY ? 0.0f : ex2_approx(kept_m[r] - m[r]);
+                kept_m[r] = m[r];
+                float *row = o_s + (warp * 8 + 2 * t4 + r) * C::kPad;
+#pragma unroll
+                for (int c = 0; c < C::NV; ++c)
+#pragma unroll
+                    for (int x = 0; x < C::EV / 2; ++x) {
+                        const int j = c * (C::EV / 2) + x;
+                        float2 *at = reinterpret_cast<float2 *>(row + (g + 8 * c) * C::EV + 2 * x);
+                        float2 y = make_float2(o[j][r] * grown, o[j][2 + r] * grown);
+                        if (some) y = make_float2(fmaf(at->x, f, y.x), fmaf(at->y, f, y.y));
+                        *at = y;
+                    }
+            }
+            some = true;
+        };
 
         constexpr int NG = C::KB / 16;
         const int pitch = D * C::EB, k0 = warp * C::KB;
         for (int u = w.from; u < w.to; ++u, slot += 2) {
+            if (!C::F32 && u > w.from && (u - w.from) % kKeptUnits == 0) {
+                put();
+#pragma unroll
+                for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+            }
             const int ksl = slot % SLOTS, vsl = (slot + 1) % SLOTS;
             const uint8_t *k_at = ring + ksl * C::kSlotBytes, *v_at = ring + vsl * C::kSlotBytes;
             const int p0 = u * C::UNIT + k0;         // the warp's first key in the sequence
@@ -1099,7 +1127,6 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
             }
             leave(vsl);
         }
-        const float grown = C::CODED ? __uint_as_float((uint32_t)(127 + min(unit, 126)) << 23) : 1.0f;
 
         // ---- the tile's end: the warps' sums by way of shared memory, two rows a warp --------------------------------------
         const int part = run.part();
@@ -1111,15 +1138,8 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
             if (g == 0) ml_s[warp][2 * t4 + r] = make_float2(m[r], l[r]);
-            float *row = o_s + (warp * 8 + 2 * t4 + r) * C::kPad;
-#pragma unroll
-            for (int c = 0; c < C::NV; ++c)
-#pragma unroll
-                for (int x = 0; x < C::EV / 2; ++x) {
-                    const int j = c * (C::EV / 2) + x;
-                    *reinterpret_cast<float2 *>(row + (g + 8 * c) * C::EV + 2 * x) = make_float2(o[j][r] * grown, o[j][2 + r] * grown);
-                }
         }
+        put();
         meet();
         for (int r = warp; r < 8; r += kWarps) {
             const int row = row0 + r;

@@ -38,6 +38,9 @@ constexpr int kWideners = 128, kThreads = 512;
 constexpr int kSoftRegs = 184, kWidenRegs = 88, kIssueRegs = 56;
 constexpr int kHalf = 64, kSlots = 3;  // keys of a half tile of codes, half tiles in the ring
 constexpr float kRescaleStep = 8.0f;
+// Units after which the sums in TMEM are added to what the block keeps of them in memory: the tensor pipe cuts off towards zero, 2^-24 to 2^-23 of the sum for each sixteen keys, so after 32768 keys 2^-12 at most, an
+// eighth of what rounding a result to bf16 may take.  (Every 64 units: 9 % of a long call.)
+constexpr int kKept = 256;
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
 
 __device__ int g_paged_status = 0;
@@ -489,101 +492,131 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int limit = mine ? limit_of(a, w.s, (int)row) : 0;
             const int least_limit = wfirst < rows ? limit_of(a, w.s, (int)wfirst) : 1 << 30;       // (rows behind the last: their results are not looked at)
             float m = -INFINITY, l = 0.0f;
-            for (int i = 0; i < units; ++i) {
-                const int st = (n + i) % kStages, tb = (n + i) % kTables, p0 = (w.from + i) * kKeys;
-                wait(&s_full[half], ns++ & 1, 4);
-                tc_fence_after();
-                const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
-                const bool masked = p0 + kKeys > least_limit || there != 255u;
-                float v[4][32];
-                if constexpr (WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);                  // (what was divided out comes with the values)
-                if constexpr (!SCALED) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, v[q]);
-                    tmem_wait_ld();
-                } else {
-                    // times the scales of their keys; those of 32 come while the scores do
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float4 f[8];
-                        tmem_ld32(s_addr + q * 32, v[q]);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) f[c] = *reinterpret_cast<const float4 *>(&ks_s[tb][q * 32 + c * 4]);
+            // Where a long run's sums are kept, and behind them their reference maximum: the place of its part, or where the tile is whole, that of the tile that goes on behind the run, the last
+            // of all.  Column after column, so that the lanes' rows lie beside each other.  (Worked out when it is needed: what lives through the loop costs it registers.)
+            auto place = [&] {
+                const int part = run.part();
+                return a.parts + (size_t)(part >= 0 ? part : 2 * (int)blockIdx.x + 1) * kRows * (DP + 2) + r;
+            };
+            auto factor_of = [&](const float *kept) { return kept[DP * kRows] == -INFINITY ? 0.0f : ex2_approx(kept[DP * kRows] - m); };
+            for (int i0 = 0; i0 < units; i0 += kKept) {
+                if (i0 > 0) {
+                    wait(&s_full[half], ns & 1, 4);  // (what was summed before has come: its products were issued before those of these scores)
+                    tc_fence_after();
+                    float *const kept = place();
+                    const float f = i0 > kKept ? factor_of(kept) : 0.0f;
+#pragma unroll 1
+                    for (int hh = 0; hh < DP / 16; ++hh) {
+                        float x[16];
+                        tmem_ld16(o_addr + hh * 16, x);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const float2 lo = fmul2(make_float2(v[q][4 * c], v[q][4 * c + 1]), make_float2(f[c].x, f[c].y)), hi = fmul2(make_float2(v[q][4 * c + 2], v[q][4 * c + 3]), make_float2(f[c].z, f[c].w));
-                            v[q][4 * c] = lo.x; v[q][4 * c + 1] = lo.y; v[q][4 * c + 2] = hi.x; v[q][4 * c + 3] = hi.y;
+                        for (int c = 0; c < 16; ++c) {
+                            float *at = kept + (hh * 16 + c) * kRows;
+                            *at = i0 > kKept ? fmaf(*at, f, x[c]) : x[c];
+                            x[c] = 0.0f;
                         }
+                        tmem_st16(o_addr + hh * 16, x);
                     }
+                    kept[DP * kRows] = m;
+                    tmem_wait_st();
                 }
-                if (masked) {
+                for (int i = i0; i < min(units, i0 + kKept); ++i) {
+                    const int st = (n + i) % kStages, tb = (n + i) % kTables, p0 = (w.from + i) * kKeys;
+                    wait(&s_full[half], ns++ & 1, 4);
+                    tc_fence_after();
+                    const uint32_t there = *reinterpret_cast<volatile uint32_t *>(&there_s[tb]);
+                    const bool masked = p0 + kKeys > least_limit || there != 255u;
+                    float v[4][32];
+                    if constexpr (WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);                  // (what was divided out comes with the values)
+                    if constexpr (!SCALED) {
 #pragma unroll
-                    for (int c = 0; c < kKeys; ++c) v[c / 32][c % 32] = p0 + c < limit && (there >> (c >> 4) & 1) ? v[c / 32][c % 32] : -INFINITY;
-                }
-                // what the scores of each 64 keys are multiplied by, and (codes) the exponent that their values were divided by: P takes it
-                float factor[2] = {row_factor, row_factor}, up[2] = {0.0f, 0.0f};
-                if constexpr (CODED) {
-                    if constexpr (!WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);
+                        for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, v[q]);
+                        tmem_wait_ld();
+                    } else {
+                        // times the scales of their keys; those of 32 come while the scores do
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {    // (a masked score times 0 would be NaN)
-                        factor[h] = fminf(fmaxf(factor[h] * *reinterpret_cast<volatile float *>(&k_unit[tb][h]), 1.17549435e-38f), 3.402823466e38f);
-                        up[h] = *reinterpret_cast<volatile float *>(&v_exp[tb][h]);
-                    }
-                }
-                float mx = -INFINITY;
+                        for (int q = 0; q < 4; ++q) {
+                            float4 f[8];
+                            tmem_ld32(s_addr + q * 32, v[q]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 64 * h; c < 64 * h + 64; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], v[c / 32][c % 32], v[c / 32][c % 32 + 1]);
-                    mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), factor[h], up[h]));
-                }
-                if (i == 0) {
-                    m = mx;
-                } else {
-                    const bool grow = m == -INFINITY ? mx > m : mx > m + kRescaleStep;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
-                        if (grow) m = mx;
-                        l *= alpha;
-                        // what was summed before has come: its products were issued before those of these scores
-#pragma unroll 1
-                        for (int hh = 0; hh < DP / 16; ++hh) {
-                            float x[16];
-                            tmem_ld16(o_addr + hh * 16, x);
+                            for (int c = 0; c < 8; ++c) f[c] = *reinterpret_cast<const float4 *>(&ks_s[tb][q * 32 + c * 4]);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) x[c] *= alpha;
-                            tmem_st16(o_addr + hh * 16, x);
+                            for (int c = 0; c < 8; ++c) {
+                                const float2 lo = fmul2(make_float2(v[q][4 * c], v[q][4 * c + 1]), make_float2(f[c].x, f[c].y)), hi = fmul2(make_float2(v[q][4 * c + 2], v[q][4 * c + 3]), make_float2(f[c].z, f[c].w));
+                                v[q][4 * c] = lo.x; v[q][4 * c + 1] = lo.y; v[q][4 * c + 2] = hi.x; v[q][4 * c + 3] = hi.y;
+                            }
                         }
                     }
-                }
-                // (fp16: P up to 2^14, its small values too)
-                const float ref = m == -INFINITY ? 0.0f : m - kBias;
+                    if (masked) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t pk[16];
-                    const float2 f2 = make_float2(factor[q >> 1], factor[q >> 1]), nref = make_float2(up[q >> 1] - ref, up[q >> 1] - ref);
-                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                        for (int c = 0; c < kKeys; ++c) v[c / 32][c % 32] = p0 + c < limit && (there >> (c >> 4) & 1) ? v[c / 32][c % 32] : -INFINITY;
+                    }
+                    // what the scores of each 64 keys are multiplied by, and (codes) the exponent that their values were divided by: P takes it
+                    float factor[2] = {row_factor, row_factor}, up[2] = {0.0f, 0.0f};
+                    if constexpr (CODED) {
+                        if constexpr (!WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float2 x = ffma2(make_float2(v[q][c], v[q][c + 1]), f2, nref), y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                        sum[c / 2 % 2] = fadd2(sum[c / 2 % 2], y);
-                        pk[c / 2] = CODED ? half2_of(y.x, y.y) : pack_bf16(y.x, y.y);
+                        for (int h = 0; h < 2; ++h) {    // (a masked score times 0 would be NaN)
+                            factor[h] = fminf(fmaxf(factor[h] * *reinterpret_cast<volatile float *>(&k_unit[tb][h]), 1.17549435e-38f), 3.402823466e38f);
+                            up[h] = *reinterpret_cast<volatile float *>(&v_exp[tb][h]);
+                        }
                     }
-                    const float part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                    l = CODED ? fmaf(part, __uint_as_float((uint32_t)(127 - (int)up[q >> 1]) << 23), l) : l + part;
-                    tmem_st16_u32(s_addr + q * 16, pk);
-                    if (q == 1) {
-                        tmem_wait_st();
-                        tc_fence_before();
-                        arrive(&p_full[half][0]);
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 64 * h; c < 64 * h + 64; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], v[c / 32][c % 32], v[c / 32][c % 32 + 1]);
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), factor[h], up[h]));
                     }
+                    if (i == 0) {
+                        m = mx;
+                    } else {
+                        const bool grow = m == -INFINITY ? mx > m : mx > m + kRescaleStep;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
+                            if (grow) m = mx;
+                            l *= alpha;
+                            // what was summed before has come: its products were issued before those of these scores
+#pragma unroll 1
+                            for (int hh = 0; hh < DP / 16; ++hh) {
+                                float x[16];
+                                tmem_ld16(o_addr + hh * 16, x);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) x[c] *= alpha;
+                                tmem_st16(o_addr + hh * 16, x);
+                            }
+                        }
+                    }
+                    // (fp16: P up to 2^14, its small values too)
+                    const float ref = m == -INFINITY ? 0.0f : m - kBias;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
+                        const float2 f2 = make_float2(factor[q >> 1], factor[q >> 1]), nref = make_float2(up[q >> 1] - ref, up[q >> 1] - ref);
+                        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const float2 x = ffma2(make_float2(v[q][c], v[q][c + 1]), f2, nref), y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                            sum[c / 2 % 2] = fadd2(sum[c / 2 % 2], y);
+                            pk[c / 2] = CODED ? half2_of(y.x, y.y) : pack_bf16(y.x, y.y);
+                        }
+                        const float part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                        l = CODED ? fmaf(part, __uint_as_float((uint32_t)(127 - (int)up[q >> 1]) << 23), l) : l + part;
+                        tmem_st16_u32(s_addr + q * 16, pk);
+                        if (q == 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            arrive(&p_full[half][0]);
+                        }
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    arrive(&p_full[half][1]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                arrive(&p_full[half][1]);
             }
             n += max(u0, u1);
             // ---- the tile's end ---------------------------------------------------------------------------------
@@ -595,8 +628,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const bool store = !abort_flag;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bool wild = false;
+            if (units > kKept) {
+                const float *const kept = place();
+                const float f = factor_of(kept);
+#pragma unroll 1
+                for (int hh = 0; hh < DP / 16; ++hh) {
+                    float x[16];
+                    tmem_ld16(o_addr + hh * 16, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = fmaf(kept[(hh * 16 + e) * kRows], f, x[e]);
+                    tmem_st16(o_addr + hh * 16, x);
+                }
+                tmem_wait_st();
+            }
             if (part >= 0) {
-                // a part: column after column, so that the lanes' rows lie beside each other
                 float *dst = a.parts + (size_t)part * kRows * (DP + 2) + r;
 #pragma unroll 1
                 for (int hh = 0; hh < DP / 16; ++hh) {

@@ -340,7 +340,7 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *   hipgpt_paged_attention     out[t][h] = softmax(scale q k^T) v over the keys of t's sequence: causal != 0 those up to t's position, 0 all lengths[b].
  *                              q, out [tokens][H * head_dim], H a multiple of the cache's heads: H / heads query heads in a row share one.  A row that sees no key gets zeros
  *                              (as one whose scores are all minus infinity).  What lies in masked places, NaN too, does not matter.  scale > 0.
- *                              Products on the tensor pipe, sums in fp32.  fp32: of three bf16 pieces of each operand (24 bits), against codes of two fp16 pieces (22 bits, a power of
+ *                              Products on the tensor pipe, sums in fp32 (bf16: up to 32768 keys of them in the tensor core's accumulators, which cut off towards zero, 2^-12 of a sum at most).  fp32: of three bf16 pieces of each operand (24 bits), against codes of two fp16 pieces (22 bits, a power of
  *                              two for each row of q); an infinity in q or a key can make NaN of the scores that it meets, one in a value makes infinities.  bf16, plain cache: probabilities are rounded to bf16 before
  *                              the second product.  8-bit caches: probabilities times their values' scales are held in fp16 over a power of two that follows the largest: a value whose scale is
  *                              below 2^-38 of its sequence's largest is lost.  bf16 with many rows a sequence: in int8 a value times its scale is rounded to fp16, and values share a power of two

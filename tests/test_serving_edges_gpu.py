@@ -173,3 +173,40 @@ def test_averages_of_the_largest_numbers(dtype, fmt, seqs, H):
     want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5)), dtype, fmt)
     within(out, want, bound)
     assert _status() == 0
+
+
+# ---- sums over many keys --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", ["plain", "e4m3", "int8"])
+@pytest.mark.parametrize("n,heads,H,D,copies", [(1, 16, 16, 32, 28), (1, 16, 192, 32, 28), (2400, 1, 16, 64, 1), (80, 2, 64, 64, 4)], ids=["tokens", "some", "wide", "many"])
+def test_sums_over_a_million_keys(fmt, n, heads, H, D, copies):
+    """Keys of zeros: every row is the average of all values.  What a sum in the tensor core's accumulators cuts off, always towards zero, must not add up over a long run of keys."""
+    page, length = 1024, 1 << 20
+    batch = Batch([(n, length)], page, seed=2)
+    cache = serving.PagedCache(batch.num_pages, page, heads, D, dtype=BF16, format=fmt)
+    cache.k.view(torch.uint8).zero_()
+    gen = _gen(6)
+    mean = torch.zeros(heads, D, dtype=torch.float64, device="cuda")
+    lean = torch.rand(heads, 1, D, generator=gen, device="cuda") * 0.25
+    used = torch.zeros(batch.num_pages, dtype=torch.float64)
+    used[batch.table[0].long()] = 1.0
+    for some in torch.arange(batch.num_pages, device="cuda").split(64):
+        x = torch.rand(len(some), heads, page, D, generator=gen, device="cuda") * 0.7 + 1.0 + lean
+        if fmt == "plain":
+            cache.v[some] = x.to(BF16)
+            x = x.to(BF16).double()
+        else:
+            code, unit = su.quantised(x, fmt)
+            cache.v.view(torch.uint8)[some] = code.to(cache.v.dtype).view(torch.uint8)
+            cache.v_scale[some], cache.k_scale[some] = unit.float(), 1.0
+            x = code * unit[..., None]
+        mean += torch.einsum("phkd,p->hd", x, used[some.cpu()].cuda())
+    mean = (mean / length).repeat_interleave(H // heads, 0)
+    offsets = torch.arange(0, n * copies + 1, n, dtype=torch.int32, device="cuda")          # (the sequences share their pages)
+    lengths, pages = torch.full((copies,), length, dtype=torch.int32, device="cuda"), batch.pages.expand(copies, -1).contiguous()
+    q = _normal(gen, n * copies, H, D, dtype=BF16)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, offsets, lengths, pages, n * copies, copies, H, causal=False)
+    # Half a step of the result (2^-8 where it is from 1 to 2), and on top of it: a value times its scale in fp16 (int8, the scale too: 2^-11 each, to nearest, 2^-17 on the average of these values); 2048 steps of
+    # 2^-23 in an accumulator, 2^-12; sums and weights in fp32.  Values below 2.
+    assert float((out.double() - mean).abs().max()) <= 2.0 ** -8 + 2.0 * (2.0 ** -12 + 2.0 ** -14)
