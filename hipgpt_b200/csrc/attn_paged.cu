@@ -201,9 +201,10 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
 
     // sites: 11 keys or values landed, 12 place free
     auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
-        if (mbar_test(bar, parity)) return true;
+        const bool over = a.expire != 0 && expires_now(a.expire, site);
+        if (!over && mbar_test(bar, parity)) return true;
         if (!abort_flag) {
-            if (mbar_wait(bar, parity)) return true;
+            if (!over && mbar_wait(bar, parity)) return true;
             abort_flag = 1;
             atomicCAS(&g_rows_status, 0, site);
             linger();
@@ -593,7 +594,6 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
         // ---- the tile's end ---------------------------------------------------------------------------------------
         const int part = run.part();
         if (part >= 0 && (part & 1)) cut = run.cut();
-        const bool store = !abort_flag;
         float *dst = part < 0 ? nullptr : a.parts + (size_t)part * C::ROWS * (DP + 2);
         // columns of TILES' tile c * EV + e: values (2 t4 + 8 c) EV + e and (2 t4 + 1 + 8 c) EV + e
         if constexpr (!SPLITROWS) {
@@ -639,6 +639,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 put(warp);                           // (a thread reads and writes the same places)
             }
             meet();
+            const bool store = !abort_flag;          // (behind the meeting: what a warp whose wait ran out has left there is in everybody's rows)
             for (int r = warp; r < 16; r += kWarps) {
                 const int row = row0 + r;
                 if (row >= rows) break;
@@ -668,6 +669,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 }
             }
         } else {
+            const bool store = !abort_flag;
             bool wild = false;
 #pragma unroll
             for (int mt = 0; mt < C::MT; ++mt)
@@ -769,9 +771,10 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
     dependents_may_start();
 
     auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
-        if (mbar_test(bar, parity)) return true;
+        const bool over = a.expire != 0 && expires_now(a.expire, site);
+        if (!over && mbar_test(bar, parity)) return true;
         if (!abort_flag) {
-            if (mbar_wait(bar, parity)) return true;
+            if (!over && mbar_wait(bar, parity)) return true;
             abort_flag = 1;
             atomicCAS(&g_rows_status, 0, site);
             linger();
@@ -1131,7 +1134,6 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
         // ---- the tile's end: the warps' sums by way of shared memory, two rows a warp --------------------------------------
         const int part = run.part();
         if (part >= 0 && (part & 1)) cut = run.cut();
-        const bool store = !abort_flag;
         float *dst = part < 0 ? nullptr : a.parts + (size_t)part * 8 * (DP + 2);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -1141,6 +1143,7 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
         }
         put();
         meet();
+        const bool store = !abort_flag;              // (behind the meeting: what a warp whose wait ran out has left there is in everybody's rows)
         for (int r = warp; r < 8; r += kWarps) {
             const int row = row0 + r;
             if (row >= rows) break;
@@ -1262,7 +1265,6 @@ int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
     const long long room = (long long)a.c.most_pages << a.c.shift;
     const long long most = (room + C::UNIT - 1) / C::UNIT > 1 ? (room + C::UNIT - 1) / C::UNIT : 1;      // units of a tile
     const long long tiles = ((long long)a.c.T * a.group / C::ROWS + (a.c.T < a.c.B ? a.c.T : a.c.B)) * a.c.heads;
-    a.least = 1;
     if (tiles < (1LL << 40) / most && tiles * most < grid) grid = (int)(tiles * most);
     const bool cuts = most > 1;
     StreamWorkspace::Lease ws;
@@ -1294,6 +1296,7 @@ int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
         e = launch_overlapped(paged_cut_kernel<C>, dim3((unsigned)(pieces / C::kSlotBytes)), dim3(128), 0, st, a.c, a.cut_k, a.cut_v, a.cut_units);
         if (e != cudaSuccess) return fail(HIPGPT_ERR_CUDA, "paged_cut_kernel: %s", cudaGetErrorString(e));
     }
+    a.expire = take_expiry(1000);
     e = launch_overlapped(kern, dim3((unsigned)grid), dim3(kThreads), C::kSmem, st, a);
     if (e == cudaSuccess && cuts) e = launch_overlapped(paged_join_kernel<T, FMT, C::ROWS, DP>, dim3((unsigned)grid, (unsigned)(C::ROWS + 15) / 16), dim3(256), 0, st, a);
     return e == cudaSuccess ? check_launch("paged attention") : fail(HIPGPT_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
@@ -1371,7 +1374,6 @@ extern "C" int hipgpt_paged_attention(const hipgpt_paged_cache *cache, const hip
     a.q_stride = q_stride; a.out_stride = out_stride;
     a.group = H / cache->heads;
     a.causal = causal != 0;
-    a.scale = scale;
     a.cscale = scale * kLog2e;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return cache->type == HIPGPT_TYPE_F32 ? launch_paged<float>(cache->format, a, st) : launch_paged<__nv_bfloat16>(cache->format, a, st);

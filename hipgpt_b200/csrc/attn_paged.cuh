@@ -17,8 +17,8 @@ struct AttnArgs {
     void *out;
     long long q_stride, out_stride;
     int group, causal;
-    float scale, cscale;                 // and scale * log2 e
-    int least;                           // units a block takes at least
+    float cscale;                        // scale * log2 e
+    int expire;                          // test hook (attn_paged.cu's kernels)
     float *parts;                        // [2 * blocks][ROWS][DP + 2]: sums, then reference maximum (log2 domain) and sum of exponentials of each row
     int4 *cuts;                          // [blocks]: the tile that begins here and goes on: sequence, head, tile, last block (w < 0: none)
     int *whole;                          // [blocks]: 0 where a wait ran out
@@ -112,7 +112,7 @@ struct Run {
         const long long total = block_sum<THREADS>(mine, shared);
         // (64-bit divisions take a hundred instructions)
         per = total < 1 << 30 ? (int)(((unsigned)total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
-        per = max(per, (long long)a.least);
+        per = max(per, 1LL);
         u = start = (long long)blockIdx.x * per;
         end = min(total, u + per);
         if (u >= end) return false;

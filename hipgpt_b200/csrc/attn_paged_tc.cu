@@ -896,7 +896,6 @@ int launch_tc(AttnArgs a, cudaStream_t st)
     const long long most = (room + kKeys - 1) / kKeys > 1 ? (room + kKeys - 1) / kKeys : 1;
     const long long tiles = ((long long)a.c.T * a.group / kRows + (a.c.T < a.c.B ? a.c.T : a.c.B)) * a.c.heads;
     int grid = sms;
-    a.least = 1;
     if (tiles < (1LL << 40) / most && tiles * most < grid) grid = (int)(tiles * most);
     const bool cuts = most > 1;
     StreamWorkspace::Lease ws;

@@ -461,7 +461,7 @@ int hipgpt_shard_range(int B, int world, int rank, int *b_begin, int *b_end)
 int hipgpt_debug_expire_wait(int code, int block)
 {
     const int family = code / 100 * 100, site = code % 100;
-    if ((family != 500 && family != 600 && family != 700 && family != 1000) || site == 0 || block < 0 || block >= 1 << 22) return fail(HIPGPT_ERR_BAD_ARG, "no wait has code %d, or block %d", code, block);
+    if ((family != 500 && family != 600 && family != 700 && family != 1000) || site == 0 || (family == 1000 && site > 12) || block < 0 || block >= 1 << 22) return fail(HIPGPT_ERR_BAD_ARG, "no wait has code %d, or block %d", code, block);
     g_expire_family = family;
     g_expire = block << 8 | site;
     return HIPGPT_OK;

@@ -524,7 +524,7 @@ HIPGPT_API int hipgpt_set_full_range(int on);
  *       arrives, with a limit of `limit_cycles` SM cycles (at most 2^24, a few milliseconds).  Afterwards
  *       hipgpt_kernel_status() reports 907 and d_canary[0..n) is untouched.
  *   hipgpt_debug_expire_wait  in the calling thread's next call of a tensor-core projection (code 501 ... 504) or of a tensor-core
- *       backward (601 ... 627) or loss, forward or backward (701 ... 704), or of attention of many rows over a paged cache (1001 ... 1010), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
+ *       backward (601 ... 627) or loss, forward or backward (701 ... 704), or of attention over a paged cache (1001 ... 1010 in bf16 with many rows a sequence, 1011 and 1012 otherwise), the wait that hipgpt_kernel_status reports with this code runs out at once in block `block` of
  *       each of the call's launches that has it, if it has to wait at all.
  *   hipgpt_gpt_debug_stall_barrier  makes the NEXT hipgpt_gpt_generate call give up: in the persistent mode it starts with a
  *       grid-barrier counter that cannot complete, and every block gives up at its first barrier; by clusters the first block's

@@ -170,3 +170,8 @@ def test_paged_caches_that_are_refused():
             serving.PagedCache(**full)
     with pytest.raises(ValueError):
         serving.PagedCache(2, 16, 2, 32, k=torch.zeros(2, 2, 16, 32), v=torch.zeros(2, 2, 16, 32))
+
+
+def test_waits_that_no_kernel_has():
+    for code in (1000, 1013, 1099, 1100):
+        assert _capi.lib().hipgpt_debug_expire_wait(code, 0) == _capi.ERR_BAD_ARG

@@ -210,3 +210,32 @@ def test_sums_over_a_million_keys(fmt, n, heads, H, D, copies):
     # Half a step of the result (2^-8 where it is from 1 to 2), and on top of it: a value times its scale in fp16 (int8, the scale too: 2^-11 each, to nearest, 2^-17 on the average of these values); 2048 steps of
     # 2^-23 in an accumulator, 2^-12; sums and weights in fp32.  Values below 2.
     assert float((out.double() - mean).abs().max()) <= 2.0 ** -8 + 2.0 * (2.0 ** -12 + 2.0 ** -14)
+
+
+# ---- waits that run out ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,fmt,seqs,H", [(BF16, "e4m3", [(1, 150000), (1, 60000), (1, 200)], 8), (F32, "plain", [(1, 90000), (1, 9000), (1, 200)], 8), (BF16, "plain", [(10, 80000), (8, 900)], 4),
+                                              (F32, "int8", [(100, 20000), (60, 900)], 4), (F32, "plain", [(300, 5000), (200, 900)], 4)], ids=["tokens", "tokens32", "some", "many32", "cut"])
+@pytest.mark.parametrize("code,block", [(1011, 0), (1011, 3), (1012, 1), (1012, 2)])
+def test_an_expired_wait_of_few_rows_and_of_fp32(dtype, fmt, seqs, H, code, block):
+    """Every row of the result is as ever, or nothing was stored there; the next call is as ever."""
+    batch, heads, D = Batch(seqs, 64, seed=3), 2, 128
+    cache, k, v = su.filled_cache(batch, heads, D, dtype, fmt)
+    q = _normal(_gen(5), batch.T, H, D, dtype=dtype)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, *batch.args, H)
+    status = 0
+    for _ in range(40):
+        got = torch.full_like(out, -7.0)
+        _capi.check(_capi.lib().hipgpt_debug_expire_wait(code, block))
+        serving.paged_attention(cache, q, got, *batch.args, H)
+        torch.cuda.synchronize()
+        status = _status()
+        same, left = (got == out).all(-1), (got == -7.0).all(-1)
+        assert bool((same | left).all())
+        if status:
+            break
+    assert status == code and _status() == 0
+    assert bool(left.any()) and bool(same.any())
+    serving.paged_attention(cache, q, got, *batch.args, H)
+    assert torch.equal(got, out)
