@@ -159,16 +159,19 @@ static int fetch_status_words(int *status)
     if (rc == HIPGPT_OK) rc = bf16_status_fetch(&b);
     if (rc == HIPGPT_OK) rc = tc16_status_fetch(&d);
     if (rc == HIPGPT_OK) rc = head_status_fetch(&h);
-    int pr = 0, gm = 0, bw = 0, ls = 0, em = 0, pg = 0;
+    int pr = 0, gm = 0, bw = 0, bh = 0, ls = 0, em = 0, pg = 0, pw = 0;
     if (rc == HIPGPT_OK) rc = probe_status_fetch(&pr);
     if (rc == HIPGPT_OK) rc = mha_backward_tc_status_fetch(&bw);
-    if (rc == HIPGPT_OK && !bw) rc = mha_backward_head_status_fetch(&bw);
+    if (rc == HIPGPT_OK) rc = mha_backward_head_status_fetch(&bh);
     if (rc == HIPGPT_OK) rc = gemm_tc_status_fetch(&gm);
     if (rc == HIPGPT_OK) rc = loss_status_fetch(&ls);
     if (rc == HIPGPT_OK) rc = embedding_status_fetch(&em);
     if (rc == HIPGPT_OK) rc = paged_status_fetch(&pg);
-    if (rc == HIPGPT_OK && !pg) rc = paged_rows_status_fetch(&pg);
+    if (rc == HIPGPT_OK) rc = paged_rows_status_fetch(&pw);
     if (rc != HIPGPT_OK) return rc;
+    // (all words have been cleared: a second one must not wait for the next call)
+    bw = bw ? bw : bh;
+    pg = pg ? pg : pw;
     *status = a ? a : (b ? 100 + b : (d ? 300 + d : (h ? 400 + h : (gm ? 500 + gm : (bw ? 600 + bw : (ls ? 700 + ls : (em ? 800 + em : (pr ? 900 + pr : (pg ? 1000 + pg : 0)))))))));
     return HIPGPT_OK;
 }

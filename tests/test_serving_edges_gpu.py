@@ -239,3 +239,16 @@ def test_an_expired_wait_of_few_rows_and_of_fp32(dtype, fmt, seqs, H, code, bloc
     assert bool(left.any()) and bool(same.any())
     serving.paged_attention(cache, q, got, *batch.args, H)
     assert torch.equal(got, out)
+
+
+def test_the_status_is_of_launches_since_the_last_time():
+    """Two kernels of attention gave up: the status says so once."""
+    lib = _capi.lib()
+    for dtype, code in ((BF16, 1003), (F32, 1011)):
+        batch = Batch([(300, 3000)], 64, seed=3)
+        cache, _, _ = su.filled_cache(batch, 2, 64, dtype, "plain")
+        q = _normal(_gen(5), batch.T, 4, 64, dtype=dtype)
+        _capi.check(lib.hipgpt_debug_expire_wait(code, 0))
+        serving.paged_attention(cache, q, torch.empty_like(q), *batch.args, 4)
+    assert _status() in (1003, 1011)
+    assert _status() == 0
