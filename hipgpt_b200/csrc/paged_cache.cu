@@ -35,9 +35,9 @@ __device__ __forceinline__ void places_of(const MoveArgs &a, int t0, long long (
         if (some < min(kThreads, a.c.B - b0)) break;
     }
     if ((int)threadIdx.x < a.tokens) {
-        const int t = t0 + threadIdx.x;
         long long place = -2;
-        if (t < a.c.T) {
+        if ((int)threadIdx.x < a.c.T - t0) {         // (t0 + 31 may be beyond an int)
+            const int t = t0 + threadIdx.x;
             int b = below;
             while (b < a.c.B && __ldg(a.c.offsets + b + 1) <= t) ++b;
             if (b < a.c.B) {
@@ -135,10 +135,10 @@ cache_write_kernel(const MoveArgs a)
     // (every thread of the warp takes part in the shuffles: those without a row have zeros)
     auto fetch = [&](int i0) {
         row_at(a, i0 >> a.log_lanes, t, head);
-        const bool here = i0 < all && t0 + t < a.c.T;
+        const bool here = i0 < all && t < a.c.T - t0;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            const T *src = static_cast<const T *>(w ? a.v : a.k) + (t0 + t) * (w ? a.v_stride : a.k_stride) + head * D;
+            const T *src = static_cast<const T *>(w ? a.v : a.k) + ((long long)t0 + t) * (w ? a.v_stride : a.k_stride) + head * D;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
                 const int d = (lane + c * a.lanes) * N;

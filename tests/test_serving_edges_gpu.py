@@ -252,3 +252,21 @@ def test_the_status_is_of_launches_since_the_last_time():
         serving.paged_attention(cache, q, torch.empty_like(q), *batch.args, 4)
     assert _status() in (1003, 1011)
     assert _status() == 0
+
+
+# ---- sizes ----------------------------------------------------------------------------------------------------------------
+
+def test_as_many_tokens_as_an_int_holds():
+    """The last block of tokens begins less than its own length before the largest int; the last tokens alone have a place."""
+    torch.cuda.empty_cache()
+    T, D = (1 << 31) - 5, 16
+    if torch.cuda.mem_get_info()[0] < T * D * 2 + (8 << 30):
+        pytest.skip("64 GB of rows do not fit beside what others hold")
+    x = torch.empty(T, 1, D, device="cuda", dtype=BF16)
+    x[-3:] = _normal(_gen(4), 3, 1, D, dtype=BF16)
+    cache = serving.PagedCache(1, 16, 1, D, dtype=BF16, format="plain")
+    offsets, lengths, pages = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, T], [3], [[0]]))
+    serving.cache_write(cache, x, x, offsets, lengths, pages, T, 1)
+    assert torch.equal(cache.k[0, 0, :3], x[-3:, 0]) and torch.equal(cache.v[0, 0, :3], x[-3:, 0])
+    del x
+    torch.cuda.empty_cache()
