@@ -285,7 +285,9 @@ void *rows_at(Tensors &t, int i, const char *name, at::ScalarType type, int64_t 
         rows = rows && (x.size(d) == 1 || x.stride(d) == inner);
         inner *= x.size(d);
     }
-    if (x.dim() >= 2 && !(inner == width || (whole && (x.size(-1) == D || x.size(-1) == width)))) PyErr_Format(PyExc_ValueError, "%s has rows of %lld values, %lld are expected", name, (long long)inner, (long long)width);
+    // rows as one, or with the tokens in more dimensions than one: [...][width], [...][H][D], or heads one behind the other [T * H][D]
+    const bool heads = whole && x.dim() >= 2 && x.size(-1) == D && (x.dim() == 2 || x.size(-2) == H);
+    if (x.dim() >= 2 && !(inner == width || heads || (whole && x.size(-1) == width))) PyErr_Format(PyExc_ValueError, "%s has rows of %lld values, %lld are expected", name, (long long)inner, (long long)width);
     else if (!(x.is_cuda() && x.scalar_type() == type && (whole || rows))) PyErr_Format(PyExc_ValueError, "%s: expected a CUDA %s tensor, contiguous but for its first dimension", name, kind);
     else if (x.get_device() != c10::cuda::current_device()) PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, another is the current device", name, (int)x.get_device());
     else if (x.numel() < T * width) PyErr_Format(PyExc_ValueError, "%s holds %lld values, %lld are needed", name, (long long)x.numel(), (long long)(T * width));

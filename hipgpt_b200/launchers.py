@@ -93,7 +93,9 @@ def _rows_of(name, t, dtype, T, H, D):
     for n in t.shape[1:]:
         inner *= n
     whole = t.is_contiguous()
-    if t.dim() >= 2 and not (inner == width or (whole and t.shape[-1] in (D, width))):
+    # rows as one, or with the tokens in more dimensions than one: [...][width], [...][H][D], or heads one behind the other [T * H][D]
+    heads = whole and t.dim() >= 2 and t.shape[-1] == D and (t.dim() == 2 or t.shape[-2] == H)
+    if t.dim() >= 2 and not (inner == width or heads or (whole and t.shape[-1] == width)):
         raise ValueError(f"{name} has rows of {inner} values, {width} are expected")
     if not (t.is_cuda and t.dtype == dtype and (whole or (t.dim() >= 2 and t.shape[0] and t[0].is_contiguous()))):
         raise ValueError(f"{name}: expected a CUDA {dtype} tensor, contiguous but for its first dimension")

@@ -175,3 +175,20 @@ def test_paged_caches_that_are_refused():
 def test_waits_that_no_kernel_has():
     for code in (1000, 1013, 1099, 1100):
         assert _capi.lib().hipgpt_debug_expire_wait(code, 0) == _capi.ERR_BAD_ARG
+
+
+def test_rows_of_another_number_of_heads(calls):
+    """A tensor of more heads than the call says is no tensor of its rows, although its heads have the right width."""
+    i, p, c = torch.zeros(3, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32), _fake_cache()
+    for shape in ((8, 5, 32), (2, 4, 6, 32), (8, 8, 32)):
+        x = torch.zeros(shape)
+        with pytest.raises(ValueError, match="q has rows of"):
+            calls.paged_attention(c, x, x, i, i, p, 8, 2, 4)
+        with pytest.raises(ValueError, match="x has rows of"):
+            calls.rotary(x, i, i, x, 8, 4, 32, 32)
+        with pytest.raises(ValueError, match="k has rows of"):
+            calls.cache_write(c, x, x, i, i, p, 8, 2)
+    for shape in ((8, 4, 32), (2, 4, 4, 32), (8, 128), (2, 4, 128), (32, 32), (1024,)):         # what their rows may be told as; CPU tensors are refused as such
+        x = torch.zeros(shape)
+        with pytest.raises(ValueError, match="q: expected a CUDA"):
+            calls.paged_attention(c, x, x, i, i, p, 8, 2, 4)
