@@ -49,7 +49,10 @@ def rotary(x, positions, words, out, T: int, H: int, D: int, R: int, *, interlea
 
 class PagedCache:
     """Keys and values in pages: k, v [num_pages, heads, page_size, head_dim] of `dtype` (format "plain"), float8_e4m3fn ("e4m3") or int8 ("int8"), the latter two with scales
-    k_scale, v_scale [num_pages, heads, page_size] float32.  What is not given is allocated (not set) on the current device."""
+    k_scale, v_scale [num_pages, heads, page_size] float32.  What is not given is allocated (not set) on the current device.  The arrays are a cache's for good: another needs another PagedCache."""
+
+    k, v = property(lambda self: self._arrays[0]), property(lambda self: self._arrays[1])
+    k_scale, v_scale = property(lambda self: self._arrays[2]), property(lambda self: self._arrays[3])
 
     def __init__(self, num_pages: int, page_size: int, heads: int, head_dim: int, *, dtype=torch.float32, format: str = "plain", k=None, v=None, k_scale=None, v_scale=None):
         num_pages, page_size, heads, head_dim = launchers._sizes(num_pages, page_size, heads, head_dim)
@@ -61,7 +64,7 @@ class PagedCache:
             raise ValueError(f"bad size: {num_pages} pages of {page_size} tokens, {heads} heads of {head_dim} values (pages hold a power of two from 16 to 1024 tokens)")
         shape = (num_pages, heads, page_size, head_dim)
         held = {"plain": dtype, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}[format]
-        device = next((t.device for t in (k, v, k_scale, v_scale) if t is not None), None)
+        device = next((t.device for t in (k, v, k_scale, v_scale) if isinstance(t, torch.Tensor)), None)
 
         def array(name, t, shape, dtype):
             if t is None:
@@ -70,15 +73,13 @@ class PagedCache:
                 raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor of shape {list(shape)}, all of a cache on one device")
             return t
 
-        self.k, self.v = array("k", k, shape, held), array("v", v, shape, held)
-        if format == "plain":
-            if k_scale is not None or v_scale is not None:
-                raise ValueError("a plain cache has no scales")
-            self.k_scale = self.v_scale = None
-        else:
-            self.k_scale, self.v_scale = array("k_scale", k_scale, shape[:3], torch.float32), array("v_scale", v_scale, shape[:3], torch.float32)
+        if format == "plain" and (k_scale is not None or v_scale is not None):
+            raise ValueError("a plain cache has no scales")
+        self._arrays = array("k", k, shape, held), array("v", v, shape, held), None, None
+        if format != "plain":
+            self._arrays = *self._arrays[:2], array("k_scale", k_scale, shape[:3], torch.float32), array("v_scale", v_scale, shape[:3], torch.float32)
         self.num_pages, self.page_size, self.heads, self.head_dim, self.dtype, self.format = num_pages, page_size, heads, head_dim, dtype, format
-        at = [t.data_ptr() if t is not None else None for t in (self.k, self.v, self.k_scale, self.v_scale)]
+        at = [t.data_ptr() if t is not None else None for t in self._arrays]
         self._struct = launchers._PagedCache(*at, num_pages, page_size, heads, head_dim, launchers._TYPES[dtype], FORMATS[format])
         self._address, self._device = C.addressof(self._struct), self.k.device.index
 

@@ -192,3 +192,15 @@ def test_rows_of_another_number_of_heads(calls):
         x = torch.zeros(shape)
         with pytest.raises(ValueError, match="q: expected a CUDA"):
             calls.paged_attention(c, x, x, i, i, p, 8, 2, 4)
+
+
+def test_a_caches_arrays_stay_its_own():
+    """What the library writes to is what the handle shows and keeps."""
+    c = _fake_cache()
+    c._arrays = tuple(torch.zeros(1) for _ in range(4))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, torch.zeros(1))
+    for bad in ([1.0], 7, "x"):
+        with pytest.raises(ValueError, match="k: expected"):
+            serving.PagedCache(2, 16, 2, 32, k=bad, v=torch.zeros(2, 2, 16, 32))
