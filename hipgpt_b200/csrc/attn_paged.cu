@@ -249,7 +249,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                if (lane == 0) q_unit[r] = pow2_scale(most);
+                if (lane == 0) q_unit[r] = row_unit(most);
             }
             meet();
         }
@@ -291,8 +291,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 const int rr = mt * 16 + g + 8 * r;
                 limit[mt][r] = wrow + rr < rows ? limit_of(a, s, wrow + rr) : 0;
                 factor[mt][r] = a.cscale;
-                // (a masked score times 0 would be NaN)
-                if constexpr (HALF) factor[mt][r] = fmaxf(a.cscale * pow2_inverse(q_unit[wrow - row0 + rr]), 1.17549435e-38f);
+                if constexpr (HALF) factor[mt][r] = a.cscale * pow2_inverse(q_unit[wrow - row0 + rr]);
             }
         const int least_limit = wrow < rows ? limit_of(a, s, wrow) : 0;
         const int keys = tile_keys<C::ROWS>(a, s, w.tile);
@@ -442,8 +441,9 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                         for (int e = 0; e < 4; ++e) {
                             float x = z[mt][j][e];
                             if constexpr (C::NQ > 1) x += zc[mt][j][e];
-                            if constexpr (C::CODED) x *= (e & 1) ? ks2[j].y : ks2[j].x;
-                            z[mt][j][e] = x * factor[mt][e >> 1];
+                            // (the two factors first: small queries and large keys, or the other way round, must not pass fp32's range on the way)
+                            if constexpr (C::CODED) z[mt][j][e] = x * (((e & 1) ? ks2[j].y : ks2[j].x) * factor[mt][e >> 1]);
+                            else z[mt][j][e] = x * factor[mt][e >> 1];
                         }
                     if (masked) {
 #pragma unroll
@@ -816,7 +816,7 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                if (lane == 0) q_unit[r] = pow2_scale(most);
+                if (lane == 0) q_unit[r] = row_unit(most);
             }
             meet();
         }
@@ -849,7 +849,7 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
             const int row = row0 + 2 * t4 + r;
             limit[r] = row < rows ? limit_of(a, s, row) : 0;
             factor[r] = a.cscale;
-            if constexpr (HALF) factor[r] = fmaxf(a.cscale * pow2_inverse(q_unit[2 * t4 + r]), 1.17549435e-38f);       // (a masked score times 0 would be NaN)
+            if constexpr (HALF) factor[r] = a.cscale * pow2_inverse(q_unit[2 * t4 + r]);
         }
         const int least_limit = limit_of(a, s, row0), keys = tile_keys<8>(a, s, w.tile);
         int unit = -126;                             // codes: o is divided by 2^unit, which follows the largest scale of the values
@@ -1005,8 +1005,9 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
                 for (int e = 0; e < 4; ++e) {
                     float x = z[j][e];
                     if constexpr (C::NQ > 1) x += zc[j][e];
-                    if constexpr (C::CODED) x *= ks[j][e >> 1];
-                    z[j][e] = x * factor[e & 1];
+                    // (the two factors first: small queries and large keys, or the other way round, must not pass fp32's range on the way)
+                    if constexpr (C::CODED) z[j][e] = x * (ks[j][e >> 1] * factor[e & 1]);
+                    else z[j][e] = x * factor[e & 1];
                 }
             auto seen = [&](int j, int e) { return p0 + 16 * j + 8 * (e >> 1) + g < limit[e & 1] && (there >> j & 1); };
             if (masked) {

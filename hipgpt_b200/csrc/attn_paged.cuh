@@ -26,6 +26,9 @@ struct AttnArgs {
     int cut_units, cut_unit;             // keys a place (0: keys as they lie in the cache)
 };
 
+// The power of two that brings the largest value of a row of q to [2^14, 2^15) (2^126 at most); 1 for zeros, infinities and NaN
+__device__ __forceinline__ float row_unit(float most) { return most <= 3.0e38f ? pow2_scale(most) : most <= 3.402823466e38f ? 0x1p-113f : 1.0f; }
+
 // One tile's run of units in a block
 struct Tile {
     int b, head, tile, units;            // units of the whole tile

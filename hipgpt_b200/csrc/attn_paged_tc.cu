@@ -61,7 +61,7 @@ template <int FMT> constexpr int kUp = FMT == HIPGPT_CACHE_E4M3 ? 6 : 7;
 // Codes that were widened before the call's attention: rows of fp16 of each sequence and head, one behind the other
 struct Wide {
     void *k, *v;                         // [sequence][head][room][D]
-    float *scale;                        // [sequence][head][room]: int8, the scales of the keys
+    float *scale;                        // [sequence][head][room]: int8, the scales of the keys over their 64's power of two
     float *k_unit, *v_exp;               // [sequence][head][room / 64]
     int room;                            // keys, a multiple of 128
 };
@@ -90,7 +90,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ uint64_t k_full[kStages], v_full[kStages], k_free[kStages], v_free[kStages], q_full[2], s_full[2], p_full[2][2], o_done[2];
     __shared__ uint64_t landed[WIDENS ? kSlots : kStages], raw_free[kSlots];
     __shared__ __align__(16) float scale_s[WIDENS ? kSlots : 1][kHalf];
-    __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys];       // int8: the scales of the keys
+    __shared__ __align__(16) float ks_s[SCALED ? kTables : 1][kKeys];       // int8: the scales of the keys, over their 64's power of two
     __shared__ float k_unit[kTables][2], v_exp[kTables][2];          // codes: the power of two that each 64 keys of a tile were divided by, the exponent of that of the values
     __shared__ float q_unit[CODED ? 2 * 128 : 1];                    // and that of a row of Q
     __shared__ uint32_t there_s[kTables];            // whether each 16 keys of a tile have a page
@@ -296,34 +296,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             raw[i] = ok ? *reinterpret_cast<const uint4 *>(raw_s + sl * C::kSlot + key * D + c * 16) : make_uint4(0u, 0u, 0u, 0u);
                             scale[i] = ok ? scale_s[sl][key] : 0.0f;
                         }
-                        int e = 0;
-                        float key_scale = 0.0f;
-                        if (!SCALED || which) {
-                            uint32_t most = 0;
+                        uint32_t most = 0;
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t bits = holds(lane + 32 * i) ? __float_as_uint(scale_s[sl][lane + 32 * i]) : 0u;
-                                most = max(most, bits < 0x7F800000u ? bits : 0u);
-                            }
-                            most = __reduce_max_sync(0xffffffffu, most);
-                            e = (int)(most >> 23) - 127 - kUp<FMT>;
-                            if (which) {
-                                // Values far below those before them need not fill fp16, and all of one size with P: a tile of zeros must not carry the sum of exponentials out of fp32
-                                e = max(max(e, v_most - 20), -96);
-                                v_most = max(v_most, e);
-                            }
-                            e = min(max(e, -126), 120);
-                        } else if (pt < kHalf) {
-                            key_scale = holds(pt) ? scale_s[sl][pt] : 0.0f;
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t bits = holds(lane + 32 * i) ? __float_as_uint(scale_s[sl][lane + 32 * i]) : 0u;
+                            most = max(most, bits < 0x7F800000u ? bits : 0u);
                         }
+                        most = __reduce_max_sync(0xffffffffu, most);
+                        int e = (int)(most >> 23) - 127 - kUp<FMT>;
+                        if (which) {
+                            // Values far below those before them need not fill fp16, and all of one size with P: a tile of zeros must not carry the sum of exponentials out of fp32
+                            e = max(max(e, v_most - 20), -96);
+                            v_most = max(v_most, e);
+                        }
+                        e = min(max(e, -126), 120);
+                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                        float key_scale = 0.0f;
+                        if (SCALED && !which && pt < kHalf) key_scale = holds(pt) ? scale_s[sl][pt] * down : 0.0f;
                         if (n >= kStages && (part & 1) == 0) wait(which ? &v_free[st] : &k_free[st], ph ^ 1, which ? 8 : 7);
                         if (pt == 0) {
                             if (which) v_exp[n % kTables][part & 1] = (float)e;
-                            else k_unit[n % kTables][part & 1] = SCALED ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
+                            else k_unit[n % kTables][part & 1] = __uint_as_float((uint32_t)(127 + e) << 23);
                         }
                         if constexpr (SCALED)
                             if (which == 0 && pt < kHalf) ks_s[n % kTables][base_key + pt] = key_scale;
-                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
                         uint8_t *tile = (which ? v_s : k_s) + st * C::kTile + (c0 / 8) * (kKeys * 128) + base_key * 128;
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
@@ -478,7 +474,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
 #pragma unroll
                         for (int o = 1; o < CH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        const float up = pow2_scale(most);
+                        const float up = row_unit(most);
                         x = make_uint4(half2_of(v[0] * up, v[1] * up), half2_of(v[2] * up, v[3] * up), half2_of(v[4] * up, v[5] * up), half2_of(v[6] * up, v[7] * up));
                         if (c == 0) q_unit[half * 128 + quad * 32 + rr] = pow2_inverse(up);
                     }
@@ -769,14 +765,15 @@ paged_widen_kernel(const PagedView c, const Wide wide)
         }
         most = __reduce_max_sync(0xffffffffu, most);
         // (values: a tile of zeros must not carry the sum of exponentials out of fp32)
-        const int e = SCALED && !which ? 0 : min(max((int)(most >> 23) - 127 - kUp<FMT>, which ? -96 : -126), 120);
+        const int e = min(max((int)(most >> 23) - 127 - kUp<FMT>, which ? -96 : -126), 120);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             scale_s[which][lane + 32 * i] = SCALED && !which ? 1.0f : f[i];
-            if (SCALED && !which) wide.scale[(size_t)bh * wide.room + p0 + lane + 32 * i] = f[i];
+            if (SCALED && !which) wide.scale[(size_t)bh * wide.room + p0 + lane + 32 * i] = f[i] * down;
         }
         if (lane == 0) {
-            down_s[which] = __uint_as_float((uint32_t)(127 - e) << 23);
+            down_s[which] = SCALED && !which ? 1.0f : down;
             if (which) wide.v_exp[(size_t)bh * groups + g] = (float)e;
             else wide.k_unit[(size_t)bh * groups + g] = __uint_as_float((uint32_t)(127 + e) << 23);
         }

@@ -270,3 +270,45 @@ def test_as_many_tokens_as_an_int_holds():
     assert torch.equal(cache.k[0, 0, :3], x[-3:, 0]) and torch.equal(cache.v[0, 0, :3], x[-3:, 0])
     del x
     torch.cuda.empty_cache()
+
+
+# ---- powers of two far from one another ----------------------------------------------------------------------------------
+
+CODED = [(BF16, [(1, 900), (4, 500)], 4), (F32, [(1, 900), (4, 500)], 4), (BF16, [(20, 1700)], 4), (F32, [(20, 1700)], 4), (F32, [(70, 900)], 4), (BF16, [(300, 2000), (70, 80)], 4), (BF16, [(1000, 4000), (700, 800)], 8),
+         (BF16, [(40, 20000)], 4)]
+CODED_IDS = ["tokens", "tokens32", "some", "some32", "many32", "tcgen05", "widened", "parts"]
+
+
+def _one(dtype, seqs, H, fmt, wild, spread=1.0, scale=None, turn=None):
+    batch, heads, D = Batch(seqs, 64, seed=13), 2, 64
+    cache, k, v = su.filled_cache(batch, heads, D, dtype, fmt, wild=wild)
+    q = _normal(_gen(5), batch.T, H, D, dtype=dtype, scale=spread)
+    if turn is not None:
+        turn(q)
+    out = torch.zeros_like(q)
+    serving.paged_attention(cache, q, out, *batch.args, H, scale=scale)
+    want, bound, _ = su.attention(batch, k, v, q, H, True, float(torch.tensor(D ** -0.5 if scale is None else scale)), dtype, fmt)
+    within(out, want, bound)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype,seqs,H", CODED, ids=CODED_IDS)
+def test_queries_and_keys_at_both_ends_of_the_range(dtype, seqs, H, fmt):
+    def large(name, x):
+        if name == "k":
+            x *= 2.0 ** 115
+    _one(dtype, seqs, H, fmt, large, spread=2.0 ** -115)
+
+    def small(name, x):
+        if name == "k":
+            x *= 2.0 ** -100
+    _one(dtype, seqs, H, fmt, small, spread=2.0 ** 100)
+
+    def smaller(name, x):
+        if name == "k":
+            x *= 1e-28
+
+    def largest(q):
+        q[-2:, :, 3], q[-1:, :, 7] = 3.3e38, -3.2e38
+    _one(dtype, seqs, H, fmt, smaller, scale=1e-10, turn=largest)
