@@ -57,6 +57,8 @@ __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, int si
 
 // The largest scale of 64 keys goes to [2^k, 2^(k + 1)) in fp16: 128 * 2^8 and 448 * 2^7 are still numbers there, and rows whose scale is 2^-21 of it keep their digits
 template <int FMT> constexpr int kUp = FMT == HIPGPT_CACHE_E4M3 ? 6 : 7;
+// ... and values whose own power of two is 2^-kFar of those before them take 2^-kFar of that: they need not fill fp16, and the exponents that P takes from tile to tile stay near each other
+constexpr int kFar = 20;
 
 // Codes that were widened before the call's attention: rows of fp16 of each sequence and head, one behind the other
 struct Wide {
@@ -260,6 +262,23 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     wait(&landed[st], ph, 9);
                     if constexpr (WIDENED) {
                         if constexpr (SCALED) *reinterpret_cast<float4 *>(&ks_s[n % kTables][lane * 4]) = scales;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = (int)__shfl_sync(0xffffffffu, unit, 2 + h), x = max(e, v_most - kFar), d = x - e;
+                            v_most = max(v_most, x);
+                            if (lane == 2 + h) unit = (float)x;
+                            if (d > 0) {             // (seldom: the kernel before did not know those before)
+                                const uint32_t f = d < 15 ? (uint32_t)(15 - d) << 10 : d < 25 ? 1u << (24 - d) : 0u, f2 = f | f << 16;
+                                for (int i = lane; i < kHalf * 8; i += 32)
+#pragma unroll
+                                    for (int nb = 0; nb < DP / 64; ++nb) {
+                                        uint4 *at = reinterpret_cast<uint4 *>(v_s + st * C::kTile + nb * (kKeys * 128) + h * (kHalf * 128) + i * 16);
+                                        const uint4 w = *at;
+                                        *at = make_uint4(mul_f16x2(w.x, f2), mul_f16x2(w.y, f2), mul_f16x2(w.z, f2), mul_f16x2(w.w, f2));
+                                    }
+                                proxy_fence();
+                            }
+                        }
                         if (lane < 4) (lane < 2 ? k_unit : v_exp)[n % kTables][lane & 1] = unit;
                         if (u + 1 < w.from + units) fetch(u + 1);
                     }
@@ -306,7 +325,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         int e = (int)(most >> 23) - 127 - kUp<FMT>;
                         if (which) {
                             // Values far below those before them need not fill fp16, and all of one size with P: a tile of zeros must not carry the sum of exponentials out of fp32
-                            e = max(max(e, v_most - 20), -96);
+                            e = max(max(e, v_most - kFar), -96);
                             v_most = max(v_most, e);
                         }
                         e = min(max(e, -126), 120);
@@ -551,6 +570,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                     // what the scores of each 64 keys are multiplied by, and (codes) the exponent that their values were divided by: P takes it
                     float factor[2] = {row_factor, row_factor}, up[2] = {0.0f, 0.0f};
+                    bool drop = false;
                     if constexpr (CODED) {
                         if constexpr (!WIDENED) wait(&v_full[st], ((n + i) / kStages) & 1, 2);
 #pragma unroll
@@ -558,6 +578,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             factor[h] = fminf(fmaxf(factor[h] * *reinterpret_cast<volatile float *>(&k_unit[tb][h]), 1.17549435e-38f), 3.402823466e38f);
                             up[h] = *reinterpret_cast<volatile float *>(&v_exp[tb][h]);
                         }
+                        // (values that are nothing beside the tile's others: their P, over their own power of two, would be lost, and with it their share of the sum)
+                        drop = up[1] - up[0] > 60.0f;
+                        if (drop) up[0] = up[1] - 60.0f;
                     }
                     float mx = -INFINITY;
 #pragma unroll
@@ -572,9 +595,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     } else {
                         const bool grow = m == -INFINITY ? mx > m : mx > m + kRescaleStep;
                         if (__any_sync(0xffffffffu, grow)) {
-                            const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
+                            // (codes: the maximum follows the values' exponents too, and the sum of probabilities, which does not, must not be lost where they jump: half the way twice)
+                            const float step = grow ? ex2_approx(CODED ? 0.5f * (m - mx) : m - mx) : 1.0f, alpha = CODED ? step * step : step;
                             if (grow) m = mx;
-                            l *= alpha;
+                            l = CODED ? l * step * step : l * alpha;
                             // what was summed before has come: its products were issued before those of these scores
 #pragma unroll 1
                             for (int hh = 0; hh < DP / 16; ++hh) {
@@ -604,6 +628,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         l = CODED ? fmaf(part, __uint_as_float((uint32_t)(127 - (int)up[q >> 1]) << 23), l) : l + part;
                         tmem_st16_u32(s_addr + q * 16, pk);
                         if (q == 1) {
+                            if (drop) {              // (seldom)
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) pk[c] = 0u;
+                                tmem_wait_st();
+                                tmem_st16_u32(s_addr, pk);
+                                tmem_st16_u32(s_addr + 16, pk);
+                            }
                             tmem_wait_st();
                             tc_fence_before();
                             arrive(&p_full[half][0]);
@@ -833,9 +864,12 @@ paged_tc_join_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = p[(c0 + e) * kRows];
             const float m2 = p[DP * kRows], l2 = p[(DP + 1) * kRows], mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.0f : mn;
-            const float f1 = ex2_approx(m - base), f2 = ex2_approx(m2 - base);
+            // (codes: the sums of probabilities go half the way twice, as in the kernel before)
+            constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN;
+            const float s1 = ex2_approx(CODED ? 0.5f * (m - base) : m - base), s2 = ex2_approx(CODED ? 0.5f * (m2 - base) : m2 - base);
+            const float f1 = CODED ? s1 * s1 : s1, f2 = CODED ? s2 * s2 : s2;
             m = mn;
-            l = fmaf(l, f1, l2 * f2);
+            l = CODED ? fmaf(l * s1, s1, l2 * s2 * s2) : fmaf(l, f1, l2 * f2);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = fmaf(o[e], f1, x[e] * f2);
         }

@@ -293,6 +293,19 @@ def _one(dtype, seqs, H, fmt, wild, spread=1.0, scale=None, turn=None):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("powers", [(None, 60, None, -60), (60, None, None, 30), (None, 100, -100, 0), (-90, -20, 40, 110)])
+@pytest.mark.parametrize("dtype,seqs,H", CODED, ids=CODED_IDS)
+def test_values_of_powers_far_apart(dtype, seqs, H, fmt, powers):
+    """Pages of zeros and of tiny and huge values beside each other: their keys keep their share of the probabilities, whatever their values count for."""
+    def wild(name, x):
+        if name == "v":
+            for page in range(len(x)):
+                p = powers[page % 4]
+                x[page] *= 0.0 if p is None else 2.0 ** p
+    _one(dtype, seqs, H, fmt, wild)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("dtype,seqs,H", CODED, ids=CODED_IDS)
 def test_queries_and_keys_at_both_ends_of_the_range(dtype, seqs, H, fmt):
     def large(name, x):
