@@ -34,8 +34,10 @@ namespace {
 constexpr int kRows = 256, kKeys = 128, kStages = 2;
 constexpr int kTables = 4;            // a tile's scales and pages are read until its scores have been: the products of the tile after the next say so
 constexpr int kWideners = 128, kThreads = 512;
-// Registers a thread of each warpgroup: 128 at launch; 184 + 184 + 88 + 56 = 4 x 128
-constexpr int kSoftRegs = 184, kWidenRegs = 88, kIssueRegs = 56;
+// Registers a thread of each warpgroup: 128 at launch; 184 + 184 + 88 + 56 = 4 x 128, and where no codes are widened here 200 + 200 + 56 + 56 (4096 tokens over 32768 int8 keys: 2205 -> 2148 us)
+template <bool WIDENS> constexpr int kSoftRegs = WIDENS ? 184 : 200;
+template <bool WIDENS> constexpr int kWidenRegs = WIDENS ? 88 : 56;
+constexpr int kIssueRegs = 56;
 constexpr int kHalf = 64, kSlots = 3;  // keys of a half tile of codes, half tiles in the ring
 constexpr float kRescaleStep = 8.0f;
 // Units after which the sums in TMEM are added to what the block keeps of them in memory: the tensor pipe cuts off towards zero, 2^-24 to 2^-23 of the sum for each sixteen keys, so after 32768 keys 2^-12 at most, an
@@ -236,7 +238,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         __syncwarp();
         if (abort_flag) linger();
     } else if (warp >= 8 && warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs<WIDENS>));
         // ================= codes to operands; rows behind the last key ===========================================
         const int pt = tid - 256, D = a.c.D;
         uint32_t n = 0, slot = 0;
@@ -439,7 +441,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         if (abort_flag) linger();
     } else {
         // ================= softmax ===============================================================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs<WIDENS>));
         const int half = warp >> 2, quad = warp & 3, D = a.c.D;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + kColS + half * 128 + lanes, o_addr = tmem + kColO + half * 128 + lanes;
