@@ -87,8 +87,7 @@ struct Shape {
     static constexpr bool F32 = sizeof(T) == 4, CODED = FMT != HIPGPT_CACHE_PLAIN, CUT = CUT_;
     static constexpr int EB = CODED ? 1 : (int)sizeof(T);               // bytes of an element of the cache
     static constexpr int NQ = !F32 ? 1 : CODED ? 2 : 3, NK = F32 && !CODED ? 3 : 1;  // pieces of Q and P, of K and V
-    static constexpr int MT = 1;                                        // tiles of 16 rows a warp
-    static constexpr int ROWS = 16 * MT * (SPLITROWS ? kWarps : 1);
+    static constexpr int ROWS = 16 * (SPLITROWS ? kWarps : 1);
     static constexpr int KB = 4096 / (DP * EB) >= 32 ? 32 : 16;         // keys a warp takes at a time
     static constexpr int UNIT = CUT && DP > 32 ? 32 : SPLITROWS ? 64 : kWarps * KB;      // keys of a place in the ring
     static constexpr int EC = least_of(16 / EB, DP / 4), NC = DP / 4 / EC;       // K: elements of a chunk, chunks a thread
@@ -279,36 +278,31 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
             }
         }
         meet();
-        const uint4 *q_w = q_s + (SPLITROWS ? warp * C::MT * C::STEPS * 32 : 0) + lane;
+        const uint4 *q_w = q_s + (SPLITROWS ? warp * C::STEPS * 32 : 0) + lane;
 
-        int limit[C::MT][2];
-        float factor[C::MT][2];                      // of the scores, to the logarithm to base two
-        const int wrow = row0 + (SPLITROWS ? warp * 16 * C::MT : 0);
+        int limit[2];
+        float factor[2];                             // of the scores, to the logarithm to base two
+        const int wrow = row0 + (SPLITROWS ? warp * 16 : 0);
 #pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int rr = mt * 16 + g + 8 * r;
-                limit[mt][r] = wrow + rr < rows ? limit_of(a, s, wrow + rr) : 0;
-                factor[mt][r] = a.cscale;
-                if constexpr (HALF) factor[mt][r] = a.cscale * pow2_inverse(q_unit[wrow - row0 + rr]);
-            }
+        for (int r = 0; r < 2; ++r) {
+            const int rr = g + 8 * r;
+            limit[r] = wrow + rr < rows ? limit_of(a, s, wrow + rr) : 0;
+            factor[r] = a.cscale;
+            if constexpr (HALF) factor[r] *= pow2_inverse(q_unit[wrow - row0 + rr]);
+        }
         const int least_limit = wrow < rows ? limit_of(a, s, wrow) : 0;
         const int keys = tile_keys<C::ROWS>(a, s, w.tile);
-        const int wlast = min(wrow + 16 * C::MT, rows) - 1;              // this warp's rows end here, and their keys
+        const int wlast = min(wrow + 16, rows) - 1;              // this warp's rows end here, and their keys
         const int wkeys = !SPLITROWS ? keys : wlast < wrow ? 0 : limit_of(a, s, wlast);
 
-        float o[C::MT][C::TILES][4], m[C::MT][2], l[C::MT][2];
+        float o[C::TILES][4], m[2], l[2];
         int unit = -126;                             // codes: o is divided by 2^unit, which follows the largest scale of the values
 #pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
+        for (int j = 0; j < C::TILES; ++j)
 #pragma unroll
-            for (int j = 0; j < C::TILES; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.0f;
-        }
+            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
 
         // ---- blocks of KB keys ------------------------------------------------------------------------------------
         constexpr int NG = C::KB / 16, NJ = C::KB / 8, BLOCKS = SPLITROWS ? C::UNIT / C::KB : 1;
@@ -327,16 +321,14 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 const bool partial = p0 + C::KB > wkeys || there != (1u << NG) - 1;          // places without keys
                 const bool masked = p0 + C::KB > least_limit || there != (1u << NG) - 1;
                 // scores: the main products, and apart from them those of the smaller pieces
-                float z[C::MT][NJ][4], zc[C::NQ > 1 ? C::MT : 1][C::NQ > 1 ? NJ : 1][4];
+                float z[NJ][4], zc[C::NQ > 1 ? NJ : 1][4];
 #pragma unroll
-                for (int mt = 0; mt < C::MT; ++mt)
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            z[mt][j][e] = 0.0f;
-                            if constexpr (C::NQ > 1) zc[mt][j][e] = 0.0f;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        z[j][e] = 0.0f;
+                        if constexpr (C::NQ > 1) zc[j][e] = 0.0f;
+                    }
                 constexpr int PER = C::EC / 4;       // instructions a chunk
 #pragma unroll
                 for (int i = 0; i < C::NC; ++i) {
@@ -356,11 +348,9 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                     }
 #pragma unroll
                     for (int x = 0; x < PER; ++x) {
-                        uint4 q[C::NQ][C::MT];
+                        uint4 q[C::NQ];
 #pragma unroll
-                        for (int n = 0; n < C::NQ; ++n)
-#pragma unroll
-                            for (int mt = 0; mt < C::MT; ++mt) q[n][mt] = q_w[(n * (C::ROWS / 16) + mt) * C::STEPS * 32 + (i * PER + x) * 32];
+                        for (int n = 0; n < C::NQ; ++n) q[n] = q_w[n * (C::ROWS / 16) * C::STEPS * 32 + (i * PER + x) * 32];
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) {
                             uint32_t b[C::NK][2];
@@ -381,13 +371,10 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                                 }
                             }
 #pragma unroll
-                            for (int mt = 0; mt < C::MT; ++mt) {
+                            for (int order = C::NQ - 1; order >= 1; --order)
 #pragma unroll
-                                for (int order = C::NQ - 1; order >= 1; --order)
-#pragma unroll
-                                    for (int n = 0; n <= order && n < C::NK; ++n) mma16<HALF>(zc[mt][j], q[order - n][mt], b[n][0], b[n][1]);
-                                mma16<HALF>(z[mt][j], q[0][mt], b[0][0], b[0][1]);
-                            }
+                                for (int n = 0; n <= order && n < C::NK; ++n) mma16<HALF>(zc[j], q[order - n], b[n][0], b[n][1]);
+                            mma16<HALF>(z[j], q[0], b[0][0], b[0][1]);
                         }
                     }
                 }
@@ -401,7 +388,7 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 }
 
                 // ---- softmax ----------------------------------------------------------------------------------------------
-                auto seen = [&](int mt, int j, int e) { return p0 + 8 * j + 2 * t4 + (e & 1) < limit[mt][e >> 1] && (there >> (j >> 1) & 1); };
+                auto seen = [&](int j, int e) { return p0 + 8 * j + 2 * t4 + (e & 1) < limit[e >> 1] && (there >> (j >> 1) & 1); };
                 float shrink = 1.0f;
                 if constexpr (C::CODED) {
                     // P times the scales of the values, over 2^unit: at most 2^15
@@ -431,80 +418,77 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                         vs2[j].y *= down;
                     }
                 }
-                uint4 p[C::NQ][C::MT][NG];
+                uint4 p[C::NQ][NG];
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int mt = 0; mt < C::MT; ++mt) {
-                    float top[2] = {-INFINITY, -INFINITY};
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = z[j][e];
+                        if constexpr (C::NQ > 1) x += zc[j][e];
+                        // (the two factors first: small queries and large keys, or the other way round, must not pass fp32's range on the way)
+                        if constexpr (C::CODED) z[j][e] = x * (((e & 1) ? ks2[j].y : ks2[j].x) * factor[e >> 1]);
+                        else z[j][e] = x * factor[e >> 1];
+                    }
+                if (masked) {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = z[mt][j][e];
-                            if constexpr (C::NQ > 1) x += zc[mt][j][e];
-                            // (the two factors first: small queries and large keys, or the other way round, must not pass fp32's range on the way)
-                            if constexpr (C::CODED) z[mt][j][e] = x * (((e & 1) ? ks2[j].y : ks2[j].x) * factor[mt][e >> 1]);
-                            else z[mt][j][e] = x * factor[mt][e >> 1];
-                        }
-                    if (masked) {
+                        for (int e = 0; e < 4; ++e) z[j][e] = seen(j, e) ? z[j][e] : -INFINITY;
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], z[j][e]);
+                float base[2], alpha[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    const float now = fmaxf(m[r], top[r]);
+                    base[r] = now == -INFINITY ? 0.0f : now;
+                    alpha[r] = ex2_approx(m[r] - base[r]);
+                    m[r] = now;
+                    l[r] *= alpha[r];
+                    alpha[r] *= shrink;
+                }
+                if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                    for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e >> 1];
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = ex2_approx(z[j][e] - base[e >> 1]);
+                        l[e >> 1] += y;
+                        z[j][e] = y;
+                    }
+                if constexpr (C::CODED) {
+                    if (!masked) {
 #pragma unroll
                         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) z[mt][j][e] = seen(mt, j, e) ? z[mt][j][e] : -INFINITY;
+                            for (int e = 0; e < 4; ++e) z[j][e] *= (e & 1) ? vs2[j].y : vs2[j].x;
+                    } else {
+                        // (the scale of a value that a row does not see may be anything)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[j][e] = seen(j, e) ? z[j][e] * ((e & 1) ? vs2[j].y : vs2[j].x) : 0.0f;
                     }
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], z[mt][j][e]);
-                    float base[2], alpha[2];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                        const float now = fmaxf(m[mt][r], top[r]);
-                        base[r] = now == -INFINITY ? 0.0f : now;
-                        alpha[r] = ex2_approx(m[mt][r] - base[r]);
-                        m[mt][r] = now;
-                        l[mt][r] *= alpha[r];
-                        alpha[r] *= shrink;
-                    }
-                    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-                        for (int j = 0; j < C::TILES; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[e >> 1];
-                    }
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float y = ex2_approx(z[mt][j][e] - base[e >> 1]);
-                            l[mt][e >> 1] += y;
-                            z[mt][j][e] = y;
-                        }
-                    if constexpr (C::CODED) {
-                        if (!masked) {
-#pragma unroll
-                            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) z[mt][j][e] *= (e & 1) ? vs2[j].y : vs2[j].x;
-                        } else {
-                            // (the scale of a value that a row does not see may be anything)
-#pragma unroll
-                            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) z[mt][j][e] = seen(mt, j, e) ? z[mt][j][e] * ((e & 1) ? vs2[j].y : vs2[j].x) : 0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < NG; ++i)
-#pragma unroll
-                        for (int n = 0; n < C::NQ; ++n) {
-                            p[n][mt][i].x = next_piece<HALF>(z[mt][2 * i][0], z[mt][2 * i][1], n == C::NQ - 1);
-                            p[n][mt][i].y = next_piece<HALF>(z[mt][2 * i][2], z[mt][2 * i][3], n == C::NQ - 1);
-                            p[n][mt][i].z = next_piece<HALF>(z[mt][2 * i + 1][0], z[mt][2 * i + 1][1], n == C::NQ - 1);
-                            p[n][mt][i].w = next_piece<HALF>(z[mt][2 * i + 1][2], z[mt][2 * i + 1][3], n == C::NQ - 1);
-                        }
                 }
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+#pragma unroll
+                    for (int n = 0; n < C::NQ; ++n) {
+                        p[n][i].x = next_piece<HALF>(z[2 * i][0], z[2 * i][1], n == C::NQ - 1);
+                        p[n][i].y = next_piece<HALF>(z[2 * i][2], z[2 * i][3], n == C::NQ - 1);
+                        p[n][i].z = next_piece<HALF>(z[2 * i + 1][0], z[2 * i + 1][1], n == C::NQ - 1);
+                        p[n][i].w = next_piece<HALF>(z[2 * i + 1][2], z[2 * i + 1][3], n == C::NQ - 1);
+                    }
 
                 if (blk == BLOCKS - 1 || p0 + C::KB >= wkeys) leave(ksl);        // (what was read of it has been used: an arrival does not wait for loads)
 
@@ -554,20 +538,18 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                             }
                         }
 #pragma unroll
-                        for (int x = 0; x < W; ++x)
+                        for (int x = 0; x < W; ++x) {
+                            const int j = c * C::EV + e + x;
+                            float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int mt = 0; mt < C::MT; ++mt) {
-                                const int j = c * C::EV + e + x;
-                                float d4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            for (int order = C::NQ - 1; order >= 0; --order)
 #pragma unroll
-                                for (int order = C::NQ - 1; order >= 0; --order)
+                                for (int n = 0; n <= order && n < C::NK; ++n)
 #pragma unroll
-                                    for (int n = 0; n <= order && n < C::NK; ++n)
+                                    for (int i = 0; i < NG; ++i) mma16<HALF>(d4, p[order - n][i], b[i][x][n][0], b[i][x][n][1]);
 #pragma unroll
-                                        for (int i = 0; i < NG; ++i) mma16<HALF>(d4, p[order - n][mt][i], b[i][x][n][0], b[i][x][n][1]);
-#pragma unroll
-                                for (int y = 0; y < 4; ++y) o[mt][j][y] += d4[y];
-                            }
+                            for (int y = 0; y < 4; ++y) o[j][y] += d4[y];
+                        }
                     }
                 }
             }
@@ -578,18 +560,15 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
         }
         const float grown = C::CODED ? __uint_as_float((uint32_t)(127 + min(unit, 126)) << 23) : 1.0f;
 #pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 1);
-                l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 2);
-            }
-            if constexpr (C::CODED)
-#pragma unroll
-                for (int j = 0; j < C::TILES; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[mt][j][e] *= grown;
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
+        if constexpr (C::CODED)
+#pragma unroll
+            for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] *= grown;
 
         // ---- the tile's end ---------------------------------------------------------------------------------------
         const int part = run.part();
@@ -607,10 +586,10 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                     for (int c = 0; c < C::NV; ++c)
 #pragma unroll
                         for (int e = 0; e < C::EV; ++e) {
-                            row[(2 * t4 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r];
-                            row[(2 * t4 + 1 + 8 * c) * C::EV + e] = o[0][c * C::EV + e][2 * r + 1];
+                            row[(2 * t4 + 8 * c) * C::EV + e] = o[c * C::EV + e][2 * r];
+                            row[(2 * t4 + 1 + 8 * c) * C::EV + e] = o[c * C::EV + e][2 * r + 1];
                         }
-                    if (t4 == 0) ml_s[buf][g + 8 * r] = make_float2(m[0][r], l[0][r]);
+                    if (t4 == 0) ml_s[buf][g + 8 * r] = make_float2(m[r], l[r]);
                 }
             };
             if (warp >= 2) put(warp - 2);
@@ -622,16 +601,16 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
                 __syncwarp();
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float now = fmaxf(m[0][r], other[r].x), base = now == -INFINITY ? 0.0f : now;
-                    const float f0 = ex2_approx(m[0][r] - base), f1 = ex2_approx(other[r].x - base);
+                    const float now = fmaxf(m[r], other[r].x), base = now == -INFINITY ? 0.0f : now;
+                    const float f0 = ex2_approx(m[r] - base), f1 = ex2_approx(other[r].x - base);
                     const float *row = row_at(warp, r);
-                    m[0][r] = now;
-                    l[0][r] = fmaf(l[0][r], f0, other[r].y * f1);
+                    m[r] = now;
+                    l[r] = fmaf(l[r], f0, other[r].y * f1);
 #pragma unroll
                     for (int c = 0; c < C::NV; ++c)
 #pragma unroll
                         for (int e = 0; e < C::EV; ++e) {
-                            float *x = &o[0][c * C::EV + e][2 * r];
+                            float *x = &o[c * C::EV + e][2 * r];
                             x[0] = fmaf(x[0], f0, row[(2 * t4 + 8 * c) * C::EV + e] * f1);
                             x[1] = fmaf(x[1], f0, row[(2 * t4 + 1 + 8 * c) * C::EV + e] * f1);
                         }
@@ -672,32 +651,30 @@ paged_rows_kernel(const __grid_constant__ AttnArgs a)
             const bool store = !abort_flag;
             bool wild = false;
 #pragma unroll
-            for (int mt = 0; mt < C::MT; ++mt)
+            for (int r = 0; r < 2; ++r) {
+                const int rr = warp * 16 + g + 8 * r, row = row0 + rr;
+                const float sum = l[r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const bool here = row < rows && store;
+                const long long t = s.first + row / a.group;
+                T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + row % a.group) * D;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int rr = (warp * C::MT + mt) * 16 + g + 8 * r, row = row0 + rr;
-                    const float sum = l[mt][r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const bool here = row < rows && store;
-                    const long long t = s.first + row / a.group;
-                    T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)(w.head * a.group + row % a.group) * D;
+                for (int c = 0; c < C::NV; ++c)
 #pragma unroll
-                    for (int c = 0; c < C::NV; ++c)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int e = 0; e < C::EV; ++e) {
-                                const int d = (2 * t4 + x + 8 * c) * C::EV + e;
-                                const float y = o[mt][c * C::EV + e][2 * r + x];
-                                if (dst) {
-                                    if (here) dst[(size_t)rr * DP + d] = y;
-                                } else {
-                                    const float v = sum == 0.0f ? 0.0f : y * inv;
-                                    wild = wild || (here && !finite(v) && sum == sum);
-                                    if (here && d < D) out[d] = from_float<T>(v);
-                                }
+                        for (int e = 0; e < C::EV; ++e) {
+                            const int d = (2 * t4 + x + 8 * c) * C::EV + e;
+                            const float y = o[c * C::EV + e][2 * r + x];
+                            if (dst) {
+                                if (here) dst[(size_t)rr * DP + d] = y;
+                            } else {
+                                const float v = sum == 0.0f ? 0.0f : y * inv;
+                                wild = wild || (here && !finite(v) && sum == sum);
+                                if (here && d < D) out[d] = from_float<T>(v);
                             }
-                    if (dst && here && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[mt][r], sum);
-                }
+                        }
+                if (dst && here && t4 == 0) reinterpret_cast<float2 *>(dst + C::ROWS * DP)[rr] = make_float2(m[r], sum);
+            }
             if (__any_sync(0xffffffffu, wild) && lane == 0) atomicOr(&mend_s, 1u << (number & 31));
         }
     }
@@ -849,7 +826,7 @@ paged_token_kernel(const __grid_constant__ AttnArgs a)
             const int row = row0 + 2 * t4 + r;
             limit[r] = row < rows ? limit_of(a, s, row) : 0;
             factor[r] = a.cscale;
-            if constexpr (HALF) factor[r] = a.cscale * pow2_inverse(q_unit[2 * t4 + r]);
+            if constexpr (HALF) factor[r] *= pow2_inverse(q_unit[2 * t4 + r]);
         }
         const int least_limit = limit_of(a, s, row0), keys = tile_keys<8>(a, s, w.tile);
         int unit = -126;                             // codes: o is divided by 2^unit, which follows the largest scale of the values
@@ -1303,7 +1280,11 @@ int launch_kernel(void (*kern)(AttnArgs), AttnArgs a, cudaStream_t st)
     return e == cudaSuccess ? check_launch("paged attention") : fail(HIPGPT_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
 }
 
-// Rows a sequence, on the average: eight at most (single tokens of a small group), some, many
+// Rows a sequence, on the average: eight at most (single tokens of a small group), some, many.  32 sequences of up to 8192 keys, 8 heads, us with the three kernels (the third in bf16: tcgen05):
+//   bf16 of 128     4 rows 114 / 118 / 171, 8 146 / 120 / 171, 15 229 / 168 / 173, 31 435 / 269 / 174;  e4m3 of 128  4 73 / 101 / 327, 8 94 / 104 / 328, 15 147 / 147 / 328, 31 265 / 233 / 330, 41 343 / 302 / 329
+//   int8 of 64      4 53 / 63 / 305, 8 71 / 68 / 305, 31 198 / 146 / 305, 61 374 / 257 / 305
+//   fp32 of 64      4 123 / 160 / 491, 8 161 / 161 / 491, 31 491 / 381 / 591, 61 936 / 694 / 943;  over int8 of 128  4 98 / 133 / 385, 8 126 / 134 / 385, 31 378 / 306 / 472, 61 715 / 558 / 762
+// One limit for all types: plain bf16 of 17 to 32 rows and fp32 of 33 to 61 would be faster by the next kernel.
 enum { kTokens, kSome, kMany };
 template <typename T, int FMT, int DP>
 int launch_width(int rows, const AttnArgs &a, cudaStream_t st)

@@ -340,16 +340,18 @@ HIPGPT_API int hipgpt_mha_decode_noalloc(const float *d_q, const float *d_kcache
  *   hipgpt_paged_attention     out[t][h] = softmax(scale q k^T) v over the keys of t's sequence: causal != 0 those up to t's position, 0 all lengths[b].
  *                              q, out [tokens][H * head_dim], H a multiple of the cache's heads: H / heads query heads in a row share one.  A row that sees no key gets zeros
  *                              (as one whose scores are all minus infinity).  What lies in masked places, NaN too, does not matter.  scale > 0.
- *                              Products on the tensor pipe, sums in fp32 (bf16: up to 32768 keys of them in the tensor core's accumulators, which cut off towards zero, 2^-12 of a sum at most).  fp32: of three bf16 pieces of each operand (24 bits), against codes of two fp16 pieces (22 bits, a power of
- *                              two for each row of q); an infinity in q or a key can make NaN of the scores that it meets, one in a value makes infinities.  bf16, plain cache: probabilities are rounded to bf16 before
- *                              the second product.  8-bit caches: probabilities times their values' scales are held in fp16 over a power of two that follows the largest: a value whose scale is
- *                              below 2^-38 of its sequence's largest is lost.  bf16 with many rows a sequence: in int8 a value times its scale is rounded to fp16, and values share a power of two
- *                              with the 63 keys beside them: scales down to 2^-21 of their largest keep all digits.
+ *                              Products on the tensor pipe, sums in fp32 (bf16: up to 32768 keys of them in the tensor core's accumulators, which cut off towards zero, 2^-12 of a sum
+ *                              at most).  fp32: of three bf16 pieces of each operand (24 bits), against codes of two fp16 pieces (22 bits, a power of two for each row of q); an infinity in q or
+ *                              a key can make NaN of the scores that it meets, one in a value makes infinities.  bf16, plain cache: probabilities are rounded to bf16 before the second product.
+ *                              8-bit caches: probabilities times their values' scales are held in fp16 over a power of two that follows the largest: a value whose scale is below 2^-38 of
+ *                              its sequence's largest is lost.  bf16 with many rows a sequence: in int8 a value's scale is rounded to fp16, and its product with the code once more; values share a power of
+ *                              two, 2^-96 at least, with the 63 keys beside them: scales down to 2^-21 of their largest keep all digits, and of 2^-20 of the largest before them.
  *                              Keys are split over blocks where rows are few; buffers of the library (per device and stream, at most eight; hipgpt_release_workspace()
  *                              frees them; a captured call gets buffers of its graph) hold the parts.  The same bits run to run on the same GPU.
- *                              bf16 with 1536 rows (tokens * H / heads) a sequence and more on average: where it takes at most 2^30 bytes, the buffer also holds the 8-bit cache's rows in
- *                              16 bits, sequences * most_pages * page_size * heads * (4 head_dim + 4) bytes; fp32 over a plain cache with 160 rows and more (64 from head_dim 65 on): the keys and values as their
- *                              pieces, three times the bytes of the sequences' keys and values in 16 bits, head_dim counted as 32, 64 or 128.
+ *                              By rows (tokens * H / heads) a sequence on average, and where it takes at most 2^30 bytes, the buffer also holds: bf16 over 8 bits, 1536 rows and more: the cache's rows in
+ *                              16 bits, sequences * most_pages * page_size * heads * (4 head_dim + 4) bytes; fp32 over a plain cache, 112 rows and more (160 for head_dim from 33 to 64, 64 beyond): keys and values as
+ *                              their pieces, sequences * most_pages * page_size * heads * 12 head_dim bytes, head_dim counted as 32, 64 or 128.  Both go by the table's width, whatever the lengths are:
+ *                              a table should be no wider than its batch needs.
  */
 #define HIPGPT_CACHE_PLAIN 0
 #define HIPGPT_CACHE_E4M3  1
