@@ -5,7 +5,8 @@
 // Bound for single tokens: HBM, the cache is read once (the group's rows share it).  One warp brings K and V as they lie in their pages into a ring in shared memory by bulk copies, a lane a
 // run of keys in one page; four warps multiply (sixteen rows by eight keys an instruction; what tcgen05 adds is not needed where the bytes decide, and its operands would have to be
 // laid out once more).  (32 sequences of 8192 to 32768 tokens, 8 heads of 128 codes: loads straight into registers
-// 641 us, 2.2 TB/s, too few bytes on their way; copies 316 us; with the products the other way round, below, 244 to 264 us, 5.4 to 5.8 TB/s.)
+// 641 us, 2.2 TB/s, too few bytes on their way; copies 316 us; with the products the other way round, below, 244; without the kernel's arguments copied to
+// every thread's stack 227 us, 6.2 TB/s, and 253 in long runs.)
 //   * which 16 values of a row an instruction sums over does not matter as long as Q's are the same, so a thread of the four that share a key takes 16
 //     consecutive bytes of its row, and Q is laid out to match;
 //   * P's layout as a result (keys 2t, 2t+1, 8+2t, 9+2t of sixteen) is its layout as an operand, so a thread takes 16 consecutive bytes of each of those four rows of V, and the

@@ -216,19 +216,6 @@ struct Run {
 // worked out again over the keys that it sees: when the block's whole run is done and nobody in it waits for anything any more (a long row
 // takes longer than a wait may), or where parts are joined.
 
-// One value of a row of the cache
-template <typename T, int FMT>
-__device__ __forceinline__ float cached(const uint8_t *base, const float *scale, long long row, int D, int d)
-{
-    if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-        return to_float(reinterpret_cast<const T *>(base)[row * D + d]);
-    } else {
-        uint32_t lo, hi;
-        codes_to_half<FMT>(base[row * D + d], lo, hi);
-        return floats_of(lo).x * scale[row];
-    }
-}
-
 // Sixteen values in a row of the cache, of codes without their scale
 template <typename T, int FMT>
 __device__ __forceinline__ void cached16(const uint8_t *base, long long row, int D, int d, float (&x)[16])
@@ -282,98 +269,142 @@ __device__ __forceinline__ int last_wild(const AttnArgs &a, int b, int head, int
     return top;
 }
 
-// One warp: values c0 .. c1 of row `row` of (sequence b, head of the cache), 32 keys at a time: a lane a key for the scores (sixteen sums each), a lane every 32nd value for the sums over
-// the keys, which are added up 32 by 32 and kept as half of their average so far: nothing passes fp32's range that does not end outside it.  About 40 clocks a key with eight warps an SM; one key after the other, with its look-ups and shuffles in a chain, it was several hundred.
+// Four values from column `d` on in a row of the cache, of codes without their scale
 template <typename T, int FMT>
-__device__ __noinline__ void row_again(const AttnArgs &a, int b, int head, const Sequence &s, int row, int c0, int c1)
+__device__ __forceinline__ float4 cached4(const uint8_t *base, long long row, int D, int d)
 {
-    const int lane = threadIdx.x & 31, D = a.c.D, limit = limit_of(a, s, row);
-    const long long t = s.first + row / a.group;
-    const int h = head * a.group + row % a.group;
-    const T *q = static_cast<const T *>(a.q) + t * a.q_stride + (long long)h * D;
-    float qv[4], o[4], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        qv[i] = lane + 32 * i < D ? to_float(q[lane + 32 * i]) : 0.0f;
-        o[i] = 0.0f;
+    if constexpr (FMT != HIPGPT_CACHE_PLAIN) {
+        uint32_t lo, hi;
+        codes_to_half<FMT>(*reinterpret_cast<const uint32_t *>(base + row * D + d), lo, hi);
+        const float2 p = floats_of(lo), q = floats_of(hi);
+        return make_float4(p.x, p.y, q.x, q.y);
+    } else {
+        float x[4];
+        load_values<T, 4>(reinterpret_cast<const T *>(base) + row * D + d, x);
+        return make_float4(x[0], x[1], x[2], x[3]);
     }
-    for (int p0 = 0; p0 < limit; p0 += 32) {
-        const int p = p0 + lane;
-        const long long r = p < limit ? row_of(a.c, b, head, p) : -1;
-        float z[16];
+}
+
+// One warp: values c0 .. c1 of one or two rows (-1: none) of (sequence b, head of the cache), 32 keys at a time: a lane a key for the scores, a lane four values for the sums over the keys, which are added up
+// 32 by 32 and kept as half of their average so far: nothing passes fp32's range that does not end outside it.  What is fetched serves both rows, and four keys' values are on their way at once.
+// (More of either takes registers that the kernels which call it then do not have: fp32 prompts 78 -> 90 us.)
+template <typename T, int FMT>
+__device__ __noinline__ void rows_again(const AttnArgs &a, int b, int head, int2 which, int c0, int c1)
+{
+    constexpr bool CODED = FMT != HIPGPT_CACHE_PLAIN;
+    constexpr int N = 2, kAhead = 4;
+    const int lane = threadIdx.x & 31, D = a.c.D, d0 = 4 * lane, row[N] = {which.x, which.y};
+    const Sequence s = sequence_of(a.c, b);
+    int limit[N], most = 0;
+    float q[N][4], o[N][4], factor[N], m[N], l[N];
+    auto place = [&](int n, long long stride) { return (s.first + row[n] / a.group) * stride + (long long)(head * a.group + row[n] % a.group) * D + d0; };
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = 0.0f;
+    for (int n = 0; n < N; ++n) {
+        limit[n] = row[n] >= 0 ? limit_of(a, s, row[n]) : 0;
+        most = max(most, limit[n]);
+        float largest = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (16 * c >= D) break;
-            float k[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) k[e] = 0.0f;
-            if (r >= 0) cached16<T, FMT>(a.c.k, r, D, 16 * c, k);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) z[e] = fmaf(__shfl_sync(0xffffffffu, qv[c / 2], 16 * (c % 2) + e), k[e], z[e]);
+        for (int e = 0; e < 4; ++e) {
+            q[n][e] = row[n] >= 0 && d0 < D ? to_float((static_cast<const T *>(a.q) + place(n, a.q_stride))[e]) : 0.0f;
+            largest = fmaxf(largest, fabsf(q[n][e]));
+            o[n][e] = 0.0f;
         }
+        factor[n] = a.cscale;
+        if constexpr (CODED) {                       // (as in the kernels: small queries and large scales, or the other way round)
 #pragma unroll
-        for (int n = 8; n; n >>= 1)
+            for (int off = 16; off; off >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+            const float unit = row_unit(largest);
+            factor[n] *= pow2_inverse(unit);
 #pragma unroll
-            for (int e = 0; e < n; ++e) z[e] += z[e + n];
-        float score = z[0] * a.cscale, weight = 1.0f;
-        if constexpr (FMT != HIPGPT_CACHE_PLAIN)
-            if (r >= 0) {
-                score *= a.c.ks[r];
-                weight = a.c.vs[r];
-            }
-        if (r < 0) score = -INFINITY;
-        float top = score;
-#pragma unroll
-        for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = exp2f(m - base), e = exp2f(score - base);
-        m = mn;
-        float sum = e;
-#pragma unroll
-        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        const float before = l * alpha;
-        l = before + sum;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        // (one lane's scale and place after the other; a place that is none is not looked at)
-        const float f = r < 0 ? 0.0f : 0.5f * (e * inv) * weight;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = 0; e < 4; ++e) q[n][e] *= unit;
+        }
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+    }
+    for (int p0 = 0; p0 < most; p0 += 32) {
+        const int p = p0 + lane;
+        const long long mine = p < most ? row_of(a.c, b, head, p) : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, mine >= 0);
+        if (!there) continue;
+        // (a lane without a key reads another's: loads without conditions go out together)
+        const long long other = __shfl_sync(0xffffffffu, mine, __ffs((int)there) - 1), r = mine >= 0 ? mine : other;
+        float z[N] = {0.0f, 0.0f};
 #pragma unroll 4
-        for (int j = 0; j < 32; ++j) {
-            const long long rj = __shfl_sync(0xffffffffu, r, j);
-            const float fj = __shfl_sync(0xffffffffu, f, j);
-            if (rj < 0) continue;
+        for (int c = 0; c < D; c += 16) {
+            float k[16];
+            cached16<T, FMT>(a.c.k, r, D, c, k);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (lane + 32 * i >= D) continue;
-                float v;
-                if constexpr (FMT == HIPGPT_CACHE_PLAIN) {
-                    v = to_float(reinterpret_cast<const T *>(a.c.v)[rj * D + lane + 32 * i]);
-                } else {
-                    uint32_t lo, hi;
-                    codes_to_half<FMT>(a.c.v[rj * D + lane + 32 * i], lo, hi);
-                    v = floats_of(lo).x;
-                }
-                x[i] = fmaf(fj, v, x[i]);
+            for (int n = 0; n < N; ++n) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum = fmaf(__shfl_sync(0xffffffffu, q[n][e & 3], c / 4 + (e >> 2)), k[e], sum);
+                z[n] += sum;
             }
+        }
+        float unit = 1.0f, weight = 0.5f;
+        if constexpr (CODED) {
+            unit = a.c.ks[r];
+            weight *= a.c.vs[r];
+        }
+        unsigned seen[N];
+        float f[N], keep[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const bool sees = mine >= 0 && p < limit[n];
+            seen[n] = __ballot_sync(0xffffffffu, sees);
+            const float score = sees ? z[n] * (unit * factor[n]) : -INFINITY;
+            float top = score;
+#pragma unroll
+            for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float now = fmaxf(m[n], top), base = now == -INFINITY ? 0.0f : now;
+            const float e = exp2f(score - base), before = l[n] * exp2f(m[n] - base);
+            m[n] = now;
+            float sum = e;
+#pragma unroll
+            for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            l[n] = before + sum;
+            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
+            keep[n] = before * inv;
+            f[n] = e * inv * weight;                 // (of the keys that the row sees)
+        }
+        float x[N][4] = {};
+#pragma unroll 1
+        for (int j0 = 0; j0 < 32; j0 += kAhead) {
+            float4 v[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) v[j] = cached4<T, FMT>(a.c.v, __shfl_sync(0xffffffffu, r, j0 + j), D, min(d0, D - 4));
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const float fj = __shfl_sync(0xffffffffu, f[n], j0 + j);
+                    if (seen[n] >> (j0 + j) & 1) {
+                        x[n][0] = fmaf(fj, v[j].x, x[n][0]);
+                        x[n][1] = fmaf(fj, v[j].y, x[n][1]);
+                        x[n][2] = fmaf(fj, v[j].z, x[n][2]);
+                        x[n][3] = fmaf(fj, v[j].w, x[n][3]);
+                    }
+                }
         }
         bool number = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            o[i] = fmaf(o[i], before * inv, x[i]);
-            number = number || (lane + 32 * i < D && o[i] == o[i]);
-        }
-        // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
-        if (l != l || !__any_sync(0xffffffffu, number)) break;
-    }
-    T *out = static_cast<T *>(a.out) + t * a.out_stride + (long long)h * D;
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // (an average of finite values that rounding took beyond the largest)
-        const float y = finite(o[i]) ? fminf(fmaxf(2.0f * o[i], -3.402823466e38f), 3.402823466e38f) : o[i];
-        if (lane + 32 * i >= c0 && lane + 32 * i < min(c1, D)) out[lane + 32 * i] = from_float<T>(y);
+            for (int e = 0; e < 4; ++e) {
+                o[n][e] = fmaf(o[n][e], keep[n], x[n][e]);
+                number = number || (row[n] >= 0 && d0 < D && o[n][e] == o[n][e]);
+            }
+        // NaN stays NaN: where all are, the rest of a long sequence need not be gone through
+        if (!__any_sync(0xffffffffu, number)) break;
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            // (an average of finite values that rounding took beyond the largest)
+            const float y = l[n] != l[n] ? l[n] : finite(o[n][e]) ? fminf(fmaxf(2.0f * o[n][e], -3.402823466e38f), 3.402823466e38f) : o[n][e];
+            if (row[n] >= 0 && d0 + e >= c0 && d0 + e < min(c1, D)) (static_cast<T *>(a.out) + place(n, a.out_stride))[e] = from_float<T>(y);
+        }
 }
 
 // The keys that a tile's rows have been multiplied with: those they see, and where these were cut before, to the end of the last place
@@ -396,6 +427,7 @@ __device__ __forceinline__ void mend_tile(const AttnArgs &a, int b, int head, in
     };
     const int top = last(least, keys);               // (rows that see it see all of them)
     if (top < 0 && last(0, least) >= 0) return;
+    int found = -1;                                  // rows are worked out two at a time
     for (int r = first; r < rows; r += step) {
         const int row = row0 + r;
         if (top >= 0 && limit_of(a, s, row) > top) break;
@@ -406,8 +438,11 @@ __device__ __forceinline__ void mend_tile(const AttnArgs &a, int b, int head, in
             const int d = lane + 32 * i;
             if (d >= c0 && d < min(c1, a.c.D)) wild = wild || !finite(to_float(out[d]));
         }
-        if (__any_sync(0xffffffffu, wild)) row_again<T, FMT>(a, b, head, s, row, c0, c1);
+        if (!__any_sync(0xffffffffu, wild)) continue;
+        if (found >= 0) rows_again<T, FMT>(a, b, head, make_int2(found, row), c0, c1);
+        found = found >= 0 ? -1 : row;
     }
+    if (found >= 0) rows_again<T, FMT>(a, b, head, make_int2(found, -1), c0, c1);
 }
 
 // The tiles of a block's run whose number (modulo 32) is in `which`

@@ -15,8 +15,8 @@
 //                    6 bytes a clock; bulk copies bring 24.)
 // Bound: neither pipe yet.  At D = 128 a unit's products are 2048 clocks of the tensor pipe and its exponentials as many of the special-function unit; plain rows take 4150, the chain from P to the next scores
 // (P V's second half, Q K^T, two commits: 1750) and the softmax (2300) of a tile one after the other, the two tiles half a turn apart.  Widening codes here takes 6500 (four half
-// tiles of 1600).  32 heads over 8 of 128: five ragged sequences of 1100 new tokens in 8000, plain: 446 us, 857 TFLOP/s; 4096 new tokens in 32768, int8: 2.12 ms, 972 TFLOP/s, widened before;
-// 3.03 ms, widened here.
+// tiles of 1600).  32 heads over 8 of 128: five ragged sequences of 1100 new tokens in 8000, plain: 423 us, 903 TFLOP/s; 4096 new tokens in 32768, int8: 2.18 ms, 946 TFLOP/s, widened before;
+// 3.10 ms, widened here.
 // Every wait is bounded: on expiry the block raises a flag that cuts all later waits short, records a status code, skips its stores, lets what is on its way land,
 // frees its TMEM and returns.
 #include "attn_paged.cuh"

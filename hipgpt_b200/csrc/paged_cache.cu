@@ -5,8 +5,8 @@
 //   int8  scale max|x| / 127 (rounded to fp32); the code is the whole number nearest to x / scale, ties to even, of the exact quotient: the rounded product
 //         with 1 / scale may be one off beside a border, and the remainder x - code * scale, which one multiply-add gives exactly, says so
 //
-// Bound: issue slots of the conversion to codes, then HBM, for prompts (12 of up to 4096 tokens, 8 heads of 128, bf16 to int8 and back: 94 us, 4.4 TB/s; 172 us with a look-up for each row and rounding by the
-// special-function unit); the launch for single tokens (64 tokens written and read: 7.9 us).  A block takes some tokens; where each goes is looked up once for all its heads.  A row is read 16 bytes a thread by as many neighbouring
+// Bound: issue slots of the conversion to codes, then HBM, for prompts (12 of up to 4096 tokens, 8 heads of 128, bf16 to int8 and back: 92 us, 4.5 TB/s; 172 us with a look-up for each row and rounding by the
+// special-function unit); the launch for single tokens (64 tokens written and read: 7.3 us).  A block takes some tokens; where each goes is looked up once for all its heads.  A row is read 16 bytes a thread by as many neighbouring
 // threads as it needs (a power of two of them), the largest magnitude goes round by shuffles, and a thread has its parts of K and of V on their way at once.
 #include "paged.cuh"
 
